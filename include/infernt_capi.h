@@ -108,7 +108,7 @@ INFERNT_API int infernt_gemm_f32(const float* A, const float* B, float* C, int M
  * is finishing and stream its weights then, but it reads every other input
  * and writes its outputs only after that kernel has completed.  So the
  * weights must not be written by the kernel launched just before.       */
-enum { INFERNT_DTYPE_F32 = 0, INFERNT_DTYPE_BF16 = 1 };
+enum { INFERNT_DTYPE_F32 = 0, INFERNT_DTYPE_BF16 = 1, INFERNT_DTYPE_F16 = 2 /* paged operators only */ };
 
 /* y[n] = sum_k W[n][k] * xn[k] with xn = rmsnorm(x, norm_w, eps) when norm_w != NULL
  * (llama_layer.cpp:11-23 with the rmsnorm fused).  Rows of W0, W1, W2 (any of W1/W2 NULL)
@@ -550,6 +550,161 @@ INFERNT_API int infernt_batch_attention(const float* q, const void* k_cache, con
                                         const int* positions, int T, int nq, int nkv, int head_dim,
                                         int max_seq, int splits, int min_chunk, int stages,
                                         float* partials, void* attn, float* attn_f32, void* stream);
+
+/* -------------------------------------------- operators over paged caches ---
+ * Rotary positions with the append of K and V rows, attention of new tokens,
+ * and copies of pages, over the batched engine's page layout.  No counterpart
+ * in the reference (its caches are contiguous, one sequence each,
+ * include/kv_cache.h:7-15; cuda/rope.cu:13-34, cuda/kv_cache.cu:4-14 and
+ * cuda/attention.cu:9-42 are the arithmetic per token).
+ *
+ * The pools of one layer: K and V [num_pages][num_kv_heads][page_size]
+ * [head_dim], 16-byte aligned, of type INFERNT_DTYPE_BF16 or _F16. */
+typedef struct infernt_paged_cache {
+    void* k;
+    void* v;
+    int num_pages;
+    int num_kv_heads;
+    int page_size; /* positions per page, any number from 1 */
+    int head_dim;  /* 64 or 128 */
+    int dtype;
+} infernt_paged_cache;
+
+/* New tokens of several sequences, rows [0, num_rows) of the token buffers:
+ * sequence s has the rows [q_start[s], q_start[s + 1]) and kv_len[s] positions
+ * in the cache, its new tokens (the last ones) included, so its i-th new
+ * token is at position kv_len[s] - (q_start[s + 1] - q_start[s]) + i.  A row
+ * whose position is negative (a batch padded in front) is a row without
+ * keys.  Position p of sequence s lives in page block_table[s * table_stride
+ * + p / page_size] at row p % page_size; entries past the sequence's last
+ * page are not read.  The three arrays are device memory and are read by the
+ * kernels, so a captured call follows their values at replay; num_seqs,
+ * num_rows and max_q_len are host values.  Rows at and after
+ * q_start[num_seqs] are left as they are.
+ *
+ * What the kernels cannot use sets a bit of *err (device word, or NULL)
+ * without an access out of range: bit 3, a page outside [0, num_pages) (its
+ * rows are read as zeros and are not written); bit 4, a
+ * sequence whose rows or length are out of range (q_start not ascending or
+ * above num_rows, more than max_q_len new tokens, kv_len negative, above
+ * table_stride x page_size or above 2^30): the sequence is skipped, its rows
+ * stay. */
+typedef struct infernt_ragged_batch {
+    const int* q_start;     /* [num_seqs + 1] */
+    const int* kv_len;      /* [num_seqs] */
+    const int* block_table; /* [num_seqs][table_stride] */
+    int num_seqs;           /* 0 to 65535 */
+    int num_rows;           /* rows of the token buffers, below 2^30 */
+    int max_q_len;          /* no sequence has more new tokens */
+    int table_stride;
+} infernt_ragged_batch;
+
+/* Rotary positions: pair i of the rotated part [0, rotary_dim) of a head is
+ * the elements (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when interleaved;
+ * at position p it turns by p f_i, f_i = theta^(-2 i / rotary_dim) scaled:
+ *   NONE    as it is
+ *   LINEAR  f / factor (position interpolation)
+ *   LLAMA3  t = original_max_len f / 2 pi turns over the original context:
+ *           f / factor below `low` turns, f above `high`, between them the
+ *           mean of the two weighted by (t - low) / (high - low)
+ *   YARN    f / factor for the pairs of few turns (`low`, usually 1), f for
+ *           those of many (`high`, usually 32), a ramp over the pair index
+ *           between the two borders; cosine and sine multiplied by
+ *           0.1 ln(factor) + 1
+ * Angles are reduced in 64 bits, so far positions lose nothing. */
+enum { INFERNT_ROPE_NONE = 0, INFERNT_ROPE_LINEAR = 1, INFERNT_ROPE_LLAMA3 = 2, INFERNT_ROPE_YARN = 3 };
+typedef struct infernt_rope_params {
+    double theta;
+    int rotary_dim; /* even, 2 to head_dim; the rest of a head is copied */
+    int interleaved;
+    int scaling;
+    int original_max_len;
+    double factor;
+    double low;
+    double high;
+} infernt_rope_params;
+
+/* q_out[r][h] = RoPE(q[r][h]) for the rows of the batch, and the RoPE'd K
+ * rows and the V rows into their pages, each rounded once to the cache's
+ * type (FP32 arithmetic).  q [num_rows][nq][head_dim], k and v [num_rows]
+ * [num_kv_heads][head_dim] of type src_dtype (F32, BF16 or F16), rows ldq,
+ * ldk and ldv elements apart (views of a stacked projection's rows, say);
+ * q_out of the cache's type, rows ldo apart.  q and q_out may be NULL (append
+ * only), or k and v (rotation only).  q_out may be q itself when the types
+ * and row strides agree.  Rows with a negative position are skipped.  Two
+ * sequences of a batch must not write the same row of a page. */
+INFERNT_API int infernt_paged_rope_append(void* q_out, int ldo, const void* q, int ldq, int nq, const void* k,
+                                          int ldk, const void* v, int ldv, int src_dtype,
+                                          const infernt_paged_cache* cache, const infernt_ragged_batch* batch,
+                                          const infernt_rope_params* rope, unsigned* err, void* stream);
+
+/* Attention of the batch's new tokens over the pages (their own K and V rows
+ * already appended): the token at position pos attends to the positions p <=
+ * pos of its sequence, with window > 0 only to p > pos - window and to the
+ * first `sinks` positions:
+ *   out[r][h] = sum_p w_p V[p] / sum_p w_p,  w_p = exp(scale q[r][h] . K[p]),
+ *   lse[r][h] = ln sum_p w_p
+ * of KV head h / (nq / num_kv_heads).  scale 0 means 1 / sqrt(head_dim).
+ * q and out [num_rows][nq][head_dim] of the cache's type, rows ldq and ldo
+ * elements apart (multiples of 8, pointers 16-byte aligned); lse [num_rows]
+ * [nq] FP32 or NULL.  A row without a visible key gets zeros and an lse of
+ * -infinity.  What lies in rows that a token does not see (unwritten rows of
+ * a page, NaN, infinity) does not reach its output.  FP32 scores, softmax
+ * statistics and sums; the probabilities enter the tensor cores in the
+ * cache's type.  nq a multiple of num_kv_heads, at most 128 query heads per
+ * KV head.
+ * workspace: infernt_paged_attention_workspace_bytes() bytes, zeroed once
+ * before its first use (calls leave its counters at zero; calls that share
+ * it must not overlap, two captured graphs among them).  Asynchronous; may
+ * be captured.  err as above; bit 0 if a bounded wait ran out. */
+INFERNT_API size_t infernt_paged_attention_workspace_bytes(void);
+INFERNT_API int infernt_paged_attention(void* out, int ldo, const void* q, int ldq, int nq,
+                                        const infernt_paged_cache* cache, const infernt_ragged_batch* batch,
+                                        int window, int sinks, float scale, float* lse, void* workspace,
+                                        unsigned* err, void* stream);
+
+/* Page src[i] into page dst[i], for i in [0, n), in each of n_pools pools
+ * (device pointers, 16-byte aligned) of num_pages pages of page_bytes bytes
+ * (a multiple of 16): every layer's K and V in one call.  pools, src and dst
+ * are host arrays, read before the call returns.  A page may be copied to
+ * several others; a destination may be neither another destination nor a
+ * source (INFERNT_ERR_INVALID_ARGUMENT).  Pools must not overlap.
+ * Asynchronous; may be captured. */
+INFERNT_API int infernt_pages_copy(void* const* pools, int n_pools, size_t page_bytes, int num_pages,
+                                   const int* src, const int* dst, int n, void* stream);
+/* infernt_pages_copy over every layer's K and V pools of a paged engine, on
+ * its stream, before its next step. */
+INFERNT_API int infernt_batch_engine_copy_pages(infernt_batch_engine* e, const int* src, const int* dst, int n);
+
+/* Which sequence holds which pages (host logic, no GPU): pages are counted
+ * by the sequences that hold them, so a fork shares them and a write to a
+ * shared page copies it first.  Calls that hand out pages fail as a whole
+ * with INFERNT_ERR_OUT_OF_MEMORY, changing nothing, when the pool has too
+ * few free ones.  The copies that a call reports (src[i] into dst[i], for
+ * infernt_pages_copy) must run before the pages are next written, and a
+ * caller's arrays hold at least num_pages entries. */
+typedef struct infernt_page_pool infernt_page_pool;
+INFERNT_API int infernt_page_pool_create(int num_pages, int page_size, int max_seqs, infernt_page_pool** out);
+INFERNT_API int infernt_page_pool_destroy(infernt_page_pool* pool);
+/* Pages for positions [0, n_positions) of seq: more are taken (the lowest
+ * free ones), surplus ones given back; 0 frees the sequence. */
+INFERNT_API int infernt_page_pool_resize(infernt_page_pool* pool, int seq, int n_positions);
+/* dst (which must hold no pages) shares src's pages of [0, n_positions). */
+INFERNT_API int infernt_page_pool_fork(infernt_page_pool* pool, int src_seq, int dst_seq, int n_positions);
+/* Before positions [from, to) of seq are written: each page of theirs that
+ * another sequence holds too is replaced by a free one and reported as a
+ * copy. */
+INFERNT_API int infernt_page_pool_write(infernt_page_pool* pool, int seq, int from, int to, int* src, int* dst,
+                                        int* n);
+/* Moves the highest pages in use into the lowest free ones until the pages
+ * in use are the lowest of the pool; tables of all sequences follow. */
+INFERNT_API int infernt_page_pool_compact(infernt_page_pool* pool, int* src, int* dst, int* n);
+/* The pages of seq (up to cap of them into pages) and their number. */
+INFERNT_API int infernt_page_pool_pages(infernt_page_pool* pool, int seq, int* pages, int cap, int* n);
+/* Free pages, pages held by more than one sequence, and the highest page in
+ * use (-1: none). */
+INFERNT_API int infernt_page_pool_stats(infernt_page_pool* pool, int* free_pages, int* shared_pages,
+                                        int* highest);
 
 /* ----------------------------------------- tensor parallelism ---
  * The 8B-class configuration decoded by tp_size GPUs, one process per GPU

@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libinfernt_b200.so")
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_F16 = 2  # the operators over paged caches
 
 # Phase-timeline fields (infernt_plan_set_trace): phase start, input loaded,
 # work done, barrier passed, producer issued last tile (ns); consumer wait
@@ -238,6 +239,19 @@ _SIGS = {
     "infernt_plan_set_wait_budget": (_I, [_P, ctypes.c_longlong]),
     "infernt_plan_set_stream_depth": (_I, [_P, _I]),
     "infernt_plan_stream_depth": (_I, [_P, _P, _P]),
+    "infernt_paged_rope_append": (_I, [_P, _I, _P, _I, _I, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "infernt_paged_attention_workspace_bytes": (_S, []),
+    "infernt_paged_attention": (_I, [_P, _I, _P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _P, _P]),
+    "infernt_pages_copy": (_I, [_P, _I, _S, _I, _P, _P, _I, _P]),
+    "infernt_batch_engine_copy_pages": (_I, [_P, _P, _P, _I]),
+    "infernt_page_pool_create": (_I, [_I, _I, _I, _P]),
+    "infernt_page_pool_destroy": (_I, [_P]),
+    "infernt_page_pool_resize": (_I, [_P, _I, _I]),
+    "infernt_page_pool_fork": (_I, [_P, _I, _I, _I]),
+    "infernt_page_pool_write": (_I, [_P, _I, _I, _I, _P, _P, _P]),
+    "infernt_page_pool_compact": (_I, [_P, _P, _P, _P]),
+    "infernt_page_pool_pages": (_I, [_P, _I, _P, _I, _P]),
+    "infernt_page_pool_stats": (_I, [_P, _P, _P, _P]),
 }
 
 IPC_HANDLE_BYTES = 64
@@ -468,6 +482,15 @@ class BatchEngine:
         a, b, c = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
         call("infernt_batch_engine_paging", self._h, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c))
         return a.value, b.value, c.value
+
+    def copy_pages(self, src, dst):
+        """Page src[i] into page dst[i] in every layer's K and V pools, before
+        the next step (infernt_batch_engine_copy_pages)."""
+        if len(src) != len(dst):
+            raise ValueError("copy_pages: %d sources, %d destinations" % (len(src), len(dst)))
+        n = len(src)
+        call("infernt_batch_engine_copy_pages", self._h, (ctypes.c_int * max(1, n))(*src),
+             (ctypes.c_int * max(1, n))(*dst), n)
 
     def set_salts(self, salts):
         """Per-sequence sampling salts (None: none)."""
@@ -854,3 +877,206 @@ class TPEngine:
         a, b = ctypes.c_int(), ctypes.c_int()
         call("infernt_plan_stream_depth", self._plan(), ctypes.byref(a), ctypes.byref(b))
         return a.value, b.value
+
+
+# ------------------------------------------ operators over paged caches
+_TORCH_DTYPES = {}
+
+
+def _dtype(t):
+    """DTYPE_* of a torch tensor."""
+    d = _TORCH_DTYPES.get(t.dtype)
+    if d is None:
+        d = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}.get(str(t.dtype))
+        if d is None:
+            raise ValueError("type %s (float32, bfloat16 or float16)" % t.dtype)
+        _TORCH_DTYPES[t.dtype] = d
+    return d
+
+
+def _ints(t, what):
+    """Device pointer of a contiguous int32 tensor."""
+    if str(t.dtype) != "torch.int32" or not t.is_contiguous():
+        raise ValueError("%s: a contiguous int32 tensor is needed" % what)
+    return t.data_ptr()
+
+
+class PagedCache(ctypes.Structure):
+    """``infernt_paged_cache``: the K and V pools of one layer, contiguous
+    tensors [num_pages][num_kv_heads][page_size][head_dim] of bfloat16 or
+    float16."""
+    _fields_ = [("k", _P), ("v", _P), ("num_pages", _I), ("num_kv_heads", _I), ("page_size", _I), ("head_dim", _I),
+                ("dtype", _I)]
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("PagedCache: k %s %s, v %s %s" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("PagedCache: the pools must be contiguous")
+        super().__init__(k.data_ptr(), v.data_ptr(), *k.shape, _dtype(k))
+        self.tensors = (k, v)
+
+
+class RaggedBatch(ctypes.Structure):
+    """``infernt_ragged_batch``: new tokens of several sequences.  q_start
+    [num_seqs + 1], kv_len [num_seqs] and block_table [num_seqs][pages per
+    sequence] are int32 device tensors, read when the kernels run."""
+    _fields_ = [("q_start", _P), ("kv_len", _P), ("block_table", _P), ("num_seqs", _I), ("num_rows", _I),
+                ("max_q_len", _I), ("table_stride", _I)]
+
+    def __init__(self, q_start, kv_len, block_table, num_rows, max_q_len):
+        n = kv_len.numel()
+        if q_start.numel() != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
+            raise ValueError("RaggedBatch: %d starts, %d lengths, table %s"
+                             % (q_start.numel(), n, tuple(block_table.shape)))
+        super().__init__(_ints(q_start, "q_start"), _ints(kv_len, "kv_len"), _ints(block_table, "block_table"), n,
+                         num_rows, max_q_len, block_table.shape[1])
+        self.tensors = (q_start, kv_len, block_table)
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
+
+
+class RopeParams(ctypes.Structure):
+    """``infernt_rope_params``; scaling is a name of ROPE_SCALINGS."""
+    _fields_ = [("theta", ctypes.c_double), ("rotary_dim", _I), ("interleaved", _I), ("scaling", _I),
+                ("original_max_len", _I), ("factor", ctypes.c_double), ("low", ctypes.c_double),
+                ("high", ctypes.c_double)]
+
+    def __init__(self, theta=10000.0, rotary_dim=128, interleaved=False, scaling="none", original_max_len=0,
+                 factor=1.0, low=1.0, high=4.0):
+        if scaling not in ROPE_SCALINGS:
+            raise ValueError("RopeParams: scaling %r (%s)" % (scaling, ", ".join(ROPE_SCALINGS)))
+        super().__init__(theta, rotary_dim, int(interleaved), ROPE_SCALINGS[scaling], original_max_len, factor, low,
+                         high)
+
+
+def _rows(t, rows, heads, dim, what):
+    """Row stride of a [rows][heads][dim] tensor whose heads lie next to each
+    other (a slice of stacked rows, for one)."""
+    if t.dim() != 3 or t.shape[0] < rows or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError("%s: shape %s for %d rows of %s heads of %d" % (what, tuple(t.shape), rows, heads, dim))
+    r, h, e = t.stride()
+    if e != 1 or (h != dim and t.shape[1] > 1):
+        raise ValueError("%s: strides %s; only rows may be apart" % (what, t.stride()))
+    # one row has no stride of its own
+    return r if t.shape[0] > 1 else max(r, t.shape[1] * dim)
+
+
+def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
+    """Rotary positions of the batch's q rows into q_out, the rotated k rows
+    and the v rows into their pages (infernt_paged_rope_append).  q and q_out,
+    or k and v, may be None.  stream: a cudaStream_t as an integer."""
+    n, dim = batch.num_rows, cache.head_dim
+    one = q if q is not None else k
+    nq = ldo = ldq = ldk = ldv = 0
+    if q is not None:
+        nq = q.shape[1]
+        ldq, ldo = _rows(q, n, None, dim, "q"), _rows(q_out, n, nq, dim, "q_out")
+        if _dtype(q_out) != cache.dtype:
+            raise ValueError("paged_rope_append: q_out has another type than the cache")
+    if k is not None:
+        ldk, ldv = _rows(k, n, cache.num_kv_heads, dim, "k"), _rows(v, n, cache.num_kv_heads, dim, "v")
+        if k.dtype != v.dtype or k.dtype != one.dtype:
+            raise ValueError("paged_rope_append: q, k and v of different types")
+    call("infernt_paged_rope_append", ptr(q_out), ldo, ptr(q), ldq, nq, ptr(k), ldk, ptr(v), ldv, _dtype(one),
+         ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(rope), ptr(err), stream)
+
+
+def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.0, lse=None, err=None, stream=None):
+    """Attention of the batch's new tokens over the pages
+    (infernt_paged_attention).  workspace: a zeroed uint8 tensor of
+    paged_attention_workspace_bytes() bytes."""
+    n, dim, nq = batch.num_rows, cache.head_dim, q.shape[1]
+    if _dtype(q) != cache.dtype or _dtype(out) != cache.dtype:
+        raise ValueError("paged_attention: q, out and the cache must have one type")
+    if lse is not None and (tuple(lse.shape[1:]) != (nq,) or lse.shape[0] < n or not lse.is_contiguous()
+                            or _dtype(lse) != DTYPE_F32):
+        raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(lse.shape), n, nq))
+    if workspace.numel() * workspace.element_size() < paged_attention_workspace_bytes():
+        raise ValueError("paged_attention: a workspace of %d bytes is needed" % paged_attention_workspace_bytes())
+    call("infernt_paged_attention", out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(),
+         _rows(q, n, None, dim, "q"), nq, ctypes.byref(cache), ctypes.byref(batch), window, sinks, scale, ptr(lse),
+         workspace.data_ptr(), ptr(err), stream)
+
+
+def paged_attention_workspace_bytes():
+    return lib().infernt_paged_attention_workspace_bytes()
+
+
+def copy_pages(pools, src, dst, stream=None):
+    """Page src[i] into page dst[i] in every pool (infernt_pages_copy): a
+    contiguous tensor [pools][pages][...], or a list of contiguous tensors
+    [pages][...] of one shape and type."""
+    if len(src) != len(dst):
+        raise ValueError("copy_pages: %d sources, %d destinations" % (len(src), len(dst)))
+    many = isinstance(pools, (list, tuple))
+    if many:
+        first = pools[0]
+        if any(p.shape != first.shape or p.dtype != first.dtype or not p.is_contiguous() for p in pools):
+            raise ValueError("copy_pages: the pools must be contiguous tensors of one shape and type")
+        base, count = [p.data_ptr() for p in pools], len(pools)
+    else:
+        if not pools.is_contiguous() or pools.dim() < 3:
+            raise ValueError("copy_pages: a contiguous tensor [pools][pages][...] is needed")
+        count, first = pools.shape[0], pools[0]
+        size = first.numel() * first.element_size()
+        base = [pools.data_ptr() + i * size for i in range(count)]
+    pages, n = first.shape[0], len(src)
+    call("infernt_pages_copy", (ctypes.c_void_p * max(1, count))(*base), count,
+         first.numel() // pages * first.element_size(), pages, (ctypes.c_int * max(1, n))(*src),
+         (ctypes.c_int * max(1, n))(*dst), n, stream)
+
+
+class PagePool:
+    """Which sequence holds which pages of a paged cache (infernt_page_pool_*;
+    host only).  write and compact return the copies (sources, destinations)
+    that copy_pages must run before the pages are next written."""
+
+    def __init__(self, num_pages, page_size, max_seqs):
+        h = ctypes.c_void_p()
+        call("infernt_page_pool_create", num_pages, page_size, max_seqs, ctypes.byref(h))
+        self._h, self.num_pages = h, num_pages
+
+    def close(self):
+        if self._h:
+            lib().infernt_page_pool_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def resize(self, seq, n_positions):
+        """Pages of seq for positions [0, n_positions); 0 frees it."""
+        call("infernt_page_pool_resize", self._h, seq, n_positions)
+
+    def fork(self, src_seq, dst_seq, n_positions):
+        """dst_seq shares src_seq's pages of [0, n_positions)."""
+        call("infernt_page_pool_fork", self._h, src_seq, dst_seq, n_positions)
+
+    def _copies(self, name, *args):
+        src, dst, n = (ctypes.c_int * self.num_pages)(), (ctypes.c_int * self.num_pages)(), ctypes.c_int()
+        call(name, self._h, *args, src, dst, ctypes.byref(n))
+        return src[:n.value], dst[:n.value]
+
+    def write(self, seq, start, stop):
+        """Copies to run before positions [start, stop) of seq are written."""
+        return self._copies("infernt_page_pool_write", seq, start, stop)
+
+    def compact(self):
+        """Moves the pages in use to the front of the pool."""
+        return self._copies("infernt_page_pool_compact")
+
+    def pages(self, seq):
+        out, n = (ctypes.c_int * self.num_pages)(), ctypes.c_int()
+        call("infernt_page_pool_pages", self._h, seq, out, self.num_pages, ctypes.byref(n))
+        return out[:n.value]
+
+    def stats(self):
+        """(free pages, pages held by several sequences, highest page in use)."""
+        a, b, c = ctypes.c_int(), ctypes.c_int(), ctypes.c_int()
+        call("infernt_page_pool_stats", self._h, ctypes.byref(a), ctypes.byref(b), ctypes.byref(c))
+        return a.value, b.value, c.value

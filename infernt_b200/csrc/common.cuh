@@ -20,6 +20,8 @@ enum : unsigned {
     kErrWaitTimeout = 1u << 0,   // an mbarrier / counter wait ran out of iterations
     kErrPosition = 1u << 1,      // decode position outside [0, max_seq_len)
     kErrToken = 1u << 2,         // token id outside [0, vocab_size)
+    kErrPage = 1u << 3,          // page id outside the pool
+    kErrBatch = 1u << 4,         // a ragged batch's rows or lengths out of range
 };
 
 // Iteration limit of every spin-wait (try_wait already suspends for a

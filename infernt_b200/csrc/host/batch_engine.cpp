@@ -855,6 +855,20 @@ int infernt_batch_engine_paging(infernt_batch_engine* e, int* page_size, int* nu
     return INFERNT_OK;
 }
 
+int infernt_batch_engine_copy_pages(infernt_batch_engine* e, const int* src, const int* dst, int n) {
+    INFERNT_REQUIRE(e, "batch_engine_copy_pages: null engine");
+    INFERNT_REQUIRE(e->page_size > 0, "batch_engine_copy_pages: the engine's caches are not paged");
+    std::vector<void*> pools;
+    try {
+        pools.insert(pools.end(), e->kc.begin(), e->kc.end());
+        pools.insert(pools.end(), e->vc.begin(), e->vc.end());
+    } catch (const std::bad_alloc&) {
+        return fail(INFERNT_ERR_OUT_OF_MEMORY, "batch_engine_copy_pages: host allocation failed");
+    }
+    return infernt_pages_copy(pools.data(), (int)pools.size(), (size_t)e->nkv_l * e->page_size * e->cfg.head_dim * 2,
+                              e->num_pages, src, dst, n, e->stream);
+}
+
 int infernt_batch_engine_set_salts(infernt_batch_engine* e, const uint64_t* salts) {
     INFERNT_REQUIRE(e, "batch_engine_set_salts: null engine");
     INFERNT_CUDA_TRY(cudaStreamSynchronize(e->stream));

@@ -1,0 +1,478 @@
+// paged_attention.cu — attention of the new tokens of a ragged batch over
+// paged KV caches, causal, with an optional sliding window and first tokens
+// that stay visible (cuda/attention.cu:9-42 and cuda/softmax.cu:13-48 are one
+// token of one sequence over a contiguous cache).
+//
+// For the token at position pos of a sequence and the query head h,
+//   s_p = scale q . K[p],  m = max s_p,  l = sum e^(s_p - m),
+//   out = sum e^(s_p - m) V[p] / l,  lse = m + ln l
+// over the p that it sees: p <= pos and (p > pos - window or p < sinks).
+// One pass over the keys with a running (m, l, out), in base 2.
+//
+// The query rows of a KV head are its new tokens times its G query heads,
+// row = token G + head of the group, so all rows of a tile share the K and V
+// rows that the tile reads, whatever G is.
+#include <cmath>
+#include <cstdint>
+
+#include "paged.cuh"
+#include "warp_mma.cuh"
+
+namespace infernt {
+namespace {
+
+constexpr int kTileKeys = 64;   // keys of a K / V tile
+constexpr int kItemRows = 64;   // query rows of an item: four warps of 16
+constexpr int kThreads = 128;
+constexpr int kStages = 3;
+constexpr float kRescale = 8.0f;  // log2 of the largest unnormalised probability
+constexpr size_t kWorkspaceBytes = 64u << 20;
+
+struct AttnArgs {
+    PagedBatch b;
+    const void* q;
+    void* out;
+    const void* k;
+    const void* v;
+    float* lse;
+    long long ldq, ldo;
+    int nq, G, window, sinks;
+    float scale, scale_log2;
+    unsigned* err;
+};
+
+// Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
+// keys that they see: [0, sink_end) and [lo, hi), as tiles of kTileKeys keys.
+struct Item {
+    int kvh, row0, rows;
+    int sink_end, lo, hi;  // hi: one past the last row's position (0 when it sees nothing)
+    int sink_tiles, tiles;
+    int pos_first, pos_last;
+};
+
+__device__ __forceinline__ int row_pos(const PagedSeq& s, int token) { return s.len - s.n_new + token; }
+
+__device__ __forceinline__ Item make_item(const AttnArgs& a, const PagedSeq& s, int kvh, int row0) {
+    Item it;
+    it.kvh = kvh;
+    it.row0 = row0;
+    it.rows = min(kItemRows, s.n_new * a.G - row0);
+    it.pos_first = row_pos(s, row0 / a.G);
+    it.pos_last = row_pos(s, (row0 + it.rows - 1) / a.G);
+    it.hi = max(0, it.pos_last + 1);
+    it.lo = a.window > 0 ? max(0, it.pos_first - a.window + 1) : 0;
+    it.sink_end = min(a.sinks, it.lo);
+    const int lo_tile = it.lo / kTileKeys;
+    it.sink_tiles = min((it.sink_end + kTileKeys - 1) / kTileKeys, lo_tile);
+    it.tiles = it.hi > 0 ? it.sink_tiles + (it.hi - 1) / kTileKeys - lo_tile + 1 : 0;
+    return it;
+}
+
+__device__ __forceinline__ int tile_key(const Item& it, int j) {
+    return (j < it.sink_tiles ? j : it.lo / kTileKeys + (j - it.sink_tiles)) * kTileKeys;
+}
+
+// Whether some row of the item sees key p.
+__device__ __forceinline__ bool item_sees(const Item& it, int p) {
+    return p < it.hi && (p >= it.lo || p < it.sink_end);
+}
+
+// Pool row of position p of sequence s for KV head kvh, or -1 (a page that
+// the pool does not have).
+__device__ __forceinline__ int pool_row(const PagedBatch& b, int s, int kvh, int p, unsigned* err) {
+    const int pi = p / b.page_size, page = b.table[(size_t)s * b.table_stride + pi];
+    if (page < 0 || page >= b.num_pages) {
+        if (err) atomicOr(err, kErrPage);
+        return -1;
+    }
+    return (page * b.nkv + kvh) * b.page_size + (p - pi * b.page_size);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                                         uint32_t b1) {
+    mma_bf16_16816(c, a, b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// One row by one warp, term by term: what a row is computed with when its
+// result is not finite.  The tiles above multiply a hidden position's value
+// by a probability of 0, which is NaN where the value is infinite or NaN;
+// here only what the row sees is touched, so what a row does see that is not
+// finite still shows in its result as in the formula.
+template <typename T, int D>
+__device__ void exact_row(const AttnArgs& a, const PagedSeq& seq, int s, int kvh, int row) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31, token = row / a.G, head = kvh * a.G + row % a.G;
+    const int pos = row_pos(seq, token);
+    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, sink_end = min(a.sinks, lo);
+    const T* q = static_cast<const T*>(a.q) + (long long)(seq.row0 + token) * a.ldq + (long long)head * D + lane * E;
+    float qv[E], acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        qv[e] = Half16<T>::value(q[e]);
+        acc[e] = 0.0f;
+    }
+    float m = -INFINITY, l = 0.0f;
+    for (int p = 0; p <= pos; ++p) {
+        if (p == sink_end) p = lo;  // lo <= pos
+        const int r = pool_row(a.b, s, kvh, p, a.err);
+        const T* k = static_cast<const T*>(a.k) + (long long)r * D + lane * E;
+        const T* v = static_cast<const T*>(a.v) + (long long)r * D + lane * E;
+        float dot = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) dot = fmaf(qv[e], r >= 0 ? Half16<T>::value(k[e]) : 0.0f, dot);
+        const float sc = warp_sum(dot) * a.scale, m_new = fmaxf(m, sc);
+        const float f = m == -INFINITY ? 0.0f : expf(m - m_new), w = expf(sc - m_new);
+        l = l * f + w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + w * (r >= 0 ? Half16<T>::value(v[e]) : 0.0f);
+        m = m_new;
+    }
+    T* o = static_cast<T*>(a.out) + (long long)(seq.row0 + token) * a.ldo + (long long)head * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = Half16<T>::round(acc[e] / l);
+    if (a.lse && lane == 0) a.lse[(long long)(seq.row0 + token) * a.nq + head] = m + logf(l);
+}
+
+// Shared memory: the ring of K / V tiles (reused for the merge of the warps'
+// results), the pool rows of two tiles, and a flag per query row.
+template <int D>
+struct Layout {
+    static constexpr int kRowBytes = D * 2;
+    static constexpr int kTileBytes = kTileKeys * kRowBytes;
+    static constexpr int kRing = kStages * 2 * kTileBytes;
+    static constexpr int kBytes = kRing + 2 * kTileKeys * 4 + kItemRows;
+};
+
+// The tiles [j0, j1) of an item by four warps: RB blocks of 16 rows, each by
+// 4 / RB warps that share a tile's keys between them.  Leaves every warp's
+// (m, l, out) of its rows in shared memory: slot (key share, row) of
+// `m_s`, `l_s` and `o_s`.
+template <typename T, int D, int RB>
+__device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq, int s, const Item& it, int j0,
+                                          int j1, unsigned char* smem) {
+    using L = Layout<D>;
+    constexpr int KS = 4 / RB, WK = kTileKeys / KS, NT = WK / 8;  // key shares, keys and n-tiles per warp
+    constexpr int CH = L::kRowBytes / 16, KC = D / 16, DB = D / 8;
+    constexpr int ROWS_PER_PASS = kThreads / CH, PASSES = kTileKeys / ROWS_PER_PASS;
+    int* rows_s = reinterpret_cast<int*>(smem + L::kRing);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
+    const int rb = warp % RB, ks = warp / RB;
+    const uint32_t ring = smem_addr(smem);
+    const unsigned char* kb = static_cast<const unsigned char*>(a.k);
+    const unsigned char* vb = static_cast<const unsigned char*>(a.v);
+
+    // pool row of key `tid` of tile j; -1 where no row of the item sees it
+    auto row_of = [&](int j) {
+        if (tid >= kTileKeys || j >= j1) return -1;
+        const int p = tile_key(it, j) + tid;
+        return item_sees(it, p) ? pool_row(a.b, s, it.kvh, p, a.err) : -1;
+    };
+    // tile j into stage (j - j0) % kStages; rows that nobody sees become zeros
+    auto issue = [&](int j) {
+        if (j < j1) {
+            const uint32_t st = ring + (uint32_t)((j - j0) % kStages) * 2 * L::kTileBytes;
+            const int* rows = rows_s + (j & 1) * kTileKeys;
+#pragma unroll
+            for (int e = 0; e < PASSES; ++e) {
+                const int row = e * ROWS_PER_PASS + tid / CH, ch = tid % CH;
+                const int pr = rows[row];
+                const size_t off = (size_t)(pr < 0 ? 0 : pr) * L::kRowBytes + ch * 16;
+                const uint32_t dst = st + (uint32_t)(row * L::kRowBytes + ((ch ^ (row & 7)) << 4));
+                cp_async16(dst, kb + off, pr < 0 ? 0u : 16u);
+                cp_async16(dst + L::kTileBytes, vb + off, pr < 0 ? 0u : 16u);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (tid < kTileKeys) rows_s[((j0 + i) & 1) * kTileKeys + tid] = row_of(j0 + i);
+        __syncthreads();
+        issue(j0 + i);
+    }
+    if (tid < kTileKeys) {
+        const int r = row_of(j0 + kStages - 1);
+        rows_s[((j0 + kStages - 1) & 1) * kTileKeys + tid] = r;  // its slot was read two issues ago
+    }
+
+    // query fragments of rows g and g + 8 of the warp's block
+    uint32_t qa[KC][4];
+    int pos[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = rb * 16 + g + 8 * h, row = it.row0 + r, token = row / a.G;
+        const bool ok = r < it.rows;
+        pos[h] = ok ? row_pos(seq, token) : -1;
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(
+            static_cast<const uint16_t*>(a.q) + (ok ? (long long)(seq.row0 + token) * a.ldq +
+                                                          (long long)(it.kvh * a.G + row % a.G) * D + 2 * tig
+                                                    : 0));
+#pragma unroll
+        for (int k = 0; k < KC; ++k) {
+            qa[k][h] = ok ? q[8 * k] : 0u;
+            qa[k][h + 2] = ok ? q[8 * k + 4] : 0u;
+        }
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float acc[DB][4];
+#pragma unroll
+    for (int b = 0; b < DB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.0f;
+    const bool busy = rb * 16 < it.rows;
+
+    for (int j = j0; j < j1; ++j) {
+        cp_async_wait<kStages - 2>();  // this thread's copies of tile j have landed
+        __syncthreads();               // everyone's, the rows of tile j + 2 too; tile j - 1's stage is free
+        issue(j + kStages - 1);
+        const int next = row_of(j + kStages);
+        if (busy) {
+            const int k0 = tile_key(it, j);
+            const uint32_t kt = ring + (uint32_t)((j - j0) % kStages) * 2 * L::kTileBytes, vt = kt + L::kTileBytes;
+            float sc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KC; ++k)
+#pragma unroll
+                for (int n = 0; n < NT / 2; ++n) {
+                    const int x = lane >> 3, row = ks * WK + 8 * (2 * n + (x >> 1)) + (lane & 7), ch = 2 * k + (x & 1);
+                    uint32_t b0, b1, b2, b3;
+                    ldsm_x4(kt + (uint32_t)(row * L::kRowBytes + ((ch ^ (row & 7)) << 4)), b0, b1, b2, b3);
+                    mma_16816<T>(sc[2 * n], qa[k], b0, b1);
+                    mma_16816<T>(sc[2 * n + 1], qa[k], b2, b3);
+                }
+            // a tile that every row sees whole needs no mask
+            const bool whole = k0 + kTileKeys - 1 <= it.pos_first &&
+                               (a.window == 0 || k0 > it.pos_last - a.window || k0 + kTileKeys <= a.sinks);
+            float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int h = e >> 1, p = k0 + ks * WK + 8 * n + 2 * tig + (e & 1);
+                    const bool sees = whole || (p <= pos[h] && (a.window == 0 || p > pos[h] - a.window || p < a.sinks));
+                    sc[n][e] = sees ? sc[n][e] * a.scale_log2 : -INFINITY;
+                    mx[h] = fmaxf(mx[h], sc[n][e]);
+                }
+            bool grow = false;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                grow |= mx[h] > m[h] + kRescale;
+            }
+            // the reference maximum moves only when probabilities would pass 2^8
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float n = fmaxf(m[h], mx[h]);
+                    const float f = m[h] == -INFINITY ? 0.0f : ex2(m[h] - n);
+                    m[h] = n;
+                    l[h] *= f;
+#pragma unroll
+                    for (int b = 0; b < DB; ++b) {
+                        acc[b][2 * h] *= f;
+                        acc[b][2 * h + 1] *= f;
+                    }
+                }
+            }
+            const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[n][e] = ex2(sc[n][e] - ref[e >> 1]);
+                    l[e >> 1] += sc[n][e];
+                }
+            // the score fragments of two n-tiles are the A fragment of 16 probabilities
+#pragma unroll
+            for (int kk = 0; kk < NT / 2; ++kk) {
+                const uint32_t pa[4] = {Half16<T>::pack(sc[2 * kk][0], sc[2 * kk][1]),
+                                        Half16<T>::pack(sc[2 * kk][2], sc[2 * kk][3]),
+                                        Half16<T>::pack(sc[2 * kk + 1][0], sc[2 * kk + 1][1]),
+                                        Half16<T>::pack(sc[2 * kk + 1][2], sc[2 * kk + 1][3])};
+#pragma unroll
+                for (int b = 0; b < DB / 2; ++b) {
+                    const int x = lane >> 3, row = ks * WK + 16 * kk + 8 * (x & 1) + (lane & 7), ch = 2 * b + (x >> 1);
+                    uint32_t v0, v1, v2, v3;
+                    ldsm_x4_trans(vt + (uint32_t)(row * L::kRowBytes + ((ch ^ (row & 7)) << 4)), v0, v1, v2, v3);
+                    mma_16816<T>(acc[2 * b], pa, v0, v1);
+                    mma_16816<T>(acc[2 * b + 1], pa, v2, v3);
+                }
+            }
+        }
+        if (tid < kTileKeys) rows_s[((j + kStages) & 1) * kTileKeys + tid] = next;
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // the ring is free
+    float* o_s = reinterpret_cast<float*>(smem);           // [KS][RB 16][D]
+    float* m_s = o_s + 4 * 16 * D;                          // [KS][RB 16]
+    float* l_s = m_s + 64;
+    if (busy) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            const int slot = (ks * RB + rb) * 16 + g + 8 * h;
+            if (tig == 0) {
+                m_s[slot] = m[h];
+                l_s[slot] = l[h];
+            }
+#pragma unroll
+            for (int b = 0; b < DB; ++b)
+                *reinterpret_cast<float2*>(o_s + slot * D + 8 * b + 2 * tig) =
+                    make_float2(acc[b][2 * h], acc[b][2 * h + 1]);
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) paged_attn(const AttnArgs a) {
+    using L = Layout<D>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int tid = threadIdx.x;
+    // Item blockIdx.x / nkv: sequence s has the items from
+    // floor(q_start[s] G / 64) + s on, which leaves room for its own
+    const int kvh = blockIdx.x % a.b.nkv, slot = blockIdx.x / a.b.nkv;
+    int lo = 0, hi = a.b.num_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if ((long long)a.b.q_start[mid] * a.G / kItemRows + mid <= slot)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const PagedSeq seq = paged_seq(a.b, lo, tid == 0 ? a.err : nullptr);
+    const long long first = (long long)seq.row0 * a.G / kItemRows + lo;
+    const long long row0 = (slot - first) * kItemRows;
+    if (row0 < 0 || row0 >= (long long)seq.n_new * a.G) return;
+    const Item it = make_item(a, seq, kvh, (int)row0);
+    int shares = 4;
+    if (it.rows <= 16)
+        run_tiles<T, D, 1>(a, seq, lo, it, 0, it.tiles, smem);
+    else if (it.rows <= 32) {
+        run_tiles<T, D, 2>(a, seq, lo, it, 0, it.tiles, smem);
+        shares = 2;
+    } else {
+        run_tiles<T, D, 4>(a, seq, lo, it, 0, it.tiles, smem);
+        shares = 1;
+    }
+    const float* o_s = reinterpret_cast<const float*>(smem);
+    const float* m_s = o_s + 4 * 16 * D;
+    const float* l_s = m_s + 64;
+    unsigned char* flag = smem + L::kRing + 2 * kTileKeys * 4;
+    if (tid < kItemRows) flag[tid] = 0;
+    __syncthreads();
+    const int stride = 64 / shares;  // rows of one share
+    for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
+        const int r = e / (D / 2), d = 2 * (e % (D / 2));
+        const int row = it.row0 + r, token = row / a.G, head = kvh * a.G + row % a.G;
+        float M = -INFINITY;
+        for (int k = 0; k < shares; ++k) M = fmaxf(M, m_s[k * stride + r]);
+        float lsum = 0.0f, x = 0.0f, y = 0.0f;
+        for (int k = 0; k < shares; ++k) {
+            const float mk = m_s[k * stride + r], f = mk == -INFINITY ? 0.0f : ex2(mk - M);
+            const float2 o = *reinterpret_cast<const float2*>(o_s + (k * stride + r) * D + d);
+            lsum = fmaf(l_s[k * stride + r], f, lsum);
+            x = fmaf(o.x, f, x);
+            y = fmaf(o.y, f, y);
+        }
+        float lse;
+        if (row_pos(seq, token) < 0) {
+            x = y = 0.0f;
+            lse = -INFINITY;
+        } else {
+            const float inv = 1.0f / lsum;
+            x *= inv;
+            y *= inv;
+            lse = (M + log2f(lsum)) * 0.6931471805599453f;
+            if (!(fabsf(x) < INFINITY && fabsf(y) < INFINITY)) flag[r] = 1;
+        }
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + token) * a.ldo +
+                                     (long long)head * D + d) = Half16<T>::pack(x, y);
+        if (a.lse && d == 0) a.lse[(long long)(seq.row0 + token) * a.nq + head] = lse;
+    }
+    __syncthreads();
+    for (int r = tid >> 5; r < it.rows; r += kThreads / 32)
+        if (flag[r]) exact_row<T, D>(a, seq, lo, kvh, it.row0 + r);
+}
+
+template <typename T, int D>
+int launch(const AttnArgs& a, cudaStream_t st) {
+    using L = Layout<D>;
+    static_assert(4 * 16 * D * 4 + 2 * 64 * 4 <= L::kRing, "the merge must fit the ring");
+    INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+    const long long ctas = ((long long)a.b.num_rows * a.G / kItemRows + a.b.num_seqs) * a.b.nkv;
+    INFERNT_REQUIRE(ctas < (1ll << 31), "paged_attention: %lld items", ctas);
+    paged_attn<T, D><<<(unsigned)ctas, kThreads, L::kBytes, st>>>(a);
+    INFERNT_CUDA_TRY(cudaGetLastError());
+    return INFERNT_OK;
+}
+
+}  // namespace
+}  // namespace infernt
+
+extern "C" size_t infernt_paged_attention_workspace_bytes(void) { return infernt::kWorkspaceBytes; }
+
+extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ldq, int nq,
+                                       const infernt_paged_cache* cache, const infernt_ragged_batch* batch, int window,
+                                       int sinks, float scale, float* lse, void* workspace, unsigned* err,
+                                       void* stream) {
+    using namespace infernt;
+    const char* op = "paged_attention";
+    if (int s = check_paged_cache(op, cache)) return s;
+    if (int s = check_ragged_batch(op, batch)) return s;
+    INFERNT_REQUIRE(q && out && workspace, "%s: null pointer", op);
+    const int D = cache->head_dim, nkv = cache->num_kv_heads;
+    INFERNT_REQUIRE(nq >= 1 && nq % nkv == 0 && nq / nkv <= 128, "%s: %d query heads, %d KV heads", op, nq, nkv);
+    INFERNT_REQUIRE(ldq >= (long long)nq * D && ldo >= (long long)nq * D && ldq % 8 == 0 && ldo % 8 == 0,
+                    "%s: rows %d and %d apart for %d heads of %d (multiples of 8)", op, ldq, ldo, nq, D);
+    INFERNT_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace),
+                    "%s: q, out and workspace must be 16-byte aligned", op);
+    INFERNT_REQUIRE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "%s: window %d, sinks %d", op, window,
+                    sinks);
+    INFERNT_REQUIRE(std::isfinite(scale), "%s: scale", op);
+    INFERNT_REQUIRE((long long)batch->num_rows * (nq / nkv) < (1ll << 31), "%s: %d rows of %d heads", op,
+                    batch->num_rows, nq);
+    if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
+    if (int s = check_device_pointer(op, "the cache", cache->k)) return s;
+    if (int s = check_device_pointer(op, "q", q)) return s;
+    if (int s = check_device_pointer(op, "out", out)) return s;
+    AttnArgs a;
+    a.b = paged_batch(*cache, *batch);
+    a.q = q;
+    a.out = out;
+    a.k = cache->k;
+    a.v = cache->v;
+    a.lse = lse;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.nq = nq;
+    a.G = nq / nkv;
+    a.window = window < kMaxPositions ? window : kMaxPositions;
+    a.sinks = sinks;
+    a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)D);
+    a.scale_log2 = a.scale * 1.4426950408889634f;
+    a.err = err;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (cache->dtype == INFERNT_DTYPE_BF16)
+        return D == 64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
+    return D == 64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+}

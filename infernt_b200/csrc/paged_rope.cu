@@ -1,0 +1,268 @@
+// paged_rope.cu — rotary positions of a ragged batch of new tokens and the
+// append of their K and V rows into pages (cuda/rope.cu:13-34 and
+// cuda/kv_cache.cu:4-14 are one token of one sequence, split-half, unscaled).
+//
+//   (x, y) -> m (x cos a - y sin a, y cos a + x sin a),  a = p f_i
+//
+// for the pairs of the rotated part of each q and k head.  Positions run to
+// 10^5 and more, where an FP32 product p f_i is off by 10^-2 radians, so
+// f_i / 2 pi is held in 64 bits: p f_i / 2 pi mod 1 is exact to about 2^-36
+// at p = 2^17 and enters the FP32 sine and cosine as a fraction of a turn.
+#include <cmath>
+#include <cstdint>
+
+#include "paged.cuh"
+
+namespace infernt {
+
+int check_paged_cache(const char* op, const infernt_paged_cache* c) {
+    INFERNT_REQUIRE(c && c->k && c->v, "%s: null cache", op);
+    INFERNT_REQUIRE(c->num_pages >= 1 && c->num_kv_heads >= 1 && c->page_size >= 1,
+                    "%s: %d pages of %d positions, %d KV heads", op, c->num_pages, c->page_size, c->num_kv_heads);
+    // page rows are counted in 32 bits, bytes in 64
+    INFERNT_REQUIRE((long long)c->num_kv_heads * c->page_size < (1ll << 31) &&
+                        (long long)c->num_pages * ((long long)c->num_kv_heads * c->page_size) < (1ll << 31),
+                    "%s: a pool of 2^31 rows or more", op);
+    INFERNT_REQUIRE(c->head_dim == 64 || c->head_dim == 128, "%s: head_dim %d (64 or 128)", op, c->head_dim);
+    INFERNT_REQUIRE(c->dtype == INFERNT_DTYPE_BF16 || c->dtype == INFERNT_DTYPE_F16, "%s: cache type %d (bf16 or fp16)",
+                    op, c->dtype);
+    INFERNT_REQUIRE(aligned16(c->k) && aligned16(c->v), "%s: pools not 16-byte aligned", op);
+    return INFERNT_OK;
+}
+
+int check_ragged_batch(const char* op, const infernt_ragged_batch* b) {
+    INFERNT_REQUIRE(b, "%s: null batch", op);
+    INFERNT_REQUIRE(b->num_seqs >= 0 && b->num_seqs <= 65535 && b->num_rows >= 0 && b->num_rows < kMaxPositions &&
+                        b->max_q_len >= 0 && b->table_stride >= 0,
+                    "%s: %d sequences, %d rows, at most %d new tokens, table rows of %d", op, b->num_seqs, b->num_rows,
+                    b->max_q_len, b->table_stride);
+    INFERNT_REQUIRE(b->num_seqs == 0 || (b->q_start && b->kv_len && (b->block_table || b->table_stride == 0)),
+                    "%s: null batch array", op);
+    return INFERNT_OK;
+}
+
+int check_device_pointer(const char* op, const char* what, const void* p) {
+    cudaPointerAttributes at;
+    INFERNT_CUDA_TRY(cudaPointerGetAttributes(&at, p));
+    INFERNT_REQUIRE(at.type == cudaMemoryTypeManaged ||
+                        (at.type == cudaMemoryTypeDevice && at.device == current_device()),
+                    "%s: %s is not memory of the current device", op, what);
+    return INFERNT_OK;
+}
+
+namespace {
+
+constexpr int kRopeThreads = 128;
+constexpr int kMaxPairs = 64;
+
+struct RopeDev {
+    double turns[kMaxPairs];  // f_i / 2 pi
+    float magnitude;
+    int half, interleaved;
+};
+
+struct RopeArgs {
+    PagedBatch b;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    void* kp;
+    void* vp;
+    long long ldq, ldk, ldv, ldo;
+    int nq, D;
+    unsigned* err;
+};
+
+// The sequence that holds row r (the last s with q_start[s] <= r), by a
+// search of 32 places a round: one round trip for up to 32 sequences, two
+// for up to 1024.  Whatever the array holds, the result is in [0, n).
+__device__ __forceinline__ int find_seq(const int* q_start, int n, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n;  // the answer is in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int at = lo + lane * step;
+        const unsigned le = __ballot_sync(0xffffffffu, at < hi && q_start[at] <= r);
+        const int k = le ? 31 - __clz(le) : 0;
+        lo = lo + k * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
+template <typename S>
+__device__ __forceinline__ float source_value(const S* p) {
+    return to_f32(*p);
+}
+template <>
+__device__ __forceinline__ float source_value<__half>(const __half* p) {
+    return __half2float(*p);
+}
+
+// One block per token row.  Thread: the rotated pairs of the q and k heads,
+// then the elements that are copied.
+template <typename S, typename T>
+__global__ void __launch_bounds__(kRopeThreads) paged_rope(const RopeArgs a, const RopeDev rope) {
+    __shared__ float2 cs[kMaxPairs];
+    const int r = blockIdx.x, tid = threadIdx.x, D = a.D, half = rope.half, nkv = a.b.nkv;
+    const int s = find_seq(a.b.q_start, a.b.num_seqs, r);
+    const PagedSeq seq = paged_seq(a.b, s, a.err);
+    const int i = r - seq.row0;
+    if (i < 0 || i >= seq.n_new) return;  // behind the last sequence, or a sequence that is skipped
+    const int pos = seq.len - seq.n_new + i;
+    if (pos < 0) return;
+    if (tid < half) {
+        const double t = (double)pos * rope.turns[tid];
+        const float f = (float)(t - rint(t));  // [-1/2, 1/2] turns
+        float sn, c;
+        sincospif(2.0f * f, &sn, &c);
+        cs[tid] = make_float2(c * rope.magnitude, sn * rope.magnitude);
+    }
+    long long row = -1;  // the page row of head 0
+    if (a.k) {
+        const int page = a.b.table[(size_t)s * a.b.table_stride + pos / a.b.page_size];
+        if (page >= 0 && page < a.b.num_pages)
+            row = (long long)page * nkv * a.b.page_size + pos % a.b.page_size;
+        else if (a.err && tid == 0)
+            atomicOr(a.err, kErrPage);
+    }
+    __syncthreads();
+    const int heads = (a.q ? a.nq : 0) + (row >= 0 ? nkv : 0), h0 = a.q ? 0 : a.nq;
+    auto src_of = [&](int h) {
+        return h < a.nq ? static_cast<const S*>(a.q) + r * a.ldq + (long long)h * D
+                        : static_cast<const S*>(a.k) + r * a.ldk + (long long)(h - a.nq) * D;
+    };
+    auto dst_of = [&](int h) {
+        return h < a.nq ? static_cast<T*>(a.q_out) + r * a.ldo + (long long)h * D
+                        : static_cast<T*>(a.kp) + (row + (long long)(h - a.nq) * a.b.page_size) * D;
+    };
+    for (int u = tid; u < heads * half; u += kRopeThreads) {
+        const int h = h0 + u / half, p = u % half;
+        const int e0 = rope.interleaved ? 2 * p : p, e1 = rope.interleaved ? 2 * p + 1 : p + half;
+        const S* src = src_of(h);
+        T* dst = dst_of(h);
+        const float x = source_value(src + e0), y = source_value(src + e1);
+        dst[e0] = Half16<T>::round(x * cs[p].x - y * cs[p].y);
+        dst[e1] = Half16<T>::round(y * cs[p].x + x * cs[p].y);
+    }
+    const int rest = D - 2 * half;
+    for (int u = tid; u < heads * rest; u += kRopeThreads) {
+        const int h = h0 + u / rest, e = 2 * half + u % rest;
+        dst_of(h)[e] = Half16<T>::round(source_value(src_of(h) + e));
+    }
+    if (row >= 0)
+        for (int u = tid; u < nkv * D; u += kRopeThreads) {
+            const int h = u / D, e = u % D;
+            static_cast<T*>(a.vp)[(row + (long long)h * a.b.page_size) * D + e] =
+                Half16<T>::round(source_value(static_cast<const S*>(a.v) + r * a.ldv + u));
+        }
+}
+
+int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
+    const int R = p.rotary_dim;
+    INFERNT_REQUIRE(R >= 2 && R <= head_dim && R % 2 == 0, "paged_rope_append: rotary_dim %d of %d", R, head_dim);
+    INFERNT_REQUIRE(std::isfinite(p.theta) && p.theta > 0, "paged_rope_append: theta %g", p.theta);
+    INFERNT_REQUIRE(p.scaling >= INFERNT_ROPE_NONE && p.scaling <= INFERNT_ROPE_YARN, "paged_rope_append: scaling %d",
+                    p.scaling);
+    INFERNT_REQUIRE(p.scaling == INFERNT_ROPE_NONE || (std::isfinite(p.factor) && p.factor > 0),
+                    "paged_rope_append: factor %g", p.factor);
+    if (p.scaling == INFERNT_ROPE_LLAMA3 || p.scaling == INFERNT_ROPE_YARN)
+        INFERNT_REQUIRE(p.original_max_len >= 1 && std::isfinite(p.low) && std::isfinite(p.high) && p.low > 0 &&
+                            p.high > p.low,
+                        "paged_rope_append: original_max_len %d, low %g, high %g", p.original_max_len, p.low, p.high);
+    INFERNT_REQUIRE(p.scaling != INFERNT_ROPE_YARN || p.theta > 1.0, "paged_rope_append: YaRN needs theta above 1");
+    const double two_pi = 6.283185307179586476925;
+    double lo = 0, hi = 0;
+    out->half = R / 2;
+    out->interleaved = p.interleaved != 0;
+    out->magnitude = 1.0f;
+    if (p.scaling == INFERNT_ROPE_YARN) {
+        // the pair index at which a pair makes t turns over the original context
+        auto border = [&](double t) { return R * std::log(p.original_max_len / (t * two_pi)) / (2 * std::log(p.theta)); };
+        lo = std::fmax(0.0, std::floor(border(p.high)));
+        hi = std::fmin(R - 1.0, std::ceil(border(p.low)));
+        out->magnitude = (float)(0.1 * std::log(p.factor) + 1.0);
+    }
+    // f_i by repeated products: 64 of them are off by 64 x 2^-53
+    const double ratio = std::pow(p.theta, -2.0 / R);
+    double f = 1.0;
+    for (int i = 0; i < R / 2; ++i, f *= ratio) {
+        double g = f, keep = 1.0;  // share of f, the rest is f / factor
+        if (p.scaling == INFERNT_ROPE_LINEAR) keep = 0.0;
+        if (p.scaling == INFERNT_ROPE_LLAMA3)
+            keep = (p.original_max_len * f / two_pi - p.low) / (p.high - p.low);
+        if (p.scaling == INFERNT_ROPE_YARN) keep = 1.0 - (i - lo) / std::fmax(hi - lo, 0.001);
+        keep = std::fmin(1.0, std::fmax(0.0, keep));
+        if (p.scaling != INFERNT_ROPE_NONE) g = f * keep + f / p.factor * (1.0 - keep);
+        out->turns[i] = g / two_pi;
+    }
+    return INFERNT_OK;
+}
+
+template <typename S, typename T>
+int launch(const RopeArgs& a, const RopeDev& d, cudaStream_t st) {
+    paged_rope<S, T><<<a.b.num_rows, kRopeThreads, 0, st>>>(a, d);
+    INFERNT_CUDA_TRY(cudaGetLastError());
+    return INFERNT_OK;
+}
+
+template <typename T>
+int launch_src(const RopeArgs& a, const RopeDev& d, int src, cudaStream_t st) {
+    if (src == INFERNT_DTYPE_F32) return launch<float, T>(a, d, st);
+    if (src == INFERNT_DTYPE_BF16) return launch<__nv_bfloat16, T>(a, d, st);
+    return launch<__half, T>(a, d, st);
+}
+
+}  // namespace
+}  // namespace infernt
+
+extern "C" int infernt_paged_rope_append(void* q_out, int ldo, const void* q, int ldq, int nq, const void* k, int ldk,
+                                         const void* v, int ldv, int src_dtype, const infernt_paged_cache* cache,
+                                         const infernt_ragged_batch* batch, const infernt_rope_params* rope,
+                                         unsigned* err, void* stream) {
+    using namespace infernt;
+    const char* op = "paged_rope_append";
+    if (int s = check_paged_cache(op, cache)) return s;
+    if (int s = check_ragged_batch(op, batch)) return s;
+    INFERNT_REQUIRE(rope, "%s: null rope parameters", op);
+    INFERNT_REQUIRE((q != nullptr) == (q_out != nullptr) && (k != nullptr) == (v != nullptr) && (q || k),
+                    "%s: q with q_out, k with v", op);
+    INFERNT_REQUIRE(src_dtype == INFERNT_DTYPE_F32 || src_dtype == INFERNT_DTYPE_BF16 || src_dtype == INFERNT_DTYPE_F16,
+                    "%s: source type %d", op, src_dtype);
+    const int D = cache->head_dim;
+    const long long kvd = (long long)cache->num_kv_heads * D;
+    INFERNT_REQUIRE(!q || (nq >= 1 && ldq >= (long long)nq * D && ldo >= (long long)nq * D),
+                    "%s: %d query heads, rows %d and %d apart", op, nq, ldq, ldo);
+    INFERNT_REQUIRE(!k || (ldk >= kvd && ldv >= kvd), "%s: k and v rows %d and %d apart for %lld values", op, ldk, ldv,
+                    kvd);
+    INFERNT_REQUIRE(!q || q != q_out || (src_dtype == cache->dtype && ldq == ldo),
+                    "%s: q_out may be q only with its type and row stride", op);
+    const unsigned esize = src_dtype == INFERNT_DTYPE_F32 ? 4u : 2u;
+    for (const void* p : {q, k, v})
+        INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(p) % esize == 0, "%s: misaligned source", op);
+    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(q_out) % 2 == 0, "%s: misaligned q_out", op);
+    RopeArgs a;
+    RopeDev d;
+    if (int s = rope_frequencies(*rope, D, &d)) return s;
+    if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
+    if (int s = check_device_pointer(op, "the cache", cache->k)) return s;
+    if (int s = check_device_pointer(op, q ? "q" : "k", q ? q : k)) return s;
+    a.b = paged_batch(*cache, *batch);
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.kp = cache->k;
+    a.vp = cache->v;
+    a.ldq = ldq;
+    a.ldk = ldk;
+    a.ldv = ldv;
+    a.ldo = ldo;
+    a.nq = q ? nq : 0;
+    a.D = D;
+    a.err = err;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return cache->dtype == INFERNT_DTYPE_BF16 ? launch_src<__nv_bfloat16>(a, d, src_dtype, st)
+                                              : launch_src<__half>(a, d, src_dtype, st);
+}
