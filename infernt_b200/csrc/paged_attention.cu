@@ -26,7 +26,12 @@ constexpr int kItemRows = 64;   // query rows of an item: four warps of 16
 constexpr int kThreads = 128;
 constexpr int kStages = 3;
 constexpr float kRescale = 8.0f;  // log2 of the largest unnormalised probability
+
+// Workspace: the tickets of split items, then two slots of partial results
+// for each CTA.
 constexpr size_t kWorkspaceBytes = 64u << 20;
+constexpr int kMaxCtas = 640;
+constexpr size_t kSlotsAt = 4096;
 
 struct AttnArgs {
     PagedBatch b;
@@ -38,38 +43,125 @@ struct AttnArgs {
     long long ldq, ldo;
     int nq, G, window, sinks;
     float scale, scale_log2;
+    int min_tiles;      // least tiles of a CTA
+    unsigned* tickets;  // [CTAs], zero between calls
+    float* slots;
     unsigned* err;
 };
 
 // Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
-// keys that they see: [0, sink_end) and [lo, hi), as tiles of kTileKeys keys.
+// keys that they see: [0, sink_end) and [lo, hi), as tiles of N keys.
 struct Item {
     int kvh, row0, rows;
     int sink_end, lo, hi;  // hi: one past the last row's position (0 when it sees nothing)
-    int sink_tiles, tiles;
+    int lo_tile, sink_tiles, tiles;
     int pos_first, pos_last;
 };
 
 __device__ __forceinline__ int row_pos(const PagedSeq& s, int token) { return s.len - s.n_new + token; }
 
+template <int M, int N>
 __device__ __forceinline__ Item make_item(const AttnArgs& a, const PagedSeq& s, int kvh, int row0) {
     Item it;
     it.kvh = kvh;
     it.row0 = row0;
-    it.rows = min(kItemRows, s.n_new * a.G - row0);
+    it.rows = min(M, s.n_new * a.G - row0);
     it.pos_first = row_pos(s, row0 / a.G);
     it.pos_last = row_pos(s, (row0 + it.rows - 1) / a.G);
     it.hi = max(0, it.pos_last + 1);
     it.lo = a.window > 0 ? max(0, it.pos_first - a.window + 1) : 0;
     it.sink_end = min(a.sinks, it.lo);
-    const int lo_tile = it.lo / kTileKeys;
-    it.sink_tiles = min((it.sink_end + kTileKeys - 1) / kTileKeys, lo_tile);
-    it.tiles = it.hi > 0 ? it.sink_tiles + (it.hi - 1) / kTileKeys - lo_tile + 1 : 0;
+    it.lo_tile = it.lo / N;
+    it.sink_tiles = min((it.sink_end + N - 1) / N, it.lo_tile);
+    it.tiles = it.hi > 0 ? it.sink_tiles + (it.hi - 1) / N - it.lo_tile + 1 : 0;
     return it;
 }
 
+template <int N>
 __device__ __forceinline__ int tile_key(const Item& it, int j) {
-    return (j < it.sink_tiles ? j : it.lo / kTileKeys + (j - it.sink_tiles)) * kTileKeys;
+    return (j < it.sink_tiles ? j : it.lo_tile + (j - it.sink_tiles)) * N;
+}
+
+// ------------------------------------------------------------- schedule
+// The work of a call is a line of units: for each sequence, each KV head,
+// each item of M query rows, one unit per tile of keys (one where a row sees
+// nothing: its zeros have to be written).  CTA b takes the units [b c, (b + 1)
+// c), so every CTA reads the same number of tiles whatever the lengths, and
+// an item that crosses a border is split: its CTAs leave partial results
+// (two slots a CTA are enough: one for an item that began before it, one for
+// an item that goes on after it), and the last of them to arrive joins them
+// in CTA order.  Lengths are device data; each CTA finds its own place by a
+// scan over the sequences.
+template <int M, int N>
+__device__ __forceinline__ int units_of(const AttnArgs& a, const PagedSeq& s) {
+    int n = 0;
+    for (int row0 = 0; row0 < s.n_new * a.G; row0 += M) n += max(1, make_item<M, N>(a, s, 0, row0).tiles);
+    return n;  // of one KV head
+}
+
+struct Place {
+    int seq;
+    long long before;  // units before the sequence
+    long long total;
+};
+
+// The sequence that holds unit `c` x blockIdx.x, c chosen from the total;
+// seq = -1 when this CTA has nothing.  All threads of the block.
+template <int M, int N, int NT>
+__device__ Place find_place(const AttnArgs& a, long long& c) {
+    __shared__ long long warp_sum_s[NT / 32];
+    __shared__ Place place_s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.b.num_seqs;
+    long long mine = 0, total = 0, before = 0;
+    // the sum of a block's values before this thread's, and of all of them
+    auto scan = [&](long long v, long long& all) {
+        long long x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum_s[warp] = x;
+        __syncthreads();
+        long long pre = 0;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) {
+            if (w < warp) pre += warp_sum_s[w];
+            all += warp_sum_s[w];
+        }
+        return pre + x - v;
+    };
+    auto units = [&](int s) {
+        return s < n ? (long long)units_of<M, N>(a, paged_seq(a.b, s, blockIdx.x == 0 ? a.err : nullptr)) * a.b.nkv : 0;
+    };
+    if (tid == 0) place_s.seq = -1;
+    for (int base = 0; base < n; base += NT) {
+        long long all;
+        mine = units(base + tid);
+        before = total + scan(mine, all);
+        total += all;
+    }
+    c = max((long long)a.min_tiles, (total + gridDim.x - 1) / gridDim.x);
+    const long long at = c * blockIdx.x;
+    long long sum = 0;
+    for (int base = 0; base < n; base += NT) {
+        if (n > NT) {  // a second pass; up to NT sequences are still in registers
+            long long all;
+            mine = units(base + tid);
+            before = sum + scan(mine, all);
+            sum += all;
+        }
+        if (before <= at && at < before + mine) {
+            place_s.seq = base + tid;
+            place_s.before = before;
+        }
+    }
+    __syncthreads();
+    Place p = place_s;
+    p.total = total;
+    return p;
 }
 
 // Whether some row of the item sees key p.
@@ -181,7 +273,7 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
     // pool row of key `tid` of tile j; -1 where no row of the item sees it
     auto row_of = [&](int j) {
         if (tid >= kTileKeys || j >= j1) return -1;
-        const int p = tile_key(it, j) + tid;
+        const int p = tile_key<kTileKeys>(it, j) + tid;
         return item_sees(it, p) ? pool_row(a.b, s, it.kvh, p, a.err) : -1;
     };
     // tile j into stage (j - j0) % kStages; rows that nobody sees become zeros
@@ -242,7 +334,7 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
         issue(j + kStages - 1);
         const int next = row_of(j + kStages);
         if (busy) {
-            const int k0 = tile_key(it, j);
+            const int k0 = tile_key<kTileKeys>(it, j);
             const uint32_t kt = ring + (uint32_t)((j - j0) % kStages) * 2 * L::kTileBytes, vt = kt + L::kTileBytes;
             float sc[NT][4];
 #pragma unroll
@@ -343,85 +435,172 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
     __syncthreads();
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) paged_attn(const AttnArgs a) {
-    using L = Layout<D>;
-    extern __shared__ __align__(128) unsigned char smem[];
-    const int tid = threadIdx.x;
-    // Item blockIdx.x / nkv: sequence s has the items from
-    // floor(q_start[s] G / 64) + s on, which leaves room for its own
-    const int kvh = blockIdx.x % a.b.nkv, slot = blockIdx.x / a.b.nkv;
-    int lo = 0, hi = a.b.num_seqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if ((long long)a.b.q_start[mid] * a.G / kItemRows + mid <= slot)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    const PagedSeq seq = paged_seq(a.b, lo, tid == 0 ? a.err : nullptr);
-    const long long first = (long long)seq.row0 * a.G / kItemRows + lo;
-    const long long row0 = (slot - first) * kItemRows;
-    if (row0 < 0 || row0 >= (long long)seq.n_new * a.G) return;
-    const Item it = make_item(a, seq, kvh, (int)row0);
-    int shares = 4;
-    if (it.rows <= 16)
-        run_tiles<T, D, 1>(a, seq, lo, it, 0, it.tiles, smem);
-    else if (it.rows <= 32) {
-        run_tiles<T, D, 2>(a, seq, lo, it, 0, it.tiles, smem);
-        shares = 2;
-    } else {
-        run_tiles<T, D, 4>(a, seq, lo, it, 0, it.tiles, smem);
-        shares = 1;
-    }
-    const float* o_s = reinterpret_cast<const float*>(smem);
-    const float* m_s = o_s + 4 * 16 * D;
+// Joined values of row r, columns d and d + 1, of an item's partial results:
+// `shares` sets of (m, l, out) in shared memory.
+struct Joined {
+    float m, l, x, y;
+};
+
+template <int D>
+__device__ __forceinline__ Joined join_shares(const float* o_s, int shares, int r, int d) {
+    const float* m_s = o_s + 64 * D;
     const float* l_s = m_s + 64;
-    unsigned char* flag = smem + L::kRing + 2 * kTileKeys * 4;
-    if (tid < kItemRows) flag[tid] = 0;
-    __syncthreads();
     const int stride = 64 / shares;  // rows of one share
-    for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
-        const int r = e / (D / 2), d = 2 * (e % (D / 2));
-        const int row = it.row0 + r, token = row / a.G, head = kvh * a.G + row % a.G;
-        float M = -INFINITY;
-        for (int k = 0; k < shares; ++k) M = fmaxf(M, m_s[k * stride + r]);
-        float lsum = 0.0f, x = 0.0f, y = 0.0f;
-        for (int k = 0; k < shares; ++k) {
-            const float mk = m_s[k * stride + r], f = mk == -INFINITY ? 0.0f : ex2(mk - M);
-            const float2 o = *reinterpret_cast<const float2*>(o_s + (k * stride + r) * D + d);
-            lsum = fmaf(l_s[k * stride + r], f, lsum);
-            x = fmaf(o.x, f, x);
-            y = fmaf(o.y, f, y);
-        }
-        float lse;
-        if (row_pos(seq, token) < 0) {
-            x = y = 0.0f;
-            lse = -INFINITY;
-        } else {
-            const float inv = 1.0f / lsum;
-            x *= inv;
-            y *= inv;
-            lse = (M + log2f(lsum)) * 0.6931471805599453f;
-            if (!(fabsf(x) < INFINITY && fabsf(y) < INFINITY)) flag[r] = 1;
-        }
-        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + token) * a.ldo +
-                                     (long long)head * D + d) = Half16<T>::pack(x, y);
-        if (a.lse && d == 0) a.lse[(long long)(seq.row0 + token) * a.nq + head] = lse;
+    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < shares; ++k) v.m = fmaxf(v.m, m_s[k * stride + r]);
+    for (int k = 0; k < shares; ++k) {
+        const float mk = m_s[k * stride + r], f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
+        const float2 o = *reinterpret_cast<const float2*>(o_s + (k * stride + r) * D + d);
+        v.l = fmaf(l_s[k * stride + r], f, v.l);
+        v.x = fmaf(o.x, f, v.x);
+        v.y = fmaf(o.y, f, v.y);
+    }
+    return v;
+}
+
+// A slot: out [M][D], m [M], l [M] of an item's rows.
+template <int M, int D>
+constexpr size_t slot_floats() {
+    return (size_t)M * (D + 2);
+}
+
+// The slot of CTA b for an item whose first CTA is `first`.
+template <int M, int D>
+__device__ __forceinline__ float* slot_of(const AttnArgs& a, long long b, long long first) {
+    return a.slots + (size_t)(2 * b + (b == first)) * slot_floats<M, D>();
+}
+
+template <int M, int D>
+__device__ __forceinline__ Joined join_slots(const AttnArgs& a, long long first, long long last, int r, int d) {
+    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    for (long long b = first; b <= last; ++b) v.m = fmaxf(v.m, __ldcg(slot_of<M, D>(a, b, first) + M * D + r));
+    for (long long b = first; b <= last; ++b) {
+        const float* p = slot_of<M, D>(a, b, first);
+        const float mk = __ldcg(p + M * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
+        const float2 o = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
+        v.l = fmaf(__ldcg(p + M * D + M + r), f, v.l);
+        v.x = fmaf(o.x, f, v.x);
+        v.y = fmaf(o.y, f, v.y);
+    }
+    return v;
+}
+
+// Columns d and d + 1 of a row's result; true when it is not finite.
+template <typename T, int D>
+__device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& seq, int kvh, int row, int d, Joined v) {
+    const int token = row / a.G, head = kvh * a.G + row % a.G;
+    const bool sees = row_pos(seq, token) >= 0;
+    const float inv = 1.0f / v.l;
+    const float x = sees ? v.x * inv : 0.0f, y = sees ? v.y * inv : 0.0f;
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + token) * a.ldo +
+                                 (long long)head * D + d) = Half16<T>::pack(x, y);
+    if (a.lse && d == 0)
+        a.lse[(long long)(seq.row0 + token) * a.nq + head] =
+            sees ? (v.m + log2f(v.l)) * 0.6931471805599453f : -INFINITY;
+    return !(fabsf(x) < INFINITY && fabsf(y) < INFINITY);
+}
+
+// Counts this CTA's arrival at an item split over `parts` CTAs; true for the
+// last one, which then sees the others' slots.
+__device__ __forceinline__ bool last_to_arrive(unsigned* ticket, long long parts) {
+    __shared__ int s_last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s_last = atomicAdd(ticket, 1u) + 1u == (unsigned)parts;
+        if (s_last) *ticket = 0u;  // ready for the next call
     }
     __syncthreads();
-    for (int r = tid >> 5; r < it.rows; r += kThreads / 32)
-        if (flag[r]) exact_row<T, D>(a, seq, lo, kvh, it.row0 + r);
+    __threadfence();
+    return s_last != 0;
 }
 
 template <typename T, int D>
-int launch(const AttnArgs& a, cudaStream_t st) {
+__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) paged_attn(const AttnArgs a) {
+    using L = Layout<D>;
+    constexpr int M = kItemRows, N = kTileKeys;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int tid = threadIdx.x;
+    float* o_s = reinterpret_cast<float*>(smem);
+    unsigned char* flag = smem + L::kRing + 2 * kTileKeys * 4;
+    long long c;
+    const Place place = find_place<M, N, kThreads>(a, c);
+    if (place.seq < 0) return;
+    long long at = c * blockIdx.x;
+    const long long end = min(at + c, place.total);
+    long long before = place.before;
+    for (int s = place.seq; at < end; ++s) {
+        const PagedSeq seq = paged_seq(a.b, s, nullptr);
+        const int per_head = units_of<M, N>(a, seq);
+        // this sequence's units are [before, before + per_head nkv)
+        for (int kvh = per_head ? (int)((at - before) / per_head) : a.b.nkv; kvh < a.b.nkv && at < end; ++kvh) {
+            long long u0 = before + (long long)kvh * per_head;
+            for (int row0 = 0; row0 < seq.n_new * a.G && at < end; row0 += M) {
+                const Item it = make_item<M, N>(a, seq, kvh, row0);
+                const int units = max(1, it.tiles);
+                if (at < u0 + units) {
+                    const int j0 = (int)(at - u0), j1 = min(it.tiles, (int)min((long long)units, end - u0));
+                    int shares;
+                    if (it.rows <= 16) {
+                        run_tiles<T, D, 1>(a, seq, s, it, j0, j1, smem);
+                        shares = 4;
+                    } else if (it.rows <= 32) {
+                        run_tiles<T, D, 2>(a, seq, s, it, j0, j1, smem);
+                        shares = 2;
+                    } else {
+                        run_tiles<T, D, 4>(a, seq, s, it, j0, j1, smem);
+                        shares = 1;
+                    }
+                    const long long first = u0 / c, last = (u0 + units - 1) / c;
+                    bool write = true;
+                    if (first != last) {
+                        float* slot = slot_of<M, D>(a, blockIdx.x, first);
+                        for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
+                            const int r = e / (D / 2), d = 2 * (e % (D / 2));
+                            const Joined v = join_shares<D>(o_s, shares, r, d);
+                            *reinterpret_cast<float2*>(slot + r * D + d) = make_float2(v.x, v.y);
+                            if (d == 0) {
+                                slot[M * D + r] = v.m;
+                                slot[M * D + M + r] = v.l;
+                            }
+                        }
+                        write = last_to_arrive(a.tickets + first, last - first + 1);
+                    }
+                    if (write) {
+                        if (tid < M) flag[tid] = 0;
+                        __syncthreads();
+                        for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
+                            const int r = e / (D / 2), d = 2 * (e % (D / 2));
+                            const Joined v = first != last ? join_slots<M, D>(a, first, last, r, d)
+                                                           : join_shares<D>(o_s, shares, r, d);
+                            if (write_pair<T, D>(a, seq, kvh, row0 + r, d, v)) flag[r] = 1;
+                        }
+                        __syncthreads();
+                        for (int r = tid >> 5; r < it.rows; r += kThreads / 32)
+                            if (flag[r]) exact_row<T, D>(a, seq, s, kvh, row0 + r);
+                    }
+                    __syncthreads();  // shared memory is free for the next item
+                    at = u0 + units;
+                }
+                u0 += units;
+            }
+        }
+        before += (long long)per_head * a.b.nkv;
+    }
+}
+
+template <typename T, int D>
+int launch(const AttnArgs& args, cudaStream_t st) {
     using L = Layout<D>;
     static_assert(4 * 16 * D * 4 + 2 * 64 * 4 <= L::kRing, "the merge must fit the ring");
+    static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<kItemRows, D>() * 4 <= kWorkspaceBytes && kMaxCtas * 4 <= kSlotsAt,
+                  "the slots must fit the workspace");
+    AttnArgs a = args;
     INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-    const long long ctas = ((long long)a.b.num_rows * a.G / kItemRows + a.b.num_seqs) * a.b.nkv;
-    INFERNT_REQUIRE(ctas < (1ll << 31), "paged_attention: %lld items", ctas);
-    paged_attn<T, D><<<(unsigned)ctas, kThreads, L::kBytes, st>>>(a);
+    // as many CTAs as the SMs hold at once
+    int ctas = sm_count() * (D == 64 ? 4 : 2);
+    if (ctas > kMaxCtas) ctas = kMaxCtas;
+    paged_attn<T, D><<<ctas, kThreads, L::kBytes, st>>>(a);
     INFERNT_CUDA_TRY(cudaGetLastError());
     return INFERNT_OK;
 }
@@ -470,6 +649,9 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.sinks = sinks;
     a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)D);
     a.scale_log2 = a.scale * 1.4426950408889634f;
+    a.min_tiles = 4;
+    a.tickets = static_cast<unsigned*>(workspace);
+    a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (cache->dtype == INFERNT_DTYPE_BF16)
