@@ -644,7 +644,7 @@ INFERNT_API int infernt_paged_rope_append(void* q_out, int ldo, const void* q, i
  * first `sinks` positions:
  *   out[r][h] = sum_p w_p V[p] / sum_p w_p,  w_p = exp(scale q[r][h] . K[p]),
  *   lse[r][h] = ln sum_p w_p
- * of KV head h / (nq / num_kv_heads).  scale 0 means 1 / sqrt(head_dim).
+ * of KV head h / (nq / num_kv_heads).  scale >= 0; 0 means 1 / sqrt(head_dim).
  * q and out [num_rows][nq][head_dim] of the cache's type, rows ldq and ldo
  * elements apart (multiples of 8, pointers 16-byte aligned); lse [num_rows]
  * [nq] FP32 or NULL.  A row without a visible key gets zeros and an lse of

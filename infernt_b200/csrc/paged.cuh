@@ -16,6 +16,22 @@ namespace infernt {
 // Positions and rows stay below it, so that sums of two of them fit an int.
 constexpr int kMaxPositions = 1 << 30;
 
+// n / d for 0 <= n < 2^31 by a product: with 2^(L - 1) < d <= 2^L the factor
+// ceil(2^(31 + L) / d) is off by less than d / 2^(31 + L), which the quotient
+// of such an n does not see (Granlund and Montgomery 1994).
+struct FastDiv {
+    uint32_t factor;
+    int shift;
+    __device__ __forceinline__ int operator()(int n) const {
+        return (int)(((unsigned long long)(uint32_t)n * factor) >> shift);
+    }
+};
+inline FastDiv fast_div(int d) {
+    int L = 0;
+    while (L < 31 && (1ll << L) < d) ++L;
+    return {(uint32_t)(((1ull << (31 + L)) + (unsigned)d - 1) / (unsigned)d), 31 + L};
+}
+
 // infernt_ragged_batch and the pool geometry as the kernels take them.
 struct PagedBatch {
     const int* q_start;
@@ -23,6 +39,7 @@ struct PagedBatch {
     const int* table;
     int table_stride, num_seqs, num_rows, max_q_len;
     int num_pages, page_size, nkv;
+    FastDiv by_page;
 };
 
 // One sequence of a batch: rows [row0, row0 + n_new), length len.
@@ -101,6 +118,7 @@ inline PagedBatch paged_batch(const infernt_paged_cache& c, const infernt_ragged
     r.num_pages = c.num_pages;
     r.page_size = c.page_size;
     r.nkv = c.num_kv_heads;
+    r.by_page = fast_div(c.page_size);
     return r;
 }
 

@@ -12,10 +12,11 @@
 // The query rows of a KV head are its new tokens times its G query heads,
 // row = token G + head of the group, so all rows of a tile share the K and V
 // rows that the tile reads, whatever G is.
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
-#include "paged.cuh"
+#include "paged_attention.cuh"
 #include "warp_mma.cuh"
 
 namespace infernt {
@@ -25,166 +26,6 @@ constexpr int kTileKeys = 64;   // keys of a K / V tile
 constexpr int kItemRows = 64;   // query rows of an item: four warps of 16
 constexpr int kThreads = 128;
 constexpr int kStages = 3;
-constexpr float kRescale = 8.0f;  // log2 of the largest unnormalised probability
-
-// Workspace: the tickets of split items, then two slots of partial results
-// for each CTA.
-constexpr size_t kWorkspaceBytes = 64u << 20;
-constexpr int kMaxCtas = 640;
-constexpr size_t kSlotsAt = 4096;
-
-struct AttnArgs {
-    PagedBatch b;
-    const void* q;
-    void* out;
-    const void* k;
-    const void* v;
-    float* lse;
-    long long ldq, ldo;
-    int nq, G, window, sinks;
-    float scale, scale_log2;
-    int min_tiles;      // least tiles of a CTA
-    unsigned* tickets;  // [CTAs], zero between calls
-    float* slots;
-    unsigned* err;
-};
-
-// Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
-// keys that they see: [0, sink_end) and [lo, hi), as tiles of N keys.
-struct Item {
-    int kvh, row0, rows;
-    int sink_end, lo, hi;  // hi: one past the last row's position (0 when it sees nothing)
-    int lo_tile, sink_tiles, tiles;
-    int pos_first, pos_last;
-};
-
-__device__ __forceinline__ int row_pos(const PagedSeq& s, int token) { return s.len - s.n_new + token; }
-
-template <int M, int N>
-__device__ __forceinline__ Item make_item(const AttnArgs& a, const PagedSeq& s, int kvh, int row0) {
-    Item it;
-    it.kvh = kvh;
-    it.row0 = row0;
-    it.rows = min(M, s.n_new * a.G - row0);
-    it.pos_first = row_pos(s, row0 / a.G);
-    it.pos_last = row_pos(s, (row0 + it.rows - 1) / a.G);
-    it.hi = max(0, it.pos_last + 1);
-    it.lo = a.window > 0 ? max(0, it.pos_first - a.window + 1) : 0;
-    it.sink_end = min(a.sinks, it.lo);
-    it.lo_tile = it.lo / N;
-    it.sink_tiles = min((it.sink_end + N - 1) / N, it.lo_tile);
-    it.tiles = it.hi > 0 ? it.sink_tiles + (it.hi - 1) / N - it.lo_tile + 1 : 0;
-    return it;
-}
-
-template <int N>
-__device__ __forceinline__ int tile_key(const Item& it, int j) {
-    return (j < it.sink_tiles ? j : it.lo_tile + (j - it.sink_tiles)) * N;
-}
-
-// ------------------------------------------------------------- schedule
-// The work of a call is a line of units: for each sequence, each KV head,
-// each item of M query rows, one unit per tile of keys (one where a row sees
-// nothing: its zeros have to be written).  CTA b takes the units [b c, (b + 1)
-// c), so every CTA reads the same number of tiles whatever the lengths, and
-// an item that crosses a border is split: its CTAs leave partial results
-// (two slots a CTA are enough: one for an item that began before it, one for
-// an item that goes on after it), and the last of them to arrive joins them
-// in CTA order.  Lengths are device data; each CTA finds its own place by a
-// scan over the sequences.
-template <int M, int N>
-__device__ __forceinline__ int units_of(const AttnArgs& a, const PagedSeq& s) {
-    int n = 0;
-    for (int row0 = 0; row0 < s.n_new * a.G; row0 += M) n += max(1, make_item<M, N>(a, s, 0, row0).tiles);
-    return n;  // of one KV head
-}
-
-struct Place {
-    int seq;
-    long long before;  // units before the sequence
-    long long total;
-};
-
-// The sequence that holds unit `c` x blockIdx.x, c chosen from the total;
-// seq = -1 when this CTA has nothing.  All threads of the block.
-template <int M, int N, int NT>
-__device__ Place find_place(const AttnArgs& a, long long& c) {
-    __shared__ long long warp_sum_s[NT / 32];
-    __shared__ Place place_s;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.b.num_seqs;
-    long long mine = 0, total = 0, before = 0;
-    // the sum of a block's values before this thread's, and of all of them
-    auto scan = [&](long long v, long long& all) {
-        long long x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) warp_sum_s[warp] = x;
-        __syncthreads();
-        long long pre = 0;
-        all = 0;
-#pragma unroll
-        for (int w = 0; w < NT / 32; ++w) {
-            if (w < warp) pre += warp_sum_s[w];
-            all += warp_sum_s[w];
-        }
-        return pre + x - v;
-    };
-    auto units = [&](int s) {
-        return s < n ? (long long)units_of<M, N>(a, paged_seq(a.b, s, blockIdx.x == 0 ? a.err : nullptr)) * a.b.nkv : 0;
-    };
-    if (tid == 0) place_s.seq = -1;
-    for (int base = 0; base < n; base += NT) {
-        long long all;
-        mine = units(base + tid);
-        before = total + scan(mine, all);
-        total += all;
-    }
-    c = max((long long)a.min_tiles, (total + gridDim.x - 1) / gridDim.x);
-    const long long at = c * blockIdx.x;
-    long long sum = 0;
-    for (int base = 0; base < n; base += NT) {
-        if (n > NT) {  // a second pass; up to NT sequences are still in registers
-            long long all;
-            mine = units(base + tid);
-            before = sum + scan(mine, all);
-            sum += all;
-        }
-        if (before <= at && at < before + mine) {
-            place_s.seq = base + tid;
-            place_s.before = before;
-        }
-    }
-    __syncthreads();
-    Place p = place_s;
-    p.total = total;
-    return p;
-}
-
-// Whether some row of the item sees key p.
-__device__ __forceinline__ bool item_sees(const Item& it, int p) {
-    return p < it.hi && (p >= it.lo || p < it.sink_end);
-}
-
-// Pool row of position p of sequence s for KV head kvh, or -1 (a page that
-// the pool does not have).
-__device__ __forceinline__ int pool_row(const PagedBatch& b, int s, int kvh, int p, unsigned* err) {
-    const int pi = p / b.page_size, page = b.table[(size_t)s * b.table_stride + pi];
-    if (page < 0 || page >= b.num_pages) {
-        if (err) atomicOr(err, kErrPage);
-        return -1;
-    }
-    return (page * b.nkv + kvh) * b.page_size + (p - pi * b.page_size);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -200,46 +41,6 @@ __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t 
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// One row by one warp, term by term: what a row is computed with when its
-// result is not finite.  The tiles above multiply a hidden position's value
-// by a probability of 0, which is NaN where the value is infinite or NaN;
-// here only what the row sees is touched, so what a row does see that is not
-// finite still shows in its result as in the formula.
-template <typename T, int D>
-__device__ void exact_row(const AttnArgs& a, const PagedSeq& seq, int s, int kvh, int row) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, token = row / a.G, head = kvh * a.G + row % a.G;
-    const int pos = row_pos(seq, token);
-    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, sink_end = min(a.sinks, lo);
-    const T* q = static_cast<const T*>(a.q) + (long long)(seq.row0 + token) * a.ldq + (long long)head * D + lane * E;
-    float qv[E], acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qv[e] = Half16<T>::value(q[e]);
-        acc[e] = 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int p = 0; p <= pos; ++p) {
-        if (p == sink_end) p = lo;  // lo <= pos
-        const int r = pool_row(a.b, s, kvh, p, a.err);
-        const T* k = static_cast<const T*>(a.k) + (long long)r * D + lane * E;
-        const T* v = static_cast<const T*>(a.v) + (long long)r * D + lane * E;
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) dot = fmaf(qv[e], r >= 0 ? Half16<T>::value(k[e]) : 0.0f, dot);
-        const float sc = warp_sum(dot) * a.scale, m_new = fmaxf(m, sc);
-        const float f = m == -INFINITY ? 0.0f : expf(m - m_new), w = expf(sc - m_new);
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + w * (r >= 0 ? Half16<T>::value(v[e]) : 0.0f);
-        m = m_new;
-    }
-    T* o = static_cast<T*>(a.out) + (long long)(seq.row0 + token) * a.ldo + (long long)head * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = Half16<T>::round(acc[e] / l);
-    if (a.lse && lane == 0) a.lse[(long long)(seq.row0 + token) * a.nq + head] = m + logf(l);
 }
 
 // Shared memory: the ring of K / V tiles (reused for the merge of the warps'
@@ -309,12 +110,12 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
     int pos[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int r = rb * 16 + g + 8 * h, row = it.row0 + r, token = row / a.G;
+        const int r = rb * 16 + g + 8 * h, row = it.row0 + r, token = a.by_g(row);
         const bool ok = r < it.rows;
         pos[h] = ok ? row_pos(seq, token) : -1;
         const uint32_t* q = reinterpret_cast<const uint32_t*>(
             static_cast<const uint16_t*>(a.q) + (ok ? (long long)(seq.row0 + token) * a.ldq +
-                                                          (long long)(it.kvh * a.G + row % a.G) * D + 2 * tig
+                                                          (long long)(it.kvh * a.G + row - token * a.G) * D + 2 * tig
                                                     : 0));
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
@@ -435,12 +236,7 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
     __syncthreads();
 }
 
-// Joined values of row r, columns d and d + 1, of an item's partial results:
 // `shares` sets of (m, l, out) in shared memory.
-struct Joined {
-    float m, l, x, y;
-};
-
 template <int D>
 __device__ __forceinline__ Joined join_shares(const float* o_s, int shares, int r, int d) {
     const float* m_s = o_s + 64 * D;
@@ -456,18 +252,6 @@ __device__ __forceinline__ Joined join_shares(const float* o_s, int shares, int 
         v.y = fmaf(o.y, f, v.y);
     }
     return v;
-}
-
-// A slot: out [M][D], m [M], l [M] of an item's rows.
-template <int M, int D>
-constexpr size_t slot_floats() {
-    return (size_t)M * (D + 2);
-}
-
-// The slot of CTA b for an item whose first CTA is `first`.
-template <int M, int D>
-__device__ __forceinline__ float* slot_of(const AttnArgs& a, long long b, long long first) {
-    return a.slots + (size_t)(2 * b + (b == first)) * slot_floats<M, D>();
 }
 
 template <int M, int D>
@@ -488,7 +272,7 @@ __device__ __forceinline__ Joined join_slots(const AttnArgs& a, long long first,
 // Columns d and d + 1 of a row's result; true when it is not finite.
 template <typename T, int D>
 __device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& seq, int kvh, int row, int d, Joined v) {
-    const int token = row / a.G, head = kvh * a.G + row % a.G;
+    const int token = a.by_g(row), head = kvh * a.G + row - token * a.G;
     const bool sees = row_pos(seq, token) >= 0;
     const float inv = 1.0f / v.l;
     const float x = sees ? v.x * inv : 0.0f, y = sees ? v.y * inv : 0.0f;
@@ -496,7 +280,7 @@ __device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& se
                                  (long long)head * D + d) = Half16<T>::pack(x, y);
     if (a.lse && d == 0)
         a.lse[(long long)(seq.row0 + token) * a.nq + head] =
-            sees ? (v.m + log2f(v.l)) * 0.6931471805599453f : -INFINITY;
+            sees ? (v.m + log2f(v.l)) * kLn2 : -INFINITY;
     return !(fabsf(x) < INFINITY && fabsf(y) < INFINITY);
 }
 
@@ -518,75 +302,53 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* ticket, long long parts
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) paged_attn(const AttnArgs a) {
     using L = Layout<D>;
-    constexpr int M = kItemRows, N = kTileKeys;
+    constexpr int M = kItemRows;
     extern __shared__ __align__(128) unsigned char smem[];
     const int tid = threadIdx.x;
     float* o_s = reinterpret_cast<float*>(smem);
     unsigned char* flag = smem + L::kRing + 2 * kTileKeys * 4;
-    long long c;
-    const Place place = find_place<M, N, kThreads>(a, c);
+    const Place place = find_place<M, kTileKeys, kThreads>(a);
     if (place.seq < 0) return;
-    long long at = c * blockIdx.x;
-    const long long end = min(at + c, place.total);
-    long long before = place.before;
-    for (int s = place.seq; at < end; ++s) {
-        const PagedSeq seq = paged_seq(a.b, s, nullptr);
-        const int per_head = units_of<M, N>(a, seq);
-        // this sequence's units are [before, before + per_head nkv)
-        for (int kvh = per_head ? (int)((at - before) / per_head) : a.b.nkv; kvh < a.b.nkv && at < end; ++kvh) {
-            long long u0 = before + (long long)kvh * per_head;
-            for (int row0 = 0; row0 < seq.n_new * a.G && at < end; row0 += M) {
-                const Item it = make_item<M, N>(a, seq, kvh, row0);
-                const int units = max(1, it.tiles);
-                if (at < u0 + units) {
-                    const int j0 = (int)(at - u0), j1 = min(it.tiles, (int)min((long long)units, end - u0));
-                    int shares;
-                    if (it.rows <= 16) {
-                        run_tiles<T, D, 1>(a, seq, s, it, j0, j1, smem);
-                        shares = 4;
-                    } else if (it.rows <= 32) {
-                        run_tiles<T, D, 2>(a, seq, s, it, j0, j1, smem);
-                        shares = 2;
-                    } else {
-                        run_tiles<T, D, 4>(a, seq, s, it, j0, j1, smem);
-                        shares = 1;
-                    }
-                    const long long first = u0 / c, last = (u0 + units - 1) / c;
-                    bool write = true;
-                    if (first != last) {
-                        float* slot = slot_of<M, D>(a, blockIdx.x, first);
-                        for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
-                            const int r = e / (D / 2), d = 2 * (e % (D / 2));
-                            const Joined v = join_shares<D>(o_s, shares, r, d);
-                            *reinterpret_cast<float2*>(slot + r * D + d) = make_float2(v.x, v.y);
-                            if (d == 0) {
-                                slot[M * D + r] = v.m;
-                                slot[M * D + M + r] = v.l;
-                            }
-                        }
-                        write = last_to_arrive(a.tickets + first, last - first + 1);
-                    }
-                    if (write) {
-                        if (tid < M) flag[tid] = 0;
-                        __syncthreads();
-                        for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
-                            const int r = e / (D / 2), d = 2 * (e % (D / 2));
-                            const Joined v = first != last ? join_slots<M, D>(a, first, last, r, d)
-                                                           : join_shares<D>(o_s, shares, r, d);
-                            if (write_pair<T, D>(a, seq, kvh, row0 + r, d, v)) flag[r] = 1;
-                        }
-                        __syncthreads();
-                        for (int r = tid >> 5; r < it.rows; r += kThreads / 32)
-                            if (flag[r]) exact_row<T, D>(a, seq, s, kvh, row0 + r);
-                    }
-                    __syncthreads();  // shared memory is free for the next item
-                    at = u0 + units;
+    walk<M, kTileKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
+        int shares;
+        if (it.rows <= 16) {
+            run_tiles<T, D, 1>(a, seq, p.s, it, p.j0, p.j1, smem);
+            shares = 4;
+        } else if (it.rows <= 32) {
+            run_tiles<T, D, 2>(a, seq, p.s, it, p.j0, p.j1, smem);
+            shares = 2;
+        } else {
+            run_tiles<T, D, 4>(a, seq, p.s, it, p.j0, p.j1, smem);
+            shares = 1;
+        }
+        const bool split = p.first != p.last;
+        if (split) {
+            float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
+            for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
+                const int r = e / (D / 2), d = 2 * (e % (D / 2));
+                const Joined v = join_shares<D>(o_s, shares, r, d);
+                *reinterpret_cast<float2*>(slot + r * D + d) = make_float2(v.x, v.y);
+                if (d == 0) {
+                    slot[M * D + r] = v.m;
+                    slot[M * D + M + r] = v.l;
                 }
-                u0 += units;
             }
         }
-        before += (long long)per_head * a.b.nkv;
-    }
+        if (!split || last_to_arrive(a.tickets + p.first, p.last - p.first + 1)) {
+            if (tid < M) flag[tid] = 0;
+            __syncthreads();
+            for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
+                const int r = e / (D / 2), d = 2 * (e % (D / 2));
+                const Joined v =
+                    split ? join_slots<M, D>(a, p.first, p.last, r, d) : join_shares<D>(o_s, shares, r, d);
+                if (write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, v)) flag[r] = 1;
+            }
+            __syncthreads();
+            for (int r = tid >> 5; r < it.rows; r += kThreads / 32)
+                if (flag[r]) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r);
+        }
+        __syncthreads();  // shared memory is free for the next item
+    });
 }
 
 template <typename T, int D>
@@ -627,9 +389,14 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
                     "%s: q, out and workspace must be 16-byte aligned", op);
     INFERNT_REQUIRE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "%s: window %d, sinks %d", op, window,
                     sinks);
-    INFERNT_REQUIRE(std::isfinite(scale), "%s: scale", op);
-    INFERNT_REQUIRE((long long)batch->num_rows * (nq / nkv) < (1ll << 31), "%s: %d rows of %d heads", op,
-                    batch->num_rows, nq);
+    INFERNT_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "%s: scale %g", op, scale);
+    const int G = nq / nkv;
+    INFERNT_REQUIRE((long long)batch->num_rows * G < kMaxPositions, "%s: %d rows of %d heads", op, batch->num_rows, nq);
+    // the tiles of one KV head of a sequence are counted in 32 bits
+    const long long most_q = batch->max_q_len < batch->num_rows ? batch->max_q_len : batch->num_rows;
+    const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
+    INFERNT_REQUIRE((most_q * G / kItemRows + 1) * (most_kv / kTileKeys + 2) < (1ll << 31),
+                    "%s: %lld new tokens of %d heads over %lld positions (split the chunk)", op, most_q, G, most_kv);
     if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
     if (int s = check_device_pointer(op, "the cache", cache->k)) return s;
     if (int s = check_device_pointer(op, "q", q)) return s;
@@ -644,7 +411,8 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.ldq = ldq;
     a.ldo = ldo;
     a.nq = nq;
-    a.G = nq / nkv;
+    a.G = G;
+    a.by_g = fast_div(a.G);
     a.window = window < kMaxPositions ? window : kMaxPositions;
     a.sinks = sinks;
     a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)D);
@@ -654,6 +422,8 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (paged_attention_tc_pages(cache->page_size) && (long long)batch->max_q_len * a.G > kItemRows)
+        return paged_attention_tc(a, D, cache->dtype, st);
     if (cache->dtype == INFERNT_DTYPE_BF16)
         return D == 64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
     return D == 64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);

@@ -1,0 +1,509 @@
+// paged_attention_tc.cu — attention of chunks of new tokens over paged KV
+// caches on the 5th-generation tensor cores (paged_attention.cu has the
+// formulas and the kernel for single tokens).
+//
+// An item is 256 query rows (new token, head of the group) of a KV head, two
+// tiles A and B of 128 rows, the M of the MMA; a tile of keys is 128.  Per
+// key tile i and row tile X:
+//   S_X = Q_X K_i^T        A and B operands from shared memory, S in TMEM
+//   P_X = 2^(S_X scale - m) one thread per row: S out of TMEM, P back into it
+//                          in 16 bits, over the columns S has left
+//   O_X += P_X V_i         A operand from TMEM, V as the pages hold it
+// The two row tiles take turns: while the threads of one compute
+// probabilities, the tensor cores run the other's products.
+//
+// Ten warps: warp 0 loads K and V tiles page by page by TMA (a tensor map of
+// the pool [page][KV head][position][dim]; a page that no row sees, or that
+// the pool does not have, is a coordinate past its end and becomes zeros),
+// warp 1 issues the MMAs, warps 2-5 and 6-9 hold the rows of A and B.  A row's
+// 128 scores would not fit its thread's registers beside the rest, so the
+// first 64 are read from TMEM twice: for the maximum, and after the
+// probabilities of the last 64 are stored (into columns 96-127 of S; those of
+// the first 64 into 64-95).  The
+// reference maximum m moves only when a row's maximum passes it by 8, so O is
+// rescaled seldom.  V rows that no row of the item sees are zeroed in shared
+// memory, so that what lies there does not meet a probability of 0.
+#include <cmath>
+#include <cstdint>
+
+#include <cudaTypedefs.h>
+
+#include "paged_attention.cuh"
+#include "tc_mma.cuh"
+
+namespace infernt {
+
+void* tensor_map_encoder();  // bgemm.cu
+
+// The pages whose 128-key tiles are whole boxes: a tile is 128 / page_size
+// pages, or a page is a whole number of tiles.
+bool paged_attention_tc_pages(int page_size) {
+    return page_size % 128 == 0 || (page_size >= 8 && 128 % page_size == 0);
+}
+
+namespace {
+
+constexpr int kM = 256;  // query rows of an item
+constexpr int kN = 128;  // keys of a tile
+constexpr int kThreadsTc = 320;
+constexpr int kRowThreads = 256;
+constexpr uint32_t kBox = 16384;  // 128 rows of 64 values: a swizzled operand block
+
+// Shared memory: Q of both row tiles, then the stages of K and of V tiles,
+// each of D / 64 blocks.
+template <int D>
+struct LayoutTc {
+    static constexpr uint32_t kBlocks = D / 64;
+    static constexpr uint32_t kTile = kBlocks * kBox;
+    static constexpr int kStages = D == 64 ? 4 : 2;
+    static constexpr uint32_t kQ = 0;
+    static constexpr uint32_t kK = 2 * kTile;
+    static constexpr uint32_t kV = kK + kStages * kTile;
+    static constexpr uint32_t kBytes = kV + kStages * kTile + 1024;
+};
+
+struct Barriers {
+    uint64_t full_k[4], empty_k[4], full_v[4], empty_v[4];
+    uint64_t q[2], s[2], p[2], o[2];
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreadsTc, 1)
+    paged_attn_tc(const AttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    using L = LayoutTc<D>;
+    constexpr int NB = (int)L::kBlocks, ST = L::kStages;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    __shared__ Barriers bar;
+    __shared__ uint32_t tmem_s;
+    __shared__ int ok_s;
+    __shared__ int last_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&bar.full_k[i], 1);
+            mbar_init(&bar.empty_k[i], 1);
+            mbar_init(&bar.full_v[i], 1);
+            mbar_init(&bar.empty_v[i], 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&bar.q[x], 128);
+            mbar_init(&bar.s[x], 1);
+            mbar_init(&bar.p[x], 128);
+            mbar_init(&bar.o[x], 1);
+        }
+        mbar_fence_init();
+        ok_s = 1;
+    }
+    if (warp == 1) tmem_alloc(&tmem_s, 512);
+    const Place place = find_place<kM, kN, kThreadsTc>(a);  // its barriers publish the set-up
+    tc_fence_after();
+    __syncthreads();
+    const uint32_t tmem = tmem_s;  // S (and P) of A at 0, of B at 128; O of A at 256, of B at 384
+    bool ok = true;
+
+    if (place.seq >= 0 && warp == 0) {
+        // ---- K and V tiles.  n: tiles so far, over all parts.
+        uint32_t n = 0;
+        const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
+        walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+            for (int j = part.j0; j < part.j1; ++j, ++n) {
+                const int k0 = tile_key<kN>(it, j), st = (int)(n % ST);
+                const uint32_t turn = (n / ST) & 1u;
+                // the page of lane l's rows [k0 + l box_rows, + box_rows)
+                int page = a.b.num_pages, row = 0;
+                if (lane < per_tile) {
+                    const int p0 = k0 + lane * box_rows, pi = a.b.by_page(p0);
+                    row = p0 - pi * ps;
+                    // whether some row sees a key of the box
+                    if (p0 < it.hi && (p0 + box_rows > it.lo || p0 < it.sink_end)) {
+                        page = a.b.table[(size_t)part.s * a.b.table_stride + pi];
+                        if (page < 0 || page >= a.b.num_pages) {
+                            if (a.err) atomicOr(a.err, kErrPage);
+                            page = a.b.num_pages;
+                        }
+                    }
+                }
+                if (n >= ST) tc_wait_bar(&bar.empty_k[st], turn ^ 1u, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                if (lane == 0) mbar_arrive_expect_tx(&bar.full_k[st], L::kTile);
+                __syncwarp();
+                if (lane < per_tile)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        tma_load_4d(base + L::kK + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_k, 64 * b, row,
+                                    it.kvh, page, &bar.full_k[st]);
+                if (n >= ST) tc_wait_bar(&bar.empty_v[st], turn ^ 1u, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                if (lane == 0) mbar_arrive_expect_tx(&bar.full_v[st], L::kTile);
+                __syncwarp();
+                if (lane < per_tile)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+                        tma_load_4d(base + L::kV + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_v, 64 * b, row,
+                                    it.kvh, page, &bar.full_v[st]);
+            }
+        });
+    } else if (place.seq >= 0 && warp == 1) {
+        // ---- the MMAs, issued by lane 0.  n: key tiles so far, nx: those of row tile X.
+        uint32_t n = 0, nx[2] = {0, 0}, parts[2] = {0, 0};
+        const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kN), id_o = tc_instr(Half16<T>::kBf16, true, D);
+        walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+            if (part.j0 >= part.j1 || !ok) return;
+            const int tiles_x = it.rows > 128 ? 2 : 1;
+            // S_x of key tile number m
+            auto scores = [&](int x, uint32_t m) {
+                const int st = (int)(m % ST);
+                tc_wait_bar(&bar.full_k[st], (m / ST) & 1u, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t q = base + L::kQ + x * L::kTile, k = base + L::kK + st * L::kTile;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b)
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            tc_mma_ss(tmem + 128u * x, tc_desc_k(q + b * kBox) + 2 * kk, tc_desc_k(k + b * kBox) + 2 * kk,
+                                      id_s, (b | kk) ? 1u : 0u);
+                    tc_commit_to(&bar.s[x]);
+                    if (x == tiles_x - 1) tc_commit_to(&bar.empty_k[st]);
+                }
+                __syncwarp();
+            };
+            for (int x = 0; x < tiles_x; ++x) {
+                tc_wait_bar(&bar.q[x], parts[x] & 1u, ok);
+                ++parts[x];
+                scores(x, n);
+            }
+            for (int j = part.j0; j < part.j1 && ok; ++j, ++n) {
+                const int st = (int)(n % ST), k0 = tile_key<kN>(it, j);
+                for (int x = 0; x < tiles_x; ++x) {
+                    if (x == 0) {
+                        tc_wait_bar(&bar.full_v[st], (n / ST) & 1u, ok);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) return;
+                        if (k0 + kN > it.hi || (k0 < it.lo && k0 + kN > it.sink_end)) {
+                            // rows that no row of the item sees
+                            for (int r = 0; r < kN; ++r)
+                                if (!item_sees(it, k0 + r))
+                                    for (int c = lane; c < NB * 8; c += 32) {
+                                        const uint32_t at =
+                                            base + L::kV + st * L::kTile + (c >> 3) * kBox + r * 128 + (c & 7) * 16;
+                                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0)
+                                                     : "memory");
+                                    }
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                        }
+                    }
+                    tc_wait_bar(&bar.p[x], nx[x] & 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return;
+                    tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t v = base + L::kV + st * L::kTile;
+#pragma unroll
+                        for (int kk = 0; kk < kN / 16; ++kk)
+                            tc_mma_ts(tmem + 256 + 128u * x, tmem + 128u * x + 64u + 8u * kk, tc_desc_mn(v + kk * 2048u, kBox),
+                                      id_o, (j > part.j0 || kk) ? 1u : 0u);
+                        tc_commit_to(&bar.o[x]);
+                        if (x == tiles_x - 1) tc_commit_to(&bar.empty_v[st]);
+                    }
+                    __syncwarp();
+                    if (j + 1 < part.j1) {
+                        // S takes the columns that P is read from
+                        tc_wait_bar(&bar.o[x], nx[x] & 1u, ok);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) return;
+                        scores(x, n + 1);
+                        if (!ok) return;
+                    }
+                    ++nx[x];
+                }
+            }
+        });
+    } else if (place.seq >= 0 && warp >= 2) {
+        // ---- the rows: thread = TMEM lane r of row tile x
+        const int x = (warp - 2) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+        const uint32_t tm_sx = tmem + 128u * x + lanes, tm_ox = tmem + 256 + 128u * x + lanes;
+        const float sc = a.scale_log2;
+        uint32_t n = 0;  // key tiles of this row tile so far
+        walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            const int rows_x = it.rows - 128 * x;  // rows of this tile (of 128)
+            const int row = it.row0 + 128 * x + r;
+            const bool mine = r < rows_x;
+            const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
+            float m = -INFINITY, l = 0.0f;  // m in base 2
+            if (rows_x > 0 && part.j0 < part.j1) {
+                // Q rows of this warp: D / 8 lanes of 16 bytes a row
+                {
+                    constexpr int CH = D / 8, RPP = 32 / CH;
+                    const int ch = lane % CH;
+#pragma unroll 4
+                    for (int i = 0; i < 32 / RPP; ++i) {
+                        const int rr = 32 * quarter + i * RPP + lane / CH;
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (rr < rows_x) {
+                            const int qrow = it.row0 + 128 * x + rr, t = a.by_g(qrow);
+                            w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                                (long long)(seq.row0 + t) * a.ldq +
+                                                                (long long)(it.kvh * a.G + qrow - t * a.G) * D + ch * 8);
+                        }
+                        const uint32_t at = base + L::kQ + x * L::kTile + (ch >> 3) * kBox + rr * 128 +
+                                            (((ch & 7) ^ (rr & 7)) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z),
+                                     "r"(w.w)
+                                     : "memory");
+                    }
+                    fence_proxy_async_smem();
+                    mbar_arrive(&bar.q[x]);
+                }
+                for (int j = part.j0; j < part.j1; ++j, ++n) {
+                    tc_wait_bar(&bar.s[x], n & 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const int k0 = tile_key<kN>(it, j);
+                    // a tile that every row of the item sees whole needs no mask
+                    const bool whole = k0 + kN - 1 <= it.pos_first &&
+                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
+                    float sv[64];
+                    // scores of keys [64 c, 64 c + 64) of the tile
+                    auto load = [&](int c) {
+                        tmem_ld64(tm_sx + 64 * c, sv);
+                        if (!whole) {
+                            const int hi = pos - k0 - 64 * c, lo = a.window > 0 ? hi - a.window : -1;
+                            const int sink = a.sinks - k0 - 64 * c;
+#pragma unroll
+                            for (int i = 0; i < 64; ++i) sv[i] = i <= hi && (i > lo || i < sink) ? sv[i] : -INFINITY;
+                        }
+                    };
+                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        load(c);
+#pragma unroll
+                        for (int i = 0; i < 64; i += 8)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(sv[i + e], sv[i + 4 + e]));
+                    }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+                    const bool grow = top > m + kRescale;
+                    if (j == part.j0) {
+                        m = top;
+                    } else if (__any_sync(0xffffffffu, grow)) {
+                        // O must hold the products before it is rescaled
+                        tc_wait_bar(&bar.o[x], (n - 1) & 1u, ok);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) return;
+                        tc_fence_after();
+                        const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            float o[32];
+                            tmem_ld32(tm_ox + 32 * c, o);
+                            uint32_t w[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+                            tmem_st32(tm_ox + 32 * c, w);
+                        }
+                        tmem_st_wait();
+                        if (grow) {
+                            l *= f;
+                            m = top;
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.0f : m;
+                    float ls[2] = {0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 1; c >= 0; --c) {
+                        if (c == 0) load(0);
+                        uint32_t w[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
+                            ls[0] += p0;
+                            ls[1] += p1;
+                            w[e] = Half16<T>::pack(p0, p1);
+                        }
+                        tmem_st32(tm_sx + 64 + 32 * c, w);
+                    }
+                    l += ls[0] + ls[1];
+                    tmem_st_wait();
+                    tc_fence_before();
+                    mbar_arrive(&bar.p[x]);
+                }
+                tc_wait_bar(&bar.o[x], (n - 1) & 1u, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                tc_fence_after();
+            }
+            // ---- the part's result: straight to out, or through the slots
+            const bool split = part.first != part.last, some = part.j0 < part.j1 && rows_x > 0;
+            const int ri = 128 * x + r;
+            bool write = true;
+            if (split) {
+                // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
+                float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
+                if (rows_x > 0) {
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        if (some) tmem_ld32(tm_ox + 32 * c, o);
+                        if (mine)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                reinterpret_cast<float4*>(slot)[(8 * c + e) * kM + ri] =
+                                    some ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3])
+                                         : make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                    if (mine) {
+                        slot[kM * D + ri] = m;
+                        slot[kM * D + kM + ri] = l;
+                    }
+                }
+                __threadfence();
+                named_sync(1, kRowThreads);
+                if (tid == 64) {
+                    unsigned* ticket = a.tickets + part.first;
+                    last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(part.last - part.first + 1);
+                    if (last_s) *ticket = 0u;  // ready for the next call
+                }
+                named_sync(1, kRowThreads);
+                __threadfence();
+                write = last_s != 0;
+            }
+            if (write && rows_x > 0) {
+                float M = m, lsum = l;
+                if (split && mine) {
+                    M = -INFINITY;
+                    lsum = 0.0f;
+                    for (long long b = part.first; b <= part.last; ++b)
+                        M = fmaxf(M, __ldcg(slot_of<kM, D>(a, b, part.first) + kM * D + ri));
+                    for (long long b = part.first; b <= part.last; ++b) {
+                        const float* p = slot_of<kM, D>(a, b, part.first) + kM * D + ri;
+                        const float mb = __ldcg(p);
+                        lsum = fmaf(__ldcg(p + kM), mb == -INFINITY ? 0.0f : ex2(mb - M), lsum);
+                    }
+                }
+                const bool sees = mine && pos >= 0;
+                const float inv = sees ? 1.0f / lsum : 0.0f;
+                const int head = it.kvh * a.G + row - token * a.G;
+                uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
+                                                      (mine ? (long long)(seq.row0 + token) * a.ldo + (long long)head * D
+                                                            : 0));
+                bool bad = false;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                    if (!split) {
+                        if (some) tmem_ld32(tm_ox + 32 * c, o);
+                    } else if (mine) {
+                        for (long long b = part.first; b <= part.last; ++b) {
+                            const float* p = slot_of<kM, D>(a, b, part.first);
+                            const float mb = __ldcg(p + kM * D + ri), f = mb == -INFINITY ? 0.0f : ex2(mb - M);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
+                                o[4 * e] = fmaf(v.x, f, o[4 * e]);
+                                o[4 * e + 1] = fmaf(v.y, f, o[4 * e + 1]);
+                                o[4 * e + 2] = fmaf(v.z, f, o[4 * e + 2]);
+                                o[4 * e + 3] = fmaf(v.w, f, o[4 * e + 3]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = sees ? o[e] * inv : 0.0f;
+                        bad |= !(fabsf(o[e]) < INFINITY);
+                    }
+                    if (mine)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            out[4 * c + e] = make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
+                                                        Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
+                                                        Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
+                                                        Half16<T>::pack(o[8 * e + 6], o[8 * e + 7]));
+                }
+                if (mine && a.lse)
+                    a.lse[(long long)(seq.row0 + token) * a.nq + head] =
+                        sees ? (M + log2f(lsum)) * kLn2 : -INFINITY;
+                // rows that met something not finite, term by term
+                for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
+                    __syncwarp();
+                    exact_row<T, D>(a, seq, part.s, it.kvh, it.row0 + 128 * x + 32 * quarter + __ffs(left) - 1);
+                }
+            }
+            // O, S and the slots' flag are read before the next part begins
+            tc_fence_before();
+            if (split) named_sync(1, kRowThreads);
+        });
+    }
+    if (!ok) atomicExch(&ok_s, 0);
+    tc_fence_before();
+    __syncthreads();
+    if (!ok_s) {
+        // a wait ran out: tell the host, and let copies in flight land
+        if (tid == 0 && a.err) atomicOr(a.err, kErrWaitTimeout);
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20000000ll) __nanosleep(1000);
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+int encode_pool(CUtensorMap* map, const AttnArgs& a, const void* pool, int D, bool bf16) {
+    auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+    INFERNT_REQUIRE(fn, "paged_attention: cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.b.page_size, (cuuint64_t)a.b.nkv,
+                                (cuuint64_t)a.b.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)a.b.page_size * D * 2,
+                                   (cuuint64_t)a.b.nkv * a.b.page_size * D * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(a.b.page_size < kN ? a.b.page_size : kN), 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r =
+        fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool),
+           dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    INFERNT_REQUIRE(r == CUDA_SUCCESS, "paged_attention: tensor map encoding failed (%d)", (int)r);
+    return INFERNT_OK;
+}
+
+template <typename T, int D>
+int launch_tc(const AttnArgs& args, cudaStream_t st) {
+    using L = LayoutTc<D>;
+    AttnArgs a = args;
+    CUtensorMap mk, mv;
+    if (int s = encode_pool(&mk, a, a.k, D, Half16<T>::kBf16)) return s;
+    if (int s = encode_pool(&mv, a, a.v, D, Half16<T>::kBf16)) return s;
+    INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)L::kBytes));
+    // one CTA an SM, as many as have slots in the workspace
+    constexpr int most = (int)((kWorkspaceBytes - kSlotsAt) / (2 * slot_floats<kM, D>() * sizeof(float)));
+    int ctas = sm_count();
+    if (ctas > most) ctas = most;
+    if (ctas > kMaxCtas) ctas = kMaxCtas;
+    a.min_tiles = 2;
+    paged_attn_tc<T, D><<<ctas, kThreadsTc, L::kBytes, st>>>(a, mk, mv);
+    INFERNT_CUDA_TRY(cudaGetLastError());
+    return INFERNT_OK;
+}
+
+}  // namespace
+
+int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st) {
+    if (dtype == INFERNT_DTYPE_BF16)
+        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, st) : launch_tc<__nv_bfloat16, 128>(a, st);
+    return head_dim == 64 ? launch_tc<__half, 64>(a, st) : launch_tc<__half, 128>(a, st);
+}
+
+}  // namespace infernt

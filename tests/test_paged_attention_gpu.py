@@ -129,7 +129,7 @@ def test_hidden_by_a_window(torch, ws):
     assert bool(torch.isnan(c.out[shown]).all())
 
 
-@pytest.mark.parametrize("q_scale,scale", [(8.0, 0.0), (1.0, 0.5), (1.0, -0.25), (30.0, 0.0)])
+@pytest.mark.parametrize("q_scale,scale", [(8.0, 0.0), (1.0, 0.5), (1.0, 0.004), (30.0, 0.0)])
 def test_peaked_scores(torch, ws, q_scale, scale):
     c = run(Case(torch, [(1, 900), (100, 700)], 8, 2, 128, 32, q_scale=q_scale), ws, scale=scale)
     check_attention(c, scale=scale)

@@ -55,7 +55,9 @@ def test_bad_batches_are_refused(kw):
 @pytest.mark.parametrize("kw", [
     dict(out=None), dict(q=None), dict(ws=None), dict(q=A + 2), dict(out=A + 8), dict(ws=A + 4), dict(nq=0),
     dict(nq=3), dict(nq=2 * 129), dict(ldq=255), dict(ldq=260), dict(ldo=248), dict(window=-1),
-    dict(sinks=-1, window=4), dict(sinks=4), dict(scale=float("nan")), dict(scale=float("inf"))])
+    dict(sinks=-1, window=4), dict(sinks=4), dict(scale=float("nan")), dict(scale=float("inf")),
+    dict(scale=-0.1), dict(b=batch(num_rows=1 << 29), nq=4),
+    dict(b=batch(num_rows=1 << 27, max_q_len=1 << 27, table_stride=1 << 20))])
 def test_bad_attention_arguments_are_refused(kw):
     assert attention(**kw) == 1
     assert ib.lib().infernt_last_error() != b""
