@@ -255,10 +255,10 @@ __device__ __forceinline__ Joined join_shares(const float* o_s, int shares, int 
 }
 
 template <int M, int D>
-__device__ __forceinline__ Joined join_slots(const AttnArgs& a, long long first, long long last, int r, int d) {
+__device__ __forceinline__ Joined join_slots(const AttnArgs& a, int first, int last, int r, int d) {
     Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
-    for (long long b = first; b <= last; ++b) v.m = fmaxf(v.m, __ldcg(slot_of<M, D>(a, b, first) + M * D + r));
-    for (long long b = first; b <= last; ++b) {
+    for (int b = first; b <= last; ++b) v.m = fmaxf(v.m, __ldcg(slot_of<M, D>(a, b, first) + M * D + r));
+    for (int b = first; b <= last; ++b) {
         const float* p = slot_of<M, D>(a, b, first);
         const float mk = __ldcg(p + M * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
         const float2 o = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
@@ -286,7 +286,7 @@ __device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& se
 
 // Counts this CTA's arrival at an item split over `parts` CTAs; true for the
 // last one, which then sees the others' slots.
-__device__ __forceinline__ bool last_to_arrive(unsigned* ticket, long long parts) {
+__device__ __forceinline__ bool last_to_arrive(unsigned* ticket, int parts) {
     __shared__ int s_last;
     __threadfence();
     __syncthreads();
@@ -300,7 +300,7 @@ __device__ __forceinline__ bool last_to_arrive(unsigned* ticket, long long parts
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) paged_attn(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) paged_attn(const __grid_constant__ AttnArgs a) {
     using L = Layout<D>;
     constexpr int M = kItemRows;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) paged_attn(const At
     float* o_s = reinterpret_cast<float*>(smem);
     unsigned char* flag = smem + L::kRing + 2 * kTileKeys * 4;
     const Place place = find_place<M, kTileKeys, kThreads>(a);
-    if (place.seq < 0) return;
+    if (place.s < 0) return;
     walk<M, kTileKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
         int shares;
         if (it.rows <= 16) {
@@ -392,11 +392,13 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     INFERNT_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "%s: scale %g", op, scale);
     const int G = nq / nkv;
     INFERNT_REQUIRE((long long)batch->num_rows * G < kMaxPositions, "%s: %d rows of %d heads", op, batch->num_rows, nq);
-    // the tiles of one KV head of a sequence are counted in 32 bits
-    const long long most_q = batch->max_q_len < batch->num_rows ? batch->max_q_len : batch->num_rows;
+    // the units of the schedule are counted in 32 bits
     const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
-    INFERNT_REQUIRE((most_q * G / kItemRows + 1) * (most_kv / kTileKeys + 2) < (1ll << 31),
-                    "%s: %lld new tokens of %d heads over %lld positions (split the chunk)", op, most_q, G, most_kv);
+    const bool chunks = paged_attention_tc_pages(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
+    const long long tile_m = chunks ? kTcItemRows : kItemRows, tile_n = chunks ? kTcTileKeys : kTileKeys;
+    INFERNT_REQUIRE(((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv < (1ll << 30) / (most_kv / tile_n + 2),
+                    "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
+                    most_kv);
     if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
     if (int s = check_device_pointer(op, "the cache", cache->k)) return s;
     if (int s = check_device_pointer(op, "q", q)) return s;
@@ -422,8 +424,7 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (paged_attention_tc_pages(cache->page_size) && (long long)batch->max_q_len * a.G > kItemRows)
-        return paged_attention_tc(a, D, cache->dtype, st);
+    if (chunks) return paged_attention_tc(a, D, cache->dtype, st);
     if (cache->dtype == INFERNT_DTYPE_BF16)
         return D == 64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
     return D == 64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);

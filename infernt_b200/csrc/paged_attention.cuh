@@ -32,7 +32,9 @@ struct AttnArgs {
     unsigned* err;
 };
 
-// The tcgen05 kernel (paged_attention_tc.cu); pages as paged_attention_tc_pages says.
+// The tcgen05 kernel (paged_attention_tc.cu): its items and tiles; pages as paged_attention_tc_pages says.
+constexpr int kTcItemRows = 256;
+constexpr int kTcTileKeys = 128;
 int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st);
 bool paged_attention_tc_pages(int page_size);
 
@@ -124,23 +126,26 @@ __device__ __forceinline__ int find_item(const AttnArgs& a, const PagedSeq& s, i
     }
 }
 
+// Units are counted in 32 bits: the host refuses a call whose bound on them is
+// larger.
 struct Place {
-    long long c;       // units of a CTA
-    long long before;  // units before sequence seq
-    long long total;
-    int seq;           // the sequence that holds unit c x blockIdx.x; -1: nothing for this CTA
+    int c;       // units of a CTA
+    int before;  // units before sequence s
+    int total;
+    int s;       // the sequence that holds unit c x blockIdx.x; -1: nothing for this CTA
+    PagedSeq seq;
+    int per_head;  // units of one of its KV heads
 };
 
 // By all NT threads of the block.
 template <int M, int N, int NT>
 __device__ __forceinline__ Place find_place(const AttnArgs& a) {
-    __shared__ long long sums_s[NT / 32];
-    __shared__ long long before_s;
-    __shared__ int seq_s;
+    __shared__ int sums_s[NT / 32];
+    __shared__ Place place_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.b.num_seqs;
-    // units of sequence s (every thread its own); long ones by the whole warp
-    auto units = [&](int s) {
-        PagedSeq q = {0, 0, 0};
+    // units of a KV head of sequence s (every thread its own); long ones by the whole warp
+    auto units = [&](int s, PagedSeq& q) {
+        q = {0, 0, 0};
         if (s < n) q = paged_seq(a.b, s, blockIdx.x == 0 ? a.err : nullptr);
         const bool many = q.n_new * a.G > 2 * M;
         int u = many ? 0 : item_units<M, N>(a, q, 0) + item_units<M, N>(a, q, M);
@@ -151,20 +156,15 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
             const int x = head_units<M, N>(a, w);
             if (lane == k) u = x;
         }
-        return (long long)u * a.b.nkv;
+        return u;
     };
     // the sum of the values before this thread's, and of all of them
-    auto scan = [&](long long v, long long& all) {
-        long long x = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
+    auto scan = [&](int v, int& all) {
+        const int x = warp_scan(v);
         __syncthreads();
         if (lane == 31) sums_s[warp] = x;
         __syncthreads();
-        long long pre = x - v;
+        int pre = x - v;
         all = 0;
 #pragma unroll
         for (int w = 0; w < NT / 32; ++w) {
@@ -173,76 +173,77 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
         }
         return pre;
     };
-    if (tid == 0) seq_s = -1;
-    Place p;
-    long long mine = 0, before = 0;
-    p.total = 0;
+    Place p = {0, 0, 0, -1, {0, 0, 0}, 0};
+    if (tid == 0) place_s.s = -1;
+    int before = 0;
     for (int base = 0; base < n; base += NT) {
-        long long all;
-        mine = units(base + tid);
-        before = p.total + scan(mine, all);
+        int all;
+        p.per_head = units(base + tid, p.seq);
+        before = p.total + scan(p.per_head * a.b.nkv, all);
         p.total += all;
     }
-    p.c = max((long long)a.min_tiles, (p.total + gridDim.x - 1) / gridDim.x);
-    const long long at = p.c * blockIdx.x;
-    long long sum = 0;
-    for (int base = 0; base < n; base += NT) {
-        if (n > NT) {  // a second pass; up to NT sequences are still in registers
-            long long all;
-            mine = units(base + tid);
-            before = sum + scan(mine, all);
-            sum += all;
+    p.c = max(a.min_tiles, (int)(((unsigned)p.total + gridDim.x - 1) / gridDim.x));
+    const int at = p.c * (int)blockIdx.x;
+    int sum = 0;
+    if (at < p.total)
+        for (int base = 0; base < n; base += NT) {
+            if (n > NT) {  // a second pass; up to NT sequences are still in registers
+                int all;
+                p.per_head = units(base + tid, p.seq);
+                before = sum + scan(p.per_head * a.b.nkv, all);
+                sum += all;
+            }
+            if (before <= at && at - before < p.per_head * a.b.nkv) {
+                p.before = before;
+                p.s = base + tid;
+                place_s = p;
+            }
         }
-        if (before <= at && at < before + mine) {
-            seq_s = base + tid;
-            before_s = before;
-        }
-    }
     __syncthreads();
-    p.seq = seq_s;
-    p.before = before_s;
-    return p;
+    return place_s;
 }
 
 // Part [j0, j1) of an item's tiles; first and last: the CTAs that the item
 // begins and ends in.
 struct Part {
-    int s, j0, j1;
-    long long first, last;
+    int s, j0, j1, first, last;
 };
 
 // f(sequence, item, part) for the parts of this CTA, by whole warps.
 template <int M, int N, typename F>
 __device__ __forceinline__ void walk(const AttnArgs& a, const Place& p, F f) {
-    long long at = p.c * blockIdx.x, before = p.before;
-    const long long end = min(at + p.c, p.total);
-    for (int s = p.seq; at < end && s < a.b.num_seqs; ++s) {
-        const PagedSeq seq = paged_seq(a.b, s, nullptr);
-        const int per_head = head_units<M, N>(a, seq);
-        if (per_head == 0) continue;
-        int kvh = (int)((at - before) / per_head);
-        long long u0 = before + (long long)kvh * per_head;
-        int rem = (int)(at - u0);
-        int row0 = find_item<M, N>(a, seq, rem);
-        u0 += rem;
-        while (kvh < a.b.nkv && at < end) {
-            const Item it = make_item<M, N>(a, seq, kvh, row0);
-            const int units = max(1, it.tiles);
-            Part part;
-            part.s = s;
-            part.j0 = (int)(at - u0);
-            part.j1 = min(it.tiles, (int)min((long long)units, end - u0));
-            part.first = u0 / p.c;
-            part.last = (u0 + units - 1) / p.c;
-            f(seq, it, part);
-            at = u0 += units;
-            row0 += M;
-            if (row0 >= seq.n_new * a.G) {
-                row0 = 0;
-                ++kvh;
+    int at = p.c * (int)blockIdx.x, before = p.before, per_head = p.per_head;
+    const int end = min(p.c, p.total - at) + at, me = blockIdx.x;
+    PagedSeq seq = p.seq;
+    for (int s = p.s;;) {
+        if (per_head > 0) {
+            int kvh = (at - before) / per_head;
+            int u0 = before + kvh * per_head, rem = at - u0;
+            int row0 = find_item<M, N>(a, seq, rem);
+            u0 += rem;
+            while (kvh < a.b.nkv && at < end) {
+                const Item it = make_item<M, N>(a, seq, kvh, row0);
+                const int units = max(1, it.tiles);
+                Part part;
+                part.s = s;
+                part.j0 = at - u0;
+                part.j1 = min(it.tiles, min(units, end - u0));
+                // an item that neither began before this CTA nor goes on after it is its own
+                part.first = u0 >= me * p.c ? me : u0 / p.c;
+                part.last = end - u0 >= units ? me : (u0 + units - 1) / p.c;
+                f(seq, it, part);
+                at = u0 += units;
+                row0 += M;
+                if (row0 >= seq.n_new * a.G) {
+                    row0 = 0;
+                    ++kvh;
+                }
             }
+            before += per_head * a.b.nkv;
         }
-        before += (long long)per_head * a.b.nkv;
+        if (at >= end || ++s >= a.b.num_seqs) break;
+        seq = paged_seq(a.b, s, nullptr);
+        per_head = head_units<M, N>(a, seq);
     }
 }
 
@@ -274,7 +275,7 @@ __device__ __forceinline__ float ex2(float x) {
 // here only what the row sees is touched, so what a row does see that is not
 // finite still shows in its result as in the formula.
 template <typename T, int D>
-__device__ void exact_row(const AttnArgs& a, const PagedSeq& seq, int s, int kvh, int row) {
+__device__ __noinline__ void exact_row(const AttnArgs& a, const PagedSeq& seq, int s, int kvh, int row) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31, token = a.by_g(row), head = kvh * a.G + row - token * a.G;
     const int pos = row_pos(seq, token);
@@ -321,7 +322,7 @@ constexpr size_t slot_floats() {
 
 // The slot of CTA b for an item whose first CTA is `first`.
 template <int M, int D>
-__device__ __forceinline__ float* slot_of(const AttnArgs& a, long long b, long long first) {
+__device__ __forceinline__ float* slot_of(const AttnArgs& a, int b, int first) {
     return a.slots + (size_t)(2 * b + (b == first)) * slot_floats<M, D>();
 }
 

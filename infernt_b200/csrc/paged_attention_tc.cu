@@ -12,17 +12,21 @@
 // The two row tiles take turns: while the threads of one compute
 // probabilities, the tensor cores run the other's products.
 //
-// Ten warps: warp 0 loads K and V tiles page by page by TMA (a tensor map of
-// the pool [page][KV head][position][dim]; a page that no row sees, or that
+// Twelve warps: warp 0 loads K and V tiles page by page by TMA (a tensor map
+// of the pool [page][KV head][position][dim]; a page that no row sees, or that
 // the pool does not have, is a coordinate past its end and becomes zeros),
-// warp 1 issues the MMAs, warps 2-5 and 6-9 hold the rows of A and B.  A row's
-// 128 scores would not fit its thread's registers beside the rest, so the
-// first 64 are read from TMEM twice: for the maximum, and after the
-// probabilities of the last 64 are stored (into columns 96-127 of S; those of
-// the first 64 into 64-95).  The
-// reference maximum m moves only when a row's maximum passes it by 8, so O is
-// rescaled seldom.  V rows that no row of the item sees are zeroed in shared
-// memory, so that what lies there does not meet a probability of 0.
+// warp 1 issues the MMAs, warp 2 zeroes V rows that no row of the item sees
+// (so that what lies there does not meet a probability of 0), warps 4-7 and 8-11 hold the rows of A and B.  Of
+// the 384 x 168 registers of a launch the first four warps keep 88 a thread,
+// the others take 208.
+//
+// A row's reference maximum m moves only when a score passes it by 8 (in base
+// 2), so O is rescaled seldom, and a tile's probabilities are computed with
+// the m it finds, beside the search for the tile's maximum; only when some
+// row's maximum has moved are they computed again.  One pair in four takes
+// 2^x on the FMA pipe (nearest integer, then a polynomial of degree 4 on the
+// rest), since the 16 results a clock of the special function unit would take
+// as long as both products.
 #include <cmath>
 #include <cstdint>
 
@@ -43,9 +47,9 @@ bool paged_attention_tc_pages(int page_size) {
 
 namespace {
 
-constexpr int kM = 256;  // query rows of an item
-constexpr int kN = 128;  // keys of a tile
-constexpr int kThreadsTc = 320;
+constexpr int kM = kTcItemRows;  // query rows of an item
+constexpr int kN = kTcTileKeys;  // keys of a tile
+constexpr int kThreadsTc = 384;
 constexpr int kRowThreads = 256;
 constexpr uint32_t kBox = 16384;  // 128 rows of 64 values: a swizzled operand block
 
@@ -63,13 +67,76 @@ struct LayoutTc {
 };
 
 struct Barriers {
-    uint64_t full_k[4], empty_k[4], full_v[4], empty_v[4];
+    uint64_t full_k[4], empty_k[4], full_v[4], clean_v[4], empty_v[4];
     uint64_t q[2], s[2], p[2], o[2];
 };
 
+// Pairs of FP32 values, each lane rounded as the scalar operation.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 un2(F2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x of a pair without the special function unit, for x <= 100 (from -126
+// down it stays at 2^-126): n = x to the nearest integer by the addition of
+// 3 x 2^22, 2^(x - n) by the polynomial of least largest relative error on
+// [-1/2, 1/2] (2.7e-6 in FP32), n added to its exponent.
+__device__ __forceinline__ float2 ex2_pair(F2 x) {
+    const float2 v = un2(x);
+    x = f2(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    const F2 big = f2(12582912.0f, 12582912.0f), less = f2(-12582912.0f, -12582912.0f), minus = f2(-1.0f, -1.0f);
+    const F2 t = add2(x, big), f = fma2(add2(t, less), minus, x);
+    F2 p = f2(0.009570102207362652f, 0.009570102207362652f);
+    p = fma2(p, f, f2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, f2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
+    const float2 n = un2(t), q = un2(p);
+    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
+                       __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
+}
+
+// Whether the tile at key k0 has keys that no row of the item sees.
+__device__ __forceinline__ bool has_hidden(const Item& it, int k0) {
+    return k0 + kN > it.hi || (k0 < it.lo && k0 + kN > it.sink_end);
+}
+
+// V rows of a tile in shared memory at v that no row of the item sees, by a
+// warp: they may hold anything, and 0 times infinity is not 0.
+template <int NB>
+__device__ __forceinline__ void zero_rows(const Item& it, int k0, uint32_t v) {
+    for (int r = threadIdx.x & 31; r < kN; r += 32)
+        if (!item_sees(it, k0 + r))
+#pragma unroll
+            for (int c = 0; c < NB * 8; ++c)  // every lane another 16-byte column
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * kBox + r * 128 +
+                                                                             (((c ^ r) & 7) << 4)),
+                             "r"(0)
+                             : "memory");
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreadsTc, 1)
-    paged_attn_tc(const AttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    paged_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using L = LayoutTc<D>;
     constexpr int NB = (int)L::kBlocks, ST = L::kStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -84,6 +151,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             mbar_init(&bar.full_k[i], 1);
             mbar_init(&bar.empty_k[i], 1);
             mbar_init(&bar.full_v[i], 1);
+            mbar_init(&bar.clean_v[i], 1);
             mbar_init(&bar.empty_v[i], 1);
         }
         for (int x = 0; x < 2; ++x) {
@@ -101,8 +169,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     __syncthreads();
     const uint32_t tmem = tmem_s;  // S (and P) of A at 0, of B at 128; O of A at 256, of B at 384
     bool ok = true;
-
-    if (place.seq >= 0 && warp == 0) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+        if (warp == 0 && place.s >= 0) {
         // ---- K and V tiles.  n: tiles so far, over all parts.
         uint32_t n = 0;
         const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
@@ -146,91 +215,106 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                     it.kvh, page, &bar.full_v[st]);
             }
         });
-    } else if (place.seq >= 0 && warp == 1) {
-        // ---- the MMAs, issued by lane 0.  n: key tiles so far, nx: those of row tile X.
-        uint32_t n = 0, nx[2] = {0, 0}, parts[2] = {0, 0};
-        const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kN), id_o = tc_instr(Half16<T>::kBf16, true, D);
-        walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
-            if (part.j0 >= part.j1 || !ok) return;
-            const int tiles_x = it.rows > 128 ? 2 : 1;
-            // S_x of key tile number m
-            auto scores = [&](int x, uint32_t m) {
-                const int st = (int)(m % ST);
-                tc_wait_bar(&bar.full_k[st], (m / ST) & 1u, ok);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t q = base + L::kQ + x * L::kTile, k = base + L::kK + st * L::kTile;
+        } else if (warp == 1 && place.s >= 0) {
+        // ---- the MMAs, issued by one lane.  n: key tiles so far (those of A), nb: those of B.
+            // This lane's path decides how soon a row tile's next scores come,
+            // so it is kept short and rolled: one warp that runs through long
+            // code once a tile waits for its instructions.
+            uint32_t n = 0, nb = 0, parts_a = 0, parts_b = 0;
+            const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kN), id_o = tc_instr(Half16<T>::kBf16, true, D);
+            const bool leader = tc_elect();
+            walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+                if (leader && part.j0 < part.j1 && ok) {
+                    const int last_x = it.rows > 128 ? 1 : 0, tiles = part.j1 - part.j0;
+                    // O += P V of tile j - 1, then S = Q K^T of tile j over P's columns, A and B in turn
+#pragma unroll 1
+                    for (int j = 0; j <= tiles; ++j, ++n) {
+                        const uint32_t st = n % ST, m = n - 1, sv = m % ST;
+#pragma unroll 1
+                        for (int x = 0; x <= last_x; ++x) {
+                            if (j == 0) {
+                                tc_wait_bar(&bar.q[x], (x ? parts_b : parts_a) & 1u, ok);
+                                if (x == 0) tc_wait_bar(&bar.full_k[st], (n / ST) & 1u, ok);
+                            } else {
+                                const uint32_t turn = (x ? nb + j - 1 : m) & 1u;
+                                if (x == 0) {
+                                    tc_wait_bar(&bar.full_v[sv], (m / ST) & 1u, ok);
+                                    tc_wait_bar(&bar.clean_v[sv], (m / ST) & 1u, ok);
+                                    if (j < tiles) tc_wait_bar(&bar.full_k[st], (n / ST) & 1u, ok);
+                                }
+                                tc_wait_bar(&bar.p[x], turn, ok);
+                                tc_fence_after();
+                                if (!ok) break;
+                                const uint32_t d = tmem + 256 + 128u * x, p = tmem + 128u * x + 64u;
+                                const uint64_t vd = tc_desc_mn(base + L::kV + sv * L::kTile, kBox);
 #pragma unroll
-                    for (int b = 0; b < NB; ++b)
+                                for (uint32_t kk = 0; kk < kN / 16; ++kk)
+                                    tc_mma_ts(d, p + 8u * kk, vd + kk * (2048u >> 4), id_o, (uint32_t)(j - 1) | kk);
+                                tc_commit_to(&bar.o[x]);
+                                if (x == last_x) tc_commit_to(&bar.empty_v[sv]);
+                                // S takes the columns that P is read from
+                                if (j < tiles) tc_wait_bar(&bar.o[x], turn, ok);
+                            }
+                            tc_fence_after();
+                            if (!ok) break;
+                            if (j < tiles) {
+                                const uint64_t q = tc_desc_k(base + L::kQ + x * L::kTile);
+                                const uint64_t k = tc_desc_k(base + L::kK + st * L::kTile);
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            tc_mma_ss(tmem + 128u * x, tc_desc_k(q + b * kBox) + 2 * kk, tc_desc_k(k + b * kBox) + 2 * kk,
-                                      id_s, (b | kk) ? 1u : 0u);
-                    tc_commit_to(&bar.s[x]);
-                    if (x == tiles_x - 1) tc_commit_to(&bar.empty_k[st]);
+                                for (uint32_t kk = 0; kk < D / 16; ++kk) {
+                                    // 32 bytes a step within a block of 64 columns
+                                    const uint32_t at = (kk >> 2) * (kBox >> 4) + 2 * (kk & 3);
+                                    tc_mma_ss(tmem + 128u * x, q + at, k + at, id_s, kk);
+                                }
+                                tc_commit_to(&bar.s[x]);
+                                if (x == last_x) tc_commit_to(&bar.empty_k[st]);
+                            }
+                        }
+                        if (!ok) break;
+                    }
+                    --n;  // the round that only finishes the last tile
+                    ++parts_a;
+                    if (last_x) {
+                        nb += tiles;
+                        ++parts_b;
+                    }
                 }
                 __syncwarp();
-            };
-            for (int x = 0; x < tiles_x; ++x) {
-                tc_wait_bar(&bar.q[x], parts[x] & 1u, ok);
-                ++parts[x];
-                scores(x, n);
-            }
-            for (int j = part.j0; j < part.j1 && ok; ++j, ++n) {
-                const int st = (int)(n % ST), k0 = tile_key<kN>(it, j);
-                for (int x = 0; x < tiles_x; ++x) {
-                    if (x == 0) {
-                        tc_wait_bar(&bar.full_v[st], (n / ST) & 1u, ok);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) return;
-                        if (k0 + kN > it.hi || (k0 < it.lo && k0 + kN > it.sink_end)) {
-                            // rows that no row of the item sees
-                            for (int r = 0; r < kN; ++r)
-                                if (!item_sees(it, k0 + r))
-                                    for (int c = lane; c < NB * 8; c += 32) {
-                                        const uint32_t at =
-                                            base + L::kV + st * L::kTile + (c >> 3) * kBox + r * 128 + (c & 7) * 16;
-                                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0)
-                                                     : "memory");
-                                    }
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                        }
-                    }
-                    tc_wait_bar(&bar.p[x], nx[x] & 1u, ok);
+            });
+        } else if (warp == 2 && place.s >= 0) {
+            // ---- V rows that no row of the item sees become zeros
+            uint32_t n = 0;
+            walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+                for (int j = part.j0; j < part.j1; ++j, ++n) {
+                    const int k0 = tile_key<kN>(it, j);
+                    const uint32_t st = n % ST;
+                    tc_wait_bar(&bar.full_v[st], (n / ST) & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return;
-                    tc_fence_after();
-                    if (lane == 0) {
-                        const uint32_t v = base + L::kV + st * L::kTile;
-#pragma unroll
-                        for (int kk = 0; kk < kN / 16; ++kk)
-                            tc_mma_ts(tmem + 256 + 128u * x, tmem + 128u * x + 64u + 8u * kk, tc_desc_mn(v + kk * 2048u, kBox),
-                                      id_o, (j > part.j0 || kk) ? 1u : 0u);
-                        tc_commit_to(&bar.o[x]);
-                        if (x == tiles_x - 1) tc_commit_to(&bar.empty_v[st]);
-                    }
-                    __syncwarp();
-                    if (j + 1 < part.j1) {
-                        // S takes the columns that P is read from
-                        tc_wait_bar(&bar.o[x], nx[x] & 1u, ok);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) return;
-                        scores(x, n + 1);
-                        if (!ok) return;
-                    }
-                    ++nx[x];
+                    if (has_hidden(it, k0)) zero_rows<NB>(it, k0, base + L::kV + st * L::kTile);
+                    if (lane == 0) mbar_arrive(&bar.clean_v[st]);
                 }
-            }
-        });
-    } else if (place.seq >= 0 && warp >= 2) {
+            });
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
+        if (place.s >= 0) {
         // ---- the rows: thread = TMEM lane r of row tile x
-        const int x = (warp - 2) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+        const int x = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
         const uint32_t tm_sx = tmem + 128u * x + lanes, tm_ox = tmem + 256 + 128u * x + lanes;
         const float sc = a.scale_log2;
+        const F2 sc2 = f2(sc, sc);
+        constexpr int CH = D / 8, RPI = 32 / CH, LI = 32 / RPI;  // 16-byte chunks of a row, rows at once, rounds
+        const int ch = lane % CH;
+        // 16-byte chunk c of row rr of the row tile's Q (and, at the end, its result)
+        auto own_chunk = [&](int rr, int c) {
+            return base + L::kQ + x * L::kTile + (c >> 3) * kBox + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+        };
+        auto st_shared = [](uint32_t at, uint4 w) {
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                         : "memory");
+        };
         uint32_t n = 0;  // key tiles of this row tile so far
         walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
             ok = __all_sync(0xffffffffu, ok);
@@ -241,26 +325,22 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
             float m = -INFINITY, l = 0.0f;  // m in base 2
             if (rows_x > 0 && part.j0 < part.j1) {
-                // Q rows of this warp: D / 8 lanes of 16 bytes a row
+                // Q rows of this warp: D / 8 lanes of 16 bytes a row, all in flight at once
                 {
-                    constexpr int CH = D / 8, RPP = 32 / CH;
-                    const int ch = lane % CH;
-#pragma unroll 4
-                    for (int i = 0; i < 32 / RPP; ++i) {
-                        const int rr = 32 * quarter + i * RPP + lane / CH;
-                        uint4 w = make_uint4(0, 0, 0, 0);
+                    uint4 w[LI];
+#pragma unroll
+                    for (int i = 0; i < LI; ++i) {
+                        const int rr = 32 * quarter + i * RPI + lane / CH, qrow = it.row0 + 128 * x + rr;
+                        w[i] = make_uint4(0, 0, 0, 0);
                         if (rr < rows_x) {
-                            const int qrow = it.row0 + 128 * x + rr, t = a.by_g(qrow);
-                            w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                                (long long)(seq.row0 + t) * a.ldq +
-                                                                (long long)(it.kvh * a.G + qrow - t * a.G) * D + ch * 8);
+                            const int t = a.by_g(qrow);
+                            w[i] = __ldg(reinterpret_cast<const uint4*>(
+                                static_cast<const uint16_t*>(a.q) + (long long)(seq.row0 + t) * a.ldq +
+                                (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
                         }
-                        const uint32_t at = base + L::kQ + x * L::kTile + (ch >> 3) * kBox + rr * 128 +
-                                            (((ch & 7) ^ (rr & 7)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z),
-                                     "r"(w.w)
-                                     : "memory");
                     }
+#pragma unroll
+                    for (int i = 0; i < LI; ++i) st_shared(own_chunk(32 * quarter + i * RPI + lane / CH, ch), w[i]);
                     fence_proxy_async_smem();
                     mbar_arrive(&bar.q[x]);
                 }
@@ -273,68 +353,110 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     // a tile that every row of the item sees whole needs no mask
                     const bool whole = k0 + kN - 1 <= it.pos_first &&
                                        (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
-                    float sv[64];
-                    // scores of keys [64 c, 64 c + 64) of the tile
-                    auto load = [&](int c) {
-                        tmem_ld64(tm_sx + 64 * c, sv);
-                        if (!whole) {
-                            const int hi = pos - k0 - 64 * c, lo = a.window > 0 ? hi - a.window : -1;
-                            const int sink = a.sinks - k0 - 64 * c;
+                    bool done = false;
+                    if (whole && j > part.j0) {
+                        // probabilities under the m of the tiles before, and the maximum beside them
+                        const float ref = m == -INFINITY ? 0.0f : m;
+                        const F2 ref2 = f2(-ref, -ref);
+                        uint32_t w[2][32];
+                        float mx[2] = {-INFINITY, -INFINITY};
+                        F2 ls = f2(0.0f, 0.0f);
 #pragma unroll
-                            for (int i = 0; i < 64; ++i) sv[i] = i <= hi && (i > lo || i < sink) ? sv[i] : -INFINITY;
+                        for (int c = 0; c < 2; ++c) {
+                            float sv[64];
+                            tmem_ld64(tm_sx + 64 * c, sv);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float s0 = sv[2 * e], s1 = sv[2 * e + 1];
+                                mx[e & 1] = fmaxf(mx[e & 1], fmaxf(s0, s1));
+                                const F2 arg = fma2(f2(s0, s1), sc2, ref2);
+                                float2 p;
+                                if ((e & 3) == 3) {
+                                    p = ex2_pair(arg);
+                                } else {
+                                    const float2 v = un2(arg);
+                                    p = make_float2(ex2(v.x), ex2(v.y));
+                                }
+                                ls = add2(ls, f2(p.x, p.y));
+                                w[c][e] = Half16<T>::pack(p.x, p.y);
+                            }
                         }
-                    };
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        load(c);
-#pragma unroll
-                        for (int i = 0; i < 64; i += 8)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], fmaxf(sv[i + e], sv[i + 4 + e]));
+                        const bool grow = fmaxf(mx[0], mx[1]) * sc > m + kRescale;
+                        if (!__any_sync(0xffffffffu, grow)) {
+                            tmem_st32(tm_sx + 64, w[0]);
+                            tmem_st32(tm_sx + 96, w[1]);
+                            const float2 v = un2(ls);
+                            l += v.x + v.y;
+                            done = true;
+                        }
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-                    const bool grow = top > m + kRescale;
-                    if (j == part.j0) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, grow)) {
-                        // O must hold the products before it is rescaled
-                        tc_wait_bar(&bar.o[x], (n - 1) & 1u, ok);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) return;
-                        tc_fence_after();
-                        const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+                    if (!done) {
+                        // the first tile, tiles with hidden keys, and tiles whose maximum moves m
+                        float sv[64];
+                        // scores of keys [64 c, 64 c + 64) of the tile
+                        auto load = [&](int c) {
+                            tmem_ld64(tm_sx + 64 * c, sv);
+                            if (!whole) {
+                                const int hi = pos - k0 - 64 * c, lo = a.window > 0 ? hi - a.window : -1;
+                                const int sink = a.sinks - k0 - 64 * c;
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            float o[32];
-                            tmem_ld32(tm_ox + 32 * c, o);
+                                for (int i = 0; i < 64; ++i) sv[i] = i <= hi && (i > lo || i < sink) ? sv[i] : -INFINITY;
+                            }
+                        };
+                        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            load(c);
+#pragma unroll
+                            for (int i = 0; i < 64; i += 4) {
+                                mx[0] = fmaxf(mx[0], fmaxf(sv[i], sv[i + 1]));
+                                mx[1] = fmaxf(mx[1], fmaxf(sv[i + 2], sv[i + 3]));
+                            }
+                        }
+                        const float top = fmaxf(mx[0], mx[1]) * sc;
+                        const bool grow = top > m + kRescale;
+                        if (j == part.j0) {
+                            m = top;
+                        } else if (__any_sync(0xffffffffu, grow)) {
+                            // O must hold the products before it is rescaled
+                            tc_wait_bar(&bar.o[x], (n - 1) & 1u, ok);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) return;
+                            tc_fence_after();
+                            const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) {
+                                float o[32];
+                                tmem_ld32(tm_ox + 32 * c, o);
+                                uint32_t w[32];
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+                                tmem_st32(tm_ox + 32 * c, w);
+                            }
+                            tmem_st_wait();
+                            if (grow) {
+                                l *= f;
+                                m = top;
+                            }
+                        }
+                        const float ref = m == -INFINITY ? 0.0f : m;
+                        float ls[2] = {0.0f, 0.0f};
+                        // the last keys first: the columns of P lie over their scores
+#pragma unroll
+                        for (int c = 1; c >= 0; --c) {
+                            if (c == 0) load(0);
                             uint32_t w[32];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-                            tmem_st32(tm_ox + 32 * c, w);
+                            for (int e = 0; e < 32; ++e) {
+                                const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
+                                ls[0] += p0;
+                                ls[1] += p1;
+                                w[e] = Half16<T>::pack(p0, p1);
+                            }
+                            tmem_st32(tm_sx + 64 + 32 * c, w);
                         }
-                        tmem_st_wait();
-                        if (grow) {
-                            l *= f;
-                            m = top;
-                        }
+                        l += ls[0] + ls[1];
                     }
-                    const float ref = m == -INFINITY ? 0.0f : m;
-                    float ls[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 1; c >= 0; --c) {
-                        if (c == 0) load(0);
-                        uint32_t w[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
-                            ls[0] += p0;
-                            ls[1] += p1;
-                            w[e] = Half16<T>::pack(p0, p1);
-                        }
-                        tmem_st32(tm_sx + 64 + 32 * c, w);
-                    }
-                    l += ls[0] + ls[1];
                     tmem_st_wait();
                     tc_fence_before();
                     mbar_arrive(&bar.p[x]);
@@ -370,7 +492,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 __threadfence();
                 named_sync(1, kRowThreads);
-                if (tid == 64) {
+                if (tid == 128) {
                     unsigned* ticket = a.tickets + part.first;
                     last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(part.last - part.first + 1);
                     if (last_s) *ticket = 0u;  // ready for the next call
@@ -384,9 +506,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 if (split && mine) {
                     M = -INFINITY;
                     lsum = 0.0f;
-                    for (long long b = part.first; b <= part.last; ++b)
+                    for (int b = part.first; b <= part.last; ++b)
                         M = fmaxf(M, __ldcg(slot_of<kM, D>(a, b, part.first) + kM * D + ri));
-                    for (long long b = part.first; b <= part.last; ++b) {
+                    for (int b = part.first; b <= part.last; ++b) {
                         const float* p = slot_of<kM, D>(a, b, part.first) + kM * D + ri;
                         const float mb = __ldcg(p);
                         lsum = fmaf(__ldcg(p + kM), mb == -INFINITY ? 0.0f : ex2(mb - M), lsum);
@@ -394,58 +516,74 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 const bool sees = mine && pos >= 0;
                 const float inv = sees ? 1.0f / lsum : 0.0f;
-                const int head = it.kvh * a.G + row - token * a.G;
-                uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) +
-                                                      (mine ? (long long)(seq.row0 + token) * a.ldo + (long long)head * D
-                                                            : 0));
                 bool bad = false;
+                // 64 columns at a time into the row tile's Q, which the products are done with
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float o[32];
+                for (int c = 0; c < D / 64; ++c) {
+                    float o[64];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                    for (int e = 0; e < 64; ++e) o[e] = 0.0f;
                     if (!split) {
-                        if (some) tmem_ld32(tm_ox + 32 * c, o);
+                        if (some) tmem_ld64(tm_ox + 64 * c, o);
                     } else if (mine) {
-                        for (long long b = part.first; b <= part.last; ++b) {
+                        for (int b = part.first; b <= part.last; ++b) {
                             const float* p = slot_of<kM, D>(a, b, part.first);
                             const float mb = __ldcg(p + kM * D + ri), f = mb == -INFINITY ? 0.0f : ex2(mb - M);
+                            float4 v[16];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
-                                o[4 * e] = fmaf(v.x, f, o[4 * e]);
-                                o[4 * e + 1] = fmaf(v.y, f, o[4 * e + 1]);
-                                o[4 * e + 2] = fmaf(v.z, f, o[4 * e + 2]);
-                                o[4 * e + 3] = fmaf(v.w, f, o[4 * e + 3]);
+                            for (int e = 0; e < 16; ++e)
+                                v[e] = __ldcg(reinterpret_cast<const float4*>(p) + (16 * c + e) * kM + ri);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                o[4 * e] = fmaf(v[e].x, f, o[4 * e]);
+                                o[4 * e + 1] = fmaf(v[e].y, f, o[4 * e + 1]);
+                                o[4 * e + 2] = fmaf(v[e].z, f, o[4 * e + 2]);
+                                o[4 * e + 3] = fmaf(v[e].w, f, o[4 * e + 3]);
                             }
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
+                    for (int e = 0; e < 64; ++e) {
                         o[e] = sees ? o[e] * inv : 0.0f;
                         bad |= !(fabsf(o[e]) < INFINITY);
                     }
-                    if (mine)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            out[4 * c + e] = make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
-                                                        Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
-                                                        Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
-                                                        Half16<T>::pack(o[8 * e + 6], o[8 * e + 7]));
+                    for (int e = 0; e < 8; ++e)
+                        st_shared(own_chunk(r, 8 * c + e),
+                                  make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
+                                             Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
+                                             Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
+                                             Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
                 }
+                __syncwarp();
+                // whole rows by D / 8 lanes each
+#pragma unroll
+                for (int i = 0; i < LI; ++i) {
+                    const int rr = 32 * quarter + i * RPI + lane / CH, orow = it.row0 + 128 * x + rr;
+                    if (rr < rows_x) {
+                        const int t = a.by_g(orow);
+                        uint4 w;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                     : "r"(own_chunk(rr, ch))
+                                     : "memory");
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + t) * a.ldo +
+                                                  (it.kvh * a.G + orow - t * a.G) * D + ch * 8) = w;
+                    }
+                }
+                __syncwarp();
                 if (mine && a.lse)
-                    a.lse[(long long)(seq.row0 + token) * a.nq + head] =
+                    a.lse[(long long)(seq.row0 + token) * a.nq + it.kvh * a.G + row - token * a.G] =
                         sees ? (M + log2f(lsum)) * kLn2 : -INFINITY;
                 // rows that met something not finite, term by term
-                for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
-                    __syncwarp();
+                for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1)
                     exact_row<T, D>(a, seq, part.s, it.kvh, it.row0 + 128 * x + 32 * quarter + __ffs(left) - 1);
-                }
             }
             // O, S and the slots' flag are read before the next part begins
             tc_fence_before();
             if (split) named_sync(1, kRowThreads);
         });
+        }
     }
     if (!ok) atomicExch(&ok_s, 0);
     tc_fence_before();

@@ -50,6 +50,17 @@ __device__ __forceinline__ uint32_t tc_instr(bool bf16, bool b_mn, int n) {
            ((uint32_t)(128 >> 4) << 24);
 }
 
+// True in one lane of the warp, which the compiler knows to be alone: the
+// operands of an MMA then go to uniform registers without a loop over lanes.
+__device__ __forceinline__ bool tc_elect() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 // D[tmem] (+)= A[shared] B[shared], one K step of 16
 __device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, uint32_t acc) {
     asm volatile(
