@@ -3,22 +3,31 @@
 // formulas and the kernel for single tokens).
 //
 // An item is 256 query rows (new token, head of the group) of a KV head, two
-// tiles A and B of 128 rows, the M of the MMA; a tile of keys is 128.  Per
-// key tile i and row tile X:
+// tiles A and B of 128 rows, the M of the MMA; K and V arrive in tiles of 128
+// keys, worked off as two halves of 64.  Per half i and row tile X:
 //   S_X = Q_X K_i^T        A and B operands from shared memory, S in TMEM
 //   P_X = 2^(S_X scale - m) one thread per row: S out of TMEM, P back into it
-//                          in 16 bits, over the columns S has left
+//                          in 16 bits
 //   O_X += P_X V_i         A operand from TMEM, V as the pages hold it
-// The two row tiles take turns: while the threads of one compute
-// probabilities, the tensor cores run the other's products.
+// A group of MMAs ends 550 cycles after its last operand is read, so the
+// products of a row tile must not wait for one another: each row tile has
+// two score buffers of 64 columns, and while its threads work on one, S of
+// the next half goes into the other and P V of the half before is under way.
+// (Tiles of 128 keys with one buffer: 4300 cycles a pair of 128 x 128 tiles,
+// of which the products take 2048.  An MMA of 64 keys reads Q as often as one
+// of 128 and takes 49 cycles instead of 32; halves are still the better deal.)
+// At head_dim 128, O and S fill the 512 columns and P lies over the half of
+// its scores that has been read, so S of half i + 2 waits for P V of half i;
+// at 64 it has columns of its own.
 //
 // Twelve warps: warp 0 loads K and V tiles page by page by TMA (a tensor map
 // of the pool [page][KV head][position][dim]; a page that no row sees, or that
 // the pool does not have, is a coordinate past its end and becomes zeros),
-// warp 1 issues the MMAs, warp 2 zeroes V rows that no row of the item sees
-// (so that what lies there does not meet a probability of 0), warps 4-7 and 8-11 hold the rows of A and B.  Of
-// the 384 x 168 registers of a launch the first four warps keep 88 a thread,
-// the others take 208.
+// warps 1 and 3 issue the MMAs of A and of B, warp 2 zeroes V rows that no
+// row of the item sees (so that what lies there does not meet a probability
+// of 0), warps 4-7 and 8-11 hold the rows of A and B.  Of the 384 x 168
+// registers of a launch the first four warps keep 88 a thread, the others
+// take 208.
 //
 // A row's reference maximum m moves only when a score passes it by 8 (in base
 // 2), so O is rescaled seldom, and a tile's probabilities are computed with
@@ -49,6 +58,7 @@ namespace {
 
 constexpr int kM = kTcItemRows;  // query rows of an item
 constexpr int kN = kTcTileKeys;  // keys of a tile
+constexpr int kHalf = kN / 2;    // keys of a score buffer
 constexpr int kThreadsTc = 384;
 constexpr int kRowThreads = 256;
 constexpr uint32_t kBox = 16384;  // 128 rows of 64 values: a swizzled operand block
@@ -68,7 +78,8 @@ struct LayoutTc {
 
 struct Barriers {
     uint64_t full_k[4], empty_k[4], full_v[4], clean_v[4], empty_v[4];
-    uint64_t q[2], s[2], p[2], o[2];
+    uint64_t q[2];
+    uint64_t s[2][2], p[2][2], o[2][2];  // [row tile][half]
 };
 
 // Pairs of FP32 values, each lane rounded as the scalar operation.
@@ -149,16 +160,18 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             mbar_init(&bar.full_k[i], 1);
-            mbar_init(&bar.empty_k[i], 1);
+            mbar_init(&bar.empty_k[i], 2);
             mbar_init(&bar.full_v[i], 1);
             mbar_init(&bar.clean_v[i], 1);
-            mbar_init(&bar.empty_v[i], 1);
+            mbar_init(&bar.empty_v[i], 2);
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bar.q[x], 128);
-            mbar_init(&bar.s[x], 1);
-            mbar_init(&bar.p[x], 128);
-            mbar_init(&bar.o[x], 1);
+            for (int h = 0; h < 2; ++h) {
+                mbar_init(&bar.s[x][h], 1);
+                mbar_init(&bar.p[x][h], 128);
+                mbar_init(&bar.o[x][h], 1);
+            }
         }
         mbar_fence_init();
         ok_s = 1;
@@ -167,7 +180,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     const Place place = find_place<kM, kN, kThreadsTc>(a);  // its barriers publish the set-up
     tc_fence_after();
     __syncthreads();
-    const uint32_t tmem = tmem_s;  // S (and P) of A at 0, of B at 128; O of A at 256, of B at 384
+    // TMEM columns: S of A at 0 and 64, of B at 128 and 192; O of A at 256, of B D further; P
+    const uint32_t tmem = tmem_s;
+    auto tm_score = [&](int x, int h) { return tmem + 128u * x + 64u * h; };
+    auto tm_prob = [&](int x, int h) { return D == 128 ? tm_score(x, h) + 32u : tmem + 384u + 64u * x + 32u * h; };
+    auto tm_out = [&](int x) { return tmem + 256u + (uint32_t)D * x; };
     bool ok = true;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
@@ -215,68 +232,77 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                     it.kvh, page, &bar.full_v[st]);
             }
         });
-        } else if (warp == 1 && place.s >= 0) {
-        // ---- the MMAs, issued by one lane.  n: key tiles so far (those of A), nb: those of B.
-            // This lane's path decides how soon a row tile's next scores come,
-            // so it is kept short and rolled: one warp that runs through long
-            // code once a tile waits for its instructions.
-            uint32_t n = 0, nb = 0, parts_a = 0, parts_b = 0;
-            const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kN), id_o = tc_instr(Half16<T>::kBf16, true, D);
+        } else if ((warp == 1 || warp == 3) && place.s >= 0) {
+            // ---- the MMAs of row tile x, issued by one lane.  n: key tiles so far, nx: those of
+            // this row tile.  Each row tile has a warp of its own, so that neither waits for the
+            // other's probabilities.
+            const int x = warp >> 1;
+            uint32_t n = 0, nx = 0, parts = 0;
+            const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kHalf), id_o = tc_instr(Half16<T>::kBf16, true, D);
+            const uint64_t qd = tc_desc_k(base + L::kQ + x * L::kTile);
             const bool leader = tc_elect();
+            // S of half h of key tile m
+            auto scores = [&](uint32_t m, int h) {
+                const uint32_t st = m % ST;
+                const uint64_t k = tc_desc_k(base + L::kK + st * L::kTile + h * (kBox / 2));
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t kk = 0; kk < D / 16; ++kk) {
+                    // 32 bytes a step within a block of 64 columns
+                    const uint32_t at = (kk >> 2) * (kBox >> 4) + 2 * (kk & 3);
+                    tc_mma_ss(tm_score(x, h), qd + at, k + at, id_s, kk);
+                }
+                tc_commit_to(&bar.s[x][h]);
+                if (h) tc_commit_to(&bar.empty_k[st]);
+            };
             walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
-                if (leader && part.j0 < part.j1 && ok) {
-                    const int last_x = it.rows > 128 ? 1 : 0, tiles = part.j1 - part.j0;
-                    // O += P V of tile j - 1, then S = Q K^T of tile j over P's columns, A and B in turn
+                const int tiles = part.j1 - part.j0;
+                if (leader && tiles > 0 && ok) {
+                    if (it.rows <= 128 * x) {
+                        // no such rows: the stages go back unread
 #pragma unroll 1
-                    for (int j = 0; j <= tiles; ++j, ++n) {
-                        const uint32_t st = n % ST, m = n - 1, sv = m % ST;
+                        for (int j = 0; j < tiles; ++j, ++n) {
+                            const uint32_t st = n % ST, turn = (n / ST) & 1u;
+                            tc_wait_bar(&bar.full_k[st], turn, ok);
+                            mbar_arrive(&bar.empty_k[st]);
+                            tc_wait_bar(&bar.clean_v[st], turn, ok);
+                            mbar_arrive(&bar.empty_v[st]);
+                        }
+                    } else {
+                        tc_wait_bar(&bar.q[x], parts++ & 1u, ok);
+                        // round i: P V of half i - 2, then S of half i over its columns
 #pragma unroll 1
-                        for (int x = 0; x <= last_x; ++x) {
-                            if (j == 0) {
-                                tc_wait_bar(&bar.q[x], (x ? parts_b : parts_a) & 1u, ok);
-                                if (x == 0) tc_wait_bar(&bar.full_k[st], (n / ST) & 1u, ok);
-                            } else {
-                                const uint32_t turn = (x ? nb + j - 1 : m) & 1u;
-                                if (x == 0) {
-                                    tc_wait_bar(&bar.full_v[sv], (m / ST) & 1u, ok);
-                                    tc_wait_bar(&bar.clean_v[sv], (m / ST) & 1u, ok);
-                                    if (j < tiles) tc_wait_bar(&bar.full_k[st], (n / ST) & 1u, ok);
-                                }
-                                tc_wait_bar(&bar.p[x], turn, ok);
-                                tc_fence_after();
+                        for (int i = 0; i < 2 * tiles + 2 && ok; ++i) {
+                            const int h = i & 1;
+                            if (i >= 2) {
+                                const uint32_t m = n - 1, st = m % ST, turn = (m / ST) & 1u;
+                                const uint64_t v =
+                                    tc_desc_mn(base + L::kV + st * L::kTile + h * (kBox / 2), kBox);
+                                tc_wait_bar(&bar.full_v[st], turn, ok);
+                                tc_wait_bar(&bar.clean_v[st], turn, ok);
+                                tc_wait_bar(&bar.p[x][h], (nx - 1) & 1u, ok);
                                 if (!ok) break;
-                                const uint32_t d = tmem + 256 + 128u * x, p = tmem + 128u * x + 64u;
-                                const uint64_t vd = tc_desc_mn(base + L::kV + sv * L::kTile, kBox);
+                                tc_fence_after();
 #pragma unroll
-                                for (uint32_t kk = 0; kk < kN / 16; ++kk)
-                                    tc_mma_ts(d, p + 8u * kk, vd + kk * (2048u >> 4), id_o, (uint32_t)(j - 1) | kk);
-                                tc_commit_to(&bar.o[x]);
-                                if (x == last_x) tc_commit_to(&bar.empty_v[sv]);
-                                // S takes the columns that P is read from
-                                if (j < tiles) tc_wait_bar(&bar.o[x], turn, ok);
+                                for (uint32_t kk = 0; kk < kHalf / 16; ++kk)
+                                    tc_mma_ts(tm_out(x), tm_prob(x, h) + 8u * kk, v + kk * (2048u >> 4), id_o,
+                                              (uint32_t)(i - 2) | kk);
+                                tc_commit_to(&bar.o[x][h]);
+                                if (h) tc_commit_to(&bar.empty_v[st]);
                             }
-                            tc_fence_after();
-                            if (!ok) break;
-                            if (j < tiles) {
-                                const uint64_t q = tc_desc_k(base + L::kQ + x * L::kTile);
-                                const uint64_t k = tc_desc_k(base + L::kK + st * L::kTile);
-#pragma unroll
-                                for (uint32_t kk = 0; kk < D / 16; ++kk) {
-                                    // 32 bytes a step within a block of 64 columns
-                                    const uint32_t at = (kk >> 2) * (kBox >> 4) + 2 * (kk & 3);
-                                    tc_mma_ss(tmem + 128u * x, q + at, k + at, id_s, kk);
-                                }
-                                tc_commit_to(&bar.s[x]);
-                                if (x == last_x) tc_commit_to(&bar.empty_k[st]);
+                            if (i < 2 * tiles) {
+                                if (h == 0) tc_wait_bar(&bar.full_k[n % ST], (n / ST) & 1u, ok);
+                                if (D == 128 && i >= 2) tc_wait_bar(&bar.o[x][h], (nx - 1) & 1u, ok);
+                                if (!ok) break;
+                                scores(n, h);
+                            }
+                            if (h) {
+                                ++n;
+                                ++nx;
                             }
                         }
-                        if (!ok) break;
-                    }
-                    --n;  // the round that only finishes the last tile
-                    ++parts_a;
-                    if (last_x) {
-                        nb += tiles;
-                        ++parts_b;
+                        --n;  // the last round only finishes
+                        --nx;
                     }
                 }
                 __syncwarp();
@@ -302,7 +328,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         // ---- the rows: thread = TMEM lane r of row tile x
         const int x = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
         const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-        const uint32_t tm_sx = tmem + 128u * x + lanes, tm_ox = tmem + 256 + 128u * x + lanes;
+        const uint32_t tm_ox = tm_out(x) + lanes;
         const float sc = a.scale_log2;
         const F2 sc2 = f2(sc, sc);
         constexpr int CH = D / 8, RPI = 32 / CH, LI = 32 / RPI;  // 16-byte chunks of a row, rows at once, rounds
@@ -344,91 +370,74 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     fence_proxy_async_smem();
                     mbar_arrive(&bar.q[x]);
                 }
-                for (int j = part.j0; j < part.j1; ++j, ++n) {
-                    tc_wait_bar(&bar.s[x], n & 1u, ok);
+#pragma unroll 1
+                for (int i = 0; i < 2 * (part.j1 - part.j0); ++i) {
+                    const int h = i & 1, k0 = tile_key<kN>(it, part.j0 + (i >> 1)) + h * kHalf;
+                    tc_wait_bar(&bar.s[x][h], n & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return;
                     tc_fence_after();
-                    const int k0 = tile_key<kN>(it, j);
-                    // a tile that every row of the item sees whole needs no mask
-                    const bool whole = k0 + kN - 1 <= it.pos_first &&
-                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
+                    float sv[kHalf];
+                    tmem_ld64(tm_score(x, h) + lanes, sv);
+                    // keys that every row of the item sees need no mask
+                    const bool whole = k0 + kHalf - 1 <= it.pos_first &&
+                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kHalf <= a.sinks);
+                    uint32_t w[kHalf / 2];
+                    float lsum = 0.0f;
                     bool done = false;
-                    if (whole && j > part.j0) {
-                        // probabilities under the m of the tiles before, and the maximum beside them
+                    if (whole && i > 0) {
+                        // probabilities under the m of the halves before, and the maximum beside them
                         const float ref = m == -INFINITY ? 0.0f : m;
                         const F2 ref2 = f2(-ref, -ref);
-                        uint32_t w[2][32];
                         float mx[2] = {-INFINITY, -INFINITY};
                         F2 ls = f2(0.0f, 0.0f);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float sv[64];
-                            tmem_ld64(tm_sx + 64 * c, sv);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float s0 = sv[2 * e], s1 = sv[2 * e + 1];
-                                mx[e & 1] = fmaxf(mx[e & 1], fmaxf(s0, s1));
-                                const F2 arg = fma2(f2(s0, s1), sc2, ref2);
-                                float2 p;
-                                if ((e & 3) == 3) {
-                                    p = ex2_pair(arg);
-                                } else {
-                                    const float2 v = un2(arg);
-                                    p = make_float2(ex2(v.x), ex2(v.y));
-                                }
-                                ls = add2(ls, f2(p.x, p.y));
-                                w[c][e] = Half16<T>::pack(p.x, p.y);
+                        for (int e = 0; e < kHalf / 2; ++e) {
+                            const float s0 = sv[2 * e], s1 = sv[2 * e + 1];
+                            mx[e & 1] = fmaxf(mx[e & 1], fmaxf(s0, s1));
+                            const F2 arg = fma2(f2(s0, s1), sc2, ref2);
+                            float2 p;
+                            if ((e & 3) == 3) {
+                                p = ex2_pair(arg);
+                            } else {
+                                const float2 v = un2(arg);
+                                p = make_float2(ex2(v.x), ex2(v.y));
                             }
+                            ls = add2(ls, f2(p.x, p.y));
+                            w[e] = Half16<T>::pack(p.x, p.y);
                         }
-                        const bool grow = fmaxf(mx[0], mx[1]) * sc > m + kRescale;
-                        if (!__any_sync(0xffffffffu, grow)) {
-                            tmem_st32(tm_sx + 64, w[0]);
-                            tmem_st32(tm_sx + 96, w[1]);
-                            const float2 v = un2(ls);
-                            l += v.x + v.y;
-                            done = true;
-                        }
+                        done = !__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * sc > m + kRescale);
+                        const float2 v = un2(ls);
+                        lsum = v.x + v.y;
                     }
                     if (!done) {
-                        // the first tile, tiles with hidden keys, and tiles whose maximum moves m
-                        float sv[64];
-                        // scores of keys [64 c, 64 c + 64) of the tile
-                        auto load = [&](int c) {
-                            tmem_ld64(tm_sx + 64 * c, sv);
-                            if (!whole) {
-                                const int hi = pos - k0 - 64 * c, lo = a.window > 0 ? hi - a.window : -1;
-                                const int sink = a.sinks - k0 - 64 * c;
+                        // the first keys, hidden keys, and keys whose maximum moves m
+                        if (!whole) {
+                            const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sink = a.sinks - k0;
 #pragma unroll
-                                for (int i = 0; i < 64; ++i) sv[i] = i <= hi && (i > lo || i < sink) ? sv[i] : -INFINITY;
-                            }
-                        };
+                            for (int e = 0; e < kHalf; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
+                        }
                         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            load(c);
-#pragma unroll
-                            for (int i = 0; i < 64; i += 4) {
-                                mx[0] = fmaxf(mx[0], fmaxf(sv[i], sv[i + 1]));
-                                mx[1] = fmaxf(mx[1], fmaxf(sv[i + 2], sv[i + 3]));
-                            }
+                        for (int e = 0; e < kHalf; e += 4) {
+                            mx[0] = fmaxf(mx[0], fmaxf(sv[e], sv[e + 1]));
+                            mx[1] = fmaxf(mx[1], fmaxf(sv[e + 2], sv[e + 3]));
                         }
                         const float top = fmaxf(mx[0], mx[1]) * sc;
                         const bool grow = top > m + kRescale;
-                        if (j == part.j0) {
+                        if (i == 0) {
                             m = top;
                         } else if (__any_sync(0xffffffffu, grow)) {
                             // O must hold the products before it is rescaled
-                            tc_wait_bar(&bar.o[x], (n - 1) & 1u, ok);
+                            tc_wait_bar(&bar.o[x][h ^ 1], (h ? n : n - 1) & 1u, ok);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) return;
                             tc_fence_after();
                             const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < D / 32; ++c) {
                                 float o[32];
                                 tmem_ld32(tm_ox + 32 * c, o);
-                                uint32_t w[32];
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
                                 tmem_st32(tm_ox + 32 * c, w);
@@ -441,27 +450,30 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         }
                         const float ref = m == -INFINITY ? 0.0f : m;
                         float ls[2] = {0.0f, 0.0f};
-                        // the last keys first: the columns of P lie over their scores
 #pragma unroll
-                        for (int c = 1; c >= 0; --c) {
-                            if (c == 0) load(0);
-                            uint32_t w[32];
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
-                                ls[0] += p0;
-                                ls[1] += p1;
-                                w[e] = Half16<T>::pack(p0, p1);
-                            }
-                            tmem_st32(tm_sx + 64 + 32 * c, w);
+                        for (int e = 0; e < kHalf / 2; ++e) {
+                            const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
+                            ls[0] += p0;
+                            ls[1] += p1;
+                            w[e] = Half16<T>::pack(p0, p1);
                         }
-                        l += ls[0] + ls[1];
+                        lsum = ls[0] + ls[1];
                     }
+                    l += lsum;
+                    // at head_dim 64 P's columns are free once P V of two halves ago is done
+                    if (D == 64 && i >= 2) {
+                        tc_wait_bar(&bar.o[x][h], (n - 1) & 1u, ok);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) return;
+                        tc_fence_after();
+                    }
+                    tmem_st32(tm_prob(x, h) + lanes, w);
                     tmem_st_wait();
                     tc_fence_before();
-                    mbar_arrive(&bar.p[x]);
+                    mbar_arrive(&bar.p[x][h]);
+                    n += h;
                 }
-                tc_wait_bar(&bar.o[x], (n - 1) & 1u, ok);
+                tc_wait_bar(&bar.o[x][1], (n - 1) & 1u, ok);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return;
                 tc_fence_after();
