@@ -356,14 +356,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     uint4 w[LI];
 #pragma unroll
                     for (int i = 0; i < LI; ++i) {
-                        const int rr = 32 * quarter + i * RPI + lane / CH, qrow = it.row0 + 128 * x + rr;
-                        w[i] = make_uint4(0, 0, 0, 0);
-                        if (rr < rows_x) {
-                            const int t = a.by_g(qrow);
-                            w[i] = __ldg(reinterpret_cast<const uint4*>(
-                                static_cast<const uint16_t*>(a.q) + (long long)(seq.row0 + t) * a.ldq +
-                                (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
-                        }
+                        // past the item's rows its last one again: no branch around a load
+                        const int qrow = it.row0 + 128 * x + min(32 * quarter + i * RPI + lane / CH, rows_x - 1);
+                        const int t = a.by_g(qrow);
+                        w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                                    (long long)(seq.row0 + t) * a.ldq +
+                                                                    (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
                     }
 #pragma unroll
                     for (int i = 0; i < LI; ++i) st_shared(own_chunk(32 * quarter + i * RPI + lane / CH, ch), w[i]);
