@@ -29,13 +29,17 @@
 // registers of a launch the first four warps keep 88 a thread, the others
 // take 208.
 //
-// A row's reference maximum m moves only when a score passes it by 8 (in base
-// 2), so O is rescaled seldom, and a tile's probabilities are computed with
-// the m it finds, beside the search for the tile's maximum; only when some
-// row's maximum has moved are they computed again.  One pair in four takes
-// 2^x on the FMA pipe (nearest integer, then a polynomial of degree 4 on the
-// rest), since the 16 results a clock of the special function unit would take
-// as long as both products.
+// The probabilities of a half are computed with the m of the halves before,
+// with no search for their maximum: any m gives the same result, so long as
+// the probabilities fit their 16 bits, and a half whose sum stays below 2^13
+// does.  Where it does not (and for the first keys, and hidden ones) the
+// half is computed again with its own maximum, and O is rescaled if that has
+// passed m by more than 2^8.  One pair in eight takes 2^x on the FMA pipe
+// (nearest integer, then a polynomial of degree 4 on the rest): the special
+// function unit would otherwise be the longest path.  Both measured on 4096
+// tokens at 12288 positions (32/8 heads of 128, bf16): 561 us; 594 with the
+// maximum searched beside the probabilities; 580 without the polynomial, 594
+// with one pair in four (maximum searched: 578 without, 594 one in eight).
 #include <cmath>
 #include <cstdint>
 
@@ -59,6 +63,7 @@ namespace {
 constexpr int kM = kTcItemRows;  // query rows of an item
 constexpr int kN = kTcTileKeys;  // keys of a tile
 constexpr int kHalf = kN / 2;    // keys of a score buffer
+constexpr float kMostSum = 8192.0f;  // of a half's probabilities: each then fits fp16
 constexpr int kThreadsTc = 384;
 constexpr int kRowThreads = 256;
 constexpr uint32_t kBox = 16384;  // 128 rows of 64 values: a swizzled operand block
@@ -384,29 +389,27 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     float lsum = 0.0f;
                     bool done = false;
                     if (whole && i > 0) {
-                        // probabilities under the m of the halves before, and the maximum beside them
+                        // probabilities under the m of the halves before, unless their sum
+                        // says that a score has passed it by far
                         const float ref = m == -INFINITY ? 0.0f : m;
                         const F2 ref2 = f2(-ref, -ref);
-                        float mx[2] = {-INFINITY, -INFINITY};
-                        F2 ls = f2(0.0f, 0.0f);
+                        F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
                         for (int e = 0; e < kHalf / 2; ++e) {
-                            const float s0 = sv[2 * e], s1 = sv[2 * e + 1];
-                            mx[e & 1] = fmaxf(mx[e & 1], fmaxf(s0, s1));
-                            const F2 arg = fma2(f2(s0, s1), sc2, ref2);
+                            const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
                             float2 p;
-                            if ((e & 3) == 3) {
+                            if ((e & 7) == 7) {
                                 p = ex2_pair(arg);
                             } else {
                                 const float2 v = un2(arg);
                                 p = make_float2(ex2(v.x), ex2(v.y));
                             }
-                            ls = add2(ls, f2(p.x, p.y));
+                            ls[e & 1] = add2(ls[e & 1], f2(p.x, p.y));
                             w[e] = Half16<T>::pack(p.x, p.y);
                         }
-                        done = !__any_sync(0xffffffffu, fmaxf(mx[0], mx[1]) * sc > m + kRescale);
-                        const float2 v = un2(ls);
+                        const float2 v = un2(add2(ls[0], ls[1]));
                         lsum = v.x + v.y;
+                        done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
                     }
                     if (!done) {
                         // the first keys, hidden keys, and keys whose maximum moves m
