@@ -34,7 +34,7 @@ struct AttnArgs {
 
 // The tcgen05 kernel (paged_attention_tc.cu): its items and tiles; pages as paged_attention_tc_pages says.
 constexpr int kTcItemRows = 256;
-constexpr int kTcTileKeys = 128;
+constexpr int kTcTileKeys = 64;
 int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st);
 bool paged_attention_tc_pages(int page_size);
 
@@ -73,17 +73,26 @@ __device__ __forceinline__ int tile_key(const Item& it, int j) {
 
 // ------------------------------------------------------------- schedule
 // The work of a call is a line of units: for each sequence, each KV head,
-// each item of M query rows, one unit per tile of N keys (one where a row
-// sees nothing: its zeros have to be written).  CTA b takes the units [b c,
-// (b + 1) c), so every CTA reads the same number of tiles whatever the
-// lengths, and an item that crosses a border is split: its CTAs leave partial
-// results (two slots a CTA are enough: one for an item that began before it,
-// one for an item that goes on after it), and the last of them to arrive
-// joins them in CTA order.  Lengths are device data; each CTA finds its own
-// place by a scan over the sequences.
+// each item of M query rows, one unit per tile of N keys and kItemCost more
+// for its start and end.  CTA b takes the units from b c to (b + 1) c, so the
+// CTAs finish together whatever the lengths.  A border less than kLeast units
+// from an end of an item moves to that end; an item with a border still
+// inside is split: its CTAs leave partial results (two slots a CTA are
+// enough: one for an item that began before it, one for an item that goes on
+// after it), and the last of them to arrive joins them in CTA order.
+// Lengths are device data; each CTA finds its own place by a scan over the
+// sequences.
+//
+// In a split item border k c is inside when u0 + kLeast <= k c <= u1 -
+// kLeast; the CTAs from the first such k, less one, to the last such k share
+// it.  An item that is not split belongs to the CTA of the last border that
+// is not past its first kLeast units.
+constexpr int kItemCost = 3;
+constexpr int kLeast = kItemCost + 2;
+
 template <int M, int N>
 __device__ __forceinline__ int item_units(const AttnArgs& a, const PagedSeq& s, int row0) {
-    return row0 < s.n_new * a.G ? max(1, make_item<M, N>(a, s, 0, row0).tiles) : 0;
+    return row0 < s.n_new * a.G ? make_item<M, N>(a, s, 0, row0).tiles + kItemCost : 0;
 }
 
 // Units of one KV head of s, by a whole warp.
@@ -203,8 +212,7 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
     return place_s;
 }
 
-// Part [j0, j1) of an item's tiles; first and last: the CTAs that the item
-// begins and ends in.
+// Part [j0, j1) of an item's tiles; first and last: the CTAs that share it.
 struct Part {
     int s, j0, j1, first, last;
 };
@@ -212,8 +220,8 @@ struct Part {
 // f(sequence, item, part) for the parts of this CTA, by whole warps.
 template <int M, int N, typename F>
 __device__ __forceinline__ void walk(const AttnArgs& a, const Place& p, F f) {
-    int at = p.c * (int)blockIdx.x, before = p.before, per_head = p.per_head;
-    const int end = min(p.c, p.total - at) + at, me = blockIdx.x;
+    const int me = blockIdx.x, begin = p.c * me, end = min(p.c, p.total - begin) + begin;
+    int at = begin, before = p.before, per_head = p.per_head;
     PagedSeq seq = p.seq;
     for (int s = p.s;;) {
         if (per_head > 0) {
@@ -221,27 +229,32 @@ __device__ __forceinline__ void walk(const AttnArgs& a, const Place& p, F f) {
             int u0 = before + kvh * per_head, rem = at - u0;
             int row0 = find_item<M, N>(a, seq, rem);
             u0 += rem;
-            while (kvh < a.b.nkv && at < end) {
+            while (kvh < a.b.nkv) {
                 const Item it = make_item<M, N>(a, seq, kvh, row0);
-                const int units = max(1, it.tiles);
-                Part part;
-                part.s = s;
-                part.j0 = at - u0;
-                part.j1 = min(it.tiles, min(units, end - u0));
-                // an item that neither began before this CTA nor goes on after it is its own
-                part.first = u0 >= me * p.c ? me : u0 / p.c;
-                part.last = end - u0 >= units ? me : (u0 + units - 1) / p.c;
-                f(seq, it, part);
-                at = u0 += units;
+                const int u1 = u0 + it.tiles + kItemCost;
+                const bool more = begin > u0 && begin - u0 >= kLeast;  // it began in an earlier CTA
+                if (end <= u0 || (end < u1 && end - u0 < kLeast && end < p.total)) return;
+                if (!(begin > u0 && begin - u0 >= kLeast && u1 - begin < kLeast)) {
+                    const bool cut = end < u1 && u1 - end >= kLeast;  // it goes on in a later one
+                    Part part;
+                    part.s = s;
+                    part.j0 = more ? begin - u0 - kItemCost : 0;
+                    part.j1 = cut ? end - u0 - kItemCost : it.tiles;
+                    part.first = more ? (u0 + kLeast + p.c - 1) / p.c - 1 : me;
+                    part.last = cut ? (u1 - kLeast) / p.c : me;
+                    f(seq, it, part);
+                }
+                if (end < u1) return;
+                u0 = u1;
                 row0 += M;
                 if (row0 >= seq.n_new * a.G) {
                     row0 = 0;
                     ++kvh;
                 }
             }
-            before += per_head * a.b.nkv;
+            at = before += per_head * a.b.nkv;
         }
-        if (at >= end || ++s >= a.b.num_seqs) break;
+        if (at >= end || ++s >= a.b.num_seqs) return;
         seq = paged_seq(a.b, s, nullptr);
         per_head = head_units<M, N>(a, seq);
     }

@@ -3,8 +3,8 @@
 // formulas and the kernel for single tokens).
 //
 // An item is 256 query rows (new token, head of the group) of a KV head, two
-// tiles A and B of 128 rows, the M of the MMA; K and V arrive in tiles of 128
-// keys, worked off as two halves of 64.  Per half i and row tile X:
+// row tiles A and B of 128, the M of the MMA; K and V arrive in tiles of 64
+// keys.  Per tile i and row tile X:
 //   S_X = Q_X K_i^T        A and B operands from shared memory, S in TMEM
 //   P_X = 2^(S_X scale - m) one thread per row: S out of TMEM, P back into it
 //                          in 16 bits
@@ -12,13 +12,13 @@
 // A group of MMAs ends 550 cycles after its last operand is read, so the
 // products of a row tile must not wait for one another: each row tile has
 // two score buffers of 64 columns, and while its threads work on one, S of
-// the next half goes into the other and P V of the half before is under way.
+// the next tile goes into the other and P V of the one before is under way.
 // (Tiles of 128 keys with one buffer: 4300 cycles a pair of 128 x 128 tiles,
 // of which the products take 2048.  An MMA of 64 keys reads Q as often as one
-// of 128 and takes 49 cycles instead of 32; halves are still the better deal.)
-// At head_dim 128, O and S fill the 512 columns and P lies over the half of
-// its scores that has been read, so S of half i + 2 waits for P V of half i;
-// at 64 it has columns of its own.
+// of 128 and takes 49 cycles instead of 32; two buffers are still the better
+// deal.)  At head_dim 128, O and S fill the 512 columns and P lies over the
+// half of its scores that has been read, so S of tile i + 2 waits for P V of
+// tile i; at 64 it has columns of its own.
 //
 // Twelve warps: warp 0 loads K and V tiles page by page by TMA (a tensor map
 // of the pool [page][KV head][position][dim]; a page that no row sees, or that
@@ -29,11 +29,11 @@
 // registers of a launch the first four warps keep 88 a thread, the others
 // take 208.
 //
-// The probabilities of a half are computed with the m of the halves before,
+// The probabilities of a tile are computed with the m of the tiles before,
 // with no search for their maximum: any m gives the same result, so long as
-// the probabilities fit their 16 bits, and a half whose sum stays below 2^13
-// does.  Where it does not (and for the first keys, and hidden ones) the
-// half is computed again with its own maximum, and O is rescaled if that has
+// the probabilities fit their 16 bits, and a tile whose sum stays below 2^13
+// does.  Where it does not (and for the first keys, and hidden ones) the tile
+// is computed again with its own maximum, and O is rescaled if that has
 // passed m by more than 2^8.  One pair in eight takes 2^x on the FMA pipe
 // (nearest integer, then a polynomial of degree 4 on the rest): the special
 // function unit would otherwise be the longest path.  Both measured on 4096
@@ -52,31 +52,32 @@ namespace infernt {
 
 void* tensor_map_encoder();  // bgemm.cu
 
-// The pages whose 128-key tiles are whole boxes: a tile is 128 / page_size
+// The pages whose 64-key tiles are whole boxes: a tile is 64 / page_size
 // pages, or a page is a whole number of tiles.
 bool paged_attention_tc_pages(int page_size) {
-    return page_size % 128 == 0 || (page_size >= 8 && 128 % page_size == 0);
+    return page_size % kTcTileKeys == 0 || (page_size >= 8 && kTcTileKeys % page_size == 0);
 }
 
 namespace {
 
 constexpr int kM = kTcItemRows;  // query rows of an item
 constexpr int kN = kTcTileKeys;  // keys of a tile
-constexpr int kHalf = kN / 2;    // keys of a score buffer
-constexpr float kMostSum = 8192.0f;  // of a half's probabilities: each then fits fp16
+constexpr float kMostSum = 8192.0f;  // of a tile's probabilities: each then fits fp16
 constexpr int kThreadsTc = 384;
 constexpr int kRowThreads = 256;
-constexpr uint32_t kBox = 16384;  // 128 rows of 64 values: a swizzled operand block
+constexpr uint32_t kBoxQ = 16384;  // 128 rows of 64 values: a swizzled operand block
+constexpr uint32_t kBox = 8192;    // 64 rows
 
 // Shared memory: Q of both row tiles, then the stages of K and of V tiles,
 // each of D / 64 blocks.
 template <int D>
 struct LayoutTc {
     static constexpr uint32_t kBlocks = D / 64;
+    static constexpr uint32_t kTileQ = kBlocks * kBoxQ;
     static constexpr uint32_t kTile = kBlocks * kBox;
-    static constexpr int kStages = D == 64 ? 4 : 2;
+    static constexpr int kStages = 4;
     static constexpr uint32_t kQ = 0;
-    static constexpr uint32_t kK = 2 * kTile;
+    static constexpr uint32_t kK = 2 * kTileQ;
     static constexpr uint32_t kV = kK + kStages * kTile;
     static constexpr uint32_t kBytes = kV + kStages * kTile + 1024;
 };
@@ -84,7 +85,7 @@ struct LayoutTc {
 struct Barriers {
     uint64_t full_k[4], empty_k[4], full_v[4], clean_v[4], empty_v[4];
     uint64_t q[2];
-    uint64_t s[2][2], p[2][2], o[2][2];  // [row tile][half]
+    uint64_t s[2][2], p[2][2], o[2][2];  // [row tile][score buffer]
 };
 
 // Pairs of FP32 values, each lane rounded as the scalar operation.
@@ -172,10 +173,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(&bar.q[x], 128);
-            for (int h = 0; h < 2; ++h) {
-                mbar_init(&bar.s[x][h], 1);
-                mbar_init(&bar.p[x][h], 128);
-                mbar_init(&bar.o[x][h], 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bar.s[x][b], 1);
+                mbar_init(&bar.p[x][b], 128);
+                mbar_init(&bar.o[x][b], 1);
             }
         }
         mbar_fence_init();
@@ -187,8 +188,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     __syncthreads();
     // TMEM columns: S of A at 0 and 64, of B at 128 and 192; O of A at 256, of B D further; P
     const uint32_t tmem = tmem_s;
-    auto tm_score = [&](int x, int h) { return tmem + 128u * x + 64u * h; };
-    auto tm_prob = [&](int x, int h) { return D == 128 ? tm_score(x, h) + 32u : tmem + 384u + 64u * x + 32u * h; };
+    auto tm_score = [&](int x, int b) { return tmem + 128u * x + 64u * b; };
+    auto tm_prob = [&](int x, int b) { return D == 128 ? tm_score(x, b) + 32u : tmem + 384u + 64u * x + 32u * b; };
     auto tm_out = [&](int x) { return tmem + 256u + (uint32_t)D * x; };
     bool ok = true;
     if (warp < 4) {
@@ -243,22 +244,22 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             // other's probabilities.
             const int x = warp >> 1;
             uint32_t n = 0, nx = 0, parts = 0;
-            const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kHalf), id_o = tc_instr(Half16<T>::kBf16, true, D);
-            const uint64_t qd = tc_desc_k(base + L::kQ + x * L::kTile);
+            const uint32_t id_s = tc_instr(Half16<T>::kBf16, false, kN), id_o = tc_instr(Half16<T>::kBf16, true, D);
+            const uint64_t qd = tc_desc_k(base + L::kQ + x * L::kTileQ);
             const bool leader = tc_elect();
-            // S of half h of key tile m
-            auto scores = [&](uint32_t m, int h) {
+            // S of key tile m into buffer b
+            auto scores = [&](uint32_t m, uint32_t b) {
                 const uint32_t st = m % ST;
-                const uint64_t k = tc_desc_k(base + L::kK + st * L::kTile + h * (kBox / 2));
+                const uint64_t k = tc_desc_k(base + L::kK + st * L::kTile);
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t kk = 0; kk < D / 16; ++kk) {
                     // 32 bytes a step within a block of 64 columns
-                    const uint32_t at = (kk >> 2) * (kBox >> 4) + 2 * (kk & 3);
-                    tc_mma_ss(tm_score(x, h), qd + at, k + at, id_s, kk);
+                    const uint32_t c = kk >> 2, r = 2 * (kk & 3);
+                    tc_mma_ss(tm_score(x, b), qd + c * (kBoxQ >> 4) + r, k + c * (kBox >> 4) + r, id_s, kk);
                 }
-                tc_commit_to(&bar.s[x][h]);
-                if (h) tc_commit_to(&bar.empty_k[st]);
+                tc_commit_to(&bar.s[x][b]);
+                tc_commit_to(&bar.empty_k[st]);
             };
             walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
                 const int tiles = part.j1 - part.j0;
@@ -275,39 +276,34 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         }
                     } else {
                         tc_wait_bar(&bar.q[x], parts++ & 1u, ok);
-                        // round i: P V of half i - 2, then S of half i over its columns
+                        // round i: P V of tile i - 2, then S of tile i over its columns
 #pragma unroll 1
-                        for (int i = 0; i < 2 * tiles + 2 && ok; ++i) {
-                            const int h = i & 1;
+                        for (int i = 0; i < tiles + 2 && ok; ++i) {
+                            const uint32_t b = (nx + i) & 1u, turn = ((nx + i - 2) >> 1) & 1u, m = n + i - 2;
                             if (i >= 2) {
-                                const uint32_t m = n - 1, st = m % ST, turn = (m / ST) & 1u;
-                                const uint64_t v =
-                                    tc_desc_mn(base + L::kV + st * L::kTile + h * (kBox / 2), kBox);
-                                tc_wait_bar(&bar.full_v[st], turn, ok);
-                                tc_wait_bar(&bar.clean_v[st], turn, ok);
-                                tc_wait_bar(&bar.p[x][h], (nx - 1) & 1u, ok);
+                                const uint32_t st = m % ST;
+                                const uint64_t v = tc_desc_mn(base + L::kV + st * L::kTile, kBox);
+                                tc_wait_bar(&bar.full_v[st], (m / ST) & 1u, ok);
+                                tc_wait_bar(&bar.clean_v[st], (m / ST) & 1u, ok);
+                                tc_wait_bar(&bar.p[x][b], turn, ok);
                                 if (!ok) break;
                                 tc_fence_after();
 #pragma unroll
-                                for (uint32_t kk = 0; kk < kHalf / 16; ++kk)
-                                    tc_mma_ts(tm_out(x), tm_prob(x, h) + 8u * kk, v + kk * (2048u >> 4), id_o,
+                                for (uint32_t kk = 0; kk < kN / 16; ++kk)
+                                    tc_mma_ts(tm_out(x), tm_prob(x, b) + 8u * kk, v + kk * (2048u >> 4), id_o,
                                               (uint32_t)(i - 2) | kk);
-                                tc_commit_to(&bar.o[x][h]);
-                                if (h) tc_commit_to(&bar.empty_v[st]);
+                                tc_commit_to(&bar.o[x][b]);
+                                tc_commit_to(&bar.empty_v[st]);
                             }
-                            if (i < 2 * tiles) {
-                                if (h == 0) tc_wait_bar(&bar.full_k[n % ST], (n / ST) & 1u, ok);
-                                if (D == 128 && i >= 2) tc_wait_bar(&bar.o[x][h], (nx - 1) & 1u, ok);
+                            if (i < tiles) {
+                                tc_wait_bar(&bar.full_k[(n + i) % ST], ((n + i) / ST) & 1u, ok);
+                                if (D == 128 && i >= 2) tc_wait_bar(&bar.o[x][b], turn, ok);
                                 if (!ok) break;
-                                scores(n, h);
-                            }
-                            if (h) {
-                                ++n;
-                                ++nx;
+                                scores(n + i, b);
                             }
                         }
-                        --n;  // the last round only finishes
-                        --nx;
+                        n += tiles;
+                        nx += tiles;
                     }
                 }
                 __syncwarp();
@@ -340,7 +336,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         const int ch = lane % CH;
         // 16-byte chunk c of row rr of the row tile's Q (and, at the end, its result)
         auto own_chunk = [&](int rr, int c) {
-            return base + L::kQ + x * L::kTile + (c >> 3) * kBox + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+            return base + L::kQ + x * L::kTileQ + (c >> 3) * kBoxQ + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
         };
         auto st_shared = [](uint32_t at, uint4 w) {
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
@@ -374,18 +370,19 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     mbar_arrive(&bar.q[x]);
                 }
 #pragma unroll 1
-                for (int i = 0; i < 2 * (part.j1 - part.j0); ++i) {
-                    const int h = i & 1, k0 = tile_key<kN>(it, part.j0 + (i >> 1)) + h * kHalf;
-                    tc_wait_bar(&bar.s[x][h], n & 1u, ok);
+                for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
+                    const int k0 = tile_key<kN>(it, part.j0 + i);
+                    const uint32_t b = n & 1u;
+                    tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return;
                     tc_fence_after();
-                    float sv[kHalf];
-                    tmem_ld64(tm_score(x, h) + lanes, sv);
+                    float sv[kN];
+                    tmem_ld64(tm_score(x, b) + lanes, sv);
                     // keys that every row of the item sees need no mask
-                    const bool whole = k0 + kHalf - 1 <= it.pos_first &&
-                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kHalf <= a.sinks);
-                    uint32_t w[kHalf / 2];
+                    const bool whole = k0 + kN - 1 <= it.pos_first &&
+                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
+                    uint32_t w[kN / 2];
                     float lsum = 0.0f;
                     bool done = false;
                     if (whole && i > 0) {
@@ -395,7 +392,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         const F2 ref2 = f2(-ref, -ref);
                         F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
-                        for (int e = 0; e < kHalf / 2; ++e) {
+                        for (int e = 0; e < kN / 2; ++e) {
                             const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
                             float2 p;
                             if ((e & 7) == 7) {
@@ -414,13 +411,19 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     if (!done) {
                         // the first keys, hidden keys, and keys whose maximum moves m
                         if (!whole) {
-                            const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sink = a.sinks - k0;
+                            const int hi = pos - k0;
+                            if (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks) {
 #pragma unroll
-                            for (int e = 0; e < kHalf; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
+                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
+                            } else {
+                                const int lo = hi - a.window, sink = a.sinks - k0;
+#pragma unroll
+                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
+                            }
                         }
                         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                        for (int e = 0; e < kHalf; e += 4) {
+                        for (int e = 0; e < kN; e += 4) {
                             mx[0] = fmaxf(mx[0], fmaxf(sv[e], sv[e + 1]));
                             mx[1] = fmaxf(mx[1], fmaxf(sv[e + 2], sv[e + 3]));
                         }
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             m = top;
                         } else if (__any_sync(0xffffffffu, grow)) {
                             // O must hold the products before it is rescaled
-                            tc_wait_bar(&bar.o[x][h ^ 1], (h ? n : n - 1) & 1u, ok);
+                            tc_wait_bar(&bar.o[x][b ^ 1], ((n - 1) >> 1) & 1u, ok);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) return;
                             tc_fence_after();
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         const float ref = m == -INFINITY ? 0.0f : m;
                         float ls[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int e = 0; e < kHalf / 2; ++e) {
+                        for (int e = 0; e < kN / 2; ++e) {
                             const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
                             ls[0] += p0;
                             ls[1] += p1;
@@ -463,18 +466,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     l += lsum;
                     // at head_dim 64 P's columns are free once P V of two halves ago is done
                     if (D == 64 && i >= 2) {
-                        tc_wait_bar(&bar.o[x][h], (n - 1) & 1u, ok);
+                        tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) return;
                         tc_fence_after();
                     }
-                    tmem_st32(tm_prob(x, h) + lanes, w);
+                    tmem_st32(tm_prob(x, b) + lanes, w);
                     tmem_st_wait();
                     tc_fence_before();
-                    mbar_arrive(&bar.p[x][h]);
-                    n += h;
+                    mbar_arrive(&bar.p[x][b]);
                 }
-                tc_wait_bar(&bar.o[x][1], (n - 1) & 1u, ok);
+                tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) return;
                 tc_fence_after();
@@ -643,7 +645,7 @@ int launch_tc(const AttnArgs& args, cudaStream_t st) {
     int ctas = sm_count();
     if (ctas > most) ctas = most;
     if (ctas > kMaxCtas) ctas = kMaxCtas;
-    a.min_tiles = 2;
+    a.min_tiles = 8;
     paged_attn_tc<T, D><<<ctas, kThreadsTc, L::kBytes, st>>>(a, mk, mv);
     INFERNT_CUDA_TRY(cudaGetLastError());
     return INFERNT_OK;
