@@ -15,17 +15,28 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "paged_attention.cuh"
+#include "tc_mma.cuh"
 #include "warp_mma.cuh"
 
 namespace infernt {
 namespace {
 
+// This file's kernel takes query rows by the dozen: single tokens, drafts of
+// a few, and any chunk whose pages do not make whole boxes.  It is bound by
+// the bytes of K and V.  A CTA is a producer warp, which streams the CTA's
+// tiles of 64 keys through a ring of shared memory without a pause between
+// items, and four warps that consume them on mma.sync; two CTAs share an SM
+// and keep 128 KB in flight there.  (Without the producer, each item's start
+// waited for its own first tiles and each tile for a barrier of the CTA:
+// 64 sequences of 512 to 2048 positions, 32/4 heads of 64, took 38 us.)
 constexpr int kTileKeys = 64;   // keys of a K / V tile
 constexpr int kItemRows = 64;   // query rows of an item: four warps of 16
-constexpr int kThreads = 128;
-constexpr int kStages = 3;
+constexpr int kConsumers = 128;
+constexpr int kThreads = kConsumers + 32;
+constexpr uint32_t kBlock = kTileKeys * 128;  // a block of 64 columns: rows of 128 bytes
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -43,100 +54,173 @@ __device__ __forceinline__ void mma_16816<__half>(float (&c)[4], const uint32_t 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Shared memory: the ring of K / V tiles (reused for the merge of the warps'
-// results), the pool rows of two tiles, and a flag per query row.
+// Shared memory: the ring (per stage the blocks of K, then those of V; the
+// 16-byte chunk c of row r lies at c ^ (r & 7), as a tensor map with 128-byte
+// swizzle writes it), then the scratch in which the warps' results meet: up
+// to three sets of 8 rows.
 template <int D>
 struct Layout {
-    static constexpr int kRowBytes = D * 2;
-    static constexpr int kTileBytes = kTileKeys * kRowBytes;
-    static constexpr int kRing = kStages * 2 * kTileBytes;
-    static constexpr int kBytes = kRing + 2 * kTileKeys * 4 + kItemRows;
+    static constexpr int kBlocks = D / 64;
+    static constexpr int kStages = D == 64 ? 6 : 3;
+    static constexpr uint32_t kTile = kBlocks * kBlock;
+    static constexpr uint32_t kScratch = kStages * 2 * kTile;
+    static constexpr uint32_t kBytes = kScratch + 3 * 8 * (D + 2) * 4 + 1024;
+};
+
+template <int ST>
+struct Ring {
+    uint64_t full[ST], empty[ST];
+};
+
+// Address of 16-byte chunk ch of a tile's row.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t tile, int row, int ch) {
+    return tile + (uint32_t)(ch >> 3) * kBlock + (uint32_t)(row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+}
+
+// The producer warp: K and V tiles of the CTA's parts, in order.  BOXES: page
+// by page through the tensor maps (a page that no row sees, or that the pool
+// does not have, becomes zeros); otherwise row by row, hidden rows as zeros.
+template <int D, bool BOXES>
+__device__ __forceinline__ void produce(const AttnArgs& a, const Place& place, const CUtensorMap& tm_k,
+                                        const CUtensorMap& tm_v, uint32_t base, Ring<Layout<D>::kStages>& ring,
+                                        bool& ok) {
+    using L = Layout<D>;
+    constexpr int ST = L::kStages;
+    const int lane = threadIdx.x & 31;
+    const int ps = a.b.page_size, per_tile = ps < kTileKeys ? kTileKeys / ps : 1;
+    const int box_rows = ps < kTileKeys ? ps : kTileKeys;
+    uint32_t st = 0, turn = 1;  // the first round's stages are free
+    walk<kItemRows, kTileKeys>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+#pragma unroll 1
+        for (int j = part.j0; j < part.j1; ++j) {
+            const int k0 = tile_key<kTileKeys>(it, j);
+            const uint32_t kt = base + st * 2 * L::kTile, vt = kt + L::kTile;
+            if (BOXES) {
+                int page = a.b.num_pages, row = 0;
+                if (lane < per_tile) {
+                    const int p0 = k0 + lane * box_rows, pi = a.b.by_page(p0);
+                    row = p0 - pi * ps;
+                    if (p0 < it.hi && (p0 + box_rows > it.lo || p0 < it.sink_end)) {
+                        page = a.b.table[(size_t)part.s * a.b.table_stride + pi];
+                        if (page < 0 || page >= a.b.num_pages) {
+                            if (a.err) atomicOr(a.err, kErrPage);
+                            page = a.b.num_pages;
+                        }
+                    }
+                }
+                tc_wait_bar(&ring.empty[st], turn, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                if (lane == 0) mbar_arrive_expect_tx(&ring.full[st], 2 * L::kTile);
+                __syncwarp();
+                if (lane < per_tile)
+#pragma unroll
+                    for (int b = 0; b < L::kBlocks; ++b) {
+                        tma_load_4d(kt + b * kBlock + lane * box_rows * 128, &tm_k, 64 * b, row, it.kvh, page,
+                                    &ring.full[st]);
+                        tma_load_4d(vt + b * kBlock + lane * box_rows * 128, &tm_v, 64 * b, row, it.kvh, page,
+                                    &ring.full[st]);
+                    }
+            } else {
+                // rows `lane` and `lane + 32` of the tile; -1: zeros
+                int rows[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int p = k0 + lane + 32 * h;
+                    rows[h] = item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
+                }
+                tc_wait_bar(&ring.empty[st], turn, ok);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                constexpr int CH = D / 8, RPI = 32 / CH;  // chunks of a row, rows at once
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll 4
+                    for (int i = 0; i < 32 / RPI; ++i) {
+                        const int r = i * RPI + lane / CH, ch = lane % CH;
+                        const int pr = __shfl_sync(0xffffffffu, rows[h], r);
+                        const size_t off = (size_t)(pr < 0 ? 0 : pr) * (D * 2) + ch * 16;
+                        const uint32_t at = chunk_at(0, r + 32 * h, ch);
+                        cp_async16(kt + at, static_cast<const char*>(a.k) + off, pr < 0 ? 0u : 16u);
+                        cp_async16(vt + at, static_cast<const char*>(a.v) + off, pr < 0 ? 0u : 16u);
+                    }
+                // this lane's arrival, once its copies have landed
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_addr(&ring.full[st]))
+                             : "memory");
+            }
+            if (++st == ST) {
+                st = 0;
+                turn ^= 1;
+            }
+        }
+    });
+    if (!BOXES) cp_async_wait<0>();
+}
+
+// What a warp knows of its 16 rows after a part: lane (g, tig) has rows g and
+// g + 8, of each the columns 8 b + 2 tig and + 1.
+template <int D>
+struct RowState {
+    float m[2], l[2];
+    float acc[D / 8][4];
 };
 
 // The tiles [j0, j1) of an item by four warps: RB blocks of 16 rows, each by
-// 4 / RB warps that share a tile's keys between them.  Leaves every warp's
-// (m, l, out) of its rows in shared memory: slot (key share, row) of
-// `m_s`, `l_s` and `o_s`.
-template <typename T, int D, int RB>
-__device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq, int s, const Item& it, int j0,
-                                          int j1, unsigned char* smem) {
+// 4 / RB warps that share a tile's keys between them.  The result is in the
+// warps of the first key share (warp < RB).
+template <typename T, int D, int RB, bool BOXES>
+__device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq& seq, const Item& it, const Part& part,
+                                               uint32_t base, float* scratch, Ring<Layout<D>::kStages>& ring,
+                                               uint32_t& st, uint32_t& turn, bool& ok) {
     using L = Layout<D>;
-    constexpr int KS = 4 / RB, WK = kTileKeys / KS, NT = WK / 8;  // key shares, keys and n-tiles per warp
-    constexpr int CH = L::kRowBytes / 16, KC = D / 16, DB = D / 8;
-    constexpr int ROWS_PER_PASS = kThreads / CH, PASSES = kTileKeys / ROWS_PER_PASS;
-    int* rows_s = reinterpret_cast<int*>(smem + L::kRing);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
+    constexpr int KS = 4 / RB, WK = kTileKeys / KS, NT = WK / 8;  // key shares, keys and n-tiles of a warp
+    constexpr int KC = D / 16, DB = D / 8, ST = L::kStages;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
     const int rb = warp % RB, ks = warp / RB;
-    const uint32_t ring = smem_addr(smem);
-    const unsigned char* kb = static_cast<const unsigned char*>(a.k);
-    const unsigned char* vb = static_cast<const unsigned char*>(a.v);
-
-    // pool row of key `tid` of tile j; -1 where no row of the item sees it
-    auto row_of = [&](int j) {
-        if (tid >= kTileKeys || j >= j1) return -1;
-        const int p = tile_key<kTileKeys>(it, j) + tid;
-        return item_sees(it, p) ? pool_row(a.b, s, it.kvh, p, a.err) : -1;
-    };
-    // tile j into stage (j - j0) % kStages; rows that nobody sees become zeros
-    auto issue = [&](int j) {
-        if (j < j1) {
-            const uint32_t st = ring + (uint32_t)((j - j0) % kStages) * 2 * L::kTileBytes;
-            const int* rows = rows_s + (j & 1) * kTileKeys;
-#pragma unroll
-            for (int e = 0; e < PASSES; ++e) {
-                const int row = e * ROWS_PER_PASS + tid / CH, ch = tid % CH;
-                const int pr = rows[row];
-                const size_t off = (size_t)(pr < 0 ? 0 : pr) * L::kRowBytes + ch * 16;
-                const uint32_t dst = st + (uint32_t)(row * L::kRowBytes + ((ch ^ (row & 7)) << 4));
-                cp_async16(dst, kb + off, pr < 0 ? 0u : 16u);
-                cp_async16(dst + L::kTileBytes, vb + off, pr < 0 ? 0u : 16u);
-            }
-        }
-        cp_async_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        if (tid < kTileKeys) rows_s[((j0 + i) & 1) * kTileKeys + tid] = row_of(j0 + i);
-        __syncthreads();
-        issue(j0 + i);
-    }
-    if (tid < kTileKeys) {
-        const int r = row_of(j0 + kStages - 1);
-        rows_s[((j0 + kStages - 1) & 1) * kTileKeys + tid] = r;  // its slot was read two issues ago
-    }
-
     // query fragments of rows g and g + 8 of the warp's block
     uint32_t qa[KC][4];
     int pos[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int r = rb * 16 + g + 8 * h, row = it.row0 + r, token = a.by_g(row);
-        const bool ok = r < it.rows;
-        pos[h] = ok ? row_pos(seq, token) : -1;
-        const uint32_t* q = reinterpret_cast<const uint32_t*>(
-            static_cast<const uint16_t*>(a.q) + (ok ? (long long)(seq.row0 + token) * a.ldq +
-                                                          (long long)(it.kvh * a.G + row - token * a.G) * D + 2 * tig
-                                                    : 0));
+        const int r = rb * 16 + g + 8 * h, row = it.row0 + min(r, it.rows - 1), token = a.by_g(row);
+        pos[h] = r < it.rows ? row_pos(seq, token) : -1;
+        const uint32_t* q = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(a.q) +
+                                                              (long long)(seq.row0 + token) * a.ldq +
+                                                              (it.kvh * a.G + row - token * a.G) * D + 2 * tig);
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
-            qa[k][h] = ok ? q[8 * k] : 0u;
-            qa[k][h + 2] = ok ? q[8 * k + 4] : 0u;
+            qa[k][h] = __ldg(q + 8 * k);
+            qa[k][h + 2] = __ldg(q + 8 * k + 4);
         }
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    float acc[DB][4];
+    RowState<D> s;
 #pragma unroll
-    for (int b = 0; b < DB; ++b) acc[b][0] = acc[b][1] = acc[b][2] = acc[b][3] = 0.0f;
+    for (int h = 0; h < 2; ++h) {
+        s.m[h] = -INFINITY;
+        s.l[h] = 0.0f;
+    }
+#pragma unroll
+    for (int b = 0; b < DB; ++b) s.acc[b][0] = s.acc[b][1] = s.acc[b][2] = s.acc[b][3] = 0.0f;
     const bool busy = rb * 16 < it.rows;
 
-    for (int j = j0; j < j1; ++j) {
-        cp_async_wait<kStages - 2>();  // this thread's copies of tile j have landed
-        __syncthreads();               // everyone's, the rows of tile j + 2 too; tile j - 1's stage is free
-        issue(j + kStages - 1);
-        const int next = row_of(j + kStages);
+#pragma unroll 1
+    for (int j = part.j0; j < part.j1; ++j) {
+        const int k0 = tile_key<kTileKeys>(it, j);
+        const uint32_t kt = base + st * 2 * L::kTile, vt = kt + L::kTile;
+        tc_wait_bar(&ring.full[st], turn, ok);
         if (busy) {
-            const int k0 = tile_key<kTileKeys>(it, j);
-            const uint32_t kt = ring + (uint32_t)((j - j0) % kStages) * 2 * L::kTileBytes, vt = kt + L::kTileBytes;
+            if (BOXES && (k0 + kTileKeys > it.hi || (k0 < it.lo && k0 + kTileKeys > it.sink_end))) {
+                // V rows of this warp's keys that no row of the item sees may
+                // hold anything, and 0 times infinity is not 0
+                for (int r = ks * WK + lane; r < (ks + 1) * WK; r += 32)
+                    if (!item_sees(it, k0 + r))
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at(vt, r, c)), "r"(0)
+                                         : "memory");
+                fence_proxy_async_smem();  // before the stage is loaded again
+                __syncwarp();
+            }
             float sc[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
@@ -144,54 +228,56 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
             for (int k = 0; k < KC; ++k)
 #pragma unroll
                 for (int n = 0; n < NT / 2; ++n) {
-                    const int x = lane >> 3, row = ks * WK + 8 * (2 * n + (x >> 1)) + (lane & 7), ch = 2 * k + (x & 1);
+                    const int x = lane >> 3, row = ks * WK + 8 * (2 * n + (x >> 1)) + (lane & 7);
                     uint32_t b0, b1, b2, b3;
-                    ldsm_x4(kt + (uint32_t)(row * L::kRowBytes + ((ch ^ (row & 7)) << 4)), b0, b1, b2, b3);
+                    ldsm_x4(chunk_at(kt, row, 2 * k + (x & 1)), b0, b1, b2, b3);
                     mma_16816<T>(sc[2 * n], qa[k], b0, b1);
                     mma_16816<T>(sc[2 * n + 1], qa[k], b2, b3);
                 }
             // a tile that every row sees whole needs no mask
-            const bool whole = k0 + kTileKeys - 1 <= it.pos_first &&
-                               (a.window == 0 || k0 > it.pos_last - a.window || k0 + kTileKeys <= a.sinks);
+            if (!(k0 + kTileKeys - 1 <= it.pos_first &&
+                  (a.window == 0 || k0 > it.pos_last - a.window || k0 + kTileKeys <= a.sinks))) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int p = k0 + ks * WK + 8 * n + 2 * tig + (e & 1), ph = pos[e >> 1];
+                        if (!(p <= ph && (a.window == 0 || p > ph - a.window || p < a.sinks))) sc[n][e] = -INFINITY;
+                    }
+            }
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int h = e >> 1, p = k0 + ks * WK + 8 * n + 2 * tig + (e & 1);
-                    const bool sees = whole || (p <= pos[h] && (a.window == 0 || p > pos[h] - a.window || p < a.sinks));
-                    sc[n][e] = sees ? sc[n][e] * a.scale_log2 : -INFINITY;
-                    mx[h] = fmaxf(mx[h], sc[n][e]);
-                }
+                for (int e = 0; e < 4; ++e) mx[e >> 1] = fmaxf(mx[e >> 1], sc[n][e]);
             bool grow = false;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                grow |= mx[h] > m[h] + kRescale;
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * a.scale_log2;
+                grow |= mx[h] > s.m[h] + kRescale;
             }
             // the reference maximum moves only when probabilities would pass 2^8
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float n = fmaxf(m[h], mx[h]);
-                    const float f = m[h] == -INFINITY ? 0.0f : ex2(m[h] - n);
-                    m[h] = n;
-                    l[h] *= f;
+                    const float n = fmaxf(s.m[h], mx[h]), f = s.m[h] == -INFINITY ? 0.0f : ex2(s.m[h] - n);
+                    s.m[h] = n;
+                    s.l[h] *= f;
 #pragma unroll
                     for (int b = 0; b < DB; ++b) {
-                        acc[b][2 * h] *= f;
-                        acc[b][2 * h + 1] *= f;
+                        s.acc[b][2 * h] *= f;
+                        s.acc[b][2 * h + 1] *= f;
                     }
                 }
             }
-            const float ref[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+            const float ref[2] = {s.m[0] == -INFINITY ? 0.0f : s.m[0], s.m[1] == -INFINITY ? 0.0f : s.m[1]};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sc[n][e] = ex2(sc[n][e] - ref[e >> 1]);
-                    l[e >> 1] += sc[n][e];
+                    sc[n][e] = ex2(fmaf(sc[n][e], a.scale_log2, -ref[e >> 1]));
+                    s.l[e >> 1] += sc[n][e];
                 }
             // the score fragments of two n-tiles are the A fragment of 16 probabilities
 #pragma unroll
@@ -202,71 +288,76 @@ __device__ __forceinline__ void run_tiles(const AttnArgs& a, const PagedSeq& seq
                                         Half16<T>::pack(sc[2 * kk + 1][2], sc[2 * kk + 1][3])};
 #pragma unroll
                 for (int b = 0; b < DB / 2; ++b) {
-                    const int x = lane >> 3, row = ks * WK + 16 * kk + 8 * (x & 1) + (lane & 7), ch = 2 * b + (x >> 1);
+                    const int x = lane >> 3, row = ks * WK + 16 * kk + 8 * (x & 1) + (lane & 7);
                     uint32_t v0, v1, v2, v3;
-                    ldsm_x4_trans(vt + (uint32_t)(row * L::kRowBytes + ((ch ^ (row & 7)) << 4)), v0, v1, v2, v3);
-                    mma_16816<T>(acc[2 * b], pa, v0, v1);
-                    mma_16816<T>(acc[2 * b + 1], pa, v2, v3);
+                    ldsm_x4_trans(chunk_at(vt, row, 2 * b + (x >> 1)), v0, v1, v2, v3);
+                    mma_16816<T>(s.acc[2 * b], pa, v0, v1);
+                    mma_16816<T>(s.acc[2 * b + 1], pa, v2, v3);
                 }
             }
         }
-        if (tid < kTileKeys) rows_s[((j + kStages) & 1) * kTileKeys + tid] = next;
-    }
-    cp_async_wait<0>();
-    __syncthreads();  // the ring is free
-    float* o_s = reinterpret_cast<float*>(smem);           // [KS][RB 16][D]
-    float* m_s = o_s + 4 * 16 * D;                          // [KS][RB 16]
-    float* l_s = m_s + 64;
-    if (busy) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            const int slot = (ks * RB + rb) * 16 + g + 8 * h;
-            if (tig == 0) {
-                m_s[slot] = m[h];
-                l_s[slot] = l[h];
-            }
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-                *reinterpret_cast<float2*>(o_s + slot * D + 8 * b + 2 * tig) =
-                    make_float2(acc[b][2 * h], acc[b][2 * h + 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ring.empty[st]);
+        if (++st == ST) {
+            st = 0;
+            turn ^= 1;
         }
     }
-    __syncthreads();
-}
-
-// `shares` sets of (m, l, out) in shared memory.
-template <int D>
-__device__ __forceinline__ Joined join_shares(const float* o_s, int shares, int r, int d) {
-    const float* m_s = o_s + 64 * D;
-    const float* l_s = m_s + 64;
-    const int stride = 64 / shares;  // rows of one share
-    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
-    for (int k = 0; k < shares; ++k) v.m = fmaxf(v.m, m_s[k * stride + r]);
-    for (int k = 0; k < shares; ++k) {
-        const float mk = m_s[k * stride + r], f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
-        const float2 o = *reinterpret_cast<const float2*>(o_s + (k * stride + r) * D + d);
-        v.l = fmaf(l_s[k * stride + r], f, v.l);
-        v.x = fmaf(o.x, f, v.x);
-        v.y = fmaf(o.y, f, v.y);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 1);
+        s.l[h] += __shfl_xor_sync(0xffffffffu, s.l[h], 2);
     }
-    return v;
-}
-
-template <int M, int D>
-__device__ __forceinline__ Joined join_slots(const AttnArgs& a, int first, int last, int r, int d) {
-    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
-    for (int b = first; b <= last; ++b) v.m = fmaxf(v.m, __ldcg(slot_of<M, D>(a, b, first) + M * D + r));
-    for (int b = first; b <= last; ++b) {
-        const float* p = slot_of<M, D>(a, b, first);
-        const float mk = __ldcg(p + M * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
-        const float2 o = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
-        v.l = fmaf(__ldcg(p + M * D + M + r), f, v.l);
-        v.x = fmaf(o.x, f, v.x);
-        v.y = fmaf(o.y, f, v.y);
+    // the key shares of a block of rows, joined in order by its first warp
+    if (KS > 1) {
+        float* m_s = scratch + 3 * 8 * D;
+        float* l_s = m_s + 3 * 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (8 * h >= it.rows) break;
+            const int set = (ks - 1) * RB + rb;
+            if (h) named_sync(1, kConsumers);  // the first rows have been read
+            if (ks > 0) {
+                if (tig == 0) {
+                    m_s[set * 8 + g] = s.m[h];
+                    l_s[set * 8 + g] = s.l[h];
+                }
+#pragma unroll
+                for (int b = 0; b < DB; ++b)
+                    *reinterpret_cast<float2*>(scratch + (set * 8 + g) * D + 8 * b + 2 * tig) =
+                        make_float2(s.acc[b][2 * h], s.acc[b][2 * h + 1]);
+            }
+            named_sync(1, kConsumers);
+            if (ks == 0) {
+                float M = s.m[h], f[KS];
+#pragma unroll
+                for (int k = 1; k < KS; ++k) M = fmaxf(M, m_s[((k - 1) * RB + rb) * 8 + g]);
+                f[0] = s.m[h] == -INFINITY ? 0.0f : ex2(s.m[h] - M);
+                s.m[h] = M;
+                s.l[h] *= f[0];
+#pragma unroll
+                for (int k = 1; k < KS; ++k) {
+                    const float mk = m_s[((k - 1) * RB + rb) * 8 + g];
+                    f[k] = mk == -INFINITY ? 0.0f : ex2(mk - M);
+                    s.l[h] = fmaf(l_s[((k - 1) * RB + rb) * 8 + g], f[k], s.l[h]);
+                }
+#pragma unroll
+                for (int b = 0; b < DB; ++b) {
+                    float x = s.acc[b][2 * h] * f[0], y = s.acc[b][2 * h + 1] * f[0];
+#pragma unroll
+                    for (int k = 1; k < KS; ++k) {
+                        const float2 o = *reinterpret_cast<const float2*>(
+                            scratch + (((k - 1) * RB + rb) * 8 + g) * D + 8 * b + 2 * tig);
+                        x = fmaf(o.x, f[k], x);
+                        y = fmaf(o.y, f[k], y);
+                    }
+                    s.acc[b][2 * h] = x;
+                    s.acc[b][2 * h + 1] = y;
+                }
+            }
+        }
     }
-    return v;
+    return s;
 }
 
 // Columns d and d + 1 of a row's result; true when it is not finite.
@@ -284,87 +375,154 @@ __device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& se
     return !(fabsf(x) < INFINITY && fabsf(y) < INFINITY);
 }
 
-// Counts this CTA's arrival at an item split over `parts` CTAs; true for the
-// last one, which then sees the others' slots.
-__device__ __forceinline__ bool last_to_arrive(unsigned* ticket, int parts) {
-    __shared__ int s_last;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        s_last = atomicAdd(ticket, 1u) + 1u == (unsigned)parts;
-        if (s_last) *ticket = 0u;  // ready for the next call
+// Columns d and d + 1 of row r of a split item, joined over its CTAs in order.
+template <int M, int D>
+__device__ __forceinline__ Joined join_slots(const AttnArgs& a, int first, int last, int r, int d) {
+    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int b = first; b <= last; ++b) v.m = fmaxf(v.m, __ldcg(slot_of<M, D>(a, b, first) + M * D + r));
+#pragma unroll 4
+    for (int b = first; b <= last; ++b) {
+        const float* p = slot_of<M, D>(a, b, first);
+        const float mk = __ldcg(p + M * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
+        const float2 o = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
+        v.l = fmaf(__ldcg(p + M * D + M + r), f, v.l);
+        v.x = fmaf(o.x, f, v.x);
+        v.y = fmaf(o.y, f, v.y);
     }
-    __syncthreads();
-    __threadfence();
-    return s_last != 0;
+    return v;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) paged_attn(const __grid_constant__ AttnArgs a) {
+template <typename T, int D, bool BOXES>
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_attn(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v) {
     using L = Layout<D>;
-    constexpr int M = kItemRows;
-    extern __shared__ __align__(128) unsigned char smem[];
-    const int tid = threadIdx.x;
-    float* o_s = reinterpret_cast<float*>(smem);
-    unsigned char* flag = smem + L::kRing + 2 * kTileKeys * 4;
-    const Place place = find_place<M, kTileKeys, kThreads>(a);
+    constexpr int M = kItemRows, ST = L::kStages;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ Ring<ST> ring;
+    __shared__ int last_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
+    const uint32_t base = (smem_addr(smem) + 1023u) & ~1023u;
+    float* scratch = reinterpret_cast<float*>(smem + (base - smem_addr(smem)) + L::kScratch);
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&ring.full[i], BOXES ? 1 : 32);
+            mbar_init(&ring.empty[i], kConsumers / 32);
+        }
+        mbar_fence_init();
+    }
+    const Place place = find_place<M, kTileKeys, kThreads>(a);  // its barriers publish the set-up
     if (place.s < 0) return;
-    walk<M, kTileKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
-        int shares;
-        if (it.rows <= 16) {
-            run_tiles<T, D, 1>(a, seq, p.s, it, p.j0, p.j1, smem);
-            shares = 4;
-        } else if (it.rows <= 32) {
-            run_tiles<T, D, 2>(a, seq, p.s, it, p.j0, p.j1, smem);
-            shares = 2;
-        } else {
-            run_tiles<T, D, 4>(a, seq, p.s, it, p.j0, p.j1, smem);
-            shares = 1;
-        }
-        const bool split = p.first != p.last;
-        if (split) {
-            float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
-            for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
-                const int r = e / (D / 2), d = 2 * (e % (D / 2));
-                const Joined v = join_shares<D>(o_s, shares, r, d);
-                *reinterpret_cast<float2*>(slot + r * D + d) = make_float2(v.x, v.y);
-                if (d == 0) {
-                    slot[M * D + r] = v.m;
-                    slot[M * D + M + r] = v.l;
+    bool ok = true;
+    if (warp == kConsumers / 32) {
+        produce<D, BOXES>(a, place, tm_k, tm_v, base, ring, ok);
+    } else {
+        uint32_t st = 0, turn = 0;
+        walk<M, kTileKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
+            // the part, its rows' results and what becomes of them, for RB blocks of rows
+            auto run = [&](auto blocks) {
+                constexpr int RB = decltype(blocks)::value;
+                const RowState<D> s = consume<T, D, RB, BOXES>(a, seq, it, p, base, scratch, ring, st, turn, ok);
+                const bool split = p.first != p.last;
+                unsigned bad = 0;  // bit h: row g + 8 h is not finite
+                if (warp < RB) {
+                    float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = warp * 16 + g + 8 * h;
+                        if (r >= it.rows) continue;
+                        if (split) {
+#pragma unroll
+                            for (int b = 0; b < D / 8; ++b)
+                                *reinterpret_cast<float2*>(slot + r * D + 8 * b + 2 * tig) =
+                                    make_float2(s.acc[b][2 * h], s.acc[b][2 * h + 1]);
+                            if (tig == 0) {
+                                slot[M * D + r] = s.m[h];
+                                slot[M * D + M + r] = s.l[h];
+                            }
+                        } else {
+#pragma unroll
+                            for (int b = 0; b < D / 8; ++b)
+                                if (write_pair<T, D>(a, seq, it.kvh, it.row0 + r, 8 * b + 2 * tig,
+                                                     {s.m[h], s.l[h], s.acc[b][2 * h], s.acc[b][2 * h + 1]}))
+                                    bad |= 1u << h;
+                        }
+                    }
+                    __syncwarp();
+                    if (!split)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            for (unsigned left = __ballot_sync(0xffffffffu, bad >> h & 1u); left;) {
+                                const int q = (__ffs(left) - 1) >> 2;  // row g of the warp's block
+                                exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + warp * 16 + q + 8 * h);
+                                left &= ~(15u << (4 * q));
+                            }
                 }
-            }
-        }
-        if (!split || last_to_arrive(a.tickets + p.first, p.last - p.first + 1)) {
-            if (tid < M) flag[tid] = 0;
-            __syncthreads();
-            for (int e = tid; e < it.rows * (D / 2); e += kThreads) {
-                const int r = e / (D / 2), d = 2 * (e % (D / 2));
-                const Joined v =
-                    split ? join_slots<M, D>(a, p.first, p.last, r, d) : join_shares<D>(o_s, shares, r, d);
-                if (write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, v)) flag[r] = 1;
-            }
-            __syncthreads();
-            for (int r = tid >> 5; r < it.rows; r += kThreads / 32)
-                if (flag[r]) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r);
-        }
-        __syncthreads();  // shared memory is free for the next item
-    });
+                if (!split) return;
+                __threadfence();
+                named_sync(1, kConsumers);
+                if (tid == 0) {
+                    unsigned* ticket = a.tickets + p.first;
+                    last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(p.last - p.first + 1);
+                    if (last_s) *ticket = 0u;  // ready for the next call
+                }
+                named_sync(1, kConsumers);
+                if (!last_s) return;
+                __threadfence();
+                // a warp a row, two columns a lane
+                for (int r = warp; r < it.rows; r += kConsumers / 32) {
+                    bool off = false;
+#pragma unroll
+                    for (int d = 2 * lane; d < D; d += 64)
+                        off |= write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d,
+                                                join_slots<M, D>(a, p.first, p.last, r, d));
+                    __syncwarp();
+                    if (__any_sync(0xffffffffu, off)) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r);
+                }
+            };
+            if (it.rows <= 16)
+                run(std::integral_constant<int, 1>());
+            else if (it.rows <= 32)
+                run(std::integral_constant<int, 2>());
+            else
+                run(std::integral_constant<int, 4>());
+            // the scratch is free, and everyone has read last_s
+            named_sync(1, kConsumers);
+        });
+    }
+    if (!ok) {
+        // a wait ran out: tell the host, and let copies in flight land
+        if (a.err) atomicOr(a.err, kErrWaitTimeout);
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20000000ll) __nanosleep(1000);
+    }
 }
 
-template <typename T, int D>
-int launch(const AttnArgs& args, cudaStream_t st) {
+template <typename T, int D, bool BOXES>
+int launch_boxes(const AttnArgs& args, cudaStream_t st) {
     using L = Layout<D>;
-    static_assert(4 * 16 * D * 4 + 2 * 64 * 4 <= L::kRing, "the merge must fit the ring");
-    static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<kItemRows, D>() * 4 <= kWorkspaceBytes && kMaxCtas * 4 <= kSlotsAt,
-                  "the slots must fit the workspace");
     AttnArgs a = args;
-    INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-    // as many CTAs as the SMs hold at once
-    int ctas = sm_count() * (D == 64 ? 4 : 2);
+    CUtensorMap mk = {}, mv = {};
+    if (BOXES) {
+        if (int s = paged_pool_map(&mk, a, a.k, D, Half16<T>::kBf16, kTileKeys)) return s;
+        if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kTileKeys)) return s;
+    }
+    INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn<T, D, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          (int)L::kBytes));
+    static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<kItemRows, D>() * 4 <= kWorkspaceBytes &&
+                      kMaxCtas * 4 <= kSlotsAt,
+                  "the slots must fit the workspace");
+    int ctas = sm_count() * 2;  // as many as the SMs hold at once
     if (ctas > kMaxCtas) ctas = kMaxCtas;
-    paged_attn<T, D><<<ctas, kThreads, L::kBytes, st>>>(a);
+    paged_attn<T, D, BOXES><<<ctas, kThreads, L::kBytes, st>>>(a, mk, mv);
     INFERNT_CUDA_TRY(cudaGetLastError());
     return INFERNT_OK;
+}
+
+template <typename T, int D>
+int launch(const AttnArgs& a, cudaStream_t st) {
+    return paged_attention_boxes(a.b.page_size) ? launch_boxes<T, D, true>(a, st) : launch_boxes<T, D, false>(a, st);
 }
 
 }  // namespace
@@ -394,7 +552,7 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     INFERNT_REQUIRE((long long)batch->num_rows * G < kMaxPositions, "%s: %d rows of %d heads", op, batch->num_rows, nq);
     // the units of the schedule are counted in 32 bits
     const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
-    const bool chunks = paged_attention_tc_pages(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
+    const bool chunks = paged_attention_boxes(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
     const long long tile_m = chunks ? kTcItemRows : kItemRows, tile_n = chunks ? kTcTileKeys : kTileKeys;
     INFERNT_REQUIRE(((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv < (1ll << 30) / (most_kv / tile_n + 2),
                     "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
@@ -419,7 +577,7 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.sinks = sinks;
     a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)D);
     a.scale_log2 = a.scale * 1.4426950408889634f;
-    a.min_tiles = 4;
+    a.min_tiles = 8;
     a.tickets = static_cast<unsigned*>(workspace);
     a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;

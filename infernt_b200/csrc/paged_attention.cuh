@@ -3,6 +3,8 @@
 // the CTAs, the partial results of split items, and the term-by-term row.
 #pragma once
 
+#include <cuda.h>
+
 #include "paged.cuh"
 
 namespace infernt {
@@ -32,11 +34,16 @@ struct AttnArgs {
     unsigned* err;
 };
 
-// The tcgen05 kernel (paged_attention_tc.cu): its items and tiles; pages as paged_attention_tc_pages says.
+// Whether tiles of 64 keys of such pages can be loaded as boxes of a tensor
+// map, and that map of a pool: [page][KV head][position][dim], boxes of 64
+// columns by the rows of a tile or of a page, 128-byte swizzle.
+bool paged_attention_boxes(int page_size);
+int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D, bool bf16, int tile_keys);
+
+// The tcgen05 kernel (paged_attention_tc.cu): its items and tiles.
 constexpr int kTcItemRows = 256;
 constexpr int kTcTileKeys = 64;
 int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st);
-bool paged_attention_tc_pages(int page_size);
 
 // Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
 // keys that they see: [0, sink_end) and [lo, hi), as tiles of N keys.

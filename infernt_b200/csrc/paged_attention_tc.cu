@@ -52,12 +52,6 @@ namespace infernt {
 
 void* tensor_map_encoder();  // bgemm.cu
 
-// The pages whose 64-key tiles are whole boxes: a tile is 64 / page_size
-// pages, or a page is a whole number of tiles.
-bool paged_attention_tc_pages(int page_size) {
-    return page_size % kTcTileKeys == 0 || (page_size >= 8 && kTcTileKeys % page_size == 0);
-}
-
 namespace {
 
 constexpr int kM = kTcItemRows;  // query rows of an item
@@ -344,8 +338,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         };
         uint32_t n = 0;  // key tiles of this row tile so far
         walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
+            // A wait that runs out ends the work on the scores, but not the barriers
+            // that the threads of both row tiles meet at.
             const int rows_x = it.rows - 128 * x;  // rows of this tile (of 128)
             const int row = it.row0 + 128 * x + r;
             const bool mine = r < rows_x;
@@ -375,7 +369,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     const uint32_t b = n & 1u;
                     tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return;
+                    if (!ok) break;
                     tc_fence_after();
                     float sv[kN];
                     tmem_ld64(tm_score(x, b) + lanes, sv);
@@ -435,7 +429,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             // O must hold the products before it is rescaled
                             tc_wait_bar(&bar.o[x][b ^ 1], ((n - 1) >> 1) & 1u, ok);
                             ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) return;
+                            if (!ok) break;
                             tc_fence_after();
                             const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
 #pragma unroll 1
@@ -468,7 +462,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     if (D == 64 && i >= 2) {
                         tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
                         ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) return;
+                        if (!ok) break;
                         tc_fence_after();
                     }
                     tmem_st32(tm_prob(x, b) + lanes, w);
@@ -478,7 +472,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
                 ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
                 tc_fence_after();
             }
             // ---- the part's result: straight to out, or through the slots
@@ -615,29 +608,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     }
 }
 
-int encode_pool(CUtensorMap* map, const AttnArgs& a, const void* pool, int D, bool bf16) {
-    auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
-    INFERNT_REQUIRE(fn, "paged_attention: cuTensorMapEncodeTiled is not available");
-    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.b.page_size, (cuuint64_t)a.b.nkv,
-                                (cuuint64_t)a.b.num_pages};
-    const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)a.b.page_size * D * 2,
-                                   (cuuint64_t)a.b.nkv * a.b.page_size * D * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(a.b.page_size < kN ? a.b.page_size : kN), 1, 1}, one[4] = {1, 1, 1, 1};
-    const CUresult r =
-        fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool),
-           dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    INFERNT_REQUIRE(r == CUDA_SUCCESS, "paged_attention: tensor map encoding failed (%d)", (int)r);
-    return INFERNT_OK;
-}
-
 template <typename T, int D>
 int launch_tc(const AttnArgs& args, cudaStream_t st) {
     using L = LayoutTc<D>;
     AttnArgs a = args;
     CUtensorMap mk, mv;
-    if (int s = encode_pool(&mk, a, a.k, D, Half16<T>::kBf16)) return s;
-    if (int s = encode_pool(&mv, a, a.v, D, Half16<T>::kBf16)) return s;
+    if (int s = paged_pool_map(&mk, a, a.k, D, Half16<T>::kBf16, kN)) return s;
+    if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kN)) return s;
     INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)L::kBytes));
     // one CTA an SM, as many as have slots in the workspace
@@ -652,6 +629,28 @@ int launch_tc(const AttnArgs& args, cudaStream_t st) {
 }
 
 }  // namespace
+
+// 64-key tiles are whole boxes: a tile is 64 / page_size pages, or a page is
+// a whole number of tiles.
+bool paged_attention_boxes(int page_size) {
+    return page_size % 64 == 0 || (page_size >= 8 && 64 % page_size == 0);
+}
+
+int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D, bool bf16, int tile_keys) {
+    auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encoder());
+    INFERNT_REQUIRE(fn, "paged_attention: cuTensorMapEncodeTiled is not available");
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.b.page_size, (cuuint64_t)a.b.nkv,
+                                (cuuint64_t)a.b.num_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)a.b.page_size * D * 2,
+                                   (cuuint64_t)a.b.nkv * a.b.page_size * D * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(a.b.page_size < tile_keys ? a.b.page_size : tile_keys), 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUresult r =
+        fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool),
+           dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    INFERNT_REQUIRE(r == CUDA_SUCCESS, "paged_attention: tensor map encoding failed (%d)", (int)r);
+    return INFERNT_OK;
+}
 
 int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st) {
     if (dtype == INFERNT_DTYPE_BF16)
