@@ -375,20 +375,37 @@ __device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& se
     return !(fabsf(x) < INFINITY && fabsf(y) < INFINITY);
 }
 
-// Columns d and d + 1 of row r of a split item, joined over its CTAs in order.
+// Columns d and d + 1 of row r of a split item, joined over its CTAs in order;
+// four of them are read at once.
 template <int M, int D>
 __device__ __forceinline__ Joined join_slots(const AttnArgs& a, int first, int last, int r, int d) {
     Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int b = first; b <= last; ++b) v.m = fmaxf(v.m, __ldcg(slot_of<M, D>(a, b, first) + M * D + r));
-#pragma unroll 4
-    for (int b = first; b <= last; ++b) {
-        const float* p = slot_of<M, D>(a, b, first);
-        const float mk = __ldcg(p + M * D + r), f = mk == -INFINITY ? 0.0f : ex2(mk - v.m);
-        const float2 o = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
-        v.l = fmaf(__ldcg(p + M * D + M + r), f, v.l);
-        v.x = fmaf(o.x, f, v.x);
-        v.y = fmaf(o.y, f, v.y);
+    for (int b = first; b <= last; b += 4) {
+        float m[4], l[4];
+        float2 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* p = slot_of<M, D>(a, min(b + i, last), first);
+            m[i] = __ldcg(p + M * D + r);
+            l[i] = __ldcg(p + M * D + M + r);
+            o[i] = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
+        }
+        float top = v.m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b + i > last) m[i] = -INFINITY;
+            top = fmaxf(top, m[i]);
+        }
+        const float f = v.m == -INFINITY ? 0.0f : ex2(v.m - top);
+        v = {top, v.l * f, v.x * f, v.y * f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = m[i] == -INFINITY ? 0.0f : ex2(m[i] - top);
+            if (b + i > last) continue;
+            v.l = fmaf(l[i], w, v.l);
+            v.x = fmaf(o[i].x, w, v.x);
+            v.y = fmaf(o[i].y, w, v.y);
+        }
     }
     return v;
 }
@@ -460,25 +477,31 @@ __global__ void __launch_bounds__(kThreads, 2)
                             }
                 }
                 if (!split) return;
-                __threadfence();
                 named_sync(1, kConsumers);
                 if (tid == 0) {
+                    // the others' writes, ordered before by the barrier, become visible with this thread's fence
+                    __threadfence();
                     unsigned* ticket = a.tickets + p.first;
                     last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(p.last - p.first + 1);
                     if (last_s) *ticket = 0u;  // ready for the next call
+                    __threadfence();
                 }
                 named_sync(1, kConsumers);
                 if (!last_s) return;
-                __threadfence();
-                // a warp a row, two columns a lane
-                for (int r = warp; r < it.rows; r += kConsumers / 32) {
-                    bool off = false;
+                // a warp a row, two columns a lane, two rows at once
+                for (int r = warp; r < it.rows; r += 2 * (kConsumers / 32)) {
+                    const int r2 = r + kConsumers / 32;
+                    bool off = false, off2 = false;
 #pragma unroll
-                    for (int d = 2 * lane; d < D; d += 64)
-                        off |= write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d,
-                                                join_slots<M, D>(a, p.first, p.last, r, d));
+                    for (int d = 2 * lane; d < D; d += 64) {
+                        const Joined v = join_slots<M, D>(a, p.first, p.last, r, d);
+                        const Joined v2 = join_slots<M, D>(a, p.first, p.last, min(r2, it.rows - 1), d);
+                        off |= write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, v);
+                        if (r2 < it.rows) off2 |= write_pair<T, D>(a, seq, it.kvh, it.row0 + r2, d, v2);
+                    }
                     __syncwarp();
                     if (__any_sync(0xffffffffu, off)) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r);
+                    if (__any_sync(0xffffffffu, off2)) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r2);
                 }
             };
             if (it.rows <= 16)
@@ -577,7 +600,7 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.sinks = sinks;
     a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)D);
     a.scale_log2 = a.scale * 1.4426950408889634f;
-    a.min_tiles = 8;
+    a.min_tiles = kLeast;
     a.tickets = static_cast<unsigned*>(workspace);
     a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;

@@ -498,15 +498,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         slot[kM * D + kM + ri] = l;
                     }
                 }
-                __threadfence();
                 named_sync(1, kRowThreads);
                 if (tid == 128) {
+                    // the others' writes, ordered before by the barrier, become visible with this thread's fence
+                    __threadfence();
                     unsigned* ticket = a.tickets + part.first;
                     last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(part.last - part.first + 1);
                     if (last_s) *ticket = 0u;  // ready for the next call
+                    __threadfence();
                 }
                 named_sync(1, kRowThreads);
-                __threadfence();
                 write = last_s != 0;
             }
             if (write && rows_x > 0) {
