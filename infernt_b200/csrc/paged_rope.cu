@@ -100,33 +100,175 @@ __device__ __forceinline__ float source_value<__half>(const __half* p) {
     return __half2float(*p);
 }
 
-// One block per token row.  Thread: the rotated pairs of the q and k heads,
-// then the elements that are copied.
-template <typename S, typename T>
-__global__ void __launch_bounds__(kRopeThreads) paged_rope(const RopeArgs a, const RopeDev rope) {
-    __shared__ float2 cs[kMaxPairs];
-    const int r = blockIdx.x, tid = threadIdx.x, D = a.D, half = rope.half, nkv = a.b.nkv;
+// Where row r of the batch goes: its sequence's position, and the page row of
+// head 0 (-1: nowhere).  False: the row stays as it is.
+__device__ __forceinline__ bool place_row(const RopeArgs& a, int r, int& pos, long long& row) {
     const int s = find_seq(a.b.q_start, a.b.num_seqs, r);
     const PagedSeq seq = paged_seq(a.b, s, a.err);
     const int i = r - seq.row0;
-    if (i < 0 || i >= seq.n_new) return;  // behind the last sequence, or a sequence that is skipped
-    const int pos = seq.len - seq.n_new + i;
-    if (pos < 0) return;
-    if (tid < half) {
-        const double t = (double)pos * rope.turns[tid];
-        const float f = (float)(t - rint(t));  // [-1/2, 1/2] turns
-        float sn, c;
-        sincospif(2.0f * f, &sn, &c);
-        cs[tid] = make_float2(c * rope.magnitude, sn * rope.magnitude);
-    }
-    long long row = -1;  // the page row of head 0
+    if (i < 0 || i >= seq.n_new) return false;  // behind the last sequence, or a sequence that is skipped
+    pos = seq.len - seq.n_new + i;
+    if (pos < 0) return false;
+    row = -1;
     if (a.k) {
-        const int page = a.b.table[(size_t)s * a.b.table_stride + pos / a.b.page_size];
+        const int pi = a.b.by_page(pos), page = a.b.table[(size_t)s * a.b.table_stride + pi];
         if (page >= 0 && page < a.b.num_pages)
-            row = (long long)page * nkv * a.b.page_size + pos % a.b.page_size;
-        else if (a.err && tid == 0)
+            row = (long long)page * a.b.nkv * a.b.page_size + (pos - pi * a.b.page_size);
+        else if (a.err && threadIdx.x == 0)
             atomicOr(a.err, kErrPage);
     }
+    return true;
+}
+
+// Cosine and sine of pair p at position pos, times the magnitude.
+__device__ __forceinline__ float2 turn_of(const RopeDev& rope, int p, int pos) {
+    const double t = (double)pos * rope.turns[p];
+    const float f = (float)(t - rint(t));  // [-1/2, 1/2] turns
+    float sn, c;
+    sincospif(2.0f * f, &sn, &c);
+    return make_float2(c * rope.magnitude, sn * rope.magnitude);
+}
+
+// Eight values of a row as loaded, and as FP32.
+template <typename S>
+struct Eight {
+    uint4 w[sizeof(S) / 2];
+};
+template <typename S>
+__device__ __forceinline__ Eight<S> load_eight(const S* p) {
+    Eight<S> v;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(S) / 2; ++i) v.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    return v;
+}
+__device__ __forceinline__ void to_floats(const Eight<float>& v, float (&x)[8]) {
+    const uint32_t w[8] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w, v.w[1].x, v.w[1].y, v.w[1].z, v.w[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+}
+template <typename S>
+__device__ __forceinline__ void to_floats(const Eight<S>& v, float (&x)[8]) {
+    const uint32_t w[4] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = Half16<S>::unpack(w[i]);
+        x[2 * i] = p.x;
+        x[2 * i + 1] = p.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_eight(T* p, const float (&x)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(Half16<T>::pack(x[0], x[1]), Half16<T>::pack(x[2], x[3]),
+                                              Half16<T>::pack(x[4], x[5]), Half16<T>::pack(x[6], x[7]));
+}
+
+// A block per token row; for rotary_dim a multiple of 16 and rows that allow
+// 16-byte loads.  The unit of work is two blocks of eight values, D / 16 to a
+// head: of the rotated part, block w of its first half and of its second
+// (which hold whole pairs in either layout), of the rest likewise.  The
+// block's threads are a multiple of D / 16, so a thread keeps its w, and with
+// it 8 cosines and sines in registers, for all heads.  A thread's first units
+// are loaded before the row's position is known, which takes three dependent
+// loads.  HBM-bound for chunks (8192 tokens of 32/8 heads of 128, bf16: 37 us,
+// 5.5 TB/s; 121 us value by value), latency-bound for single tokens.
+constexpr int kAhead = 3;
+
+template <typename S, typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRopeThreads) paged_rope_wide(const RopeArgs a, const __grid_constant__ RopeDev rope) {
+    __shared__ float2 cs_s[kMaxPairs];
+    const int r = blockIdx.x, tid = threadIdx.x, D = a.D, R = 2 * rope.half, nkv = a.b.nkv;
+    const int log_u = D == 64 ? 2 : 3, w = tid & ((1 << log_u) - 1);
+    const int heads_q = a.q ? a.nq : 0, heads = heads_q + (a.k ? 2 * nkv : 0);
+    const bool turns = w < R / 16;
+    // this thread's two blocks of a q or k head, and of a v head
+    const int lo = turns ? 8 * w : R + 8 * (w - R / 16), hi = turns ? lo + R / 2 : lo + (D - R) / 2;
+    auto source = [&](int h) {
+        if (h < heads_q) return static_cast<const S*>(a.q) + r * a.ldq + (long long)h * D;
+        h -= heads_q;
+        return h < nkv ? static_cast<const S*>(a.k) + r * a.ldk + (long long)h * D
+                       : static_cast<const S*>(a.v) + r * a.ldv + (long long)(h - nkv) * D;
+    };
+    const int h0 = tid >> log_u, step = kRopeThreads >> log_u;
+    Eight<S> x[kAhead], y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int h = min(h0 + i * step, heads - 1);
+        const S* p = source(h);
+        const bool is_v = h >= heads_q + nkv;
+        x[i] = load_eight(p + (is_v ? 8 * w : lo));
+        y[i] = load_eight(p + (is_v ? D / 2 + 8 * w : hi));
+    }
+    int pos;
+    long long row;
+    if (!place_row(a, r, pos, row)) return;
+    if (tid < rope.half) cs_s[tid] = turn_of(rope, tid, pos);
+    __syncthreads();
+    // of pair e of the first block; interleaved, the first block has four pairs, then the second's
+    float2 cs[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        cs[e] = !turns ? make_float2(1.0f, 0.0f)
+                       : cs_s[!INTERLEAVED ? 8 * w + e : e < 4 ? 4 * w + e : rope.half / 2 + 4 * w + e - 4];
+    auto finish = [&](int h, const Eight<S>& ex, const Eight<S>& ey) {
+        float u[8], v[8];
+        to_floats(ex, u);
+        to_floats(ey, v);
+        if (h < heads_q + nkv) {
+            if (INTERLEAVED) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float u0 = u[2 * e], u1 = u[2 * e + 1], v0 = v[2 * e], v1 = v[2 * e + 1];
+                    u[2 * e] = u0 * cs[e].x - u1 * cs[e].y;
+                    u[2 * e + 1] = u1 * cs[e].x + u0 * cs[e].y;
+                    v[2 * e] = v0 * cs[4 + e].x - v1 * cs[4 + e].y;
+                    v[2 * e + 1] = v1 * cs[4 + e].x + v0 * cs[4 + e].y;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float u0 = u[e], v0 = v[e];
+                    u[e] = u0 * cs[e].x - v0 * cs[e].y;
+                    v[e] = v0 * cs[e].x + u0 * cs[e].y;
+                }
+            }
+        }
+        T* dst;
+        int at = lo, to = hi;
+        if (h < heads_q) {
+            dst = static_cast<T*>(a.q_out) + r * a.ldo + (long long)h * D;
+        } else {
+            if (row < 0) return;
+            const int kh = h - heads_q;
+            const bool is_v = kh >= nkv;
+            dst = static_cast<T*>(is_v ? a.vp : a.kp) + (row + (long long)(is_v ? kh - nkv : kh) * a.b.page_size) * D;
+            if (is_v) {
+                at = 8 * w;
+                to = D / 2 + 8 * w;
+            }
+        }
+        store_eight(dst + at, u);
+        store_eight(dst + to, v);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        if (h0 + i * step < heads) finish(h0 + i * step, x[i], y[i]);
+    for (int h = h0 + kAhead * step; h < heads; h += step) {
+        const S* p = source(h);
+        const bool is_v = h >= heads_q + nkv;
+        finish(h, load_eight(p + (is_v ? 8 * w : lo)), load_eight(p + (is_v ? D / 2 + 8 * w : hi)));
+    }
+}
+
+// Any other rotary_dim, stride or alignment: a block per token row, value by
+// value.
+template <typename S, typename T>
+__global__ void __launch_bounds__(kRopeThreads) paged_rope(const RopeArgs a, const __grid_constant__ RopeDev rope) {
+    __shared__ float2 cs[kMaxPairs];
+    const int r = blockIdx.x, tid = threadIdx.x, D = a.D, half = rope.half, nkv = a.b.nkv;
+    int pos;
+    long long row;
+    if (!place_row(a, r, pos, row)) return;
+    if (tid < half) cs[tid] = turn_of(rope, tid, pos);
     __syncthreads();
     const int heads = (a.q ? a.nq : 0) + (row >= 0 ? nkv : 0), h0 = a.q ? 0 : a.nq;
     auto src_of = [&](int h) {
@@ -202,7 +344,17 @@ int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
 
 template <typename S, typename T>
 int launch(const RopeArgs& a, const RopeDev& d, cudaStream_t st) {
-    paged_rope<S, T><<<a.b.num_rows, kRopeThreads, 0, st>>>(a, d);
+    // rows of S or T `ld` apart that start where 16 bytes may be loaded
+    auto wide = [](const void* p, long long ld, size_t size) { return !p || (aligned16(p) && ld * size % 16 == 0); };
+    if (d.half % 8 == 0 && wide(a.q, a.ldq, sizeof(S)) && wide(a.k, a.ldk, sizeof(S)) && wide(a.v, a.ldv, sizeof(S)) &&
+        wide(a.q_out, a.ldo, sizeof(T))) {
+        if (d.interleaved)
+            paged_rope_wide<S, T, true><<<a.b.num_rows, kRopeThreads, 0, st>>>(a, d);
+        else
+            paged_rope_wide<S, T, false><<<a.b.num_rows, kRopeThreads, 0, st>>>(a, d);
+    } else {
+        paged_rope<S, T><<<a.b.num_rows, kRopeThreads, 0, st>>>(a, d);
+    }
     INFERNT_CUDA_TRY(cudaGetLastError());
     return INFERNT_OK;
 }
