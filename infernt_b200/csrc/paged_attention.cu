@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         mbar_fence_init();
     }
     const Place place = find_place<M, kTileKeys, kThreads>(a);  // its barriers publish the set-up
+    pdl_launch_dependents();  // the tcgen05 kernel may take SMs as they become free
     if (place.s < 0) return;
     bool ok = true;
     if (warp == kConsumers / 32) {
@@ -533,7 +534,7 @@ int launch_boxes(const AttnArgs& args, cudaStream_t st) {
     }
     INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn<T, D, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)L::kBytes));
-    static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<kItemRows, D>() * 4 <= kWorkspaceBytes &&
+    static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<kItemRows, D>() * 4 <= kTcWorkspaceAt &&
                       kMaxCtas * 4 <= kSlotsAt,
                   "the slots must fit the workspace");
     int ctas = sm_count() * 2;  // as many as the SMs hold at once
@@ -577,7 +578,7 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
     const bool chunks = paged_attention_boxes(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
     const long long tile_m = chunks ? kTcItemRows : kItemRows, tile_n = chunks ? kTcTileKeys : kTileKeys;
-    INFERNT_REQUIRE(((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv < (1ll << 30) / (most_kv / tile_n + 2),
+    INFERNT_REQUIRE(((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv < (1ll << 30) / (most_kv / tile_n + 2 + kItemCost),
                     "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
                     most_kv);
     if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
@@ -600,13 +601,28 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.sinks = sinks;
     a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt((float)D);
     a.scale_log2 = a.scale * 1.4426950408889634f;
-    a.min_tiles = kLeast;
+    a.min_units = kLeast;
+    a.min_rows = 0;
+    a.max_rows = kMaxPositions;
     a.tickets = static_cast<unsigned*>(workspace);
     a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (chunks) return paged_attention_tc(a, D, cache->dtype, st);
-    if (cache->dtype == INFERNT_DTYPE_BF16)
-        return D == 64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
-    return D == 64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+    // Sequences of up to kItemRows query rows are bound by the bytes of their
+    // keys, which the mma.sync kernel streams faster; longer ones by their
+    // products.  Where the batch's counts do not say that all sequences are
+    // as long as the longest, each kernel takes its own.
+    const bool both = chunks && batch->num_rows < (long long)batch->num_seqs * batch->max_q_len;
+    if (both) a.max_rows = kItemRows;
+    if (!chunks || both) {
+        int s;
+        if (cache->dtype == INFERNT_DTYPE_BF16)
+            s = D == 64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
+        else
+            s = D == 64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+        if (s || !chunks) return s;
+        a.min_rows = kItemRows;
+        a.max_rows = kMaxPositions;
+    }
+    return paged_attention_tc(a, D, cache->dtype, both, st);
 }

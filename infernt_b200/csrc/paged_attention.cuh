@@ -11,11 +11,13 @@ namespace infernt {
 
 constexpr float kRescale = 8.0f;  // log2 of the largest unnormalised probability
 
-// Workspace: the tickets of split items, then two slots of partial results
-// for each CTA.
+// Workspace: for each of the two kernels (a call may run both, the second
+// while the first ends) the tickets of split items, then two slots of partial
+// results for each CTA.
 constexpr size_t kWorkspaceBytes = 64u << 20;
-constexpr int kMaxCtas = 640;
-constexpr size_t kSlotsAt = 4096;
+constexpr int kMaxCtas = 320;
+constexpr size_t kSlotsAt = 2048;
+constexpr size_t kTcWorkspaceAt = 24u << 20;
 
 struct AttnArgs {
     PagedBatch b;
@@ -28,7 +30,8 @@ struct AttnArgs {
     int nq, G, window, sinks;
     FastDiv by_g;
     float scale, scale_log2;
-    int min_tiles;      // least tiles of a CTA
+    int min_rows, max_rows;  // a sequence of min_rows query rows or fewer, or more than max_rows, is another kernel's
+    int min_units;      // least units of a CTA
     unsigned* tickets;  // [CTAs], zero between calls
     float* slots;
     unsigned* err;
@@ -41,9 +44,10 @@ bool paged_attention_boxes(int page_size);
 int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D, bool bf16, int tile_keys);
 
 // The tcgen05 kernel (paged_attention_tc.cu): its items and tiles.
+// after_other: the kernel launched just before on st is paged_attn.
 constexpr int kTcItemRows = 256;
 constexpr int kTcTileKeys = 64;
-int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st);
+int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st);
 
 // Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
 // keys that they see: [0, sink_end) and [lo, hi), as tiles of N keys.
@@ -97,9 +101,15 @@ __device__ __forceinline__ int tile_key(const Item& it, int j) {
 constexpr int kItemCost = 3;
 constexpr int kLeast = kItemCost + 2;
 
+// Query rows of a KV head that are this kernel's.
+__device__ __forceinline__ int rows_of(const AttnArgs& a, const PagedSeq& s) {
+    const int rows = s.n_new * a.G;
+    return rows > a.min_rows && rows <= a.max_rows ? rows : 0;
+}
+
 template <int M, int N>
 __device__ __forceinline__ int item_units(const AttnArgs& a, const PagedSeq& s, int row0) {
-    return row0 < s.n_new * a.G ? make_item<M, N>(a, s, 0, row0).tiles + kItemCost : 0;
+    return row0 < rows_of(a, s) ? make_item<M, N>(a, s, 0, row0).tiles + kItemCost : 0;
 }
 
 // Units of one KV head of s, by a whole warp.
@@ -107,7 +117,7 @@ template <int M, int N>
 __device__ __forceinline__ int head_units(const AttnArgs& a, const PagedSeq& s) {
     const int lane = threadIdx.x & 31;
     int n = 0;
-    for (int row0 = lane * M; row0 < s.n_new * a.G; row0 += 32 * M) n += item_units<M, N>(a, s, row0);
+    for (int row0 = lane * M; row0 < rows_of(a, s); row0 += 32 * M) n += item_units<M, N>(a, s, row0);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
@@ -163,7 +173,7 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
     auto units = [&](int s, PagedSeq& q) {
         q = {0, 0, 0};
         if (s < n) q = paged_seq(a.b, s, blockIdx.x == 0 ? a.err : nullptr);
-        const bool many = q.n_new * a.G > 2 * M;
+        const bool many = rows_of(a, q) > 2 * M;
         int u = many ? 0 : item_units<M, N>(a, q, 0) + item_units<M, N>(a, q, M);
         for (unsigned left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
             const int k = __ffs(left) - 1;
@@ -198,7 +208,7 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
         before = p.total + scan(p.per_head * a.b.nkv, all);
         p.total += all;
     }
-    p.c = max(a.min_tiles, (int)(((unsigned)p.total + gridDim.x - 1) / gridDim.x));
+    p.c = max(a.min_units, (int)(((unsigned)p.total + gridDim.x - 1) / gridDim.x));
     const int at = p.c * (int)blockIdx.x;
     int sum = 0;
     if (at < p.total)

@@ -607,10 +607,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         tc_fence_after();
         tmem_free(tmem, 512);
     }
+    pdl_wait();  // this kernel's end is the call's end
 }
 
 template <typename T, int D>
-int launch_tc(const AttnArgs& args, cudaStream_t st) {
+int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
     using L = LayoutTc<D>;
     AttnArgs a = args;
     CUtensorMap mk, mv;
@@ -618,14 +619,29 @@ int launch_tc(const AttnArgs& args, cudaStream_t st) {
     if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kN)) return s;
     INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                           (int)L::kBytes));
+    a.tickets += kTcWorkspaceAt / sizeof(unsigned);
+    a.slots += kTcWorkspaceAt / sizeof(float);
     // one CTA an SM, as many as have slots in the workspace
-    constexpr int most = (int)((kWorkspaceBytes - kSlotsAt) / (2 * slot_floats<kM, D>() * sizeof(float)));
+    constexpr int most =
+        (int)((kWorkspaceBytes - kTcWorkspaceAt - kSlotsAt) / (2 * slot_floats<kM, D>() * sizeof(float)));
     int ctas = sm_count();
     if (ctas > most) ctas = most;
     if (ctas > kMaxCtas) ctas = kMaxCtas;
-    a.min_tiles = 8;
-    paged_attn_tc<T, D><<<ctas, kThreadsTc, L::kBytes, st>>>(a, mk, mv);
-    INFERNT_CUDA_TRY(cudaGetLastError());
+    a.min_units = 8;
+    // beside the end of the kernel launched just before, when that is the
+    // other kernel of this call: neither touches what the other writes
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kThreadsTc);
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = after_other ? 1 : 0;
+    INFERNT_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_attn_tc<T, D>, static_cast<const AttnArgs>(a),
+                                        static_cast<const CUtensorMap>(mk), static_cast<const CUtensorMap>(mv)));
     return INFERNT_OK;
 }
 
@@ -653,10 +669,10 @@ int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D,
     return INFERNT_OK;
 }
 
-int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, cudaStream_t st) {
+int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st) {
     if (dtype == INFERNT_DTYPE_BF16)
-        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, st) : launch_tc<__nv_bfloat16, 128>(a, st);
-    return head_dim == 64 ? launch_tc<__half, 64>(a, st) : launch_tc<__half, 128>(a, st);
+        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, after_other, st) : launch_tc<__nv_bfloat16, 128>(a, after_other, st);
+    return head_dim == 64 ? launch_tc<__half, 64>(a, after_other, st) : launch_tc<__half, 128>(a, after_other, st);
 }
 
 }  // namespace infernt
