@@ -880,25 +880,21 @@ class TPEngine:
 
 
 # ------------------------------------------ operators over paged caches
+# These wrappers stand in a decode step's path, so their checks are few and
+# plain: each costs a fraction of a microsecond.
 _TORCH_DTYPES = {}
 
 
 def _dtype(t):
-    """DTYPE_* of a torch tensor."""
+    """DTYPE_* of a torch tensor (-1: int32)."""
     d = _TORCH_DTYPES.get(t.dtype)
     if d is None:
-        d = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}.get(str(t.dtype))
+        d = {"torch.float32": DTYPE_F32, "torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16,
+             "torch.int32": -1}.get(str(t.dtype))
         if d is None:
             raise ValueError("type %s (float32, bfloat16 or float16)" % t.dtype)
         _TORCH_DTYPES[t.dtype] = d
     return d
-
-
-def _ints(t, what):
-    """Device pointer of a contiguous int32 tensor."""
-    if str(t.dtype) != "torch.int32" or not t.is_contiguous():
-        raise ValueError("%s: a contiguous int32 tensor is needed" % what)
-    return t.data_ptr()
 
 
 class PagedCache(ctypes.Structure):
@@ -909,11 +905,12 @@ class PagedCache(ctypes.Structure):
                 ("dtype", _I)]
 
     def __init__(self, k, v):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
-            raise ValueError("PagedCache: k %s %s, v %s %s" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
-        if not (k.is_contiguous() and v.is_contiguous()):
-            raise ValueError("PagedCache: the pools must be contiguous")
-        super().__init__(k.data_ptr(), v.data_ptr(), *k.shape, _dtype(k))
+        shape, d = k.shape, _dtype(k)
+        if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.get_device() != k.get_device():
+            raise ValueError("PagedCache: k %s %s, v %s %s" % (tuple(shape), k.dtype, tuple(v.shape), v.dtype))
+        if not (k.is_contiguous() and v.is_contiguous()) or d < 0:
+            raise ValueError("PagedCache: the pools must be contiguous, of a floating type")
+        super().__init__(k.data_ptr(), v.data_ptr(), *shape, d)
         self.tensors = (k, v)
 
 
@@ -925,12 +922,14 @@ class RaggedBatch(ctypes.Structure):
                 ("max_q_len", _I), ("table_stride", _I)]
 
     def __init__(self, q_start, kv_len, block_table, num_rows, max_q_len):
-        n = kv_len.numel()
-        if q_start.numel() != n + 1 or block_table.dim() != 2 or block_table.shape[0] != n:
-            raise ValueError("RaggedBatch: %d starts, %d lengths, table %s"
-                             % (q_start.numel(), n, tuple(block_table.shape)))
-        super().__init__(_ints(q_start, "q_start"), _ints(kv_len, "kv_len"), _ints(block_table, "block_table"), n,
-                         num_rows, max_q_len, block_table.shape[1])
+        n, shape = kv_len.numel(), block_table.shape
+        if q_start.numel() != n + 1 or len(shape) != 2 or shape[0] != n:
+            raise ValueError("RaggedBatch: %d starts, %d lengths, table %s" % (q_start.numel(), n, tuple(shape)))
+        for t in (q_start, kv_len, block_table):
+            if _dtype(t) != -1 or not t.is_contiguous():
+                raise ValueError("RaggedBatch: contiguous int32 tensors are needed")
+        super().__init__(q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), n, num_rows, max_q_len,
+                         shape[1])
         self.tensors = (q_start, kv_len, block_table)
 
 
@@ -945,87 +944,95 @@ class RopeParams(ctypes.Structure):
 
     def __init__(self, theta=10000.0, rotary_dim=128, interleaved=False, scaling="none", original_max_len=0,
                  factor=1.0, low=1.0, high=4.0):
-        if scaling not in ROPE_SCALINGS:
+        code = ROPE_SCALINGS.get(scaling)
+        if code is None:
             raise ValueError("RopeParams: scaling %r (%s)" % (scaling, ", ".join(ROPE_SCALINGS)))
-        super().__init__(theta, rotary_dim, int(interleaved), ROPE_SCALINGS[scaling], original_max_len, factor, low,
-                         high)
+        super().__init__(theta, rotary_dim, bool(interleaved), code, original_max_len, factor, low, high)
 
 
 def _rows(t, rows, heads, dim, what):
     """Row stride of a [rows][heads][dim] tensor whose heads lie next to each
     other (a slice of stacked rows, for one)."""
-    if t.dim() != 3 or t.shape[0] < rows or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError("%s: shape %s for %d rows of %s heads of %d" % (what, tuple(t.shape), rows, heads, dim))
+    shape = t.shape
+    if len(shape) != 3 or shape[0] < rows or shape[1] != heads or shape[2] != dim:
+        raise ValueError("%s: shape %s for %d rows of %d heads of %d" % (what, tuple(shape), rows, heads, dim))
     r, h, e = t.stride()
-    if e != 1 or (h != dim and t.shape[1] > 1):
+    if e != 1 or (h != dim and heads > 1):
         raise ValueError("%s: strides %s; only rows may be apart" % (what, t.stride()))
     # one row has no stride of its own
-    return r if t.shape[0] > 1 else max(r, t.shape[1] * dim)
+    return r if shape[0] > 1 else max(r, heads * dim)
 
 
 def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
     """Rotary positions of the batch's q rows into q_out, the rotated k rows
     and the v rows into their pages (infernt_paged_rope_append).  q and q_out,
     or k and v, may be None.  stream: a cudaStream_t as an integer."""
-    n, dim = batch.num_rows, cache.head_dim
-    one = q if q is not None else k
+    n, dim, src = batch.num_rows, cache.head_dim, None
+    qp = op = kp = vp = None
     nq = ldo = ldq = ldk = ldv = 0
     if q is not None:
-        nq = q.shape[1]
-        ldq, ldo = _rows(q, n, None, dim, "q"), _rows(q_out, n, nq, dim, "q_out")
+        nq, src, qp, op = q.shape[1], q.dtype, q.data_ptr(), q_out.data_ptr()
+        ldq, ldo = _rows(q, n, nq, dim, "q"), _rows(q_out, n, nq, dim, "q_out")
         if _dtype(q_out) != cache.dtype:
             raise ValueError("paged_rope_append: q_out has another type than the cache")
     if k is not None:
-        ldk, ldv = _rows(k, n, cache.num_kv_heads, dim, "k"), _rows(v, n, cache.num_kv_heads, dim, "v")
-        if k.dtype != v.dtype or k.dtype != one.dtype:
+        nkv, kp, vp = cache.num_kv_heads, k.data_ptr(), v.data_ptr()
+        ldk, ldv = _rows(k, n, nkv, dim, "k"), _rows(v, n, nkv, dim, "v")
+        if k.dtype != v.dtype or (src is not None and src != k.dtype):
             raise ValueError("paged_rope_append: q, k and v of different types")
-    call("infernt_paged_rope_append", ptr(q_out), ldo, ptr(q), ldq, nq, ptr(k), ldk, ptr(v), ldv, _dtype(one),
+    call("infernt_paged_rope_append", op, ldo, qp, ldq, nq, kp, ldk, vp, ldv, _dtype(q if k is None else k),
          ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(rope), ptr(err), stream)
+
+
+_workspace_bytes = 0
+
+
+def paged_attention_workspace_bytes():
+    global _workspace_bytes
+    if not _workspace_bytes:
+        _workspace_bytes = lib().infernt_paged_attention_workspace_bytes()
+    return _workspace_bytes
 
 
 def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.0, lse=None, err=None, stream=None):
     """Attention of the batch's new tokens over the pages
-    (infernt_paged_attention).  workspace: a zeroed uint8 tensor of
+    (infernt_paged_attention).  workspace: a zeroed tensor of
     paged_attention_workspace_bytes() bytes."""
     n, dim, nq = batch.num_rows, cache.head_dim, q.shape[1]
-    if _dtype(q) != cache.dtype or _dtype(out) != cache.dtype:
+    if _dtype(q) != cache.dtype or q.dtype != out.dtype:
         raise ValueError("paged_attention: q, out and the cache must have one type")
-    if lse is not None and (tuple(lse.shape[1:]) != (nq,) or lse.shape[0] < n or not lse.is_contiguous()
-                            or _dtype(lse) != DTYPE_F32):
-        raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(lse.shape), n, nq))
-    if workspace.numel() * workspace.element_size() < paged_attention_workspace_bytes():
+    if lse is not None:
+        shape = lse.shape
+        if len(shape) != 2 or shape[1] != nq or shape[0] < n or _dtype(lse) != DTYPE_F32 or not lse.is_contiguous():
+            raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(shape), n, nq))
+    if workspace.nbytes < paged_attention_workspace_bytes():
         raise ValueError("paged_attention: a workspace of %d bytes is needed" % paged_attention_workspace_bytes())
     call("infernt_paged_attention", out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(),
-         _rows(q, n, None, dim, "q"), nq, ctypes.byref(cache), ctypes.byref(batch), window, sinks, scale, ptr(lse),
+         _rows(q, n, nq, dim, "q"), nq, ctypes.byref(cache), ctypes.byref(batch), window, sinks, scale, ptr(lse),
          workspace.data_ptr(), ptr(err), stream)
-
-
-def paged_attention_workspace_bytes():
-    return lib().infernt_paged_attention_workspace_bytes()
 
 
 def copy_pages(pools, src, dst, stream=None):
     """Page src[i] into page dst[i] in every pool (infernt_pages_copy): a
     contiguous tensor [pools][pages][...], or a list of contiguous tensors
     [pages][...] of one shape and type."""
-    if len(src) != len(dst):
-        raise ValueError("copy_pages: %d sources, %d destinations" % (len(src), len(dst)))
-    many = isinstance(pools, (list, tuple))
-    if many:
-        first = pools[0]
+    n = len(src)
+    if n != len(dst):
+        raise ValueError("copy_pages: %d sources, %d destinations" % (n, len(dst)))
+    if isinstance(pools, (list, tuple)):
+        first, count = pools[0], len(pools)
         if any(p.shape != first.shape or p.dtype != first.dtype or not p.is_contiguous() for p in pools):
             raise ValueError("copy_pages: the pools must be contiguous tensors of one shape and type")
-        base, count = [p.data_ptr() for p in pools], len(pools)
+        base = [p.data_ptr() for p in pools]
+        pages, size = first.shape[0], first.nbytes
     else:
         if not pools.is_contiguous() or pools.dim() < 3:
             raise ValueError("copy_pages: a contiguous tensor [pools][pages][...] is needed")
-        count, first = pools.shape[0], pools[0]
-        size = first.numel() * first.element_size()
-        base = [pools.data_ptr() + i * size for i in range(count)]
-    pages, n = first.shape[0], len(src)
-    call("infernt_pages_copy", (ctypes.c_void_p * max(1, count))(*base), count,
-         first.numel() // pages * first.element_size(), pages, (ctypes.c_int * max(1, n))(*src),
-         (ctypes.c_int * max(1, n))(*dst), n, stream)
+        count, pages = pools.shape[:2]
+        size, start = pools.nbytes // max(1, count), pools.data_ptr()
+        base = range(start, start + count * size, size) if size else ()
+    call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, (_I * n)(*src), (_I * n)(*dst), n,
+         stream)
 
 
 class PagePool:

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "internal.h"
 
@@ -99,6 +101,18 @@ struct Half16<__half> {
     static __device__ __forceinline__ __half round(float a) { return __float2half_rn(a); }
     static __device__ __forceinline__ float value(__half a) { return __half2float(a); }
 };
+
+// Lets kernel use `bytes` of dynamic shared memory: once a kernel and device,
+// since the setting stays (set_on has a bit per device).
+template <typename K>
+inline int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& set_on) {
+    const int d = current_device();
+    const unsigned long long bit = d >= 0 && d < 64 ? 1ull << d : 0;
+    if (set_on.load(std::memory_order_acquire) & bit) return INFERNT_OK;
+    INFERNT_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    set_on.fetch_or(bit, std::memory_order_release);
+    return INFERNT_OK;
+}
 
 // Argument checks that the operators share (paged_rope.cu).
 int check_paged_cache(const char* op, const infernt_paged_cache* c);

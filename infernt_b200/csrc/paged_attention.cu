@@ -532,8 +532,8 @@ int launch_boxes(const AttnArgs& args, cudaStream_t st) {
         if (int s = paged_pool_map(&mk, a, a.k, D, Half16<T>::kBf16, kTileKeys)) return s;
         if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kTileKeys)) return s;
     }
-    INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn<T, D, BOXES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)L::kBytes));
+    static std::atomic<unsigned long long> set_on{0};
+    if (int s = allow_smem(paged_attn<T, D, BOXES>, (int)L::kBytes, set_on)) return s;
     static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<kItemRows, D>() * 4 <= kTcWorkspaceAt &&
                       kMaxCtas * 4 <= kSlotsAt,
                   "the slots must fit the workspace");

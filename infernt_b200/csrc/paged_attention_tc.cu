@@ -617,8 +617,8 @@ int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
     CUtensorMap mk, mv;
     if (int s = paged_pool_map(&mk, a, a.k, D, Half16<T>::kBf16, kN)) return s;
     if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kN)) return s;
-    INFERNT_CUDA_TRY(cudaFuncSetAttribute(paged_attn_tc<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                          (int)L::kBytes));
+    static std::atomic<unsigned long long> set_on{0};
+    if (int s = allow_smem(paged_attn_tc<T, D>, (int)L::kBytes, set_on)) return s;
     a.tickets += kTcWorkspaceAt / sizeof(unsigned);
     a.slots += kTcWorkspaceAt / sizeof(float);
     // one CTA an SM, as many as have slots in the workspace

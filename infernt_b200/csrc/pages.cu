@@ -92,8 +92,7 @@ extern "C" int infernt_pages_copy(void* const* pools, int n_pools, size_t page_b
     }
     INFERNT_REQUIRE(clash < 0, "pages_copy: page %d is a destination twice, or a source too", clash);
     if (n_pools == 0 || n == 0) return INFERNT_OK;
-    for (int i = 0; i < n_pools; ++i)
-        if (int s = check_device_pointer("pages_copy", "a pool", pools[i])) return s;
+    if (int s = check_device_pointer("pages_copy", "the first pool", pools[0])) return s;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // a short list keeps the parameters of a fork's launch small
     if (n_pools <= 64 && n <= 32) return launch_copy<64, 32>(pools, n_pools, page_bytes, src, dst, n, st);
