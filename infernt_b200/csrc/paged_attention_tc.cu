@@ -32,8 +32,8 @@
 // The probabilities of a tile are computed with the m of the tiles before,
 // with no search for their maximum: any m gives the same result, so long as
 // the probabilities fit their 16 bits, and a tile whose sum stays below 2^13
-// does.  Where it does not (and for the first keys, and hidden ones) the tile
-// is computed again with its own maximum, and O is rescaled if that has
+// does.  Where it does not (and for a row's first keys) the tile is computed
+// again with its own maximum, and O is rescaled if that has
 // passed m by more than 2^8.  One pair in eight takes 2^x on the FMA pipe
 // (nearest integer, then a polynomial of degree 4 on the rest): the special
 // function unit would otherwise be the longest path.  Both measured on 4096
@@ -105,13 +105,13 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
     return r;
 }
 
-// 2^x of a pair without the special function unit, for x <= 100 (from -126
-// down it stays at 2^-126): n = x to the nearest integer by the addition of
-// 3 x 2^22, 2^(x - n) by the polynomial of least largest relative error on
-// [-1/2, 1/2] (2.7e-6 in FP32), n added to its exponent.
-__device__ __forceinline__ float2 ex2_pair(F2 x) {
-    const float2 v = un2(x);
-    x = f2(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+// 2^x of a pair without the special function unit, for x <= 100: n = x to the
+// nearest integer by the addition of 3 x 2^22, 2^(x - n) by the polynomial of
+// least largest relative error on [-1/2, 1/2] (2.7e-6 in FP32), n added to its
+// exponent.  Below -125 (hidden keys' minus infinity among it) 0; NaN stays.
+__device__ __forceinline__ float2 ex2_pair(F2 arg) {
+    const float2 v = un2(arg);
+    const F2 x = f2(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
     const F2 big = f2(12582912.0f, 12582912.0f), less = f2(-12582912.0f, -12582912.0f), minus = f2(-1.0f, -1.0f);
     const F2 t = add2(x, big), f = fma2(add2(t, less), minus, x);
     F2 p = f2(0.009570102207362652f, 0.009570102207362652f);
@@ -120,8 +120,10 @@ __device__ __forceinline__ float2 ex2_pair(F2 x) {
     p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
     p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
     const float2 n = un2(t), q = un2(p);
-    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
-                       __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
+    const F2 r = f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
+                    __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
+    const float2 w = un2(fma2(arg, f2(0.0f, 0.0f), r));  // NaN where arg is
+    return make_float2(v.x < -125.0f ? 0.0f : w.x, v.y < -125.0f ? 0.0f : w.y);
 }
 
 // Whether the tile at key k0 has keys that no row of the item sees.
@@ -374,13 +376,27 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     float sv[kN];
                     tmem_ld64(tm_score(x, b) + lanes, sv);
                     // keys that every row of the item sees need no mask
-                    const bool whole = k0 + kN - 1 <= it.pos_first &&
-                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
+                    const bool all_hi = k0 + kN - 1 <= it.pos_first;
+                    const bool all_lo = a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks;
+                    bool sees = true;  // whether this row sees one of them
+                    if (!(all_hi && all_lo)) {
+                        const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sink = a.sinks - k0;
+                        if (all_lo) {
+#pragma unroll
+                            for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
+                            sees = hi >= 0;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
+                            sees = hi >= 0 && (lo < kN - 1 || sink > 0);
+                        }
+                    }
                     uint32_t w[kN / 2];
                     float lsum = 0.0f;
                     bool done = false;
-                    if (whole && i > 0) {
-                        // probabilities under the m of the halves before, unless their sum
+                    // a row without an m has no measure yet for what it sees
+                    if (!__any_sync(0xffffffffu, m == -INFINITY && sees)) {
+                        // probabilities under the m of the tiles before, unless their sum
                         // says that a score has passed it by far
                         const float ref = m == -INFINITY ? 0.0f : m;
                         const F2 ref2 = f2(-ref, -ref);
@@ -403,18 +419,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
                     }
                     if (!done) {
-                        // the first keys, hidden keys, and keys whose maximum moves m
-                        if (!whole) {
-                            const int hi = pos - k0;
-                            if (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks) {
-#pragma unroll
-                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
-                            } else {
-                                const int lo = hi - a.window, sink = a.sinks - k0;
-#pragma unroll
-                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
-                            }
-                        }
+                        // a row's first keys, and keys whose maximum moves m
                         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                         for (int e = 0; e < kN; e += 4) {
@@ -534,21 +539,27 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     for (int e = 0; e < 64; ++e) o[e] = 0.0f;
                     if (!split) {
                         if (some) tmem_ld64(tm_ox + 64 * c, o);
-                    } else if (mine) {
+                    } else {
+#pragma unroll 1
                         for (int b = part.first; b <= part.last; ++b) {
                             const float* p = slot_of<kM, D>(a, b, part.first);
-                            const float mb = __ldcg(p + kM * D + ri), f = mb == -INFINITY ? 0.0f : ex2(mb - M);
-                            float4 v[16];
+                            float v[64];
+                            if (b == (int)blockIdx.x) {  // its own is still here
+                                tmem_ld64(tm_ox + 64 * c, v);
+                            } else {
 #pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                v[e] = __ldcg(reinterpret_cast<const float4*>(p) + (16 * c + e) * kM + ri);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                o[4 * e] = fmaf(v[e].x, f, o[4 * e]);
-                                o[4 * e + 1] = fmaf(v[e].y, f, o[4 * e + 1]);
-                                o[4 * e + 2] = fmaf(v[e].z, f, o[4 * e + 2]);
-                                o[4 * e + 3] = fmaf(v[e].w, f, o[4 * e + 3]);
+                                for (int e = 0; e < 16; ++e) {
+                                    const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p) + (16 * c + e) * kM + ri);
+                                    v[4 * e] = f4.x;
+                                    v[4 * e + 1] = f4.y;
+                                    v[4 * e + 2] = f4.z;
+                                    v[4 * e + 3] = f4.w;
+                                }
                             }
+                            const float mb = mine ? __ldcg(p + kM * D + ri) : -INFINITY;
+                            const float f = mb == -INFINITY ? 0.0f : ex2(mb - M);
+#pragma unroll
+                            for (int e = 0; e < 64; ++e) o[e] = fmaf(v[e], f, o[e]);
                         }
                     }
 #pragma unroll

@@ -81,6 +81,16 @@ def test_long_windowed_chunk(torch, ws, window, sinks):
     check_attention(c, window, sinks, rows=[0, 1, 31, 63, 64, 255, 256, 300, 511, 512, 600, 699])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [4, 8])
+def test_windows_that_begin_with_a_tile(torch, ws, G, D):
+    """The first key of the last rows of a block of query rows is the first of
+    a tile of keys, while the first rows' windows begin in the tile before."""
+    for window in (448, 449, 447, 64, 128):
+        c = run(Case(torch, [(256, 2048)], 2 * G, 2, D, 64), ws, window)
+        check_attention(c, window, rows=[0, 1, 31, 32, 62, 63, 64, 127, 128, 191, 255])
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (30, 2)])
 def test_rows_that_see_nothing(torch, ws, window, sinks):
     """More new tokens than positions: the first rows have negative positions
@@ -114,6 +124,18 @@ def test_hidden_rows_that_are_not_finite(torch, ws, chunk, length, bad):
     s = torch.einsum("d,pd->p", c.q[first, G].double(), k[:at + 1, 1]) / math.sqrt(128)
     want = torch.softmax(s, 0) @ v[:at + 1, 1]
     assert bool((torch.isfinite(want) == torch.isfinite(seen[0, G])).all())
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_scores_that_are_not_finite(torch, ws, bad):
+    """One key of a KV head is not finite: every row that sees it has no
+    finite result there, wherever in a tile it lies; the other head is whole."""
+    for at in list(range(64, 130)) + [5, 190]:
+        c = Case(torch, [(100, 300)], 4, 2, 64, 16)
+        c.k[c.pages[0][at // 16], 1, at % 16] = bad
+        run(c, ws)
+        assert not bool(torch.isfinite(c.out[:, 2:].float()).any()), at
+        assert bool(torch.isfinite(c.out[:, :2].float()).all()), at
 
 
 def test_hidden_by_a_window(torch, ws):
