@@ -108,10 +108,14 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 // 2^x of a pair without the special function unit, for x <= 100: n = x to the
 // nearest integer by the addition of 3 x 2^22, 2^(x - n) by the polynomial of
 // least largest relative error on [-1/2, 1/2] (2.7e-6 in FP32), n added to its
-// exponent.  Below -125 (hidden keys' minus infinity among it) 0; NaN stays.
+// exponent.  Below -126 (hidden keys' minus infinity among it) x becomes
+// -126.49, whose result is subnormal and flushed to 0.  NaN becomes NaN or
+// the largest number, and so the sum of a tile too large either way.
 __device__ __forceinline__ float2 ex2_pair(F2 arg) {
-    const float2 v = un2(arg);
-    const F2 x = f2(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+    float2 v = un2(arg);
+    asm("max.NaN.f32 %0, %0, 0fC2FCFAE1;" : "+f"(v.x));
+    asm("max.NaN.f32 %0, %0, 0fC2FCFAE1;" : "+f"(v.y));
+    const F2 x = f2(v.x, v.y), one = f2(1.0f, 1.0f);
     const F2 big = f2(12582912.0f, 12582912.0f), less = f2(-12582912.0f, -12582912.0f), minus = f2(-1.0f, -1.0f);
     const F2 t = add2(x, big), f = fma2(add2(t, less), minus, x);
     F2 p = f2(0.009570102207362652f, 0.009570102207362652f);
@@ -120,10 +124,10 @@ __device__ __forceinline__ float2 ex2_pair(F2 arg) {
     p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
     p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
     const float2 n = un2(t), q = un2(p);
-    const F2 r = f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
-                    __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
-    const float2 w = un2(fma2(arg, f2(0.0f, 0.0f), r));  // NaN where arg is
-    return make_float2(v.x < -125.0f ? 0.0f : w.x, v.y < -125.0f ? 0.0f : w.y);
+    F2 r = f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
+              __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
+    asm("mul.rn.ftz.f32x2 %0, %0, %1;" : "+l"(r) : "l"(one));
+    return un2(r);
 }
 
 // Whether the tile at key k0 has keys that no row of the item sees.
@@ -347,6 +351,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const bool mine = r < rows_x;
             const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
             float m = -INFINITY, l = 0.0f;  // m in base 2
+            bool settled = false;           // every row of the warp has its m
             if (rows_x > 0 && part.j0 < part.j1) {
                 // Q rows of this warp: D / 8 lanes of 16 bytes a row, all in flight at once
                 {
@@ -395,7 +400,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     float lsum = 0.0f;
                     bool done = false;
                     // a row without an m has no measure yet for what it sees
-                    if (!__any_sync(0xffffffffu, m == -INFINITY && sees)) {
+                    if (settled || !__any_sync(0xffffffffu, m == -INFINITY && sees)) {
                         // probabilities under the m of the tiles before, unless their sum
                         // says that a score has passed it by far
                         const float ref = m == -INFINITY ? 0.0f : m;
@@ -451,6 +456,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                 m = top;
                             }
                         }
+                        settled = !__any_sync(0xffffffffu, m == -INFINITY);
                         const float ref = m == -INFINITY ? 0.0f : m;
                         float ls[2] = {0.0f, 0.0f};
 #pragma unroll
