@@ -646,17 +646,20 @@ INFERNT_API int infernt_paged_rope_append(void* q_out, int ldo, const void* q, i
  *   lse[r][h] = ln sum_p w_p
  * of KV head h / (nq / num_kv_heads).  scale >= 0; 0 means 1 / sqrt(head_dim).
  * q and out [num_rows][nq][head_dim] of the cache's type, rows ldq and ldo
- * elements apart (multiples of 8, pointers 16-byte aligned); lse [num_rows]
- * [nq] FP32 or NULL.  A row without a visible key gets zeros and an lse of
+ * elements apart (multiples of 8, pointers 16-byte aligned, out apart from
+ * q); lse [num_rows][nq] FP32 or NULL.  A row without a visible key gets zeros and an lse of
  * -infinity.  What lies in rows that a token does not see (unwritten rows of
  * a page, NaN, infinity) does not reach its output.  FP32 scores, softmax
  * statistics and sums; the probabilities enter the tensor cores in the
  * cache's type.  nq a multiple of num_kv_heads, at most 128 query heads per
  * KV head.
+ * Table entries of pages that no new token sees are not read, so pages behind
+ * a window may have been given back.
  * workspace: infernt_paged_attention_workspace_bytes() bytes, zeroed once
  * before its first use (calls leave its counters at zero; calls that share
  * it must not overlap, two captured graphs among them).  Asynchronous; may
- * be captured.  err as above; bit 0 if a bounded wait ran out. */
+ * be captured.  err as above; bit 0 if a bounded wait ran out: the results
+ * are then void, and the workspace has to be zeroed again. */
 INFERNT_API size_t infernt_paged_attention_workspace_bytes(void);
 INFERNT_API int infernt_paged_attention(void* out, int ldo, const void* q, int ldq, int nq,
                                         const infernt_paged_cache* cache, const infernt_ragged_batch* batch,

@@ -569,6 +569,7 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
                     "%s: rows %d and %d apart for %d heads of %d (multiples of 8)", op, ldq, ldo, nq, D);
     INFERNT_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace),
                     "%s: q, out and workspace must be 16-byte aligned", op);
+    INFERNT_REQUIRE(q != out, "%s: out may not be q", op);
     INFERNT_REQUIRE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "%s: window %d, sinks %d", op, window,
                     sinks);
     INFERNT_REQUIRE(std::isfinite(scale) && scale >= 0.0f, "%s: scale %g", op, scale);

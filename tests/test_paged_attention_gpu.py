@@ -184,6 +184,48 @@ def test_many_sequences(torch, ws, n):
     check_attention(c)
 
 
+def test_many_sequences_with_chunks(torch, ws):
+    """More sequences than a block has threads, some of them long enough for
+    the tensor cores' kernel, some with many blocks of rows."""
+    seqs = [(60 if i % 90 == 7 else 300 if i == 500 else 1, 1 + (i * 53) % 90) for i in range(900)]
+    seqs = [(a, max(a, b)) for a, b in seqs]
+    c = run(Case(torch, seqs, 4, 2, 64, 16, fill=math.nan), ws)
+    check_attention(c)
+
+
+@pytest.mark.parametrize("new", [1, 30, 200])
+@pytest.mark.parametrize("window,sinks", [(100, 5), (300, 0), (64, 70)])
+def test_pages_behind_a_window_are_not_read(torch, ws, new, window, sinks):
+    """Pages that only hold positions between the sinks and the window may
+    have been given back: their table entries mean nothing."""
+    c = Case(torch, [(new, 1500), (1, 40)], 8, 2, 64, 16)
+    first = max(0, 1500 - new - window + 1)
+    for i in range(first // 16):
+        if i * 16 >= sinks:
+            c.table[0, i] = -7
+    run(c, ws, window, sinks)
+    assert int(c.err) == 0
+    check_attention(c, window, sinks)
+
+
+def test_every_sequence_a_chunk(torch, ws):
+    """All sequences as long as the longest, so that one kernel has them all;
+    then the same rows with a shorter sequence among them."""
+    c = run(Case(torch, [(100, 130), (100, 1000), (100, 100)], 8, 2, 128, 32, fill=math.nan), ws)
+    check_attention(c, rows=[0, 1, 31, 32, 63, 64, 99])
+    c = run(Case(torch, [(100, 130), (7, 1000), (100, 100)], 8, 2, 128, 32, fill=math.nan), ws)
+    check_attention(c, rows=[0, 1, 6, 31, 32, 63, 64, 99])
+
+
+def test_the_workspace_is_left_for_the_next_call(torch):
+    """Counters are zero after calls that split items in either kernel."""
+    ws = new_workspace(torch)
+    for seqs in ([(1, 9000), (1, 4000)], [(300, 3000)], [(200, 2000), (1, 5000)]):
+        c = run(Case(torch, seqs, 8, 2, 128, 32), ws)
+        check_attention(c, rows=[0, 100, 199, 299])
+        assert not bool(ws[:2048].any()) and not bool(ws[24 << 20:(24 << 20) + 2048].any())
+
+
 def test_pages_shared_by_sequences(torch, ws):
     c = Case(torch, [(1, 100), (1, 100), (3, 90)], 8, 2, 64, 16)
     c.pages[1], c.pages[2] = c.pages[0], c.pages[0][:6] + [-1]

@@ -27,7 +27,7 @@ def batch(**kw):
     return b
 
 
-def attention(c=None, b=None, out=A, ldo=256, q=A, ldq=256, nq=4, window=0, sinks=0, scale=0.0, ws=A):
+def attention(c=None, b=None, out=2 * A, ldo=256, q=A, ldq=256, nq=4, window=0, sinks=0, scale=0.0, ws=A):
     return ib.lib().infernt_paged_attention(out, ldo, q, ldq, nq, ctypes.byref(c or cache()),
                                             ctypes.byref(b or batch()), window, sinks, scale, None, ws, None, None)
 
@@ -53,7 +53,7 @@ def test_bad_batches_are_refused(kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(out=None), dict(q=None), dict(ws=None), dict(q=A + 2), dict(out=A + 8), dict(ws=A + 4), dict(nq=0),
+    dict(out=None), dict(q=None), dict(out=A), dict(ws=None), dict(q=A + 2), dict(out=A + 8), dict(ws=A + 4), dict(nq=0),
     dict(nq=3), dict(nq=2 * 129), dict(ldq=255), dict(ldq=260), dict(ldo=248), dict(window=-1),
     dict(sinks=-1, window=4), dict(sinks=4), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(scale=-0.1), dict(b=batch(num_rows=1 << 29), nq=4),
@@ -249,9 +249,9 @@ def test_wrapper_checks():
     q = torch.zeros(4, 4, 64, dtype=torch.bfloat16)
     ws = torch.zeros(ib.paged_attention_workspace_bytes(), dtype=torch.uint8)
     for bad in (lambda: ib.paged_attention(q, q.half(), c, b, ws), lambda: ib.paged_attention(q[:2], q, c, b, ws),
-                lambda: ib.paged_attention(q, q.transpose(0, 1), c, b, ws),
-                lambda: ib.paged_attention(q, q, c, b, ws[:100]),
-                lambda: ib.paged_attention(q, q, c, b, ws, lse=torch.zeros(4, 3)),
+                lambda: ib.paged_attention(q.clone(), q.transpose(0, 1), c, b, ws),
+                lambda: ib.paged_attention(q.clone(), q, c, b, ws[:100]),
+                lambda: ib.paged_attention(q.clone(), q, c, b, ws, lse=torch.zeros(4, 3)),
                 lambda: ib.paged_rope_append(q, q, k[0, 0], k[0, 0], c, b, ib.RopeParams()),
                 lambda: ib.paged_rope_append(q.half(), q, None, None, c, b, ib.RopeParams()),
                 lambda: ib.copy_pages([k, k[:2]], [0], [1]), lambda: ib.copy_pages([k], [0], [1, 2])):
