@@ -42,6 +42,7 @@
 // with one pair in four (maximum searched: 578 without, 594 one in eight).
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include <cudaTypedefs.h>
 
@@ -370,21 +371,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     fence_proxy_async_smem();
                     mbar_arrive(&bar.q[x]);
                 }
-#pragma unroll 1
-                for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
-                    const int k0 = tile_key<kN>(it, part.j0 + i);
-                    const uint32_t b = n & 1u;
-                    tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
+                // One tile; in two copies, so that the tiles that every row of the item sees
+                // whole, most of a chunk's, run through code without a mask.
+                auto tile = [&](auto masked, int i, int k0, uint32_t b, bool all_lo) {
+                    constexpr bool MASKED = decltype(masked)::value;
                     float sv[kN];
                     tmem_ld64(tm_score(x, b) + lanes, sv);
-                    // keys that every row of the item sees need no mask
-                    const bool all_hi = k0 + kN - 1 <= it.pos_first;
-                    const bool all_lo = a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks;
-                    bool sees = true;  // whether this row sees one of them
-                    if (!(all_hi && all_lo)) {
+                    bool sees = true;  // whether this row sees one of the keys
+                    if (MASKED) {
                         const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sink = a.sinks - k0;
                         if (all_lo) {
 #pragma unroll
@@ -439,7 +433,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             // O must hold the products before it is rescaled
                             tc_wait_bar(&bar.o[x][b ^ 1], ((n - 1) >> 1) & 1u, ok);
                             ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) break;
+                            if (!ok) return;
                             tc_fence_after();
                             const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
 #pragma unroll 1
@@ -473,13 +467,29 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     if (D == 64 && i >= 2) {
                         tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
                         ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
+                        if (!ok) return;
                         tc_fence_after();
                     }
                     tmem_st32(tm_prob(x, b) + lanes, w);
                     tmem_st_wait();
                     tc_fence_before();
                     mbar_arrive(&bar.p[x][b]);
+                };
+#pragma unroll 1
+                for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
+                    const int k0 = tile_key<kN>(it, part.j0 + i);
+                    const uint32_t b = n & 1u;
+                    tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool all_hi = k0 + kN - 1 <= it.pos_first;
+                    const bool all_lo = a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks;
+                    if (all_hi && all_lo)
+                        tile(std::false_type(), i, k0, b, all_lo);
+                    else
+                        tile(std::true_type(), i, k0, b, all_lo);
+                    if (!ok) break;
                 }
                 tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
                 ok = __all_sync(0xffffffffu, ok);
