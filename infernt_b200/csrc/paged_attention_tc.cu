@@ -20,6 +20,10 @@
 // half of its scores that has been read, so S of tile i + 2 waits for P V of
 // tile i; at 64 it has columns of its own.
 //
+// Code that runs once a part is kept rolled: an instruction that is not yet
+// in the instruction cache costs about 20 cycles, so an unrolled epilogue took
+// 24000 cycles where its loads and stores need a quarter of that.
+//
 // Twelve warps: warp 0 loads K and V tiles page by page by TMA (a tensor map
 // of the pool [page][KV head][position][dim]; a page that no row sees, or that
 // the pool does not have, is a coordinate past its end and becomes zeros),
@@ -354,20 +358,25 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             float m = -INFINITY, l = 0.0f;  // m in base 2
             bool settled = false;           // every row of the warp has its m
             if (rows_x > 0 && part.j0 < part.j1) {
-                // Q rows of this warp: D / 8 lanes of 16 bytes a row, all in flight at once
+                // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
                 {
-                    uint4 w[LI];
+#pragma unroll 1
+                    for (int i0 = 0; i0 < LI; i0 += 8) {
+                        uint4 w[8];
 #pragma unroll
-                    for (int i = 0; i < LI; ++i) {
-                        // past the item's rows its last one again: no branch around a load
-                        const int qrow = it.row0 + 128 * x + min(32 * quarter + i * RPI + lane / CH, rows_x - 1);
-                        const int t = a.by_g(qrow);
-                        w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                                    (long long)(seq.row0 + t) * a.ldq +
-                                                                    (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
+                        for (int i = 0; i < 8; ++i) {
+                            // past the item's rows its last one again: no branch around a load
+                            const int qrow =
+                                it.row0 + 128 * x + min(32 * quarter + (i0 + i) * RPI + lane / CH, rows_x - 1);
+                            const int t = a.by_g(qrow);
+                            w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                                        (long long)(seq.row0 + t) * a.ldq +
+                                                                        (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            st_shared(own_chunk(32 * quarter + (i0 + i) * RPI + lane / CH, ch), w[i]);
                     }
-#pragma unroll
-                    for (int i = 0; i < LI; ++i) st_shared(own_chunk(32 * quarter + i * RPI + lane / CH, ch), w[i]);
                     fence_proxy_async_smem();
                     mbar_arrive(&bar.q[x]);
                 }
@@ -503,7 +512,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
                 float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
                 if (rows_x > 0) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
                         float o[32];
                         if (some) tmem_ld32(tm_ox + 32 * c, o);
@@ -547,45 +556,47 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 const bool sees = mine && pos >= 0;
                 const float inv = sees ? 1.0f / lsum : 0.0f;
                 bool bad = false;
-                // 64 columns at a time into the row tile's Q, which the products are done with
-#pragma unroll
-                for (int c = 0; c < D / 64; ++c) {
-                    float o[64];
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) o[e] = 0.0f;
+                // 32 columns at a time into the row tile's Q, which the products are done with
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    float o[32];
                     if (!split) {
-                        if (some) tmem_ld64(tm_ox + 64 * c, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                        if (some) tmem_ld32(tm_ox + 32 * c, o);
                     } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
 #pragma unroll 1
                         for (int b = part.first; b <= part.last; ++b) {
                             const float* p = slot_of<kM, D>(a, b, part.first);
-                            float v[64];
+                            const float mb = mine ? __ldcg(p + kM * D + ri) : -INFINITY;
+                            float v[32];
                             if (b == (int)blockIdx.x) {  // its own is still here
-                                tmem_ld64(tm_ox + 64 * c, v);
+                                tmem_ld32(tm_ox + 32 * c, v);
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) {
-                                    const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p) + (16 * c + e) * kM + ri);
+                                for (int e = 0; e < 8; ++e) {
+                                    const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
                                     v[4 * e] = f4.x;
                                     v[4 * e + 1] = f4.y;
                                     v[4 * e + 2] = f4.z;
                                     v[4 * e + 3] = f4.w;
                                 }
                             }
-                            const float mb = mine ? __ldcg(p + kM * D + ri) : -INFINITY;
                             const float f = mb == -INFINITY ? 0.0f : ex2(mb - M);
 #pragma unroll
-                            for (int e = 0; e < 64; ++e) o[e] = fmaf(v[e], f, o[e]);
+                            for (int e = 0; e < 32; ++e) o[e] = fmaf(v[e], f, o[e]);
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
+                    for (int e = 0; e < 32; ++e) {
                         o[e] = sees ? o[e] * inv : 0.0f;
                         bad |= !(fabsf(o[e]) < INFINITY);
                     }
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        st_shared(own_chunk(r, 8 * c + e),
+                    for (int e = 0; e < 4; ++e)
+                        st_shared(own_chunk(r, 4 * c + e),
                                   make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
                                              Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
                                              Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
@@ -593,7 +604,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 __syncwarp();
                 // whole rows by D / 8 lanes each
-#pragma unroll
+#pragma unroll 2
                 for (int i = 0; i < LI; ++i) {
                     const int rr = 32 * quarter + i * RPI + lane / CH, orow = it.row0 + 128 * x + rr;
                     if (rr < rows_x) {
