@@ -36,8 +36,8 @@
 // The probabilities of a tile are computed with the m of the tiles before,
 // with no search for their maximum: any m gives the same result, so long as
 // the probabilities fit their 16 bits, and a tile whose sum stays below 2^13
-// does.  Where it does not (and for a row's first keys) the tile is computed
-// again with its own maximum, and O is rescaled if that has
+// does.  Where it does not (and for first keys and hidden ones) the tile is
+// computed again with its own maximum, and O is rescaled if that has
 // passed m by more than 2^8.  One pair in eight takes 2^x on the FMA pipe
 // (nearest integer, then a polynomial of degree 4 on the rest): the special
 // function unit would otherwise be the longest path.  Both measured on 4096
@@ -46,7 +46,6 @@
 // with one pair in four (maximum searched: 578 without, 594 one in eight).
 #include <cmath>
 #include <cstdint>
-#include <type_traits>
 
 #include <cudaTypedefs.h>
 
@@ -113,14 +112,14 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
 // 2^x of a pair without the special function unit, for x <= 100: n = x to the
 // nearest integer by the addition of 3 x 2^22, 2^(x - n) by the polynomial of
 // least largest relative error on [-1/2, 1/2] (2.7e-6 in FP32), n added to its
-// exponent.  Below -126 (hidden keys' minus infinity among it) x becomes
-// -126.49, whose result is subnormal and flushed to 0.  NaN becomes NaN or
-// the largest number, and so the sum of a tile too large either way.
+// exponent.  Below -126 x becomes -126.49, whose result is subnormal.  NaN
+// becomes NaN or the largest number, and so the sum of a tile too large
+// either way.
 __device__ __forceinline__ float2 ex2_pair(F2 arg) {
     float2 v = un2(arg);
     asm("max.NaN.f32 %0, %0, 0fC2FCFAE1;" : "+f"(v.x));
     asm("max.NaN.f32 %0, %0, 0fC2FCFAE1;" : "+f"(v.y));
-    const F2 x = f2(v.x, v.y), one = f2(1.0f, 1.0f);
+    const F2 x = f2(v.x, v.y);
     const F2 big = f2(12582912.0f, 12582912.0f), less = f2(-12582912.0f, -12582912.0f), minus = f2(-1.0f, -1.0f);
     const F2 t = add2(x, big), f = fma2(add2(t, less), minus, x);
     F2 p = f2(0.009570102207362652f, 0.009570102207362652f);
@@ -129,9 +128,8 @@ __device__ __forceinline__ float2 ex2_pair(F2 arg) {
     p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
     p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
     const float2 n = un2(t), q = un2(p);
-    F2 r = f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
+    const F2 r = f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
               __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
-    asm("mul.rn.ftz.f32x2 %0, %0, %1;" : "+l"(r) : "l"(one));
     return un2(r);
 }
 
@@ -356,7 +354,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const bool mine = r < rows_x;
             const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
             float m = -INFINITY, l = 0.0f;  // m in base 2
-            bool settled = false;           // every row of the warp has its m
+            bool settled = false;           // every row of the warp has an m
             if (rows_x > 0 && part.j0 < part.j1) {
                 // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
                 {
@@ -380,34 +378,26 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     fence_proxy_async_smem();
                     mbar_arrive(&bar.q[x]);
                 }
-                // One tile; in two copies, so that the tiles that every row of the item sees
-                // whole, most of a chunk's, run through code without a mask.
-                auto tile = [&](auto masked, int i, int k0, uint32_t b, bool all_lo) {
-                    constexpr bool MASKED = decltype(masked)::value;
+#pragma unroll 1
+                for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
+                    const int k0 = tile_key<kN>(it, part.j0 + i);
+                    const uint32_t b = n & 1u;
+                    tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
                     float sv[kN];
                     tmem_ld64(tm_score(x, b) + lanes, sv);
-                    bool sees = true;  // whether this row sees one of the keys
-                    if (MASKED) {
-                        const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sink = a.sinks - k0;
-                        if (all_lo) {
-#pragma unroll
-                            for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
-                            sees = hi >= 0;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
-                            sees = hi >= 0 && (lo < kN - 1 || sink > 0);
-                        }
-                    }
+                    // keys that every row of the item sees need no mask
+                    const bool whole = k0 + kN - 1 <= it.pos_first &&
+                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
                     uint32_t w[kN / 2];
                     float lsum = 0.0f;
                     bool done = false;
-                    // a row without an m has no measure yet for what it sees
-                    if (settled || !__any_sync(0xffffffffu, m == -INFINITY && sees)) {
+                    if (whole && settled) {
                         // probabilities under the m of the tiles before, unless their sum
                         // says that a score has passed it by far
-                        const float ref = m == -INFINITY ? 0.0f : m;
-                        const F2 ref2 = f2(-ref, -ref);
+                        const F2 ref2 = f2(-m, -m);
                         F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
                         for (int e = 0; e < kN / 2; ++e) {
@@ -427,7 +417,18 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
                     }
                     if (!done) {
-                        // a row's first keys, and keys whose maximum moves m
+                        // a row's first keys, hidden keys, and keys whose maximum moves m
+                        if (!whole) {
+                            const int hi = pos - k0;
+                            if (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks) {
+#pragma unroll
+                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
+                            } else {
+                                const int lo = hi - a.window, sink = a.sinks - k0;
+#pragma unroll
+                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
+                            }
+                        }
                         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                         for (int e = 0; e < kN; e += 4) {
@@ -442,7 +443,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             // O must hold the products before it is rescaled
                             tc_wait_bar(&bar.o[x][b ^ 1], ((n - 1) >> 1) & 1u, ok);
                             ok = __all_sync(0xffffffffu, ok);
-                            if (!ok) return;
+                            if (!ok) break;
                             tc_fence_after();
                             const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
 #pragma unroll 1
@@ -476,29 +477,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     if (D == 64 && i >= 2) {
                         tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
                         ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) return;
+                        if (!ok) break;
                         tc_fence_after();
                     }
                     tmem_st32(tm_prob(x, b) + lanes, w);
                     tmem_st_wait();
                     tc_fence_before();
                     mbar_arrive(&bar.p[x][b]);
-                };
-#pragma unroll 1
-                for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
-                    const int k0 = tile_key<kN>(it, part.j0 + i);
-                    const uint32_t b = n & 1u;
-                    tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const bool all_hi = k0 + kN - 1 <= it.pos_first;
-                    const bool all_lo = a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks;
-                    if (all_hi && all_lo)
-                        tile(std::false_type(), i, k0, b, all_lo);
-                    else
-                        tile(std::true_type(), i, k0, b, all_lo);
-                    if (!ok) break;
                 }
                 tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
                 ok = __all_sync(0xffffffffu, ok);
