@@ -20,10 +20,6 @@
 // half of its scores that has been read, so S of tile i + 2 waits for P V of
 // tile i; at 64 it has columns of its own.
 //
-// Code that runs once a part is kept rolled: an instruction that is not yet
-// in the instruction cache costs about 20 cycles, so an unrolled epilogue took
-// 24000 cycles where its loads and stores need a quarter of that.
-//
 // Twelve warps: warp 0 loads K and V tiles page by page by TMA (a tensor map
 // of the pool [page][KV head][position][dim]; a page that no row sees, or that
 // the pool does not have, is a coordinate past its end and becomes zeros),
@@ -41,9 +37,9 @@
 // passed m by more than 2^8.  One pair in eight takes 2^x on the FMA pipe
 // (nearest integer, then a polynomial of degree 4 on the rest): the special
 // function unit would otherwise be the longest path.  Both measured on 4096
-// tokens at 12288 positions (32/8 heads of 128, bf16): 561 us; 594 with the
-// maximum searched beside the probabilities; 580 without the polynomial, 594
-// with one pair in four (maximum searched: 578 without, 594 one in eight).
+// tokens at 12288 positions (32/8 heads of 128, bf16), at the time: 561 us; 594
+// with the maximum searched beside the probabilities; 580 without the
+// polynomial.  Now 570 us, 1205 TFLOP/s; back to back, at the power limit, 673.
 #include <cmath>
 #include <cstdint>
 
@@ -358,7 +354,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             if (rows_x > 0 && part.j0 < part.j1) {
                 // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
                 {
-#pragma unroll 1
+#pragma unroll
                     for (int i0 = 0; i0 < LI; i0 += 8) {
                         uint4 w[8];
 #pragma unroll
@@ -497,7 +493,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
                 float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
                 if (rows_x > 0) {
-#pragma unroll 1
+#pragma unroll
                     for (int c = 0; c < D / 32; ++c) {
                         float o[32];
                         if (some) tmem_ld32(tm_ox + 32 * c, o);
@@ -542,7 +538,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 const float inv = sees ? 1.0f / lsum : 0.0f;
                 bool bad = false;
                 // 32 columns at a time into the row tile's Q, which the products are done with
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < D / 32; ++c) {
                     float o[32];
                     if (!split) {
@@ -589,7 +585,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 __syncwarp();
                 // whole rows by D / 8 lanes each
-#pragma unroll 2
+#pragma unroll
                 for (int i = 0; i < LI; ++i) {
                     const int rr = 32 * quarter + i * RPI + lane / CH, orow = it.row0 + 128 * x + rr;
                     if (rr < rows_x) {
