@@ -897,6 +897,10 @@ def _dtype(t):
     return d
 
 
+_struct_init = ctypes.Structure.__init__
+_byref = ctypes.byref
+
+
 class PagedCache(ctypes.Structure):
     """``infernt_paged_cache``: the K and V pools of one layer, contiguous
     tensors [num_pages][num_kv_heads][page_size][head_dim] of bfloat16 or
@@ -905,13 +909,16 @@ class PagedCache(ctypes.Structure):
                 ("dtype", _I)]
 
     def __init__(self, k, v):
-        shape, d = k.shape, _dtype(k)
-        if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.get_device() != k.get_device():
-            raise ValueError("PagedCache: k %s %s, v %s %s" % (tuple(shape), k.dtype, tuple(v.shape), v.dtype))
-        if not (k.is_contiguous() and v.is_contiguous()) or d < 0:
+        shape, t = k.shape, k.dtype
+        d = _TORCH_DTYPES.get(t)
+        if d is None:
+            d = _dtype(k)
+        if len(shape) != 4 or v.shape != shape or v.dtype != t or v.get_device() != k.get_device():
+            raise ValueError("PagedCache: k %s %s, v %s %s" % (tuple(shape), t, tuple(v.shape), v.dtype))
+        if d < 0 or not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("PagedCache: the pools must be contiguous, of a floating type")
-        super().__init__(k.data_ptr(), v.data_ptr(), *shape, d)
-        self.tensors = (k, v)
+        _struct_init(self, k.data_ptr(), v.data_ptr(), *shape, d)
+        self.tensors = k, v
 
 
 class RaggedBatch(ctypes.Structure):
@@ -922,15 +929,15 @@ class RaggedBatch(ctypes.Structure):
                 ("max_q_len", _I), ("table_stride", _I)]
 
     def __init__(self, q_start, kv_len, block_table, num_rows, max_q_len):
-        n, shape = kv_len.numel(), block_table.shape
-        if q_start.numel() != n + 1 or len(shape) != 2 or shape[0] != n:
+        n, shape, t = kv_len.numel(), block_table.shape, kv_len.dtype
+        if len(shape) != 2 or shape[0] != n or q_start.numel() != n + 1:
             raise ValueError("RaggedBatch: %d starts, %d lengths, table %s" % (q_start.numel(), n, tuple(shape)))
-        for t in (q_start, kv_len, block_table):
-            if _dtype(t) != -1 or not t.is_contiguous():
-                raise ValueError("RaggedBatch: contiguous int32 tensors are needed")
-        super().__init__(q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), n, num_rows, max_q_len,
-                         shape[1])
-        self.tensors = (q_start, kv_len, block_table)
+        if _dtype(kv_len) != -1 or q_start.dtype != t or block_table.dtype != t or not (
+                q_start.is_contiguous() and kv_len.is_contiguous() and block_table.is_contiguous()):
+            raise ValueError("RaggedBatch: contiguous int32 tensors are needed")
+        _struct_init(self, q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), n, num_rows, max_q_len,
+                     shape[1])
+        self.tensors = q_start, kv_len, block_table
 
 
 ROPE_SCALINGS = {"none": 0, "linear": 1, "llama3": 2, "yarn": 3}
@@ -947,20 +954,19 @@ class RopeParams(ctypes.Structure):
         code = ROPE_SCALINGS.get(scaling)
         if code is None:
             raise ValueError("RopeParams: scaling %r (%s)" % (scaling, ", ".join(ROPE_SCALINGS)))
-        super().__init__(theta, rotary_dim, bool(interleaved), code, original_max_len, factor, low, high)
+        _struct_init(self, theta, rotary_dim, bool(interleaved), code, original_max_len, factor, low, high)
 
 
 def _rows(t, rows, heads, dim, what):
     """Row stride of a [rows][heads][dim] tensor whose heads lie next to each
     other (a slice of stacked rows, for one)."""
-    shape = t.shape
-    if len(shape) != 3 or shape[0] < rows or shape[1] != heads or shape[2] != dim:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or shape[0] < rows:
         raise ValueError("%s: shape %s for %d rows of %d heads of %d" % (what, tuple(shape), rows, heads, dim))
-    r, h, e = t.stride()
-    if e != 1 or (h != dim and heads > 1):
-        raise ValueError("%s: strides %s; only rows may be apart" % (what, t.stride()))
+    if strides[2] != 1 or (strides[1] != dim and heads > 1):
+        raise ValueError("%s: strides %s; only rows may be apart" % (what, strides))
     # one row has no stride of its own
-    return r if shape[0] > 1 else max(r, heads * dim)
+    return strides[0] if shape[0] > 1 else max(strides[0], heads * dim)
 
 
 def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
@@ -976,12 +982,15 @@ def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None)
         if _dtype(q_out) != cache.dtype:
             raise ValueError("paged_rope_append: q_out has another type than the cache")
     if k is not None:
-        nkv, kp, vp = cache.num_kv_heads, k.data_ptr(), v.data_ptr()
+        nkv, kp, vp, t = cache.num_kv_heads, k.data_ptr(), v.data_ptr(), k.dtype
         ldk, ldv = _rows(k, n, nkv, dim, "k"), _rows(v, n, nkv, dim, "v")
-        if k.dtype != v.dtype or (src is not None and src != k.dtype):
+        if v.dtype != t or (src is not None and src != t):
             raise ValueError("paged_rope_append: q, k and v of different types")
-    call("infernt_paged_rope_append", op, ldo, qp, ldq, nq, kp, ldk, vp, ldv, _dtype(q if k is None else k),
-         ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(rope), ptr(err), stream)
+    status = (_lib or lib()).infernt_paged_rope_append(
+        op, ldo, qp, ldq, nq, kp, ldk, vp, ldv, _dtype(q if k is None else k), _byref(cache), _byref(batch),
+        _byref(rope), None if err is None else err.data_ptr(), stream)
+    if status:
+        check(status, "infernt_paged_rope_append")
 
 
 _workspace_bytes = 0
@@ -998,18 +1007,20 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
     """Attention of the batch's new tokens over the pages
     (infernt_paged_attention).  workspace: a zeroed tensor of
     paged_attention_workspace_bytes() bytes."""
-    n, dim, nq = batch.num_rows, cache.head_dim, q.shape[1]
+    n, dim, nq, lp = batch.num_rows, cache.head_dim, q.shape[1], None
     if _dtype(q) != cache.dtype or q.dtype != out.dtype:
         raise ValueError("paged_attention: q, out and the cache must have one type")
     if lse is not None:
-        shape = lse.shape
+        shape, lp = lse.shape, lse.data_ptr()
         if len(shape) != 2 or shape[1] != nq or shape[0] < n or _dtype(lse) != DTYPE_F32 or not lse.is_contiguous():
             raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(shape), n, nq))
-    if workspace.nbytes < paged_attention_workspace_bytes():
+    if workspace.nbytes < (_workspace_bytes or paged_attention_workspace_bytes()):
         raise ValueError("paged_attention: a workspace of %d bytes is needed" % paged_attention_workspace_bytes())
-    call("infernt_paged_attention", out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(),
-         _rows(q, n, nq, dim, "q"), nq, ctypes.byref(cache), ctypes.byref(batch), window, sinks, scale, ptr(lse),
-         workspace.data_ptr(), ptr(err), stream)
+    status = (_lib or lib()).infernt_paged_attention(
+        out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(), _rows(q, n, nq, dim, "q"), nq, _byref(cache),
+        _byref(batch), window, sinks, scale, lp, workspace.data_ptr(), None if err is None else err.data_ptr(), stream)
+    if status:
+        check(status, "infernt_paged_attention")
 
 
 def copy_pages(pools, src, dst, stream=None):
