@@ -275,16 +275,22 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         }
                     } else {
                         tc_wait_bar(&bar.q[x], parts++ & 1u, ok);
-                        // round i: P V of tile i - 2, then S of tile i over its columns
+                        // round i: P V of tile i - 2 and S of tile i.  At head_dim 128 S goes over
+                        // P's columns, after P V; at 64 S, for which rows wait, goes first.
 #pragma unroll 1
                         for (int i = 0; i < tiles + 2 && ok; ++i) {
                             const uint32_t b = (nx + i) & 1u, turn = ((nx + i - 2) >> 1) & 1u, m = n + i - 2;
+                            if (i >= 2) tc_wait_bar(&bar.p[x][b], turn, ok);
+                            if (D == 64 && i < tiles) {
+                                tc_wait_bar(&bar.full_k[(n + i) % ST], ((n + i) / ST) & 1u, ok);
+                                if (!ok) break;
+                                scores(n + i, b);
+                            }
                             if (i >= 2) {
                                 const uint32_t st = m % ST;
                                 const uint64_t v = tc_desc_mn(base + L::kV + st * L::kTile, kBox);
                                 tc_wait_bar(&bar.full_v[st], (m / ST) & 1u, ok);
                                 tc_wait_bar(&bar.clean_v[st], (m / ST) & 1u, ok);
-                                tc_wait_bar(&bar.p[x][b], turn, ok);
                                 if (!ok) break;
                                 tc_fence_after();
 #pragma unroll
@@ -294,9 +300,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                 tc_commit_to(&bar.o[x][b]);
                                 tc_commit_to(&bar.empty_v[st]);
                             }
-                            if (i < tiles) {
+                            if (D == 128 && i < tiles) {
                                 tc_wait_bar(&bar.full_k[(n + i) % ST], ((n + i) / ST) & 1u, ok);
-                                if (D == 128 && i >= 2) tc_wait_bar(&bar.o[x][b], turn, ok);
+                                if (i >= 2) tc_wait_bar(&bar.o[x][b], turn, ok);
                                 if (!ok) break;
                                 scores(n + i, b);
                             }
