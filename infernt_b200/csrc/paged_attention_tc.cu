@@ -34,12 +34,14 @@
 // the probabilities fit their 16 bits, and a tile whose sum stays below 2^13
 // does.  Where it does not (and for first keys and hidden ones) the tile is
 // computed again with its own maximum, and O is rescaled if that has
-// passed m by more than 2^8.  One pair in eight takes 2^x on the FMA pipe
-// (nearest integer, then a polynomial of degree 4 on the rest): the special
-// function unit would otherwise be the longest path.  Both measured on 4096
-// tokens at 12288 positions (32/8 heads of 128, bf16), at the time: 561 us; 594
-// with the maximum searched beside the probabilities; 580 without the
-// polynomial.  Now 570 us, 1205 TFLOP/s; back to back, at the power limit, 673.
+// passed m by more than 2^8.  P goes to TMEM eight columns at a time.
+//
+// 4096 tokens at 12288 positions (32/8 heads of 128, bf16): 541 us, 1271
+// TFLOP/s (632 us back to back, at the power limit); 594 with the maximum
+// searched beside the probabilities, 559 with P stored as a whole.  The
+// tensor pipe is busy for 80 % of it; a part of the 2^x on the FMA pipe
+// instead of the special function unit changes nothing any more, nor do
+// turns at the exponentials between the warps of a scheduler (622 us).
 #include <cmath>
 #include <cstdint>
 
@@ -103,30 +105,6 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
     F2 r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
-}
-
-// 2^x of a pair without the special function unit, for x <= 100: n = x to the
-// nearest integer by the addition of 3 x 2^22, 2^(x - n) by the polynomial of
-// least largest relative error on [-1/2, 1/2] (2.7e-6 in FP32), n added to its
-// exponent.  Below -126 x becomes -126.49, whose result is subnormal.  NaN
-// becomes NaN or the largest number, and so the sum of a tile too large
-// either way.
-__device__ __forceinline__ float2 ex2_pair(F2 arg) {
-    float2 v = un2(arg);
-    asm("max.NaN.f32 %0, %0, 0fC2FCFAE1;" : "+f"(v.x));
-    asm("max.NaN.f32 %0, %0, 0fC2FCFAE1;" : "+f"(v.y));
-    const F2 x = f2(v.x, v.y);
-    const F2 big = f2(12582912.0f, 12582912.0f), less = f2(-12582912.0f, -12582912.0f), minus = f2(-1.0f, -1.0f);
-    const F2 t = add2(x, big), f = fma2(add2(t, less), minus, x);
-    F2 p = f2(0.009570102207362652f, 0.009570102207362652f);
-    p = fma2(p, f, f2(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, f2(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
-    const float2 n = un2(t), q = un2(p);
-    const F2 r = f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)),
-              __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
-    return un2(r);
 }
 
 // Whether the tile at key k0 has keys that no row of the item sees.
@@ -393,7 +371,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     // keys that every row of the item sees need no mask
                     const bool whole = k0 + kN - 1 <= it.pos_first &&
                                        (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
-                    uint32_t w[kN / 2];
+                    // at head_dim 64 P's columns are free once P V of two tiles ago is done
+                    if (D == 64 && i >= 2) {
+                        tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        tc_fence_after();
+                    }
+                    const uint32_t tm_px = tm_prob(x, b) + lanes;
                     float lsum = 0.0f;
                     bool done = false;
                     if (whole && settled) {
@@ -402,23 +387,24 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         const F2 ref2 = f2(-m, -m);
                         F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
-                        for (int e = 0; e < kN / 2; ++e) {
-                            const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
-                            float2 p;
-                            if ((e & 7) == 7) {
-                                p = ex2_pair(arg);
-                            } else {
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 8 * c; e < 8 * c + 8; ++e) {
+                                const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
                                 const float2 v = un2(arg);
-                                p = make_float2(ex2(v.x), ex2(v.y));
+                                const float p0 = ex2(v.x), p1 = ex2(v.y);
+                                ls[e & 1] = add2(ls[e & 1], f2(p0, p1));
+                                w[e & 7] = Half16<T>::pack(p0, p1);
                             }
-                            ls[e & 1] = add2(ls[e & 1], f2(p.x, p.y));
-                            w[e] = Half16<T>::pack(p.x, p.y);
+                            tmem_st8(tm_px + 8 * c, w);
                         }
                         const float2 v = un2(add2(ls[0], ls[1]));
                         lsum = v.x + v.y;
                         done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
                     }
                     if (!done) {
+                        tmem_st_wait();  // the stores that are made again
                         // a row's first keys, hidden keys, and keys whose maximum moves m
                         if (!whole) {
                             const int hi = pos - k0;
@@ -451,6 +437,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll 1
                             for (int c = 0; c < D / 32; ++c) {
                                 float o[32];
+                                uint32_t w[32];
                                 tmem_ld32(tm_ox + 32 * c, o);
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
@@ -466,23 +453,20 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         const float ref = m == -INFINITY ? 0.0f : m;
                         float ls[2] = {0.0f, 0.0f};
 #pragma unroll
-                        for (int e = 0; e < kN / 2; ++e) {
-                            const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
-                            ls[0] += p0;
-                            ls[1] += p1;
-                            w[e] = Half16<T>::pack(p0, p1);
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[8];
+#pragma unroll
+                            for (int e = 8 * c; e < 8 * c + 8; ++e) {
+                                const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
+                                ls[0] += p0;
+                                ls[1] += p1;
+                                w[e & 7] = Half16<T>::pack(p0, p1);
+                            }
+                            tmem_st8(tm_px + 8 * c, w);
                         }
                         lsum = ls[0] + ls[1];
                     }
                     l += lsum;
-                    // at head_dim 64 P's columns are free once P V of two halves ago is done
-                    if (D == 64 && i >= 2) {
-                        tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        tc_fence_after();
-                    }
-                    tmem_st32(tm_prob(x, b) + lanes, w);
                     tmem_st_wait();
                     tc_fence_before();
                     mbar_arrive(&bar.p[x][b]);
