@@ -965,8 +965,7 @@ def _rows(t, rows, heads, dim, what):
         raise ValueError("%s: shape %s for %d rows of %d heads of %d" % (what, tuple(shape), rows, heads, dim))
     if strides[2] != 1 or (strides[1] != dim and heads > 1):
         raise ValueError("%s: strides %s; only rows may be apart" % (what, strides))
-    # one row has no stride of its own
-    return strides[0] if shape[0] > 1 else max(strides[0], heads * dim)
+    return strides[0] if shape[0] > 1 else heads * dim  # one row has no stride of its own
 
 
 def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
@@ -1031,11 +1030,15 @@ def copy_pages(pools, src, dst, stream=None):
     if n != len(dst):
         raise ValueError("copy_pages: %d sources, %d destinations" % (n, len(dst)))
     if isinstance(pools, (list, tuple)):
+        if not pools:
+            raise ValueError("copy_pages: no pools")
         first, count = pools[0], len(pools)
-        if any(p.shape != first.shape or p.dtype != first.dtype or not p.is_contiguous() for p in pools):
-            raise ValueError("copy_pages: the pools must be contiguous tensors of one shape and type")
+        shape, dtype, device = first.shape, first.dtype, first.get_device()
+        if any(p.shape != shape or p.dtype != dtype or p.get_device() != device or not p.is_contiguous()
+               for p in pools):
+            raise ValueError("copy_pages: the pools must be contiguous tensors of one shape, type and device")
         base = [p.data_ptr() for p in pools]
-        pages, size = first.shape[0], first.nbytes
+        pages, size = shape[0], first.nbytes
     else:
         if not pools.is_contiguous() or pools.dim() < 3:
             raise ValueError("copy_pages: a contiguous tensor [pools][pages][...] is needed")

@@ -117,8 +117,9 @@ inline int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& set_
 // Argument checks that the operators share (paged_rope.cu).
 int check_paged_cache(const char* op, const infernt_paged_cache* c);
 int check_ragged_batch(const char* op, const infernt_ragged_batch* b);
-// p must be memory that the current device reads in place.
+// p (or NULL) must be memory that the current device reads in place.
 int check_device_pointer(const char* op, const char* what, const void* p);
+int check_batch_pointers(const char* op, const infernt_paged_cache* c, const infernt_ragged_batch* b, const void* err);
 
 inline PagedBatch paged_batch(const infernt_paged_cache& c, const infernt_ragged_batch& b) {
     PagedBatch r;

@@ -569,6 +569,8 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
                     "%s: rows %d and %d apart for %d heads of %d (multiples of 8)", op, ldq, ldo, nq, D);
     INFERNT_REQUIRE(aligned16(q) && aligned16(out) && aligned16(workspace),
                     "%s: q, out and workspace must be 16-byte aligned", op);
+    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(lse) % 4 == 0 && reinterpret_cast<uintptr_t>(err) % 4 == 0,
+                    "%s: misaligned lse or err", op);
     INFERNT_REQUIRE(q != out, "%s: out may not be q", op);
     INFERNT_REQUIRE(window >= 0 && sinks >= 0 && (window > 0 || sinks == 0), "%s: window %d, sinks %d", op, window,
                     sinks);
@@ -583,9 +585,11 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
                     "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
                     most_kv);
     if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
-    if (int s = check_device_pointer(op, "the cache", cache->k)) return s;
+    if (int s = check_batch_pointers(op, cache, batch, err)) return s;
     if (int s = check_device_pointer(op, "q", q)) return s;
     if (int s = check_device_pointer(op, "out", out)) return s;
+    if (int s = check_device_pointer(op, "lse", lse)) return s;
+    if (int s = check_device_pointer(op, "workspace", workspace)) return s;
     AttnArgs a;
     a.b = paged_batch(*cache, *batch);
     a.q = q;

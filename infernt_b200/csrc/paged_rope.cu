@@ -38,16 +38,28 @@ int check_ragged_batch(const char* op, const infernt_ragged_batch* b) {
                     b->max_q_len, b->table_stride);
     INFERNT_REQUIRE(b->num_seqs == 0 || (b->q_start && b->kv_len && (b->block_table || b->table_stride == 0)),
                     "%s: null batch array", op);
+    for (const int* p : {b->q_start, b->kv_len, b->block_table})
+        INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(p) % sizeof(int) == 0, "%s: misaligned batch array", op);
     return INFERNT_OK;
 }
 
 int check_device_pointer(const char* op, const char* what, const void* p) {
+    if (!p) return INFERNT_OK;
     cudaPointerAttributes at;
     INFERNT_CUDA_TRY(cudaPointerGetAttributes(&at, p));
     INFERNT_REQUIRE(at.type == cudaMemoryTypeManaged ||
                         (at.type == cudaMemoryTypeDevice && at.device == current_device()),
                     "%s: %s is not memory of the current device", op, what);
     return INFERNT_OK;
+}
+
+int check_batch_pointers(const char* op, const infernt_paged_cache* c, const infernt_ragged_batch* b, const void* err) {
+    if (int s = check_device_pointer(op, "the K pool", c->k)) return s;
+    if (int s = check_device_pointer(op, "the V pool", c->v)) return s;
+    if (int s = check_device_pointer(op, "q_start", b->q_start)) return s;
+    if (int s = check_device_pointer(op, "kv_len", b->kv_len)) return s;
+    if (int s = check_device_pointer(op, "block_table", b->block_table)) return s;
+    return check_device_pointer(op, "err", err);
 }
 
 namespace {
@@ -393,13 +405,17 @@ extern "C" int infernt_paged_rope_append(void* q_out, int ldo, const void* q, in
     const unsigned esize = src_dtype == INFERNT_DTYPE_F32 ? 4u : 2u;
     for (const void* p : {q, k, v})
         INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(p) % esize == 0, "%s: misaligned source", op);
-    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(q_out) % 2 == 0, "%s: misaligned q_out", op);
+    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(q_out) % 2 == 0 && reinterpret_cast<uintptr_t>(err) % 4 == 0,
+                    "%s: misaligned q_out or err", op);
     RopeArgs a;
     RopeDev d;
     if (int s = rope_frequencies(*rope, D, &d)) return s;
     if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
-    if (int s = check_device_pointer(op, "the cache", cache->k)) return s;
-    if (int s = check_device_pointer(op, q ? "q" : "k", q ? q : k)) return s;
+    if (int s = check_batch_pointers(op, cache, batch, err)) return s;
+    if (int s = check_device_pointer(op, "q", q)) return s;
+    if (int s = check_device_pointer(op, "q_out", q_out)) return s;
+    if (int s = check_device_pointer(op, "k", k)) return s;
+    if (int s = check_device_pointer(op, "v", v)) return s;
     a.b = paged_batch(*cache, *batch);
     a.q = q;
     a.k = k;

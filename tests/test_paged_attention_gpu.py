@@ -273,12 +273,23 @@ def test_sequences_out_of_range_are_skipped(torch, ws, what):
 
 
 def test_host_memory_is_refused(torch, ws):
-    c = Case(torch, [(1, 10)], 4, 2, 64, 16)
-    cpu = c.q.cpu()
-    with pytest.raises(ib.InferntError):
-        ib.paged_attention(c.out, cpu, c.cache(), c.batch(), ws)
-    with pytest.raises(ib.InferntError):
-        ib.paged_attention(c.out, c.q, ib.PagedCache(c.k.cpu(), c.v.cpu()), c.batch(), ws)
+    c = Case(torch, [(1, 10), (2, 20)], 4, 2, 64, 16)
+    cache, batch = c.cache(), c.batch()
+    cpu = {k: getattr(c, k).cpu() for k in ("q", "out", "lse", "k", "v", "q_start", "kv_len", "table", "err")}
+    with_cpu = ib.RaggedBatch
+    for call in (lambda: ib.paged_attention(c.out, cpu["q"], cache, batch, ws),
+                 lambda: ib.paged_attention(cpu["out"], c.q, cache, batch, ws),
+                 lambda: ib.paged_attention(c.out, c.q, cache, batch, ws, lse=cpu["lse"]),
+                 lambda: ib.paged_attention(c.out, c.q, cache, batch, ws, err=cpu["err"]),
+                 lambda: ib.paged_attention(c.out, c.q, cache, batch, ws.cpu()),
+                 lambda: ib.paged_attention(c.out, c.q, ib.PagedCache(cpu["k"], cpu["v"]), batch, ws),
+                 lambda: ib.paged_attention(c.out, c.q, cache, with_cpu(cpu["q_start"], c.kv_len, c.table, 3, 2), ws),
+                 lambda: ib.paged_attention(c.out, c.q, cache, with_cpu(c.q_start, cpu["kv_len"], c.table, 3, 2), ws),
+                 lambda: ib.paged_attention(c.out, c.q, cache, with_cpu(c.q_start, c.kv_len, cpu["table"], 3, 2), ws)):
+        with pytest.raises(ib.InferntError):
+            call()
+    run(c, ws)
+    check_attention(c)
 
 
 def test_two_streams_with_their_own_workspaces(torch, ws):

@@ -63,6 +63,21 @@ def test_bad_attention_arguments_are_refused(kw):
     assert ib.lib().infernt_last_error() != b""
 
 
+@pytest.mark.parametrize("field", ["q_start", "kv_len", "block_table"])
+def test_misaligned_batch_arrays_are_refused(field):
+    assert attention(b=batch(**{field: A + 2})) == 1
+    assert rope(b=batch(**{field: A + 2})) == 1
+
+
+def test_misaligned_lse_and_err_are_refused():
+    f, c, b = ib.lib().infernt_paged_attention, ctypes.byref(cache()), ctypes.byref(batch())
+    for lse, err in ((A + 2, None), (None, A + 1), (None, A + 2)):
+        assert f(2 * A, 256, A, 256, 4, c, b, 0, 0, 0.0, lse, A, err, None) == 1
+    p = ib.RopeParams(rotary_dim=64)
+    assert ib.lib().infernt_paged_rope_append(A, 256, A, 256, 4, A, 128, A, 128, ib.DTYPE_BF16, c, b, ctypes.byref(p),
+                                              A + 2, None) == 1
+
+
 def test_empty_batches_are_no_work():
     assert attention(b=batch(num_seqs=0)) == 0
     assert attention(b=batch(num_rows=0)) == 0
@@ -254,6 +269,7 @@ def test_wrapper_checks():
                 lambda: ib.paged_attention(q.clone(), q, c, b, ws, lse=torch.zeros(4, 3)),
                 lambda: ib.paged_rope_append(q, q, k[0, 0], k[0, 0], c, b, ib.RopeParams()),
                 lambda: ib.paged_rope_append(q.half(), q, None, None, c, b, ib.RopeParams()),
-                lambda: ib.copy_pages([k, k[:2]], [0], [1]), lambda: ib.copy_pages([k], [0], [1, 2])):
+                lambda: ib.copy_pages([k, k[:2]], [0], [1]), lambda: ib.copy_pages([k], [0], [1, 2]),
+                lambda: ib.copy_pages([], [0], [1])):
         with pytest.raises(ValueError):
             bad()

@@ -269,3 +269,13 @@ def test_captured_call_and_side_stream(torch):
     g.replay()
     torch.cuda.synchronize()
     r.check()
+
+
+def test_host_memory_is_refused(torch):
+    r = Rope(torch, [(2, 20)], 4, 2, 64, 16)
+    cache, batch, p = r.c.cache(), r.c.batch(), ib.RopeParams(**r.params)
+    for q_out, q, k, v in ((r.q_out.cpu(), r.q, r.kn, r.vn), (r.q_out, r.q.cpu(), r.kn, r.vn),
+                           (r.q_out, r.q, r.kn.cpu(), r.vn), (r.q_out, r.q, r.kn, r.vn.cpu())):
+        with pytest.raises(ib.InferntError):
+            ib.paged_rope_append(q_out, q, k, v, cache, batch, p)
+    r.run().check()

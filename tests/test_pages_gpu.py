@@ -71,6 +71,8 @@ def test_captured_copy_keeps_its_list(torch):
 def test_host_memory_is_refused(torch):
     with pytest.raises(ib.InferntError):
         ib.copy_pages(torch.zeros(2, 4, 16), [0], [1])
+    with pytest.raises(ValueError):
+        ib.copy_pages([torch.zeros(4, 16, device="cuda"), torch.zeros(4, 16)], [0], [1])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
