@@ -31,8 +31,8 @@ struct AttnArgs {
     FastDiv by_g;
     float scale, scale_log2;
     int min_rows, max_rows;  // a sequence of min_rows query rows or fewer, or more than max_rows, is another kernel's
-    int min_units;      // least units of a CTA
-    unsigned* tickets;  // [CTAs], zero between calls
+    int min_units;           // least units of a CTA
+    unsigned* tickets;       // [CTAs], zero between calls
     float* slots;
     unsigned* err;
 };
@@ -327,7 +327,8 @@ __device__ __noinline__ void exact_row(const AttnArgs& a, const PagedSeq& seq, i
 #pragma unroll
         for (int e = 0; e < E; ++e) dot = fmaf(qv[e], r >= 0 ? Half16<T>::value(k[e]) : 0.0f, dot);
         const float sc = warp_sum(dot) * a.scale, m_new = fmaxf(m, sc);
-        const float f = m == -INFINITY ? 0.0f : expf(m - m_new), w = expf(sc - m_new);
+        // e^-infinity is 0, before the row has met a finite score too
+        const float f = m == -INFINITY ? 0.0f : expf(m - m_new), w = sc == -INFINITY ? 0.0f : expf(sc - m_new);
         l = l * f + w;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + w * (r >= 0 ? Half16<T>::value(v[e]) : 0.0f);

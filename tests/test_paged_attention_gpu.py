@@ -7,7 +7,7 @@ import math
 import pytest
 
 import infernt_b200 as ib
-from paged_reference import Case, check_attention, new_workspace
+from paged_reference import HALF_STEP, Case, attention_row, check_attention, new_workspace
 
 pytestmark = pytest.mark.gpu
 
@@ -136,6 +136,28 @@ def test_scores_that_are_not_finite(torch, ws, bad):
         run(c, ws)
         assert not bool(torch.isfinite(c.out[:, 2:].float()).any()), at
         assert bool(torch.isfinite(c.out[:, :2].float()).all()), at
+
+
+@pytest.mark.parametrize("new", [2, 100])
+def test_a_first_score_of_minus_infinity(torch, ws, new):
+    """Position 0 has no weight where its score is -infinity, also in rows
+    whose tile holds a hidden value that is not finite."""
+    n = 150
+    c = Case(torch, [(new, n)], 4, 2, 64, 16)
+    c.q.abs_().add_(0.1)
+    c.k[c.pages[0][0], :, 0] = -math.inf
+    c.v[c.pages[0][(n - 1) // 16], :, (n - 1) % 16] = math.nan
+    run(c, ws)
+    k, v = c.dense(c.k, 0)[1:], c.dense(c.v, 0)[1:]
+    for i in range(new - 1):
+        pos = n - new + i
+        out, lse, big, vmax = attention_row(c, c.q[i], k, v, pos - 1, 0, 0, 0.125)
+        es = (64 + 2) * 2.0 ** -23 * 0.125 * big  # as in check_attention
+        assert float((c.out[i].double() - out).abs().amax()) <= vmax * (2 * HALF_STEP["bf16"] + 4 * es +
+                                                                       (pos + 65) * 2.0 ** -22), i
+        far = (c.lse[i].double() - lse).abs()
+        assert bool((far <= es + (pos + 9) * 2.0 ** -22 + 2.0 ** -21 * lse.abs()).all()), i
+    assert bool(torch.isnan(c.out[new - 1]).all())
 
 
 def test_hidden_by_a_window(torch, ws):
