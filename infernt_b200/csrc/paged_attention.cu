@@ -581,7 +581,8 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
     const bool chunks = paged_attention_boxes(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
     const long long tile_m = chunks ? kTcItemRows : kItemRows, tile_n = chunks ? kTcTileKeys : kTileKeys;
-    INFERNT_REQUIRE(((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv < (1ll << 30) / (most_kv / tile_n + 2 + kItemCost),
+    const long long items = ((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv;
+    INFERNT_REQUIRE(items < (1ll << 30) / (most_kv / tile_n + 2 + kItemCost),
                     "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
                     most_kv);
     if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;

@@ -130,7 +130,8 @@ __device__ __forceinline__ void zero_rows(const Item& it, int k0, uint32_t v) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreadsTc, 1)
-    paged_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    paged_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v) {
     using L = LayoutTc<D>;
     constexpr int NB = (int)L::kBlocks, ST = L::kStages;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -172,49 +173,49 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
         if (warp == 0 && place.s >= 0) {
-        // ---- K and V tiles.  n: tiles so far, over all parts.
-        uint32_t n = 0;
-        const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
-        walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
-            for (int j = part.j0; j < part.j1; ++j, ++n) {
-                const int k0 = tile_key<kN>(it, j), st = (int)(n % ST);
-                const uint32_t turn = (n / ST) & 1u;
-                // the page of lane l's rows [k0 + l box_rows, + box_rows)
-                int page = a.b.num_pages, row = 0;
-                if (lane < per_tile) {
-                    const int p0 = k0 + lane * box_rows, pi = a.b.by_page(p0);
-                    row = p0 - pi * ps;
-                    // whether some row sees a key of the box
-                    if (p0 < it.hi && (p0 + box_rows > it.lo || p0 < it.sink_end)) {
-                        page = a.b.table[(size_t)part.s * a.b.table_stride + pi];
-                        if (page < 0 || page >= a.b.num_pages) {
-                            if (a.err) atomicOr(a.err, kErrPage);
-                            page = a.b.num_pages;
+            // ---- K and V tiles.  n: tiles so far, over all parts.
+            uint32_t n = 0;
+            const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
+            walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+                for (int j = part.j0; j < part.j1; ++j, ++n) {
+                    const int k0 = tile_key<kN>(it, j), st = (int)(n % ST);
+                    const uint32_t turn = (n / ST) & 1u;
+                    // the page of lane l's rows [k0 + l box_rows, + box_rows)
+                    int page = a.b.num_pages, row = 0;
+                    if (lane < per_tile) {
+                        const int p0 = k0 + lane * box_rows, pi = a.b.by_page(p0);
+                        row = p0 - pi * ps;
+                        // whether some row sees a key of the box
+                        if (p0 < it.hi && (p0 + box_rows > it.lo || p0 < it.sink_end)) {
+                            page = a.b.table[(size_t)part.s * a.b.table_stride + pi];
+                            if (page < 0 || page >= a.b.num_pages) {
+                                if (a.err) atomicOr(a.err, kErrPage);
+                                page = a.b.num_pages;
+                            }
                         }
                     }
+                    if (n >= ST) tc_wait_bar(&bar.empty_k[st], turn ^ 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return;
+                    if (lane == 0) mbar_arrive_expect_tx(&bar.full_k[st], L::kTile);
+                    __syncwarp();
+                    if (lane < per_tile)
+    #pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            tma_load_4d(base + L::kK + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_k, 64 * b, row,
+                                        it.kvh, page, &bar.full_k[st]);
+                    if (n >= ST) tc_wait_bar(&bar.empty_v[st], turn ^ 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) return;
+                    if (lane == 0) mbar_arrive_expect_tx(&bar.full_v[st], L::kTile);
+                    __syncwarp();
+                    if (lane < per_tile)
+    #pragma unroll
+                        for (int b = 0; b < NB; ++b)
+                            tma_load_4d(base + L::kV + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_v, 64 * b, row,
+                                        it.kvh, page, &bar.full_v[st]);
                 }
-                if (n >= ST) tc_wait_bar(&bar.empty_k[st], turn ^ 1u, ok);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                if (lane == 0) mbar_arrive_expect_tx(&bar.full_k[st], L::kTile);
-                __syncwarp();
-                if (lane < per_tile)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-                        tma_load_4d(base + L::kK + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_k, 64 * b, row,
-                                    it.kvh, page, &bar.full_k[st]);
-                if (n >= ST) tc_wait_bar(&bar.empty_v[st], turn ^ 1u, ok);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                if (lane == 0) mbar_arrive_expect_tx(&bar.full_v[st], L::kTile);
-                __syncwarp();
-                if (lane < per_tile)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-                        tma_load_4d(base + L::kV + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_v, 64 * b, row,
-                                    it.kvh, page, &bar.full_v[st]);
-            }
-        });
+            });
         } else if ((warp == 1 || warp == 3) && place.s >= 0) {
             // ---- the MMAs of row tile x, issued by one lane.  n: key tiles so far, nx: those of
             // this row tile.  Each row tile has a warp of its own, so that neither waits for the
@@ -309,298 +310,298 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
         if (place.s >= 0) {
-        // ---- the rows: thread = TMEM lane r of row tile x
-        const int x = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
-        const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
-        const uint32_t tm_ox = tm_out(x) + lanes;
-        const float sc = a.scale_log2;
-        const F2 sc2 = f2(sc, sc);
-        constexpr int CH = D / 8, RPI = 32 / CH, LI = 32 / RPI;  // 16-byte chunks of a row, rows at once, rounds
-        const int ch = lane % CH;
-        // 16-byte chunk c of row rr of the row tile's Q (and, at the end, its result)
-        auto own_chunk = [&](int rr, int c) {
-            return base + L::kQ + x * L::kTileQ + (c >> 3) * kBoxQ + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-        };
-        auto st_shared = [](uint32_t at, uint4 w) {
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                         : "memory");
-        };
-        uint32_t n = 0;  // key tiles of this row tile so far
-        walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
-            // A wait that runs out ends the work on the scores, but not the barriers
-            // that the threads of both row tiles meet at.
-            const int rows_x = it.rows - 128 * x;  // rows of this tile (of 128)
-            const int row = it.row0 + 128 * x + r;
-            const bool mine = r < rows_x;
-            const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
-            float m = -INFINITY, l = 0.0f;  // m in base 2
-            bool settled = false;           // every row of the warp has an m
-            if (rows_x > 0 && part.j0 < part.j1) {
-                // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
-                {
-#pragma unroll
-                    for (int i0 = 0; i0 < LI; i0 += 8) {
-                        uint4 w[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            // past the item's rows its last one again: no branch around a load
-                            const int qrow =
-                                it.row0 + 128 * x + min(32 * quarter + (i0 + i) * RPI + lane / CH, rows_x - 1);
-                            const int t = a.by_g(qrow);
-                            w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                                        (long long)(seq.row0 + t) * a.ldq +
-                                                                        (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
+            // ---- the rows: thread = TMEM lane r of row tile x
+            const int x = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
+            const uint32_t lanes = (uint32_t)(32 * quarter) << 16;
+            const uint32_t tm_ox = tm_out(x) + lanes;
+            const float sc = a.scale_log2;
+            const F2 sc2 = f2(sc, sc);
+            constexpr int CH = D / 8, RPI = 32 / CH, LI = 32 / RPI;  // 16-byte chunks of a row, rows at once, rounds
+            const int ch = lane % CH;
+            // 16-byte chunk c of row rr of the row tile's Q (and, at the end, its result)
+            auto own_chunk = [&](int rr, int c) {
+                return base + L::kQ + x * L::kTileQ + (c >> 3) * kBoxQ + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+            };
+            auto st_shared = [](uint32_t at, uint4 w) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                             : "memory");
+            };
+            uint32_t n = 0;  // key tiles of this row tile so far
+            walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
+                // A wait that runs out ends the work on the scores, but not the barriers
+                // that the threads of both row tiles meet at.
+                const int rows_x = it.rows - 128 * x;  // rows of this tile (of 128)
+                const int row = it.row0 + 128 * x + r;
+                const bool mine = r < rows_x;
+                const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
+                float m = -INFINITY, l = 0.0f;  // m in base 2
+                bool settled = false;           // every row of the warp has an m
+                if (rows_x > 0 && part.j0 < part.j1) {
+                    // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
+                    {
+    #pragma unroll
+                        for (int i0 = 0; i0 < LI; i0 += 8) {
+                            uint4 w[8];
+    #pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                // past the item's rows its last one again: no branch around a load
+                                const int qrow =
+                                    it.row0 + 128 * x + min(32 * quarter + (i0 + i) * RPI + lane / CH, rows_x - 1);
+                                const int t = a.by_g(qrow);
+                                w[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                                            (long long)(seq.row0 + t) * a.ldq +
+                                                                            (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
+                            }
+    #pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                st_shared(own_chunk(32 * quarter + (i0 + i) * RPI + lane / CH, ch), w[i]);
                         }
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            st_shared(own_chunk(32 * quarter + (i0 + i) * RPI + lane / CH, ch), w[i]);
+                        fence_proxy_async_smem();
+                        mbar_arrive(&bar.q[x]);
                     }
-                    fence_proxy_async_smem();
-                    mbar_arrive(&bar.q[x]);
-                }
-#pragma unroll 1
-                for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
-                    const int k0 = tile_key<kN>(it, part.j0 + i);
-                    const uint32_t b = n & 1u;
-                    tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    float sv[kN];
-                    tmem_ld64(tm_score(x, b) + lanes, sv);
-                    // keys that every row of the item sees need no mask
-                    const bool whole = k0 + kN - 1 <= it.pos_first &&
-                                       (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
-                    // at head_dim 64 P's columns are free once P V of two tiles ago is done
-                    if (D == 64 && i >= 2) {
-                        tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
+    #pragma unroll 1
+                    for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
+                        const int k0 = tile_key<kN>(it, part.j0 + i);
+                        const uint32_t b = n & 1u;
+                        tc_wait_bar(&bar.s[x][b], (n >> 1) & 1u, ok);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         tc_fence_after();
-                    }
-                    const uint32_t tm_px = tm_prob(x, b) + lanes;
-                    float lsum = 0.0f;
-                    bool done = false;
-                    if (whole && settled) {
-                        // probabilities under the m of the tiles before, unless their sum
-                        // says that a score has passed it by far
-                        const F2 ref2 = f2(-m, -m);
-                        F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int e = 8 * c; e < 8 * c + 8; ++e) {
-                                const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
-                                const float2 v = un2(arg);
-                                const float p0 = ex2(v.x), p1 = ex2(v.y);
-                                ls[e & 1] = add2(ls[e & 1], f2(p0, p1));
-                                w[e & 7] = Half16<T>::pack(p0, p1);
-                            }
-                            tmem_st8(tm_px + 8 * c, w);
-                        }
-                        const float2 v = un2(add2(ls[0], ls[1]));
-                        lsum = v.x + v.y;
-                        done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
-                    }
-                    if (!done) {
-                        tmem_st_wait();  // the stores that are made again
-                        // a row's first keys, hidden keys, and keys whose maximum moves m
-                        if (!whole) {
-                            const int hi = pos - k0;
-                            if (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks) {
-#pragma unroll
-                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
-                            } else {
-                                const int lo = hi - a.window, sink = a.sinks - k0;
-#pragma unroll
-                                for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
-                            }
-                        }
-                        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                        for (int e = 0; e < kN; e += 4) {
-                            mx[0] = fmaxf(mx[0], fmaxf(sv[e], sv[e + 1]));
-                            mx[1] = fmaxf(mx[1], fmaxf(sv[e + 2], sv[e + 3]));
-                        }
-                        const float top = fmaxf(mx[0], mx[1]) * sc;
-                        const bool grow = top > m + kRescale;
-                        if (i == 0) {
-                            m = top;
-                        } else if (__any_sync(0xffffffffu, grow)) {
-                            // O must hold the products before it is rescaled
-                            tc_wait_bar(&bar.o[x][b ^ 1], ((n - 1) >> 1) & 1u, ok);
+                        float sv[kN];
+                        tmem_ld64(tm_score(x, b) + lanes, sv);
+                        // keys that every row of the item sees need no mask
+                        const bool whole = k0 + kN - 1 <= it.pos_first &&
+                                           (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
+                        // at head_dim 64 P's columns are free once P V of two tiles ago is done
+                        if (D == 64 && i >= 2) {
+                            tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             tc_fence_after();
-                            const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-#pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                float o[32];
-                                uint32_t w[32];
-                                tmem_ld32(tm_ox + 32 * c, o);
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-                                tmem_st32(tm_ox + 32 * c, w);
-                            }
-                            tmem_st_wait();
-                            if (grow) {
-                                l *= f;
-                                m = top;
-                            }
                         }
-                        settled = !__any_sync(0xffffffffu, m == -INFINITY);
-                        const float ref = m == -INFINITY ? 0.0f : m;
-                        float ls[2] = {0.0f, 0.0f};
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t w[8];
-#pragma unroll
-                            for (int e = 8 * c; e < 8 * c + 8; ++e) {
-                                const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
-                                ls[0] += p0;
-                                ls[1] += p1;
-                                w[e & 7] = Half16<T>::pack(p0, p1);
+                        const uint32_t tm_px = tm_prob(x, b) + lanes;
+                        float lsum = 0.0f;
+                        bool done = false;
+                        if (whole && settled) {
+                            // probabilities under the m of the tiles before, unless their sum
+                            // says that a score has passed it by far
+                            const F2 ref2 = f2(-m, -m);
+                            F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+    #pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t w[8];
+    #pragma unroll
+                                for (int e = 8 * c; e < 8 * c + 8; ++e) {
+                                    const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
+                                    const float2 v = un2(arg);
+                                    const float p0 = ex2(v.x), p1 = ex2(v.y);
+                                    ls[e & 1] = add2(ls[e & 1], f2(p0, p1));
+                                    w[e & 7] = Half16<T>::pack(p0, p1);
+                                }
+                                tmem_st8(tm_px + 8 * c, w);
                             }
-                            tmem_st8(tm_px + 8 * c, w);
+                            const float2 v = un2(add2(ls[0], ls[1]));
+                            lsum = v.x + v.y;
+                            done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
                         }
-                        lsum = ls[0] + ls[1];
-                    }
-                    l += lsum;
-                    tmem_st_wait();
-                    tc_fence_before();
-                    mbar_arrive(&bar.p[x][b]);
-                }
-                tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
-                ok = __all_sync(0xffffffffu, ok);
-                tc_fence_after();
-            }
-            // ---- the part's result: straight to out, or through the slots
-            const bool split = part.first != part.last, some = part.j0 < part.j1 && rows_x > 0;
-            const int ri = 128 * x + r;
-            bool write = true;
-            if (split) {
-                // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
-                float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
-                if (rows_x > 0) {
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        if (some) tmem_ld32(tm_ox + 32 * c, o);
-                        if (mine)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                reinterpret_cast<float4*>(slot)[(8 * c + e) * kM + ri] =
-                                    some ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3])
-                                         : make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-                    if (mine) {
-                        slot[kM * D + ri] = m;
-                        slot[kM * D + kM + ri] = l;
-                    }
-                }
-                named_sync(1, kRowThreads);
-                if (tid == 128) {
-                    // the others' writes, ordered before by the barrier, become visible with this thread's fence
-                    __threadfence();
-                    unsigned* ticket = a.tickets + part.first;
-                    last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(part.last - part.first + 1);
-                    if (last_s) *ticket = 0u;  // ready for the next call
-                    __threadfence();
-                }
-                named_sync(1, kRowThreads);
-                write = last_s != 0;
-            }
-            if (write && rows_x > 0) {
-                float M = m, lsum = l;
-                if (split && mine) {
-                    M = -INFINITY;
-                    lsum = 0.0f;
-                    for (int b = part.first; b <= part.last; ++b)
-                        M = fmaxf(M, __ldcg(slot_of<kM, D>(a, b, part.first) + kM * D + ri));
-                    for (int b = part.first; b <= part.last; ++b) {
-                        const float* p = slot_of<kM, D>(a, b, part.first) + kM * D + ri;
-                        const float mb = __ldcg(p);
-                        lsum = fmaf(__ldcg(p + kM), mb == -INFINITY ? 0.0f : ex2(mb - M), lsum);
-                    }
-                }
-                const bool sees = mine && pos >= 0;
-                const float inv = sees ? 1.0f / lsum : 0.0f;
-                bool bad = false;
-                // 32 columns at a time into the row tile's Q, which the products are done with
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    float o[32];
-                    if (!split) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-                        if (some) tmem_ld32(tm_ox + 32 * c, o);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-#pragma unroll 1
-                        for (int b = part.first; b <= part.last; ++b) {
-                            const float* p = slot_of<kM, D>(a, b, part.first);
-                            const float mb = mine ? __ldcg(p + kM * D + ri) : -INFINITY;
-                            float v[32];
-                            if (b == (int)blockIdx.x) {  // its own is still here
-                                tmem_ld32(tm_ox + 32 * c, v);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
-                                    v[4 * e] = f4.x;
-                                    v[4 * e + 1] = f4.y;
-                                    v[4 * e + 2] = f4.z;
-                                    v[4 * e + 3] = f4.w;
+                        if (!done) {
+                            tmem_st_wait();  // the stores that are made again
+                            // a row's first keys, hidden keys, and keys whose maximum moves m
+                            if (!whole) {
+                                const int hi = pos - k0;
+                                if (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks) {
+    #pragma unroll
+                                    for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
+                                } else {
+                                    const int lo = hi - a.window, sink = a.sinks - k0;
+    #pragma unroll
+                                    for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
                                 }
                             }
-                            const float f = mb == -INFINITY ? 0.0f : ex2(mb - M);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = fmaf(v[e], f, o[e]);
+                            float mx[2] = {-INFINITY, -INFINITY};
+    #pragma unroll
+                            for (int e = 0; e < kN; e += 4) {
+                                mx[0] = fmaxf(mx[0], fmaxf(sv[e], sv[e + 1]));
+                                mx[1] = fmaxf(mx[1], fmaxf(sv[e + 2], sv[e + 3]));
+                            }
+                            const float top = fmaxf(mx[0], mx[1]) * sc;
+                            const bool grow = top > m + kRescale;
+                            if (i == 0) {
+                                m = top;
+                            } else if (__any_sync(0xffffffffu, grow)) {
+                                // O must hold the products before it is rescaled
+                                tc_wait_bar(&bar.o[x][b ^ 1], ((n - 1) >> 1) & 1u, ok);
+                                ok = __all_sync(0xffffffffu, ok);
+                                if (!ok) break;
+                                tc_fence_after();
+                                const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
+    #pragma unroll 1
+                                for (int c = 0; c < D / 32; ++c) {
+                                    float o[32];
+                                    uint32_t w[32];
+                                    tmem_ld32(tm_ox + 32 * c, o);
+    #pragma unroll
+                                    for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+                                    tmem_st32(tm_ox + 32 * c, w);
+                                }
+                                tmem_st_wait();
+                                if (grow) {
+                                    l *= f;
+                                    m = top;
+                                }
+                            }
+                            settled = !__any_sync(0xffffffffu, m == -INFINITY);
+                            const float ref = m == -INFINITY ? 0.0f : m;
+                            float ls[2] = {0.0f, 0.0f};
+    #pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t w[8];
+    #pragma unroll
+                                for (int e = 8 * c; e < 8 * c + 8; ++e) {
+                                    const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
+                                    ls[0] += p0;
+                                    ls[1] += p1;
+                                    w[e & 7] = Half16<T>::pack(p0, p1);
+                                }
+                                tmem_st8(tm_px + 8 * c, w);
+                            }
+                            lsum = ls[0] + ls[1];
+                        }
+                        l += lsum;
+                        tmem_st_wait();
+                        tc_fence_before();
+                        mbar_arrive(&bar.p[x][b]);
+                    }
+                    tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                }
+                // ---- the part's result: straight to out, or through the slots
+                const bool split = part.first != part.last, some = part.j0 < part.j1 && rows_x > 0;
+                const int ri = 128 * x + r;
+                bool write = true;
+                if (split) {
+                    // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
+                    float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
+                    if (rows_x > 0) {
+    #pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            float o[32];
+                            if (some) tmem_ld32(tm_ox + 32 * c, o);
+                            if (mine)
+    #pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    reinterpret_cast<float4*>(slot)[(8 * c + e) * kM + ri] =
+                                        some ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3])
+                                             : make_float4(0.f, 0.f, 0.f, 0.f);
+                        }
+                        if (mine) {
+                            slot[kM * D + ri] = m;
+                            slot[kM * D + kM + ri] = l;
                         }
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        o[e] = sees ? o[e] * inv : 0.0f;
-                        bad |= !(fabsf(o[e]) < INFINITY);
+                    named_sync(1, kRowThreads);
+                    if (tid == 128) {
+                        // the others' writes, ordered before by the barrier, become visible with this thread's fence
+                        __threadfence();
+                        unsigned* ticket = a.tickets + part.first;
+                        last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(part.last - part.first + 1);
+                        if (last_s) *ticket = 0u;  // ready for the next call
+                        __threadfence();
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        st_shared(own_chunk(r, 4 * c + e),
-                                  make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
-                                             Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
-                                             Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
-                                             Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
+                    named_sync(1, kRowThreads);
+                    write = last_s != 0;
                 }
-                __syncwarp();
-                // whole rows by D / 8 lanes each
-#pragma unroll
-                for (int i = 0; i < LI; ++i) {
-                    const int rr = 32 * quarter + i * RPI + lane / CH, orow = it.row0 + 128 * x + rr;
-                    if (rr < rows_x) {
-                        const int t = a.by_g(orow);
-                        uint4 w;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                                     : "r"(own_chunk(rr, ch))
-                                     : "memory");
-                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + t) * a.ldo +
-                                                  (it.kvh * a.G + orow - t * a.G) * D + ch * 8) = w;
+                if (write && rows_x > 0) {
+                    float M = m, lsum = l;
+                    if (split && mine) {
+                        M = -INFINITY;
+                        lsum = 0.0f;
+                        for (int b = part.first; b <= part.last; ++b)
+                            M = fmaxf(M, __ldcg(slot_of<kM, D>(a, b, part.first) + kM * D + ri));
+                        for (int b = part.first; b <= part.last; ++b) {
+                            const float* p = slot_of<kM, D>(a, b, part.first) + kM * D + ri;
+                            const float mb = __ldcg(p);
+                            lsum = fmaf(__ldcg(p + kM), mb == -INFINITY ? 0.0f : ex2(mb - M), lsum);
+                        }
                     }
+                    const bool sees = mine && pos >= 0;
+                    const float inv = sees ? 1.0f / lsum : 0.0f;
+                    bool bad = false;
+                    // 32 columns at a time into the row tile's Q, which the products are done with
+    #pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        if (!split) {
+    #pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+                            if (some) tmem_ld32(tm_ox + 32 * c, o);
+                        } else {
+    #pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+    #pragma unroll 1
+                            for (int b = part.first; b <= part.last; ++b) {
+                                const float* p = slot_of<kM, D>(a, b, part.first);
+                                const float mb = mine ? __ldcg(p + kM * D + ri) : -INFINITY;
+                                float v[32];
+                                if (some && b == (int)blockIdx.x) {  // its own is still here
+                                    tmem_ld32(tm_ox + 32 * c, v);
+                                } else {
+    #pragma unroll
+                                    for (int e = 0; e < 8; ++e) {
+                                        const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
+                                        v[4 * e] = f4.x;
+                                        v[4 * e + 1] = f4.y;
+                                        v[4 * e + 2] = f4.z;
+                                        v[4 * e + 3] = f4.w;
+                                    }
+                                }
+                                const float f = mb == -INFINITY ? 0.0f : ex2(mb - M);
+    #pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = fmaf(v[e], f, o[e]);
+                            }
+                        }
+    #pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            o[e] = sees ? o[e] * inv : 0.0f;
+                            bad |= !(fabsf(o[e]) < INFINITY);
+                        }
+    #pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            st_shared(own_chunk(r, 4 * c + e),
+                                      make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
+                                                 Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
+                                                 Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
+                                                 Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
+                    }
+                    __syncwarp();
+                    // whole rows by D / 8 lanes each
+    #pragma unroll
+                    for (int i = 0; i < LI; ++i) {
+                        const int rr = 32 * quarter + i * RPI + lane / CH, orow = it.row0 + 128 * x + rr;
+                        if (rr < rows_x) {
+                            const int t = a.by_g(orow);
+                            uint4 w;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                         : "r"(own_chunk(rr, ch))
+                                         : "memory");
+                            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + t) * a.ldo +
+                                                      (it.kvh * a.G + orow - t * a.G) * D + ch * 8) = w;
+                        }
+                    }
+                    __syncwarp();
+                    if (mine && a.lse)
+                        a.lse[(long long)(seq.row0 + token) * a.nq + it.kvh * a.G + row - token * a.G] =
+                            sees ? (M + log2f(lsum)) * kLn2 : -INFINITY;
+                    // rows that met something not finite, term by term
+                    for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1)
+                        exact_row<T, D>(a, seq, part.s, it.kvh, it.row0 + 128 * x + 32 * quarter + __ffs(left) - 1);
                 }
-                __syncwarp();
-                if (mine && a.lse)
-                    a.lse[(long long)(seq.row0 + token) * a.nq + it.kvh * a.G + row - token * a.G] =
-                        sees ? (M + log2f(lsum)) * kLn2 : -INFINITY;
-                // rows that met something not finite, term by term
-                for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1)
-                    exact_row<T, D>(a, seq, part.s, it.kvh, it.row0 + 128 * x + 32 * quarter + __ffs(left) - 1);
-            }
-            // O, S and the slots' flag are read before the next part begins
-            tc_fence_before();
-            if (split) named_sync(1, kRowThreads);
-        });
+                // O, S and the slots' flag are read before the next part begins
+                tc_fence_before();
+                if (split) named_sync(1, kRowThreads);
+            });
         }
     }
     if (!ok) atomicExch(&ok_s, 0);
@@ -669,7 +670,8 @@ int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D,
                                 (cuuint64_t)a.b.num_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)a.b.page_size * D * 2,
                                    (cuuint64_t)a.b.nkv * a.b.page_size * D * 2};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(a.b.page_size < tile_keys ? a.b.page_size : tile_keys), 1, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(a.b.page_size < tile_keys ? a.b.page_size : tile_keys), 1, 1};
+    const cuuint32_t one[4] = {1, 1, 1, 1};
     const CUresult r =
         fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool),
            dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -680,8 +682,10 @@ int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D,
 
 int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st) {
     if (dtype == INFERNT_DTYPE_BF16)
-        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, after_other, st) : launch_tc<__nv_bfloat16, 128>(a, after_other, st);
-    return head_dim == 64 ? launch_tc<__half, 64>(a, after_other, st) : launch_tc<__half, 128>(a, after_other, st);
+        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, after_other, st)
+                              : launch_tc<__nv_bfloat16, 128>(a, after_other, st);
+    return head_dim == 64 ? launch_tc<__half, 64>(a, after_other, st)
+                          : launch_tc<__half, 128>(a, after_other, st);
 }
 
 }  // namespace infernt

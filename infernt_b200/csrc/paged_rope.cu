@@ -186,7 +186,8 @@ __device__ __forceinline__ void store_eight(T* p, const float (&x)[8]) {
 constexpr int kAhead = 3;
 
 template <typename S, typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRopeThreads) paged_rope_wide(const RopeArgs a, const __grid_constant__ RopeDev rope) {
+__global__ void __launch_bounds__(kRopeThreads)
+    paged_rope_wide(const RopeArgs a, const __grid_constant__ RopeDev rope) {
     __shared__ float2 cs_s[kMaxPairs];
     const int r = blockIdx.x, tid = threadIdx.x, D = a.D, R = 2 * rope.half, nkv = a.b.nkv;
     const int log_u = D == 64 ? 2 : 3, w = tid & ((1 << log_u) - 1);
@@ -333,7 +334,9 @@ int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
     out->magnitude = 1.0f;
     if (p.scaling == INFERNT_ROPE_YARN) {
         // the pair index at which a pair makes t turns over the original context
-        auto border = [&](double t) { return R * std::log(p.original_max_len / (t * two_pi)) / (2 * std::log(p.theta)); };
+        auto border = [&](double t) {
+            return R * std::log(p.original_max_len / (t * two_pi)) / (2 * std::log(p.theta));
+        };
         lo = std::fmax(0.0, std::floor(border(p.high)));
         hi = std::fmin(R - 1.0, std::ceil(border(p.low)));
         out->magnitude = (float)(0.1 * std::log(p.factor) + 1.0);
