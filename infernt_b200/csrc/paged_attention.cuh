@@ -282,6 +282,29 @@ __device__ __forceinline__ bool item_sees(const Item& it, int p) {
     return p < it.hi && (p >= it.lo || p < it.sink_end);
 }
 
+// Pages of the boxes of tiles j, j + 1, ... of a part, a box a lane (per_tile
+// of them, a power of two, to a tile), so that a trip to the table serves up to
+// 32 tiles: the box's page (a page past the pool when no row sees the box, or
+// the pool does not have it), and its first row there.
+template <int N>
+__device__ __forceinline__ int2 look_up(const AttnArgs& a, const Item& it, const Part& part, int j, int per_tile,
+                                        int box_rows) {
+    const int lane = threadIdx.x & 31, tile = j + lane / per_tile;
+    int2 at = make_int2(a.b.num_pages, 0);
+    if (tile < part.j1) {
+        const int p0 = tile_key<N>(it, tile) + lane % per_tile * box_rows, pi = a.b.by_page(p0);
+        at.y = p0 - pi * a.b.page_size;
+        if (p0 < it.hi && (p0 + box_rows > it.lo || p0 < it.sink_end)) {
+            at.x = a.b.table[(size_t)part.s * a.b.table_stride + pi];
+            if (at.x < 0 || at.x >= a.b.num_pages) {
+                if (a.err) atomicOr(a.err, kErrPage);
+                at.x = a.b.num_pages;
+            }
+        }
+    }
+    return at;
+}
+
 // Pool row of position p of sequence s for KV head kvh, or -1 (a page that
 // the pool does not have).
 __device__ __forceinline__ int pool_row(const PagedBatch& b, int s, int kvh, int p, unsigned* err) {

@@ -60,6 +60,7 @@ constexpr int kM = kTcItemRows;  // query rows of an item
 constexpr int kN = kTcTileKeys;  // keys of a tile
 constexpr float kMostSum = 8192.0f;  // of a tile's probabilities: each then fits fp16
 constexpr int kThreadsTc = 384;
+constexpr int kJoin = 2;  // parts of a split item that are read at once
 constexpr int kRowThreads = 256;
 constexpr uint32_t kBoxQ = 16384;  // 128 rows of 64 values: a swizzled operand block
 constexpr uint32_t kBox = 8192;    // 64 rows
@@ -128,6 +129,99 @@ __device__ __forceinline__ void zero_rows(const Item& it, int k0, uint32_t v) {
     __syncwarp();
 }
 
+// 16-byte chunk c of row r of a row tile's Q (and, at the end, its result) at
+// `tile` in shared memory.
+__device__ __forceinline__ uint32_t row_chunk(uint32_t tile, int r, int c) {
+    return tile + (c >> 3) * kBoxQ + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                 : "memory");
+}
+
+// 32 columns of a result, the chunks from c on of row r; true when one is not
+// finite.
+template <typename T>
+__device__ __forceinline__ bool put_result(uint32_t tile, int r, int c, float (&o)[32], bool sees, float inv) {
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        o[e] = sees ? o[e] * inv : 0.0f;
+        bad |= !(fabsf(o[e]) < INFINITY);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        st_shared(row_chunk(tile, r, c + e),
+                  make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]), Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
+                             Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]), Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
+    return bad;
+}
+
+// Row ri (r of its row tile) of a split item, joined over its CTAs in order
+// into shared memory: kJoin parts of 32 columns are read at once, since each
+// read is a trip to L2.  A function of its own, so that its registers are not
+// the tiles'.
+template <typename T, int D>
+__device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, int ri, uint32_t tile, int r, bool sees,
+                                      float* lse) {
+    float M = -INFINITY, l = 0.0f;
+    for (int b = first; b <= last; b += 4) {
+        float mb[4], lb[4], top = M;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* p = slot_of<kM, D>(a, min(b + i, last), first) + kM * D + ri;
+            mb[i] = __ldcg(p);
+            lb[i] = __ldcg(p + kM);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b + i > last) mb[i] = -INFINITY;
+            top = fmaxf(top, mb[i]);
+        }
+        l *= M == -INFINITY ? 0.0f : ex2(M - top);
+        M = top;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (mb[i] != -INFINITY) l = fmaf(lb[i], ex2(mb[i] - M), l);
+    }
+    if (lse) *lse = sees ? (M + log2f(l)) * kLn2 : -INFINITY;
+    const float inv = 1.0f / l;
+    bool bad = false;
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+#pragma unroll 1
+        for (int b = first; b <= last; b += kJoin) {
+            float mb[kJoin];
+            float4 v[kJoin][8];
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) {
+                if (b + i > last) break;
+                const float* p = slot_of<kM, D>(a, b + i, first);
+                mb[i] = __ldcg(p + kM * D + ri);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[i][e] = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
+            }
+#pragma unroll
+            for (int i = 0; i < kJoin; ++i) {
+                if (b + i > last) break;
+                const float f = mb[i] == -INFINITY ? 0.0f : ex2(mb[i] - M);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    o[4 * e] = fmaf(v[i][e].x, f, o[4 * e]);
+                    o[4 * e + 1] = fmaf(v[i][e].y, f, o[4 * e + 1]);
+                    o[4 * e + 2] = fmaf(v[i][e].z, f, o[4 * e + 2]);
+                    o[4 * e + 3] = fmaf(v[i][e].w, f, o[4 * e + 3]);
+                }
+            }
+        }
+        bad |= put_result<T>(tile, r, 4 * c, o, sees, inv);
+    }
+    return bad;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreadsTc, 1)
     paged_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
@@ -176,31 +270,26 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             // ---- K and V tiles.  n: tiles so far, over all parts.
             uint32_t n = 0;
             const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
+            const int run = 32 / per_tile;  // tiles of a look-up
             walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
-                for (int j = part.j0; j < part.j1; ++j, ++n) {
-                    const int k0 = tile_key<kN>(it, j), st = (int)(n % ST);
+                int2 boxes = {};
+                for (int j = part.j0, k = run; j < part.j1; ++j, ++n) {
+                    const int st = (int)(n % ST);
                     const uint32_t turn = (n / ST) & 1u;
-                    // the page of lane l's rows [k0 + l box_rows, + box_rows)
-                    int page = a.b.num_pages, row = 0;
-                    if (lane < per_tile) {
-                        const int p0 = k0 + lane * box_rows, pi = a.b.by_page(p0);
-                        row = p0 - pi * ps;
-                        // whether some row sees a key of the box
-                        if (p0 < it.hi && (p0 + box_rows > it.lo || p0 < it.sink_end)) {
-                            page = a.b.table[(size_t)part.s * a.b.table_stride + pi];
-                            if (page < 0 || page >= a.b.num_pages) {
-                                if (a.err) atomicOr(a.err, kErrPage);
-                                page = a.b.num_pages;
-                            }
-                        }
+                    if (k == run) {
+                        boxes = look_up<kN>(a, it, part, j, per_tile, box_rows);
+                        k = 0;
                     }
+                    const int page = __shfl_sync(0xffffffffu, boxes.x, k * per_tile + lane),
+                              row = __shfl_sync(0xffffffffu, boxes.y, k * per_tile + lane);
+                    ++k;
                     if (n >= ST) tc_wait_bar(&bar.empty_k[st], turn ^ 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return;
                     if (lane == 0) mbar_arrive_expect_tx(&bar.full_k[st], L::kTile);
                     __syncwarp();
                     if (lane < per_tile)
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < NB; ++b)
                             tma_load_4d(base + L::kK + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_k, 64 * b, row,
                                         it.kvh, page, &bar.full_k[st]);
@@ -210,7 +299,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     if (lane == 0) mbar_arrive_expect_tx(&bar.full_v[st], L::kTile);
                     __syncwarp();
                     if (lane < per_tile)
-    #pragma unroll
+#pragma unroll
                         for (int b = 0; b < NB; ++b)
                             tma_load_4d(base + L::kV + st * L::kTile + b * kBox + lane * box_rows * 128, &tm_v, 64 * b, row,
                                         it.kvh, page, &bar.full_v[st]);
@@ -318,14 +407,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const F2 sc2 = f2(sc, sc);
             constexpr int CH = D / 8, RPI = 32 / CH, LI = 32 / RPI;  // 16-byte chunks of a row, rows at once, rounds
             const int ch = lane % CH;
-            // 16-byte chunk c of row rr of the row tile's Q (and, at the end, its result)
-            auto own_chunk = [&](int rr, int c) {
-                return base + L::kQ + x * L::kTileQ + (c >> 3) * kBoxQ + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-            };
-            auto st_shared = [](uint32_t at, uint4 w) {
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                             : "memory");
-            };
+            const uint32_t own = base + L::kQ + x * L::kTileQ;  // the row tile's Q
             uint32_t n = 0;  // key tiles of this row tile so far
             walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
                 // A wait that runs out ends the work on the scores, but not the barriers
@@ -339,10 +421,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 if (rows_x > 0 && part.j0 < part.j1) {
                     // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
                     {
-    #pragma unroll
+#pragma unroll
                         for (int i0 = 0; i0 < LI; i0 += 8) {
                             uint4 w[8];
-    #pragma unroll
+#pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 // past the item's rows its last one again: no branch around a load
                                 const int qrow =
@@ -352,14 +434,14 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                                                             (long long)(seq.row0 + t) * a.ldq +
                                                                             (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
                             }
-    #pragma unroll
+#pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                st_shared(own_chunk(32 * quarter + (i0 + i) * RPI + lane / CH, ch), w[i]);
+                                st_shared(row_chunk(own, 32 * quarter + (i0 + i) * RPI + lane / CH, ch), w[i]);
                         }
                         fence_proxy_async_smem();
                         mbar_arrive(&bar.q[x]);
                     }
-    #pragma unroll 1
+#pragma unroll 1
                     for (int i = 0; i < part.j1 - part.j0; ++i, ++n) {
                         const int k0 = tile_key<kN>(it, part.j0 + i);
                         const uint32_t b = n & 1u;
@@ -387,10 +469,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             // says that a score has passed it by far
                             const F2 ref2 = f2(-m, -m);
                             F2 ls[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
-    #pragma unroll
+#pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t w[8];
-    #pragma unroll
+#pragma unroll
                                 for (int e = 8 * c; e < 8 * c + 8; ++e) {
                                     const F2 arg = fma2(f2(sv[2 * e], sv[2 * e + 1]), sc2, ref2);
                                     const float2 v = un2(arg);
@@ -410,16 +492,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             if (!whole) {
                                 const int hi = pos - k0;
                                 if (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks) {
-    #pragma unroll
+#pragma unroll
                                     for (int e = 0; e < kN; ++e) sv[e] = e <= hi ? sv[e] : -INFINITY;
                                 } else {
                                     const int lo = hi - a.window, sink = a.sinks - k0;
-    #pragma unroll
+#pragma unroll
                                     for (int e = 0; e < kN; ++e) sv[e] = e <= hi && (e > lo || e < sink) ? sv[e] : -INFINITY;
                                 }
                             }
                             float mx[2] = {-INFINITY, -INFINITY};
-    #pragma unroll
+#pragma unroll
                             for (int e = 0; e < kN; e += 4) {
                                 mx[0] = fmaxf(mx[0], fmaxf(sv[e], sv[e + 1]));
                                 mx[1] = fmaxf(mx[1], fmaxf(sv[e + 2], sv[e + 3]));
@@ -435,12 +517,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                 if (!ok) break;
                                 tc_fence_after();
                                 const float f = !grow ? 1.0f : m == -INFINITY ? 0.0f : ex2(m - top);
-    #pragma unroll 1
+#pragma unroll 1
                                 for (int c = 0; c < D / 32; ++c) {
                                     float o[32];
                                     uint32_t w[32];
                                     tmem_ld32(tm_ox + 32 * c, o);
-    #pragma unroll
+#pragma unroll
                                     for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
                                     tmem_st32(tm_ox + 32 * c, w);
                                 }
@@ -453,10 +535,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             settled = !__any_sync(0xffffffffu, m == -INFINITY);
                             const float ref = m == -INFINITY ? 0.0f : m;
                             float ls[2] = {0.0f, 0.0f};
-    #pragma unroll
+#pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t w[8];
-    #pragma unroll
+#pragma unroll
                                 for (int e = 8 * c; e < 8 * c + 8; ++e) {
                                     const float p0 = ex2(fmaf(sv[2 * e], sc, -ref)), p1 = ex2(fmaf(sv[2 * e + 1], sc, -ref));
                                     ls[0] += p0;
@@ -484,12 +566,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
                     float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
                     if (rows_x > 0) {
-    #pragma unroll
+#pragma unroll
                         for (int c = 0; c < D / 32; ++c) {
                             float o[32];
                             if (some) tmem_ld32(tm_ox + 32 * c, o);
                             if (mine)
-    #pragma unroll
+#pragma unroll
                                 for (int e = 0; e < 8; ++e)
                                     reinterpret_cast<float4*>(slot)[(8 * c + e) * kM + ri] =
                                         some ? make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3])
@@ -513,70 +595,29 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     write = last_s != 0;
                 }
                 if (write && rows_x > 0) {
-                    float M = m, lsum = l;
-                    if (split && mine) {
-                        M = -INFINITY;
-                        lsum = 0.0f;
-                        for (int b = part.first; b <= part.last; ++b)
-                            M = fmaxf(M, __ldcg(slot_of<kM, D>(a, b, part.first) + kM * D + ri));
-                        for (int b = part.first; b <= part.last; ++b) {
-                            const float* p = slot_of<kM, D>(a, b, part.first) + kM * D + ri;
-                            const float mb = __ldcg(p);
-                            lsum = fmaf(__ldcg(p + kM), mb == -INFINITY ? 0.0f : ex2(mb - M), lsum);
-                        }
-                    }
                     const bool sees = mine && pos >= 0;
-                    const float inv = sees ? 1.0f / lsum : 0.0f;
                     bool bad = false;
+                    float* lse = mine && a.lse ? a.lse + (long long)(seq.row0 + token) * a.nq + it.kvh * a.G + row -
+                                                     token * a.G
+                                               : nullptr;
                     // 32 columns at a time into the row tile's Q, which the products are done with
-    #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        if (!split) {
-    #pragma unroll
+                    if (split) {
+                        bad = join_row<T, D>(a, part.first, part.last, ri, own, r, sees, lse);
+                    } else {
+                        if (lse) *lse = sees ? (m + log2f(l)) * kLn2 : -INFINITY;
+                        const float inv = sees ? 1.0f / l : 0.0f;
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) {
+                            float o[32];
+#pragma unroll
                             for (int e = 0; e < 32; ++e) o[e] = 0.0f;
                             if (some) tmem_ld32(tm_ox + 32 * c, o);
-                        } else {
-    #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-    #pragma unroll 1
-                            for (int b = part.first; b <= part.last; ++b) {
-                                const float* p = slot_of<kM, D>(a, b, part.first);
-                                const float mb = mine ? __ldcg(p + kM * D + ri) : -INFINITY;
-                                float v[32];
-                                if (some && b == (int)blockIdx.x) {  // its own is still here
-                                    tmem_ld32(tm_ox + 32 * c, v);
-                                } else {
-    #pragma unroll
-                                    for (int e = 0; e < 8; ++e) {
-                                        const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
-                                        v[4 * e] = f4.x;
-                                        v[4 * e + 1] = f4.y;
-                                        v[4 * e + 2] = f4.z;
-                                        v[4 * e + 3] = f4.w;
-                                    }
-                                }
-                                const float f = mb == -INFINITY ? 0.0f : ex2(mb - M);
-    #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = fmaf(v[e], f, o[e]);
-                            }
+                            bad |= put_result<T>(own, r, 4 * c, o, sees, inv);
                         }
-    #pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            o[e] = sees ? o[e] * inv : 0.0f;
-                            bad |= !(fabsf(o[e]) < INFINITY);
-                        }
-    #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            st_shared(own_chunk(r, 4 * c + e),
-                                      make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]),
-                                                 Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
-                                                 Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]),
-                                                 Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
                     }
                     __syncwarp();
                     // whole rows by D / 8 lanes each
-    #pragma unroll
+#pragma unroll
                     for (int i = 0; i < LI; ++i) {
                         const int rr = 32 * quarter + i * RPI + lane / CH, orow = it.row0 + 128 * x + rr;
                         if (rr < rows_x) {
@@ -584,16 +625,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             uint4 w;
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
-                                         : "r"(own_chunk(rr, ch))
+                                         : "r"(row_chunk(own, rr, ch))
                                          : "memory");
                             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + t) * a.ldo +
                                                       (it.kvh * a.G + orow - t * a.G) * D + ch * 8) = w;
                         }
                     }
                     __syncwarp();
-                    if (mine && a.lse)
-                        a.lse[(long long)(seq.row0 + token) * a.nq + it.kvh * a.G + row - token * a.G] =
-                            sees ? (M + log2f(lsum)) * kLn2 : -INFINITY;
                     // rows that met something not finite, term by term
                     for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1)
                         exact_row<T, D>(a, seq, part.s, it.kvh, it.row0 + 128 * x + 32 * quarter + __ffs(left) - 1);
