@@ -341,18 +341,21 @@ int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
         hi = std::fmin(R - 1.0, std::ceil(border(p.low)));
         out->magnitude = (float)(0.1 * std::log(p.factor) + 1.0);
     }
-    // f_i by repeated products: 64 of them are off by 64 x 2^-53
-    const double ratio = std::pow(p.theta, -2.0 / R);
+    // f_i by repeated products: 64 of them are off by 64 x 2^-53; divisions
+    // stay out of the loop, which runs at each call
+    const double ratio = std::pow(p.theta, -2.0 / R), turns = 1.0 / two_pi;
+    const double shrink = p.scaling == INFERNT_ROPE_NONE ? 1.0 : 1.0 / p.factor, llama3 = 1.0 / (p.high - p.low),
+                 yarn = 1.0 / std::fmax(hi - lo, 0.001);
     double f = 1.0;
     for (int i = 0; i < R / 2; ++i, f *= ratio) {
         double g = f, keep = 1.0;  // share of f, the rest is f / factor
         if (p.scaling == INFERNT_ROPE_LINEAR) keep = 0.0;
         if (p.scaling == INFERNT_ROPE_LLAMA3)
-            keep = (p.original_max_len * f / two_pi - p.low) / (p.high - p.low);
-        if (p.scaling == INFERNT_ROPE_YARN) keep = 1.0 - (i - lo) / std::fmax(hi - lo, 0.001);
+            keep = (p.original_max_len * f * turns - p.low) * llama3;
+        if (p.scaling == INFERNT_ROPE_YARN) keep = 1.0 - (i - lo) * yarn;
         keep = std::fmin(1.0, std::fmax(0.0, keep));
-        if (p.scaling != INFERNT_ROPE_NONE) g = f * keep + f / p.factor * (1.0 - keep);
-        out->turns[i] = g / two_pi;
+        if (p.scaling != INFERNT_ROPE_NONE) g = f * keep + f * shrink * (1.0 - keep);
+        out->turns[i] = g * turns;
     }
     return INFERNT_OK;
 }
