@@ -277,6 +277,14 @@ __device__ __forceinline__ void walk(const AttnArgs& a, const Place& p, F f) {
     }
 }
 
+// Tickets taken for a split item so far; what their CTAs wrote is visible to a
+// thread that has met this one at a barrier.
+__device__ __forceinline__ unsigned tickets_taken(const AttnArgs& a, const Part& part) {
+    unsigned n;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.tickets + part.first) : "memory");
+    return n;
+}
+
 // Whether some row of the item sees key p.
 __device__ __forceinline__ bool item_sees(const Item& it, int p) {
     return p < it.hi && (p >= it.lo || p < it.sink_end);

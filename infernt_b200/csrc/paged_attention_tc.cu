@@ -161,18 +161,19 @@ __device__ __forceinline__ bool put_result(uint32_t tile, int r, int c, float (&
 // Row ri (r of its row tile) of a split item, joined over its CTAs in order
 // into shared memory: kJoin parts of 32 columns are read at once, since each
 // read is a trip to L2.  A function of its own, so that its registers are not
-// the tiles' (two parts: three spill, 533 -> 609 us in the case above).
+// the tiles' (two parts: three spill, 533 -> 609 us in the case above).  Of CTA
+// own, m, l and O are still in its registers and TMEM (O when it had tiles).
 template <typename T, int D>
 __device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, int ri, uint32_t tile, int r, bool sees,
-                                      float* lse) {
+                                      float* lse, int own, bool some, uint32_t tm_o, float m_own, float l_own) {
     float M = -INFINITY, l = 0.0f;
     for (int b = first; b <= last; b += 4) {
         float mb[4], lb[4], top = M;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float* p = slot_of<kM, D>(a, min(b + i, last), first) + kM * D + ri;
-            mb[i] = __ldcg(p);
-            lb[i] = __ldcg(p + kM);
+            mb[i] = b + i == own ? m_own : __ldcg(p);
+            lb[i] = b + i == own ? l_own : __ldcg(p + kM);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -200,6 +201,16 @@ __device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, in
 #pragma unroll
             for (int i = 0; i < kJoin; ++i) {
                 if (b + i > last) break;
+                if (b + i == own) {
+                    mb[i] = m_own;
+                    float t[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) t[e] = 0.0f;
+                    if (some) tmem_ld32(tm_o + 32 * c, t);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] = make_float4(t[4 * e], t[4 * e + 1], t[4 * e + 2], t[4 * e + 3]);
+                    continue;
+                }
                 const float* p = slot_of<kM, D>(a, b + i, first);
                 mb[i] = __ldcg(p + kM * D + ri);
 #pragma unroll
@@ -233,7 +244,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     __shared__ Barriers bar;
     __shared__ uint32_t tmem_s;
     __shared__ int ok_s;
-    __shared__ int last_s;
+    __shared__ int last_s, early_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     if (tid == 0) {
@@ -419,6 +430,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 const int token = mine ? a.by_g(row) : 0, pos = mine ? row_pos(seq, token) : -1;
                 float m = -INFINITY, l = 0.0f;  // m in base 2
                 bool settled = false;           // every row of the warp has an m
+                unsigned taken = 0;
+                const bool split = part.first != part.last, some = part.j0 < part.j1 && rows_x > 0;
                 if (rows_x > 0 && part.j0 < part.j1) {
                     // Q rows of this warp: D / 8 lanes of 16 bytes a row, eight rounds in flight
                     {
@@ -555,15 +568,24 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         tc_fence_before();
                         mbar_arrive(&bar.p[x][b]);
                     }
+                    if (split && tid == 128) taken = tickets_taken(a, part);
                     tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
                 }
                 // ---- the part's result: straight to out, or through the slots
-                const bool split = part.first != part.last, some = part.j0 < part.j1 && rows_x > 0;
                 const int ri = 128 * x + r;
-                bool write = true;
+                bool write = true, early = false;
                 if (split) {
+                    // where all others have arrived, this CTA's part stays where it is
+                    if (tid == 128) {
+                        early_s = taken == (unsigned)(part.last - part.first);
+                        if (early_s) a.tickets[part.first] = 0u;  // ready for the next call
+                    }
+                    named_sync(1, kRowThreads);
+                    early = early_s != 0;
+                }
+                if (split && !early) {
                     // columns [4 c, 4 c + 4) of row ri at float4 c kM + ri: neighbours in a row of threads
                     float* slot = slot_of<kM, D>(a, blockIdx.x, part.first);
                     if (rows_x > 0) {
@@ -603,7 +625,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                                : nullptr;
                     // 32 columns at a time into the row tile's Q, which the products are done with
                     if (split) {
-                        bad = join_row<T, D>(a, part.first, part.last, ri, own, r, sees, lse);
+                        bad = join_row<T, D>(a, part.first, part.last, ri, own, r, sees, lse, early ? (int)blockIdx.x : -1, some,
+                                              tm_ox, m, l);
                     } else {
                         if (lse) *lse = sees ? (m + log2f(l)) * kLn2 : -INFINITY;
                         const float inv = sees ? 1.0f / l : 0.0f;
