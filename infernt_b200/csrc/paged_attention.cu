@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     constexpr int M = kItemRows, ST = L::kStages;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ Ring<ST> ring;
-    __shared__ int last_s;
+    __shared__ int last_s, early_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
     const uint32_t base = (smem_addr(smem) + 1023u) & ~1023u;
     float* scratch = reinterpret_cast<float*>(smem + (base - smem_addr(smem)) + L::kScratch);
@@ -443,6 +443,8 @@ __global__ void __launch_bounds__(kThreads, 2)
                 constexpr int RB = decltype(blocks)::value;
                 const RowState<D> s = consume<T, D, RB, BOXES>(a, seq, it, p, base, scratch, ring, st, turn, ok);
                 const bool split = p.first != p.last;
+                unsigned taken = 0;
+                if (split && tid == 0) taken = tickets_taken(a, p);
                 unsigned bad = 0;  // bit h: row g + 8 h is not finite
                 if (warp < RB) {
                     float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
@@ -478,8 +480,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                             }
                 }
                 if (!split) return;
-                named_sync(1, kConsumers);
+                // where all others have arrived already, no ticket is needed
                 if (tid == 0) {
+                    early_s = taken == (unsigned)(p.last - p.first);
+                    if (early_s) a.tickets[p.first] = 0u;  // ready for the next call
+                }
+                named_sync(1, kConsumers);
+                const bool early = early_s != 0;
+                if (!early && tid == 0) {
                     // the others' writes, ordered before by the barrier, become visible with this thread's fence
                     __threadfence();
                     unsigned* ticket = a.tickets + p.first;
@@ -487,8 +495,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                     if (last_s) *ticket = 0u;  // ready for the next call
                     __threadfence();
                 }
-                named_sync(1, kConsumers);
-                if (!last_s) return;
+                if (!early) {
+                    named_sync(1, kConsumers);
+                    if (!last_s) return;
+                }
                 // a warp a row, two columns a lane, two rows at once
                 for (int r = warp; r < it.rows; r += 2 * (kConsumers / 32)) {
                     const int r2 = r + kConsumers / 32;
