@@ -36,11 +36,11 @@
 // computed again with its own maximum, and O is rescaled if that has
 // passed m by more than 2^8.  P goes to TMEM eight columns at a time.
 //
-// 4096 tokens at 12288 positions (32/8 heads of 128, bf16): 533 us, 1288
-// TFLOP/s (627 us back to back, at the power limit); 594 with the maximum
+// 4096 tokens at 12288 positions (32/8 heads of 128, bf16): 529 us, 1299
+// TFLOP/s (613 us back to back, at the power limit); 594 with the maximum
 // searched beside the probabilities, 559 with P stored as a whole, 548 with
-// the join of split items in line with the tiles.  The tensor pipe is busy for
-// 80 % of it; a part of the 2^x on the FMA pipe
+// the join of split items in line with the tiles.  The busiest unit is at 77 %,
+// the special function unit at 64 %; a part of the 2^x on the FMA pipe
 // instead of the special function unit changes nothing any more, nor do
 // turns at the exponentials between the warps of a scheduler (622 us).
 #include <cmath>
@@ -161,7 +161,7 @@ __device__ __forceinline__ bool put_result(uint32_t tile, int r, int c, float (&
 // Row ri (r of its row tile) of a split item, joined over its CTAs in order
 // into shared memory: kJoin parts of 32 columns are read at once, since each
 // read is a trip to L2.  A function of its own, so that its registers are not
-// the tiles' (two parts: three spill, 533 -> 609 us in the case above).  Of CTA
+// the tiles' (two parts: three spill, 528 -> 609 us in the case above).  Of CTA
 // own, m, l and O are still in its registers and TMEM (O when it had tiles).
 template <typename T, int D>
 __device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, int ri, uint32_t tile, int r, bool sees,
