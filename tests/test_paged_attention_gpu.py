@@ -396,3 +396,18 @@ def test_long_context(torch, ws):
     """One token and a short chunk over 70000 positions (FP32 sums of many terms)."""
     c = run(Case(torch, [(1, 70001), (20, 66000)], 8, 1, 128, 64), ws)
     check_attention(c, rows=[0, 1, 19])
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [2, 90])
+def test_split_rows_with_a_hidden_value_that_is_not_finite(torch, ws, new, D):
+    """Items shared by many blocks, whose last token's value is not finite:
+    the joined rows before it are computed again, the last one shows it."""
+    n = 9000
+    c = Case(torch, [(new, n)], 4, 1, D, 64)
+    c.v[c.pages[0][(n - 1) // 64], 0, (n - 1) % 64, 3] = math.inf
+    for _ in range(2):
+        run(c, ws)
+        check_attention(c, rows=[0, new // 2 - 1, new - 2])
+        assert bool(torch.isinf(c.out[new - 1, :, 3]).all()) and bool(torch.isfinite(c.out[new - 1, :, 4:].float()).all())
+        assert int(c.err) == 0
