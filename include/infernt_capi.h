@@ -653,8 +653,9 @@ INFERNT_API int infernt_paged_rope_append(void* q_out, int ldo, const void* q, i
  * -infinity.  What lies in rows that a token does not see (unwritten rows of
  * a page, NaN, infinity) does not reach its output.  FP32 scores, softmax
  * statistics and sums; the probabilities enter the tensor cores in the
- * cache's type.  nq a multiple of num_kv_heads, at most 128 query heads per
- * KV head.
+ * cache's type (fp16: those below 2^-18 of a row's largest in steps of 2^-28
+ * of it).  nq a multiple of num_kv_heads, at most 128 query heads per KV
+ * head.
  * Table entries of pages that no new token sees are not read, so pages behind
  * a window may have been given back.
  * workspace: infernt_paged_attention_workspace_bytes() bytes, zeroed once

@@ -255,9 +255,10 @@ __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq
             for (int h = 0; h < 2; ++h) {
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * a.scale_log2;
+                mx[h] -= kShift<T>;
                 grow |= mx[h] > s.m[h] + kRescale;
             }
-            // the reference maximum moves only when probabilities would pass 2^8
+            // the reference moves only when probabilities would pass 2^(kRescale + kShift)
             if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

@@ -9,7 +9,23 @@
 
 namespace infernt {
 
-constexpr float kRescale = 8.0f;  // log2 of the largest unnormalised probability
+// A row's probabilities are 2^(s - m), s in base 2; m is the largest score met
+// less kShift, and moves when a score passes that one by kRescale.  The
+// tcgen05 kernel takes a tile's probabilities under an older m as long as
+// their sum is at most kMostSum.  Their common factor 2^kShift leaves out and
+// lse as they are and puts the probabilities where their 16 bits hold them:
+// bf16 as none above 1, so that sums of V's largest values stay finite; fp16
+// where a weight of 2^-18 of the row's largest is still a normal number and
+// what is lost of a smaller one is 2^-29 of the largest.  (At a shift of 0
+// that was 2^-25, and 2^15 such keys were two half-steps of the result.  A
+// higher shift lowers the sums that pass, and rows whose first tile shows them
+// few keys compute more of the next ones twice: two chunks of 2039 tokens with
+// a window of 1000, fp16, take 97 us at a shift of 5 and 2^15, 90 here.)
+constexpr float kRescale = 8.0f;
+template <typename T>
+constexpr float kShift = Half16<T>::kBf16 ? -13.0f : 4.0f;
+template <typename T>
+constexpr float kMostSum = Half16<T>::kBf16 ? 1.0f : 65504.0f;
 
 // Workspace: for each of the two kernels (a call may run both, the second
 // while the first ends) the tickets of split items, then two slots of partial

@@ -31,10 +31,11 @@
 //
 // The probabilities of a tile are computed with the m of the tiles before,
 // with no search for their maximum: any m gives the same result, so long as
-// the probabilities fit their 16 bits, and a tile whose sum stays below 2^13
-// does.  Where it does not (and for first keys and hidden ones) the tile is
-// computed again with its own maximum, and O is rescaled if that has
-// passed m by more than 2^8.  P goes to TMEM eight columns at a time.
+// the probabilities fit their 16 bits, and a tile whose sum is at most
+// kMostSum does.  Where it is not (and for first keys and hidden ones) the
+// tile is computed again with its own maximum, and O is rescaled if m moves: by
+// more than kRescale, or at all after such a sum, so that the next tiles pass.
+// P goes to TMEM eight columns at a time.
 //
 // 4096 tokens at 12288 positions (32/8 heads of 128, bf16): 529 us, 1299
 // TFLOP/s (613 us back to back, at the power limit); 594 with the maximum
@@ -59,7 +60,6 @@ namespace {
 
 constexpr int kM = kTcItemRows;  // query rows of an item
 constexpr int kN = kTcTileKeys;  // keys of a tile
-constexpr float kMostSum = 8192.0f;  // of a tile's probabilities: each then fits fp16
 constexpr int kThreadsTc = 384;
 constexpr int kJoin = 2;  // parts of a split item that are read at once
 constexpr int kRowThreads = 256;
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                             }
                             const float2 v = un2(add2(ls[0], ls[1]));
                             lsum = v.x + v.y;
-                            done = !__any_sync(0xffffffffu, !(lsum <= kMostSum));
+                            done = !__any_sync(0xffffffffu, !(lsum <= kMostSum<T>));
                         }
                         if (!done) {
                             tmem_st_wait();  // the stores that are made again
@@ -520,8 +520,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                 mx[0] = fmaxf(mx[0], fmaxf(sv[e], sv[e + 1]));
                                 mx[1] = fmaxf(mx[1], fmaxf(sv[e + 2], sv[e + 3]));
                             }
-                            const float top = fmaxf(mx[0], mx[1]) * sc;
-                            const bool grow = top > m + kRescale;
+                            const float top = fmaxf(mx[0], mx[1]) * sc - kShift<T>;
+                            const bool grow = top > m + (lsum > kMostSum<T> ? 0.0f : kRescale);
                             if (i == 0) {
                                 m = top;
                             } else if (__any_sync(0xffffffffu, grow)) {
