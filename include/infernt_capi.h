@@ -651,7 +651,9 @@ INFERNT_API int infernt_paged_rope_append(void* q_out, int ldo, const void* q, i
  * elements apart (multiples of 8, pointers 16-byte aligned, out apart from
  * q); lse [num_rows][nq] FP32 or NULL.  A row without a visible key gets zeros and an lse of
  * -infinity.  What lies in rows that a token does not see (unwritten rows of
- * a page, NaN, infinity) does not reach its output.  FP32 scores, softmax
+ * a page, NaN, infinity) does not reach its output.  A value that it does see
+ * and that is not finite makes its results in that column so (NaN in place of
+ * infinity where the value's weight is rounded to 0), at no cost in time.  FP32 scores, softmax
  * statistics and sums; the probabilities enter the tensor cores in the
  * cache's type (fp16: those below 2^-18 of a row's largest in steps of 2^-28
  * of it).  nq a multiple of num_kv_heads, at most 128 query heads per KV

@@ -83,7 +83,15 @@ struct Half16<__nv_bfloat16> {
         return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
     }
     static __device__ __forceinline__ __nv_bfloat16 round(float a) { return __float2bfloat16_rn(a); }
-    static __device__ __forceinline__ float value(__nv_bfloat16 a) { return __bfloat162float(a); }
+    static __device__ __forceinline__ uint32_t add_zero_times(uint32_t v, uint32_t sum) {
+        uint32_t r;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(sum));
+        return r;
+    }
+    // ones in each half that is infinite or NaN: an exponent of ones carries into the sign
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+        return ((((v & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu;
+    }
 };
 
 template <>
@@ -99,7 +107,14 @@ struct Half16<__half> {
                            __half2float(__ushort_as_half((unsigned short)(v >> 16))));
     }
     static __device__ __forceinline__ __half round(float a) { return __float2half_rn(a); }
-    static __device__ __forceinline__ float value(__half a) { return __half2float(a); }
+    static __device__ __forceinline__ uint32_t add_zero_times(uint32_t v, uint32_t sum) {
+        uint32_t r;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(v), "r"(0u), "r"(sum));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t not_finite(uint32_t v) {
+        return ((((v & 0x7c007c00u) + 0x04000400u) & 0x80008000u) >> 15) * 0xffffu;
+    }
 };
 
 // Lets kernel use `bytes` of dynamic shared memory: once a kernel and device,

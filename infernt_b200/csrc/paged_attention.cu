@@ -37,6 +37,7 @@ constexpr int kItemRows = 64;   // query rows of an item: four warps of 16
 constexpr int kConsumers = 128;
 constexpr int kThreads = kConsumers + 32;
 constexpr uint32_t kBlock = kTileKeys * 128;  // a block of 64 columns: rows of 128 bytes
+static_assert(kBlock == 8192, "as chunk_at has it");
 
 template <typename T>
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -71,11 +72,6 @@ template <int ST>
 struct Ring {
     uint64_t full[ST], empty[ST];
 };
-
-// Address of 16-byte chunk ch of a tile's row.
-__device__ __forceinline__ uint32_t chunk_at(uint32_t tile, int row, int ch) {
-    return tile + (uint32_t)(ch >> 3) * kBlock + (uint32_t)(row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-}
 
 // The producer warp: K and V tiles of the CTA's parts, in order.  BOXES: page
 // by page through the tensor maps (a page that no row sees, or that the pool
@@ -171,7 +167,8 @@ struct RowState {
 template <typename T, int D, int RB, bool BOXES>
 __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq& seq, const Item& it, const Part& part,
                                                uint32_t base, float* scratch, Ring<Layout<D>::kStages>& ring,
-                                               uint32_t& st, uint32_t& turn, bool& ok) {
+                                               uint32_t& st, uint32_t& turn, const Current* cur,
+                                               volatile int* found_in, bool& ok) {
     using L = Layout<D>;
     constexpr int KS = 4 / RB, WK = kTileKeys / KS, NT = WK / 8;  // key shares, keys and n-tiles of a warp
     constexpr int KC = D / 16, DB = D / 8, ST = L::kStages;
@@ -201,7 +198,7 @@ __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq
     }
 #pragma unroll
     for (int b = 0; b < DB; ++b) s.acc[b][0] = s.acc[b][1] = s.acc[b][2] = s.acc[b][3] = 0.0f;
-    const bool busy = rb * 16 < it.rows;
+    const bool busy = rb * 16 < it.rows, mixed = it.pos_first != it.pos_last;
 
 #pragma unroll 1
     for (int j = part.j0; j < part.j1; ++j) {
@@ -209,18 +206,9 @@ __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq
         const uint32_t kt = base + st * 2 * L::kTile, vt = kt + L::kTile;
         tc_wait_bar(&ring.full[st], turn, ok);
         if (busy) {
-            if (BOXES && (k0 + kTileKeys > it.hi || (k0 < it.lo && k0 + kTileKeys > it.sink_end))) {
-                // V rows of this warp's keys that no row of the item sees may
-                // hold anything, and 0 times infinity is not 0
-                for (int r = ks * WK + lane; r < (ks + 1) * WK; r += 32)
-                    if (!item_sees(it, k0 + r))
-#pragma unroll
-                        for (int c = 0; c < D / 8; ++c)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at(vt, r, c)), "r"(0)
-                                         : "memory");
-                fence_proxy_async_smem();  // before the stage is loaded again
-                __syncwarp();
-            }
+            const bool whole = seen_whole<kTileKeys>(a, it, k0);
+            if (!whole && (mixed || (BOXES && has_hidden<kTileKeys>(it, k0))))
+                clean_rows<T, D, WK>(cur[warp], k0, vt, ks * WK, mixed, found_in);
             float sc[NT][4];
 #pragma unroll
             for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
@@ -235,15 +223,12 @@ __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq
                     mma_16816<T>(sc[2 * n + 1], qa[k], b2, b3);
                 }
             // a tile that every row sees whole needs no mask
-            if (!(k0 + kTileKeys - 1 <= it.pos_first &&
-                  (a.window == 0 || k0 > it.pos_last - a.window || k0 + kTileKeys <= a.sinks))) {
+            if (!whole) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int p = k0 + ks * WK + 8 * n + 2 * tig + (e & 1), ph = pos[e >> 1];
-                        if (!(p <= ph && (a.window == 0 || p > ph - a.window || p < a.sinks))) sc[n][e] = -INFINITY;
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        if (!row_sees(a, pos[e >> 1], k0 + ks * WK + 8 * n + 2 * tig + (e & 1))) sc[n][e] = -INFINITY;
             }
             float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -361,9 +346,9 @@ __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq
     return s;
 }
 
-// Columns d and d + 1 of a row's result; true when it is not finite.
+// Columns d and d + 1 of a row's result.
 template <typename T, int D>
-__device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& seq, int kvh, int row, int d, Joined v) {
+__device__ __forceinline__ void write_pair(const AttnArgs& a, const PagedSeq& seq, int kvh, int row, int d, Joined v) {
     const int token = a.by_g(row), head = kvh * a.G + row - token * a.G;
     const bool sees = row_pos(seq, token) >= 0;
     const float inv = 1.0f / v.l;
@@ -373,7 +358,35 @@ __device__ __forceinline__ bool write_pair(const AttnArgs& a, const PagedSeq& se
     if (a.lse && d == 0)
         a.lse[(long long)(seq.row0 + token) * a.nq + head] =
             sees ? (v.m + log2f(v.l)) * kLn2 : -INFINITY;
-    return !(fabsf(x) < INFINITY && fabsf(y) < INFINITY);
+}
+
+// The values that clean_rows took out of a part's tiles, added to the results
+// of the rows r0 + g and r0 + g + 8 that see them: to this lane's columns, as it
+// has just written them to the slot, or to out.  (On memory, and with the part
+// read from shared memory: on registers in line with the tiles, 32 sequences
+// with a window of 4096 took 105 us, not 98.)
+template <typename T, int D>
+__device__ __noinline__ void restore_rows(const AttnArgs& a, const Current& cur, int row_base, int r0, float* slot) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
+    each_not_finite<T, D, kTileKeys>(a, cur, [&](int p, const T* v) {
+        for (int r = r0 + g; r < min(cur.it.rows, r0 + 16); r += 8) {
+            const int row = cur.it.row0 + r, token = a.by_g(row), head = cur.it.kvh * a.G + row - token * a.G;
+            if (!row_sees(a, cur.it.pos_first + token - a.by_g(cur.it.row0), p)) continue;
+            T* out = static_cast<T*>(a.out) + (long long)(row_base + token) * a.ldo + (long long)head * D;
+            for (int d = 2 * tig; d < D; d += 8) {
+                const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(v + d));
+                const float2 x = Half16<T>::unpack(w & Half16<T>::not_finite(w));
+                if (slot) {
+                    float2* at = reinterpret_cast<float2*>(slot + r * D + d);
+                    *at = make_float2(at->x + x.x, at->y + x.y);
+                } else {
+                    uint32_t* at = reinterpret_cast<uint32_t*>(out + d);
+                    const float2 o = Half16<T>::unpack(*at);
+                    *at = Half16<T>::pack(o.x + x.x, o.y + x.y);
+                }
+            }
+        }
+    });
 }
 
 // Columns d and d + 1 of row r of a split item, joined over its CTAs in order;
@@ -419,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     constexpr int M = kItemRows, ST = L::kStages;
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ Ring<ST> ring;
-    __shared__ int last_s, early_s;
+    __shared__ int last_s, early_s, found_s;  // found_s: the last part in which clean_rows found something
+    __shared__ Current cur_s[kConsumers / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
     const uint32_t base = (smem_addr(smem) + 1023u) & ~1023u;
     float* scratch = reinterpret_cast<float*>(smem + (base - smem_addr(smem)) + L::kScratch);
@@ -429,6 +443,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             mbar_init(&ring.empty[i], kConsumers / 32);
         }
         mbar_fence_init();
+        found_s = 0;
+        for (Current& c : cur_s) c.no = 0;
     }
     const Place place = find_place<M, kTileKeys, kThreads>(a);  // its barriers publish the set-up
     pdl_launch_dependents();  // the tcgen05 kernel may take SMs as they become free
@@ -439,14 +455,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else {
         uint32_t st = 0, turn = 0;
         walk<M, kTileKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
+            set_current(cur_s[warp], it, p);
             // the part, its rows' results and what becomes of them, for RB blocks of rows
             auto run = [&](auto blocks) {
                 constexpr int RB = decltype(blocks)::value;
-                const RowState<D> s = consume<T, D, RB, BOXES>(a, seq, it, p, base, scratch, ring, st, turn, ok);
+                const RowState<D> s = consume<T, D, RB, BOXES>(a, seq, it, p, base, scratch, ring, st, turn, cur_s,
+                                                                   &found_s, ok);
                 const bool split = p.first != p.last;
                 unsigned taken = 0;
                 if (split && tid == 0) taken = tickets_taken(a, p);
-                unsigned bad = 0;  // bit h: row g + 8 h is not finite
                 if (warp < RB) {
                     float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
 #pragma unroll
@@ -465,20 +482,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                         } else {
 #pragma unroll
                             for (int b = 0; b < D / 8; ++b)
-                                if (write_pair<T, D>(a, seq, it.kvh, it.row0 + r, 8 * b + 2 * tig,
-                                                     {s.m[h], s.l[h], s.acc[b][2 * h], s.acc[b][2 * h + 1]}))
-                                    bad |= 1u << h;
+                                write_pair<T, D>(a, seq, it.kvh, it.row0 + r, 8 * b + 2 * tig,
+                                                 {s.m[h], s.l[h], s.acc[b][2 * h], s.acc[b][2 * h + 1]});
                         }
                     }
-                    __syncwarp();
-                    if (!split)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            for (unsigned left = __ballot_sync(0xffffffffu, bad >> h & 1u); left;) {
-                                const int q = (__ffs(left) - 1) >> 2;  // row g of the warp's block
-                                exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + warp * 16 + q + 8 * h);
-                                left &= ~(15u << (4 * q));
-                            }
+                    // by this warp, or by one whose keys have met these rows at the barrier of their join
+                    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found_s) >= cur_s[warp].no))
+                        restore_rows<T, D>(a, cur_s[warp], seq.row0, warp * 16, split ? slot : nullptr);
                 }
                 if (!split) return;
                 // where all others have arrived already, no ticket is needed
@@ -503,17 +513,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                 // a warp a row, two columns a lane, two rows at once
                 for (int r = warp; r < it.rows; r += 2 * (kConsumers / 32)) {
                     const int r2 = r + kConsumers / 32;
-                    bool off = false, off2 = false;
 #pragma unroll
                     for (int d = 2 * lane; d < D; d += 64) {
                         const Joined v = join_slots<M, D>(a, p.first, p.last, r, d);
                         const Joined v2 = join_slots<M, D>(a, p.first, p.last, min(r2, it.rows - 1), d);
-                        off |= write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, v);
-                        if (r2 < it.rows) off2 |= write_pair<T, D>(a, seq, it.kvh, it.row0 + r2, d, v2);
+                        write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, v);
+                        if (r2 < it.rows) write_pair<T, D>(a, seq, it.kvh, it.row0 + r2, d, v2);
                     }
-                    __syncwarp();
-                    if (__any_sync(0xffffffffu, off)) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r);
-                    if (__any_sync(0xffffffffu, off2)) exact_row<T, D>(a, seq, p.s, it.kvh, it.row0 + r2);
                 }
             };
             if (it.rows <= 16)

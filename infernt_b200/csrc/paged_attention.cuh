@@ -1,6 +1,6 @@
 // paged_attention.cuh — what the two attention kernels over paged caches
 // share: the query rows and keys of an item, the even split of the work over
-// the CTAs, the partial results of split items, and the term-by-term row.
+// the CTAs, the partial results of split items, and values that are not finite.
 #pragma once
 
 #include <cuda.h>
@@ -348,45 +348,152 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// One row by one warp, term by term: what a row is computed with when its
-// result is not finite.  The tiles above multiply a hidden position's value
-// by a probability of 0, which is NaN where the value is infinite or NaN;
-// here only what the row sees is touched, so what a row does see that is not
-// finite still shows in its result as in the formula.
-template <typename T, int D>
-__device__ __noinline__ void exact_row(const AttnArgs& a, const PagedSeq& seq, int s, int kvh, int row) {
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31, token = a.by_g(row), head = kvh * a.G + row - token * a.G;
-    const int pos = row_pos(seq, token);
-    const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0, sink_end = min(a.sinks, lo);
-    const T* q = static_cast<const T*>(a.q) + (long long)(seq.row0 + token) * a.ldq + (long long)head * D + lane * E;
-    float qv[E], acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        qv[e] = Half16<T>::value(q[e]);
-        acc[e] = 0.0f;
+// ------------------------------------------------- values that are not finite
+// A tile multiplies the value of a key that a row does not see by a
+// probability of 0, which is NaN where the value is infinite or NaN.  So V
+// rows that no row of the item sees become zeros in shared memory, and where
+// some rows see a key that others do not, so do its values that are not
+// finite.  Those are then added to the sums of the rows that see them
+// (restore_*): w V is V for any w > 0.  That is work for the few tiles at the
+// ends of an item's keys alone, whatever V holds and however long the cache,
+// so no wait of these kernels depends on it.  In tiles that every row sees
+// whole the products give what the formula does.
+
+__device__ __forceinline__ bool row_sees(const AttnArgs& a, int pos, int p) {
+    return p <= pos && (a.window == 0 || p > pos - a.window || p < a.sinks);
+}
+
+// Whether every row of the item sees all N keys of the tile at k0.  Where not,
+// and the item has several positions, some rows may see a key that others do
+// not.
+template <int N>
+__device__ __forceinline__ bool seen_whole(const AttnArgs& a, const Item& it, int k0) {
+    return k0 + N - 1 <= it.pos_first && (a.window == 0 || k0 > it.pos_last - a.window || k0 + N <= a.sinks);
+}
+
+// Whether the tile at k0 has keys that no row of the item sees.
+template <int N>
+__device__ __forceinline__ bool has_hidden(const Item& it, int k0) {
+    return k0 + N > it.hi || (k0 < it.lo && k0 + N > it.sink_end);
+}
+
+// Address of 16-byte chunk ch of row `row` of a tile of 64 rows in shared
+// memory: blocks of 64 columns, rows of 128 bytes, as a tensor map with
+// 128-byte swizzle writes them.
+__device__ __forceinline__ uint32_t chunk_at(uint32_t tile, int row, int ch) {
+    return tile + (uint32_t)(ch >> 3) * 8192u + (uint32_t)(row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ uint4 ld_shared(uint32_t at) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                 : "r"(at)
+                 : "memory");
+    return w;
+}
+__device__ __forceinline__ void st_shared(uint32_t at, uint4 w) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                 : "memory");
+}
+
+// Ones where eight values are not finite.
+template <typename T>
+__device__ __forceinline__ uint4 not_finite(uint4 w) {
+    return make_uint4(Half16<T>::not_finite(w.x), Half16<T>::not_finite(w.y), Half16<T>::not_finite(w.z),
+                      Half16<T>::not_finite(w.w));
+}
+__device__ __forceinline__ bool any_bit(uint4 w) { return (w.x | w.y | w.z | w.w) != 0u; }
+
+// A warp's part, in shared memory for what runs rarely: the loops over the
+// tiles then need not keep all of it in registers.
+struct Current {
+    Item it;
+    Part part;
+    int no;  // counts the parts
+};
+__device__ __forceinline__ void set_current(Current& cur, const Item& it, const Part& part) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+        cur.it = it;
+        cur.part = part;
+        ++cur.no;
     }
-    float m = -INFINITY, l = 0.0f;
-    for (int p = 0; p <= pos; ++p) {
-        if (p == sink_end) p = lo;  // lo <= pos
-        const int r = pool_row(a.b, s, kvh, p, a.err);
-        const T* k = static_cast<const T*>(a.k) + (long long)r * D + lane * E;
-        const T* v = static_cast<const T*>(a.v) + (long long)r * D + lane * E;
-        float dot = 0.0f;
+    __syncwarp();
+}
+
+// The rows [r0, r0 + ROWS) of the V tile of keys k0 ... by a warp: zeros in
+// rows that no row of the item sees and, where `some`, for values that are not
+// finite.  When there were any, *found_in is the part before they go, so that a
+// warp that cleans the same rows and meets them gone finds it there.
+template <typename T, int D, int ROWS>
+__device__ __noinline__ void clean_rows(const Current& cur, int k0, uint32_t tile, int r0, bool some,
+                                        volatile int* found_in) {
+    constexpr int kAtOnce = ROWS < 32 ? ROWS : 32, kPerLane = D / 8 * kAtOnce / 32;  // rows; chunks of a lane's row
+    static_assert(kPerLane % 4 == 0, "");
+    const int lane = threadIdx.x & 31, c0 = lane / kAtOnce * kPerLane;
+    const Item it = cur.it;
+    // 0 v is 0, or NaN where v is not finite: one step for two values
+    uint32_t sum[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int e = 0; e < E; ++e) dot = fmaf(qv[e], r >= 0 ? Half16<T>::value(k[e]) : 0.0f, dot);
-        const float sc = warp_sum(dot) * a.scale, m_new = fmaxf(m, sc);
-        // e^-infinity is 0, before the row has met a finite score too
-        const float f = m == -INFINITY ? 0.0f : expf(m - m_new), w = sc == -INFINITY ? 0.0f : expf(sc - m_new);
-        l = l * f + w;
+    for (int h = 0; h < ROWS; h += kAtOnce) {
+        const int r = r0 + h + lane % kAtOnce;
+        if (!item_sees(it, k0 + r)) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * f + w * (r >= 0 ? Half16<T>::value(v[e]) : 0.0f);
-        m = m_new;
+            for (int c = 0; c < kPerLane; ++c) st_shared(chunk_at(tile, r, c0 + c), make_uint4(0u, 0u, 0u, 0u));
+        } else if (some) {
+#pragma unroll
+            for (int c = 0; c < kPerLane; c += 4) {
+                uint4 w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = ld_shared(chunk_at(tile, r, c0 + c + i));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum[0] = Half16<T>::add_zero_times(w[i].x, sum[0]);
+                    sum[1] = Half16<T>::add_zero_times(w[i].y, sum[1]);
+                    sum[2] = Half16<T>::add_zero_times(w[i].z, sum[2]);
+                    sum[3] = Half16<T>::add_zero_times(w[i].w, sum[3]);
+                }
+            }
+        }
     }
-    T* o = static_cast<T*>(a.out) + (long long)(seq.row0 + token) * a.ldo + (long long)head * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = Half16<T>::round(acc[e] / l);
-    if (a.lse && lane == 0) a.lse[(long long)(seq.row0 + token) * a.nq + head] = m + logf(l);
+    if (__any_sync(0xffffffffu, any_bit(not_finite<T>(make_uint4(sum[0], sum[1], sum[2], sum[3]))))) {
+        if (lane == 0) *found_in = cur.no;
+        __threadfence_block();
+        __syncwarp();
+        for (int i = lane; i < ROWS * (D / 8); i += 32) {
+            const uint32_t at = chunk_at(tile, r0 + i % ROWS, i / ROWS);
+            const uint4 w = ld_shared(at), x = not_finite<T>(w);
+            if (any_bit(x)) st_shared(at, make_uint4(w.x & ~x.x, w.y & ~x.y, w.z & ~x.z, w.w & ~x.w));
+        }
+    }
+    fence_proxy_async_smem();  // before the products read the tile, and before it is loaded again
+    __syncwarp();
+}
+
+// f(key, its V row in the pool) for the keys of a part's tiles that some rows
+// may see and others not, and that have values that are not finite, by a whole
+// warp.
+template <typename T, int D, int N, typename F>
+__device__ __forceinline__ void each_not_finite(const AttnArgs& a, const Current& cur, F f) {
+    const int lane = threadIdx.x & 31;
+    const Item& it = cur.it;
+    for (int j = cur.part.j0; j < cur.part.j1; ++j) {
+        const int k0 = tile_key<N>(it, j);
+        if (seen_whole<N>(a, it, k0)) continue;
+        for (int h = 0; h < N; h += 32) {
+            const int p = k0 + h + lane, row = item_sees(it, p) ? pool_row(a.b, cur.part.s, it.kvh, p, nullptr) : -1;
+            bool bad = false;
+            if (row >= 0) {
+                const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v) + (long long)row * D);
+#pragma unroll 4
+                for (int c = 0; c < D / 8; ++c) bad |= any_bit(not_finite<T>(__ldg(v + c)));
+            }
+            for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1) {
+                const int k = __ffs(left) - 1;
+                f(k0 + h + k, static_cast<const T*>(a.v) + (long long)__shfl_sync(0xffffffffu, row, k) * D);
+            }
+        }
+    }
 }
 
 // Joined values of row r, columns d and d + 1, of an item's partial results.

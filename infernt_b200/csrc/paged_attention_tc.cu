@@ -23,9 +23,9 @@
 // Twelve warps: warp 0 loads K and V tiles page by page by TMA (a tensor map
 // of the pool [page][KV head][position][dim]; a page that no row sees, or that
 // the pool does not have, is a coordinate past its end and becomes zeros),
-// warps 1 and 3 issue the MMAs of A and of B, warp 2 zeroes V rows that no
-// row of the item sees (so that what lies there does not meet a probability
-// of 0), warps 4-7 and 8-11 hold the rows of A and B.  Of the 384 x 168
+// warps 1 and 3 issue the MMAs of A and of B, warp 2 takes out of V what must
+// not meet a probability of 0 (clean_rows), warps 4-7 and 8-11 hold the rows of
+// A and B.  Of the 384 x 168
 // registers of a launch the first four warps keep 88 a thread, the others
 // take 208.
 //
@@ -64,7 +64,7 @@ constexpr int kThreadsTc = 384;
 constexpr int kJoin = 2;  // parts of a split item that are read at once
 constexpr int kRowThreads = 256;
 constexpr uint32_t kBoxQ = 16384;  // 128 rows of 64 values: a swizzled operand block
-constexpr uint32_t kBox = 8192;    // 64 rows
+constexpr uint32_t kBox = 8192;    // 64 rows: a block of chunk_at
 
 // Shared memory: Q of both row tiles, then the stages of K and of V tiles,
 // each of D / 64 blocks.
@@ -109,53 +109,46 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
     return r;
 }
 
-// Whether the tile at key k0 has keys that no row of the item sees.
-__device__ __forceinline__ bool has_hidden(const Item& it, int k0) {
-    return k0 + kN > it.hi || (k0 < it.lo && k0 + kN > it.sink_end);
-}
-
-// V rows of a tile in shared memory at v that no row of the item sees, by a
-// warp: they may hold anything, and 0 times infinity is not 0.
-template <int NB>
-__device__ __forceinline__ void zero_rows(const Item& it, int k0, uint32_t v) {
-    for (int r = threadIdx.x & 31; r < kN; r += 32)
-        if (!item_sees(it, k0 + r))
-#pragma unroll
-            for (int c = 0; c < NB * 8; ++c)  // every lane another 16-byte column
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(v + (c >> 3) * kBox + r * 128 +
-                                                                             (((c ^ r) & 7) << 4)),
-                             "r"(0)
-                             : "memory");
-    fence_proxy_async_smem();
-    __syncwarp();
-}
-
 // 16-byte chunk c of row r of a row tile's Q (and, at the end, its result) at
 // `tile` in shared memory.
 __device__ __forceinline__ uint32_t row_chunk(uint32_t tile, int r, int c) {
     return tile + (c >> 3) * kBoxQ + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
-__device__ __forceinline__ void st_shared(uint32_t at, uint4 w) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
-                 : "memory");
-}
 
-// 32 columns of a result, the chunks from c on of row r; true when one is not
-// finite.
+// 32 columns of a result, the chunks from c on of row r.
 template <typename T>
-__device__ __forceinline__ bool put_result(uint32_t tile, int r, int c, float (&o)[32], bool sees, float inv) {
-    bool bad = false;
+__device__ __forceinline__ void put_result(uint32_t tile, int r, int c, float (&o)[32], bool sees, float inv) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-        o[e] = sees ? o[e] * inv : 0.0f;
-        bad |= !(fabsf(o[e]) < INFINITY);
-    }
+    for (int e = 0; e < 32; ++e) o[e] = sees ? o[e] * inv : 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         st_shared(row_chunk(tile, r, c + e),
                   make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]), Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
                              Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]), Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
-    return bad;
+}
+
+// The values that clean_rows took out of a part's tiles, added to O of the
+// row at pos (a row of tm_o a lane) where the row sees them.
+template <typename T, int D>
+__device__ __noinline__ void restore_values(const AttnArgs& a, const Current& cur, int pos, uint32_t tm_o) {
+    each_not_finite<T, D, kN>(a, cur, [&](int p, const T* v) {
+        const bool sees = row_sees(a, pos, p);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            uint32_t w[32];
+            tmem_ld32(tm_o + 32 * c, o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t x = __ldg(reinterpret_cast<const uint32_t*>(v + 32 * c) + e);
+                const float2 y = Half16<T>::unpack(x & Half16<T>::not_finite(x));
+                w[2 * e] = __float_as_uint(sees ? o[2 * e] + y.x : o[2 * e]);
+                w[2 * e + 1] = __float_as_uint(sees ? o[2 * e + 1] + y.y : o[2 * e + 1]);
+            }
+            tmem_st32(tm_o + 32 * c, w);
+            tmem_st_wait();
+        }
+    });
 }
 
 // Row ri (r of its row tile) of a split item, joined over its CTAs in order
@@ -164,7 +157,7 @@ __device__ __forceinline__ bool put_result(uint32_t tile, int r, int c, float (&
 // the tiles' (two parts: three spill, 528 -> 609 us in the case above).  Of CTA
 // own, m, l and O are still in its registers and TMEM (O when it had tiles).
 template <typename T, int D>
-__device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, int ri, uint32_t tile, int r, bool sees,
+__device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, int ri, uint32_t tile, int r, bool sees,
                                       float* lse, int own, bool some, uint32_t tm_o, float m_own, float l_own) {
     float M = -INFINITY, l = 0.0f;
     for (int b = first; b <= last; b += 4) {
@@ -188,7 +181,6 @@ __device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, in
     }
     if (lse) *lse = sees ? (M + log2f(l)) * kLn2 : -INFINITY;
     const float inv = 1.0f / l;
-    bool bad = false;
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
         float o[32];
@@ -229,9 +221,8 @@ __device__ __noinline__ bool join_row(const AttnArgs& a, int first, int last, in
                 }
             }
         }
-        bad |= put_result<T>(tile, r, 4 * c, o, sees, inv);
+        put_result<T>(tile, r, 4 * c, o, sees, inv);
     }
-    return bad;
 }
 
 template <typename T, int D>
@@ -244,7 +235,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     __shared__ Barriers bar;
     __shared__ uint32_t tmem_s;
     __shared__ int ok_s;
-    __shared__ int last_s, early_s;
+    __shared__ int last_s, early_s, found_s;  // found_s: the last part in which clean_rows found something
+    __shared__ Current cur_s[kThreadsTc / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     if (tid == 0) {
@@ -265,6 +257,8 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         }
         mbar_fence_init();
         ok_s = 1;
+        found_s = 0;
+        for (Current& c : cur_s) c.no = 0;
     }
     if (warp == 1) tmem_alloc(&tmem_s, 512);
     const Place place = find_place<kM, kN, kThreadsTc>(a);  // its barriers publish the set-up
@@ -394,16 +388,19 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 __syncwarp();
             });
         } else if (warp == 2 && place.s >= 0) {
-            // ---- V rows that no row of the item sees become zeros
+            // ---- what of V must not meet a probability of 0 becomes zeros
             uint32_t n = 0;
             walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+                set_current(cur_s[2], it, part);
+                const bool mixed = it.pos_first != it.pos_last;
                 for (int j = part.j0; j < part.j1; ++j, ++n) {
                     const int k0 = tile_key<kN>(it, j);
                     const uint32_t st = n % ST;
                     tc_wait_bar(&bar.full_v[st], (n / ST) & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) return;
-                    if (has_hidden(it, k0)) zero_rows<NB>(it, k0, base + L::kV + st * L::kTile);
+                    if (!seen_whole<kN>(a, it, k0) && (mixed || has_hidden<kN>(it, k0)))
+                        clean_rows<T, D, kN>(cur_s[2], k0, base + L::kV + st * L::kTile, 0, mixed, &found_s);
                     if (lane == 0) mbar_arrive(&bar.clean_v[st]);
                 }
             });
@@ -422,6 +419,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             const uint32_t own = base + L::kQ + x * L::kTileQ;  // the row tile's Q
             uint32_t n = 0;  // key tiles of this row tile so far
             walk<kM, kN>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& part) {
+                set_current(cur_s[warp], it, part);
                 // A wait that runs out ends the work on the scores, but not the barriers
                 // that the threads of both row tiles meet at.
                 const int rows_x = it.rows - 128 * x;  // rows of this tile (of 128)
@@ -466,8 +464,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         float sv[kN];
                         tmem_ld64(tm_score(x, b) + lanes, sv);
                         // keys that every row of the item sees need no mask
-                        const bool whole = k0 + kN - 1 <= it.pos_first &&
-                                           (a.window == 0 || k0 > it.pos_last - a.window || k0 + kN <= a.sinks);
+                        const bool whole = seen_whole<kN>(a, it, k0);
                         // at head_dim 64 P's columns are free once P V of two tiles ago is done
                         if (D == 64 && i >= 2) {
                             tc_wait_bar(&bar.o[x][b], ((n - 2) >> 1) & 1u, ok);
@@ -572,6 +569,9 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     tc_wait_bar(&bar.o[x][(n - 1) & 1u], ((n - 1) >> 1) & 1u, ok);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
+                    // written before V was ready for the products that this thread has waited for
+                    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found_s) >= cur_s[warp].no))
+                        restore_values<T, D>(a, cur_s[warp], pos, tm_ox);
                 }
                 // ---- the part's result: straight to out, or through the slots
                 const int ri = 128 * x + r;
@@ -619,13 +619,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 if (write && rows_x > 0) {
                     const bool sees = mine && pos >= 0;
-                    bool bad = false;
                     float* lse = mine && a.lse ? a.lse + (long long)(seq.row0 + token) * a.nq + it.kvh * a.G + row -
                                                      token * a.G
                                                : nullptr;
                     // 32 columns at a time into the row tile's Q, which the products are done with
                     if (split) {
-                        bad = join_row<T, D>(a, part.first, part.last, ri, own, r, sees, lse, early ? (int)blockIdx.x : -1, some,
+                        join_row<T, D>(a, part.first, part.last, ri, own, r, sees, lse, early ? (int)blockIdx.x : -1, some,
                                               tm_ox, m, l);
                     } else {
                         if (lse) *lse = sees ? (m + log2f(l)) * kLn2 : -INFINITY;
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
                             for (int e = 0; e < 32; ++e) o[e] = 0.0f;
                             if (some) tmem_ld32(tm_ox + 32 * c, o);
-                            bad |= put_result<T>(own, r, 4 * c, o, sees, inv);
+                            put_result<T>(own, r, 4 * c, o, sees, inv);
                         }
                     }
                     __syncwarp();
@@ -656,9 +655,6 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                         }
                     }
                     __syncwarp();
-                    // rows that met something not finite, term by term
-                    for (unsigned left = __ballot_sync(0xffffffffu, bad); left; left &= left - 1)
-                        exact_row<T, D>(a, seq, part.s, it.kvh, it.row0 + 128 * x + 32 * quarter + __ffs(left) - 1);
                 }
                 // O, S and the slots' flag are read before the next part begins
                 tc_fence_before();

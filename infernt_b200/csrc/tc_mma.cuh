@@ -12,7 +12,10 @@
 namespace infernt {
 
 // Clock limit of a wait (about a second); every wait of these kernels is
-// bounded by it.
+// bounded by it.  The longest work that one waits for is the end of a part:
+// the join of an item over all CTAs (about 300 slots, some 10^6 cycles) or the
+// values that are not finite of a dozen tiles (768 keys of some 800 cycles);
+// neither grows with the cache.
 constexpr long long kTcWaitCycles = 2000000000ll;
 
 // Waits for phase `parity` of bar unless an earlier wait has run out.
