@@ -557,8 +557,7 @@ INFERNT_API int infernt_batch_attention(const float* q, const void* k_cache, con
  * in the reference (its caches are contiguous, one sequence each,
  * include/kv_cache.h:7-15; cuda/rope.cu:13-34, cuda/kv_cache.cu:4-14 and
  * cuda/attention.cu:9-42 are the arithmetic per token).  Every data pointer
- * must be device or managed memory of the current device; others are refused
- * (of a copy's pools, the first is looked at).
+ * must be device or managed memory of the current device; others are refused.
  *
  * The pools of one layer: K and V [num_pages][num_kv_heads][page_size]
  * [head_dim], 16-byte aligned, of type INFERNT_DTYPE_BF16 or _F16. */

@@ -47,6 +47,9 @@ int bt_fill_kv_launch(uint16_t* cache, int seq, int layer, int nkv, int max_seq,
                       float std_dev, int h0, int nkv_all, cudaStream_t st, const int* pages, int page_size);
 int bt_page_copy_launch(uint16_t* pool, uint16_t* flat, const int* pages, int page_size, int nkv, int max_seq, int D,
                         int p0, int p1, bool to_pages, cudaStream_t st);
+// known: the pools are this library's own and need no look at their addresses
+int pages_copy_launch(void* const* pools, int n_pools, size_t page_bytes, int num_pages, const int* src, const int* dst,
+                      int n, bool known, cudaStream_t st);
 int bt_argmax_launch(const float* logits, int T, int V, int* tokens, int* positions, int* hist, float* cand_v,
                      int* cand_i, unsigned* tickets, float inv_t, uint64_t seed, cudaStream_t st,
                      const uint64_t* salts);
@@ -865,8 +868,9 @@ int infernt_batch_engine_copy_pages(infernt_batch_engine* e, const int* src, con
     } catch (const std::bad_alloc&) {
         return fail(INFERNT_ERR_OUT_OF_MEMORY, "batch_engine_copy_pages: host allocation failed");
     }
-    return infernt_pages_copy(pools.data(), (int)pools.size(), (size_t)e->nkv_l * e->page_size * e->cfg.head_dim * 2,
-                              e->num_pages, src, dst, n, e->stream);
+    return infernt::pages_copy_launch(pools.data(), (int)pools.size(),
+                                      (size_t)e->nkv_l * e->page_size * e->cfg.head_dim * 2, e->num_pages, src, dst, n,
+                                      true, e->stream);
 }
 
 int infernt_batch_engine_set_salts(infernt_batch_engine* e, const uint64_t* salts) {

@@ -11,6 +11,8 @@
 #include <new>
 #include <vector>
 
+#include <cudaTypedefs.h>
+
 #include "common.cuh"
 #include "internal.h"
 #include "paged.cuh"
@@ -56,12 +58,31 @@ int launch_copy(void* const* pools, int n_pools, size_t page_bytes, const int* s
     return INFERNT_OK;
 }
 
-}  // namespace
-}  // namespace infernt
+// Every pool must be memory that the current device reads in place.  Pools that
+// begin in an allocation that has been looked at are: layers of one tensor,
+// most often (a look at each of 64 pools takes 8 us, as long as the call).
+int check_pools(void* const* pools, int n_pools) {
+    static const auto range_of = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuMemGetAddressRange", &f, cudaEnableDefault, &found) != cudaSuccess) f = nullptr;
+        return reinterpret_cast<PFN_cuMemGetAddressRange_v3020>(f);
+    }();
+    CUdeviceptr base = 0;
+    size_t bytes = 0;
+    for (int i = 0; i < n_pools; ++i) {
+        const CUdeviceptr p = reinterpret_cast<CUdeviceptr>(pools[i]);
+        if (p >= base && p - base < bytes) continue;
+        if (int s = check_device_pointer("pages_copy", "a pool", pools[i])) return s;
+        if (i + 1 < n_pools && (!range_of || range_of(&base, &bytes, p) != CUDA_SUCCESS)) bytes = 0;
+    }
+    return INFERNT_OK;
+}
 
-extern "C" int infernt_pages_copy(void* const* pools, int n_pools, size_t page_bytes, int num_pages, const int* src,
-                                  const int* dst, int n, void* stream) {
-    using namespace infernt;
+}  // namespace
+
+int pages_copy_launch(void* const* pools, int n_pools, size_t page_bytes, int num_pages, const int* src, const int* dst,
+                      int n, bool known, cudaStream_t st) {
     INFERNT_REQUIRE(n_pools >= 0 && n >= 0 && num_pages >= 1, "pages_copy: %d pools of %d pages, %d copies", n_pools,
                     num_pages, n);
     INFERNT_REQUIRE((n_pools == 0 || pools) && (n == 0 || (src && dst)), "pages_copy: null array");
@@ -92,10 +113,17 @@ extern "C" int infernt_pages_copy(void* const* pools, int n_pools, size_t page_b
     }
     INFERNT_REQUIRE(clash < 0, "pages_copy: page %d is a destination twice, or a source too", clash);
     if (n_pools == 0 || n == 0) return INFERNT_OK;
-    // the first speaks for the others: to look at 64 pools takes as long as the call (8 us)
-    if (int s = check_device_pointer("pages_copy", "the first pool", pools[0])) return s;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!known)
+        if (int s = check_pools(pools, n_pools)) return s;
     // a short list keeps the parameters of a fork's launch small
     if (n_pools <= 64 && n <= 32) return launch_copy<64, 32>(pools, n_pools, page_bytes, src, dst, n, st);
     return launch_copy<256, 2048>(pools, n_pools, page_bytes, src, dst, n, st);
+}
+
+}  // namespace infernt
+
+extern "C" int infernt_pages_copy(void* const* pools, int n_pools, size_t page_bytes, int num_pages, const int* src,
+                                  const int* dst, int n, void* stream) {
+    return infernt::pages_copy_launch(pools, n_pools, page_bytes, num_pages, src, dst, n, false,
+                                      static_cast<cudaStream_t>(stream));
 }
