@@ -899,6 +899,21 @@ def _dtype(t):
 
 _struct_init = ctypes.Structure.__init__
 _byref = ctypes.byref
+_raw_stream = None
+
+
+def _current_stream(t):
+    """torch's current stream on the device of tensor t, as an integer (None
+    for a host tensor: the call refuses it)."""
+    global _raw_stream
+    device = t.get_device()
+    if device < 0:
+        return None
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: torch.cuda.current_stream(d).cuda_stream)
+    return _raw_stream(device)
 
 
 class PagedCache(ctypes.Structure):
@@ -971,7 +986,8 @@ def _rows(t, rows, heads, dim, what):
 def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
     """Rotary positions of the batch's q rows into q_out, the rotated k rows
     and the v rows into their pages (infernt_paged_rope_append).  q and q_out,
-    or k and v, may be None.  stream: a cudaStream_t as an integer."""
+    or k and v, may be None.  stream: a cudaStream_t as an integer; without it,
+    torch's current stream."""
     n, dim, src = batch.num_rows, cache.head_dim, None
     qp = op = kp = vp = None
     nq = ldo = ldq = ldk = ldv = 0
@@ -985,6 +1001,8 @@ def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None)
         ldk, ldv = _rows(k, n, nkv, dim, "k"), _rows(v, n, nkv, dim, "v")
         if v.dtype != t or (src is not None and src != t):
             raise ValueError("paged_rope_append: q, k and v of different types")
+    if stream is None:
+        stream = _current_stream(q if k is None else k)
     status = (_lib or lib()).infernt_paged_rope_append(
         op, ldo, qp, ldq, nq, kp, ldk, vp, ldv, _dtype(q if k is None else k), _byref(cache), _byref(batch),
         _byref(rope), None if err is None else err.data_ptr(), stream)
@@ -1005,7 +1023,8 @@ def paged_attention_workspace_bytes():
 def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.0, lse=None, err=None, stream=None):
     """Attention of the batch's new tokens over the pages
     (infernt_paged_attention).  workspace: a zeroed tensor of
-    paged_attention_workspace_bytes() bytes."""
+    paged_attention_workspace_bytes() bytes.  stream: a cudaStream_t as an
+    integer; without it, torch's current stream."""
     n, dim, nq, lp = batch.num_rows, cache.head_dim, q.shape[1], None
     if _dtype(q) != cache.dtype or q.dtype != out.dtype:
         raise ValueError("paged_attention: q, out and the cache must have one type")
@@ -1015,6 +1034,8 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
             raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(shape), n, nq))
     if workspace.nbytes < (_workspace_bytes or paged_attention_workspace_bytes()):
         raise ValueError("paged_attention: a workspace of %d bytes is needed" % paged_attention_workspace_bytes())
+    if stream is None:
+        stream = _current_stream(q)
     status = (_lib or lib()).infernt_paged_attention(
         out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(), _rows(q, n, nq, dim, "q"), nq, _byref(cache),
         _byref(batch), window, sinks, scale, lp, workspace.data_ptr(), None if err is None else err.data_ptr(), stream)
@@ -1025,7 +1046,8 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
 def copy_pages(pools, src, dst, stream=None):
     """Page src[i] into page dst[i] in every pool (infernt_pages_copy): a
     contiguous tensor [pools][pages][...], or a list of contiguous tensors
-    [pages][...] of one shape and type."""
+    [pages][...] of one shape and type.  stream: a cudaStream_t as an integer;
+    without it, torch's current stream."""
     n = len(src)
     if n != len(dst):
         raise ValueError("copy_pages: %d sources, %d destinations" % (n, len(dst)))
@@ -1038,6 +1060,7 @@ def copy_pages(pools, src, dst, stream=None):
                for p in pools):
             raise ValueError("copy_pages: the pools must be contiguous tensors of one shape, type and device")
         base = [p.data_ptr() for p in pools]
+        pools = first
         pages, size = shape[0], first.nbytes
     else:
         if not pools.is_contiguous() or pools.dim() < 3:
@@ -1045,6 +1068,8 @@ def copy_pages(pools, src, dst, stream=None):
         count, pages = pools.shape[:2]
         size, start = pools.nbytes // max(1, count), pools.data_ptr()
         base = range(start, start + count * size, size) if size else ()
+    if stream is None:
+        stream = _current_stream(pools)
     call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, (_I * n)(*src), (_I * n)(*dst), n,
          stream)
 
