@@ -611,7 +611,7 @@ typedef struct infernt_ragged_batch {
  *   YARN    f / factor for the pairs of few turns (`low`, usually 1), f for
  *           those of many (`high`, usually 32), a ramp over the pair index
  *           between the two borders; cosine and sine multiplied by
- *           0.1 ln(factor) + 1
+ *           0.1 ln(factor) + 1 (1 for a factor below 1)
  * Angles are reduced in 64 bits, so far positions lose nothing. */
 enum { INFERNT_ROPE_NONE = 0, INFERNT_ROPE_LINEAR = 1, INFERNT_ROPE_LLAMA3 = 2, INFERNT_ROPE_YARN = 3 };
 typedef struct infernt_rope_params {

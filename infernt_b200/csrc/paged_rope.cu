@@ -339,7 +339,8 @@ int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
         };
         lo = std::fmax(0.0, std::floor(border(p.high)));
         hi = std::fmin(R - 1.0, std::ceil(border(p.low)));
-        out->magnitude = (float)(0.1 * std::log(p.factor) + 1.0);
+        // a factor up to 1 stretches nothing, and its logarithm would shrink or flip q and k
+        out->magnitude = p.factor > 1.0 ? (float)(0.1 * std::log(p.factor) + 1.0) : 1.0f;
     }
     // f_i by repeated products: 64 of them are off by 64 x 2^-53; divisions
     // stay out of the loop, which runs at each call
