@@ -983,6 +983,15 @@ def _rows(t, rows, heads, dim, what):
     return strides[0] if shape[0] > 1 else heads * dim  # one row has no stride of its own
 
 
+def _err_word(err):
+    """Address of an error word (None: none)."""
+    if err is None:
+        return None
+    if _dtype(err) != -1 or err.numel() < 1:
+        raise ValueError("err: an int32 tensor of one element is needed")
+    return err.data_ptr()
+
+
 def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
     """Rotary positions of the batch's q rows into q_out, the rotated k rows
     and the v rows into their pages (infernt_paged_rope_append).  q and q_out,
@@ -1005,7 +1014,7 @@ def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None)
         stream = _current_stream(q if k is None else k)
     status = (_lib or lib()).infernt_paged_rope_append(
         op, ldo, qp, ldq, nq, kp, ldk, vp, ldv, _dtype(q if k is None else k), _byref(cache), _byref(batch),
-        _byref(rope), None if err is None else err.data_ptr(), stream)
+        _byref(rope), _err_word(err), stream)
     if status:
         check(status, "infernt_paged_rope_append")
 
@@ -1038,7 +1047,7 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
         stream = _current_stream(q)
     status = (_lib or lib()).infernt_paged_attention(
         out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(), _rows(q, n, nq, dim, "q"), nq, _byref(cache),
-        _byref(batch), window, sinks, scale, lp, workspace.data_ptr(), None if err is None else err.data_ptr(), stream)
+        _byref(batch), window, sinks, scale, lp, workspace.data_ptr(), _err_word(err), stream)
     if status:
         check(status, "infernt_paged_attention")
 

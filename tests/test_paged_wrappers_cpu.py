@@ -1,0 +1,39 @@
+"""What the wrappers of the operators over paged caches refuse before a call:
+an error word of another type."""
+import pytest
+
+import infernt_b200 as ib
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture
+def args(monkeypatch):
+    """A small batch, and a library whose calls fail the test."""
+    class Unreached:
+        def __getattr__(self, name):
+            def call(*a):
+                raise AssertionError("%s is reached" % name)
+            return call
+
+    monkeypatch.setattr(ib, "_workspace_bytes", 64)
+    monkeypatch.setattr(ib, "_lib", Unreached())
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    i32 = torch.zeros(3, dtype=torch.int32)
+    table = torch.zeros(2, 4, dtype=torch.int32)
+    return dict(cache=ib.PagedCache(k, k), i32=i32, table=table, batch=ib.RaggedBatch(i32, i32[:2], table, 4, 4),
+                q=torch.zeros(4, 4, 64, dtype=torch.bfloat16), kv=torch.zeros(4, 2, 64, dtype=torch.bfloat16),
+                ws=torch.zeros(64, dtype=torch.uint8))
+
+
+BAD_ERR = [torch.zeros(1, dtype=torch.uint8), torch.zeros(4, dtype=torch.bfloat16), torch.zeros(1),
+           torch.zeros(1, dtype=torch.int64), torch.zeros(0, dtype=torch.int32)]
+
+
+@pytest.mark.parametrize("err", BAD_ERR)
+def test_an_error_word_of_another_type(args, err):
+    with pytest.raises(ValueError):
+        ib.paged_attention(args["q"].clone(), args["q"], args["cache"], args["batch"], args["ws"], err=err)
+    with pytest.raises(ValueError):
+        ib.paged_rope_append(args["q"], args["q"], args["kv"], args["kv"], args["cache"], args["batch"],
+                             ib.RopeParams(rotary_dim=64), err=err)
