@@ -1041,8 +1041,9 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
         shape, lp = lse.shape, lse.data_ptr()
         if len(shape) != 2 or shape[1] != nq or shape[0] < n or _dtype(lse) != DTYPE_F32 or not lse.is_contiguous():
             raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(shape), n, nq))
-    if workspace.nbytes < (_workspace_bytes or paged_attention_workspace_bytes()):
-        raise ValueError("paged_attention: a workspace of %d bytes is needed" % paged_attention_workspace_bytes())
+    if workspace.nbytes < (_workspace_bytes or paged_attention_workspace_bytes()) or not workspace.is_contiguous():
+        raise ValueError("paged_attention: a contiguous workspace of %d bytes is needed" %
+                         paged_attention_workspace_bytes())
     if stream is None:
         stream = _current_stream(q)
     status = (_lib or lib()).infernt_paged_attention(

@@ -1,5 +1,6 @@
 """What the wrappers of the operators over paged caches refuse before a call:
-an error word of another type."""
+an error word or a workspace of the
+wrong kind."""
 import pytest
 
 import infernt_b200 as ib
@@ -37,3 +38,9 @@ def test_an_error_word_of_another_type(args, err):
     with pytest.raises(ValueError):
         ib.paged_rope_append(args["q"], args["q"], args["kv"], args["kv"], args["cache"], args["batch"],
                              ib.RopeParams(rotary_dim=64), err=err)
+
+
+@pytest.mark.parametrize("ws", [torch.zeros(1, dtype=torch.uint8).expand(64), torch.zeros(128, dtype=torch.uint8)[::2]])
+def test_a_workspace_with_gaps(args, ws):
+    with pytest.raises(ValueError):
+        ib.paged_attention(args["q"].clone(), args["q"], args["cache"], args["batch"], ws)
