@@ -1078,6 +1078,8 @@ def copy_pages(pools, src, dst, stream=None):
         count, pages = pools.shape[:2]
         size, start = pools.nbytes // max(1, count), pools.data_ptr()
         base = range(start, start + count * size, size) if size else ()
+    if not pages:
+        raise ValueError("copy_pages: pools of no pages")
     if stream is None:
         stream = _current_stream(pools)
     call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, (_I * n)(*src), (_I * n)(*dst), n,

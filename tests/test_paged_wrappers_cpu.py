@@ -1,6 +1,6 @@
 """What the wrappers of the operators over paged caches refuse before a call:
 an error word or a workspace of the
-wrong kind."""
+wrong kind, pools of no pages."""
 import pytest
 
 import infernt_b200 as ib
@@ -44,3 +44,9 @@ def test_an_error_word_of_another_type(args, err):
 def test_a_workspace_with_gaps(args, ws):
     with pytest.raises(ValueError):
         ib.paged_attention(args["q"].clone(), args["q"], args["cache"], args["batch"], ws)
+
+
+@pytest.mark.parametrize("pools", [torch.zeros(3, 0, 16), [torch.zeros(0, 16)], [torch.zeros(0, 16)] * 2])
+def test_pools_of_no_pages(args, pools):
+    with pytest.raises(ValueError):
+        ib.copy_pages(pools, [], [])
