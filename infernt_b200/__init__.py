@@ -488,9 +488,7 @@ class BatchEngine:
         the next step (infernt_batch_engine_copy_pages)."""
         if len(src) != len(dst):
             raise ValueError("copy_pages: %d sources, %d destinations" % (len(src), len(dst)))
-        n = len(src)
-        call("infernt_batch_engine_copy_pages", self._h, (ctypes.c_int * max(1, n))(*src),
-             (ctypes.c_int * max(1, n))(*dst), n)
+        call("infernt_batch_engine_copy_pages", self._h, _pages(src), _pages(dst), len(src))
 
     def set_salts(self, salts):
         """Per-sequence sampling salts (None: none)."""
@@ -899,6 +897,7 @@ def _dtype(t):
 
 _struct_init = ctypes.Structure.__init__
 _byref = ctypes.byref
+_MOST = 2 ** 31 - 1  # a C int; ctypes takes larger numbers without their high bits
 _raw_stream = None
 
 
@@ -950,6 +949,8 @@ class RaggedBatch(ctypes.Structure):
         if _dtype(kv_len) != -1 or q_start.dtype != t or block_table.dtype != t or not (
                 q_start.is_contiguous() and kv_len.is_contiguous() and block_table.is_contiguous()):
             raise ValueError("RaggedBatch: contiguous int32 tensors are needed")
+        if num_rows > _MOST or max_q_len > _MOST:
+            raise ValueError("RaggedBatch: %d rows, at most %d new tokens" % (num_rows, max_q_len))
         _struct_init(self, q_start.data_ptr(), kv_len.data_ptr(), block_table.data_ptr(), n, num_rows, max_q_len,
                      shape[1])
         self.tensors = q_start, kv_len, block_table
@@ -969,6 +970,8 @@ class RopeParams(ctypes.Structure):
         code = ROPE_SCALINGS.get(scaling)
         if code is None:
             raise ValueError("RopeParams: scaling %r (%s)" % (scaling, ", ".join(ROPE_SCALINGS)))
+        if rotary_dim > _MOST or original_max_len > _MOST:
+            raise ValueError("RopeParams: rotary_dim %d, original_max_len %d" % (rotary_dim, original_max_len))
         _struct_init(self, theta, rotary_dim, bool(interleaved), code, original_max_len, factor, low, high)
 
 
@@ -978,7 +981,7 @@ def _rows(t, rows, heads, dim, what):
     shape, strides = t.shape, t.stride()
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim or shape[0] < rows:
         raise ValueError("%s: shape %s for %d rows of %d heads of %d" % (what, tuple(shape), rows, heads, dim))
-    if strides[2] != 1 or (strides[1] != dim and heads > 1):
+    if strides[2] != 1 or (strides[1] != dim and heads > 1) or (strides[0] > _MOST and shape[0] > 1):
         raise ValueError("%s: strides %s; only rows may be apart" % (what, strides))
     return strides[0] if shape[0] > 1 else heads * dim  # one row has no stride of its own
 
@@ -1044,6 +1047,8 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
     if workspace.nbytes < (_workspace_bytes or paged_attention_workspace_bytes()) or not workspace.is_contiguous():
         raise ValueError("paged_attention: a contiguous workspace of %d bytes is needed" %
                          paged_attention_workspace_bytes())
+    if window > _MOST or sinks > _MOST:
+        raise ValueError("paged_attention: window %d, sinks %d" % (window, sinks))
     if stream is None:
         stream = _current_stream(q)
     status = (_lib or lib()).infernt_paged_attention(
@@ -1051,6 +1056,13 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
         _byref(batch), window, sinks, scale, lp, workspace.data_ptr(), _err_word(err), stream)
     if status:
         check(status, "infernt_paged_attention")
+
+
+def _pages(pages):
+    """A list of page numbers as the C calls take it."""
+    if any(p > _MOST or p < -_MOST for p in pages):
+        raise ValueError("a page number past 2^31")
+    return (_I * max(1, len(pages)))(*pages)
 
 
 def copy_pages(pools, src, dst, stream=None):
@@ -1082,8 +1094,7 @@ def copy_pages(pools, src, dst, stream=None):
         raise ValueError("copy_pages: pools of no pages")
     if stream is None:
         stream = _current_stream(pools)
-    call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, (_I * n)(*src), (_I * n)(*dst), n,
-         stream)
+    call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, _pages(src), _pages(dst), n, stream)
 
 
 class PagePool:

@@ -1,6 +1,6 @@
 """What the wrappers of the operators over paged caches refuse before a call:
-an error word or a workspace of the
-wrong kind, pools of no pages."""
+an error word or a workspace of the wrong kind, pools of no pages, numbers that
+do not fit a C int."""
 import pytest
 
 import infernt_b200 as ib
@@ -50,3 +50,27 @@ def test_a_workspace_with_gaps(args, ws):
 def test_pools_of_no_pages(args, pools):
     with pytest.raises(ValueError):
         ib.copy_pages(pools, [], [])
+
+
+@pytest.mark.parametrize("kw", [dict(window=2 ** 31), dict(window=2 ** 32 + 5), dict(window=9, sinks=2 ** 32)])
+def test_windows_past_an_int(args, kw):
+    with pytest.raises(ValueError):
+        ib.paged_attention(args["q"].clone(), args["q"], args["cache"], args["batch"], args["ws"], **kw)
+
+
+def test_other_numbers_past_an_int(args):
+    for rows, most in ((2 ** 32, 4), (4, 2 ** 32 + 4)):
+        with pytest.raises(ValueError):
+            ib.RaggedBatch(args["i32"], args["i32"][:2], args["table"], rows, most)
+    with pytest.raises(ValueError):
+        ib.RopeParams(rotary_dim=2 ** 32 + 64)
+    with pytest.raises(ValueError):
+        ib.RopeParams(rotary_dim=64, original_max_len=2 ** 32 + 1)
+    for src, dst in (([2 ** 32], [1]), ([0], [2 ** 32 + 1]), ([-2 ** 32], [1])):
+        with pytest.raises(ValueError):
+            ib.copy_pages(torch.zeros(3, 4, 16), src, dst)
+    one = torch.empty(256, dtype=torch.bfloat16).as_strided((1, 4, 64), (2 ** 32 + 256, 64, 1))
+    rows = torch.empty(0, dtype=torch.bfloat16, device="meta").as_strided((4, 4, 64), (2 ** 32 + 256, 64, 1))
+    with pytest.raises(ValueError):
+        ib._rows(rows, 4, 4, 64, "q")
+    assert ib._rows(one, 1, 4, 64, "q") == 256  # one row has no stride of its own
