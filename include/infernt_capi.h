@@ -589,7 +589,10 @@ typedef struct infernt_paged_cache {
  * sequence whose rows or length are out of range (q_start not ascending or
  * above num_rows, more than max_q_len new tokens, kv_len negative, above
  * table_stride x page_size or above 2^30): the sequence is skipped, its rows
- * stay. */
+ * stay.  (Where q_start descends, sequences around that place may hold the
+ * same rows; what these then hold is undefined.  An attention call may skip
+ * all sequences of such a batch when they add up to more work than num_rows
+ * rows can have.) */
 typedef struct infernt_ragged_batch {
     const int* q_start;     /* [num_seqs + 1] */
     const int* kv_len;      /* [num_seqs] */

@@ -168,8 +168,13 @@ __device__ __forceinline__ int find_item(const AttnArgs& a, const PagedSeq& s, i
     }
 }
 
-// Units are counted in 32 bits: the host refuses a call whose bound on them is
-// larger.
+// Units are counted in 32 bits, up to kMostUnits: the host refuses a call whose
+// bound on them is larger.  Sequences that overlap (a q_start that descends
+// somewhere, so that several hold the same rows) can have more; such a batch is
+// not computed.
+constexpr unsigned kMostUnits = 1u << 30;
+__device__ __forceinline__ int add_units(int a, int b) { return (int)min((unsigned)a + (unsigned)b, kMostUnits); }
+
 struct Place {
     int c;       // units of a CTA
     int before;  // units before sequence s
@@ -202,16 +207,21 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
     };
     // the sum of the values before this thread's, and of all of them
     auto scan = [&](int v, int& all) {
-        const int x = warp_scan(v);
+        int x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x = add_units(x, y);
+        }
         __syncthreads();
         if (lane == 31) sums_s[warp] = x;
         __syncthreads();
-        int pre = x - v;
+        int pre = x - v;  // (of no use once a sum is kMostUnits)
         all = 0;
 #pragma unroll
         for (int w = 0; w < NT / 32; ++w) {
-            if (w < warp) pre += sums_s[w];
-            all += sums_s[w];
+            if (w < warp) pre = add_units(pre, sums_s[w]);
+            all = add_units(all, sums_s[w]);
         }
         return pre;
     };
@@ -221,8 +231,12 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a) {
     for (int base = 0; base < n; base += NT) {
         int all;
         p.per_head = units(base + tid, p.seq);
-        before = p.total + scan(p.per_head * a.b.nkv, all);
-        p.total += all;
+        before = add_units(p.total, scan(p.per_head * a.b.nkv, all));
+        p.total = add_units(p.total, all);
+    }
+    if (p.total >= (int)kMostUnits) {
+        if (tid == 0 && blockIdx.x == 0 && a.err) atomicOr(a.err, kErrBatch);
+        p.total = 0;
     }
     p.c = max(a.min_units, (int)(((unsigned)p.total + gridDim.x - 1) / gridDim.x));
     const int at = p.c * (int)blockIdx.x;
