@@ -132,6 +132,13 @@ __device__ __forceinline__ bool place_row(const RopeArgs& a, int r, int& pos, lo
     return true;
 }
 
+// Error bits of the sequences: this block's share of them, since one that no row
+// leads to (no new tokens, or a start above its end) is met nowhere else.
+__device__ __forceinline__ void check_sequences(const RopeArgs& a) {
+    if (a.err && threadIdx.x == kRopeThreads - 1)
+        for (int s = blockIdx.x; s < a.b.num_seqs; s += gridDim.x) paged_seq(a.b, s, a.err);
+}
+
 // Cosine and sine of pair p at position pos, times the magnitude.
 __device__ __forceinline__ float2 turn_of(const RopeDev& rope, int p, int pos) {
     const double t = (double)pos * rope.turns[p];
@@ -213,7 +220,10 @@ __global__ void __launch_bounds__(kRopeThreads)
     }
     int pos;
     long long row;
-    if (!place_row(a, r, pos, row)) return;
+    if (!place_row(a, r, pos, row)) {
+        check_sequences(a);
+        return;
+    }
     if (tid < rope.half) cs_s[tid] = turn_of(rope, tid, pos);
     __syncthreads();
     // of pair e of the first block; interleaved, the first block has four pairs, then the second's
@@ -270,6 +280,7 @@ __global__ void __launch_bounds__(kRopeThreads)
         const bool is_v = h >= heads_q + nkv;
         finish(h, load_eight(p + (is_v ? 8 * w : lo)), load_eight(p + (is_v ? D / 2 + 8 * w : hi)));
     }
+    check_sequences(a);
 }
 
 // Any other rotary_dim, stride or alignment: a block per token row, value by
@@ -280,7 +291,10 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope(const RopeArgs a, con
     const int r = blockIdx.x, tid = threadIdx.x, D = a.D, half = rope.half, nkv = a.b.nkv;
     int pos;
     long long row;
-    if (!place_row(a, r, pos, row)) return;
+    if (!place_row(a, r, pos, row)) {
+        check_sequences(a);
+        return;
+    }
     if (tid < half) cs[tid] = turn_of(rope, tid, pos);
     __syncthreads();
     const int heads = (a.q ? a.nq : 0) + (row >= 0 ? nkv : 0), h0 = a.q ? 0 : a.nq;
@@ -312,6 +326,7 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope(const RopeArgs a, con
             static_cast<T*>(a.vp)[(row + (long long)h * a.b.page_size) * D + e] =
                 Half16<T>::round(source_value(static_cast<const S*>(a.v) + r * a.ldv + u));
         }
+    check_sequences(a);
 }
 
 int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
