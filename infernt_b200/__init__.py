@@ -8,6 +8,7 @@ anything: if the library is missing, ``lib()`` raises.
 
 Configurations follow the reference's ``ModelConfig`` (include/config.h).
 """
+import array
 import ctypes
 import os
 from dataclasses import dataclass, replace
@@ -488,7 +489,8 @@ class BatchEngine:
         the next step (infernt_batch_engine_copy_pages)."""
         if len(src) != len(dst):
             raise ValueError("copy_pages: %d sources, %d destinations" % (len(src), len(dst)))
-        call("infernt_batch_engine_copy_pages", self._h, _pages(src), _pages(dst), len(src))
+        src, dst = _pages(src), _pages(dst)
+        call("infernt_batch_engine_copy_pages", self._h, src.buffer_info()[0], dst.buffer_info()[0], len(src))
 
     def set_salts(self, salts):
         """Per-sequence sampling salts (None: none)."""
@@ -1059,10 +1061,12 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
 
 
 def _pages(pages):
-    """A list of page numbers as the C calls take it."""
-    if any(p > _MOST or p < -_MOST for p in pages):
-        raise ValueError("a page number past 2^31")
-    return (_I * max(1, len(pages)))(*pages)
+    """A list of page numbers as an array of C ints (which looks at each in a
+    tenth of the time of a loop)."""
+    try:
+        return array.array("i", pages)
+    except OverflowError:
+        raise ValueError("a page number past 2^31") from None
 
 
 def copy_pages(pools, src, dst, stream=None):
@@ -1094,7 +1098,9 @@ def copy_pages(pools, src, dst, stream=None):
         raise ValueError("copy_pages: pools of no pages")
     if stream is None:
         stream = _current_stream(pools)
-    call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, _pages(src), _pages(dst), n, stream)
+    src, dst = _pages(src), _pages(dst)
+    call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, src.buffer_info()[0],
+         dst.buffer_info()[0], n, stream)
 
 
 class PagePool:

@@ -9,6 +9,13 @@
 
 namespace infernt {
 
+// Probabilities are rounded to V's type, since a matrix instruction takes both
+// operands in one: half a step each, independent of one another, next to the
+// half step of the result (bf16: 2.0e-3 to 2.3e-3 of the outputs in all, where
+// FP32 probabilities leave 1.7e-3).  A split into three terms, as the decode
+// attention over contiguous caches has it, would be three products P V where
+// chunks are bound by the one.  The denominator sums them in FP32, unrounded.
+//
 // A row's probabilities are 2^(s - m), s in base 2; m is the largest score met
 // less kShift, and moves when a score passes that one by kRescale.  The
 // tcgen05 kernel takes a tile's probabilities under an older m as long as
