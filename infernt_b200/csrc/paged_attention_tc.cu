@@ -37,13 +37,17 @@
 // more than kRescale, or at all after such a sum, so that the next tiles pass.
 // P goes to TMEM eight columns at a time.
 //
-// 4096 tokens at 12288 positions (32/8 heads of 128, bf16): 529 us, 1299
-// TFLOP/s (613 us back to back, at the power limit); 594 with the maximum
-// searched beside the probabilities, 559 with P stored as a whole, 548 with
-// the join of split items in line with the tiles.  The busiest unit is at 77 %,
-// the special function unit at 64 %; a part of the 2^x on the FMA pipe
-// instead of the special function unit changes nothing any more, nor do
-// turns at the exponentials between the warps of a scheduler (622 us).
+// 4096 tokens at 12288 positions (32/8 heads of 128, bf16): 555 us in bursts,
+// 1238 TFLOP/s (636 us back to back, at the power limit).  What was tried stood
+// beside 529 us, in bursts, at its time: 594 with the maximum searched beside
+// the probabilities, 559 with P stored as a whole, 548 with the join of split
+// items in line with the tiles, 622 with turns at the exponentials between the
+// warps of a scheduler; a part of the 2^x on the FMA pipe instead of the special
+// function unit changes nothing.  The call at a part's end that puts values back
+// (restore_values) costs 15 of the 555 us by the registers around it, not by its
+// own time (543 without it, all else the same; 565 in line, 575 with its
+// arguments in registers).  The busiest unit is at 77 %, the special function
+// unit at 64 %.
 #include <cmath>
 #include <cstdint>
 
