@@ -1000,8 +1000,9 @@ def _err_word(err):
 def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
     """Rotary positions of the batch's q rows into q_out, the rotated k rows
     and the v rows into their pages (infernt_paged_rope_append).  q and q_out,
-    or k and v, may be None.  stream: a cudaStream_t as an integer; without it,
-    torch's current stream."""
+    or k and v, may be None.  err: an int32 tensor of one element that gets the
+    error bits.  stream: a cudaStream_t as an integer; without it, torch's
+    current stream."""
     n, dim, src = batch.num_rows, cache.head_dim, None
     qp = op = kp = vp = None
     nq = ldo = ldq = ldk = ldv = 0
@@ -1037,8 +1038,9 @@ def paged_attention_workspace_bytes():
 def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.0, lse=None, err=None, stream=None):
     """Attention of the batch's new tokens over the pages
     (infernt_paged_attention).  workspace: a zeroed tensor of
-    paged_attention_workspace_bytes() bytes.  stream: a cudaStream_t as an
-    integer; without it, torch's current stream."""
+    paged_attention_workspace_bytes() bytes.  err: an int32 tensor of one
+    element that gets the error bits.  stream: a cudaStream_t as an integer;
+    without it, torch's current stream."""
     n, dim, nq, lp = batch.num_rows, cache.head_dim, q.shape[1], None
     if _dtype(q) != cache.dtype or q.dtype != out.dtype:
         raise ValueError("paged_attention: q, out and the cache must have one type")
