@@ -686,6 +686,148 @@ INFERNT_API int infernt_pages_copy(void* const* pools, int n_pools, size_t page_
  * its stream, before its next step. */
 INFERNT_API int infernt_batch_engine_copy_pages(infernt_batch_engine* e, const int* src, const int* dst, int n);
 
+/* Pages that hold K and V in 4 bits: a quarter of the bytes of 16-bit pages
+ * (D + 4 a position and KV head instead of 4 D).  The vector x of a KV head
+ * at a position is held as codes c_i of 4 bits (element 2 i in the low half
+ * of byte i) and a 16-bit scale word:
+ *   s = (max(x, 0) - min(x, 0)) / 15, rounded up to four significant bits,
+ *   z = round(-min(x, 0) / s), c_i = min(max(round(x_i / s) + z, 0), 15),
+ * which stand for the values (c_i - z) s, at most s / 2 from x_i (s where
+ * that rounding would pass the type's largest number).  The values are
+ * numbers of the cache's type as they are, so every operator sees the same
+ * ones.  FP32 arithmetic, correctly rounded, ties to even; s is at least
+ * 2^-100 (bf16) or 2^-21 (fp16).  Word: the upper twelve bits of s as a bf16,
+ * z in the low four.  scales has the K vector's word in the low half of each
+ * element, the V vector's in the high half.  A vector with a value that is
+ * not finite in the cache's type is stored as one of NaN.
+ *
+ * k and v 16-byte aligned; page numbers, block tables and infernt_pages_copy
+ * (for pools whose pages are multiples of 16 bytes) as for 16-bit pools. */
+typedef struct infernt_paged_cache4 {
+    void* k;          /* [num_pages][num_kv_heads][page_size][head_dim / 2] */
+    void* v;
+    unsigned* scales; /* [num_pages][num_kv_heads][page_size] */
+    int num_pages;
+    int num_kv_heads;
+    int page_size; /* positions per page, any number from 1 */
+    int head_dim;  /* 64 or 128 */
+    int dtype;     /* of the values: INFERNT_DTYPE_BF16 or _F16 */
+} infernt_paged_cache4;
+
+/* infernt_paged_rope_append into such pages, its arguments, rows and error
+ * bits.  q_out as there; K is turned in 64 bits and rounded once to FP32
+ * before it is held in 4 bits, so what a page holds does not depend on the
+ * last bits of an FP32 sine. */
+INFERNT_API int infernt_paged4_rope_append(void* q_out, int ldo, const void* q, int ldq, int nq, const void* k,
+                                           int ldk, const void* v, int ldv, int src_dtype,
+                                           const infernt_paged_cache4* cache, const infernt_ragged_batch* batch,
+                                           const infernt_rope_params* rope, unsigned* err, void* stream);
+
+/* infernt_paged_attention over such pages: its formulas, rows, arguments,
+ * workspace (the same bytes; calls that share it must not overlap, of either
+ * kind) and error bits, over the values that the codes stand for.  Any page
+ * size is served alike.  A V vector of NaN makes the results of the rows that
+ * see it NaN. */
+INFERNT_API int infernt_paged4_attention(void* out, int ldo, const void* q, int ldq, int nq,
+                                         const infernt_paged_cache4* cache, const infernt_ragged_batch* batch,
+                                         int window, int sinks, float scale, float* lse, void* workspace,
+                                         unsigned* err, void* stream);
+
+/* The values of page src[i] of 4-bit pools into page dst[i] of 16-bit pools
+ * of the same heads, page size and type, for i in [0, n), K and V (a sequence
+ * handed to an engine with 16-bit pages, for one).  src and dst are device
+ * arrays, read when the kernel runs; a page may go to several others, no two
+ * into the same.  A page number outside its pool sets bit 3 of *err, and
+ * nothing is moved for it.  Asynchronous; may be captured. */
+INFERNT_API int infernt_paged4_unpack(const infernt_paged_cache4* from, const infernt_paged_cache* to, const int* src,
+                                      const int* dst, int n, unsigned* err, void* stream);
+
+/* Pages of sequences whose lengths are known on the device alone (drafted
+ * tokens that were verified there, say): block tables, the pages each
+ * sequence holds, and the free ones.  All arrays are device memory of the
+ * caller's.
+ *   block_table [num_seqs][table_stride]: the pages of sequence s are its
+ *       first held[s] entries.
+ *   free_pages [num_pages]: a ring; state[0] is the place of its first free
+ *       page, state[1] their number, state[2] and [3] are 0 between calls.
+ * An empty pool: held 0, free_pages 0 .. num_pages - 1, state {0, num_pages,
+ * 0, 0}.  A page has one holder here (infernt_page_pool_* has shared ones). */
+typedef struct infernt_page_tables {
+    int* block_table;
+    int* held;
+    int* free_pages;
+    int* state; /* [4] */
+    int num_seqs;     /* 0 to 65535 */
+    int num_pages;    /* num_pages x page_size below 2^31 */
+    int page_size;
+    int table_stride;
+} infernt_page_tables;
+
+/* One step's batch: sequence s keeps its first len[s] positions and gets
+ * new_len[s] more (0: none), and holds pages for just these afterwards.
+ * Missing pages come from the front of the ring, in the order of the
+ * sequences; surplus ones go to its end, in that order, for later calls, and
+ * their table entries become -1.  Writes the ragged batch, q_start [num_seqs
+ * + 1] and kv_len [num_seqs] (kv_len may be len itself), and for each new
+ * token its position and its slot, page x page_size + row (positions and
+ * slots [max_rows] or NULL; elements past the last token stay).
+ * A sequence waits when the pages missing up to it, its own included, are
+ * more than are free, and when new_len up to it add up to more than
+ * max_rows: it gets no rows (kv_len[s] = len[s]) and keeps its pages.  One
+ * that needs no further page never waits for pages.
+ * Bits of *err (device word, or NULL): 4, a sequence with len, new_len or
+ * held out of range (len + new_len above table_stride x page_size or 2^30,
+ * held above table_stride) gets no rows and keeps its pages, or a ring whose
+ * state is out of range, with which nothing is done (q_start all 0); 5, a
+ * sequence waits.  Asynchronous; may be captured; calls on the same tables
+ * must not overlap. */
+INFERNT_API int infernt_paged_batch_plan(const infernt_page_tables* tables, const int* len, const int* new_len,
+                                         int* q_start, int* kv_len, int* positions, int* slots, int max_rows,
+                                         unsigned* err, void* stream);
+
+/* Drafted tokens against the target model's distributions (speculative
+ * sampling; Leviathan et al. 2023).  Rows as in a ragged batch: sequence s has
+ * rows [q_start[s], q_start[s + 1]), a row each for its last known token and
+ * the drafts after it, tokens[r] the token fed in row r; the target's row r
+ * judges tokens[r + 1].  With p the target's distribution of row r, q =
+ * draft_probs row r the one that the draft was drawn from (NULL: drafts
+ * without a distribution, q = 1 at the draft), u in [0, 1):
+ *   the draft d = tokens[r + 1] is accepted while u[r] q(d) < p(d);
+ *   at the first row r* where it is not, the next token is drawn from
+ *   max(p - q, 0) / sum; after the last row without a draft, from p:
+ * the lowest i whose sum of weights up to i is above u[last row of s] x their
+ * sum (p in place of weights that are all 0).
+ * out_tokens of the sequence's rows: the accepted drafts, the drawn token,
+ * then -1; accepted[s]: the drafts accepted; kept[s] = kv_len[s] less the
+ * rejected ones (kv_len and kept both or neither; they may be one array).
+ * A sequence without rows has accepted 0 and no token.
+ *   target [num_rows][vocab_size], rows ld elements apart, of type F32, BF16
+ *   or F16: logits, p = softmax(row / temperature[s]); with probabilities != 0
+ *   they are p, and only what is asked of them is read.  temperature
+ *   [num_seqs] FP32, or NULL for 1; where it is not above 0 the sequence is
+ *   greedy: p is 1 at the row's largest element (the lowest of equal ones)
+ *   and drafts are accepted where they are it.
+ * Logits of -infinity have probability 0.  A row that has to be read and has
+ * a NaN, an infinite or no finite logit (a NaN, negative or infinite
+ * probability, or none above 0) ends its sequence there with its largest
+ * element that is a number (0 if there is none) and bit 6 of *err.
+ * Other bits: 4, rows out of range (the sequence's outputs stay), 2, a drafted
+ * token outside [0, vocab_size) (it is rejected, the token drawn from p).
+ * Sums for acceptance in FP32; the drawn token's weights, sums and borders in
+ * 64 bits, so a token is the formula's own except within about 1e-13 of a
+ * border (an acceptance within about 1e-6 of u q = p).  u below 0 or NaN is
+ * taken as 0, from 1 on as the largest below 1; elements of draft_probs that
+ * are not finite give weight 0.  workspace: infernt_verify_drafts_workspace_bytes(num_rows,
+ * num_seqs) bytes, 16-byte aligned, of any content (calls that share it must
+ * not overlap, two captured graphs among them).  Asynchronous; may be
+ * captured. */
+INFERNT_API size_t infernt_verify_drafts_workspace_bytes(int num_rows, int num_seqs);
+INFERNT_API int infernt_verify_drafts(int* out_tokens, int* accepted, const void* target, long long ld,
+                                      int target_dtype, int probabilities, const float* draft_probs,
+                                      long long draft_ld, const int* tokens, const int* q_start, int num_seqs,
+                                      int num_rows, int vocab_size, const float* temperature, const float* u,
+                                      const int* kv_len, int* kept, void* workspace, unsigned* err, void* stream);
+
 /* Which sequence holds which pages (host logic, no GPU): pages are counted
  * by the sequences that hold them, so a fork shares them and a write to a
  * shared page copies it first.  Calls that hand out pages fail as a whole

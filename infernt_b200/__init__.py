@@ -244,6 +244,13 @@ _SIGS = {
     "infernt_paged_attention_workspace_bytes": (_S, []),
     "infernt_paged_attention": (_I, [_P, _I, _P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _P, _P]),
     "infernt_pages_copy": (_I, [_P, _I, _S, _I, _P, _P, _I, _P]),
+    "infernt_paged4_rope_append": (_I, [_P, _I, _P, _I, _I, _P, _I, _P, _I, _I, _P, _P, _P, _P, _P]),
+    "infernt_paged4_attention": (_I, [_P, _I, _P, _I, _I, _P, _P, _I, _I, _F, _P, _P, _P, _P]),
+    "infernt_paged4_unpack": (_I, [_P, _P, _P, _P, _I, _P, _P]),
+    "infernt_paged_batch_plan": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P]),
+    "infernt_verify_drafts_workspace_bytes": (_S, [_I, _I]),
+    "infernt_verify_drafts": (_I, [_P, _P, _P, ctypes.c_longlong, _I, _I, _P, ctypes.c_longlong, _P, _P, _I, _I, _I, _P,
+                                   _P, _P, _P, _P, _P, _P]),
     "infernt_batch_engine_copy_pages": (_I, [_P, _P, _P, _I]),
     "infernt_page_pool_create": (_I, [_I, _I, _I, _P]),
     "infernt_page_pool_destroy": (_I, [_P]),
@@ -1003,6 +1010,11 @@ def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None)
     or k and v, may be None.  err: an int32 tensor of one element that gets the
     error bits.  stream: a cudaStream_t as an integer; without it, torch's
     current stream."""
+    _rope_append((_lib or lib()).infernt_paged_rope_append, "paged_rope_append", q_out, q, k, v, cache, batch, rope, err,
+                 stream)
+
+
+def _rope_append(call_, what, q_out, q, k, v, cache, batch, rope, err, stream):
     n, dim, src = batch.num_rows, cache.head_dim, None
     qp = op = kp = vp = None
     nq = ldo = ldq = ldk = ldv = 0
@@ -1010,19 +1022,19 @@ def paged_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None)
         nq, src, qp, op = q.shape[1], q.dtype, q.data_ptr(), q_out.data_ptr()
         ldq, ldo = _rows(q, n, nq, dim, "q"), _rows(q_out, n, nq, dim, "q_out")
         if _dtype(q_out) != cache.dtype:
-            raise ValueError("paged_rope_append: q_out has another type than the cache")
+            raise ValueError("%s: q_out has another type than the cache" % what)
     if k is not None:
         nkv, kp, vp, t = cache.num_kv_heads, k.data_ptr(), v.data_ptr(), k.dtype
         ldk, ldv = _rows(k, n, nkv, dim, "k"), _rows(v, n, nkv, dim, "v")
         if v.dtype != t or (src is not None and src != t):
-            raise ValueError("paged_rope_append: q, k and v of different types")
+            raise ValueError("%s: q, k and v of different types" % what)
     if stream is None:
         stream = _current_stream(q if k is None else k)
-    status = (_lib or lib()).infernt_paged_rope_append(
+    status = call_(
         op, ldo, qp, ldq, nq, kp, ldk, vp, ldv, _dtype(q if k is None else k), _byref(cache), _byref(batch),
         _byref(rope), _err_word(err), stream)
     if status:
-        check(status, "infernt_paged_rope_append")
+        check(status, "infernt_" + what)
 
 
 _workspace_bytes = 0
@@ -1041,25 +1053,30 @@ def paged_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.
     paged_attention_workspace_bytes() bytes.  err: an int32 tensor of one
     element that gets the error bits.  stream: a cudaStream_t as an integer;
     without it, torch's current stream."""
+    _attention((_lib or lib()).infernt_paged_attention, "paged_attention", out, q, cache, batch, workspace, window, sinks,
+               scale, lse, err, stream)
+
+
+def _attention(call_, what, out, q, cache, batch, workspace, window, sinks, scale, lse, err, stream):
     n, dim, nq, lp = batch.num_rows, cache.head_dim, q.shape[1], None
     if _dtype(q) != cache.dtype or q.dtype != out.dtype:
-        raise ValueError("paged_attention: q, out and the cache must have one type")
+        raise ValueError("%s: q, out and the cache must have one type" % what)
     if lse is not None:
         shape, lp = lse.shape, lse.data_ptr()
         if len(shape) != 2 or shape[1] != nq or shape[0] < n or _dtype(lse) != DTYPE_F32 or not lse.is_contiguous():
-            raise ValueError("paged_attention: lse %s for %d rows of %d heads" % (tuple(shape), n, nq))
+            raise ValueError("%s: lse %s for %d rows of %d heads" % (what, tuple(shape), n, nq))
     if workspace.nbytes < (_workspace_bytes or paged_attention_workspace_bytes()) or not workspace.is_contiguous():
-        raise ValueError("paged_attention: a contiguous workspace of %d bytes is needed" %
-                         paged_attention_workspace_bytes())
+        raise ValueError("%s: a contiguous workspace of %d bytes is needed" %
+                         (what, paged_attention_workspace_bytes()))
     if window > _MOST or sinks > _MOST:
-        raise ValueError("paged_attention: window %d, sinks %d" % (window, sinks))
+        raise ValueError("%s: window %d, sinks %d" % (what, window, sinks))
     if stream is None:
         stream = _current_stream(q)
-    status = (_lib or lib()).infernt_paged_attention(
+    status = call_(
         out.data_ptr(), _rows(out, n, nq, dim, "out"), q.data_ptr(), _rows(q, n, nq, dim, "q"), nq, _byref(cache),
         _byref(batch), window, sinks, scale, lp, workspace.data_ptr(), _err_word(err), stream)
     if status:
-        check(status, "infernt_paged_attention")
+        check(status, "infernt_" + what)
 
 
 def _pages(pages):
@@ -1103,6 +1120,171 @@ def copy_pages(pools, src, dst, stream=None):
     src, dst = _pages(src), _pages(dst)
     call("infernt_pages_copy", (_P * count)(*base), count, size // pages, pages, src.buffer_info()[0],
          dst.buffer_info()[0], n, stream)
+
+
+# ------------------------------------------ pages of 4 bits, drafted tokens
+def _torch_dtype(d):
+    """DTYPE_BF16 or DTYPE_F16 of a torch type."""
+    code = {"torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}.get(str(d))
+    if code is None:
+        raise ValueError("type %s (bfloat16 or float16)" % d)
+    return code
+
+
+class PagedCache4(ctypes.Structure):
+    """``infernt_paged_cache4``: the pools of one layer in 4 bits.  k and v are
+    contiguous uint8 tensors [num_pages][num_kv_heads][page_size][head_dim / 2],
+    scales a contiguous int32 tensor [num_pages][num_kv_heads][page_size];
+    dtype (torch.bfloat16 or torch.float16) is the type of the values that they
+    stand for."""
+    _fields_ = [("k", _P), ("v", _P), ("scales", _P), ("num_pages", _I), ("num_kv_heads", _I), ("page_size", _I),
+                ("head_dim", _I), ("dtype", _I)]
+
+    def __init__(self, k, v, scales, dtype):
+        shape, device = k.shape, k.get_device()
+        if len(shape) != 4 or v.shape != shape or scales.shape != shape[:3] or v.get_device() != device or (
+                scales.get_device() != device):
+            raise ValueError("PagedCache4: k %s, v %s, scales %s" % (tuple(shape), tuple(v.shape), tuple(scales.shape)))
+        if str(k.dtype) != "torch.uint8" or v.dtype != k.dtype or str(scales.dtype) != "torch.int32" or not (
+                k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("PagedCache4: contiguous uint8 codes and int32 scales are needed")
+        pages, heads, page, half = shape
+        _struct_init(self, k.data_ptr(), v.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half,
+                     _torch_dtype(dtype))
+        self.tensors = k, v, scales
+
+
+def paged4_rope_append(q_out, q, k, v, cache, batch, rope, err=None, stream=None):
+    """paged_rope_append into a PagedCache4 (infernt_paged4_rope_append)."""
+    _rope_append((_lib or lib()).infernt_paged4_rope_append, "paged4_rope_append", q_out, q, k, v, cache, batch, rope, err,
+                 stream)
+
+
+def paged4_attention(out, q, cache, batch, workspace, window=0, sinks=0, scale=0.0, lse=None, err=None, stream=None):
+    """paged_attention over a PagedCache4 (infernt_paged4_attention), with the
+    same workspace."""
+    _attention((_lib or lib()).infernt_paged4_attention, "paged4_attention", out, q, cache, batch, workspace, window, sinks,
+               scale, lse, err, stream)
+
+
+def _int_array(t, n, what):
+    """Address of a contiguous int32 tensor of at least n elements (None: none)."""
+    if t is None:
+        return None
+    if _dtype(t) != -1 or t.numel() < n or not t.is_contiguous():
+        raise ValueError("%s: a contiguous int32 tensor of %d elements is needed" % (what, n))
+    return t.data_ptr()
+
+
+def paged4_unpack(cache, to, src, dst, err=None, stream=None):
+    """The values of page src[i] of a PagedCache4 into page dst[i] of a
+    PagedCache of the same heads, page size and type (infernt_paged4_unpack).
+    src and dst: int32 device tensors, read when the kernel runs."""
+    n = src.numel()
+    if dst.numel() != n:
+        raise ValueError("paged4_unpack: %d sources, %d destinations" % (n, dst.numel()))
+    if stream is None:
+        stream = _current_stream(to.tensors[0])
+    status = (_lib or lib()).infernt_paged4_unpack(_byref(cache), _byref(to), _int_array(src, n, "src"),
+                                                   _int_array(dst, n, "dst"), n, _err_word(err), stream)
+    if status:
+        check(status, "infernt_paged4_unpack")
+
+
+class PageTables(ctypes.Structure):
+    """``infernt_page_tables``: which pages sequences hold, on the device.
+    Contiguous int32 tensors: block_table [num_seqs][table entries], held
+    [num_seqs], free_pages [num_pages] (a ring), state [4].  An empty pool:
+    PageTables.empty."""
+    _fields_ = [("block_table", _P), ("held", _P), ("free_pages", _P), ("state", _P), ("num_seqs", _I),
+                ("num_pages", _I), ("page_size", _I), ("table_stride", _I)]
+
+    def __init__(self, block_table, held, free_pages, state, page_size):
+        shape = block_table.shape
+        if len(shape) != 2 or held.numel() != shape[0] or state.numel() != 4:
+            raise ValueError("PageTables: table %s, held %s, state %s" % (tuple(shape), tuple(held.shape),
+                                                                          tuple(state.shape)))
+        if page_size > _MOST:
+            raise ValueError("PageTables: pages of %d positions" % page_size)
+        _struct_init(self, _int_array(block_table, 0, "block_table"), _int_array(held, 0, "held"),
+                     _int_array(free_pages, 0, "free_pages"), _int_array(state, 4, "state"), shape[0],
+                     free_pages.numel(), page_size, shape[1])
+        self.tensors = block_table, held, free_pages, state
+
+    @classmethod
+    def empty(cls, num_seqs, num_pages, page_size, max_pages, device="cuda"):
+        """No sequence holds a page; all num_pages are free."""
+        import torch
+        i32 = dict(dtype=torch.int32, device=device)
+        return cls(torch.full((num_seqs, max_pages), -1, **i32), torch.zeros(num_seqs, **i32),
+                   torch.arange(num_pages, **i32), torch.tensor([0, num_pages, 0, 0], **i32), page_size)
+
+
+def plan_batch(tables, lens, new_lens, q_start, kv_len, positions=None, slots=None, err=None, stream=None):
+    """Pages, starts and lengths of a step's batch from what each sequence keeps
+    and wants, all int32 device tensors (infernt_paged_batch_plan).  kv_len may
+    be lens itself.  positions, slots: the new tokens' positions and places in
+    the pool; their length bounds the batch's rows."""
+    n = tables.num_seqs
+    rows = (1 << 30) - 1
+    for t in (positions, slots):
+        if t is not None:
+            rows = min(rows, t.numel())
+    if stream is None:
+        stream = _current_stream(q_start)
+    status = (_lib or lib()).infernt_paged_batch_plan(
+        _byref(tables), _int_array(lens, n, "lens"), _int_array(new_lens, n, "new_lens"),
+        _int_array(q_start, n + 1, "q_start"), _int_array(kv_len, n, "kv_len"), _int_array(positions, 0, "positions"),
+        _int_array(slots, 0, "slots"), rows, _err_word(err), stream)
+    if status:
+        check(status, "infernt_paged_batch_plan")
+
+
+def verify_drafts_workspace_bytes(num_rows, num_seqs):
+    return lib().infernt_verify_drafts_workspace_bytes(num_rows, num_seqs)
+
+
+def _float_array(t, n, what):
+    """Address of a contiguous float32 tensor of at least n elements (None: none)."""
+    if t is None:
+        return None
+    if _dtype(t) != DTYPE_F32 or t.numel() < n or not t.is_contiguous():
+        raise ValueError("%s: a contiguous float32 tensor of %d elements is needed" % (what, n))
+    return t.data_ptr()
+
+
+def verify_drafts(out_tokens, accepted, target, tokens, q_start, u, workspace, draft_probs=None, temperature=None,
+                  probabilities=False, kv_len=None, kept=None, err=None, stream=None):
+    """Drafted tokens against the target's rows [num_rows][vocab] (logits, or
+    probabilities), and the token after the accepted ones
+    (infernt_verify_drafts).  tokens [num_rows]: what was fed; q_start
+    [num_seqs + 1]; u [num_rows] in [0, 1); out_tokens [num_rows], accepted
+    [num_seqs].  draft_probs: float32 rows like the target's.  kv_len and kept:
+    lengths with all drafts in, and without the rejected ones.  workspace: a
+    tensor of verify_drafts_workspace_bytes(num_rows, num_seqs) bytes."""
+    shape, n = target.shape, accepted.numel()
+    if len(shape) != 2 or (target.stride(1) != 1 and shape[1] > 1):
+        raise ValueError("verify_drafts: target %s with strides %s" % (tuple(shape), target.stride()))
+    rows, vocab = shape
+    dp, ldd = None, vocab
+    if draft_probs is not None:
+        if draft_probs.dim() != 2 or draft_probs.shape[1] != vocab or draft_probs.shape[0] < rows or (
+                _dtype(draft_probs) != DTYPE_F32 or (draft_probs.stride(1) != 1 and vocab > 1)):
+            raise ValueError("verify_drafts: draft_probs %s for %d rows of %d" % (tuple(draft_probs.shape), rows, vocab))
+        dp, ldd = draft_probs.data_ptr(), draft_probs.stride(0) if draft_probs.shape[0] > 1 else vocab
+    if workspace.nbytes < verify_drafts_workspace_bytes(rows, n) or not workspace.is_contiguous():
+        raise ValueError("verify_drafts: a contiguous workspace of %d bytes is needed" %
+                         verify_drafts_workspace_bytes(rows, n))
+    if stream is None:
+        stream = _current_stream(target)
+    status = (_lib or lib()).infernt_verify_drafts(
+        _int_array(out_tokens, rows, "out_tokens"), _int_array(accepted, n, "accepted"), target.data_ptr(),
+        target.stride(0) if rows > 1 else vocab, _dtype(target), bool(probabilities), dp, ldd,
+        _int_array(tokens, rows, "tokens"), _int_array(q_start, n + 1, "q_start"), n, rows, vocab,
+        _float_array(temperature, n, "temperature"), _float_array(u, rows, "u"), _int_array(kv_len, n, "kv_len"),
+        _int_array(kept, n, "kept"), workspace.data_ptr(), _err_word(err), stream)
+    if status:
+        check(status, "infernt_verify_drafts")
 
 
 class PagePool:

@@ -22,6 +22,8 @@ enum : unsigned {
     kErrToken = 1u << 2,         // token id outside [0, vocab_size)
     kErrPage = 1u << 3,          // page id outside the pool
     kErrBatch = 1u << 4,         // a ragged batch's rows or lengths out of range
+    kErrNoRoom = 1u << 5,        // a sequence waits for pages or rows
+    kErrValue = 1u << 6,         // a distribution that is none
 };
 
 // Iteration limit of every spin-wait (try_wait already suspends for a
@@ -95,6 +97,14 @@ __device__ __forceinline__ void bulk_g2s_plain(void* dst, const void* src, uint3
     asm volatile(
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
             smem_addr(dst)),
+        "l"(src), "r"(bytes), "r"(smem_addr(bar))
+        : "memory");
+}
+
+// The same to a shared-memory address.
+__device__ __forceinline__ void bulk_g2s_plain_at(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
         "l"(src), "r"(bytes), "r"(smem_addr(bar))
         : "memory");
 }

@@ -1,5 +1,5 @@
 // paged.cuh — what the operators over paged caches share (paged_rope.cu,
-// paged_attention.cu): the ragged batch on the device, the way from a token
+// paged_attention.cu, paged4.cu, page_tables.cu, verify.cu): the ragged batch on the device, the way from a token
 // row to its sequence, the argument checks, and the two 16-bit types.
 #pragma once
 
@@ -64,6 +64,23 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s, unsign
         r.row0 = r.n_new = r.len = 0;
     }
     return r;
+}
+
+// The sequence that holds row r (the last s with q_start[s] <= r), by a
+// search of 32 places a round: one round trip for up to 32 sequences, two
+// for up to 1024.  Whatever the array holds, the result is in [0, n).
+__device__ __forceinline__ int find_seq(const int* q_start, int n, int r) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = n;  // the answer is in [lo, hi)
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int at = lo + lane * step;
+        const unsigned le = __ballot_sync(0xffffffffu, at < hi && q_start[at] <= r);
+        const int k = le ? 31 - __clz(le) : 0;
+        lo = lo + k * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
 }
 
 // bf16 and fp16 as the tensor cores and the stores take them.

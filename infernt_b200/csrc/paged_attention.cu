@@ -346,20 +346,6 @@ __device__ __forceinline__ RowState<D> consume(const AttnArgs& a, const PagedSeq
     return s;
 }
 
-// Columns d and d + 1 of a row's result.
-template <typename T, int D>
-__device__ __forceinline__ void write_pair(const AttnArgs& a, const PagedSeq& seq, int kvh, int row, int d, Joined v) {
-    const int token = a.by_g(row), head = kvh * a.G + row - token * a.G;
-    const bool sees = row_pos(seq, token) >= 0;
-    const float inv = 1.0f / v.l;
-    const float x = sees ? v.x * inv : 0.0f, y = sees ? v.y * inv : 0.0f;
-    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + token) * a.ldo +
-                                 (long long)head * D + d) = Half16<T>::pack(x, y);
-    if (a.lse && d == 0)
-        a.lse[(long long)(seq.row0 + token) * a.nq + head] =
-            sees ? (v.m + log2f(v.l)) * kLn2 : -INFINITY;
-}
-
 // The values that clean_rows took out of a part's tiles, added to the results
 // of the rows r0 + g and r0 + g + 8 that see them: to this lane's columns, as it
 // has just written them to the slot, or to out.  (On memory, and with the part
@@ -387,41 +373,6 @@ __device__ __noinline__ void restore_rows(const AttnArgs& a, const Current& cur,
             }
         }
     });
-}
-
-// Columns d and d + 1 of row r of a split item, joined over its CTAs in order;
-// four of them are read at once.
-template <int M, int D>
-__device__ __forceinline__ Joined join_slots(const AttnArgs& a, int first, int last, int r, int d) {
-    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
-    for (int b = first; b <= last; b += 4) {
-        float m[4], l[4];
-        float2 o[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float* p = slot_of<M, D>(a, min(b + i, last), first);
-            m[i] = __ldcg(p + M * D + r);
-            l[i] = __ldcg(p + M * D + M + r);
-            o[i] = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
-        }
-        float top = v.m;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (b + i > last) m[i] = -INFINITY;
-            top = fmaxf(top, m[i]);
-        }
-        const float f = v.m == -INFINITY ? 0.0f : ex2(v.m - top);
-        v = {top, v.l * f, v.x * f, v.y * f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float w = m[i] == -INFINITY ? 0.0f : ex2(m[i] - top);
-            if (b + i > last) continue;
-            v.l = fmaf(l[i], w, v.l);
-            v.x = fmaf(o[i].x, w, v.x);
-            v.y = fmaf(o[i].y, w, v.y);
-        }
-    }
-    return v;
 }
 
 template <typename T, int D, bool BOXES>
@@ -571,12 +522,11 @@ int launch(const AttnArgs& a, cudaStream_t st) {
 
 extern "C" size_t infernt_paged_attention_workspace_bytes(void) { return infernt::kWorkspaceBytes; }
 
-extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ldq, int nq,
-                                       const infernt_paged_cache* cache, const infernt_ragged_batch* batch, int window,
-                                       int sinks, float scale, float* lse, void* workspace, unsigned* err,
-                                       void* stream) {
-    using namespace infernt;
-    const char* op = "paged_attention";
+namespace infernt {
+
+int attention_args(const char* op, void* out, int ldo, const void* q, int ldq, int nq, const infernt_paged_cache* cache,
+                   const infernt_ragged_batch* batch, int window, int sinks, float scale, float* lse, void* workspace,
+                   unsigned* err, int item_rows, int tile_keys, AttnArgs* args, bool* empty) {
     if (int s = check_paged_cache(op, cache)) return s;
     if (int s = check_ragged_batch(op, batch)) return s;
     INFERNT_REQUIRE(q && out && workspace, "%s: null pointer", op);
@@ -596,19 +546,18 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     INFERNT_REQUIRE((long long)batch->num_rows * G < kMaxPositions, "%s: %d rows of %d heads", op, batch->num_rows, nq);
     // the units of the schedule are counted in 32 bits
     const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
-    const bool chunks = paged_attention_boxes(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
-    const long long tile_m = chunks ? kTcItemRows : kItemRows, tile_n = chunks ? kTcTileKeys : kTileKeys;
-    const long long items = ((long long)batch->num_rows * G / tile_m + batch->num_seqs) * nkv;
-    INFERNT_REQUIRE(items < (1ll << 30) / (most_kv / tile_n + 2 + kItemCost),
+    const long long items = ((long long)batch->num_rows * G / item_rows + batch->num_seqs) * nkv;
+    INFERNT_REQUIRE(items < (1ll << 30) / (most_kv / tile_keys + 2 + kItemCost),
                     "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
                     most_kv);
-    if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
+    *empty = batch->num_seqs == 0 || batch->num_rows == 0;
+    if (*empty) return INFERNT_OK;
     if (int s = check_batch_pointers(op, cache, batch, err)) return s;
     if (int s = check_device_pointer(op, "q", q)) return s;
     if (int s = check_device_pointer(op, "out", out)) return s;
     if (int s = check_device_pointer(op, "lse", lse)) return s;
     if (int s = check_device_pointer(op, "workspace", workspace)) return s;
-    AttnArgs a;
+    AttnArgs& a = *args;
     a.b = paged_batch(*cache, *batch);
     a.q = q;
     a.out = out;
@@ -630,6 +579,28 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     a.tickets = static_cast<unsigned*>(workspace);
     a.slots = reinterpret_cast<float*>(static_cast<char*>(workspace) + kSlotsAt);
     a.err = err;
+    a.scales = nullptr;
+    return INFERNT_OK;
+}
+
+}  // namespace infernt
+
+extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ldq, int nq,
+                                       const infernt_paged_cache* cache, const infernt_ragged_batch* batch, int window,
+                                       int sinks, float scale, float* lse, void* workspace, unsigned* err,
+                                       void* stream) {
+    using namespace infernt;
+    const char* op = "paged_attention";
+    if (int s = check_paged_cache(op, cache)) return s;
+    if (int s = check_ragged_batch(op, batch)) return s;
+    const int D = cache->head_dim, nkv = cache->num_kv_heads, G = nq / nkv;
+    const bool chunks = paged_attention_boxes(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
+    AttnArgs a;
+    bool empty;
+    if (int s = attention_args(op, out, ldo, q, ldq, nq, cache, batch, window, sinks, scale, lse, workspace, err,
+                               chunks ? kTcItemRows : kItemRows, chunks ? kTcTileKeys : kTileKeys, &a, &empty))
+        return s;
+    if (empty) return INFERNT_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // Sequences of up to kItemRows query rows are bound by the bytes of their
     // keys, which the mma.sync kernel streams faster; longer ones by their

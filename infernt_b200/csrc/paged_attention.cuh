@@ -58,6 +58,7 @@ struct AttnArgs {
     unsigned* tickets;       // [CTAs], zero between calls
     float* slots;
     unsigned* err;
+    const unsigned* scales;  // of pages of 4 bits (paged4.cuh), whose codes k and v then are
 };
 
 // Whether tiles of 64 keys of such pages can be loaded as boxes of a tensor
@@ -71,6 +72,16 @@ int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D,
 constexpr int kTcItemRows = 256;
 constexpr int kTcTileKeys = 64;
 int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st);
+// The same over pages of 4 bits; the other kernel is paged4_attn.
+int paged4_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st);
+
+// Checks of an attention call's arguments and its AttnArgs but for `scales`
+// (paged_attention.cu).  Items of at least item_rows query rows (but for a
+// sequence's last) and tiles of at least tile_keys keys bound its work;
+// *empty: nothing to do.
+int attention_args(const char* op, void* out, int ldo, const void* q, int ldq, int nq, const infernt_paged_cache* cache,
+                   const infernt_ragged_batch* batch, int window, int sinks, float scale, float* lse, void* workspace,
+                   unsigned* err, int item_rows, int tile_keys, AttnArgs* args, bool* empty);
 
 // Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
 // keys that they see: [0, sink_end) and [lo, hi), as tiles of N keys.
@@ -535,5 +546,54 @@ __device__ __forceinline__ float* slot_of(const AttnArgs& a, int b, int first) {
 }
 
 constexpr float kLn2 = 0.6931471805599453f;
+
+// Columns d and d + 1 of row r of a split item, joined over its CTAs in order;
+// four of them are read at once.
+template <int M, int D>
+__device__ __forceinline__ Joined join_slots(const AttnArgs& a, int first, int last, int r, int d) {
+    Joined v = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    for (int b = first; b <= last; b += 4) {
+        float m[4], l[4];
+        float2 o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* p = slot_of<M, D>(a, min(b + i, last), first);
+            m[i] = __ldcg(p + M * D + r);
+            l[i] = __ldcg(p + M * D + M + r);
+            o[i] = __ldcg(reinterpret_cast<const float2*>(p + r * D + d));
+        }
+        float top = v.m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b + i > last) m[i] = -INFINITY;
+            top = fmaxf(top, m[i]);
+        }
+        const float f = v.m == -INFINITY ? 0.0f : ex2(v.m - top);
+        v = {top, v.l * f, v.x * f, v.y * f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = m[i] == -INFINITY ? 0.0f : ex2(m[i] - top);
+            if (b + i > last) continue;
+            v.l = fmaf(l[i], w, v.l);
+            v.x = fmaf(o[i].x, w, v.x);
+            v.y = fmaf(o[i].y, w, v.y);
+        }
+    }
+    return v;
+}
+
+// Columns d and d + 1 of a row's result.
+template <typename T, int D>
+__device__ __forceinline__ void write_pair(const AttnArgs& a, const PagedSeq& seq, int kvh, int row, int d, Joined v) {
+    const int token = a.by_g(row), head = kvh * a.G + row - token * a.G;
+    const bool sees = row_pos(seq, token) >= 0;
+    const float inv = 1.0f / v.l;
+    const float x = sees ? v.x * inv : 0.0f, y = sees ? v.y * inv : 0.0f;
+    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + (long long)(seq.row0 + token) * a.ldo +
+                                 (long long)head * D + d) = Half16<T>::pack(x, y);
+    if (a.lse && d == 0)
+        a.lse[(long long)(seq.row0 + token) * a.nq + head] =
+            sees ? (v.m + log2f(v.l)) * kLn2 : -INFINITY;
+}
 
 }  // namespace infernt

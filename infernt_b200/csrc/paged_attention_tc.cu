@@ -53,6 +53,7 @@
 
 #include <cudaTypedefs.h>
 
+#include "paged4.cuh"
 #include "paged_attention.cuh"
 #include "tc_mma.cuh"
 
@@ -155,6 +156,141 @@ __device__ __noinline__ void restore_values(const AttnArgs& a, const Current& cu
     });
 }
 
+// ------------------------------------------------- pages of 4 bits
+// The tiles are the same, in 16 bits, but for how they get there: warp 0 makes
+// the K tiles and warp 2 the V tiles out of codes (paged4.cuh), in registers.
+// A warp has the codes of the next tile in flight while it waits for the stage
+// of that tile.  The values are numbers of T, so
+// the products are those over 16-bit pages.  A tile is some 600 issue slots of
+// a warp, on schedulers where the row warps leave half of them.
+
+// A lane's part of a tile: 16-byte pieces of codes, of rows i kRpi + lane / kPieces.
+template <int D>
+struct Tile4 {
+    static constexpr int kPieces = D / 32, kRpi = 32 / kPieces, kRounds = kN / kRpi;
+    int rows[2];       // pool rows of keys lane, lane + 32 (-1: zeros)
+    uint32_t word[2];  // their scale words (16 bits; 0: zeros)
+    uint4 codes[kRounds];
+};
+
+template <int D>
+__device__ __forceinline__ void look4(const AttnArgs& a, const Item& it, const Part& part, int j, Tile4<D>& t) {
+    const int lane = threadIdx.x & 31, k0 = tile_key<kN>(it, j);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int p = k0 + lane + 32 * h;
+        t.rows[h] = item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
+    }
+}
+template <int D, bool IS_V>
+__device__ __forceinline__ void fetch4(const AttnArgs& a, Tile4<D>& t) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        t.word[h] = t.rows[h] >= 0 ? (__ldg(a.scales + t.rows[h]) >> (IS_V ? 16 : 0)) & 0xffffu : 0u;
+    const uint4* codes = static_cast<const uint4*>(IS_V ? a.v : a.k);
+#pragma unroll
+    for (int i = 0; i < Tile4<D>::kRounds; ++i) {
+        const int r = i * Tile4<D>::kRpi + lane / Tile4<D>::kPieces;
+        const int row = __shfl_sync(0xffffffffu, t.rows[r >> 5], r & 31);
+        t.codes[i] = row >= 0 ? __ldg(codes + (size_t)row * Tile4<D>::kPieces + lane % Tile4<D>::kPieces)
+                              : make_uint4(0u, 0u, 0u, 0u);
+    }
+}
+template <typename T, int D>
+__device__ __forceinline__ void put4(const Tile4<D>& t, uint32_t tile) {
+    const int lane = threadIdx.x & 31, c = 4 * (lane % Tile4<D>::kPieces);
+#pragma unroll
+    for (int i = 0; i < Tile4<D>::kRounds; ++i) {
+        const int r = i * Tile4<D>::kRpi + lane / Tile4<D>::kPieces;
+        const uint32_t word = __shfl_sync(0xffffffffu, t.word[i * Tile4<D>::kRpi / 32], r & 31);
+        const uint32_t z2 = Codes4<T>::zeros(word & 15u), s2 = scale_pair4<T>(word);
+        st_shared(chunk_at(tile, r, c), values4<T>(t.codes[i].x, z2, s2));
+        st_shared(chunk_at(tile, r, c + 1), values4<T>(t.codes[i].y, z2, s2));
+        st_shared(chunk_at(tile, r, c + 2), values4<T>(t.codes[i].z, z2, s2));
+        st_shared(chunk_at(tile, r, c + 3), values4<T>(t.codes[i].w, z2, s2));
+    }
+    fence_proxy_async_smem();  // before the products read the tile
+    __syncwarp();
+}
+
+// All tiles of a CTA's parts, K by warp 0 or V by warp 2.  V vectors of NaN in
+// tiles that rows see in part become zeros, and *found_in the part.
+template <typename T, int D, bool IS_V>
+__device__ __forceinline__ void produce4(const AttnArgs& a, const Place& place, uint32_t base, Barriers& bar, Current& cur,
+                                         volatile int* found_in, bool& ok) {
+    using L = LayoutTc<D>;
+    constexpr int ST = L::kStages;
+    const int lane = threadIdx.x & 31;
+    uint32_t n = 0;  // tiles so far, over all parts
+    walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
+        if (IS_V) set_current(cur, it, part);
+        const bool mixed = it.pos_first != it.pos_last;
+        Tile4<D> t;
+        if (part.j0 < part.j1) {
+            look4<D>(a, it, part, part.j0, t);
+            fetch4<D, IS_V>(a, t);
+        }
+#pragma unroll 1
+        for (int j = part.j0; j < part.j1; ++j, ++n) {
+            const uint32_t st = n % ST, turn = (n / ST) & 1u;
+            if (IS_V && mixed && !seen_whole<kN>(a, it, tile_key<kN>(it, j))) {
+                bool none = false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if ((t.word[h] & 0x7f80u) == 0x7f80u) {
+                        t.word[h] = 0u;
+                        none = true;
+                    }
+                if (__any_sync(0xffffffffu, none)) {
+                    if (lane == 0) *found_in = cur.no;
+                    __threadfence_block();
+                }
+            }
+            if (n >= ST) tc_wait_bar(IS_V ? &bar.empty_v[st] : &bar.empty_k[st], turn ^ 1u, ok);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) return;
+            put4<T, D>(t, base + (IS_V ? L::kV : L::kK) + st * L::kTile);
+            if (lane == 0) {
+                mbar_arrive(IS_V ? &bar.full_v[st] : &bar.full_k[st]);
+                if (IS_V) mbar_arrive(&bar.clean_v[st]);
+            }
+            if (j + 1 < part.j1) {
+                look4<D>(a, it, part, j + 1, t);
+                fetch4<D, IS_V>(a, t);
+            }
+        }
+    });
+}
+
+// As restore_values: rows that see a V vector of NaN have no result.
+template <int D>
+__device__ __noinline__ void restore_none(const AttnArgs& a, const Current& cur, int pos, uint32_t tm_o) {
+    const int lane = threadIdx.x & 31;
+    const Item& it = cur.it;
+    bool hit = false;
+    for (int j = cur.part.j0; j < cur.part.j1; ++j) {
+        const int k0 = tile_key<kN>(it, j);
+        if (seen_whole<kN>(a, it, k0)) continue;
+        for (int h = 0; h < kN; h += 32) {
+            const int p = k0 + h + lane, row = item_sees(it, p) ? pool_row(a.b, cur.part.s, it.kvh, p, nullptr) : -1;
+            const bool none = row >= 0 && (__ldg(a.scales + row) >> 16 & 0x7f80u) == 0x7f80u;
+            for (unsigned left = __ballot_sync(0xffffffffu, none); left; left &= left - 1)
+                hit |= row_sees(a, pos, k0 + h + __ffs(left) - 1);
+        }
+    }
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        uint32_t w[32];
+        tmem_ld32(tm_o + 32 * c, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = hit ? 0x7fffffffu : __float_as_uint(o[e]);
+        tmem_st32(tm_o + 32 * c, w);
+        tmem_st_wait();
+    }
+}
+
 // Row ri (r of its row tile) of a split item, joined over its CTAs in order
 // into shared memory: kJoin parts of 32 columns are read at once, since each
 // read is a trip to L2.  A function of its own, so that its registers are not
@@ -229,7 +365,8 @@ __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, in
     }
 }
 
-template <typename T, int D>
+// FOUR: pages of 4 bits
+template <typename T, int D, bool FOUR>
 __global__ void __launch_bounds__(kThreadsTc, 1)
     paged_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v) {
@@ -276,7 +413,11 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     bool ok = true;
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
-        if (warp == 0 && place.s >= 0) {
+        if (FOUR && warp == 0 && place.s >= 0) {
+            produce4<T, D, false>(a, place, base, bar, cur_s[0], &found_s, ok);
+        } else if (FOUR && warp == 2 && place.s >= 0) {
+            produce4<T, D, true>(a, place, base, bar, cur_s[2], &found_s, ok);
+        } else if (!FOUR && warp == 0 && place.s >= 0) {
             // ---- K and V tiles.  n: tiles so far, over all parts.
             uint32_t n = 0;
             const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
@@ -391,7 +532,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                 }
                 __syncwarp();
             });
-        } else if (warp == 2 && place.s >= 0) {
+        } else if (!FOUR && warp == 2 && place.s >= 0) {
             // ---- what of V must not meet a probability of 0 becomes zeros
             uint32_t n = 0;
             walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
@@ -574,8 +715,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after();
                     // written before V was ready for the products that this thread has waited for
-                    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found_s) >= cur_s[warp].no))
-                        restore_values<T, D>(a, cur_s[warp], pos, tm_ox);
+                    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found_s) >= cur_s[warp].no)) {
+                        if constexpr (FOUR)
+                            restore_none<D>(a, cur_s[warp], pos, tm_ox);
+                        else
+                            restore_values<T, D>(a, cur_s[warp], pos, tm_ox);
+                    }
                 }
                 // ---- the part's result: straight to out, or through the slots
                 const int ri = 128 * x + r;
@@ -682,15 +827,17 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     pdl_wait();  // this kernel's end is the call's end
 }
 
-template <typename T, int D>
+template <typename T, int D, bool FOUR>
 int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
     using L = LayoutTc<D>;
     AttnArgs a = args;
-    CUtensorMap mk, mv;
-    if (int s = paged_pool_map(&mk, a, a.k, D, Half16<T>::kBf16, kN)) return s;
-    if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kN)) return s;
+    CUtensorMap mk = {}, mv = {};
+    if (!FOUR) {
+        if (int s = paged_pool_map(&mk, a, a.k, D, Half16<T>::kBf16, kN)) return s;
+        if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kN)) return s;
+    }
     static std::atomic<unsigned long long> set_on{0};
-    if (int s = allow_smem(paged_attn_tc<T, D>, (int)L::kBytes, set_on)) return s;
+    if (int s = allow_smem(paged_attn_tc<T, D, FOUR>, (int)L::kBytes, set_on)) return s;
     a.tickets += kTcWorkspaceAt / sizeof(unsigned);
     a.slots += kTcWorkspaceAt / sizeof(float);
     // one CTA an SM, as many as have slots in the workspace
@@ -712,7 +859,7 @@ int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = after_other ? 1 : 0;
-    INFERNT_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_attn_tc<T, D>, static_cast<const AttnArgs>(a),
+    INFERNT_CUDA_TRY(cudaLaunchKernelEx(&cfg, paged_attn_tc<T, D, FOUR>, static_cast<const AttnArgs>(a),
                                         static_cast<const CUtensorMap>(mk), static_cast<const CUtensorMap>(mv)));
     return INFERNT_OK;
 }
@@ -742,12 +889,24 @@ int paged_pool_map(CUtensorMap* map, const AttnArgs& a, const void* pool, int D,
     return INFERNT_OK;
 }
 
-int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st) {
+namespace {
+
+template <bool FOUR>
+int launch_kind(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st) {
     if (dtype == INFERNT_DTYPE_BF16)
-        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64>(a, after_other, st)
-                              : launch_tc<__nv_bfloat16, 128>(a, after_other, st);
-    return head_dim == 64 ? launch_tc<__half, 64>(a, after_other, st)
-                          : launch_tc<__half, 128>(a, after_other, st);
+        return head_dim == 64 ? launch_tc<__nv_bfloat16, 64, FOUR>(a, after_other, st)
+                              : launch_tc<__nv_bfloat16, 128, FOUR>(a, after_other, st);
+    return head_dim == 64 ? launch_tc<__half, 64, FOUR>(a, after_other, st)
+                          : launch_tc<__half, 128, FOUR>(a, after_other, st);
+}
+
+}  // namespace
+
+int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st) {
+    return launch_kind<false>(a, head_dim, dtype, after_other, st);
+}
+int paged4_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st) {
+    return launch_kind<true>(a, head_dim, dtype, after_other, st);
 }
 
 }  // namespace infernt

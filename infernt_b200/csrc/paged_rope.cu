@@ -11,7 +11,7 @@
 #include <cmath>
 #include <cstdint>
 
-#include "paged.cuh"
+#include "paged_rope.cuh"
 
 namespace infernt {
 
@@ -62,124 +62,97 @@ int check_batch_pointers(const char* op, const infernt_paged_cache* c, const inf
     return check_device_pointer(op, "err", err);
 }
 
+int rope_frequencies(const char* op, const infernt_rope_params& p, int head_dim, RopeDev* out) {
+    const int R = p.rotary_dim;
+    INFERNT_REQUIRE(R >= 2 && R <= head_dim && R % 2 == 0, "%s: rotary_dim %d of %d", op, R, head_dim);
+    INFERNT_REQUIRE(std::isfinite(p.theta) && p.theta > 0, "%s: theta %g", op, p.theta);
+    INFERNT_REQUIRE(p.scaling >= INFERNT_ROPE_NONE && p.scaling <= INFERNT_ROPE_YARN, "%s: scaling %d", op,
+                    p.scaling);
+    INFERNT_REQUIRE(p.scaling == INFERNT_ROPE_NONE || (std::isfinite(p.factor) && p.factor > 0),
+                    "%s: factor %g", op, p.factor);
+    if (p.scaling == INFERNT_ROPE_LLAMA3 || p.scaling == INFERNT_ROPE_YARN)
+        INFERNT_REQUIRE(p.original_max_len >= 1 && std::isfinite(p.low) && std::isfinite(p.high) && p.low > 0 &&
+                            p.high > p.low,
+                        "%s: original_max_len %d, low %g, high %g", op, p.original_max_len, p.low, p.high);
+    INFERNT_REQUIRE(p.scaling != INFERNT_ROPE_YARN || p.theta > 1.0, "%s: YaRN needs theta above 1", op);
+    const double two_pi = 6.283185307179586476925;
+    double lo = 0, hi = 0;
+    out->half = R / 2;
+    out->interleaved = p.interleaved != 0;
+    out->magnitude64 = 1.0;
+    if (p.scaling == INFERNT_ROPE_YARN) {
+        // the pair index at which a pair makes t turns over the original context
+        auto border = [&](double t) {
+            return R * std::log(p.original_max_len / (t * two_pi)) / (2 * std::log(p.theta));
+        };
+        lo = std::fmax(0.0, std::floor(border(p.high)));
+        hi = std::fmin(R - 1.0, std::ceil(border(p.low)));
+        // a factor up to 1 stretches nothing, and its logarithm would shrink or flip q and k
+        out->magnitude64 = p.factor > 1.0 ? 0.1 * std::log(p.factor) + 1.0 : 1.0;
+    }
+    // f_i by repeated products: 64 of them are off by 64 x 2^-53; divisions
+    // stay out of the loop, which runs at each call
+    const double ratio = std::pow(p.theta, -2.0 / R), turns = 1.0 / two_pi;
+    const double shrink = p.scaling == INFERNT_ROPE_NONE ? 1.0 : 1.0 / p.factor, llama3 = 1.0 / (p.high - p.low),
+                 yarn = 1.0 / std::fmax(hi - lo, 0.001);
+    double f = 1.0;
+    for (int i = 0; i < R / 2; ++i, f *= ratio) {
+        double g = f, keep = 1.0;  // share of f, the rest is f / factor
+        if (p.scaling == INFERNT_ROPE_LINEAR) keep = 0.0;
+        if (p.scaling == INFERNT_ROPE_LLAMA3)
+            keep = (p.original_max_len * f * turns - p.low) * llama3;
+        if (p.scaling == INFERNT_ROPE_YARN) keep = 1.0 - (i - lo) * yarn;
+        keep = std::fmin(1.0, std::fmax(0.0, keep));
+        if (p.scaling != INFERNT_ROPE_NONE) g = f * keep + f * shrink * (1.0 - keep);
+        out->turns[i] = g * turns;
+    }
+    out->magnitude = (float)out->magnitude64;
+    return INFERNT_OK;
+}
+
+int rope_append_args(const char* op, void* q_out, int ldo, const void* q, int ldq, int nq, const void* k, int ldk,
+                     const void* v, int ldv, int src_dtype, int nkv, int head_dim, int dtype,
+                     const infernt_ragged_batch* batch, const infernt_rope_params* rope, const unsigned* err,
+                     RopeArgs* a, RopeDev* d, bool* empty) {
+    INFERNT_REQUIRE(rope, "%s: null rope parameters", op);
+    INFERNT_REQUIRE((q != nullptr) == (q_out != nullptr) && (k != nullptr) == (v != nullptr) && (q || k),
+                    "%s: q with q_out, k with v", op);
+    INFERNT_REQUIRE(src_dtype == INFERNT_DTYPE_F32 || src_dtype == INFERNT_DTYPE_BF16 || src_dtype == INFERNT_DTYPE_F16,
+                    "%s: source type %d", op, src_dtype);
+    const long long kvd = (long long)nkv * head_dim;
+    INFERNT_REQUIRE(!q || (nq >= 1 && ldq >= (long long)nq * head_dim && ldo >= (long long)nq * head_dim),
+                    "%s: %d query heads, rows %d and %d apart", op, nq, ldq, ldo);
+    INFERNT_REQUIRE(!k || (ldk >= kvd && ldv >= kvd), "%s: k and v rows %d and %d apart for %lld values", op, ldk, ldv,
+                    kvd);
+    INFERNT_REQUIRE(!q || q != q_out || (src_dtype == dtype && ldq == ldo),
+                    "%s: q_out may be q only with its type and row stride", op);
+    const unsigned esize = src_dtype == INFERNT_DTYPE_F32 ? 4u : 2u;
+    for (const void* p : {q, k, v})
+        INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(p) % esize == 0, "%s: misaligned source", op);
+    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(q_out) % 2 == 0 && reinterpret_cast<uintptr_t>(err) % 4 == 0,
+                    "%s: misaligned q_out or err", op);
+    if (int s = rope_frequencies(op, *rope, head_dim, d)) return s;
+    *empty = batch->num_seqs == 0 || batch->num_rows == 0;
+    if (*empty) return INFERNT_OK;
+    if (int s = check_device_pointer(op, "q", q)) return s;
+    if (int s = check_device_pointer(op, "q_out", q_out)) return s;
+    if (int s = check_device_pointer(op, "k", k)) return s;
+    if (int s = check_device_pointer(op, "v", v)) return s;
+    *a = {};
+    a->q = q;
+    a->k = k;
+    a->v = v;
+    a->q_out = q_out;
+    a->ldq = ldq;
+    a->ldk = ldk;
+    a->ldv = ldv;
+    a->ldo = ldo;
+    a->nq = q ? nq : 0;
+    a->D = head_dim;
+    return INFERNT_OK;
+}
+
 namespace {
-
-constexpr int kRopeThreads = 128;
-constexpr int kMaxPairs = 64;
-
-struct RopeDev {
-    double turns[kMaxPairs];  // f_i / 2 pi
-    float magnitude;
-    int half, interleaved;
-};
-
-struct RopeArgs {
-    PagedBatch b;
-    const void* q;
-    const void* k;
-    const void* v;
-    void* q_out;
-    void* kp;
-    void* vp;
-    long long ldq, ldk, ldv, ldo;
-    int nq, D;
-    unsigned* err;
-};
-
-// The sequence that holds row r (the last s with q_start[s] <= r), by a
-// search of 32 places a round: one round trip for up to 32 sequences, two
-// for up to 1024.  Whatever the array holds, the result is in [0, n).
-__device__ __forceinline__ int find_seq(const int* q_start, int n, int r) {
-    const int lane = threadIdx.x & 31;
-    int lo = 0, hi = n;  // the answer is in [lo, hi)
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 31) / 32;
-        const int at = lo + lane * step;
-        const unsigned le = __ballot_sync(0xffffffffu, at < hi && q_start[at] <= r);
-        const int k = le ? 31 - __clz(le) : 0;
-        lo = lo + k * step;
-        hi = min(hi, lo + step);
-    }
-    return lo;
-}
-
-template <typename S>
-__device__ __forceinline__ float source_value(const S* p) {
-    return to_f32(*p);
-}
-template <>
-__device__ __forceinline__ float source_value<__half>(const __half* p) {
-    return __half2float(*p);
-}
-
-// Where row r of the batch goes: its sequence's position, and the page row of
-// head 0 (-1: nowhere).  False: the row stays as it is.
-__device__ __forceinline__ bool place_row(const RopeArgs& a, int r, int& pos, long long& row) {
-    const int s = find_seq(a.b.q_start, a.b.num_seqs, r);
-    const PagedSeq seq = paged_seq(a.b, s, a.err);
-    const int i = r - seq.row0;
-    if (i < 0 || i >= seq.n_new) return false;  // behind the last sequence, or a sequence that is skipped
-    pos = seq.len - seq.n_new + i;
-    if (pos < 0) return false;
-    row = -1;
-    if (a.k) {
-        const int pi = a.b.by_page(pos), page = a.b.table[(size_t)s * a.b.table_stride + pi];
-        if (page >= 0 && page < a.b.num_pages)
-            row = (long long)page * a.b.nkv * a.b.page_size + (pos - pi * a.b.page_size);
-        else if (a.err && threadIdx.x == 0)
-            atomicOr(a.err, kErrPage);
-    }
-    return true;
-}
-
-// Error bits of the sequences: this block's share of them, since one that no row
-// leads to (no new tokens, or a start above its end) is met nowhere else.
-__device__ __forceinline__ void check_sequences(const RopeArgs& a) {
-    if (a.err && threadIdx.x == kRopeThreads - 1)
-        for (int s = blockIdx.x; s < a.b.num_seqs; s += gridDim.x) paged_seq(a.b, s, a.err);
-}
-
-// Cosine and sine of pair p at position pos, times the magnitude.
-__device__ __forceinline__ float2 turn_of(const RopeDev& rope, int p, int pos) {
-    const double t = (double)pos * rope.turns[p];
-    const float f = (float)(t - rint(t));  // [-1/2, 1/2] turns
-    float sn, c;
-    sincospif(2.0f * f, &sn, &c);
-    return make_float2(c * rope.magnitude, sn * rope.magnitude);
-}
-
-// Eight values of a row as loaded, and as FP32.
-template <typename S>
-struct Eight {
-    uint4 w[sizeof(S) / 2];
-};
-template <typename S>
-__device__ __forceinline__ Eight<S> load_eight(const S* p) {
-    Eight<S> v;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(S) / 2; ++i) v.w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-    return v;
-}
-__device__ __forceinline__ void to_floats(const Eight<float>& v, float (&x)[8]) {
-    const uint32_t w[8] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w, v.w[1].x, v.w[1].y, v.w[1].z, v.w[1].w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
-}
-template <typename S>
-__device__ __forceinline__ void to_floats(const Eight<S>& v, float (&x)[8]) {
-    const uint32_t w[4] = {v.w[0].x, v.w[0].y, v.w[0].z, v.w[0].w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 p = Half16<S>::unpack(w[i]);
-        x[2 * i] = p.x;
-        x[2 * i + 1] = p.y;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void store_eight(T* p, const float (&x)[8]) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(Half16<T>::pack(x[0], x[1]), Half16<T>::pack(x[2], x[3]),
-                                              Half16<T>::pack(x[4], x[5]), Half16<T>::pack(x[6], x[7]));
-}
 
 // A block per token row; for rotary_dim a multiple of 16 and rows that allow
 // 16-byte loads.  The unit of work is two blocks of eight values, D / 16 to a
@@ -329,53 +302,6 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope(const RopeArgs a, con
     check_sequences(a);
 }
 
-int rope_frequencies(const infernt_rope_params& p, int head_dim, RopeDev* out) {
-    const int R = p.rotary_dim;
-    INFERNT_REQUIRE(R >= 2 && R <= head_dim && R % 2 == 0, "paged_rope_append: rotary_dim %d of %d", R, head_dim);
-    INFERNT_REQUIRE(std::isfinite(p.theta) && p.theta > 0, "paged_rope_append: theta %g", p.theta);
-    INFERNT_REQUIRE(p.scaling >= INFERNT_ROPE_NONE && p.scaling <= INFERNT_ROPE_YARN, "paged_rope_append: scaling %d",
-                    p.scaling);
-    INFERNT_REQUIRE(p.scaling == INFERNT_ROPE_NONE || (std::isfinite(p.factor) && p.factor > 0),
-                    "paged_rope_append: factor %g", p.factor);
-    if (p.scaling == INFERNT_ROPE_LLAMA3 || p.scaling == INFERNT_ROPE_YARN)
-        INFERNT_REQUIRE(p.original_max_len >= 1 && std::isfinite(p.low) && std::isfinite(p.high) && p.low > 0 &&
-                            p.high > p.low,
-                        "paged_rope_append: original_max_len %d, low %g, high %g", p.original_max_len, p.low, p.high);
-    INFERNT_REQUIRE(p.scaling != INFERNT_ROPE_YARN || p.theta > 1.0, "paged_rope_append: YaRN needs theta above 1");
-    const double two_pi = 6.283185307179586476925;
-    double lo = 0, hi = 0;
-    out->half = R / 2;
-    out->interleaved = p.interleaved != 0;
-    out->magnitude = 1.0f;
-    if (p.scaling == INFERNT_ROPE_YARN) {
-        // the pair index at which a pair makes t turns over the original context
-        auto border = [&](double t) {
-            return R * std::log(p.original_max_len / (t * two_pi)) / (2 * std::log(p.theta));
-        };
-        lo = std::fmax(0.0, std::floor(border(p.high)));
-        hi = std::fmin(R - 1.0, std::ceil(border(p.low)));
-        // a factor up to 1 stretches nothing, and its logarithm would shrink or flip q and k
-        out->magnitude = p.factor > 1.0 ? (float)(0.1 * std::log(p.factor) + 1.0) : 1.0f;
-    }
-    // f_i by repeated products: 64 of them are off by 64 x 2^-53; divisions
-    // stay out of the loop, which runs at each call
-    const double ratio = std::pow(p.theta, -2.0 / R), turns = 1.0 / two_pi;
-    const double shrink = p.scaling == INFERNT_ROPE_NONE ? 1.0 : 1.0 / p.factor, llama3 = 1.0 / (p.high - p.low),
-                 yarn = 1.0 / std::fmax(hi - lo, 0.001);
-    double f = 1.0;
-    for (int i = 0; i < R / 2; ++i, f *= ratio) {
-        double g = f, keep = 1.0;  // share of f, the rest is f / factor
-        if (p.scaling == INFERNT_ROPE_LINEAR) keep = 0.0;
-        if (p.scaling == INFERNT_ROPE_LLAMA3)
-            keep = (p.original_max_len * f * turns - p.low) * llama3;
-        if (p.scaling == INFERNT_ROPE_YARN) keep = 1.0 - (i - lo) * yarn;
-        keep = std::fmin(1.0, std::fmax(0.0, keep));
-        if (p.scaling != INFERNT_ROPE_NONE) g = f * keep + f * shrink * (1.0 - keep);
-        out->turns[i] = g * turns;
-    }
-    return INFERNT_OK;
-}
-
 template <typename S, typename T>
 int launch(const RopeArgs& a, const RopeDev& d, cudaStream_t st) {
     // rows of S or T `ld` apart that start where 16 bytes may be loaded
@@ -411,46 +337,17 @@ extern "C" int infernt_paged_rope_append(void* q_out, int ldo, const void* q, in
     const char* op = "paged_rope_append";
     if (int s = check_paged_cache(op, cache)) return s;
     if (int s = check_ragged_batch(op, batch)) return s;
-    INFERNT_REQUIRE(rope, "%s: null rope parameters", op);
-    INFERNT_REQUIRE((q != nullptr) == (q_out != nullptr) && (k != nullptr) == (v != nullptr) && (q || k),
-                    "%s: q with q_out, k with v", op);
-    INFERNT_REQUIRE(src_dtype == INFERNT_DTYPE_F32 || src_dtype == INFERNT_DTYPE_BF16 || src_dtype == INFERNT_DTYPE_F16,
-                    "%s: source type %d", op, src_dtype);
-    const int D = cache->head_dim;
-    const long long kvd = (long long)cache->num_kv_heads * D;
-    INFERNT_REQUIRE(!q || (nq >= 1 && ldq >= (long long)nq * D && ldo >= (long long)nq * D),
-                    "%s: %d query heads, rows %d and %d apart", op, nq, ldq, ldo);
-    INFERNT_REQUIRE(!k || (ldk >= kvd && ldv >= kvd), "%s: k and v rows %d and %d apart for %lld values", op, ldk, ldv,
-                    kvd);
-    INFERNT_REQUIRE(!q || q != q_out || (src_dtype == cache->dtype && ldq == ldo),
-                    "%s: q_out may be q only with its type and row stride", op);
-    const unsigned esize = src_dtype == INFERNT_DTYPE_F32 ? 4u : 2u;
-    for (const void* p : {q, k, v})
-        INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(p) % esize == 0, "%s: misaligned source", op);
-    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(q_out) % 2 == 0 && reinterpret_cast<uintptr_t>(err) % 4 == 0,
-                    "%s: misaligned q_out or err", op);
     RopeArgs a;
     RopeDev d;
-    if (int s = rope_frequencies(*rope, D, &d)) return s;
-    if (batch->num_seqs == 0 || batch->num_rows == 0) return INFERNT_OK;
+    bool empty;
+    if (int s = rope_append_args(op, q_out, ldo, q, ldq, nq, k, ldk, v, ldv, src_dtype, cache->num_kv_heads,
+                                 cache->head_dim, cache->dtype, batch, rope, err, &a, &d, &empty))
+        return s;
+    if (empty) return INFERNT_OK;
     if (int s = check_batch_pointers(op, cache, batch, err)) return s;
-    if (int s = check_device_pointer(op, "q", q)) return s;
-    if (int s = check_device_pointer(op, "q_out", q_out)) return s;
-    if (int s = check_device_pointer(op, "k", k)) return s;
-    if (int s = check_device_pointer(op, "v", v)) return s;
     a.b = paged_batch(*cache, *batch);
-    a.q = q;
-    a.k = k;
-    a.v = v;
-    a.q_out = q_out;
     a.kp = cache->k;
     a.vp = cache->v;
-    a.ldq = ldq;
-    a.ldk = ldk;
-    a.ldv = ldv;
-    a.ldo = ldo;
-    a.nq = q ? nq : 0;
-    a.D = D;
     a.err = err;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return cache->dtype == INFERNT_DTYPE_BF16 ? launch_src<__nv_bfloat16>(a, d, src_dtype, st)

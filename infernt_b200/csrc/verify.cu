@@ -1,0 +1,622 @@
+// verify.cu — drafted tokens against the target's distributions: which drafts
+// of each sequence stand, and the token after them, drawn from given random
+// numbers (src/engine.cpp:78-104 draws one token from softmax(logits / T) on
+// the host, by the same walk along the cumulative sum).
+//
+//   p = e^((l - max l) / T) / Z;  a draft d stands while u q(d) < p(d);
+//   at the first that does not, the token is the lowest i with
+//   sum_{k <= i} w_k > u' sum_k w_k,  w = max(p - q, 0).
+//
+// Two launches: the statistics of every row (its logits are read once, HBM),
+// then a cluster of CTAs a sequence, which finds the row where the sequence
+// stops and draws.  A border of the cumulative sum is as near as 10^-6 to
+// u' sum w where there are 10^5 tokens, so what the draw is made of (Z, the
+// weights, their sums) is in 64 bits; acceptance is one comparison a row, and
+// its Z a sum in FP32.
+#include <cstdint>
+
+#include "paged.cuh"
+#include "sample.cuh"
+
+namespace infernt {
+namespace {
+
+constexpr int kStatThreads = 256;
+constexpr int kStatTile = 8192;   // elements of a row that a CTA holds in registers
+constexpr int kMostParts = 32;    // CTAs of a row
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What a CTA knows of its part of a row: e is the sum of 2^((l - m) c).
+struct RowPart {
+    float m, e;
+    int best;   // the lowest index of m; -1: no number
+    int flags;  // kBad: a NaN or an element out of range
+};
+constexpr int kBad = 1;
+
+struct VerifyArgs {
+    const void* target;
+    const float* draft;
+    long long ld, draft_ld;
+    const int* tokens;
+    const int* q_start;
+    const float* temperature;
+    const float* u;
+    const int* kv_len;
+    int* kept;
+    int* out;
+    int* accepted;
+    RowPart* parts;  // [num_rows][kMostParts]
+    int num_seqs, num_rows, V, n_parts, part;  // part: elements of one
+    unsigned* err;
+};
+
+template <typename L>
+__device__ __forceinline__ float element(const L* p) {
+    return to_f32(*p);
+}
+template <>
+__device__ __forceinline__ float element<__half>(const __half* p) {
+    return __half2float(*p);
+}
+
+__device__ __forceinline__ bool is_greedy(float t) { return !(t > 0.0f); }
+// log2(e) / T; an infinite T would make 0 of -infinity, one near 0 infinity of 0
+__device__ __forceinline__ float sharpness(float t) { return fminf(fmaxf(kLog2e / t, 1e-30f), 1e30f); }
+__device__ __forceinline__ double sharpness64(float t) {
+    return fmin(fmax(1.4426950408889634074 / (double)t, 1e-30), 1e30);
+}
+
+// What a logit or a probability may not be.
+template <bool PROBS>
+__device__ __forceinline__ bool is_none(float x) {
+    return !(x < INFINITY) || (PROBS && x < 0.0f);
+}
+
+// 16 bytes of a row as FP32
+__device__ __forceinline__ void sixteen(const float* p, float (&x)[4]) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+    x[0] = v.x;
+    x[1] = v.y;
+    x[2] = v.z;
+    x[3] = v.w;
+}
+template <typename L>
+__device__ __forceinline__ void sixteen(const L* p, float (&x)[8]) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 y = Half16<L>::unpack(w[i]);
+        x[2 * i] = y.x;
+        x[2 * i + 1] = y.y;
+    }
+}
+
+// The warp's largest by argmax_better, and its index (-1: none).
+__device__ __forceinline__ void best_of_warp(float& m, int& at) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, m, o);
+        const int oi = __shfl_xor_sync(0xffffffffu, at, o);
+        if (oi >= 0 && (at < 0 || argmax_better(om, oi, m, at))) {
+            m = om;
+            at = oi;
+        }
+    }
+}
+
+// Block (row, part).  A thread's elements come in 16-byte loads, all of them
+// before the first is used; rows that do not start on 16 bytes start their
+// first vector before the row, and the elements outside it are not loaded.
+template <typename L, bool PROBS>
+__global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) {
+    constexpr int N = 16 / (int)sizeof(L), VECS = kStatTile / N / kStatThreads;
+    __shared__ float m_s[kStatThreads / 32], e_s[kStatThreads / 32];
+    __shared__ int at_s[kStatThreads / 32], bad_s;
+    pdl_launch_dependents();
+    const int r = blockIdx.x, part = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int s = find_seq(a.q_start, a.num_seqs, r);
+    const float t = a.temperature ? a.temperature[s] : 1.0f;
+    if (PROBS && !is_greedy(t)) return;  // only what is drafted, and the row where the sequence stops, are asked for
+    const L* row = static_cast<const L*>(a.target) + (long long)r * a.ld;
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(L));
+    const float c = is_greedy(t) ? 0.0f : sharpness(t);
+    if (tid == 0) bad_s = 0;
+    float m = -INFINITY, e = 0.0f;
+    int at = -1;
+    bool bad = false;
+    for (int tile = 0; tile < a.part; tile += kStatTile) {
+        const int base = part * a.part + tile - off;
+        float x[VECS][N];
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+            const int k = base + (i * kStatThreads + tid) * N;
+            if (k >= 0 && k + N <= a.V) {
+                sixteen(row + k, x[i]);
+#pragma unroll
+                for (int j = 0; j < N; ++j) bad |= is_none<PROBS>(x[i][j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const bool in = k + j >= 0 && k + j < a.V;
+                    x[i][j] = in ? element(row + k + j) : -INFINITY;
+                    bad |= in && is_none<PROBS>(x[i][j]);
+                }
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VECS; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) top = fmaxf(top, x[i][j]);
+        const float ref = fmaxf(m, top);
+        if (c > 0.0f && ref > -INFINITY) {
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < VECS; ++i)
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    float y;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x[i][j] - ref) * c));
+                    sum[j & 1] += y;
+                }
+            e = e * (m == -INFINITY ? 0.0f : exp2f((m - ref) * c)) + sum[0] + sum[1];
+        }
+        if (top > m) {  // the lowest index of it
+            m = top;
+#pragma unroll
+            for (int i = VECS - 1; i >= 0; --i)
+#pragma unroll
+                for (int j = N - 1; j >= 0; --j)
+                    if (x[i][j] == top) at = base + (i * kStatThreads + tid) * N + j;
+        }
+    }
+    // the warps' and then the CTA's
+    float wm = m;
+    int wat = at;
+    best_of_warp(wm, wat);
+    e = warp_sum(m == -INFINITY ? 0.0f : e * exp2f((m - wm) * c));
+    __syncthreads();
+    if (bad) bad_s = 1;
+    if (lane == 0) {
+        m_s[warp] = wm;
+        e_s[warp] = e;
+        at_s[warp] = wat;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    m = lane < kStatThreads / 32 ? m_s[lane] : -INFINITY;
+    at = lane < kStatThreads / 32 ? at_s[lane] : -1;
+    e = lane < kStatThreads / 32 ? e_s[lane] : 0.0f;
+    wm = m;
+    best_of_warp(wm, at);
+    e = warp_sum(m == -INFINITY ? 0.0f : e * exp2f((m - wm) * c));
+    if (lane == 0) a.parts[(size_t)r * kMostParts + part] = {wm, e, at, bad_s ? kBad : 0};
+}
+
+// ------------------------------------------------------------------- draw
+constexpr int kDrawThreads = 256;
+constexpr int kDrawWarps = kDrawThreads / 32;
+constexpr int kCluster = 8;
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ double peer_double(const double* p, uint32_t rank) {
+    uint32_t at;
+    double v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ double warp_sum64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// 2^x for x <= 0, to about 2e-15: x = (32 n + j) / 32 + g, |g| <= 1 / 64, so
+// 2^x = 2^n 2^(j / 32) 2^g, the last by its Taylor series to the fifth power
+// (the sixth is below (ln 2 / 64)^6 / 720 = 2e-15), the middle one of a table.
+__device__ __forceinline__ double exp2_64(double x, const double* table) {
+    if (!(x > -1000.0)) return 0.0;  // -infinity too
+    const double big = 6755399441055744.0;  // 1.5 x 2^52: rounds 32 x to a whole number in its low bits
+    const double t = fma(x, 32.0, big);
+    const int k = __double2loint(t);
+    const double g = fma(t - big, -1.0 / 32.0, x) * 0.69314718055994530942;
+    double p = fma(g, 1.0 / 120.0, 1.0 / 24.0);
+    p = fma(p, g, 1.0 / 6.0);
+    p = fma(p, g, 0.5);
+    p = fma(p, g, 1.0);
+    p = fma(p, g, 1.0);
+    const double y = p * table[k & 31];
+    return __hiloint2double(__double2hiint(y) + (k >> 5) * (1 << 20), __double2loint(y));
+}
+
+// What becomes of a sequence.
+struct Stop {
+    int token;  // >= 0: the token is known
+    int minus;  // what is subtracted: 1 the draft's distribution, 2 the drafted token alone
+    float m;    // the largest logit of the row where it stops
+    unsigned err;
+};
+
+// A row's statistics, by a whole warp.
+template <bool PROBS>
+__device__ __forceinline__ RowPart row_stats(const VerifyArgs& a, int r, float c) {
+    const int lane = threadIdx.x & 31;
+    RowPart p = {-INFINITY, 0.0f, -1, 0};
+    if (lane < a.n_parts) p = a.parts[(size_t)r * kMostParts + lane];
+    const float m = p.m;
+    best_of_warp(p.m, p.best);
+    p.e = warp_sum(m == -INFINITY ? 0.0f : p.e * exp2f((m - p.m) * c));
+    p.flags = __any_sync(0xffffffffu, p.flags & kBad) || p.best < 0 || !(p.m > (PROBS ? 0.0f : -INFINITY)) ? kBad : 0;
+    return p;
+}
+
+// Element e of row r that is a probability, or less than 0.
+template <typename L>
+__device__ __forceinline__ float probability(const VerifyArgs& a, int r, int e) {
+    const float p = element(static_cast<const L*>(a.target) + (long long)r * a.ld + e);
+    return is_none<true>(p) ? -1.0f : p;
+}
+
+// A cluster of CTAs a sequence, a slice of the vocabulary each.  In every CTA
+// the warps judge the sequence's rows; then
+//   Z = sum e_i, and W = sum w_i, over the cluster;
+//   the CTA, and in it the warp, whose part of the sum has u W in it walks
+//   along it.
+// The weights are computed again in each pass (the logits are in L2): a CTA
+// then needs few registers, and the sequences' waits and sums overlap.
+template <typename L, bool PROBS>
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads) verify_draw(const VerifyArgs a) {
+    __shared__ double table[32], sum_s[3][kDrawWarps], shared_s[3];  // shared_s: what the other CTAs read
+    __shared__ int first_s;
+    __shared__ Stop stop_s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x / kCluster;
+    const uint32_t rank = cluster_rank();
+    if (tid < 32) table[tid] = exp2((double)tid / 32.0);
+    if (tid == 0) first_s = 0x7fffffff;
+    const int row0 = a.q_start[s], end = a.q_start[s + 1], n = end - row0;
+    pdl_wait();  // verify_rows; of every CTA, so that this kernel's end is the call's end
+    if (row0 < 0 || n < 0 || end > a.num_rows) {
+        if (rank == 0 && tid == 0 && a.err) atomicOr(a.err, kErrBatch);
+        return;  // the whole cluster
+    }
+    if (n == 0) {
+        if (rank == 0 && tid == 0) {
+            a.accepted[s] = 0;
+            if (a.kept) a.kept[s] = a.kv_len[s];
+        }
+        return;
+    }
+    const float t = a.temperature ? a.temperature[s] : 1.0f;
+    const bool greedy = is_greedy(t), stats = !PROBS || greedy;
+    const float c = greedy ? 0.0f : sharpness(t);
+    const double c64 = greedy ? 0.0 : sharpness64(t);
+    __syncthreads();
+    // ---- the first row whose draft does not stand (a warp a row, in turn)
+    for (int i = warp; i < n; i += kDrawWarps) {
+        const int r = row0 + i;
+        if (__any_sync(0xffffffffu, r > *static_cast<volatile int*>(&first_s))) break;
+        bool stands = false;
+        const int d = i + 1 < n ? a.tokens[r + 1] : -1;
+        const bool drafted = d >= 0 && d < a.V;
+        RowPart p = {0.0f, 1.0f, 0, 0};
+        if (stats) p = row_stats<PROBS>(a, r, c);
+        if (greedy) {
+            stands = drafted && d == p.best && !(p.flags & kBad);
+        } else if (drafted && !(p.flags & kBad)) {
+            double pd;
+            if (PROBS) {
+                pd = probability<L>(a, r, d);
+            } else {
+                const float l = element(static_cast<const L*>(a.target) + (long long)r * a.ld + d);
+                pd = exp2_64(((double)l - (double)p.m) * c64, table) / (double)p.e;
+            }
+            const float q = a.draft ? a.draft[(long long)r * a.draft_ld + d] : 1.0f;
+            float u = a.u[r];
+            u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+            stands = (double)u * (double)q < pd;
+        }
+        if (!stands && lane == 0) atomicMin(&first_s, r);
+        __syncwarp();
+    }
+    __syncthreads();
+    // ---- what becomes of the sequence, by one warp
+    const int stop = first_s;
+    if (warp == 0) {
+        Stop st = {-1, 0, 0.0f, 0u};
+        const int d = stop + 1 < end ? a.tokens[stop + 1] : -1;
+        const bool drafted = d >= 0 && d < a.V;
+        RowPart p = {0.0f, 1.0f, 0, 0};
+        if (stats) p = row_stats<PROBS>(a, stop, c);
+        if (stop + 1 < end && !drafted) st.err |= kErrToken;
+        if (p.flags & kBad) {
+            st.token = p.best < 0 ? 0 : p.best;
+            st.err |= kErrValue;
+        } else if (greedy) {
+            st.token = p.best;
+        } else if (drafted) {
+            st.minus = a.draft ? 1 : 2;
+        }
+        st.m = p.m;
+        if (lane == 0) stop_s = st;
+    }
+    __syncthreads();
+    const Stop st = stop_s;
+    if (rank == 0) {
+        const int good = stop - row0;
+        for (int i = tid; i < n; i += kDrawThreads)
+            if (i != good) a.out[row0 + i] = i < good ? a.tokens[row0 + i + 1] : -1;
+        if (tid == 0) {
+            a.accepted[s] = good;
+            if (a.kept) a.kept[s] = a.kv_len[s] - (n - 1 - good);
+            if (st.token >= 0) a.out[stop] = st.token;
+            if (a.err && st.err) atomicOr(a.err, st.err);
+        }
+    }
+    if (st.token >= 0) return;  // the whole cluster
+    // ---- the draw.  This CTA's slice, and in it the warps' segments of whole groups of 128 elements.
+    const L* row = static_cast<const L*>(a.target) + (long long)stop * a.ld;
+    const float* draft = a.draft ? a.draft + (long long)stop * a.draft_ld : nullptr;
+    const int groups = (a.V + 127) / 128, per = (groups + kCluster * kDrawWarps - 1) / (kCluster * kDrawWarps);
+    const int g0 = ((int)rank * kDrawWarps + warp) * per, g1 = min(groups, g0 + per);
+    const int d = st.minus == 2 ? a.tokens[stop + 1] : -1;
+    const double cm = c64 * (double)st.m;
+    int minus = st.minus;
+    bool bad = false;
+    auto weight = [&](int i) {  // e_i, or p_i
+        const float l = element(row + i);
+        if (!PROBS) return exp2_64(fma((double)l, c64, -cm), table);
+        bad |= is_none<true>(l);
+        return (double)l;
+    };
+    double z = 1.0;
+    // the sum over the CTA's warps into its shared_s[slot], then over the cluster, both in order
+    auto over_cluster = [&](double v, int slot) {
+        v = warp_sum64(v);
+        if (lane == 0) sum_s[slot][warp] = v;
+        __syncthreads();
+        if (tid == 0) {
+            double x = 0.0;
+            for (int w = 0; w < kDrawWarps; ++w) x += sum_s[slot][w];
+            shared_s[slot] = x;
+        }
+        cluster_sync();
+        double x = 0.0;
+        for (int k = 0; k < kCluster; ++k) x += peer_double(&shared_s[slot], k);
+        return x;
+    };
+    auto left = [&](int i, double e) {  // the weight that is drawn from
+        double w = PROBS ? e : e * z;
+        if (minus == 1) {
+            const float q = draft[i];
+            w -= fabsf(q) < INFINITY ? (double)q : INFINITY;
+        }
+        if (minus == 2 && i == d) w = 0.0;
+        return w > 0.0 ? w : 0.0;
+    };
+    if (!PROBS) {
+        double v = 0.0;
+        for (int g = g0; g < g1; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = g * 128 + 32 * j + lane;
+                if (i < a.V) v += weight(i);
+            }
+        z = 1.0 / over_cluster(v, 0);
+    }
+    double mine = 0.0, total = 0.0;
+    for (int pass = 0; pass < 2; ++pass) {
+        mine = 0.0;
+        for (int g = g0; g < g1; ++g)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = g * 128 + 32 * j + lane;
+                if (i < a.V) mine += left(i, weight(i));
+            }
+        total = over_cluster(mine, 1);
+        if (total > 0.0 || minus == 0) break;
+        minus = 0;  // nothing is left: from p itself
+        cluster_sync();  // shared_s is read
+    }
+    // a probability that is none, anywhere in the row
+    double none = 0.0;
+    if (PROBS) none = over_cluster(bad ? 1.0 : 0.0, 2);
+    if (PROBS && (none > 0.0 || !(total > 0.0))) {
+        // its largest number, by the first CTA
+        if (rank == 0) {
+            float m = -INFINITY;
+            int at = -1;
+            for (int i = tid; i < a.V; i += kDrawThreads) {
+                const float x = element(row + i);
+                if (x == x && (at < 0 || argmax_better(x, i, m, at))) {
+                    m = x;
+                    at = i;
+                }
+            }
+            best_of_warp(m, at);
+            __syncthreads();
+            __shared__ float bm_s[kDrawWarps];
+            __shared__ int bi_s[kDrawWarps];
+            if (lane == 0) {
+                bm_s[warp] = m;
+                bi_s[warp] = at;
+            }
+            __syncthreads();
+            if (warp == 0) {
+                m = lane < kDrawWarps ? bm_s[lane] : -INFINITY;
+                at = lane < kDrawWarps ? bi_s[lane] : -1;
+                best_of_warp(m, at);
+                if (lane == 0) {
+                    a.out[stop] = at < 0 ? 0 : at;
+                    if (a.err) atomicOr(a.err, kErrValue);
+                }
+            }
+        }
+        cluster_sync();  // no CTA leaves while others read its sums
+        return;
+    }
+    // ---- the CTA and the warp that have u' total in their part of the sum
+    float uf = a.u[end - 1];
+    uf = uf >= 0.0f ? fminf(uf, 0.99999994f) : 0.0f;
+    const double goal = (double)uf * total;
+    double before = 0.0;
+    int owner = -1, last_some = 0;
+    double owner_before = 0.0, last_before = 0.0;
+    for (int k = 0; k < kCluster; ++k) {
+        const double x = peer_double(&shared_s[1], k);
+        if (x > 0.0) {
+            last_some = k;
+            last_before = before;
+        }
+        if (owner < 0 && before + x > goal) {
+            owner = k;
+            owner_before = before;
+        }
+        before += x;
+    }
+    if (owner < 0) {  // by the rounding of the sums alone: the last that has any
+        owner = last_some;
+        owner_before = last_before;
+    }
+    if ((int)rank == owner) {
+        before = owner_before;
+        int w_owner = -1, w_last = 0;
+        double wb = 0.0, wb_last = 0.0;
+        for (int w = 0; w < kDrawWarps; ++w) {
+            const double x = sum_s[1][w];
+            if (x > 0.0) {
+                w_last = w;
+                wb_last = before;
+            }
+            if (w_owner < 0 && before + x > goal) {
+                w_owner = w;
+                wb = before;
+            }
+            before += x;
+        }
+        if (w_owner < 0) {
+            w_owner = w_last;
+            wb = wb_last;
+        }
+        if (warp == w_owner) {
+            before = wb;
+            int found = -1, some = 0;
+            for (int i0 = g0 * 128; i0 < min(g1 * 128, a.V) && found < 0; i0 += 32) {
+                const int i = i0 + lane;
+                const double w = i < a.V ? left(i, weight(i)) : 0.0;
+                double x = w;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xffffffffu, x, o);
+                    if (lane >= o) x += y;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && before + x > goal);
+                const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+                if (past) found = i0 + __ffs(past) - 1;
+                if (any) some = i0 + 31 - __clz(any);
+                before += __shfl_sync(0xffffffffu, x, 31);
+            }
+            if (lane == 0) a.out[stop] = found >= 0 ? found : some;
+        }
+    }
+    cluster_sync();  // no CTA leaves while others read its sums
+}
+
+template <typename L, bool PROBS>
+int launch(const VerifyArgs& a, cudaStream_t st) {
+    if (a.num_rows > 0) {
+        verify_rows<L, PROBS><<<dim3(a.num_rows, a.n_parts), kStatThreads, 0, st>>>(a);
+        INFERNT_CUDA_TRY(cudaGetLastError());
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.num_seqs * kCluster);
+    cfg.blockDim = dim3(kDrawThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = a.num_rows > 0 ? 1 : 0;  // without rows there is no kernel of this call to wait for
+    INFERNT_CUDA_TRY(cudaLaunchKernelEx(&cfg, verify_draw<L, PROBS>, static_cast<const VerifyArgs>(a)));
+    return INFERNT_OK;
+}
+
+}  // namespace
+}  // namespace infernt
+
+extern "C" size_t infernt_verify_drafts_workspace_bytes(int num_rows, int num_seqs) {
+    (void)num_seqs;
+    return num_rows < 1 ? 16 : (size_t)num_rows * infernt::kMostParts * sizeof(infernt::RowPart);
+}
+
+extern "C" int infernt_verify_drafts(int* out_tokens, int* accepted, const void* target, long long ld, int target_dtype,
+                                     int probabilities, const float* draft_probs, long long draft_ld, const int* tokens,
+                                     const int* q_start, int num_seqs, int num_rows, int vocab_size,
+                                     const float* temperature, const float* u, const int* kv_len, int* kept,
+                                     void* workspace, unsigned* err, void* stream) {
+    using namespace infernt;
+    const char* op = "verify_drafts";
+    INFERNT_REQUIRE(num_seqs >= 0 && num_seqs <= 65535 && num_rows >= 0 && num_rows < kMaxPositions && vocab_size >= 1 &&
+                        vocab_size < kMaxPositions,
+                    "%s: %d sequences, %d rows of %d", op, num_seqs, num_rows, vocab_size);
+    INFERNT_REQUIRE(target_dtype == INFERNT_DTYPE_F32 || target_dtype == INFERNT_DTYPE_BF16 ||
+                        target_dtype == INFERNT_DTYPE_F16,
+                    "%s: target type %d", op, target_dtype);
+    INFERNT_REQUIRE((kv_len != nullptr) == (kept != nullptr), "%s: kv_len with kept", op);
+    if (num_seqs == 0) return INFERNT_OK;
+    INFERNT_REQUIRE(accepted && q_start, "%s: null pointer", op);
+    INFERNT_REQUIRE(num_rows == 0 || (out_tokens && target && tokens && u && workspace), "%s: null pointer", op);
+    INFERNT_REQUIRE(ld >= vocab_size && (!draft_probs || draft_ld >= vocab_size), "%s: rows %lld and %lld apart for %d", op,
+                    ld, draft_ld, vocab_size);
+    INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(target) % (target_dtype == INFERNT_DTYPE_F32 ? 4 : 2) == 0 &&
+                        aligned16(workspace),
+                    "%s: misaligned target or workspace", op);
+    const struct {
+        const char* what;
+        const void* p;
+    } arrays[] = {{"out_tokens", out_tokens}, {"accepted", accepted},       {"draft_probs", draft_probs},
+                  {"tokens", tokens},         {"q_start", q_start},         {"temperature", temperature},
+                  {"u", u},                   {"kv_len", kv_len},           {"kept", kept},
+                  {"err", err},               {"the workspace", workspace}, {"target", target}};
+    for (int i = 0; i < 10; ++i)
+        INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(arrays[i].p) % 4 == 0, "%s: misaligned %s", op, arrays[i].what);
+    for (const auto& x : arrays)
+        if (int s = check_device_pointer(op, x.what, x.p)) return s;
+    VerifyArgs a;
+    a.target = target;
+    a.draft = draft_probs;
+    a.ld = ld;
+    a.draft_ld = draft_ld;
+    a.tokens = tokens;
+    a.q_start = q_start;
+    a.temperature = temperature;
+    a.u = u;
+    a.kv_len = kv_len;
+    a.kept = kept;
+    a.out = out_tokens;
+    a.accepted = accepted;
+    a.parts = static_cast<RowPart*>(workspace);
+    a.num_seqs = num_seqs;
+    a.num_rows = num_rows;
+    a.V = vocab_size;
+    a.err = err;
+    // parts of whole tiles; a row's first vector may start up to 7 elements before it
+    const long long tiles = ((long long)vocab_size + 7 + kStatTile - 1) / kStatTile;
+    a.part = (int)((tiles + kMostParts - 1) / kMostParts) * kStatTile;
+    a.n_parts = (int)(((long long)vocab_size + 7 + a.part - 1) / a.part);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool p = probabilities != 0;
+    if (target_dtype == INFERNT_DTYPE_F32) return p ? launch<float, true>(a, st) : launch<float, false>(a, st);
+    if (target_dtype == INFERNT_DTYPE_BF16)
+        return p ? launch<__nv_bfloat16, true>(a, st) : launch<__nv_bfloat16, false>(a, st);
+    return p ? launch<__half, true>(a, st) : launch<__half, false>(a, st);
+}
