@@ -8,8 +8,8 @@
 //   - keys are the M of the MMA, the query rows its N = 8: S^T = K Q^T and
 //     O^T = V^T P^T.  The 16 rows of an m16n8k16 are all of use, where query
 //     rows as M leave 12 of 16 empty for a group of four heads.
-//   - codes go from shared memory to the A operand by a shift, a logic
-//     operation and an exact subtraction for two of them: the operand is the
+//   - codes go from shared memory to the A operand by a logic operation and an
+//     exact fp16 one for two of them, and a shift for eight: the operand is the
 //     whole numbers c - z, the scale s of a key multiplies its scores (K) or
 //     its probabilities (V), four values a thread for 16 keys.
 //   - the contraction's order is free: a thread takes 32 neighbouring
@@ -28,50 +28,54 @@
 namespace infernt {
 namespace {
 
-constexpr int kKeys = 128;     // keys of a tile: 16 a warp
-constexpr int kWarps = 8;      // that consume
-constexpr int kConsumers = 32 * kWarps;
-constexpr int kThreads = kConsumers + 32;
+constexpr int kWarps = 4;
+constexpr int kGroups = 2;  // of 16 keys, of a tile, a warp
+constexpr int kWarpKeys = 16 * kGroups;
+constexpr int kKeys = kWarps * kWarpKeys;  // of a tile
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStages = 3;     // tiles of a warp's ring: one is worked on, two are on their way
 constexpr int kMostRows = 64;  // query rows of a KV head from which on the tcgen05 kernel is faster
-constexpr int kBulkPage = 16;  // pages from which on a page's rows are one bulk copy
 
-// A weight 2^(s - m) s_V enters the products in 16 bits.  m follows s + log2
-// s_V, so weights stay below 2^(kRescale + 1 + kUp) whatever V's scales are;
-// fp16 has its normal numbers down to 2^-18 of a row's largest.
-template <typename T>
-constexpr float kUp = Half16<T>::kBf16 ? 0.0f : 4.0f;
-// Scales below it (vectors of zeros have the least) do not lower m further:
-// the sum of 2^(s - m) stays in FP32.
-constexpr float kLeastLog = -40.0f;
+// The products are in fp16 whatever the cache's type is, since codes get there
+// with one shift for eight of them (bf16, with seven bits behind its leading
+// one, takes three): Q enters times a power of two that brings the largest
+// element of the item's rows to 2^14 (what is lost of an element is 2^-38 of
+// that one, and so of the item's largest scores),
+// and a weight is 2^(s - m) s_V.  m follows s + log2 s_V, so weights fit
+// whatever V's scales are: m moves when a key's weights would pass kMostWeight
+// and puts a row's largest at 2^kUp to 2^(kUp + 1).  Normal numbers then reach
+// down to 2^-18 of it.
+constexpr float kUp = 4.0f;
+constexpr float kMostWeight = 16384.0f;
+// Scales below it (vectors of zeros have the least) do not lower m further, and
+// m moves too where a 2^(s - m) passes 2^80: their sum stays in FP32.
+constexpr float kLeastLog = -40.0f, kMostSingle = 1.2089258196146292e24f;
 
-// Shared memory: the ring, per stage K codes, V codes and scale words; then
-// what the warps know of an item's rows, a set a warp.
+// Shared memory: a ring of its own for each warp, per stage the codes of its K
+// and V rows and their scale words.  When a part is done the ring is empty, and
+// what the warp knows of the item's rows (its set) lies over it.
 template <int D, int RB>
 struct Layout {
     static constexpr int kRows = 8 * RB;
-    static constexpr uint32_t kCodes = kKeys * D / 2;
-    static constexpr uint32_t kStage = 2 * kCodes + kKeys * 4;
-    static constexpr int kPerSm = RB == 1 ? 2 : 1;  // CTAs of an SM
+    static constexpr uint32_t kCodes = kWarpKeys * D / 2;
+    static constexpr uint32_t kStage = 2 * kCodes + kWarpKeys * 4;
     static constexpr uint32_t kSet = kRows * (D + 2) * 4;
+    static constexpr uint32_t kRing = kStages * kStage > kSet ? kStages * kStage : (kSet + 127) / 128 * 128;
+    // CTAs of an SM: what its registers hold (128, 168 or 255 a thread)
+    static constexpr int kPerSm = RB * D <= 128 ? 4 : RB * D < 256 ? 3 : 2;
     // Q as the B operands of one n-tile stay in registers; of several, in shared memory
     static constexpr bool kSharedQ = RB > 1;
-    static constexpr uint32_t kQ = kSharedQ ? RB * (D / 32) * 512 : 0;
-    static constexpr uint32_t kRoom = 227 * 1024 / kPerSm - 3 * 1024;
-    static constexpr int kFit = (int)((kRoom - kWarps * kSet - kQ) / kStage);
-    static constexpr int kStages = kFit < 8 ? kFit : 8;
-    static constexpr uint32_t kScratch = kStages * kStage;
-    static constexpr uint32_t kQAt = kScratch + kWarps * kSet;
+    static constexpr uint32_t kQ = kSharedQ ? RB * (D / 32) * 512 + 32 : 0;  // and the warps' largest
+    static constexpr uint32_t kQAt = kWarps * kRing;
     static constexpr uint32_t kBytes = kQAt + kQ + 128;
-    static_assert(kStages >= 3, "");
-};
-
-template <int ST>
-struct Ring {
-    uint64_t full[ST], empty[ST];
+    static_assert(kPerSm * (kBytes + 2048) <= 228 * 1024, "");
 };
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t src_bytes) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async16_always(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint2 ld_shared2(uint32_t at) {
     uint2 w;
@@ -83,115 +87,97 @@ __device__ __forceinline__ uint32_t ld_shared1(uint32_t at) {
     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
     return w;
 }
+// The largest, NaN where one of them is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 
-template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
-    if (Half16<T>::kBf16)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The producer warp.  Of each tile the codes of the pages that some row sees
-// (what lies in rows that none sees is a number whatever it is), and the scale
-// words, 0 for keys that no row sees or whose page the pool does not have.
-template <int D, int RB>
-__device__ __forceinline__ void produce(const AttnArgs& a, const Place& place, uint32_t base,
-                                        Ring<Layout<D, RB>::kStages>& ring, bool& ok) {
-    using L = Layout<D, RB>;
-    constexpr int ST = L::kStages, PER = kKeys / 32;
-    constexpr uint32_t ROW = D / 2;
-    const int lane = threadIdx.x & 31, ps = a.b.page_size;
-    const char* kc = static_cast<const char*>(a.k);
-    const char* vc = static_cast<const char*>(a.v);
-    uint32_t st = 0, turn = 1;  // the first round's stages are free
-    walk<L::kRows, kKeys>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
-        const int* table = a.b.table + (size_t)part.s * a.b.table_stride;
-        // pool rows of keys lane, lane + 32, ... of tile j; -1: no row sees the key, or the pool does not have it
-        auto look = [&](int j, int (&rows)[PER]) {
-            const int k0 = tile_key<kKeys>(it, j);
+// What codes become whole numbers with.  A nibble in the low bits of a half
+// under the exponent of 2^10 is 1024 + c, one four bits up under that of 2^6
+// 64 + c.  The masks come out of a register that the compiler cannot see through: as
+// immediates they take two logic operations for each pair, and those are the
+// unit that this kernel has least of.
+struct Masks {
+    uint32_t low, high, low_one, high_one;
+};
+__device__ __forceinline__ Masks make_masks() {
+    Masks k;
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(k.low));
+    asm volatile("mov.b32 %0, 0x00f000f0;" : "=r"(k.high));
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(k.low_one));
+    asm volatile("mov.b32 %0, 0x54005400;" : "=r"(k.high_one));
+    return k;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
+    return r;
+}
+__device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// A pair of zeros as what is taken off: 1024 + z and 64 + z.
+struct Zeros {
+    uint32_t low, high;
+};
+__device__ __forceinline__ Zeros make_zeros(uint32_t pair, const Masks& k) {
+    Zeros z;
+    z.low = and_or(pair, k.low, k.low_one);
+    z.high = half2_sub(z.low, 0x63806380u);  // 960
+    return z;
+}
+// The pairs of nibbles (j, j + 4) of w as c - z.
+__device__ __forceinline__ void whole(uint32_t w, const Zeros& z, const Masks& k, uint32_t (&p)[4]) {
+    const uint32_t v = w >> 8;
+    p[0] = half2_sub(and_or(w, k.low, k.low_one), z.low);
+    p[1] = half2_sub(and_or(w, k.high, k.high_one), z.high);
+    p[2] = half2_sub(and_or(v, k.low, k.low_one), z.low);
+    p[3] = half2_sub(and_or(v, k.high, k.high_one), z.high);
+}
+
+// The copies of a tile's keys of this warp, the pool row of key `lane` in row
+// (-1: no row of the item sees it, or the pool does not have its page): codes
+// (not of such keys: what lies there are numbers whatever it is, and copies of
+// one row for all of them would meet in one place of L2), and scale words, 0
+// for such keys.  Every warp fetches for itself, two tiles ahead, so none waits
+// for another; the table's entry of a key is looked up three tiles ahead.  (16
+// sequences of 32768 positions took 141 us with a warp that streamed for the
+// others, which spends a fifth of the issue slots on its loops over pages, and
+// 141 with three bulk copies a warp and tile.)
+template <int D>
+__device__ __forceinline__ void fetch(const AttnArgs& a, int row, int lane, uint32_t stage) {
+    constexpr uint32_t ROW = D / 2, CODES = kWarpKeys * ROW;
+    constexpr int CH = ROW / 16, RPI = 32 / CH;  // 16-byte pieces of a row, rows at once
+    const char* kc = static_cast<const char*>(a.k) + 16 * (lane % CH);
+    const char* vc = static_cast<const char*>(a.v) + 16 * (lane % CH);
 #pragma unroll
-            for (int h = 0; h < PER; ++h) {
-                const int p = k0 + lane + 32 * h;
-                rows[h] = item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
-            }
-        };
-        int rows[PER];
-        if (part.j0 < part.j1) look(part.j0, rows);
-#pragma unroll 1
-        for (int j = part.j0; j < part.j1; ++j) {
-            const int k0 = tile_key<kKeys>(it, j);
-            const uint32_t kt = base + st * L::kStage, vt = kt + L::kCodes, sct = vt + L::kCodes;
-            // the runs of a page, a page a lane at a time
-            const int pi0 = a.b.by_page(k0), pages = ps >= kBulkPage ? a.b.by_page(k0 + kKeys - 1) - pi0 + 1 : 0;
-            int from = 0, count = 0, at = 0;
-            if (lane < pages) {  // (at most 128 / 16 + 1)
-                const int pi = pi0 + lane, p0 = max(k0, pi * ps);
-                // up to the end of the page, the tile or the last key; (pi + 1) ps may pass 2^31 behind it
-                const int p1 = min(min(k0 + kKeys, it.hi), p0 + (ps - (p0 - pi * ps)));
-                if (p0 < p1 && (p1 > it.lo || p0 < it.sink_end)) {
-                    const int page = table[pi];
-                    if (page >= 0 && page < a.b.num_pages) {
-                        from = (page * a.b.nkv + it.kvh) * ps + (p0 - pi * ps);
-                        count = p1 - p0;
-                        at = p0 - k0;
-                    }
-                }
-            }
-            const unsigned bytes = __reduce_add_sync(0xffffffffu, (unsigned)count) * 2 * ROW;
-            int next[PER];
-            if (j + 1 < part.j1) look(j + 1, next);
-            tc_wait_bar(&ring.empty[st], turn, ok);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
-            if (lane == 0) mbar_arrive_expect_tx(&ring.full[st], bytes);
-            __syncwarp();
-            if (count > 0) {
-                bulk_g2s_plain_at(kt + at * ROW, kc + (size_t)from * ROW, count * ROW, &ring.full[st]);
-                bulk_g2s_plain_at(vt + at * ROW, vc + (size_t)from * ROW, count * ROW, &ring.full[st]);
-            }
-            if (ps < kBulkPage) {
-                constexpr int CH = ROW / 16, RPI = 32 / CH;  // chunks of a row, rows at once
-#pragma unroll
-                for (int h = 0; h < PER; ++h)
-#pragma unroll 4
-                    for (int i = 0; i < 32 / RPI; ++i) {
-                        const int r = i * RPI + lane / CH, ch = lane % CH;
-                        const int pr = __shfl_sync(0xffffffffu, rows[h], r);
-                        if (pr < 0) continue;
-                        const size_t off = (size_t)pr * ROW + ch * 16;
-                        cp_async16(kt + (r + 32 * h) * ROW + ch * 16, kc + off, 16u);
-                        cp_async16(vt + (r + 32 * h) * ROW + ch * 16, vc + off, 16u);
-                    }
-            }
-#pragma unroll
-            for (int h = 0; h < PER; ++h) {
-                cp_async4(sct + (lane + 32 * h) * 4, a.scales + max(rows[h], 0), rows[h] >= 0 ? 4u : 0u);
-                rows[h] = next[h];
-            }
-            // this lane's arrival, once its copies have landed
-            asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_addr(&ring.full[st])) : "memory");
-            if (++st == ST) {
-                st = 0;
-                turn ^= 1;
-            }
+    for (int i = 0; i < kWarpKeys / RPI; ++i) {
+        const int r = __shfl_sync(0xffffffffu, row, i * RPI + lane / CH);
+        const uint32_t at = stage + (i * RPI) * ROW + lane * 16;
+        if (r >= 0) {
+            cp_async16_always(at, kc + (size_t)r * ROW);
+            cp_async16_always(at + CODES, vc + (size_t)r * ROW);
         }
-    });
-    cp_async_wait<0>();
+    }
+    cp_async4(stage + 2 * CODES + 4 * lane, a.scales + max(row, 0), row >= 0 ? 4u : 0u);
 }
 
 // The physical key of row r of a warp's 16: neighbouring rows, and every
@@ -208,65 +194,140 @@ struct RowState {
     float acc[RB][D / 16][4];
 };
 
-// The tiles [j0, j1) of an item, 16 keys of each by every warp.
-template <typename T, int D, int RB>
-__device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, const Item& it, const Part& part,
-                                        uint32_t base, Ring<Layout<D, RB>::kStages>& ring, uint32_t& st, uint32_t& turn,
-                                        RowState<D, RB>& s, bool& ok) {
-    using L = Layout<D, RB>;
-    constexpr int KC = D / 16, ST = L::kStages, W = D / 32;  // MMA steps of a score; words of a thread's K row
-    constexpr uint32_t ROW = D / 2;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tig = lane & 3;
-    // Q of row 8 n + g, elements tig D / 4 + 8 w ... as pairs in the order of Codes4
-    auto q_of = [&](int n, int w) {
-        const int row = it.row0 + min(8 * n + g, it.rows - 1), token = a.by_g(row);
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                                             (long long)(seq.row0 + token) * a.ldq +
-                                                             (it.kvh * a.G + row - token * a.G) * D + tig * (D / 4)) + w);
-        // (0, 1) (2, 3) (4, 5) (6, 7) -> (0, 4) (1, 5) (2, 6) (3, 7)
-        return make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410),
-                          __byte_perm(x.y, x.w, 0x7632));
-    };
-    uint4 qb[L::kSharedQ ? 1 : W];
-    const uint32_t q_at = base + L::kQAt + lane * 16;
-    if (L::kSharedQ) {
-        for (int x = warp; x < RB * W; x += kWarps) st_shared(q_at + x * 512, q_of(x / W, x % W));
-        named_sync(1, kConsumers);
-    } else {
+// Eight elements of a row of T, times f, as fp16 pairs (0, 4) (1, 5) (2, 6) (3, 7).
+template <typename T>
+__device__ __forceinline__ uint4 eight_of(uint4 x, float f) {
+    float2 v[4] = {Half16<T>::unpack(x.x), Half16<T>::unpack(x.y), Half16<T>::unpack(x.z), Half16<T>::unpack(x.w)};
+    return make_uint4(Half16<__half>::pack(v[0].x * f, v[2].x * f), Half16<__half>::pack(v[0].y * f, v[2].y * f),
+                      Half16<__half>::pack(v[1].x * f, v[3].x * f), Half16<__half>::pack(v[1].y * f, v[3].y * f));
+}
+
+// Q of n-tile n as its B operand will have it: word w has the elements tig D /
+// 4 + 8 w ... of row 8 n + g.
+template <int D>
+__device__ __forceinline__ void load_q(const AttnArgs& a, const PagedSeq& seq, const Item& it, int n, int lane,
+                                       uint4 (&q)[D / 32]) {
+    const int g = lane >> 2, tig = lane & 3;
+    const int row = it.row0 + min(8 * n + g, it.rows - 1), token = a.by_g(row);
+    const uint4* at = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                     (long long)(seq.row0 + token) * a.ldq +
+                                                     (it.kvh * a.G + row - token * a.G) * D + tig * (D / 4));
 #pragma unroll
-        for (int w = 0; w < W; ++w) qb[L::kSharedQ ? 0 : w] = q_of(0, w);
+    for (int w = 0; w < D / 32; ++w) q[w] = __ldg(at + w);
+}
+// The largest finite magnitude of these, over the warp, as the bits of a float.
+template <typename T, int W>
+__device__ __forceinline__ uint32_t largest_of(const uint4 (&q)[W]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+        for (const uint32_t x : {q[w].x, q[w].y, q[w].z, q[w].w}) {
+            const float2 v = Half16<T>::unpack(x);
+            const uint32_t b0 = __float_as_uint(v.x) & 0x7fffffffu, b1 = __float_as_uint(v.y) & 0x7fffffffu;
+            top = max(top, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
+        }
+    return __reduce_max_sync(0xffffffffu, top);
+}
+// The power of two that brings it to 2^14 (within what both it and its inverse can be).
+__device__ __forceinline__ int shift_of(uint32_t top) { return min(max(14 - ((int)(top >> 23) - 127), -100), 100); }
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
+
+// The tiles [j0, j1) of an item, 32 keys of each by every warp.
+template <typename T, int D, int RB>
+__device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, const Item& it, const Part& part, int warp,
+                                        int lane, uint32_t base, RowState<D, RB>& s) {
+    using L = Layout<D, RB>;
+    constexpr int KC = D / 16, W = D / 32;  // MMA steps of a score; words of a thread's K row
+    constexpr uint32_t ROW = D / 2;
+    const int g = lane >> 2, tig = lane & 3;
+    const uint32_t ring = base + warp * L::kRing;
+    // the pool row of key `lane` of this warp in tile j
+    auto look = [&](int j) {
+        const int p = tile_key<kKeys>(it, j) + warp * kWarpKeys + lane;
+        return j < part.j1 && item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        fetch<D>(a, look(part.j0 + i), lane, ring + i * L::kStage);
+        cp_async_commit();
     }
-    int pos[RB][2];
+    int ahead = look(part.j0 + kStages - 1);
+    const Masks mk = make_masks();
+    uint4 qb[W];
+    int shift;
+    const uint32_t q_at = base + L::kQAt + lane * 16, top_at = base + L::kQAt + RB * W * 512;
+    if (L::kSharedQ) {
+        uint32_t top = 0;
+        for (int n = warp; n < RB; n += kWarps) {
+            load_q<D>(a, seq, it, n, lane, qb);
+            top = max(top, largest_of<T, W>(qb));
+        }
+        if (lane == 0) asm volatile("st.shared.b32 [%0], %1;" ::"r"(top_at + 4 * warp), "r"(top) : "memory");
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = max(top, ld_shared1(top_at + 4 * w));
+        shift = shift_of(top);
+        for (int n = warp; n < RB; n += kWarps) {
+            load_q<D>(a, seq, it, n, lane, qb);
+#pragma unroll
+            for (int w = 0; w < W; ++w) st_shared(q_at + (n * W + w) * 512, eight_of<T>(qb[w], power_of_two(shift)));
+        }
+        __syncthreads();
+    } else {
+        load_q<D>(a, seq, it, 0, lane, qb);
+        shift = shift_of(largest_of<T, W>(qb));
+#pragma unroll
+        for (int w = 0; w < W; ++w) qb[w] = eight_of<T>(qb[w], power_of_two(shift));
+    }
+    const float back = a.scale_log2 * power_of_two(-shift);
+    // rows 8 n + 2 tig + e that have an m (bit 2 n + e), and those that need one
+    unsigned set = 0, need = 0;
 #pragma unroll
     for (int n = 0; n < RB; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const int r = 8 * n + 2 * tig + e;
-            pos[n][e] = r < it.rows ? row_pos(seq, a.by_g(it.row0 + r)) : -1;
-            s.m[n][e] = -INFINITY;
+            s.m[n][e] = 0.0f;
             s.l[n][e] = 0.0f;
+            if (8 * n + 2 * tig + e < it.rows) need |= 1u << (2 * n + e);
         }
 #pragma unroll
         for (int b = 0; b < KC; ++b) s.acc[n][b][0] = s.acc[n][b][1] = s.acc[n][b][2] = s.acc[n][b][3] = 0.0f;
     }
-    const uint32_t k_at = (uint32_t)(warp * 16) * ROW;
+    bool unset = true;
+    // tiles of which every row sees all keys of this warp: not among the first ones that stay visible, not before the
+    // last row's window, not past the first row
+    const int first_key = (it.lo_tile - it.sink_tiles) * kKeys + warp * kWarpKeys;  // of tile 0, behind those
+    const int whole_lo = max(it.sink_tiles, a.window > 0 ? (max(it.pos_last - a.window + 1 - first_key, 0) + kKeys - 1) / kKeys : 0);
+    const int whole_hi = it.pos_first + 1 - kWarpKeys >= first_key ? (it.pos_first + 1 - kWarpKeys - first_key) / kKeys + 1 : 0;
+    const unsigned whole_n = (unsigned)max(whole_hi - whole_lo, 0);
+    // K rows g and g + 8 of a group of keys, the V rows of the contraction's order, their scale words
+    const int kg = key_of(g), kt0 = key_of(2 * tig), kt1 = key_of(2 * tig + 1);  // (of r + 8: 8 more)
+    const uint32_t k_at = kg * ROW + tig * (D / 8);
+    const uint32_t v_at0 = (uint32_t)L::kCodes + kt0 * ROW + g * (D / 16), v_at1 = v_at0 + (kt1 - kt0) * ROW;
+    const uint32_t s_at = 2 * L::kCodes;
+    uint32_t now = 0;  // the stage of tile j
 #pragma unroll 1
     for (int j = part.j0; j < part.j1; ++j) {
-        const int k0 = tile_key<kKeys>(it, j) + warp * 16;
-        const uint32_t kt = base + st * L::kStage + k_at, vt = kt + L::kCodes;
-        const uint32_t sct = base + st * L::kStage + 2 * L::kCodes + warp * 64;
-        tc_wait_bar(&ring.full[st], turn, ok);
+        fetch<D>(a, ahead, lane, ring + (now == 0 ? kStages - 1 : now - 1) * L::kStage);
+        cp_async_commit();
+        ahead = look(j + kStages);
+        cp_async_wait<kStages - 1>();
+        __syncwarp();
+        const uint32_t stage = ring + now * L::kStage;
+        const bool whole_tile = (unsigned)(j - whole_lo) < whole_n;
+        const int k0 = tile_key<kKeys>(it, j) + warp * kWarpKeys;
         // keys of this warp that some row sees
-        if (k0 < it.hi && (k0 + 15 >= it.lo || k0 < it.sink_end)) {
-            const uint32_t word[2] = {ld_shared1(sct + 4 * key_of(g)), ld_shared1(sct + 4 * key_of(g + 8))};
-            float sc[RB][4];
+        if (whole_tile || (k0 < it.hi && (k0 + kWarpKeys > it.lo || k0 < it.sink_end))) {
+            // what is lane's of group i is key 16 i + kg + 8 h
+            uint32_t word[kGroups][2];
+            float sc[kGroups][RB][4];
 #pragma unroll
-            for (int n = 0; n < RB; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
-            {
+            for (int i = 0; i < kGroups; ++i) {
                 uint32_t ka[2][4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t at = kt + key_of(g + 8 * h) * ROW + tig * (D / 8);
+                    word[i][h] = ld_shared1(stage + s_at + 4 * (16 * i + 8 * h) + 4 * kg);
+                    const uint32_t at = stage + k_at + (16 * i + 8 * h) * ROW;
                     if (D == 128) {
                         const uint4 x = ld_shared(at);
                         ka[h][0] = x.x;
@@ -279,148 +340,202 @@ __device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, 
                         ka[h][1] = x.y;
                     }
                 }
-                const uint32_t z0 = Codes4<T>::zeros(word[0] & 15u), z1 = Codes4<T>::zeros(word[1] & 15u);
+                const Zeros z0 = make_zeros(__byte_perm(word[i][0], word[i][0], 0x1010), mk);
+                const Zeros z1 = make_zeros(__byte_perm(word[i][1], word[i][1], 0x1010), mk);
+#pragma unroll
+                for (int n = 0; n < RB; ++n) sc[i][n][0] = sc[i][n][1] = sc[i][n][2] = sc[i][n][3] = 0.0f;
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     uint32_t x[4], y[4];
-                    whole4<T>(ka[0][w], z0, x);
-                    whole4<T>(ka[1][w], z1, y);
+                    whole(ka[0][w], z0, mk, x);
+                    whole(ka[1][w], z1, mk, y);
 #pragma unroll
                     for (int n = 0; n < RB; ++n)
                         if (RB == 1 || 8 * n < it.rows) {
-                            const uint4 q = L::kSharedQ ? ld_shared(q_at + (n * W + w) * 512) : qb[L::kSharedQ ? 0 : w];
-                            mma<T>(sc[n], x[0], y[0], x[1], y[1], q.x, q.y);
-                            mma<T>(sc[n], x[2], y[2], x[3], y[3], q.z, q.w);
+                            const uint4 q = L::kSharedQ ? ld_shared(q_at + (n * W + w) * 512) : qb[w];
+                            mma(sc[i][n], x[0], y[0], x[1], y[1], q.x, q.y);
+                            mma(sc[i][n], x[2], y[2], x[3], y[3], q.z, q.w);
                         }
                 }
             }
-            // scores, weights; key h is key_of(g + 8 h)
-            const bool whole = seen_whole<16>(a, it, k0);
-            float ks[2], vs[2], vl[2];
-            bool none[2];  // a V vector of NaN
+            // a score in base 2 is sc f
+            float f[kGroups][2], vs[kGroups][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                ks[h] = scale4(word[h]) * a.scale_log2;
-                const uint32_t v = word[h] >> 16;
-                none[h] = (v & 0x7f80u) == 0x7f80u;
-                vs[h] = none[h] ? 0.0f : scale4(v);
-                vl[h] = fmaxf((float)(int)((v >> 7) & 255u) - 127.0f, kLeastLog) - kUp<T>;
-                if (none[h]) vl[h] = -kUp<T>;
-            }
-            uint32_t pb[RB][2];
-            bool grow = false;
-            float mx[RB][2];
+            for (int i = 0; i < kGroups; ++i)
 #pragma unroll
-            for (int n = 0; n < RB; ++n)
+                for (int h = 0; h < 2; ++h) {
+                    f[i][h] = back * scale4(word[i][h]);
+                    vs[i][h] = __uint_as_float(word[i][h] & 0xfff00000u);
+                }
+            if (!whole_tile) {
+                bool none[kGroups][2];  // a K vector of NaN: of the rows that see it alone
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int i = 0; i < kGroups; ++i)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float& x = sc[n][2 * h + e];
-                        x *= ks[h];
-                        if (!whole && !row_sees(a, pos[n][e], k0 + key_of(g + 8 * h))) x = -INFINITY;
+                        none[i][h] = !(f[i][h] < INFINITY);
+                        f[i][h] = none[i][h] ? 1.0f : fmaxf(f[i][h], 1e-37f);  // -infinity times it is -infinity
                     }
-                    mx[n][e] = fmaxf(sc[n][e] + vl[0], sc[n][2 + e] + vl[1]);
-                    grow |= mx[n][e] > s.m[n][e] + kRescale;
-                }
-            // m moves only when weights would pass 2^(kRescale + kUp)
-            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int n = 0; n < RB; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
+                        const int r = 8 * n + 2 * tig + e, pos = r < it.rows ? row_pos(seq, a.by_g(it.row0 + r)) : -1;
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1)
-                            mx[n][e] = fmaxf(mx[n][e], __shfl_xor_sync(0xffffffffu, mx[n][e], o));
-                        const float top = fmaxf(s.m[n][e], mx[n][e]);
-                        const float f = s.m[n][e] == -INFINITY ? 0.0f : ex2(s.m[n][e] - top);
-                        s.m[n][e] = top;
-                        s.l[n][e] *= f;
+                        for (int i = 0; i < kGroups; ++i)
 #pragma unroll
-                        for (int b = 0; b < KC; ++b) {
-                            s.acc[n][b][e] *= f;
-                            s.acc[n][b][2 + e] *= f;
-                        }
+                            for (int h = 0; h < 2; ++h)
+                            {
+                                float& x = sc[i][n][2 * h + e];
+                                if (none[i][h]) x = __int_as_float(0x7fffffff);
+                                if (!row_sees(a, pos, k0 + 16 * i + 8 * h + kg)) x = -INFINITY;
+                            }
                     }
             }
-            // rows that see a V vector of NaN have no result
-            if (__any_sync(0xffffffffu, none[0] || none[1])) {
+            // weights under the m of the keys before; where a row's do not fit (and for its first keys), its m
+            // moves and they are computed again.  A row's m depends on its own weights alone.
+            float p[kGroups][RB][4], w[kGroups][RB][4];
+            auto weights = [&]() {
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+                    for (int n = 0; n < RB; ++n)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            p[i][n][x] = ex2(fmaf(sc[i][n][x], f[i][x >> 1], -s.m[n][x & 1]));
+                            w[i][n][x] = p[i][n][x] * vs[i][x >> 1];
+                        }
+            };
+            weights();
+            float most_p = 0.0f, most_w = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+                for (int n = 0; n < RB; ++n)
+#pragma unroll
+                    for (int x = 0; x < 4; x += 2) {
+                        most_p = max_nan(most_p, p[i][n][x], p[i][n][x + 1]);
+                        most_w = max_nan(most_w, w[i][n][x], w[i][n][x + 1]);
+                    }
+            if (unset || !__all_sync(0xffffffffu, most_w <= kMostWeight && most_p <= kMostSingle)) {
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        // a V vector of NaN: rows that see it have no result
+                        const bool none = !(vs[i][h] < INFINITY);
+                        if (__any_sync(0xffffffffu, none)) {
+#pragma unroll
+                            for (int n = 0; n < RB; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    bool hit = none && sc[i][n][2 * h + e] != -INFINITY;
+#pragma unroll
+                                    for (int o = 4; o < 32; o <<= 1) hit |= __shfl_xor_sync(0xffffffffu, (int)hit, o) != 0;
+                                    if (hit)
+#pragma unroll
+                                        for (int b = 0; b < KC; ++b)
+                                            s.acc[n][b][e] = s.acc[n][b][2 + e] = __int_as_float(0x7fffffff);
+                                }
+                        }
+                        if (none) vs[i][h] = 0.0f;
+                    }
 #pragma unroll
                 for (int n = 0; n < RB; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        bool hit = (none[0] && sc[n][e] != -INFINITY) || (none[1] && sc[n][2 + e] != -INFINITY);
+                        float top = -INFINITY, high_w = 0.0f, high_p = 0.0f;
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) hit |= __shfl_xor_sync(0xffffffffu, (int)hit, o) != 0;
-                        if (hit)
+                        for (int i = 0; i < kGroups; ++i)
 #pragma unroll
-                            for (int b = 0; b < KC; ++b) s.acc[n][b][e] = s.acc[n][b][2 + e] = __int_as_float(0x7fffffff);
+                            for (int h = 0; h < 2; ++h) {
+                                const float log = (float)((int)(__float_as_uint(vs[i][h]) >> 23) - 127);
+                                top = fmaxf(top, fmaf(sc[i][n][2 * h + e], f[i][h], fmaxf(log, kLeastLog) - kUp));
+                                high_w = fmaxf(high_w, w[i][n][2 * h + e]);
+                                high_p = fmaxf(high_p, p[i][n][2 * h + e]);
+                            }
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) {
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            high_w = fmaxf(high_w, __shfl_xor_sync(0xffffffffu, high_w, o));
+                            high_p = fmaxf(high_p, __shfl_xor_sync(0xffffffffu, high_p, o));
+                        }
+                        const unsigned bit = 1u << (2 * n + e);
+                        if (set & bit ? high_w > kMostWeight || high_p > kMostSingle : top != -INFINITY) {
+                            const float x = set & bit ? ex2(s.m[n][e] - top) : 0.0f;
+                            set |= bit;
+                            s.m[n][e] = top;
+                            s.l[n][e] *= x;
+#pragma unroll
+                            for (int b = 0; b < KC; ++b) {
+                                s.acc[n][b][e] *= x;
+                                s.acc[n][b][2 + e] *= x;
+                            }
+                        }
+                    }
+                unset = __any_sync(0xffffffffu, need & ~set);
+                weights();
+            }
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                uint32_t pb[RB][2];
+#pragma unroll
+                for (int n = 0; n < RB; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) s.l[n][e] += p[i][n][e] + p[i][n][2 + e];
+                    pb[n][0] = transpose8(Half16<__half>::pack(w[i][n][0], w[i][n][1]));
+                    pb[n][1] = transpose8(Half16<__half>::pack(w[i][n][2], w[i][n][3]));
+                }
+                // V^T: elements g D / 8 ... of keys 2 tig, + 1 and 2 tig + 8, + 9
+                uint32_t va[4][D / 64];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t at = stage + (x & 1 ? v_at1 : v_at0) + (16 * i + 8 * (x >> 1)) * ROW;
+                    if (D == 128) {
+                        const uint2 y = ld_shared2(at);
+                        va[x][0] = y.x;
+                        va[x][D / 64 - 1] = y.y;
+                    } else {
+                        va[x][0] = ld_shared1(at);
+                    }
+                }
+                Zeros zv[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t at = stage + s_at + 4 * (16 * i + 8 * h);
+                    zv[h] = make_zeros(__byte_perm(ld_shared1(at + 4 * kt0), ld_shared1(at + 4 * kt1), 0x7632), mk);
+                }
+#pragma unroll
+                for (int q = 0; q < D / 64; ++q)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {  // elements 8 q + 4 half ... + 3 of both keys of a pair
+                        const uint32_t sel = half ? 0x7632 : 0x5410;
+                        uint32_t x[4], y[4];
+                        whole(__byte_perm(va[0][q], va[1][q], sel), zv[0], mk, x);
+                        whole(__byte_perm(va[2][q], va[3][q], sel), zv[1], mk, y);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b)
+#pragma unroll
+                            for (int n = 0; n < RB; ++n)
+                                if (RB == 1 || 8 * n < it.rows)
+                                    mma(s.acc[n][4 * q + 2 * half + b], x[2 * b], x[2 * b + 1], y[2 * b], y[2 * b + 1],
+                                        pb[n][0], pb[n][1]);
                     }
             }
-#pragma unroll
-            for (int n = 0; n < RB; ++n) {
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float ref = s.m[n][e] == -INFINITY ? 0.0f : s.m[n][e];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float p = ex2(sc[n][2 * h + e] - ref);
-                        s.l[n][e] += p;
-                        w[2 * h + e] = p * vs[h];
-                    }
-                }
-                pb[n][0] = transpose8(Half16<T>::pack(w[0], w[1]));
-                pb[n][1] = transpose8(Half16<T>::pack(w[2], w[3]));
-            }
-            // V^T: elements g D / 8 ... of keys 2 tig, + 1 and 2 tig + 8, + 9
-            uint32_t zv[2], va[4][D / 64];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int key = key_of(2 * tig + (i & 1) + 8 * (i >> 1));
-                const uint32_t at = vt + key * ROW + g * (D / 16);
-                if (D == 128) {
-                    const uint2 x = ld_shared2(at);
-                    va[i][0] = x.x;
-                    va[i][D / 64 - 1] = x.y;
-                } else {
-                    va[i][0] = ld_shared1(at);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                zv[h] = Codes4<T>::zeros((ld_shared1(sct + 4 * key_of(2 * tig + 8 * h)) >> 16) & 15u,
-                                         (ld_shared1(sct + 4 * key_of(2 * tig + 1 + 8 * h)) >> 16) & 15u);
-#pragma unroll
-            for (int q = 0; q < D / 64; ++q)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {  // elements 8 q + 4 half ... + 3 of both keys of a pair
-                    const uint32_t sel = half ? 0x7632 : 0x5410;
-                    uint32_t x[4], y[4];
-                    whole4<T>(__byte_perm(va[0][q], va[1][q], sel), zv[0], x);
-                    whole4<T>(__byte_perm(va[2][q], va[3][q], sel), zv[1], y);
-#pragma unroll
-                    for (int b = 0; b < 2; ++b)
-#pragma unroll
-                        for (int n = 0; n < RB; ++n)
-                            if (RB == 1 || 8 * n < it.rows)
-                                mma<T>(s.acc[n][4 * q + 2 * half + b], x[2 * b], x[2 * b + 1], y[2 * b], y[2 * b + 1],
-                                       pb[n][0], pb[n][1]);
-                }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ring.empty[st]);
-        if (++st == ST) {
-            st = 0;
-            turn ^= 1;
-        }
+        __syncwarp();  // the stage is read
+        now = now + 1 == kStages ? 0 : now + 1;
     }
+    cp_async_wait<0>();
 #pragma unroll
     for (int n = 0; n < RB; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) s.l[n][e] += __shfl_xor_sync(0xffffffffu, s.l[n][e], o);
+#pragma unroll
+    for (int x = 0; x < 2 * RB; ++x)
+        if (!(set >> x & 1u)) s.m[x / 2][x & 1] = -INFINITY;
 }
 
 // Element 4 i of the stretch g of a row's D in a set: neighbours g for the
@@ -430,126 +545,152 @@ __device__ __forceinline__ int set_at(int row, int i, int g) {
     return row * D + i * 32 + g * 4;
 }
 
+// A split item's result from its CTAs' slots, in order, by the last of them to
+// arrive.
+template <typename T, int D, int M>
+__device__ __forceinline__ void join_item(const AttnArgs& a, const PagedSeq& seq, const Item& it, const Part& p, int tid) {
+    // four elements of a row a thread, four CTAs' at once
+    for (int x = tid; x < it.rows * (D / 4); x += kThreads) {
+        const int r = x / (D / 4), d = 4 * (x % (D / 4));
+        float top = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int b = p.first; b <= p.last; b += 4) {
+            float mb[4], lb[4], up = top;
+            float4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* at = slot_of<M, D>(a, min(b + i, p.last), p.first);
+                mb[i] = __ldcg(at + M * D + r);
+                lb[i] = __ldcg(at + M * D + M + r);
+                v[i] = __ldcg(reinterpret_cast<const float4*>(at + r * D + d));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (b + i > p.last) mb[i] = -INFINITY;
+                up = fmaxf(up, mb[i]);
+            }
+            const float f = top == -INFINITY ? 0.0f : ex2(top - up);
+            top = up;
+            l *= f;
+            o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (mb[i] == -INFINITY) continue;
+                const float w = ex2(mb[i] - top);
+                l = fmaf(lb[i], w, l);
+                o.x = fmaf(v[i].x, w, o.x);
+                o.y = fmaf(v[i].y, w, o.y);
+                o.z = fmaf(v[i].z, w, o.z);
+                o.w = fmaf(v[i].w, w, o.w);
+            }
+        }
+        write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, {top, l, o.x, o.y});
+        write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d + 2, {top, l, o.z, o.w});
+    }
+}
+
 template <typename T, int D, int RB>
 __global__ void __launch_bounds__(kThreads, (Layout<D, RB>::kPerSm)) paged4_attn(const __grid_constant__ AttnArgs a) {
     using L = Layout<D, RB>;
-    constexpr int M = L::kRows, ST = L::kStages;
+    constexpr int M = L::kRows;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ Ring<ST> ring;
     __shared__ int last_s;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
+    // out of a register that the compiler cannot see through: it would read the thread's number again and again
+    int tid;
+    asm volatile("mov.u32 %0, %%tid.x;" : "=r"(tid));
+    const int warp = tid >> 5, lane = tid & 31, g = lane >> 2, tig = lane & 3;
     const uint32_t base = (smem_addr(smem) + 127u) & ~127u;
-    float* scratch = reinterpret_cast<float*>(smem + (base - smem_addr(smem)) + L::kScratch);
-    if (tid == 0) {
-        for (int i = 0; i < ST; ++i) {
-            mbar_init(&ring.full[i], 33);
-            mbar_init(&ring.empty[i], kWarps);
-        }
-        mbar_fence_init();
-    }
-    const Place place = find_place<M, kKeys, kThreads>(a);  // its barriers publish the set-up
+    const float* sets = reinterpret_cast<const float*>(smem + (base - smem_addr(smem)));
+    const Place place = find_place<M, kKeys, kThreads>(a);
     pdl_launch_dependents();  // the tcgen05 kernel may take SMs as they become free
     if (place.s < 0) return;
-    bool ok = true;
-    if (warp == kWarps) {
-        produce<D, RB>(a, place, base, ring, ok);
-    } else {
-        uint32_t st = 0, turn = 0;
-        walk<M, kKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
-            {
-                RowState<D, RB> s;
-                consume<T, D, RB>(a, seq, it, p, base, ring, st, turn, s, ok);
-                float* set = scratch + warp * (L::kSet / 4);
+    walk<M, kKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
+        {
+            RowState<D, RB> s;
+            consume<T, D, RB>(a, seq, it, p, warp, lane, base, s);
+            float* set = const_cast<float*>(sets) + warp * (L::kRing / 4);
 #pragma unroll
-                for (int n = 0; n < RB; ++n)
+            for (int n = 0; n < RB; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int r = 8 * n + 2 * tig + e;
-                        if (r >= it.rows) continue;
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * n + 2 * tig + e;
+                    if (r >= it.rows) continue;
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i)
-                            *reinterpret_cast<float4*>(set + set_at<D>(r, i, g)) =
-                                make_float4(s.acc[n][2 * i][e], s.acc[n][2 * i][2 + e], s.acc[n][2 * i + 1][e],
-                                            s.acc[n][2 * i + 1][2 + e]);
-                        if (g == 0) {
-                            set[M * D + r] = s.m[n][e];
-                            set[M * D + M + r] = s.l[n][e];
-                        }
+                    for (int i = 0; i < D / 32; ++i)
+                        *reinterpret_cast<float4*>(set + set_at<D>(r, i, g)) =
+                            make_float4(s.acc[n][2 * i][e], s.acc[n][2 * i][2 + e], s.acc[n][2 * i + 1][e],
+                                        s.acc[n][2 * i + 1][2 + e]);
+                    if (g == 0) {
+                        set[M * D + r] = s.m[n][e];
+                        set[M * D + M + r] = s.l[n][e];
                     }
-            }
-            named_sync(1, kConsumers);
-            // the warps' results, joined in order: four elements of a row a thread
-            const bool split = p.first != p.last;
-            float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
-            for (int x = tid; x < it.rows * (D / 4); x += kConsumers) {
-                const int r = x / (D / 4), i = x / 8 % (D / 32), gg = x % 8, d = gg * (D / 8) + 4 * i;
-                float m[kWarps], top = -INFINITY, l = 0.0f;
-                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    m[w] = scratch[w * (L::kSet / 4) + M * D + r];
-                    top = fmaxf(top, m[w]);
                 }
+        }
+        __syncthreads();
+        // the warps' results, joined in order: four elements of a row a thread
+        const bool split = p.first != p.last;
+        float* slot = slot_of<M, D>(a, blockIdx.x, p.first);
+        for (int x = tid; x < it.rows * (D / 4); x += kThreads) {
+            const int r = x / (D / 4), i = x / 8 % (D / 32), gg = x % 8, d = gg * (D / 8) + 4 * i;
+            float m[kWarps], top = -INFINITY, l = 0.0f;
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float* set = scratch + w * (L::kSet / 4);
-                    const float f = m[w] == -INFINITY ? 0.0f : ex2(m[w] - top);
-                    const float4 v = *reinterpret_cast<const float4*>(set + set_at<D>(r, i, gg));
-                    l = fmaf(set[M * D + M + r], f, l);
-                    o.x = fmaf(v.x, f, o.x);
-                    o.y = fmaf(v.y, f, o.y);
-                    o.z = fmaf(v.z, f, o.z);
-                    o.w = fmaf(v.w, f, o.w);
-                }
-                if (split) {
-                    *reinterpret_cast<float4*>(slot + r * D + d) = o;
-                    if (d == 0) {
-                        slot[M * D + r] = top;
-                        slot[M * D + M + r] = l;
-                    }
-                } else {
-                    write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, {top, l, o.x, o.y});
-                    write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d + 2, {top, l, o.z, o.w});
-                }
+            for (int w = 0; w < kWarps; ++w) {
+                m[w] = sets[w * (L::kRing / 4) + M * D + r];
+                top = fmaxf(top, m[w]);
             }
-            named_sync(1, kConsumers);  // the sets are free
-            if (!split) return;
-            if (tid == 0) {
-                // the others' writes, ordered before by the barrier, become visible with this thread's fence
-                __threadfence();
-                unsigned* ticket = a.tickets + p.first;
-                last_s = atomicAdd(ticket, 1u) + 1u == (unsigned)(p.last - p.first + 1);
-                if (last_s) *ticket = 0u;  // ready for the next call
-                __threadfence();
-            }
-            named_sync(1, kConsumers);
-            if (last_s) {
-                // a warp a row, two columns a lane
-                for (int r = warp; r < it.rows; r += kWarps)
 #pragma unroll
-                    for (int d = 2 * lane; d < D; d += 64)
-                        write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, join_slots<M, D>(a, p.first, p.last, r, d));
+            for (int w = 0; w < kWarps; ++w) {
+                const float* set = sets + w * (L::kRing / 4);
+                const float f = m[w] == -INFINITY ? 0.0f : ex2(m[w] - top);
+                const float4 v = *reinterpret_cast<const float4*>(set + set_at<D>(r, i, gg));
+                l = fmaf(set[M * D + M + r], f, l);
+                o.x = fmaf(v.x, f, o.x);
+                o.y = fmaf(v.y, f, o.y);
+                o.z = fmaf(v.z, f, o.z);
+                o.w = fmaf(v.w, f, o.w);
             }
-            named_sync(1, kConsumers);  // everyone has read last_s
-        });
-    }
-    if (!ok) {
-        // a wait ran out: tell the host, and let copies in flight land
-        if (a.err) atomicOr(a.err, kErrWaitTimeout);
-        const long long t0 = clock64();
-        while (clock64() - t0 < 20000000ll) __nanosleep(1000);
-    }
+            if (split) {
+                *reinterpret_cast<float4*>(slot + r * D + d) = o;
+                if (d == 0) {
+                    slot[M * D + r] = top;
+                    slot[M * D + M + r] = l;
+                }
+            } else {
+                write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d, {top, l, o.x, o.y});
+                write_pair<T, D>(a, seq, it.kvh, it.row0 + r, d + 2, {top, l, o.z, o.w});
+            }
+        }
+        __syncthreads();  // the sets are free
+        if (!split) return;
+        if (tid == 0) {
+            // the others' writes, ordered before by the barrier, become visible with this thread's fence
+            __threadfence();
+            const unsigned sh = 16u * (p.first & 1), n = (unsigned)(p.last - p.first + 1);
+            unsigned* ticket = a.tickets + p.first / 2;
+            last_s = (atomicAdd(ticket, 1u << sh) >> sh & 0xffffu) + 1u == n;
+            if (last_s) atomicSub(ticket, n << sh);  // ready for the next call
+            __threadfence();
+        }
+        __syncthreads();
+        if (last_s) join_item<T, D, M>(a, seq, it, p, tid);
+        __syncthreads();  // everyone has read last_s
+    });
 }
+
+// CTAs of a launch at most.  Half a word of the tickets is an item's: it counts
+// to the item's CTAs.
+constexpr int kMost4Ctas = 1024;
 
 template <typename T, int D, int RB>
 int launch_rows(const AttnArgs& a, cudaStream_t st) {
     using L = Layout<D, RB>;
     static std::atomic<unsigned long long> set_on{0};
     if (int s = allow_smem(paged4_attn<T, D, RB>, (int)L::kBytes, set_on)) return s;
-    static_assert(kSlotsAt + 2 * kMaxCtas * slot_floats<L::kRows, D>() * 4 <= kTcWorkspaceAt && kMaxCtas * 4 <= kSlotsAt,
-                  "the slots must fit the workspace");
-    int ctas = sm_count() * L::kPerSm;  // as many as the SMs hold at once
-    if (ctas > kMaxCtas) ctas = kMaxCtas;
+    // as many as the SMs hold at once and the workspace has slots for
+    constexpr int room = (int)((kTcWorkspaceAt - kSlotsAt) / (2 * slot_floats<L::kRows, D>() * 4));
+    static_assert(kMost4Ctas / 2 * 4 <= kSlotsAt, "the tickets must fit the workspace");
+    const int ctas = std::min({sm_count() * L::kPerSm, room, kMost4Ctas});
     paged4_attn<T, D, RB><<<ctas, kThreads, L::kBytes, st>>>(a);
     INFERNT_CUDA_TRY(cudaGetLastError());
     return INFERNT_OK;

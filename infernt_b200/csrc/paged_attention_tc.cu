@@ -56,6 +56,7 @@
 #include "paged4.cuh"
 #include "paged_attention.cuh"
 #include "tc_mma.cuh"
+#include "warp_mma.cuh"
 
 namespace infernt {
 
@@ -83,6 +84,11 @@ struct LayoutTc {
     static constexpr uint32_t kK = 2 * kTileQ;
     static constexpr uint32_t kV = kK + kStages * kTile;
     static constexpr uint32_t kBytes = kV + kStages * kTile + 1024;
+    // Pages of 4 bits: tiles of codes and scale words behind those, of K and then of V
+    static constexpr uint32_t kCodes = kN * D / 2, kRaw = kCodes + kN * 4;
+    static constexpr int kRaws = 3;
+    static constexpr uint32_t kRawAt = kV + kStages * kTile;
+    static constexpr uint32_t kBytes4 = kRawAt + 2 * kRaws * kRaw + 1024;
 };
 
 struct Barriers {
@@ -120,16 +126,20 @@ __device__ __forceinline__ uint32_t row_chunk(uint32_t tile, int r, int c) {
     return tile + (c >> 3) * kBoxQ + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// 32 columns of a result, the chunks from c on of row r.
-template <typename T>
+// 32 columns of a result, the chunks from c on of row r.  FOUR: the columns
+// come in the order of V's tiles (put4).
+template <typename T, bool FOUR>
 __device__ __forceinline__ void put_result(uint32_t tile, int r, int c, float (&o)[32], bool sees, float inv) {
+    constexpr int at[8] = {0, FOUR ? 2 : 1, FOUR ? 4 : 2, FOUR ? 6 : 3, FOUR ? 1 : 4, FOUR ? 3 : 5, FOUR ? 5 : 6, 7};
 #pragma unroll
     for (int e = 0; e < 32; ++e) o[e] = sees ? o[e] * inv : 0.0f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 4; ++e) {
+        const float* x = o + 8 * e;
         st_shared(row_chunk(tile, r, c + e),
-                  make_uint4(Half16<T>::pack(o[8 * e], o[8 * e + 1]), Half16<T>::pack(o[8 * e + 2], o[8 * e + 3]),
-                             Half16<T>::pack(o[8 * e + 4], o[8 * e + 5]), Half16<T>::pack(o[8 * e + 6], o[8 * e + 7])));
+                  make_uint4(Half16<T>::pack(x[at[0]], x[at[1]]), Half16<T>::pack(x[at[2]], x[at[3]]),
+                             Half16<T>::pack(x[at[4]], x[at[5]]), Half16<T>::pack(x[at[6]], x[at[7]])));
+    }
 }
 
 // The values that clean_rows took out of a part's tiles, added to O of the
@@ -158,57 +168,80 @@ __device__ __noinline__ void restore_values(const AttnArgs& a, const Current& cu
 
 // ------------------------------------------------- pages of 4 bits
 // The tiles are the same, in 16 bits, but for how they get there: warp 0 makes
-// the K tiles and warp 2 the V tiles out of codes (paged4.cuh), in registers.
-// A warp has the codes of the next tile in flight while it waits for the stage
-// of that tile.  The values are numbers of T, so
-// the products are those over 16-bit pages.  A tile is some 600 issue slots of
-// a warp, on schedulers where the row warps leave half of them.
+// the K tiles and warp 2 the V tiles out of codes (paged4.cuh).  A tile's codes
+// and scale words come by cp.async, row by row, two tiles ahead of the one that
+// the warp turns into values; the table's entries are looked up three ahead.
+// The values are numbers of T, so the products are those over 16-bit pages.
+// Eight values lie in the order in which they come out of a word, (0, 4) (1, 5)
+// (2, 6) (3, 7): the row warps put Q into that order too, and take the result
+// out of it.  A tile is some 600 issue slots of each warp, on schedulers of
+// which the row warps leave half.
 
-// A lane's part of a tile: 16-byte pieces of codes, of rows i kRpi + lane / kPieces.
 template <int D>
 struct Tile4 {
-    static constexpr int kPieces = D / 32, kRpi = 32 / kPieces, kRounds = kN / kRpi;
-    int rows[2];       // pool rows of keys lane, lane + 32 (-1: zeros)
-    uint32_t word[2];  // their scale words (16 bits; 0: zeros)
-    uint4 codes[kRounds];
+    static constexpr int kPieces = D / 32;  // 16-byte pieces of a row's codes
+    static constexpr int kRpi = 32 / kPieces, kRounds = kN / kRpi;  // rows at once, rounds
 };
 
-template <int D>
-__device__ __forceinline__ void look4(const AttnArgs& a, const Item& it, const Part& part, int j, Tile4<D>& t) {
+// Pool rows of keys lane and lane + 32 of tile j (-1: no row sees the key, or
+// the pool does not have it).
+__device__ __forceinline__ void look4(const AttnArgs& a, const Item& it, const Part& part, int j, int (&rows)[2]) {
     const int lane = threadIdx.x & 31, k0 = tile_key<kN>(it, j);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int p = k0 + lane + 32 * h;
-        t.rows[h] = item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
+        rows[h] = j < part.j1 && item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
     }
 }
+// A tile's copies: zeros for rows of -1 (a scale of 0).
 template <int D, bool IS_V>
-__device__ __forceinline__ void fetch4(const AttnArgs& a, Tile4<D>& t) {
+__device__ __forceinline__ void fetch4(const AttnArgs& a, const int (&rows)[2], uint32_t raw) {
+    using X = Tile4<D>;
     const int lane = threadIdx.x & 31;
+    const char* codes = static_cast<const char*>(IS_V ? a.v : a.k) + 16 * (lane % X::kPieces);
+#pragma unroll
+    for (int i = 0; i < X::kRounds; ++i) {
+        const int r = i * X::kRpi + lane / X::kPieces;
+        const int row = __shfl_sync(0xffffffffu, rows[i * X::kRpi / 32], r & 31);
+        cp_async16(raw + r * (D / 2) + 16 * (lane % X::kPieces), codes + (size_t)max(row, 0) * (D / 2), row >= 0 ? 16u : 0u);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        t.word[h] = t.rows[h] >= 0 ? (__ldg(a.scales + t.rows[h]) >> (IS_V ? 16 : 0)) & 0xffffu : 0u;
-    const uint4* codes = static_cast<const uint4*>(IS_V ? a.v : a.k);
-#pragma unroll
-    for (int i = 0; i < Tile4<D>::kRounds; ++i) {
-        const int r = i * Tile4<D>::kRpi + lane / Tile4<D>::kPieces;
-        const int row = __shfl_sync(0xffffffffu, t.rows[r >> 5], r & 31);
-        t.codes[i] = row >= 0 ? __ldg(codes + (size_t)row * Tile4<D>::kPieces + lane % Tile4<D>::kPieces)
-                              : make_uint4(0u, 0u, 0u, 0u);
-    }
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw + kN * (D / 2) + 4 * (lane + 32 * h)),
+                     "l"(a.scales + max(rows[h], 0)), "r"(rows[h] >= 0 ? 4u : 0u)
+                     : "memory");
 }
-template <typename T, int D>
-__device__ __forceinline__ void put4(const Tile4<D>& t, uint32_t tile) {
-    const int lane = threadIdx.x & 31, c = 4 * (lane % Tile4<D>::kPieces);
+// The values of a tile of codes.  none: vectors of NaN become zeros.
+template <typename T, int D, bool IS_V>
+__device__ __forceinline__ void put4(uint32_t raw, uint32_t tile, bool none) {
+    using X = Tile4<D>;
+    const int lane = threadIdx.x & 31, piece = lane % X::kPieces;
 #pragma unroll
-    for (int i = 0; i < Tile4<D>::kRounds; ++i) {
-        const int r = i * Tile4<D>::kRpi + lane / Tile4<D>::kPieces;
-        const uint32_t word = __shfl_sync(0xffffffffu, t.word[i * Tile4<D>::kRpi / 32], r & 31);
-        const uint32_t z2 = Codes4<T>::zeros(word & 15u), s2 = scale_pair4<T>(word);
-        st_shared(chunk_at(tile, r, c), values4<T>(t.codes[i].x, z2, s2));
-        st_shared(chunk_at(tile, r, c + 1), values4<T>(t.codes[i].y, z2, s2));
-        st_shared(chunk_at(tile, r, c + 2), values4<T>(t.codes[i].z, z2, s2));
-        st_shared(chunk_at(tile, r, c + 3), values4<T>(t.codes[i].w, z2, s2));
+    for (int i0 = 0; i0 < X::kRounds; i0 += 4) {
+        uint4 w[4];
+        uint32_t word[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (i0 + i) * X::kRpi + lane / X::kPieces;
+            w[i] = ld_shared(raw + r * (D / 2) + 16 * piece);
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word[i]) : "r"(raw + kN * (D / 2) + 4 * r) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (i0 + i) * X::kRpi + lane / X::kPieces;
+            uint32_t x = IS_V ? word[i] >> 16 : word[i] & 0xffffu;
+            if (IS_V && none && (x & 0x7f80u) == 0x7f80u) x = 0u;
+            const uint32_t z2 = Codes4<T>::zeros(x & 15u), s2 = scale_pair4<T>(x);
+            const uint32_t codes[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t p[4];
+                whole4<T>(codes[c], z2, p);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = Codes4<T>::mul(p[j], s2);
+                st_shared(chunk_at(tile, r, 4 * piece + c), make_uint4(p[0], p[1], p[2], p[3]));
+            }
+        }
     }
     fence_proxy_async_smem();  // before the products read the tile
     __syncwarp();
@@ -220,28 +253,43 @@ template <typename T, int D, bool IS_V>
 __device__ __forceinline__ void produce4(const AttnArgs& a, const Place& place, uint32_t base, Barriers& bar, Current& cur,
                                          volatile int* found_in, bool& ok) {
     using L = LayoutTc<D>;
-    constexpr int ST = L::kStages;
+    constexpr int ST = L::kStages, RW = L::kRaws;
     const int lane = threadIdx.x & 31;
+    const uint32_t raw = base + L::kRawAt + (IS_V ? RW * L::kRaw : 0);
     uint32_t n = 0;  // tiles so far, over all parts
     walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
         if (IS_V) set_current(cur, it, part);
         const bool mixed = it.pos_first != it.pos_last;
-        Tile4<D> t;
-        if (part.j0 < part.j1) {
-            look4<D>(a, it, part, part.j0, t);
-            fetch4<D, IS_V>(a, t);
+        int rows[2];
+        __syncwarp();  // the raw tiles of the part before are read
+#pragma unroll
+        for (int i = 0; i < RW - 1; ++i) {
+            look4(a, it, part, part.j0 + i, rows);
+            fetch4<D, IS_V>(a, rows, raw + i * L::kRaw);
+            cp_async_commit();
         }
+        look4(a, it, part, part.j0 + RW - 1, rows);
+        uint32_t at = 0, next = RW - 1;  // raw tiles: this one's, the one to be fetched
 #pragma unroll 1
         for (int j = part.j0; j < part.j1; ++j, ++n) {
             const uint32_t st = n % ST, turn = (n / ST) & 1u;
-            if (IS_V && mixed && !seen_whole<kN>(a, it, tile_key<kN>(it, j))) {
+            fetch4<D, IS_V>(a, rows, raw + next * L::kRaw);
+            cp_async_commit();
+            look4(a, it, part, j + RW, rows);
+            cp_async_wait<RW - 1>();
+            __syncwarp();
+            const bool partly = IS_V && mixed && !seen_whole<kN>(a, it, tile_key<kN>(it, j));
+            if (partly) {
                 bool none = false;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if ((t.word[h] & 0x7f80u) == 0x7f80u) {
-                        t.word[h] = 0u;
-                        none = true;
-                    }
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t x;
+                    asm volatile("ld.shared.b32 %0, [%1];"
+                                 : "=r"(x)
+                                 : "r"(raw + at * L::kRaw + L::kCodes + 4 * (lane + 32 * h))
+                                 : "memory");
+                    none |= (x >> 16 & 0x7f80u) == 0x7f80u;
+                }
                 if (__any_sync(0xffffffffu, none)) {
                     if (lane == 0) *found_in = cur.no;
                     __threadfence_block();
@@ -249,17 +297,16 @@ __device__ __forceinline__ void produce4(const AttnArgs& a, const Place& place, 
             }
             if (n >= ST) tc_wait_bar(IS_V ? &bar.empty_v[st] : &bar.empty_k[st], turn ^ 1u, ok);
             ok = __all_sync(0xffffffffu, ok);
-            if (!ok) return;
-            put4<T, D>(t, base + (IS_V ? L::kV : L::kK) + st * L::kTile);
+            if (!ok) break;
+            put4<T, D, IS_V>(raw + at * L::kRaw, base + (IS_V ? L::kV : L::kK) + st * L::kTile, partly);
             if (lane == 0) {
                 mbar_arrive(IS_V ? &bar.full_v[st] : &bar.full_k[st]);
                 if (IS_V) mbar_arrive(&bar.clean_v[st]);
             }
-            if (j + 1 < part.j1) {
-                look4<D>(a, it, part, j + 1, t);
-                fetch4<D, IS_V>(a, t);
-            }
+            at = at + 1 == RW ? 0 : at + 1;
+            next = next + 1 == RW ? 0 : next + 1;
         }
+        cp_async_wait<0>();
     });
 }
 
@@ -296,7 +343,7 @@ __device__ __noinline__ void restore_none(const AttnArgs& a, const Current& cur,
 // read is a trip to L2.  A function of its own, so that its registers are not
 // the tiles' (two parts: three spill, 528 -> 609 us in the case above).  Of CTA
 // own, m, l and O are still in its registers and TMEM (O when it had tiles).
-template <typename T, int D>
+template <typename T, int D, bool FOUR>
 __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, int ri, uint32_t tile, int r, bool sees,
                                       float* lse, int own, bool some, uint32_t tm_o, float m_own, float l_own) {
     float M = -INFINITY, l = 0.0f;
@@ -361,7 +408,7 @@ __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, in
                 }
             }
         }
-        put_result<T>(tile, r, 4 * c, o, sees, inv);
+        put_result<T, FOUR>(tile, r, 4 * c, o, sees, inv);
     }
 }
 
@@ -592,8 +639,12 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                                                             (it.kvh * a.G + qrow - t * a.G) * D + ch * 8));
                             }
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
+                            for (int i = 0; i < 8; ++i) {
+                                if (FOUR)  // (0, 1) (2, 3) (4, 5) (6, 7) -> (0, 4) (1, 5) (2, 6) (3, 7)
+                                    w[i] = make_uint4(__byte_perm(w[i].x, w[i].z, 0x5410), __byte_perm(w[i].x, w[i].z, 0x7632),
+                                                      __byte_perm(w[i].y, w[i].w, 0x5410), __byte_perm(w[i].y, w[i].w, 0x7632));
                                 st_shared(row_chunk(own, 32 * quarter + (i0 + i) * RPI + lane / CH, ch), w[i]);
+                            }
                         }
                         fence_proxy_async_smem();
                         mbar_arrive(&bar.q[x]);
@@ -773,7 +824,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
                                                : nullptr;
                     // 32 columns at a time into the row tile's Q, which the products are done with
                     if (split) {
-                        join_row<T, D>(a, part.first, part.last, ri, own, r, sees, lse, early ? (int)blockIdx.x : -1, some,
+                        join_row<T, D, FOUR>(a, part.first, part.last, ri, own, r, sees, lse, early ? (int)blockIdx.x : -1, some,
                                               tm_ox, m, l);
                     } else {
                         if (lse) *lse = sees ? (m + log2f(l)) * kLn2 : -INFINITY;
@@ -784,7 +835,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
 #pragma unroll
                             for (int e = 0; e < 32; ++e) o[e] = 0.0f;
                             if (some) tmem_ld32(tm_ox + 32 * c, o);
-                            put_result<T>(own, r, 4 * c, o, sees, inv);
+                            put_result<T, FOUR>(own, r, 4 * c, o, sees, inv);
                         }
                     }
                     __syncwarp();
@@ -837,7 +888,8 @@ int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
         if (int s = paged_pool_map(&mv, a, a.v, D, Half16<T>::kBf16, kN)) return s;
     }
     static std::atomic<unsigned long long> set_on{0};
-    if (int s = allow_smem(paged_attn_tc<T, D, FOUR>, (int)L::kBytes, set_on)) return s;
+    constexpr uint32_t bytes = FOUR ? L::kBytes4 : L::kBytes;
+    if (int s = allow_smem(paged_attn_tc<T, D, FOUR>, (int)bytes, set_on)) return s;
     a.tickets += kTcWorkspaceAt / sizeof(unsigned);
     a.slots += kTcWorkspaceAt / sizeof(float);
     // one CTA an SM, as many as have slots in the workspace
@@ -852,7 +904,7 @@ int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kThreadsTc);
-    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
