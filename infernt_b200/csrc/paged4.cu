@@ -307,6 +307,7 @@ struct UnpackArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(kUnpackThreads) paged4_unpack(const UnpackArgs a) {
+    const Masks4 mk = make_masks4<T>();
     // y: pages, x: parts of a page
     for (int m = blockIdx.y; m < a.n; m += gridDim.y) {
         const int from = a.src[m], to = a.dst[m];
@@ -330,8 +331,8 @@ __global__ void __launch_bounds__(kUnpackThreads) paged4_unpack(const UnpackArgs
                 const int at = base + i * kUnpackThreads + (int)threadIdx.x;
                 if (at >= a.page_words) break;
                 const uint32_t sk = sc[i] & 0xffffu, sv = sc[i] >> 16;
-                a.k[out + at] = values4<T>(wk[i], Codes4<T>::zeros(sk & 15u), scale_pair4<T>(sk));
-                a.v[out + at] = values4<T>(wv[i], Codes4<T>::zeros(sv & 15u), scale_pair4<T>(sv));
+                a.k[out + at] = values4<T>(wk[i], zeros4(sk, mk), scale_pair4<T>(sk), mk);
+                a.v[out + at] = values4<T>(wv[i], zeros4(sv, mk), scale_pair4<T>(sv), mk);
             }
         }
     }

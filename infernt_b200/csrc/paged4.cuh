@@ -30,18 +30,23 @@ constexpr float kLeastScale4 = Half16<T>::kBf16 ? 7.888609052210118e-31f : 4.768
 constexpr uint32_t kNotFinite4 = 0x7ff0u;
 
 __device__ __forceinline__ float scale4(uint32_t word) { return __uint_as_float((word & 0xfff0u) << 16); }
-__device__ __forceinline__ int zero4(uint32_t word) { return (int)(word & 15u); }
 
-// Eight codes (element j in bits 4 j ...) as pairs of 16-bit floats, (j, j + 4)
-// in pair j; z2: 2^m + z of the vector's zero in both halves, m as below.
-// The exponent of 2^m puts a code in the last bits of the mantissa (bf16: m =
-// 7; fp16: 10); the difference is exact.
+// (w & mask) | one, in one operation.
+__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t one) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(one));
+    return r;
+}
+
+// Pairs of codes as 16-bit floats: the exponent of 2^m puts a code in the last
+// bits of the mantissa (bf16: m = 7; fp16: 10), and what is taken off after it,
+// 2^m + z, leaves c - z exactly.  The mask and 2^m come out of registers that
+// the compiler cannot see through: as immediates they take two operations.
 template <typename T>
 struct Codes4;
 template <>
 struct Codes4<__nv_bfloat16> {
-    static __device__ __forceinline__ uint32_t zeros(uint32_t z) { return 0x43004300u | z | z << 16; }
-    static __device__ __forceinline__ uint32_t zeros(uint32_t z_lo, uint32_t z_hi) { return 0x43004300u | z_lo | z_hi << 16; }
+    static constexpr uint32_t kOne = 0x43004300u;
     static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
         uint32_t r;
         asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -52,12 +57,10 @@ struct Codes4<__nv_bfloat16> {
         asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
         return r;
     }
-    static __device__ __forceinline__ uint32_t spread(uint32_t w) { return (w & 0x000f000fu) | 0x43004300u; }
 };
 template <>
 struct Codes4<__half> {
-    static __device__ __forceinline__ uint32_t zeros(uint32_t z) { return 0x64006400u | z | z << 16; }
-    static __device__ __forceinline__ uint32_t zeros(uint32_t z_lo, uint32_t z_hi) { return 0x64006400u | z_lo | z_hi << 16; }
+    static constexpr uint32_t kOne = 0x64006400u;
     static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
         uint32_t r;
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -68,22 +71,35 @@ struct Codes4<__half> {
         asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
         return r;
     }
-    static __device__ __forceinline__ uint32_t spread(uint32_t w) { return (w & 0x000f000fu) | 0x64006400u; }
+};
+struct Masks4 {
+    uint32_t low, one;
 };
 template <typename T>
-__device__ __forceinline__ void whole4(uint32_t w, uint32_t z2, uint32_t (&p)[4]) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = Codes4<T>::sub(Codes4<T>::spread(w >> (4 * j)), z2);
+__device__ __forceinline__ Masks4 make_masks4() {
+    Masks4 k;
+    asm volatile("mov.b32 %0, 0x000f000f;" : "=r"(k.low));
+    asm volatile("mov.b32 %0, %1;" : "=r"(k.one) : "n"(Codes4<T>::kOne));
+    return k;
+}
+// 2^m + z in both halves, of a scale word.
+__device__ __forceinline__ uint32_t zeros4(uint32_t word, const Masks4& k) {
+    return and_or(__byte_perm(word, word, 0x1010), k.low, k.one);
 }
 
-// Eight values in their order, as the 16 bytes of a row of T; s2: the scale as
-// a T in both halves.
+// Eight values, element j in bits 4 j ... of w, as pairs (j, j + 4); s2: the
+// scale as a T in both halves.
 template <typename T>
-__device__ __forceinline__ uint4 values4(uint32_t w, uint32_t z2, uint32_t s2) {
-    uint32_t p[4];
-    whole4<T>(w, z2, p);
+__device__ __forceinline__ void pairs4(uint32_t w, uint32_t z2, uint32_t s2, const Masks4& k, uint32_t (&p)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = Codes4<T>::mul(p[j], s2);
+    for (int j = 0; j < 4; ++j)
+        p[j] = Codes4<T>::mul(Codes4<T>::sub(and_or(w >> (4 * j), k.low, k.one), z2), s2);
+}
+// In their order, as the 16 bytes of a row of T.
+template <typename T>
+__device__ __forceinline__ uint4 values4(uint32_t w, uint32_t z2, uint32_t s2, const Masks4& k) {
+    uint32_t p[4];
+    pairs4<T>(w, z2, s2, k, p);
     // (0, 4) (1, 5) (2, 6) (3, 7) -> (0, 1) (2, 3) (4, 5) (6, 7)
     return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410),
                       __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));

@@ -124,11 +124,6 @@ __device__ __forceinline__ Masks make_masks() {
     asm volatile("mov.b32 %0, 0x54005400;" : "=r"(k.high_one));
     return k;
 }
-__device__ __forceinline__ uint32_t and_or(uint32_t w, uint32_t mask, uint32_t magic) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(magic));
-    return r;
-}
 __device__ __forceinline__ uint32_t half2_sub(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -158,7 +153,8 @@ __device__ __forceinline__ void whole(uint32_t w, const Zeros& z, const Masks& k
 // (not of such keys: what lies there are numbers whatever it is, and copies of
 // one row for all of them would meet in one place of L2), and scale words, 0
 // for such keys.  Every warp fetches for itself, two tiles ahead, so none waits
-// for another; the table's entry of a key is looked up three tiles ahead.  (16
+// for another; the table's entry of a key is loaded three tiles ahead and looked
+// at one tile later (looked at at once, it held the warp up).  (16
 // sequences of 32768 positions took 141 us with a warp that streamed for the
 // others, which spends a fifth of the issue slots on its loops over pages, and
 // 141 with three bulk copies a warp and tile.)
@@ -241,17 +237,22 @@ __device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, 
     constexpr uint32_t ROW = D / 2;
     const int g = lane >> 2, tig = lane & 3;
     const uint32_t ring = base + warp * L::kRing;
-    // the pool row of key `lane` of this warp in tile j
+    // where key `lane` of this warp in tile j is; its copies into stage n
+    const int* table = a.b.table + (size_t)part.s * a.b.table_stride;
     auto look = [&](int j) {
         const int p = tile_key<kKeys>(it, j) + warp * kWarpKeys + lane;
-        return j < part.j1 && item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
+        return page_of(a.b, table, p, j < part.j1 && item_sees(it, p));
     };
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        fetch<D>(a, look(part.j0 + i), lane, ring + i * L::kStage);
+    auto get = [&](PageOf at, uint32_t n) {
+        fetch<D>(a, pool_row(a.b, it.kvh, at, a.err), lane, ring + n * L::kStage);
         cp_async_commit();
-    }
-    int ahead = look(part.j0 + kStages - 1);
+    };
+    PageOf ahead[kStages];
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) ahead[i] = look(part.j0 + i);
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) get(ahead[i], i);
+    PageOf next = ahead[kStages - 1];
     const Masks mk = make_masks();
     uint4 qb[W];
     int shift;
@@ -308,9 +309,8 @@ __device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, 
     uint32_t now = 0;  // the stage of tile j
 #pragma unroll 1
     for (int j = part.j0; j < part.j1; ++j) {
-        fetch<D>(a, ahead, lane, ring + (now == 0 ? kStages - 1 : now - 1) * L::kStage);
-        cp_async_commit();
-        ahead = look(j + kStages);
+        get(next, now == 0 ? kStages - 1 : now - 1);
+        next = look(j + kStages);
         cp_async_wait<kStages - 1>();
         __syncwarp();
         const uint32_t stage = ring + now * L::kStage;

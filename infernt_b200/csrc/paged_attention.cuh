@@ -374,6 +374,22 @@ __device__ __forceinline__ int pool_row(const PagedBatch& b, int s, int kvh, int
     return (page * b.nkv + kvh) * b.page_size + (p - pi * b.page_size);
 }
 
+// The same in two steps, so that what needs the table's entry can come a tile
+// after its load: where position p is, and then its pool row.
+struct PageOf {
+    int page, row;  // the table's entry (kNoPage: not looked up), the row in the page
+};
+constexpr int kNoPage = -0x7fffffff - 1;
+__device__ __forceinline__ PageOf page_of(const PagedBatch& b, const int* table, int p, bool wanted) {
+    const int pi = b.by_page(p);
+    return {wanted ? __ldg(table + pi) : kNoPage, p - pi * b.page_size};
+}
+__device__ __forceinline__ int pool_row(const PagedBatch& b, int kvh, PageOf at, unsigned* err) {
+    if (at.page >= 0 && at.page < b.num_pages) return (at.page * b.nkv + kvh) * b.page_size + at.row;
+    if (at.page != kNoPage && err) atomicOr(err, kErrPage);
+    return -1;
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -67,7 +67,10 @@ namespace {
 constexpr int kM = kTcItemRows;  // query rows of an item
 constexpr int kN = kTcTileKeys;  // keys of a tile
 constexpr int kThreadsTc = 384;
-constexpr int kJoin = 2;  // parts of a split item that are read at once
+// Parts of a split item that are read at once (of pages of 4 bits, whose launch
+// has more threads, one: ptxas has no registers for two).
+template <bool FOUR>
+constexpr int kJoin = FOUR ? 1 : 2;
 constexpr int kRowThreads = 256;
 constexpr uint32_t kBoxQ = 16384;  // 128 rows of 64 values: a swizzled operand block
 constexpr uint32_t kBox = 8192;    // 64 rows: a block of chunk_at
@@ -84,11 +87,11 @@ struct LayoutTc {
     static constexpr uint32_t kK = 2 * kTileQ;
     static constexpr uint32_t kV = kK + kStages * kTile;
     static constexpr uint32_t kBytes = kV + kStages * kTile + 1024;
-    // Pages of 4 bits: tiles of codes and scale words behind those, of K and then of V
-    static constexpr uint32_t kCodes = kN * D / 2, kRaw = kCodes + kN * 4;
+    // Pages of 4 bits: rings of codes and scale words behind those, one for each half of K's and of V's tiles
+    static constexpr uint32_t kCodes = kN / 2 * D / 2, kRaw = kCodes + kN / 2 * 4;
     static constexpr int kRaws = 3;
     static constexpr uint32_t kRawAt = kV + kStages * kTile;
-    static constexpr uint32_t kBytes4 = kRawAt + 2 * kRaws * kRaw + 1024;
+    static constexpr uint32_t kBytes4 = kRawAt + 4 * kRaws * kRaw + 1024;
 };
 
 struct Barriers {
@@ -167,141 +170,136 @@ __device__ __noinline__ void restore_values(const AttnArgs& a, const Current& cu
 }
 
 // ------------------------------------------------- pages of 4 bits
-// The tiles are the same, in 16 bits, but for how they get there: warp 0 makes
-// the K tiles and warp 2 the V tiles out of codes (paged4.cuh).  A tile's codes
-// and scale words come by cp.async, row by row, two tiles ahead of the one that
-// the warp turns into values; the table's entries are looked up three ahead.
-// The values are numbers of T, so the products are those over 16-bit pages.
-// Eight values lie in the order in which they come out of a word, (0, 4) (1, 5)
-// (2, 6) (3, 7): the row warps put Q into that order too, and take the result
-// out of it.  A tile is some 600 issue slots of each warp, on schedulers of
-// which the row warps leave half.
+// The tiles are the same, in 16 bits, but for how they get there: four warps
+// more make them out of codes (paged4.cuh), the halves of K's by warps 12 and
+// 13, of V's by 14 and 15.  Half a tile's codes and scale words come by
+// cp.async, row by row, two tiles ahead of the one that the warp turns into
+// values; the table's entries are loaded three ahead.  The values are numbers of
+// T, so the products are those over 16-bit pages.  Eight values lie in the order
+// in which they come out of a word, (0, 4) (1, 5) (2, 6) (3, 7): the row warps
+// put Q into that order too, and take the result out of it.
+// The 512 x 128 registers of a launch are 176 a thread of the row warps and 80
+// of the others.  4096 tokens at 12288 positions, 32/8 heads of 128, bf16: 621
+// us, the time of 16-bit pages.  Before: 1259 us with the first four warps' two
+// idle ones in place of four more (a tile is 1600 instructions, one behind the
+// other), 1931 as straight code for whole tiles (waiting for instructions),
+// 705 with 64 registers, 889 with 48.
+constexpr int kThreads4 = 512;
+constexpr int kHalf = kN / 2;  // keys of a warp's half
 
 template <int D>
-struct Tile4 {
+struct Half4 {
     static constexpr int kPieces = D / 32;  // 16-byte pieces of a row's codes
-    static constexpr int kRpi = 32 / kPieces, kRounds = kN / kRpi;  // rows at once, rounds
+    static constexpr int kRpi = 32 / kPieces, kRounds = kHalf / kRpi;  // rows at once, rounds
 };
 
-// Pool rows of keys lane and lane + 32 of tile j (-1: no row sees the key, or
-// the pool does not have it).
-__device__ __forceinline__ void look4(const AttnArgs& a, const Item& it, const Part& part, int j, int (&rows)[2]) {
-    const int lane = threadIdx.x & 31, k0 = tile_key<kN>(it, j);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int p = k0 + lane + 32 * h;
-        rows[h] = j < part.j1 && item_sees(it, p) ? pool_row(a.b, part.s, it.kvh, p, a.err) : -1;
-    }
-}
-// A tile's copies: zeros for rows of -1 (a scale of 0).
-template <int D, bool IS_V>
-__device__ __forceinline__ void fetch4(const AttnArgs& a, const int (&rows)[2], uint32_t raw) {
-    using X = Tile4<D>;
-    const int lane = threadIdx.x & 31;
-    const char* codes = static_cast<const char*>(IS_V ? a.v : a.k) + 16 * (lane % X::kPieces);
+// The copies of half a tile, key `lane` at `at`: zeros (a scale of 0) for keys
+// that no row sees, and for pages that the pool does not have.
+template <int D>
+__device__ __forceinline__ void fetch4(const AttnArgs& a, const Item& it, const void* pool, PageOf at, uint32_t raw) {
+    using X = Half4<D>;
+    const int lane = threadIdx.x & 31, own = pool_row(a.b, it.kvh, at, a.err);
+    const char* codes = static_cast<const char*>(pool) + 16 * (lane % X::kPieces);
 #pragma unroll
     for (int i = 0; i < X::kRounds; ++i) {
-        const int r = i * X::kRpi + lane / X::kPieces;
-        const int row = __shfl_sync(0xffffffffu, rows[i * X::kRpi / 32], r & 31);
-        cp_async16(raw + r * (D / 2) + 16 * (lane % X::kPieces), codes + (size_t)max(row, 0) * (D / 2), row >= 0 ? 16u : 0u);
+        const int row = __shfl_sync(0xffffffffu, own, i * X::kRpi + lane / X::kPieces);
+        cp_async16(raw + 16 * lane + i * 512, codes + (size_t)max(row, 0) * (D / 2), row >= 0 ? 16u : 0u);
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw + kN * (D / 2) + 4 * (lane + 32 * h)),
-                     "l"(a.scales + max(rows[h], 0)), "r"(rows[h] >= 0 ? 4u : 0u)
-                     : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw + kHalf * (D / 2) + 4 * lane),
+                 "l"(a.scales + max(own, 0)), "r"(own >= 0 ? 4u : 0u)
+                 : "memory");
 }
-// The values of a tile of codes.  none: vectors of NaN become zeros.
-template <typename T, int D, bool IS_V>
-__device__ __forceinline__ void put4(uint32_t raw, uint32_t tile, bool none) {
-    using X = Tile4<D>;
-    const int lane = threadIdx.x & 31, piece = lane % X::kPieces;
+// The values of half a tile of codes, their scale words `shift` bits up in the
+// pair's.  none: vectors of NaN become zeros.
+template <typename T, int D>
+__device__ __forceinline__ void put4(uint32_t raw, uint32_t tile, int shift, bool none, const Masks4& mk) {
+    using X = Half4<D>;
+    const int lane = threadIdx.x & 31, piece = lane % X::kPieces, r0 = lane / X::kPieces;
+    const uint32_t words = raw + kHalf * (D / 2) + 4 * r0;
+    // rows r0 + i kRpi: kRpi is 8 or 16, so the row's place in the swizzle stays
+    const uint32_t dst = tile + (uint32_t)(piece >> 1) * kBox + r0 * 128, flip = (uint32_t)((4 * piece) & 7) ^ (r0 & 7);
+    uint4 w = ld_shared(raw + 16 * lane);
 #pragma unroll
-    for (int i0 = 0; i0 < X::kRounds; i0 += 4) {
-        uint4 w[4];
-        uint32_t word[4];
+    for (int i = 0; i < X::kRounds; ++i) {
+        uint32_t x;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(words + 4 * i * X::kRpi) : "memory");
+        const uint4 next = ld_shared(raw + 16 * lane + min(i + 1, X::kRounds - 1) * 512);
+        x = (x >> shift) & 0xffffu;
+        if (none && (x & 0x7f80u) == 0x7f80u) x = 0u;
+        const uint32_t z2 = zeros4(x, mk), s2 = scale_pair4<T>(x);
+        // pieces of the second block of columns begin with another word, or they would meet the first's in the banks
+        const bool late = piece & 2;
+        const uint32_t codes[4] = {late ? w.z : w.x, late ? w.w : w.y, late ? w.x : w.z, late ? w.y : w.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (i0 + i) * X::kRpi + lane / X::kPieces;
-            w[i] = ld_shared(raw + r * (D / 2) + 16 * piece);
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word[i]) : "r"(raw + kN * (D / 2) + 4 * r) : "memory");
+        for (int c = 0; c < 4; ++c) {
+            uint32_t p[4];
+            pairs4<T>(codes[c], z2, s2, mk, p);
+            st_shared(dst + i * X::kRpi * 128 + ((flip ^ c ^ (late ? 2u : 0u)) << 4), make_uint4(p[0], p[1], p[2], p[3]));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = (i0 + i) * X::kRpi + lane / X::kPieces;
-            uint32_t x = IS_V ? word[i] >> 16 : word[i] & 0xffffu;
-            if (IS_V && none && (x & 0x7f80u) == 0x7f80u) x = 0u;
-            const uint32_t z2 = Codes4<T>::zeros(x & 15u), s2 = scale_pair4<T>(x);
-            const uint32_t codes[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t p[4];
-                whole4<T>(codes[c], z2, p);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) p[j] = Codes4<T>::mul(p[j], s2);
-                st_shared(chunk_at(tile, r, 4 * piece + c), make_uint4(p[0], p[1], p[2], p[3]));
-            }
-        }
+        w = next;
     }
     fence_proxy_async_smem();  // before the products read the tile
     __syncwarp();
 }
 
-// All tiles of a CTA's parts, K by warp 0 or V by warp 2.  V vectors of NaN in
-// tiles that rows see in part become zeros, and *found_in the part.
-template <typename T, int D, bool IS_V>
+// A warp's halves of all tiles of a CTA's parts.  V vectors of NaN in tiles
+// that rows see in part become zeros, and *found_in the part.
+template <typename T, int D>
 __device__ __forceinline__ void produce4(const AttnArgs& a, const Place& place, uint32_t base, Barriers& bar, Current& cur,
-                                         volatile int* found_in, bool& ok) {
+                                         volatile int* found_in, bool is_v, int half, bool& ok) {
     using L = LayoutTc<D>;
     constexpr int ST = L::kStages, RW = L::kRaws;
-    const int lane = threadIdx.x & 31;
-    const uint32_t raw = base + L::kRawAt + (IS_V ? RW * L::kRaw : 0);
+    const int lane = threadIdx.x & 31, shift = is_v ? 16 : 0;
+    const uint32_t raw = base + L::kRawAt + (2 * (int)is_v + half) * (RW * L::kRaw);
+    const uint32_t tiles = base + (is_v ? L::kV : L::kK) + half * (kHalf * 128);
+    const void* pool = is_v ? a.v : a.k;
+    uint64_t* empty = is_v ? bar.empty_v : bar.empty_k;
+    uint64_t* full = is_v ? bar.full_v : bar.full_k;
+    const Masks4 mk = make_masks4<T>();
     uint32_t n = 0;  // tiles so far, over all parts
     walk<kM, kN>(a, place, [&](const PagedSeq&, const Item& it, const Part& part) {
-        if (IS_V) set_current(cur, it, part);
+        set_current(cur, it, part);
         const bool mixed = it.pos_first != it.pos_last;
-        int rows[2];
+        const int* table = a.b.table + (size_t)part.s * a.b.table_stride;
+        auto look = [&](int j) {
+            const int p = tile_key<kN>(it, j) + kHalf * half + lane;
+            return page_of(a.b, table, p, j < part.j1 && item_sees(it, p));
+        };
+        PageOf pages[RW];
         __syncwarp();  // the raw tiles of the part before are read
 #pragma unroll
+        for (int i = 0; i < RW; ++i) pages[i] = look(part.j0 + i);
+#pragma unroll
         for (int i = 0; i < RW - 1; ++i) {
-            look4(a, it, part, part.j0 + i, rows);
-            fetch4<D, IS_V>(a, rows, raw + i * L::kRaw);
+            fetch4<D>(a, it, pool, pages[i], raw + i * L::kRaw);
             cp_async_commit();
         }
-        look4(a, it, part, part.j0 + RW - 1, rows);
+        PageOf ahead = pages[RW - 1];
         uint32_t at = 0, next = RW - 1;  // raw tiles: this one's, the one to be fetched
 #pragma unroll 1
         for (int j = part.j0; j < part.j1; ++j, ++n) {
             const uint32_t st = n % ST, turn = (n / ST) & 1u;
-            fetch4<D, IS_V>(a, rows, raw + next * L::kRaw);
+            fetch4<D>(a, it, pool, ahead, raw + next * L::kRaw);
             cp_async_commit();
-            look4(a, it, part, j + RW, rows);
+            ahead = look(j + RW);
             cp_async_wait<RW - 1>();
             __syncwarp();
-            const bool partly = IS_V && mixed && !seen_whole<kN>(a, it, tile_key<kN>(it, j));
+            const bool partly = is_v && mixed && !seen_whole<kN>(a, it, tile_key<kN>(it, j));
             if (partly) {
-                bool none = false;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t x;
-                    asm volatile("ld.shared.b32 %0, [%1];"
-                                 : "=r"(x)
-                                 : "r"(raw + at * L::kRaw + L::kCodes + 4 * (lane + 32 * h))
-                                 : "memory");
-                    none |= (x >> 16 & 0x7f80u) == 0x7f80u;
-                }
-                if (__any_sync(0xffffffffu, none)) {
+                uint32_t x;
+                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(raw + at * L::kRaw + L::kCodes + 4 * lane) : "memory");
+                if (__any_sync(0xffffffffu, (x >> 16 & 0x7f80u) == 0x7f80u)) {
                     if (lane == 0) *found_in = cur.no;
                     __threadfence_block();
                 }
             }
-            if (n >= ST) tc_wait_bar(IS_V ? &bar.empty_v[st] : &bar.empty_k[st], turn ^ 1u, ok);
+            if (n >= ST) tc_wait_bar(&empty[st], turn ^ 1u, ok);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
-            put4<T, D, IS_V>(raw + at * L::kRaw, base + (IS_V ? L::kV : L::kK) + st * L::kTile, partly);
+            put4<T, D>(raw + at * L::kRaw, tiles + st * L::kTile, shift, partly, mk);
             if (lane == 0) {
-                mbar_arrive(IS_V ? &bar.full_v[st] : &bar.full_k[st]);
-                if (IS_V) mbar_arrive(&bar.clean_v[st]);
+                mbar_arrive(&full[st]);
+                if (is_v) mbar_arrive(&bar.clean_v[st]);
             }
             at = at + 1 == RW ? 0 : at + 1;
             next = next + 1 == RW ? 0 : next + 1;
@@ -374,11 +372,11 @@ __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, in
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0.0f;
 #pragma unroll 1
-        for (int b = first; b <= last; b += kJoin) {
-            float mb[kJoin];
-            float4 v[kJoin][8];
+        for (int b = first; b <= last; b += kJoin<FOUR>) {
+            float mb[kJoin<FOUR>];
+            float4 v[kJoin<FOUR>][8];
 #pragma unroll
-            for (int i = 0; i < kJoin; ++i) {
+            for (int i = 0; i < kJoin<FOUR>; ++i) {
                 if (b + i > last) break;
                 if (b + i == own) {
                     mb[i] = m_own;
@@ -396,7 +394,7 @@ __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, in
                 for (int e = 0; e < 8; ++e) v[i][e] = __ldcg(reinterpret_cast<const float4*>(p) + (8 * c + e) * kM + ri);
             }
 #pragma unroll
-            for (int i = 0; i < kJoin; ++i) {
+            for (int i = 0; i < kJoin<FOUR>; ++i) {
                 if (b + i > last) break;
                 const float f = mb[i] == -INFINITY ? 0.0f : ex2(mb[i] - M);
 #pragma unroll
@@ -414,7 +412,7 @@ __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, in
 
 // FOUR: pages of 4 bits
 template <typename T, int D, bool FOUR>
-__global__ void __launch_bounds__(kThreadsTc, 1)
+__global__ void __launch_bounds__(FOUR ? kThreads4 : kThreadsTc, 1)
     paged_attn_tc(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v) {
     using L = LayoutTc<D>;
@@ -424,15 +422,16 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     __shared__ uint32_t tmem_s;
     __shared__ int ok_s;
     __shared__ int last_s, early_s, found_s;  // found_s: the last part in which clean_rows found something
-    __shared__ Current cur_s[kThreadsTc / 32];
+    constexpr int NT = FOUR ? kThreads4 : kThreadsTc;
+    __shared__ Current cur_s[NT / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
-            mbar_init(&bar.full_k[i], 1);
+            mbar_init(&bar.full_k[i], FOUR ? 2 : 1);
             mbar_init(&bar.empty_k[i], 2);
-            mbar_init(&bar.full_v[i], 1);
-            mbar_init(&bar.clean_v[i], 1);
+            mbar_init(&bar.full_v[i], FOUR ? 2 : 1);
+            mbar_init(&bar.clean_v[i], FOUR ? 2 : 1);
             mbar_init(&bar.empty_v[i], 2);
         }
         for (int x = 0; x < 2; ++x) {
@@ -449,7 +448,7 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
         for (Current& c : cur_s) c.no = 0;
     }
     if (warp == 1) tmem_alloc(&tmem_s, 512);
-    const Place place = find_place<kM, kN, kThreadsTc>(a);  // its barriers publish the set-up
+    const Place place = find_place<kM, kN, NT>(a);  // its barriers publish the set-up
     tc_fence_after();
     __syncthreads();
     // TMEM columns: S of A at 0 and 64, of B at 128 and 192; O of A at 256, of B D further; P
@@ -458,13 +457,15 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
     auto tm_prob = [&](int x, int b) { return D == 128 ? tm_score(x, b) + 32u : tmem + 384u + 64u * x + 32u * b; };
     auto tm_out = [&](int x) { return tmem + 256u + (uint32_t)D * x; };
     bool ok = true;
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
-        if (FOUR && warp == 0 && place.s >= 0) {
-            produce4<T, D, false>(a, place, base, bar, cur_s[0], &found_s, ok);
-        } else if (FOUR && warp == 2 && place.s >= 0) {
-            produce4<T, D, true>(a, place, base, bar, cur_s[2], &found_s, ok);
-        } else if (!FOUR && warp == 0 && place.s >= 0) {
+    if (FOUR && warp >= 12) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
+        if (place.s >= 0) produce4<T, D>(a, place, base, bar, cur_s[warp], &found_s, warp >= 14, warp & 1, ok);
+    } else if (warp < 4) {
+        if (FOUR)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
+        if (!FOUR && warp == 0 && place.s >= 0) {
             // ---- K and V tiles.  n: tiles so far, over all parts.
             uint32_t n = 0;
             const int ps = a.b.page_size, per_tile = ps < kN ? kN / ps : 1, box_rows = ps < kN ? ps : kN;
@@ -598,7 +599,10 @@ __global__ void __launch_bounds__(kThreadsTc, 1)
             });
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
+        if (FOUR)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 176;" ::: "memory");
+        else
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
         if (place.s >= 0) {
             // ---- the rows: thread = TMEM lane r of row tile x
             const int x = (warp - 4) >> 2, quarter = warp & 3, r = 32 * quarter + lane;
@@ -903,7 +907,7 @@ int launch_tc(const AttnArgs& args, bool after_other, cudaStream_t st) {
     // other kernel of this call: neither touches what the other writes
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kThreadsTc);
+    cfg.blockDim = dim3(FOUR ? kThreads4 : kThreadsTc);
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = st;
     cudaLaunchAttribute attr;
