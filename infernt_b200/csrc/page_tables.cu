@@ -38,65 +38,165 @@ struct PlanArgs {
     unsigned* err;
 };
 
+// Sums that stay at kMost once they are there: such a sum is past every limit
+// that it is held to, and of numbers that no caller can mean.
+constexpr unsigned kMost = 0x7fffffffu;
+__device__ __forceinline__ unsigned add(unsigned a, unsigned b) { return min(a + b, kMost); }
+
 // Sums of N values over the threads before this one, and of all; by all
 // threads of the block.
 template <int N>
-__device__ __forceinline__ void block_scan(long long (&v)[N], long long (&all)[N], long long (*sums)[32]) {
+__device__ __forceinline__ void block_scan(unsigned (&v)[N], unsigned (&all)[N], unsigned (*sums)[32]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long x[N];
+    unsigned x[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         x[n] = v[n];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x[n], o);
-            if (lane >= o) x[n] += y;
+            const unsigned y = __shfl_up_sync(0xffffffffu, x[n], o);
+            if (lane >= o) x[n] = add(x[n], y);
         }
+        if (lane == 31) sums[n][warp] = x[n];
+        x[n] = __shfl_up_sync(0xffffffffu, x[n], 1);
+        if (lane == 0) x[n] = 0;
     }
-    __syncthreads();
-    if (lane == 31)
-#pragma unroll
-        for (int n = 0; n < N; ++n) sums[n][warp] = x[n];
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        long long w = sums[n][lane];  // of warp `lane`
+        unsigned w = sums[n][lane];  // of warp `lane`
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
+            const unsigned y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w = add(w, y);
         }
         all[n] = __shfl_sync(0xffffffffu, w, 31);
-        const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-        v[n] = x[n] - v[n] + (warp ? before : 0);
+        const unsigned before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+        v[n] = warp ? add(x[n], before) : x[n];
     }
 }
 
-// n >= 0 modulo the ring's size; more than once around it only when held is
-// not what the sequences were given.
-__device__ __forceinline__ int wrap(long long n, int size) {
-    if (n < size) return (int)n;
-    n -= size;
-    return (int)(n < size ? n : n % size);
+// a + b modulo the ring's size, a below it.  b is more than once around it only
+// when held is not what the sequences were given.
+__device__ __forceinline__ int wrap(unsigned a, unsigned b, int size) {
+    if (b >= (unsigned)size) b %= (unsigned)size;
+    const unsigned x = a + b;
+    return (int)(x < (unsigned)size ? x : x - (unsigned)size);
 }
 
-// What a sequence's pages and rows come to.
-struct Move {
-    int s, held, need;    // pages before and after
-    long long take, give; // places in the ring: the first page taken, the first given back
-    int len, n, row0;     // positions kept, new tokens, the first row
+// 1024 sequences: what the places among their rows, pages taken and pages given
+// back are found by.
+struct Chunk {
+    int len[kPlanThreads], held[kPlanThreads], need[kPlanThreads];
+    unsigned row[kPlanThreads], take[kPlanThreads], give[kPlanThreads];  // sums before each
 };
+// The last sequence of the chunk whose sum before is at most x (one with sums
+// above it then begins at it).
+__device__ __forceinline__ int owner(const unsigned* before, unsigned x) {
+    int at = 0;
+#pragma unroll
+    for (int step = kPlanThreads / 2; step > 0; step /= 2)
+        if (before[at + step] <= x) at += step;
+    return at;
+}
 
-// Pages [i0, i0 + step, ...) of a move.
-__device__ __forceinline__ void move_pages(const PlanArgs& a, const Move& m, int i0, int step) {
-    int* row = a.table + (size_t)m.s * a.stride;
+// One CTA: the scans need every sequence, and up to 1024 of them are one round
+// of loads.  Rows and pages are then dealt evenly to the threads, whoever's they
+// are.  A page that a sequence takes is read from the ring wherever it is
+// needed, so nothing waits for a store.  Latency-bound: loads, two scans, a
+// search of ten steps, the ring's and the table's loads, stores.  (A thread or a
+// warp a sequence took 20 us for the step of 256 sequences and 85 for 100
+// prompts.)
+__global__ void __launch_bounds__(kPlanThreads) paged_plan(const PlanArgs a) {
+    pdl_launch_dependents();  // paged_plan_rows waits for this kernel's end
+    __shared__ unsigned sums[3][32];
+    __shared__ Chunk ch;
+    const int tid = threadIdx.x;
+    const int head = a.state[0], count = a.state[1];
+    const bool sane = head >= 0 && head < a.num_pages && count >= 0 && count <= a.num_pages;
+    const unsigned tail = sane ? (unsigned)wrap(head, count, a.num_pages) : 0u;
+    unsigned rows_wanted = 0, pages_wanted = 0, rows = 0, taken = 0, given = 0;
+    unsigned err = sane ? 0u : kErrBatch;
+    for (int base = 0; base < a.num_seqs; base += kPlanThreads) {
+        const int s = base + tid;
+        int len = 0, n = 0, held = 0, need = 0;
+        bool fine = false;
+        if (s < a.num_seqs) {
+            len = a.len[s];
+            n = a.new_len[s];
+            held = a.held[s];
+            const long long end = (long long)len + n;
+            fine = len >= 0 && n >= 0 && end <= kMaxPositions && end <= (long long)a.stride * a.page_size && held >= 0 &&
+                   held <= a.stride;
+            if (!fine) err |= kErrBatch;
+            fine = fine && sane;
+            if (fine) need = a.by_page((int)end + a.page_size - 1);
+        }
+        const unsigned own_rows = fine ? n : 0, own_pages = fine ? max(need - held, 0) : 0;
+        unsigned want[2] = {own_rows, own_pages}, all[2];
+        block_scan<2>(want, all, sums);
+        const bool waits = (own_pages > 0 && add(pages_wanted, add(want[1], own_pages)) > (unsigned)count) ||
+                           (own_rows > 0 && add(rows_wanted, add(want[0], own_rows)) > (unsigned)a.max_rows);
+        rows_wanted = add(rows_wanted, all[0]);
+        pages_wanted = add(pages_wanted, all[1]);
+        if (waits) err |= kErrNoRoom;
+        if (!fine || waits) {
+            n = 0;
+            need = held;
+        }
+        unsigned sum[3] = {(unsigned)n, (unsigned)max(need - held, 0), (unsigned)max(held - need, 0)}, tot[3];
+        __syncthreads();  // sums is read
+        block_scan<3>(sum, tot, sums);
+        ch.len[tid] = len;
+        ch.held[tid] = held;
+        ch.need[tid] = need;
+        ch.row[tid] = sum[0];
+        ch.take[tid] = sum[1];
+        ch.give[tid] = sum[2];
+        if (s < a.num_seqs) {
+            a.q_start[s + 1] = (int)(rows + sum[0]) + n;
+            a.kv_len[s] = len + n;
+            if (need != held) a.held[s] = need;
+        }
+        __syncthreads();
+        // page x of those that the chunk takes: the i-th of sequence o, behind those that it holds
+        for (unsigned x = tid; x < tot[1]; x += kPlanThreads) {
+            const int o = owner(ch.take, x), i = ch.held[o] + (int)(x - ch.take[o]);
+            a.table[(size_t)(base + o) * a.stride + i] = a.ring[wrap(head, taken + x, a.num_pages)];
+        }
+        // of those that it gives back, behind those that it keeps (a page that was never given: no place for it)
 #pragma unroll 4
-    for (int i = m.held + i0; i < m.need; i += step) row[i] = a.ring[wrap(m.take + (i - m.held), a.num_pages)];
-#pragma unroll 4
-    for (int i = m.need + i0; i < m.held; i += step) {
-        a.ring[wrap(m.give + (i - m.need), a.num_pages)] = row[i];
-        row[i] = -1;
+        for (unsigned x = tid; x < tot[2]; x += kPlanThreads) {
+            const int o = owner(ch.give, x), i = ch.need[o] + (int)(x - ch.give[o]);
+            int* at = a.table + (size_t)(base + o) * a.stride + i;
+            a.ring[wrap(tail, add(given, x), a.num_pages)] = *at;
+            *at = -1;
+        }
+        if (a.rows_here)
+            for (unsigned x = tid; x < tot[0]; x += kPlanThreads) {
+                const int o = owner(ch.row, x), pos = ch.len[o] + (int)(x - ch.row[o]);
+                const int r = (int)(rows + x);
+                if (a.positions) a.positions[r] = pos;
+                if (a.slots) {
+                    const int pi = a.by_page(pos), held_o = ch.held[o];
+                    const int page = pi < held_o ? a.table[(size_t)(base + o) * a.stride + pi]
+                                                 : a.ring[wrap(head, taken + ch.take[o] + (pi - held_o), a.num_pages)];
+                    a.slots[r] = page * a.page_size + (pos - pi * a.page_size);
+                }
+            }
+        rows += tot[0];
+        taken += tot[1];
+        given = add(given, tot[2]);
+        __syncthreads();  // sums and ch are read
     }
+    if (tid == 0) {
+        a.q_start[0] = 0;
+        if (sane) {
+            a.state[0] = wrap(head, taken, a.num_pages);
+            a.state[1] = (int)add((unsigned)count - taken, given);
+        }
+    }
+    if (a.err && err) atomicOr(a.err, err);
 }
 
 // Row r's position and slot; the page is in its table entry.
@@ -106,98 +206,6 @@ __device__ __forceinline__ void put_row(const PlanArgs& a, int s, int pos, int r
         const int pi = a.by_page(pos);
         a.slots[r] = a.table[(size_t)s * a.stride + pi] * a.page_size + (pos - pi * a.page_size);
     }
-}
-__device__ __forceinline__ void move_rows(const PlanArgs& a, const Move& m, int i0, int step) {
-    for (int i = i0; i < m.n; i += step) put_row(a, m.s, m.len + i, m.row0 + i);
-}
-
-// One CTA: the scans need every sequence, and up to 1024 of them are one round
-// of loads.  A sequence's pages and rows are its thread's; where they are more
-// than kOwn, its warp's.  Latency-bound: loads, two scans, the ring's loads,
-// stores.
-constexpr int kOwn = 4;
-
-__global__ void __launch_bounds__(kPlanThreads) paged_plan(const PlanArgs a) {
-    __shared__ long long sums[3][32];
-    pdl_launch_dependents();  // paged_plan_rows waits for this kernel's end
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int head = a.state[0], count = a.state[1];
-    const bool sane = head >= 0 && head < a.num_pages && count >= 0 && count <= a.num_pages;
-    long long rows_wanted = 0, pages_wanted = 0, rows = 0, taken = 0, given = 0;
-    unsigned err = sane ? 0u : kErrBatch;
-    for (int base = 0; base < a.num_seqs; base += kPlanThreads) {
-        const int s = base + tid;
-        Move m = {s, 0, 0, 0, 0, 0, 0, 0};
-        bool fine = false;
-        if (s < a.num_seqs) {
-            m.len = a.len[s];
-            m.n = a.new_len[s];
-            m.held = a.held[s];
-            const long long end = (long long)m.len + m.n;
-            fine = m.len >= 0 && m.n >= 0 && end <= kMaxPositions && end <= (long long)a.stride * a.page_size &&
-                   m.held >= 0 && m.held <= a.stride;
-            if (!fine) err |= kErrBatch;
-            fine = fine && sane;
-            if (fine) m.need = a.by_page((int)end + a.page_size - 1);
-        }
-        long long want[2] = {fine ? m.n : 0, fine && m.need > m.held ? m.need - m.held : 0}, all[2];
-        const long long own[2] = {want[0], want[1]};
-        block_scan<2>(want, all, sums);
-        const bool waits = (own[1] > 0 && pages_wanted + want[1] + own[1] > count) ||
-                           (own[0] > 0 && rows_wanted + want[0] + own[0] > a.max_rows);
-        rows_wanted += all[0];
-        pages_wanted += all[1];
-        if (waits) err |= kErrNoRoom;
-        if (!fine || waits) {
-            m.n = 0;
-            m.need = m.held;
-        }
-        long long sum[3] = {m.n, m.need > m.held ? m.need - m.held : 0, m.held > m.need ? m.held - m.need : 0}, tot[3];
-        __syncthreads();  // sums is read
-        block_scan<3>(sum, tot, sums);
-        m.row0 = (int)(rows + sum[0]);
-        m.take = head + taken + sum[1];
-        m.give = (long long)head + count + given + sum[2];
-        rows += tot[0];
-        taken += tot[1];
-        given += tot[2];
-        if (s < a.num_seqs) {
-            a.q_start[s + 1] = m.row0 + m.n;
-            a.kv_len[s] = m.len + m.n;
-            if (m.need != m.held) a.held[s] = m.need;
-        }
-        // pages, then rows: by their thread, or all 32 lanes on one sequence after the other
-        const int pages = abs(m.need - m.held), here = a.rows_here ? m.n : 0;
-        const bool many = pages > kOwn || here > kOwn;
-        if (!many) {
-            move_pages(a, m, 0, 1);
-            if (here) move_rows(a, m, 0, 1);
-        }
-        for (unsigned left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
-            const int k = __ffs(left) - 1;
-            Move o;
-            o.s = __shfl_sync(0xffffffffu, m.s, k);
-            o.held = __shfl_sync(0xffffffffu, m.held, k);
-            o.need = __shfl_sync(0xffffffffu, m.need, k);
-            o.take = __shfl_sync(0xffffffffu, m.take, k);
-            o.give = __shfl_sync(0xffffffffu, m.give, k);
-            o.len = __shfl_sync(0xffffffffu, m.len, k);
-            o.n = __shfl_sync(0xffffffffu, m.n, k);
-            o.row0 = __shfl_sync(0xffffffffu, m.row0, k);
-            move_pages(a, o, lane, 32);
-            __syncwarp();  // the table's new entries are seen by all lanes
-            if (a.rows_here) move_rows(a, o, lane, 32);
-        }
-        __syncthreads();  // sums is read
-    }
-    if (tid == 0) {
-        a.q_start[0] = 0;
-        if (sane) {
-            a.state[0] = (int)((head + taken) % a.num_pages);
-            a.state[1] = (int)min((long long)count - taken + given, (long long)0x7fffffff);
-        }
-    }
-    if (a.err && err) atomicOr(a.err, err);
 }
 
 // The rows' positions and slots, by all SMs: a thread a row; a warp whose rows

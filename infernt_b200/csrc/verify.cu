@@ -29,7 +29,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // What a CTA knows of its part of a row: e is the sum of 2^((l - m) c).
 struct RowPart {
     float m, e;
-    int best;   // the lowest index of m; -1: no number
+    int best;   // of a greedy sequence the lowest index of m; -1: no number
     int flags;  // kBad: a NaN or an element out of range
 };
 constexpr int kBad = 1;
@@ -107,8 +107,10 @@ __device__ __forceinline__ void best_of_warp(float& m, int& at) {
 }
 
 // Block (row, part).  A thread's elements come in 16-byte loads, all of them
-// before the first is used; rows that do not start on 16 bytes start their
+// before the first is used, and before the row's sequence is known, which takes
+// two or three dependent loads; rows that do not start on 16 bytes start their
 // first vector before the row, and the elements outside it are not loaded.
+// HBM-bound.
 template <typename L, bool PROBS>
 __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) {
     constexpr int N = 16 / (int)sizeof(L), VECS = kStatTile / N / kStatThreads;
@@ -116,42 +118,48 @@ __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) 
     __shared__ int at_s[kStatThreads / 32], bad_s;
     pdl_launch_dependents();
     const int r = blockIdx.x, part = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int s = find_seq(a.q_start, a.num_seqs, r);
-    const float t = a.temperature ? a.temperature[s] : 1.0f;
-    if (PROBS && !is_greedy(t)) return;  // only what is drafted, and the row where the sequence stops, are asked for
     const L* row = static_cast<const L*>(a.target) + (long long)r * a.ld;
     const int off = (int)(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(L));
-    const float c = is_greedy(t) ? 0.0f : sharpness(t);
-    if (tid == 0) bad_s = 0;
-    float m = -INFINITY, e = 0.0f;
-    int at = -1;
+    float x[VECS][N], t = 1.0f;
     bool bad = false;
-    for (int tile = 0; tile < a.part; tile += kStatTile) {
-        const int base = part * a.part + tile - off;
-        float x[VECS][N];
+    auto load = [&](int base) {
 #pragma unroll
         for (int i = 0; i < VECS; ++i) {
             const int k = base + (i * kStatThreads + tid) * N;
             if (k >= 0 && k + N <= a.V) {
                 sixteen(row + k, x[i]);
-#pragma unroll
-                for (int j = 0; j < N; ++j) bad |= is_none<PROBS>(x[i][j]);
             } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const bool in = k + j >= 0 && k + j < a.V;
-                    x[i][j] = in ? element(row + k + j) : -INFINITY;
-                    bad |= in && is_none<PROBS>(x[i][j]);
-                }
+                for (int j = 0; j < N; ++j) x[i][j] = k + j >= 0 && k + j < a.V ? element(row + k + j) : -INFINITY;
             }
         }
+    };
+    // only what is drafted, and the row where the sequence stops, are asked of probabilities (but for the greedy)
+    if (!PROBS) load(part * a.part - off);
+    if (a.temperature) t = a.temperature[find_seq(a.q_start, a.num_seqs, r)];
+    const bool greedy = is_greedy(t);
+    if (PROBS) {
+        if (!greedy) return;
+        load(part * a.part - off);
+    }
+    const float c = greedy ? 0.0f : sharpness(t);
+    if (tid == 0) bad_s = 0;
+    float m = -INFINITY, e = 0.0f;
+    int at = -1;
+    for (int tile = 0; tile < a.part; tile += kStatTile) {
+        const int base = part * a.part + tile - off;
+        if (tile) load(base);
         float top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < VECS; ++i)
 #pragma unroll
-            for (int j = 0; j < N; ++j) top = fmaxf(top, x[i][j]);
+            for (int j = 0; j < N; ++j) {
+                top = fmaxf(top, x[i][j]);
+                // (what lies outside the row is -infinity)
+                bad |= PROBS ? !(x[i][j] < INFINITY) || (x[i][j] < 0.0f && x[i][j] > -INFINITY) : !(x[i][j] < INFINITY);
+            }
         const float ref = fmaxf(m, top);
-        if (c > 0.0f && ref > -INFINITY) {
+        if (!greedy && ref > -INFINITY) {
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < VECS; ++i)
@@ -163,26 +171,27 @@ __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) 
                 }
             e = e * (m == -INFINITY ? 0.0f : exp2f((m - ref) * c)) + sum[0] + sum[1];
         }
-        if (top > m) {  // the lowest index of it
-            m = top;
+        if (greedy && top > m) {  // the lowest index of it
 #pragma unroll
             for (int i = VECS - 1; i >= 0; --i)
 #pragma unroll
                 for (int j = N - 1; j >= 0; --j)
                     if (x[i][j] == top) at = base + (i * kStatThreads + tid) * N + j;
         }
+        m = ref;
     }
     // the warps' and then the CTA's
     float wm = m;
-    int wat = at;
-    best_of_warp(wm, wat);
+    best_of_warp(wm, at);
+    if (!greedy) wm = warp_max(m);
     e = warp_sum(m == -INFINITY ? 0.0f : e * exp2f((m - wm) * c));
+    bad = __any_sync(0xffffffffu, bad);
     __syncthreads();
-    if (bad) bad_s = 1;
     if (lane == 0) {
+        if (bad) bad_s = 1;
         m_s[warp] = wm;
         e_s[warp] = e;
-        at_s[warp] = wat;
+        at_s[warp] = at;
     }
     __syncthreads();
     if (warp != 0) return;
@@ -191,6 +200,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) 
     e = lane < kStatThreads / 32 ? e_s[lane] : 0.0f;
     wm = m;
     best_of_warp(wm, at);
+    if (!greedy) wm = warp_max(m);
     e = warp_sum(m == -INFINITY ? 0.0f : e * exp2f((m - wm) * c));
     if (lane == 0) a.parts[(size_t)r * kMostParts + part] = {wm, e, at, bad_s ? kBad : 0};
 }
@@ -241,22 +251,25 @@ __device__ __forceinline__ double exp2_64(double x, const double* table) {
 
 // What becomes of a sequence.
 struct Stop {
-    int token;  // >= 0: the token is known
+    int row;    // where it stops
+    int token;  // the next token: >= 0 known, kDraw, kLargest
     int minus;  // what is subtracted: 1 the draft's distribution, 2 the drafted token alone
-    float m;    // the largest logit of the row where it stops
+    float m;    // the largest logit of that row
     unsigned err;
 };
+constexpr int kDraw = -1, kLargest = -2;  // to be drawn; the row's largest number, to be looked for
 
 // A row's statistics, by a whole warp.
 template <bool PROBS>
-__device__ __forceinline__ RowPart row_stats(const VerifyArgs& a, int r, float c) {
+__device__ __forceinline__ RowPart row_stats(const VerifyArgs& a, int r, float c, bool greedy) {
     const int lane = threadIdx.x & 31;
     RowPart p = {-INFINITY, 0.0f, -1, 0};
     if (lane < a.n_parts) p = a.parts[(size_t)r * kMostParts + lane];
     const float m = p.m;
     best_of_warp(p.m, p.best);
+    if (!greedy) p.m = warp_max(m);
     p.e = warp_sum(m == -INFINITY ? 0.0f : p.e * exp2f((m - p.m) * c));
-    p.flags = __any_sync(0xffffffffu, p.flags & kBad) || p.best < 0 || !(p.m > (PROBS ? 0.0f : -INFINITY)) ? kBad : 0;
+    p.flags = __any_sync(0xffffffffu, p.flags & kBad) || !(p.m > (PROBS ? 0.0f : -INFINITY)) ? kBad : 0;
     return p;
 }
 
@@ -266,91 +279,121 @@ __device__ __forceinline__ float probability(const VerifyArgs& a, int r, int e) 
     const float p = element(static_cast<const L*>(a.target) + (long long)r * a.ld + e);
     return is_none<true>(p) ? -1.0f : p;
 }
+__device__ __forceinline__ float in_unit(float u) { return u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f; }
 
-// A cluster of CTAs a sequence, a slice of the vocabulary each.  In every CTA
-// the warps judge the sequence's rows; then
+// Row r's largest number at its lowest index into out[r] (0 if it has none), by
+// one CTA.  For rows that are no distribution.
+template <typename L>
+__device__ __noinline__ void put_largest(const VerifyArgs& a, int r) {
+    __shared__ float m_s[kDrawWarps];
+    __shared__ int at_s[kDrawWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const L* row = static_cast<const L*>(a.target) + (long long)r * a.ld;
+    float m = -INFINITY;
+    int at = -1;
+    for (int i = tid; i < a.V; i += kDrawThreads) {
+        const float x = element(row + i);
+        if (x > -INFINITY && (at < 0 || argmax_better(x, i, m, at))) {
+            m = x;
+            at = i;
+        }
+    }
+    best_of_warp(m, at);
+    if (lane == 0) {
+        m_s[warp] = m;
+        at_s[warp] = at;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    m = lane < kDrawWarps ? m_s[lane] : -INFINITY;
+    at = lane < kDrawWarps ? at_s[lane] : -1;
+    best_of_warp(m, at);
+    if (lane == 0) a.out[r] = at < 0 ? 0 : at;
+}
+
+// A cluster of CTAs a sequence, a slice of the vocabulary each, and in it a
+// stretch for each warp, in kSubs pieces.  In every CTA the warps judge the
+// sequence's rows; then
 //   Z = sum e_i, and W = sum w_i, over the cluster;
-//   the CTA, and in it the warp, whose part of the sum has u W in it walks
-//   along it.
+//   the CTA, in it the warp, and of its stretch the piece whose part of the sum
+//   has u W in it: that piece is walked along, 32 elements at a time.
 // The weights are computed again in each pass (the logits are in L2): a CTA
-// then needs few registers, and the sequences' waits and sums overlap.
+// then needs few registers, and the sequences' waits and sums overlap.  What it
+// comes to is some 30 operations in 64 bits an element.
+constexpr int kSubs = 16;
+
 template <typename L, bool PROBS>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads) verify_draw(const VerifyArgs a) {
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 4) verify_draw(const VerifyArgs a) {
     __shared__ double table[32], sum_s[3][kDrawWarps], shared_s[3];  // shared_s: what the other CTAs read
+    __shared__ double sub_s[kDrawWarps][kSubs][32];                  // the lanes' sums of the warps' pieces
     __shared__ int first_s;
-    __shared__ Stop stop_s;
+    __shared__ Stop stop_s[kDrawWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x / kCluster;
     const uint32_t rank = cluster_rank();
     if (tid < 32) table[tid] = exp2((double)tid / 32.0);
     if (tid == 0) first_s = 0x7fffffff;
     const int row0 = a.q_start[s], end = a.q_start[s + 1], n = end - row0;
-    pdl_wait();  // verify_rows; of every CTA, so that this kernel's end is the call's end
-    if (row0 < 0 || n < 0 || end > a.num_rows) {
-        if (rank == 0 && tid == 0 && a.err) atomicOr(a.err, kErrBatch);
-        return;  // the whole cluster
-    }
-    if (n == 0) {
-        if (rank == 0 && tid == 0) {
-            a.accepted[s] = 0;
-            if (a.kept) a.kept[s] = a.kv_len[s];
-        }
-        return;
-    }
+    const bool sane = row0 >= 0 && n >= 0 && end <= a.num_rows;
     const float t = a.temperature ? a.temperature[s] : 1.0f;
     const bool greedy = is_greedy(t), stats = !PROBS || greedy;
     const float c = greedy ? 0.0f : sharpness(t);
     const double c64 = greedy ? 0.0 : sharpness64(t);
     __syncthreads();
-    // ---- the first row whose draft does not stand (a warp a row, in turn)
-    for (int i = warp; i < n; i += kDrawWarps) {
-        const int r = row0 + i;
-        if (__any_sync(0xffffffffu, r > *static_cast<volatile int*>(&first_s))) break;
-        bool stands = false;
-        const int d = i + 1 < n ? a.tokens[r + 1] : -1;
-        const bool drafted = d >= 0 && d < a.V;
-        RowPart p = {0.0f, 1.0f, 0, 0};
-        if (stats) p = row_stats<PROBS>(a, r, c);
-        if (greedy) {
-            stands = drafted && d == p.best && !(p.flags & kBad);
-        } else if (drafted && !(p.flags & kBad)) {
-            double pd;
-            if (PROBS) {
-                pd = probability<L>(a, r, d);
-            } else {
-                const float l = element(static_cast<const L*>(a.target) + (long long)r * a.ld + d);
-                pd = exp2_64(((double)l - (double)p.m) * c64, table) / (double)p.e;
+    // ---- the first row whose draft does not stand (a warp a row, in turn); what does not hang on verify_rows first
+    bool waited = false;
+    if (sane)
+        for (int i = warp; i < n; i += kDrawWarps) {
+            const int r = row0 + i;
+            if (waited && __any_sync(0xffffffffu, r > *static_cast<volatile int*>(&first_s))) break;
+            const int d = i + 1 < n ? a.tokens[r + 1] : -1;
+            const bool drafted = d >= 0 && d < a.V;
+            float l = 0.0f, q = 1.0f, u = 0.0f;
+            if (drafted && !greedy) {
+                l = PROBS ? probability<L>(a, r, d) : element(static_cast<const L*>(a.target) + (long long)r * a.ld + d);
+                if (a.draft) q = a.draft[(long long)r * a.draft_ld + d];
+                u = in_unit(a.u[r]);
             }
-            const float q = a.draft ? a.draft[(long long)r * a.draft_ld + d] : 1.0f;
-            float u = a.u[r];
-            u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
-            stands = (double)u * (double)q < pd;
+            if (!waited) pdl_wait();  // verify_rows
+            waited = true;
+            RowPart p = {0.0f, 1.0f, 0, 0};
+            if (stats) p = row_stats<PROBS>(a, r, c, greedy);
+            Stop st = {r, kDraw, 0, p.m, i + 1 < n && !drafted ? (unsigned)kErrToken : 0u};
+            bool stands = false;
+            if (greedy) {
+                stands = drafted && d == p.best && !(p.flags & kBad);
+                st.token = p.best < 0 ? 0 : p.best;
+                if (p.flags & kBad) st.err |= kErrValue;
+            } else if (p.flags & kBad) {
+                st.token = kLargest;
+                st.err |= kErrValue;
+            } else if (drafted) {
+                const double pd = PROBS ? (double)l : exp2_64(((double)l - (double)p.m) * c64, table) / (double)p.e;
+                stands = (double)u * (double)q < pd;
+                st.minus = a.draft ? 1 : 2;
+            }
+            if (!stands) {
+                if (lane == 0) {
+                    stop_s[warp] = st;
+                    atomicMin(&first_s, r);
+                }
+                __syncwarp();
+                break;
+            }
         }
-        if (!stands && lane == 0) atomicMin(&first_s, r);
-        __syncwarp();
-    }
+    if (!waited) pdl_wait();  // of every thread, so that this kernel's end is the call's end
     __syncthreads();
-    // ---- what becomes of the sequence, by one warp
+    if (!sane || n == 0) {  // the whole cluster
+        if (rank == 0 && tid == 0) {
+            if (!sane && a.err) atomicOr(a.err, kErrBatch);
+            if (sane) {
+                a.accepted[s] = 0;
+                if (a.kept) a.kept[s] = a.kv_len[s];
+            }
+        }
+        return;
+    }
     const int stop = first_s;
-    if (warp == 0) {
-        Stop st = {-1, 0, 0.0f, 0u};
-        const int d = stop + 1 < end ? a.tokens[stop + 1] : -1;
-        const bool drafted = d >= 0 && d < a.V;
-        RowPart p = {0.0f, 1.0f, 0, 0};
-        if (stats) p = row_stats<PROBS>(a, stop, c);
-        if (stop + 1 < end && !drafted) st.err |= kErrToken;
-        if (p.flags & kBad) {
-            st.token = p.best < 0 ? 0 : p.best;
-            st.err |= kErrValue;
-        } else if (greedy) {
-            st.token = p.best;
-        } else if (drafted) {
-            st.minus = a.draft ? 1 : 2;
-        }
-        st.m = p.m;
-        if (lane == 0) stop_s = st;
-    }
-    __syncthreads();
-    const Stop st = stop_s;
+    const Stop st = stop_s[(stop - row0) % kDrawWarps];
     if (rank == 0) {
         const int good = stop - row0;
         for (int i = tid; i < n; i += kDrawThreads)
@@ -361,24 +404,43 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
             if (st.token >= 0) a.out[stop] = st.token;
             if (a.err && st.err) atomicOr(a.err, st.err);
         }
+        if (st.token == kLargest) put_largest<L>(a, stop);
     }
-    if (st.token >= 0) return;  // the whole cluster
-    // ---- the draw.  This CTA's slice, and in it the warps' segments of whole groups of 128 elements.
+    if (st.token != kDraw) return;  // the whole cluster
+    // ---- the draw.  This warp's stretch: groups [g0, g1) of 128 elements, `sub` of them a piece.
     const L* row = static_cast<const L*>(a.target) + (long long)stop * a.ld;
     const float* draft = a.draft ? a.draft + (long long)stop * a.draft_ld : nullptr;
     const int groups = (a.V + 127) / 128, per = (groups + kCluster * kDrawWarps - 1) / (kCluster * kDrawWarps);
-    const int g0 = ((int)rank * kDrawWarps + warp) * per, g1 = min(groups, g0 + per);
+    const int sub = (per + kSubs - 1) / kSubs;
+    const int g0 = min(groups, ((int)rank * kDrawWarps + warp) * per), g1 = min(groups, g0 + per);
     const int d = st.minus == 2 ? a.tokens[stop + 1] : -1;
     const double cm = c64 * (double)st.m;
     int minus = st.minus;
     bool bad = false;
-    auto weight = [&](int i) {  // e_i, or p_i
-        const float l = element(row + i);
+    double z = 1.0;
+    constexpr float kOutside = PROBS ? 0.0f : -INFINITY;  // has no weight
+    auto weight = [&](float l) {  // e, or p
         if (!PROBS) return exp2_64(fma((double)l, c64, -cm), table);
         bad |= is_none<true>(l);
         return (double)l;
     };
-    double z = 1.0;
+    auto left = [&](int i, float l, float q) {  // the weight that is drawn from
+        double w = weight(l);
+        if (!PROBS) w *= z;
+        if (minus == 1) w -= fabsf(q) < INFINITY ? (double)q : INFINITY;
+        if (minus == 2 && i == d) w = 0.0;
+        return w > 0.0 ? w : 0.0;
+    };
+    // four elements of a group a lane
+    auto get = [&](int g, float (&l)[4], float (&q)[4], bool draft_too) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = g * 128 + 32 * j + lane;
+            const bool in = g < g1 && i < a.V;
+            l[j] = in ? element(row + i) : kOutside;
+            q[j] = draft_too && in ? __ldg(draft + i) : 0.0f;
+        }
+    };
     // the sum over the CTA's warps into its shared_s[slot], then over the cluster, both in order
     auto over_cluster = [&](double v, int slot) {
         v = warp_sum64(v);
@@ -394,139 +456,99 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads)
         for (int k = 0; k < kCluster; ++k) x += peer_double(&shared_s[slot], k);
         return x;
     };
-    auto left = [&](int i, double e) {  // the weight that is drawn from
-        double w = PROBS ? e : e * z;
-        if (minus == 1) {
-            const float q = draft[i];
-            w -= fabsf(q) < INFINITY ? (double)q : INFINITY;
-        }
-        if (minus == 2 && i == d) w = 0.0;
-        return w > 0.0 ? w : 0.0;
-    };
     if (!PROBS) {
         double v = 0.0;
-        for (int g = g0; g < g1; ++g)
+        float l[4], q[4], next[4];
+        get(g0, l, q, false);
+        for (int g = g0; g < g1; ++g) {
+            get(g + 1, next, q, false);
+            v += (weight(l[0]) + weight(l[1])) + (weight(l[2]) + weight(l[3]));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = g * 128 + 32 * j + lane;
-                if (i < a.V) v += weight(i);
-            }
+            for (int j = 0; j < 4; ++j) l[j] = next[j];
+        }
         z = 1.0 / over_cluster(v, 0);
     }
-    double mine = 0.0, total = 0.0;
+    double total = 0.0;
     for (int pass = 0; pass < 2; ++pass) {
-        mine = 0.0;
-        for (int g = g0; g < g1; ++g)
+        double mine = 0.0, piece = 0.0;
+        float l[4], q[4], next[4], next_q[4];
+        get(g0, l, q, minus == 1);
+        for (int g = g0, k = 0; k < kSubs; ++k) {
+            for (const int stop_g = min(g1, g + sub); g < stop_g; ++g) {
+                get(g + 1, next, next_q, minus == 1);
+                const int i = g * 128 + lane;
+                piece += (left(i, l[0], q[0]) + left(i + 32, l[1], q[1])) + (left(i + 64, l[2], q[2]) + left(i + 96, l[3], q[3]));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = g * 128 + 32 * j + lane;
-                if (i < a.V) mine += left(i, weight(i));
+                for (int j = 0; j < 4; ++j) {
+                    l[j] = next[j];
+                    q[j] = next_q[j];
+                }
             }
+            sub_s[warp][k][lane] = piece;
+            mine += piece;
+            piece = 0.0;
+        }
         total = over_cluster(mine, 1);
         if (total > 0.0 || minus == 0) break;
         minus = 0;  // nothing is left: from p itself
         cluster_sync();  // shared_s is read
     }
-    // a probability that is none, anywhere in the row
-    double none = 0.0;
-    if (PROBS) none = over_cluster(bad ? 1.0 : 0.0, 2);
-    if (PROBS && (none > 0.0 || !(total > 0.0))) {
-        // its largest number, by the first CTA
-        if (rank == 0) {
-            float m = -INFINITY;
-            int at = -1;
-            for (int i = tid; i < a.V; i += kDrawThreads) {
-                const float x = element(row + i);
-                if (x == x && (at < 0 || argmax_better(x, i, m, at))) {
-                    m = x;
-                    at = i;
-                }
+    if (PROBS) {
+        // a probability that is none, anywhere in the row
+        if (over_cluster(bad ? 1.0 : 0.0, 2) > 0.0 || !(total > 0.0)) {
+            if (rank == 0) {
+                put_largest<L>(a, stop);
+                if (tid == 0 && a.err) atomicOr(a.err, kErrValue);
             }
-            best_of_warp(m, at);
-            __syncthreads();
-            __shared__ float bm_s[kDrawWarps];
-            __shared__ int bi_s[kDrawWarps];
-            if (lane == 0) {
-                bm_s[warp] = m;
-                bi_s[warp] = at;
-            }
-            __syncthreads();
-            if (warp == 0) {
-                m = lane < kDrawWarps ? bm_s[lane] : -INFINITY;
-                at = lane < kDrawWarps ? bi_s[lane] : -1;
-                best_of_warp(m, at);
-                if (lane == 0) {
-                    a.out[stop] = at < 0 ? 0 : at;
-                    if (a.err) atomicOr(a.err, kErrValue);
-                }
-            }
+            cluster_sync();  // no CTA leaves while others read its sums
+            return;
         }
-        cluster_sync();  // no CTA leaves while others read its sums
-        return;
     }
-    // ---- the CTA and the warp that have u' total in their part of the sum
-    float uf = a.u[end - 1];
-    uf = uf >= 0.0f ? fminf(uf, 0.99999994f) : 0.0f;
-    const double goal = (double)uf * total;
+    // ---- of n parts, the one that has the goal in it (by the rounding of the sums alone, none: the last that has any)
+    const double goal = (double)in_unit(a.u[end - 1]) * total;
     double before = 0.0;
-    int owner = -1, last_some = 0;
-    double owner_before = 0.0, last_before = 0.0;
-    for (int k = 0; k < kCluster; ++k) {
-        const double x = peer_double(&shared_s[1], k);
-        if (x > 0.0) {
-            last_some = k;
-            last_before = before;
-        }
-        if (owner < 0 && before + x > goal) {
-            owner = k;
-            owner_before = before;
-        }
-        before += x;
-    }
-    if (owner < 0) {  // by the rounding of the sums alone: the last that has any
-        owner = last_some;
-        owner_before = last_before;
-    }
-    if ((int)rank == owner) {
-        before = owner_before;
-        int w_owner = -1, w_last = 0;
-        double wb = 0.0, wb_last = 0.0;
-        for (int w = 0; w < kDrawWarps; ++w) {
-            const double x = sum_s[1][w];
+    auto find = [&](int parts, auto part) {
+        int owner = -1, some = 0;
+        double at = before, at_some = before, sum = before;
+        for (int k = 0; k < parts; ++k) {
+            const double x = part(k);
             if (x > 0.0) {
-                w_last = w;
-                wb_last = before;
+                some = k;
+                at_some = sum;
             }
-            if (w_owner < 0 && before + x > goal) {
-                w_owner = w;
-                wb = before;
+            if (owner < 0 && sum + x > goal) {
+                owner = k;
+                at = sum;
             }
-            before += x;
+            sum += x;
         }
-        if (w_owner < 0) {
-            w_owner = w_last;
-            wb = wb_last;
-        }
-        if (warp == w_owner) {
-            before = wb;
-            int found = -1, some = 0;
-            for (int i0 = g0 * 128; i0 < min(g1 * 128, a.V) && found < 0; i0 += 32) {
-                const int i = i0 + lane;
-                const double w = i < a.V ? left(i, weight(i)) : 0.0;
-                double x = w;
+        before = owner < 0 ? at_some : at;
+        return owner < 0 ? some : owner;
+    };
+    if (find(kCluster, [&](int k) { return peer_double(&shared_s[1], k); }) == (int)rank &&
+        find(kDrawWarps, [&](int w) { return sum_s[1][w]; }) == warp) {
+        double x = 0.0;  // of piece `lane`
+        if (lane < kSubs)
+            for (int k = 0; k < 32; ++k) x += sub_s[warp][lane][(k + lane) % 32];
+        const int piece = find(kSubs, [&](int k) { return __shfl_sync(0xffffffffu, x, k); });
+        const int first = (g0 + piece * sub) * 128, last = min(min(g1, g0 + (piece + 1) * sub) * 128, a.V);
+        int found = -1, some = min(first, a.V - 1);
+        for (int i0 = first; i0 < last && found < 0; i0 += 32) {
+            const int i = i0 + lane;
+            const double w = i < last ? left(i, element(row + i), minus == 1 ? draft[i] : 0.0f) : 0.0;
+            double upto = w;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xffffffffu, x, o);
-                    if (lane >= o) x += y;
-                }
-                const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && before + x > goal);
-                const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
-                if (past) found = i0 + __ffs(past) - 1;
-                if (any) some = i0 + 31 - __clz(any);
-                before += __shfl_sync(0xffffffffu, x, 31);
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
             }
-            if (lane == 0) a.out[stop] = found >= 0 ? found : some;
+            const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && before + upto > goal);
+            const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
+            if (past) found = i0 + __ffs(past) - 1;
+            if (any) some = i0 + 31 - __clz(any);
+            before += __shfl_sync(0xffffffffu, upto, 31);
         }
+        if (lane == 0) a.out[stop] = found >= 0 ? found : some;
     }
     cluster_sync();  // no CTA leaves while others read its sums
 }
