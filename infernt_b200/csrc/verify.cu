@@ -51,14 +51,9 @@ struct VerifyArgs {
     unsigned* err;
 };
 
-template <typename L>
-__device__ __forceinline__ float element(const L* p) {
-    return to_f32(*p);
-}
-template <>
-__device__ __forceinline__ float element<__half>(const __half* p) {
-    return __half2float(*p);
-}
+__device__ __forceinline__ float element(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float element(const __nv_bfloat16* p) { return __bfloat162float(__ldg(p)); }
+__device__ __forceinline__ float element(const __half* p) { return __half2float(__ldg(p)); }
 
 __device__ __forceinline__ bool is_greedy(float t) { return !(t > 0.0f); }
 // log2(e) / T; an infinite T would make 0 of -infinity, one near 0 infinity of 0
@@ -231,20 +226,28 @@ __device__ __forceinline__ double warp_sum64(double v) {
     return v;
 }
 
-// 2^x for x <= 0, to about 2e-15: x = (32 n + j) / 32 + g, |g| <= 1 / 64, so
-// 2^x = 2^n 2^(j / 32) 2^g, the last by its Taylor series to the fifth power
-// (the sixth is below (ln 2 / 64)^6 / 720 = 2e-15), the middle one of a table.
+// 2^x for x <= 0 above -1000, to about 2e-15: x = (32 n + j) / 32 + g, |g| <= 1 /
+// 64, so 2^x = 2^n 2^(j / 32) 2^g, the last by its Taylor series to the fifth
+// power (the sixth is below (ln 2 / 64)^6 / 720 = 2e-15), the middle one of a
+// table.  The constants are in constant memory, where the operations take them
+// from without a move.
+struct Exp2Constants {
+    double big, back;  // 1.5 x 2^52 rounds 32 x to a whole number in its low bits
+    double c[6];       // (ln 2)^k / k!
+};
+__constant__ Exp2Constants kExp2 = {6755399441055744.0,
+                                    -1.0 / 32.0,
+                                    {1.0, 0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995,
+                                     0.00961812910762847716, 0.00133335581464284434}};
 __device__ __forceinline__ double exp2_64(double x, const double* table) {
-    if (!(x > -1000.0)) return 0.0;  // -infinity too
-    const double big = 6755399441055744.0;  // 1.5 x 2^52: rounds 32 x to a whole number in its low bits
-    const double t = fma(x, 32.0, big);
+    const double t = fma(x, 32.0, kExp2.big);
     const int k = __double2loint(t);
-    const double g = fma(t - big, -1.0 / 32.0, x) * 0.69314718055994530942;
-    double p = fma(g, 1.0 / 120.0, 1.0 / 24.0);
-    p = fma(p, g, 1.0 / 6.0);
-    p = fma(p, g, 0.5);
-    p = fma(p, g, 1.0);
-    p = fma(p, g, 1.0);
+    const double g = fma(t - kExp2.big, kExp2.back, x);
+    double p = fma(g, kExp2.c[5], kExp2.c[4]);
+    p = fma(p, g, kExp2.c[3]);
+    p = fma(p, g, kExp2.c[2]);
+    p = fma(p, g, kExp2.c[1]);
+    p = fma(p, g, kExp2.c[0]);
     const double y = p * table[k & 31];
     return __hiloint2double(__double2hiint(y) + (k >> 5) * (1 << 20), __double2loint(y));
 }
@@ -367,7 +370,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
                 st.token = kLargest;
                 st.err |= kErrValue;
             } else if (drafted) {
-                const double pd = PROBS ? (double)l : exp2_64(((double)l - (double)p.m) * c64, table) / (double)p.e;
+                const double x = ((double)l - (double)p.m) * c64;
+                const double pd = PROBS ? (double)l : x > -1000.0 ? exp2_64(x, table) / (double)p.e : 0.0;
                 stands = (double)u * (double)q < pd;
                 st.minus = a.draft ? 1 : 2;
             }
@@ -414,15 +418,20 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
     const int sub = (per + kSubs - 1) / kSubs;
     const int g0 = min(groups, ((int)rank * kDrawWarps + warp) * per), g1 = min(groups, g0 + per);
     const int d = st.minus == 2 ? a.tokens[stop + 1] : -1;
-    const double cm = c64 * (double)st.m;
+    const double cm = -c64 * (double)st.m;
+    // logits from which on a weight is not 0: 2^-1000 of the largest, and never -infinity
+    const float least = fmaxf((float)((double)st.m - 1000.0 / c64), -3.4028235e38f);
     int minus = st.minus;
     bool bad = false;
     double z = 1.0;
     constexpr float kOutside = PROBS ? 0.0f : -INFINITY;  // has no weight
-    auto weight = [&](float l) {  // e, or p
-        if (!PROBS) return exp2_64(fma((double)l, c64, -cm), table);
-        bad |= is_none<true>(l);
-        return (double)l;
+    auto weight = [&](float l) {                          // e, or p
+        if (PROBS) {
+            bad |= is_none<true>(l);
+            return (double)l;
+        }
+        const double y = exp2_64(fma((double)l, c64, cm), table);
+        return l >= least ? y : 0.0;
     };
     auto left = [&](int i, float l, float q) {  // the weight that is drawn from
         double w = weight(l);
@@ -431,14 +440,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
         if (minus == 2 && i == d) w = 0.0;
         return w > 0.0 ? w : 0.0;
     };
-    // four elements of a group a lane
-    auto get = [&](int g, float (&l)[4], float (&q)[4], bool draft_too) {
+    // four elements of a group a lane; the last group's may lie behind the row
+    auto get = [&](const auto* from, int g, float none, float (&x)[4]) {
+        const auto* at = from + (long long)g * 128 + lane;
+        if (g < g1 && g * 128 + 128 <= a.V) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = g * 128 + 32 * j + lane;
-            const bool in = g < g1 && i < a.V;
-            l[j] = in ? element(row + i) : kOutside;
-            q[j] = draft_too && in ? __ldg(draft + i) : 0.0f;
+            for (int j = 0; j < 4; ++j) x[j] = element(at + 32 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = g < g1 && g * 128 + 32 * j + lane < a.V ? element(at + 32 * j) : none;
         }
     };
     // the sum over the CTA's warps into its shared_s[slot], then over the cluster, both in order
@@ -458,10 +468,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
     };
     if (!PROBS) {
         double v = 0.0;
-        float l[4], q[4], next[4];
-        get(g0, l, q, false);
+        float l[4], next[4];
+        get(row, g0, kOutside, l);
         for (int g = g0; g < g1; ++g) {
-            get(g + 1, next, q, false);
+            get(row, g + 1, kOutside, next);
             v += (weight(l[0]) + weight(l[1])) + (weight(l[2]) + weight(l[3]));
 #pragma unroll
             for (int j = 0; j < 4; ++j) l[j] = next[j];
@@ -470,12 +480,15 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
     }
     double total = 0.0;
     for (int pass = 0; pass < 2; ++pass) {
-        double mine = 0.0, piece = 0.0;
-        float l[4], q[4], next[4], next_q[4];
-        get(g0, l, q, minus == 1);
+        double mine = 0.0;
+        float l[4], q[4] = {0.0f, 0.0f, 0.0f, 0.0f}, next[4], next_q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        get(row, g0, kOutside, l);
+        if (minus == 1) get(draft, g0, 0.0f, q);
         for (int g = g0, k = 0; k < kSubs; ++k) {
+            double piece = 0.0;
             for (const int stop_g = min(g1, g + sub); g < stop_g; ++g) {
-                get(g + 1, next, next_q, minus == 1);
+                get(row, g + 1, kOutside, next);
+                if (minus == 1) get(draft, g + 1, 0.0f, next_q);
                 const int i = g * 128 + lane;
                 piece += (left(i, l[0], q[0]) + left(i + 32, l[1], q[1])) + (left(i + 64, l[2], q[2]) + left(i + 96, l[3], q[3]));
 #pragma unroll
@@ -486,7 +499,6 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
             }
             sub_s[warp][k][lane] = piece;
             mine += piece;
-            piece = 0.0;
         }
         total = over_cluster(mine, 1);
         if (total > 0.0 || minus == 0) break;
