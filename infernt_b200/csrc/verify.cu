@@ -13,10 +13,11 @@
 // u' sum w where there are 10^5 tokens, so what the draw is made of (Z, the
 // weights, their sums) is in 64 bits; acceptance is one comparison a row, and
 // its Z a sum in FP32.
+#include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "paged.cuh"
-#include "sample.cuh"
 
 namespace infernt {
 namespace {
@@ -48,6 +49,7 @@ struct VerifyArgs {
     int* accepted;
     RowPart* parts;  // [num_rows][kMostParts]
     int num_seqs, num_rows, V, n_parts, part;  // part: elements of one
+    int cluster;                               // CTAs that draw for a sequence
     unsigned* err;
 };
 
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) 
 // ------------------------------------------------------------------- draw
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr int kCluster = 8;
+constexpr int kDrawPerSm = 3;
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -228,8 +230,9 @@ __device__ __forceinline__ double warp_sum64(double v) {
 
 // 2^x for x <= 0 above -1000, to about 2e-15: x = (32 n + j) / 32 + g, |g| <= 1 /
 // 64, so 2^x = 2^n 2^(j / 32) 2^g, the last by its Taylor series to the fifth
-// power (the sixth is below (ln 2 / 64)^6 / 720 = 2e-15), the middle one of a
-// table.  The constants are in constant memory, where the operations take them
+// power (the sixth is below (ln 2 / 64)^6 / 720 = 2e-15), the middle one of the
+// 32 roots (in shared memory; from lane to lane by shuffles a call took 3 us
+// more).  The constants are in constant memory, where the operations take them
 // from without a move.
 struct Exp2Constants {
     double big, back;  // 1.5 x 2^52 rounds 32 x to a whole number in its low bits
@@ -239,7 +242,7 @@ __constant__ Exp2Constants kExp2 = {6755399441055744.0,
                                     -1.0 / 32.0,
                                     {1.0, 0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995,
                                      0.00961812910762847716, 0.00133335581464284434}};
-__device__ __forceinline__ double exp2_64(double x, const double* table) {
+__device__ __forceinline__ double exp2_64(double x, const double* roots) {
     const double t = fma(x, 32.0, kExp2.big);
     const int k = __double2loint(t);
     const double g = fma(t - kExp2.big, kExp2.back, x);
@@ -248,7 +251,7 @@ __device__ __forceinline__ double exp2_64(double x, const double* table) {
     p = fma(p, g, kExp2.c[2]);
     p = fma(p, g, kExp2.c[1]);
     p = fma(p, g, kExp2.c[0]);
-    const double y = p * table[k & 31];
+    const double y = p * roots[k & 31];
     return __hiloint2double(__double2hiint(y) + (k >> 5) * (1 << 20), __double2loint(y));
 }
 
@@ -284,17 +287,16 @@ __device__ __forceinline__ float probability(const VerifyArgs& a, int r, int e) 
 }
 __device__ __forceinline__ float in_unit(float u) { return u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f; }
 
-// Row r's largest number at its lowest index into out[r] (0 if it has none), by
+// A row's largest number at its lowest index into *out (0 if it has none), by
 // one CTA.  For rows that are no distribution.
 template <typename L>
-__device__ __noinline__ void put_largest(const VerifyArgs& a, int r) {
+__device__ __noinline__ void put_largest(const L* row, int V, int* out) {
     __shared__ float m_s[kDrawWarps];
     __shared__ int at_s[kDrawWarps];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const L* row = static_cast<const L*>(a.target) + (long long)r * a.ld;
     float m = -INFINITY;
     int at = -1;
-    for (int i = tid; i < a.V; i += kDrawThreads) {
+    for (int i = tid; i < V; i += kDrawThreads) {
         const float x = element(row + i);
         if (x > -INFINITY && (at < 0 || argmax_better(x, i, m, at))) {
             m = x;
@@ -311,7 +313,7 @@ __device__ __noinline__ void put_largest(const VerifyArgs& a, int r) {
     m = lane < kDrawWarps ? m_s[lane] : -INFINITY;
     at = lane < kDrawWarps ? at_s[lane] : -1;
     best_of_warp(m, at);
-    if (lane == 0) a.out[r] = at < 0 ? 0 : at;
+    if (lane == 0) *out = at < 0 ? 0 : at;
 }
 
 // A cluster of CTAs a sequence, a slice of the vocabulary each, and in it a
@@ -320,20 +322,24 @@ __device__ __noinline__ void put_largest(const VerifyArgs& a, int r) {
 //   Z = sum e_i, and W = sum w_i, over the cluster;
 //   the CTA, in it the warp, and of its stretch the piece whose part of the sum
 //   has u W in it: that piece is walked along, 32 elements at a time.
-// The weights are computed again in each pass (the logits are in L2): a CTA
-// then needs few registers, and the sequences' waits and sums overlap.  What it
-// comes to is some 30 operations in 64 bits an element.
+// The weights are computed again in each pass (the logits are in L2): some 25
+// operations in 64 bits an element, each waiting for the one before, so a lane
+// has eight elements on the way.  64 sequences that stop, 128256 tokens: 38 us
+// (of 14 that the operations take where none waits); three CTAs an SM with 80
+// registers a thread, four with 64 took 45.
 constexpr int kSubs = 16;
+constexpr int kEach = 8;  // elements that a lane has at once
+constexpr int kGroup = 32 * kEach;
 
 template <typename L, bool PROBS>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads, 4) verify_draw(const VerifyArgs a) {
-    __shared__ double table[32], sum_s[3][kDrawWarps], shared_s[3];  // shared_s: what the other CTAs read
-    __shared__ double sub_s[kDrawWarps][kSubs][32];                  // the lanes' sums of the warps' pieces
+__global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __grid_constant__ VerifyArgs a) {
+    __shared__ double roots[32], sum_s[3][kDrawWarps], shared_s[3];  // shared_s: what the other CTAs read
+    __shared__ double sub_s[kDrawWarps][kSubs][32];       // the lanes' sums of the warps' pieces
     __shared__ int first_s;
     __shared__ Stop stop_s[kDrawWarps];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x / kCluster;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, s = blockIdx.x / a.cluster;
     const uint32_t rank = cluster_rank();
-    if (tid < 32) table[tid] = exp2((double)tid / 32.0);
+    if (tid < 32) roots[tid] = exp2((double)tid / 32.0);
     if (tid == 0) first_s = 0x7fffffff;
     const int row0 = a.q_start[s], end = a.q_start[s + 1], n = end - row0;
     const bool sane = row0 >= 0 && n >= 0 && end <= a.num_rows;
@@ -371,7 +377,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
                 st.err |= kErrValue;
             } else if (drafted) {
                 const double x = ((double)l - (double)p.m) * c64;
-                const double pd = PROBS ? (double)l : x > -1000.0 ? exp2_64(x, table) / (double)p.e : 0.0;
+                const double pd = PROBS ? (double)l : x > -1000.0 ? exp2_64(x, roots) / (double)p.e : 0.0;
                 stands = (double)u * (double)q < pd;
                 st.minus = a.draft ? 1 : 2;
             }
@@ -408,47 +414,48 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
             if (st.token >= 0) a.out[stop] = st.token;
             if (a.err && st.err) atomicOr(a.err, st.err);
         }
-        if (st.token == kLargest) put_largest<L>(a, stop);
+        if (st.token == kLargest)
+            put_largest<L>(static_cast<const L*>(a.target) + (long long)stop * a.ld, a.V, a.out + stop);
     }
     if (st.token != kDraw) return;  // the whole cluster
-    // ---- the draw.  This warp's stretch: groups [g0, g1) of 128 elements, `sub` of them a piece.
+    // ---- the draw.  This warp's stretch: groups [g0, g1) of kGroup elements, `sub` of them a piece.
     const L* row = static_cast<const L*>(a.target) + (long long)stop * a.ld;
     const float* draft = a.draft ? a.draft + (long long)stop * a.draft_ld : nullptr;
-    const int groups = (a.V + 127) / 128, per = (groups + kCluster * kDrawWarps - 1) / (kCluster * kDrawWarps);
+    const int groups = (a.V + kGroup - 1) / kGroup, per = (groups + a.cluster * kDrawWarps - 1) / (a.cluster * kDrawWarps);
     const int sub = (per + kSubs - 1) / kSubs;
     const int g0 = min(groups, ((int)rank * kDrawWarps + warp) * per), g1 = min(groups, g0 + per);
     const int d = st.minus == 2 ? a.tokens[stop + 1] : -1;
     const double cm = -c64 * (double)st.m;
-    // logits from which on a weight is not 0: 2^-1000 of the largest, and never -infinity
-    const float least = fmaxf((float)((double)st.m - 1000.0 / c64), -3.4028235e38f);
-    int minus = st.minus;
+    // Logits are held to 2^-1000 of the largest, and weights up to 2^-990 are 0: those of tokens that are not allowed.
+    const float least = fmaxf((float)((double)st.m - 999.0 / c64), -3.4028235e38f);
+    constexpr double kLeastWeight = PROBS ? 0.0 : 9.555938177272168e-299;  // 2^-990
     bool bad = false;
     double z = 1.0;
     constexpr float kOutside = PROBS ? 0.0f : -INFINITY;  // has no weight
     auto weight = [&](float l) {                          // e, or p
-        if (PROBS) {
-            bad |= is_none<true>(l);
-            return (double)l;
-        }
-        const double y = exp2_64(fma((double)l, c64, cm), table);
-        return l >= least ? y : 0.0;
+        if (!PROBS) return exp2_64(fma((double)fmaxf(l, least), c64, cm), roots);
+        bad |= is_none<true>(l);
+        return (double)l;
     };
-    auto left = [&](int i, float l, float q) {  // the weight that is drawn from
+    // the weight that is drawn from; minus as in Stop
+    auto left = [&](auto minus, int i, float l, float q) {
         double w = weight(l);
-        if (!PROBS) w *= z;
-        if (minus == 1) w -= fabsf(q) < INFINITY ? (double)q : INFINITY;
-        if (minus == 2 && i == d) w = 0.0;
-        return w > 0.0 ? w : 0.0;
+        if (decltype(minus)::value == 1) {
+            w = fma(w, z, -(double)(fabsf(q) < INFINITY ? q : 3.0e38f));
+        } else if (!PROBS) {
+            w *= z;
+        }
+        return w > kLeastWeight && !(decltype(minus)::value == 2 && i == d) ? w : 0.0;
     };
-    // four elements of a group a lane; the last group's may lie behind the row
-    auto get = [&](const auto* from, int g, float none, float (&x)[4]) {
-        const auto* at = from + (long long)g * 128 + lane;
-        if (g < g1 && g * 128 + 128 <= a.V) {
+    // a group, kEach elements a lane; the last one's may lie behind the row
+    auto get = [&](const auto* from, int g, float none, float (&x)[kEach]) {
+        const auto* at = from + (long long)g * kGroup + lane;
+        if (g * kGroup + kGroup <= a.V) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = element(at + 32 * j);
+            for (int j = 0; j < kEach; ++j) x[j] = element(at + 32 * j);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = g < g1 && g * 128 + 32 * j + lane < a.V ? element(at + 32 * j) : none;
+            for (int j = 0; j < kEach; ++j) x[j] = g * kGroup + 32 * j + lane < a.V ? element(at + 32 * j) : none;
         }
     };
     // the sum over the CTA's warps into its shared_s[slot], then over the cluster, both in order
@@ -463,53 +470,54 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
         }
         cluster_sync();
         double x = 0.0;
-        for (int k = 0; k < kCluster; ++k) x += peer_double(&shared_s[slot], k);
+        for (int k = 0; k < a.cluster; ++k) x += peer_double(&shared_s[slot], k);
         return x;
     };
     if (!PROBS) {
         double v = 0.0;
-        float l[4], next[4];
-        get(row, g0, kOutside, l);
         for (int g = g0; g < g1; ++g) {
-            get(row, g + 1, kOutside, next);
-            v += (weight(l[0]) + weight(l[1])) + (weight(l[2]) + weight(l[3]));
+            float l[kEach];
+            get(row, g, kOutside, l);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) l[j] = next[j];
+            for (int j = 0; j < kEach; j += 2) v += weight(l[j]) + weight(l[j + 1]);
         }
         z = 1.0 / over_cluster(v, 0);
     }
-    double total = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
+    // this warp's pieces; their sum
+    auto pieces = [&](auto minus) {
         double mine = 0.0;
-        float l[4], q[4] = {0.0f, 0.0f, 0.0f, 0.0f}, next[4], next_q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        get(row, g0, kOutside, l);
-        if (minus == 1) get(draft, g0, 0.0f, q);
         for (int g = g0, k = 0; k < kSubs; ++k) {
             double piece = 0.0;
             for (const int stop_g = min(g1, g + sub); g < stop_g; ++g) {
-                get(row, g + 1, kOutside, next);
-                if (minus == 1) get(draft, g + 1, 0.0f, next_q);
-                const int i = g * 128 + lane;
-                piece += (left(i, l[0], q[0]) + left(i + 32, l[1], q[1])) + (left(i + 64, l[2], q[2]) + left(i + 96, l[3], q[3]));
+                float l[kEach], q[kEach];
+                get(row, g, kOutside, l);
+                if (decltype(minus)::value == 1) get(draft, g, 0.0f, q);
+                const int i = g * kGroup + lane;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    l[j] = next[j];
-                    q[j] = next_q[j];
-                }
+                for (int j = 0; j < kEach; j += 2)
+                    piece += left(minus, i + 32 * j, l[j], q[j]) + left(minus, i + 32 * j + 32, l[j + 1], q[j + 1]);
             }
             sub_s[warp][k][lane] = piece;
             mine += piece;
         }
-        total = over_cluster(mine, 1);
-        if (total > 0.0 || minus == 0) break;
-        minus = 0;  // nothing is left: from p itself
+        return mine;
+    };
+    using std::integral_constant;
+    int minus = st.minus;
+    double total = over_cluster(minus == 1   ? pieces(integral_constant<int, 1>())
+                                : minus == 2 ? pieces(integral_constant<int, 2>())
+                                             : pieces(integral_constant<int, 0>()),
+                                1);
+    if (minus && !(total > 0.0)) {  // nothing is left: from p itself
+        minus = 0;
         cluster_sync();  // shared_s is read
+        total = over_cluster(pieces(integral_constant<int, 0>()), 1);
     }
     if (PROBS) {
         // a probability that is none, anywhere in the row
         if (over_cluster(bad ? 1.0 : 0.0, 2) > 0.0 || !(total > 0.0)) {
             if (rank == 0) {
-                put_largest<L>(a, stop);
+                put_largest<L>(row, a.V, a.out + stop);
                 if (tid == 0 && a.err) atomicOr(a.err, kErrValue);
             }
             cluster_sync();  // no CTA leaves while others read its sums
@@ -537,17 +545,20 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDrawThreads,
         before = owner < 0 ? at_some : at;
         return owner < 0 ? some : owner;
     };
-    if (find(kCluster, [&](int k) { return peer_double(&shared_s[1], k); }) == (int)rank &&
+    if (find(a.cluster, [&](int k) { return peer_double(&shared_s[1], k); }) == (int)rank &&
         find(kDrawWarps, [&](int w) { return sum_s[1][w]; }) == warp) {
         double x = 0.0;  // of piece `lane`
         if (lane < kSubs)
             for (int k = 0; k < 32; ++k) x += sub_s[warp][lane][(k + lane) % 32];
         const int piece = find(kSubs, [&](int k) { return __shfl_sync(0xffffffffu, x, k); });
-        const int first = (g0 + piece * sub) * 128, last = min(min(g1, g0 + (piece + 1) * sub) * 128, a.V);
+        const int first = (g0 + piece * sub) * kGroup, last = min(min(g1, g0 + (piece + 1) * sub) * kGroup, a.V);
         int found = -1, some = min(first, a.V - 1);
         for (int i0 = first; i0 < last && found < 0; i0 += 32) {
             const int i = i0 + lane;
-            const double w = i < last ? left(i, element(row + i), minus == 1 ? draft[i] : 0.0f) : 0.0;
+            const float l = i < last ? element(row + i) : kOutside, q = minus == 1 && i < last ? draft[i] : 0.0f;
+            const double w = minus == 1   ? left(integral_constant<int, 1>(), i, l, q)
+                             : minus == 2 ? left(integral_constant<int, 2>(), i, l, 0.0f)
+                                          : left(integral_constant<int, 0>(), i, l, 0.0f);
             double upto = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -572,14 +583,17 @@ int launch(const VerifyArgs& a, cudaStream_t st) {
         INFERNT_CUDA_TRY(cudaGetLastError());
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.num_seqs * kCluster);
+    cfg.gridDim = dim3(a.num_seqs * a.cluster);
     cfg.blockDim = dim3(kDrawThreads);
     cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = a.num_rows > 0 ? 1 : 0;  // without rows there is no kernel of this call to wait for
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = a.cluster;
+    attrs[0].val.clusterDim.y = attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = a.num_rows > 0 ? 2 : 1;  // without rows there is no kernel of this call to wait for
     INFERNT_CUDA_TRY(cudaLaunchKernelEx(&cfg, verify_draw<L, PROBS>, static_cast<const VerifyArgs>(a)));
     return INFERNT_OK;
 }
@@ -647,6 +661,8 @@ extern "C" int infernt_verify_drafts(int* out_tokens, int* accepted, const void*
     const long long tiles = ((long long)vocab_size + 7 + kStatTile - 1) / kStatTile;
     a.part = (int)((tiles + kMostParts - 1) / kMostParts) * kStatTile;
     a.n_parts = (int)(((long long)vocab_size + 7 + a.part - 1) / a.part);
+    // as many CTAs a sequence as are sure to run at once: a cluster that has to wait for room waits for another's end
+    a.cluster = std::max(1, std::min(8, kDrawPerSm * sm_count() / num_seqs));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool p = probabilities != 0;
     if (target_dtype == INFERNT_DTYPE_F32) return p ? launch<float, true>(a, st) : launch<float, false>(a, st);
