@@ -23,27 +23,34 @@ int check_paged_cache4(const char* op, const infernt_paged_cache4* c) {
 
 namespace {
 
-// The largest and least of some values and 0, and whether all are numbers of T.
+// The largest and least of some values and 0; NaN where one of them is.
 struct Range4 {
     float hi, lo;
-    bool fine;
 };
-template <typename T, int N>
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min_of(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+template <int N>
 __device__ __forceinline__ void widen(Range4& r, const float (&x)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        r.hi = fmaxf(r.hi, x[i]);
-        r.lo = fminf(r.lo, x[i]);
-        r.fine = r.fine && fabsf(x[i]) <= kLargest4<T>;
+    for (int i = 0; i < N; i += 2) {
+        r.hi = max_of(r.hi, x[i], x[i + 1]);
+        r.lo = min_of(r.lo, x[i], x[i + 1]);
     }
 }
 // Over groups of `lanes` neighbouring lanes (a power of two), by whole warps.
 __device__ __forceinline__ void join(Range4& r, int lanes) {
     for (int o = lanes >> 1; o > 0; o >>= 1) {
-        r.hi = fmaxf(r.hi, __shfl_xor_sync(0xffffffffu, r.hi, o));
-        r.lo = fminf(r.lo, __shfl_xor_sync(0xffffffffu, r.lo, o));
-        const int other = __shfl_xor_sync(0xffffffffu, (int)r.fine, o);
-        r.fine = r.fine && other;
+        const float hi = __shfl_xor_sync(0xffffffffu, r.hi, o), lo = __shfl_xor_sync(0xffffffffu, r.lo, o);
+        r.hi = max_of(r.hi, hi, hi);
+        r.lo = min_of(r.lo, lo, lo);
     }
 }
 
@@ -54,23 +61,26 @@ struct Scale4 {
 template <typename T>
 __device__ __forceinline__ Scale4 scale_of(const Range4& r) {
     Scale4 q;
+    const bool fine = r.hi <= kLargest4<T> && r.lo >= -kLargest4<T>;  // (false for NaN)
     // halves of both sides: the range of numbers near the largest would be infinite
     const float s = __fdiv_rn(0.5f * r.hi - 0.5f * r.lo, 7.5f);
-    q.s = fmaxf(__uint_as_float((__float_as_uint(s) + 0xfffffu) & ~0xfffffu), kLeastScale4<T>);
+    q.s = fine ? fmaxf(__uint_as_float((__float_as_uint(s) + 0xfffffu) & ~0xfffffu), kLeastScale4<T>) : 1.0f;
     q.z = fminf(rintf(__fdiv_rn(-r.lo, q.s)), 15.0f);
-    q.word = (__float_as_uint(q.s) >> 16) | (uint32_t)q.z;
-    if (!r.fine) {
-        q.s = 1.0f;
-        q.word = kNotFinite4;
-    }
+    q.word = fine ? (__float_as_uint(q.s) >> 16) | (uint32_t)q.z : kNotFinite4;
     return q;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t code_of(float x, const Scale4& q) {
-    float k = rintf(__fdiv_rn(x, q.s));
-    // a rounding past the largest number of T goes the other way
-    if (fabsf(k * q.s) > kLargest4<T>) k -= copysignf(1.0f, k);
-    return (uint32_t)fminf(fmaxf(k + q.z, 0.0f), 15.0f);  // (NaN: 0)
+// The codes of N neighbouring values, the first in the lowest bits.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t codes_of(const float (&x)[N], const Scale4& q) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float k = rintf(__fdiv_rn(x[i], q.s));
+        // a rounding past the largest number of T goes the other way
+        if (fabsf(k * q.s) > kLargest4<T>) k -= copysignf(1.0f, k);
+        c |= (uint32_t)fminf(fmaxf(k + q.z, 0.0f), 15.0f) << (4 * i);  // (NaN: 0)
+    }
+    return c;
 }
 
 // As turn_of, in 64 bits.
@@ -125,18 +135,21 @@ __global__ void __launch_bounds__(kRopeThreads)
         check_sequences(a);
         return;
     }
+    // Turn e of a thread is that of element e of its first block, or (interleaved) of elements 2 e, 2 e + 1 of the
+    // first and then the second; those of neighbouring threads lie next to each other, or they would meet in the banks.
+    auto pair = [&](int e) { return 8 * e + w; };
     if (tid < rope.half) {
+        const int p = tid, late = INTERLEAVED && p >= rope.half / 2 ? 4 : 0, x = late ? p - rope.half / 2 : p;
+        const int at = INTERLEAVED ? 8 * (late + x % 4) + x / 4 : 8 * (p % 8) + p / 8;
         if (a.k) {
-            const double2 cs = turn_of64(rope, tid, pos);
-            cs64_s[tid] = cs;
-            cs_s[tid] = make_float2((float)cs.x, (float)cs.y);
+            const double2 cs = turn_of64(rope, p, pos);
+            cs64_s[at] = cs;
+            cs_s[at] = make_float2((float)cs.x, (float)cs.y);
         } else {
-            cs_s[tid] = turn_of(rope, tid, pos);
+            cs_s[at] = turn_of(rope, p, pos);
         }
     }
     __syncthreads();
-    // the pair of element e of the first block, or (interleaved) of elements 2 e, 2 e + 1 of the first and then the second
-    auto pair = [&](int e) { return !INTERLEAVED ? 8 * w + e : e < 4 ? 4 * w + e : rope.half / 2 + 4 * w + e - 4; };
     // h: the head; of a thread past the last one, that one, and nothing is stored
     auto finish = [&](int h, const Eight<S>& ex, const Eight<S>& ey) {
         const bool live = h < heads;
@@ -169,18 +182,13 @@ __global__ void __launch_bounds__(kRopeThreads)
             }
         }
         if (__all_sync(0xffffffffu, is_q)) return;
-        Range4 range = {0.0f, 0.0f, true};
-        widen<T>(range, u);
-        widen<T>(range, v);
+        Range4 range = {0.0f, 0.0f};
+        widen(range, u);
+        widen(range, v);
         join(range, 1 << log_u);
         if (is_q || !live || row < 0) return;
         const Scale4 q = scale_of<T>(range);
-        uint32_t cu = 0, cv = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            cu |= code_of<T>(u[e], q) << (4 * e);
-            cv |= code_of<T>(v[e], q) << (4 * e);
-        }
+        const uint32_t cu = codes_of<T, 8>(u, q), cv = codes_of<T, 8>(v, q);
         const int kh = h - heads_q;
         const long long at = row + (long long)(is_v ? kh - nkv : kh) * a.b.page_size;
         uint32_t* dst = static_cast<uint32_t*>(is_v ? a.vp : a.kp) + at * (D / 8);
@@ -246,15 +254,16 @@ __global__ void __launch_bounds__(kRopeThreads)
             for (int i = 0; i < N; ++i) dst[N * lane + i] = Half16<T>::round(x[i]);
             continue;
         }
-        Range4 range = {0.0f, 0.0f, true};
-        widen<T>(range, x);
+        Range4 range = {0.0f, 0.0f};
+        widen(range, x);
         join(range, 32);
         const Scale4 q = scale_of<T>(range);
         const int kh = h - heads_q;
         const long long at = row + (long long)(is_v ? kh - nkv : kh) * a.b.page_size;
         uint8_t* dst = static_cast<uint8_t*>(is_v ? a.vp : a.kp) + at * (D / 2) + lane * (N / 2);
+        const uint32_t c = codes_of<T, N>(x, q);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) dst[i / 2] = (uint8_t)(code_of<T>(x[i], q) | code_of<T>(x[i + 1], q) << 4);
+        for (int i = 0; i < N; i += 2) dst[i / 2] = (uint8_t)(c >> (4 * i));
         if (lane == 0) scales[2 * at + is_v] = (uint16_t)q.word;
     }
     check_sequences(a);
