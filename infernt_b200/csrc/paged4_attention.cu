@@ -34,7 +34,11 @@ constexpr int kWarpKeys = 16 * kGroups;
 constexpr int kKeys = kWarps * kWarpKeys;  // of a tile
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 3;     // tiles of a warp's ring: one is worked on, two are on their way
-constexpr int kMostRows = 64;  // query rows of a KV head from which on the tcgen05 kernel is faster
+// Query rows of a KV head above which the tcgen05 kernel is faster.  64 sequences
+// of 512 to 2048 positions take, here and there: of 64 elements, 24 rows 33 and
+// 51 us, 48 rows 44 and 51, 64 rows 55 and 51 (4 sequences of 32768: 61 and 70);
+// of 128, 24 rows 73 and 102, 32 rows 94 and 103, 40 rows 119 and 103 us.
+constexpr int most_rows(int dim) { return dim == 64 ? 64 : 32; }
 
 // The products are in fp16 whatever the cache's type is, since codes get there
 // with one shift for eight of them (bf16, with seven bits behind its leading
@@ -696,11 +700,16 @@ int launch_rows(const AttnArgs& a, cudaStream_t st) {
     return INFERNT_OK;
 }
 
-// rows: query rows of a KV head that most sequences have
+// rows: query rows of a KV head that most sequences have.  They make as few
+// items as can be, of up to four n-tiles, and as many n-tiles in each: a
+// part's rows cost their softmax whether they are there or not (40 rows as 24 and
+// 16 take 43 us in the first of the cases above, as 32 and 8 they took 52).
 template <typename T, int D>
 int launch(const AttnArgs& a, long long rows, cudaStream_t st) {
-    if (rows <= 8) return launch_rows<T, D, 1>(a, st);
-    if (rows <= 16) return launch_rows<T, D, 2>(a, st);
+    const long long tiles = (rows + 7) / 8, items = (tiles + 3) / 4, each = (tiles + items - 1) / items;
+    if (each <= 1) return launch_rows<T, D, 1>(a, st);
+    if (each == 2) return launch_rows<T, D, 2>(a, st);
+    if (each == 3) return launch_rows<T, D, 3>(a, st);
     return launch_rows<T, D, 4>(a, st);
 }
 
@@ -726,16 +735,16 @@ extern "C" int infernt_paged4_attention(void* out, int ldo, const void* q, int l
     a.scales = cache->scales;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int D = cache->head_dim;
-    // Sequences of up to kMostRows query rows a KV head are bound by their keys,
+    // Sequences of up to most_rows query rows a KV head are bound by their keys,
     // longer ones by their products.  Where the batch's counts do not say that
     // all sequences are as long as the longest, each kernel takes its own.
     const long long most = (long long)batch->max_q_len * a.G;
-    const bool chunks = most > kMostRows, both = chunks && batch->num_rows < (long long)batch->num_seqs * batch->max_q_len;
+    const bool chunks = most > most_rows(D), both = chunks && batch->num_rows < (long long)batch->num_seqs * batch->max_q_len;
     if (!chunks || both) {
         // rows of an item: those of the longest sequence, or, beside a chunk, what the others have on average
         long long rows = most;
         if (both) {
-            a.max_rows = kMostRows;
+            a.max_rows = most_rows(D);
             rows = std::max(1, (batch->num_rows - batch->max_q_len + batch->num_seqs - 2) / std::max(1, batch->num_seqs - 1));
             rows *= a.G;
         }
@@ -745,7 +754,7 @@ extern "C" int infernt_paged4_attention(void* out, int ldo, const void* q, int l
         else
             s = D == 64 ? launch<__half, 64>(a, rows, st) : launch<__half, 128>(a, rows, st);
         if (s || !chunks) return s;
-        a.min_rows = kMostRows;
+        a.min_rows = most_rows(D);
         a.max_rows = kMaxPositions;
     }
     return paged4_attention_tc(a, D, cache->dtype, both, st);

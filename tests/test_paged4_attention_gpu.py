@@ -60,6 +60,17 @@ def test_shapes(torch, workspace, shape, dtype):
     ref.check_attention(case)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [8, 9, 16, 17, 24, 25, 32, 33, 40, 48, 49, 64, 65])
+def test_rows_at_the_items_borders(torch, workspace, rows, D):
+    """Query rows that fill one to four blocks of eight, of one item or two, and
+    one more; alone and beside shorter and longer sequences."""
+    for seqs in ([(rows, 500), (rows, rows)], [(rows, 700), (1, 300), (0, 9), (3, 3), (100, 400)]):
+        case = ref4.Case4(torch, seqs, 2, 2, D, 16, "bf16" if rows % 2 else "fp16", seed=rows, spare_rows=1, hide=True)
+        run(torch, case, workspace)
+        ref.check_attention(case)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (5, 2), (64, 0), (100, 4), (127, 130), (1000, 1), (5000, 3)])
 @pytest.mark.parametrize("seqs", [[(1, 700), (1, 130)], [(5, 640), (2, 90)], [(20, 1500)], [(100, 900), (1, 400)]])
 def test_windows(torch, workspace, seqs, window, sinks):
