@@ -770,7 +770,8 @@ typedef struct infernt_page_tables {
  * their table entries become -1.  Writes the ragged batch, q_start [num_seqs
  * + 1] and kv_len [num_seqs] (kv_len may be len itself), and for each new
  * token its position and its slot, page x page_size + row (positions and
- * slots [max_rows] or NULL; elements past the last token stay).
+ * slots [max_rows] or NULL; elements past the last token stay).  Nothing
+ * else that it writes may overlap another array of the call.
  * A sequence waits when the pages missing up to it, its own included, are
  * more than are free, and when new_len up to it add up to more than
  * max_rows: it gets no rows (kv_len[s] = len[s]) and keeps its pages.  One
@@ -800,6 +801,7 @@ INFERNT_API int infernt_paged_batch_plan(const infernt_page_tables* tables, cons
  * out_tokens of the sequence's rows: the accepted drafts, the drawn token,
  * then -1; accepted[s]: the drafts accepted; kept[s] = kv_len[s] less the
  * rejected ones (kv_len and kept both or neither; they may be one array).
+ * Nothing else that it writes may overlap another array of the call.
  * A sequence without rows has accepted 0 and no token.
  *   target [num_rows][vocab_size], rows ld elements apart, of type F32, BF16
  *   or F16: logits, p = softmax(row / temperature[s]); with probabilities != 0

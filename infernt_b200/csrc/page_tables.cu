@@ -250,7 +250,6 @@ extern "C" int infernt_paged_batch_plan(const infernt_page_tables* t, const int*
                     "%s: a pool of 2^31 slots or more", op);
     INFERNT_REQUIRE(t->num_seqs == 0 || (len && new_len && kv_len && t->held && (t->block_table || t->table_stride == 0)),
                     "%s: null pointer", op);
-    INFERNT_REQUIRE(kv_len != new_len || t->num_seqs == 0, "%s: kv_len may not be new_len", op);
     const struct {
         const char* what;
         const void* p;
@@ -260,6 +259,19 @@ extern "C" int infernt_paged_batch_plan(const infernt_page_tables* t, const int*
                   {"slots", slots},                {"err", err}};
     for (const auto& x : arrays)
         INFERNT_REQUIRE(reinterpret_cast<uintptr_t>(x.p) % 4 == 0, "%s: misaligned %s", op, x.what);
+    const size_t seqs4 = 4 * (size_t)t->num_seqs, rows4 = 4 * (size_t)max_rows;
+    const Span spans[] = {{"block_table", t->block_table, seqs4 * t->table_stride, true},
+                          {"held", t->held, seqs4, true},
+                          {"free_pages", t->free_pages, 4 * (size_t)t->num_pages, true},
+                          {"state", t->state, 16, true},
+                          {"q_start", q_start, seqs4 + 4, true},
+                          {"kv_len", kv_len, seqs4, true},
+                          {"positions", positions, rows4, true},
+                          {"slots", slots, rows4, true},
+                          {"err", err, 4, true},
+                          {"len", len == kv_len ? nullptr : len, seqs4, false},
+                          {"new_len", new_len, seqs4, false}};
+    if (int s = check_apart(op, spans)) return s;
     for (const auto& x : arrays)
         if (int s = check_device_pointer(op, x.what, x.p)) return s;
     PlanArgs a;

@@ -151,6 +151,25 @@ int check_paged_cache(const char* op, const infernt_paged_cache* c);
 int check_ragged_batch(const char* op, const infernt_ragged_batch* b);
 // p (or NULL) must be memory that the current device reads in place.
 int check_device_pointer(const char* op, const char* what, const void* p);
+
+// An array of a call.  What a call writes may not overlap anything else of it.
+struct Span {
+    const char* what;
+    const void* p;  // or null
+    size_t bytes;
+    bool written;
+};
+template <int N>
+inline int check_apart(const char* op, const Span (&spans)[N]) {
+    for (int i = 0; i < N; ++i)
+        for (int j = 0; j < i; ++j) {
+            const Span &x = spans[i], &y = spans[j];
+            if (!(x.written || y.written) || !x.p || !y.p || !x.bytes || !y.bytes) continue;
+            const uintptr_t a = reinterpret_cast<uintptr_t>(x.p), b = reinterpret_cast<uintptr_t>(y.p);
+            INFERNT_REQUIRE(a >= b + y.bytes || b >= a + x.bytes, "%s: %s overlaps %s", op, x.what, y.what);
+        }
+    return INFERNT_OK;
+}
 int check_batch_pointers(const char* op, const infernt_paged_cache* c, const infernt_ragged_batch* b, const void* err);
 
 inline PagedBatch paged_batch(const infernt_paged_cache& c, const infernt_ragged_batch& b) {

@@ -132,6 +132,34 @@ def test_bad_verifications_are_refused(kw):
     assert ib.lib().infernt_last_error().startswith(b"verify_drafts: ")
 
 
+def test_arrays_that_overlap_are_refused():
+    """What a call writes may lie in nothing else of it, kept in kv_len and
+    kv_len in len apart."""
+    def at(n, step=1 << 20):  # arrays far from each other
+        return A + n * step
+
+    def message(status):
+        assert status in (1, 6)  # 6: there is no device whose memory they could be
+        return ib.lib().infernt_last_error()
+
+    names = dict(out=at(0), acc=at(1), target=at(2), draft=at(3), draft_ld=100, tokens=at(4), q_start=at(5), temps=at(6),
+                 u=at(7), kv=at(8), kept=at(9), ws=at(10), err=at(11))
+    assert b"overlap" not in message(verify(**names))  # no memory of a device
+    assert b"overlap" not in message(verify(**{**names, "kept": at(8)}))
+    for bad in (dict(tokens=at(0)), dict(tokens=at(0) + 16), dict(q_start=at(1) - 8), dict(kv=at(9) + 4), dict(kept=at(5)),
+                dict(acc=at(0) + 16), dict(u=at(0) - 4), dict(temps=at(1)), dict(out=at(2) + 4 * 499), dict(err=at(4) + 16),
+                dict(kept=at(3) + 400), dict(ws=at(7)), dict(u=at(10) + 5 * 512 - 4)):
+        assert b"overlap" in message(verify(**{**names, **bad})), bad
+    assert b"overlap" not in message(verify(**{**names, "tokens": at(0) + 20}))
+    t = tables(block_table=at(0), held=at(1), free_pages=at(2), state=at(3))
+    args = dict(t=t, lens=at(4), new=at(5), q_start=at(6), kv=at(7), positions=at(8), slots=at(9), err=at(10))
+    assert b"overlap" not in message(plan(**args))
+    assert b"overlap" not in message(plan(**{**args, "kv": at(4)}))
+    for bad in (dict(kv=at(5)), dict(kv=at(4) + 4), dict(q_start=at(4) - 12), dict(positions=at(9) + 36), dict(slots=at(0) + 44),
+                dict(lens=at(1)), dict(new=at(2) + 76), dict(err=at(3) + 12)):
+        assert b"overlap" in message(plan(**{**args, **bad})), bad
+
+
 # ---------------------------------------------------------------- the Python wrappers
 
 
