@@ -206,6 +206,7 @@ __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) 
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr int kDrawPerSm = 3;
+constexpr int kMostCluster = 8;
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -323,7 +324,7 @@ __device__ __noinline__ void put_largest(const L* row, int V, int* out) {
 //   as good as w Z: a pass less, 100 sequences of 32000 tokens 33 -> 29 us);
 //   W = sum w_i over the cluster;
 //   the CTA, in it the warp, and of its stretch the piece whose part of the sum
-//   has u W in it: that piece is walked along, 32 elements at a time.
+//   has u W in it: that piece is walked along, a group of elements at a time.
 // The weights are computed again in each pass (the logits are in L2): some 25
 // operations in 64 bits an element, each waiting for the one before, so a lane
 // has eight elements on the way.  64 sequences that stop, 128256 tokens: 38 us
@@ -456,8 +457,9 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
             for (int j = 0; j < kEach; ++j) x[j] = g * kGroup + 32 * j + lane < a.V ? element(at + 32 * j) : none;
         }
     };
-    // the sum over the CTA's warps into its shared_s[slot], then over the cluster, both in order
-    auto over_cluster = [&](double v, int slot) {
+    // the sum over the CTA's warps into its shared_s[slot], then over the cluster, both in order; the CTAs' sums in of
+    using Sums = double[kMostCluster];
+    auto over_cluster = [&](double v, int slot, Sums& of) {
         v = warp_sum64(v);
         if (lane == 0) sum_s[slot][warp] = v;
         __syncthreads();
@@ -467,8 +469,12 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
             shared_s[slot] = x;
         }
         cluster_sync();
-        double x = 0.0;
-        for (int k = 0; k < a.cluster; ++k) x += peer_double(&shared_s[slot], k);
+        // all on their way before the first is added
+#pragma unroll
+        for (int k = 0; k < kMostCluster; ++k) of[k] = k < a.cluster ? peer_double(&shared_s[slot], k) : 0.0;
+        double x = of[0];
+#pragma unroll
+        for (int k = 1; k < kMostCluster; ++k) x += of[k];
         return x;
     };
     if (!PROBS && st.minus == 1) {
@@ -479,7 +485,8 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
 #pragma unroll
             for (int j = 0; j < kEach; j += 2) v += weight(l[j]) + weight(l[j + 1]);
         }
-        z = 1.0 / over_cluster(v, 0);
+        Sums of;
+        z = 1.0 / over_cluster(v, 0, of);
     }
     // this warp's pieces; their sum
     auto pieces = [&](auto minus) {
@@ -502,18 +509,20 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
     };
     using std::integral_constant;
     int minus = st.minus;
+    Sums sums;
     double total = over_cluster(minus == 1   ? pieces(integral_constant<int, 1>())
                                 : minus == 2 ? pieces(integral_constant<int, 2>())
                                              : pieces(integral_constant<int, 0>()),
-                                1);
+                                1, sums);
     if (minus && !(total > 0.0)) {  // nothing is left: from p itself
         minus = 0;
         cluster_sync();  // shared_s is read
-        total = over_cluster(pieces(integral_constant<int, 0>()), 1);
+        total = over_cluster(pieces(integral_constant<int, 0>()), 1, sums);
     }
     if (PROBS) {
         // a probability that is none, anywhere in the row
-        if (over_cluster(bad ? 1.0 : 0.0, 2) > 0.0 || !(total > 0.0)) {
+        Sums of;
+        if (over_cluster(bad ? 1.0 : 0.0, 2, of) > 0.0 || !(total > 0.0)) {
             if (rank == 0) {
                 put_largest<L>(row, a.V, a.out + stop);
                 if (tid == 0 && a.err) atomicOr(a.err, kErrValue);
@@ -525,10 +534,11 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
     // ---- of n parts, the one that has the goal in it (by the rounding of the sums alone, none: the last that has any)
     const double goal = (double)in_unit(a.u[end - 1]) * total;
     double before = 0.0;
-    auto find = [&](int parts, auto part) {
+    auto find = [&](const auto& part, auto parts) {
         int owner = -1, some = 0;
         double at = before, at_some = before, sum = before;
-        for (int k = 0; k < parts; ++k) {
+#pragma unroll
+        for (int k = 0; k < decltype(parts)::value; ++k) {
             const double x = part(k);
             if (x > 0.0) {
                 some = k;
@@ -543,31 +553,45 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
         before = owner < 0 ? at_some : at;
         return owner < 0 ? some : owner;
     };
-    if (find(a.cluster, [&](int k) { return peer_double(&shared_s[1], k); }) == (int)rank &&
-        find(kDrawWarps, [&](int w) { return sum_s[1][w]; }) == warp) {
+    if (find([&](int k) { return sums[k]; }, integral_constant<int, kMostCluster>()) == (int)rank &&
+        find([&](int w) { return sum_s[1][w]; }, integral_constant<int, kDrawWarps>()) == warp) {
         double x = 0.0;  // of piece `lane`
         if (lane < kSubs)
+#pragma unroll 8
             for (int k = 0; k < 32; ++k) x += sub_s[warp][lane][(k + lane) % 32];
-        const int piece = find(kSubs, [&](int k) { return __shfl_sync(0xffffffffu, x, k); });
-        const int first = (g0 + piece * sub) * kGroup, last = min(min(g1, g0 + (piece + 1) * sub) * kGroup, a.V);
-        int found = -1, some = min(first, a.V - 1);
-        for (int i0 = first; i0 < last && found < 0; i0 += 32) {
-            const int i = i0 + lane;
-            const float l = i < last ? element(row + i) : kOutside, q = minus == 1 && i < last ? draft[i] : 0.0f;
-            const double w = minus == 1   ? left(integral_constant<int, 1>(), i, l, q)
-                             : minus == 2 ? left(integral_constant<int, 2>(), i, l, 0.0f)
-                                          : left(integral_constant<int, 0>(), i, l, 0.0f);
-            double upto = w;
+        const int piece =
+            find([&](int k) { return __shfl_sync(0xffffffffu, x, k); }, integral_constant<int, kSubs>());
+        const int first = g0 + piece * sub, last = min(g1, first + sub);
+        int found = -1, some = min(first * kGroup, a.V - 1);
+        for (int g = first; g < last && found < 0; ++g) {
+            // kEach rows of 32 elements: the sums along every one of them at once
+            float l[kEach], q[kEach] = {};
+            get(row, g, kOutside, l);
+            if (minus == 1) get(draft, g, 0.0f, q);
+            double w[kEach], upto[kEach];
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
+            for (int j = 0; j < kEach; ++j) {
+                const int i = g * kGroup + 32 * j + lane;
+                w[j] = minus == 1 ? left(integral_constant<int, 1>(), i, l[j], q[j]) : left(integral_constant<int, 0>(), i, l[j], 0.0f);
+                if (minus == 2 && i == d) w[j] = 0.0;
+                upto[j] = w[j];
             }
-            const unsigned past = __ballot_sync(0xffffffffu, w > 0.0 && before + upto > goal);
-            const unsigned any = __ballot_sync(0xffffffffu, w > 0.0);
-            if (past) found = i0 + __ffs(past) - 1;
-            if (any) some = i0 + 31 - __clz(any);
-            before += __shfl_sync(0xffffffffu, upto, 31);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    const double y = __shfl_up_sync(0xffffffffu, upto[j], o);
+                    if (lane >= o) upto[j] += y;
+                }
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const int i0 = g * kGroup + 32 * j;
+                const unsigned past = __ballot_sync(0xffffffffu, w[j] > 0.0 && before + upto[j] > goal);
+                const unsigned any = __ballot_sync(0xffffffffu, w[j] > 0.0);
+                if (past && found < 0) found = i0 + __ffs(past) - 1;
+                if (any) some = i0 + 31 - __clz(any);
+                before += __shfl_sync(0xffffffffu, upto[j], 31);
+            }
         }
         if (lane == 0) a.out[stop] = found >= 0 ? found : some;
     }
@@ -675,7 +699,7 @@ extern "C" int infernt_verify_drafts(int* out_tokens, int* accepted, const void*
     a.part = (int)((tiles + kMostParts - 1) / kMostParts) * kStatTile;
     a.n_parts = (int)(((long long)vocab_size + 7 + a.part - 1) / a.part);
     // as many CTAs a sequence as are sure to run at once: a cluster that has to wait for room waits for another's end
-    a.cluster = std::max(1, std::min(8, kDrawPerSm * sm_count() / num_seqs));
+    a.cluster = std::max(1, std::min(kMostCluster, kDrawPerSm * sm_count() / num_seqs));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool p = probabilities != 0;
     if (target_dtype == INFERNT_DTYPE_F32) return p ? launch<float, true>(a, st) : launch<float, false>(a, st);
