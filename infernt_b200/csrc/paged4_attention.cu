@@ -22,7 +22,6 @@
 
 #include "paged4.cuh"
 #include "paged_attention.cuh"
-#include "tc_mma.cuh"
 #include "warp_mma.cuh"
 
 namespace infernt {
@@ -35,10 +34,11 @@ constexpr int kKeys = kWarps * kWarpKeys;  // of a tile
 constexpr int kThreads = 32 * kWarps;
 constexpr int kStages = 3;     // tiles of a warp's ring: one is worked on, two are on their way
 // Query rows of a KV head above which the tcgen05 kernel is faster.  64 sequences
-// of 512 to 2048 positions take, here and there: of 64 elements, 24 rows 33 and
-// 51 us, 48 rows 44 and 51, 64 rows 55 and 51 (4 sequences of 32768: 61 and 70);
-// of 128, 24 rows 73 and 102, 32 rows 94 and 103, 40 rows 119 and 103 us.
-constexpr int most_rows(int dim) { return dim == 64 ? 64 : 32; }
+// of 512 to 2048 positions, and 4 of 30000 to 32768, take here and there: of 64
+// elements, 24 rows 31 and 51 us, 39 and 72; 48 rows 42 and 51, 50 and 71; 64
+// rows 51 and 51, 56 and 69; of 128, 32 rows 86 and 103, 96 and 137; 48 rows 115
+// and 104, 126 and 138; 64 rows 151 and 104, 159 and 138.
+constexpr int most_rows(int dim) { return dim == 64 ? 64 : 48; }
 
 // The products are in fp16 whatever the cache's type is, since codes get there
 // with one shift for eight of them (bf16, with seven bits behind its leading
@@ -354,12 +354,11 @@ __device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, 
                     whole(ka[0][w], z0, mk, x);
                     whole(ka[1][w], z1, mk, y);
 #pragma unroll
-                    for (int n = 0; n < RB; ++n)
-                        if (RB == 1 || 8 * n < it.rows) {
-                            const uint4 q = L::kSharedQ ? ld_shared(q_at + (n * W + w) * 512) : qb[w];
-                            mma(sc[i][n], x[0], y[0], x[1], y[1], q.x, q.y);
-                            mma(sc[i][n], x[2], y[2], x[3], y[3], q.z, q.w);
-                        }
+                    for (int n = 0; n < RB; ++n) {  // (n-tiles without rows too: asking costs as much)
+                        const uint4 q = L::kSharedQ ? ld_shared(q_at + (n * W + w) * 512) : qb[w];
+                        mma(sc[i][n], x[0], y[0], x[1], y[1], q.x, q.y);
+                        mma(sc[i][n], x[2], y[2], x[3], y[3], q.z, q.w);
+                    }
                 }
             }
             // a score in base 2 is sc f
@@ -521,9 +520,8 @@ __device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, 
                         for (int b = 0; b < 2; ++b)
 #pragma unroll
                             for (int n = 0; n < RB; ++n)
-                                if (RB == 1 || 8 * n < it.rows)
-                                    mma(s.acc[n][4 * q + 2 * half + b], x[2 * b], x[2 * b + 1], y[2 * b], y[2 * b + 1],
-                                        pb[n][0], pb[n][1]);
+                                mma(s.acc[n][4 * q + 2 * half + b], x[2 * b], x[2 * b + 1], y[2 * b], y[2 * b + 1],
+                                    pb[n][0], pb[n][1]);
                     }
             }
         }
@@ -703,7 +701,7 @@ int launch_rows(const AttnArgs& a, cudaStream_t st) {
 // rows: query rows of a KV head that most sequences have.  They make as few
 // items as can be, of up to four n-tiles, and as many n-tiles in each: a
 // part's rows cost their softmax whether they are there or not (40 rows as 24 and
-// 16 take 43 us in the first of the cases above, as 32 and 8 they took 52).
+// 16 take 42 us in the first of the cases above, as 32 and 8 they took 52).
 template <typename T, int D>
 int launch(const AttnArgs& a, long long rows, cudaStream_t st) {
     const long long tiles = (rows + 7) / 8, items = (tiles + 3) / 4, each = (tiles + items - 1) / items;
