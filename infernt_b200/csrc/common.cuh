@@ -101,14 +101,6 @@ __device__ __forceinline__ void bulk_g2s_plain(void* dst, const void* src, uint3
         : "memory");
 }
 
-// The same to a shared-memory address.
-__device__ __forceinline__ void bulk_g2s_plain_at(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-        "l"(src), "r"(bytes), "r"(smem_addr(bar))
-        : "memory");
-}
-
 // Bulk prefetch of [src, src + bytes) into L2 (no destination, no
 // completion); src and bytes multiples of 16.
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
