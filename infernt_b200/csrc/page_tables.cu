@@ -104,9 +104,9 @@ __device__ __forceinline__ int owner(const unsigned* before, unsigned x) {
 // of loads.  Rows and pages are then dealt evenly to the threads, whoever's they
 // are.  A page that a sequence takes is read from the ring wherever it is
 // needed, so nothing waits for a store.  Latency-bound: loads, two scans, a
-// search of ten steps, the ring's and the table's loads, stores.  (A thread or a
-// warp a sequence took 20 us for the step of 256 sequences and 85 for 100
-// prompts.)
+// search of ten steps, the ring's and the table's loads, stores.  The step of 256
+// sequences takes 5 us (7 from a cold cache), 100 prompts 13 and 5 for their
+// rows.  (A thread or a warp a sequence took 20 and 85.)
 __global__ void __launch_bounds__(kPlanThreads) paged_plan(const PlanArgs a) {
     pdl_launch_dependents();  // paged_plan_rows waits for this kernel's end
     __shared__ unsigned sums[3][32];
