@@ -582,8 +582,8 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const PagedSeq& seq
             o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (mb[i] == -INFINITY) continue;
-                const float w = ex2(mb[i] - top);
+                // (of a row whose scores are NaN, m is -infinity and l NaN)
+                const float w = mb[i] == -INFINITY ? 0.0f : ex2(mb[i] - top);
                 l = fmaf(lb[i], w, l);
                 o.x = fmaf(v[i].x, w, o.x);
                 o.y = fmaf(v[i].y, w, o.y);

@@ -355,14 +355,18 @@ __device__ __noinline__ void join_row(const AttnArgs& a, int first, int last, in
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (b + i > last) mb[i] = -INFINITY;
+            if (b + i > last) {
+                mb[i] = -INFINITY;
+                lb[i] = 0.0f;
+            }
             top = fmaxf(top, mb[i]);
         }
         l *= M == -INFINITY ? 0.0f : ex2(M - top);
         M = top;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (mb[i] != -INFINITY) l = fmaf(lb[i], ex2(mb[i] - M), l);
+            if (FOUR || mb[i] != -INFINITY)  // (FOUR: the lse of a row whose scores are NaN is NaN, split or not)
+                l = fmaf(lb[i], mb[i] == -INFINITY ? 0.0f : ex2(mb[i] - M), l);
     }
     if (lse) *lse = sees ? (M + log2f(l)) * kLn2 : -INFINITY;
     const float inv = 1.0f / l;

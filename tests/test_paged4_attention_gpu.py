@@ -144,11 +144,34 @@ def test_vectors_of_nan(torch, workspace, n):
             assert bool((case.out[n:] == plain.out[n:]).all())
 
 
+@pytest.mark.parametrize("n,length", [(1, 300), (1, 30000), (3, 700), (5, 20000), (40, 700), (40, 9000)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_query_rows_that_are_not_finite(torch, workspace, n, length, what):
+    """A NaN or an infinity in a head's row (an infinity in all of it, so that
+    every score is one or NaN): that row's out and lse are NaN, whether its item
+    is split or not, and all others as without it."""
+    case, plain = (ref4.Case4(torch, [(n, length), (n, n + 64)], 8, 2, 128, 16, "fp16", seed=n, hide=True) for _ in range(2))
+    r = n // 2
+    case.q[r, 1, 5] = what
+    case.q[r, 6] = what
+    run(torch, plain, workspace)
+    run(torch, case, workspace)
+    bad = torch.zeros(case.rows, 8, dtype=torch.bool, device="cuda")
+    bad[r, 1] = bad[r, 6] = True
+    assert bool(torch.isnan(case.out[bad]).all()) and bool(torch.isnan(case.lse[bad]).all())
+    case.q.copy_(plain.q)
+    case.out[bad], case.lse[bad] = plain.out[bad], plain.lse[bad]
+    ref.check_attention(case, rows=range(0, n, 7))
+
+
 @pytest.mark.parametrize("n", [1, 6, 50])
 @pytest.mark.parametrize("page", [16, 5])
 def test_as_over_unpacked_pages(torch, workspace, n, page):
     """The values are numbers of the type: both kinds of pages give the same
-    rows, each within its own bound of the other."""
+    rows but for each kernel's half steps of the probabilities (of vmax at most
+    in all) and of the result, and what scores in FP32 and weights below the
+    normal numbers leave (1e-3; of lse, scores of 128 products off by 2^-24 of
+    their sizes' sum, some 10, each: 1e-4)."""
     case = ref4.Case4(torch, [(n, 1000), (n, n + 70)], 8, 2, 128, page, "fp16", seed=n)
     run(torch, case, workspace)
     pools = [torch.zeros(*case.kc.shape[:3], 128, device="cuda", dtype=case.dtype) for _ in range(2)]
