@@ -10,6 +10,7 @@ Configurations follow the reference's ``ModelConfig`` (include/config.h).
 """
 import array
 import ctypes
+import functools
 import os
 from dataclasses import dataclass, replace
 
@@ -1123,12 +1124,14 @@ def copy_pages(pools, src, dst, stream=None):
 
 
 # ------------------------------------------ pages of 4 bits, drafted tokens
-def _torch_dtype(d):
-    """DTYPE_BF16 or DTYPE_F16 of a torch type."""
-    code = {"torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_F16}.get(str(d))
-    if code is None:
-        raise ValueError("type %s (bfloat16 or float16)" % d)
-    return code
+_PAGED4_TYPES = {}
+
+
+def _paged4_types():
+    """torch's uint8, int32, and DTYPE_* of bfloat16 and float16."""
+    import torch
+    _PAGED4_TYPES[0] = torch.uint8, torch.int32, {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16}
+    return _PAGED4_TYPES[0]
 
 
 class PagedCache4(ctypes.Structure):
@@ -1145,12 +1148,15 @@ class PagedCache4(ctypes.Structure):
         if len(shape) != 4 or v.shape != shape or scales.shape != shape[:3] or v.get_device() != device or (
                 scales.get_device() != device):
             raise ValueError("PagedCache4: k %s, v %s, scales %s" % (tuple(shape), tuple(v.shape), tuple(scales.shape)))
-        if str(k.dtype) != "torch.uint8" or v.dtype != k.dtype or str(scales.dtype) != "torch.int32" or not (
+        uint8, int32, codes = _PAGED4_TYPES.get(0) or _paged4_types()
+        if k.dtype != uint8 or v.dtype != uint8 or scales.dtype != int32 or not (
                 k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
             raise ValueError("PagedCache4: contiguous uint8 codes and int32 scales are needed")
+        code = codes.get(dtype)
+        if code is None:
+            raise ValueError("PagedCache4: type %s (bfloat16 or float16)" % dtype)
         pages, heads, page, half = shape
-        _struct_init(self, k.data_ptr(), v.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half,
-                     _torch_dtype(dtype))
+        _struct_init(self, k.data_ptr(), v.data_ptr(), scales.data_ptr(), pages, heads, page, 2 * half, code)
         self.tensors = k, v, scales
 
 
@@ -1240,6 +1246,7 @@ def plan_batch(tables, lens, new_lens, q_start, kv_len, positions=None, slots=No
         check(status, "infernt_paged_batch_plan")
 
 
+@functools.lru_cache(maxsize=64)
 def verify_drafts_workspace_bytes(num_rows, num_seqs):
     return lib().infernt_verify_drafts_workspace_bytes(num_rows, num_seqs)
 
