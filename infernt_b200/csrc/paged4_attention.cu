@@ -37,6 +37,10 @@ constexpr int kGroups = 2;  // of 16 keys, of a tile, a warp
 constexpr int kWarpKeys = 16 * kGroups;
 constexpr int kKeys = kWarps * kWarpKeys;  // of a tile
 constexpr int kThreads = 32 * kWarps;
+// Parts of one tile of 128 keys: a border moves less than with two (the 16-bit
+// kernels' tiles are of 64; 64 sequences of 512 to 2048 took 41.5 us, with three
+// 43, now 40.3).
+constexpr int kLeast4 = kItemCost + 1;
 constexpr int kStages = 3;     // tiles of a warp's ring: one is worked on, two are on their way
 // Query rows of a KV head above which the tcgen05 kernel is faster.  64 sequences
 // of 512 to 2048 positions, and 4 of 30000 to 32768, take here and there: of 64
@@ -611,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, RB>::kPerSm)) paged4_attn
     const Place place = find_place<M, kKeys, kThreads>(a);
     pdl_launch_dependents();  // the tcgen05 kernel may take SMs as they become free
     if (place.s < 0) return;
-    walk<M, kKeys>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
+    walk<M, kKeys, kLeast4>(a, place, [&](const PagedSeq& seq, const Item& it, const Part& p) {
         {
             RowState<D, RB> s;
             consume<T, D, RB>(a, seq, it, p, warp, lane, base, s);

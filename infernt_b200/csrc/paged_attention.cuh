@@ -282,8 +282,9 @@ struct Part {
     int s, j0, j1, first, last;
 };
 
-// f(sequence, item, part) for the parts of this CTA, by whole warps.
-template <int M, int N, typename F>
+// f(sequence, item, part) for the parts of this CTA, by whole warps.  LEAST (above
+// kItemCost) stands for kLeast.
+template <int M, int N, int LEAST = kLeast, typename F>
 __device__ __forceinline__ void walk(const AttnArgs& a, const Place& p, F f) {
     const int me = blockIdx.x, begin = p.c * me, end = min(p.c, p.total - begin) + begin;
     int at = begin, before = p.before, per_head = p.per_head;
@@ -297,16 +298,16 @@ __device__ __forceinline__ void walk(const AttnArgs& a, const Place& p, F f) {
             while (kvh < a.b.nkv) {
                 const Item it = make_item<M, N>(a, seq, kvh, row0);
                 const int u1 = u0 + it.tiles + kItemCost;
-                const bool more = begin > u0 && begin - u0 >= kLeast;  // it began in an earlier CTA
-                if (end <= u0 || (end < u1 && end - u0 < kLeast && end < p.total)) return;
-                if (!(begin > u0 && begin - u0 >= kLeast && u1 - begin < kLeast)) {
-                    const bool cut = end < u1 && u1 - end >= kLeast;  // it goes on in a later one
+                const bool more = begin > u0 && begin - u0 >= LEAST;  // it began in an earlier CTA
+                if (end <= u0 || (end < u1 && end - u0 < LEAST && end < p.total)) return;
+                if (!(begin > u0 && begin - u0 >= LEAST && u1 - begin < LEAST)) {
+                    const bool cut = end < u1 && u1 - end >= LEAST;  // it goes on in a later one
                     Part part;
                     part.s = s;
                     part.j0 = more ? begin - u0 - kItemCost : 0;
                     part.j1 = cut ? end - u0 - kItemCost : it.tiles;
-                    part.first = more ? (u0 + kLeast + p.c - 1) / p.c - 1 : me;
-                    part.last = cut ? (u1 - kLeast) / p.c : me;
+                    part.first = more ? (u0 + LEAST + p.c - 1) / p.c - 1 : me;
+                    part.last = cut ? (u1 - LEAST) / p.c : me;
                     f(seq, it, part);
                 }
                 if (end < u1) return;
