@@ -19,7 +19,7 @@
 // 16 sequences of 32768 positions, 32/8 heads of 128 (554 MB, 85 us of HBM): 137
 // us, 4.0 TB/s, of which 111 grow with the keys: some 23 instructions a key and
 // warp, and the rest is the first loads, unequal ends and the joins.  64
-// sequences of 512 to 2048 with 40 query rows of 64: 42 us, where 2 instructions
+// sequences of 512 to 2048 with 40 query rows of 64: 40 us, where 2 instructions
 // of 4 that could be issue a cycle: 12 warps an SM with their waits for products.
 #include <algorithm>
 #include <cmath>
@@ -38,15 +38,15 @@ constexpr int kWarpKeys = 16 * kGroups;
 constexpr int kKeys = kWarps * kWarpKeys;  // of a tile
 constexpr int kThreads = 32 * kWarps;
 // Parts of one tile of 128 keys: a border moves less than with two (the 16-bit
-// kernels' tiles are of 64; 64 sequences of 512 to 2048 took 41.5 us, with three
-// 43, now 40.3).
+// kernels' tiles are of 64; the drafts of 64 sequences of 512 to 2048 took 41.5 us
+// with two, 43 with three, 40 so).
 constexpr int kLeast4 = kItemCost + 1;
 constexpr int kStages = 3;     // tiles of a warp's ring: one is worked on, two are on their way
 // Query rows of a KV head above which the tcgen05 kernel is faster.  64 sequences
 // of 512 to 2048 positions, and 4 of 30000 to 32768, take here and there: of 64
-// elements, 24 rows 31 and 51 us, 39 and 72; 48 rows 42 and 51, 50 and 71; 64
-// rows 51 and 51, 56 and 69; of 128, 32 rows 86 and 103, 96 and 137; 48 rows 115
-// and 104, 126 and 138; 64 rows 151 and 104, 159 and 138.
+// elements, 24 rows 30 and 51 us, 39 and 71; 48 rows 41 and 51, 48 and 70; 64
+// rows 51 and 51, 56 and 70; of 128, 32 rows 85 and 102, 95 and 137; 48 rows 113
+// and 104, 125 and 138; 64 rows 147 and 105, 157 and 138.
 constexpr int most_rows(int dim) { return dim == 64 ? 64 : 48; }
 
 // The products are in fp16 whatever the cache's type is, since codes get there
@@ -710,7 +710,8 @@ int launch_rows(const AttnArgs& a, cudaStream_t st) {
 // rows: query rows of a KV head that most sequences have.  They make as few
 // items as can be, of up to four n-tiles, and as many n-tiles in each: a
 // part's rows cost their softmax whether they are there or not (40 rows as 24 and
-// 16 take 42 us in the first of the cases above, as 32 and 8 they took 52).
+// 16 take 40 us in the first of the cases above, as 32 and 8 they took 52 when they
+// were 43).
 template <typename T, int D>
 int launch(const AttnArgs& a, long long rows, cudaStream_t st) {
     const long long tiles = (rows + 7) / 8, items = (tiles + 3) / 4, each = (tiles + items - 1) / items;

@@ -135,3 +135,51 @@ def test_steps_as_a_graph(torch):
         assert int(one.err) == 0 and int(two.err) == 0
         assert all(bool((a == b).all()) for a, b in zip(one.state(), two.state()))
     assert int(one.lens.min()) > 2 * PAGE
+
+
+def test_forked_pages(torch):
+    """A page copied in its codes and scale words is the same page to a sequence
+    that holds the copy."""
+    case = ref4.Case4(torch, [(3, 75), (2, 40)], 8, 2, 128, 16, seed=6, hide=True)
+    ws = ref.new_workspace(torch)
+    ib.paged4_attention(case.out, case.q, case.cache(), case.batch(), ws, lse=case.lse, err=case.err)
+    out, lse = case.out.clone(), case.lse.clone()
+    n = case.kc.shape[0]
+    codes = torch.zeros(2, 2 * n, *case.kc.shape[1:], dtype=torch.uint8, device="cuda")
+    codes[0, :n], codes[1, :n] = case.kc, case.vc
+    words = torch.zeros(1, 2 * n, *case.scales.shape[1:], dtype=torch.int32, device="cuda")
+    words[0, :n] = case.scales
+    order = list(range(n, 2 * n))[::-1]
+    ib.copy_pages(codes, list(range(n)), order)
+    ib.copy_pages(words, list(range(n)), order)
+    codes[:, :n], words[:, :n] = 0, -1
+    table = torch.tensor(order, dtype=torch.int32, device="cuda")[case.table.long().clamp(0, n - 1)].contiguous()
+    batch = ib.RaggedBatch(case.q_start, case.kv_len, table, case.rows, case.max_q)
+    case.out.fill_(7)
+    ib.paged4_attention(case.out, case.q, ib.PagedCache4(codes[0], codes[1], words[0], case.dtype), batch, ws, lse=case.lse,
+                        err=case.err)
+    torch.cuda.synchronize()
+    assert int(case.err) == 0 and bool((out == case.out).all()) and bool((lse == case.lse).all())
+
+
+def test_models_on_streams_of_their_own(torch):
+    """Two models' steps at once, each on its stream with its workspaces, are
+    what they are one after the other."""
+    alone = []
+    for seed in (2, 3):
+        m = Model(torch, seed)
+        for _ in range(6):
+            m.step()
+        torch.cuda.synchronize()
+        assert int(m.err) in (0, 1 << 5)
+        alone.append(m.state())
+    both, streams = [Model(torch, seed) for seed in (2, 3)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for m, stream in zip(both, streams):
+            with torch.cuda.stream(stream):
+                m.step()
+    torch.cuda.synchronize()
+    for m, want in zip(both, alone):
+        for x, y in zip(m.state(), want):
+            assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
