@@ -54,17 +54,37 @@ __device__ __forceinline__ void join(Range4& r, int lanes) {
     }
 }
 
+// A vector's scale, zero and word.  k is the whole number nearest to x / s, a
+// tie's even one, which is the rounding of the correctly rounded quotient too:
+// s has four bits, so x - (k + 1/2) s is a whole number of x's last places, and
+// one of them is more than half a last place of x / s.
+constexpr float kWhole = 12582912.0f;  // 1.5 x 2^23 brings a whole number into the low bits
 struct Scale4 {
     float s, z;
+    float inverse;  // 1 / s
+    bool far;       // a rounding may carry a value past the largest number of T, or the vector is not finite
     uint32_t word;
 };
+// The low bits: k + those of kWhole.  k by x (1 / s) is off by one at most, near
+// ties, which the exact x - k s shows.
+__device__ __forceinline__ int nearest(float x, const Scale4& q) {
+    const float t = __fmaf_rn(x, q.inverse, kWhole);
+    const float r = __fmaf_rn(-__fadd_rn(t, -kWhole), q.s, x);
+    const int bits = __float_as_int(t), sign = __float_as_int(r) >> 31;  // 0 or -1
+    // past the tie, or at it with an odd k
+    const bool off = (__float_as_int(r) & 0x7fffffff) + (bits & 1) > __float_as_int(0.5f * q.s);
+    return off ? bits + (sign | 1) : bits;
+}
 template <typename T>
 __device__ __forceinline__ Scale4 scale_of(const Range4& r) {
     Scale4 q;
-    const bool fine = r.hi <= kLargest4<T> && r.lo >= -kLargest4<T>;  // (false for NaN)
+    const float most = max_of(r.hi, -r.lo, 0.0f);
+    const bool fine = most <= kLargest4<T>;  // (false for NaN)
     // halves of both sides: the range of numbers near the largest would be infinite
     const float s = __fdiv_rn(0.5f * r.hi - 0.5f * r.lo, 7.5f);
     q.s = fine ? fmaxf(__uint_as_float((__float_as_uint(s) + 0xfffffu) & ~0xfffffu), kLeastScale4<T>) : 1.0f;
+    q.inverse = __frcp_rn(q.s);
+    q.far = !(most <= 0.5f * kLargest4<T>);
     q.z = fminf(rintf(__fdiv_rn(-r.lo, q.s)), 15.0f);
     q.word = fine ? (__float_as_uint(q.s) >> 16) | (uint32_t)q.z : kNotFinite4;
     return q;
@@ -73,6 +93,12 @@ __device__ __forceinline__ Scale4 scale_of(const Range4& r) {
 template <typename T, int N>
 __device__ __forceinline__ uint32_t codes_of(const float (&x)[N], const Scale4& q) {
     uint32_t c = 0;
+    if (!q.far) {
+        const int up = (int)q.z - __float_as_int(kWhole);
+#pragma unroll
+        for (int i = 0; i < N; ++i) c |= (uint32_t)max(min(nearest(x[i], q) + up, 15), 0) << (4 * i);
+        return c;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         float k = rintf(__fdiv_rn(x[i], q.s));
@@ -99,10 +125,10 @@ __device__ __forceinline__ void turn64(float& x, float& y, double2 cs) {
 // The blocks and units of paged_rope_wide (paged_rope.cu): a block per token
 // row, a thread two blocks of eight values of a head, D / 16 threads a head.
 // These find the head's range by shuffles and store a word of codes per block.
-// 8192 bf16 rows of 32/8 heads of 128, 176 MB: 45 us, 3.9 TB/s; bound by
-// instructions, most of them a K or V value's division, rounding and packing
-// (Q alone takes 33), with more blocks an SM as fast.  Divisions by a product with 1 /
-// s and an exact look at its remainder took 10 us more.  320 FP32 rows: 7.5 us.
+// 8192 bf16 rows of 32/8 heads of 128, 176 MB: 42 us, 4.2 TB/s; bound by
+// instructions, most of them a K or V value's rounding and packing (Q alone
+// takes 33; with divisions in place of nearest 45), with more blocks an SM as
+// fast.  320 FP32 rows: 7.5 us.
 constexpr int kAhead4 = 3;
 
 template <typename S, typename T, bool INTERLEAVED>
