@@ -193,6 +193,31 @@ def test_largest_least_and_zero(torch, dtype, big):
     assert bool((off[[2, 3, 4]] <= 0.5 + 2.0 ** -20).all()) and not bool(got[3].any())
 
 
+@pytest.mark.parametrize("rotary", [64, 62])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_ties_go_to_the_even_code(torch, dtype, rotary):
+    """Values halfway between two of the scale's steps, and some last places of
+    FP32 to either side of it: every code is that of the exact quotient."""
+    n = 400
+    a = Append(torch, [(n, n)], 2, 1, 64, 16, dtype, "fp32")
+    g = torch.Generator(device="cuda").manual_seed(8)
+    m, e = (torch.randint(lo, hi, (n, 1), generator=g, device="cuda") for lo, hi in ((8, 16), (-15, 4)))
+    s = torch.ldexp(m.double(), e)
+    zero = torch.randint(0, 16, (n, 1), generator=g, device="cuda")
+    k = torch.randint(0, 15, (n, 64), generator=g, device="cuda") - zero
+    x = ((k + 0.5) * s).float()
+    x = (x.view(torch.int32) + torch.randint(-2, 3, x.shape, generator=g, device="cuda", dtype=torch.int32)).view(torch.float32)
+    x[:, 0], x[:, 1] = (-zero * s)[:, 0].float(), ((15 - zero) * s)[:, 0].float()  # the range: 15 s
+    a.vn[:, 0] = x
+    a.run(ib.RopeParams(theta=10000.0, rotary_dim=rotary))
+    rows, pages, at, pos = a.places()
+    kw, vw = ref4.split_words(a.case.scales)
+    want, want_s, want_zero = ref4.quantise(torch, x, dtype)
+    assert bool((want_s == s[:, 0]).all()) and bool((want_zero == zero[:, 0]).all())
+    assert bool((vw[pages, 0, at] == ref4.word(torch, want_s, want_zero)).all())
+    assert bool((a.case.vc[pages, 0, at] == ref4.pack(want)).all())
+
+
 def test_only_q_and_only_k(torch):
     a = Append(torch, [(3, 40)], 4, 2, 64, 16, "bf16", "bf16")
     c = a.case
