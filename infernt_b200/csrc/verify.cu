@@ -64,11 +64,8 @@ __device__ __forceinline__ double sharpness64(float t) {
     return fmin(fmax(1.4426950408889634074 / (double)t, 1e-30), 1e30);
 }
 
-// What a logit or a probability may not be.
-template <bool PROBS>
-__device__ __forceinline__ bool is_none(float x) {
-    return !(x < INFINITY) || (PROBS && x < 0.0f);
-}
+// What a probability may not be.
+__device__ __forceinline__ bool is_none(float x) { return !(x < INFINITY) || x < 0.0f; }
 
 // 16 bytes of a row as FP32
 __device__ __forceinline__ void sixteen(const float* p, float (&x)[4]) {
@@ -285,7 +282,7 @@ __device__ __forceinline__ RowPart row_stats(const VerifyArgs& a, int r, float c
 template <typename L>
 __device__ __forceinline__ float probability(const VerifyArgs& a, int r, int e) {
     const float p = element(static_cast<const L*>(a.target) + (long long)r * a.ld + e);
-    return is_none<true>(p) ? -1.0f : p;
+    return is_none(p) ? -1.0f : p;
 }
 __device__ __forceinline__ float in_unit(float u) { return u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f; }
 
@@ -438,7 +435,7 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
     constexpr float kOutside = PROBS ? 0.0f : -INFINITY;  // has no weight
     auto weight = [&](float l) {                          // e, or p
         if (!PROBS) return exp2_64(fma((double)fmaxf(l, least), c64, cm), roots);
-        bad |= is_none<true>(l);
+        bad |= is_none(l);
         return (double)l;
     };
     // the weight that is drawn from; minus as in Stop
