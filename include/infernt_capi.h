@@ -817,7 +817,8 @@ INFERNT_API int infernt_paged_batch_plan(const infernt_page_tables* tables, cons
  * token outside [0, vocab_size) (it is rejected, the token drawn from p).
  * Sums for acceptance in FP32; the drawn token's weights, sums and borders in
  * 64 bits, so a token is the formula's own except within about 1e-13 of a
- * border (an acceptance within about 1e-6 of u q = p).  u below 0 or NaN is
+ * border (an acceptance within about 1e-6 of u q = p); probabilities of
+ * 1e-298 of the row's largest and below count as 0.  u below 0 or NaN is
  * taken as 0, from 1 on as the largest below 1; elements of draft_probs that
  * are not finite give weight 0.  workspace: infernt_verify_drafts_workspace_bytes(num_rows,
  * num_seqs) bytes, 16-byte aligned, of any content (calls that share it must

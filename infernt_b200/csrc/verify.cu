@@ -227,12 +227,12 @@ __device__ __forceinline__ double warp_sum64(double v) {
     return v;
 }
 
-// 2^x for x <= 0 above -1000, to about 2e-15: x = (32 n + j) / 32 + g, |g| <= 1 /
-// 64, so 2^x = 2^n 2^(j / 32) 2^g, the last by its Taylor series to the fifth
-// power (the sixth is below (ln 2 / 64)^6 / 720 = 2e-15), the middle one of the
-// 32 roots (in shared memory; from lane to lane by shuffles a call took 3 us
-// more).  The constants are in constant memory, where the operations take them
-// from without a move.
+// 2^x for x up to 0, from -1000 on (below it as at -1000, -infinity too), to
+// about 2e-15: x = (32 n + j) / 32 + g, |g| <= 1 / 64, so 2^x = 2^n 2^(j / 32)
+// 2^g, the last by its Taylor series to the fifth power (the sixth is below (ln 2
+// / 64)^6 / 720 = 2e-15), the middle one of the 32 roots (in shared memory; from
+// lane to lane by shuffles a call took 3 us more).  The constants are in constant
+// memory, where the operations take them from without a move.
 struct Exp2Constants {
     double big, back;  // 1.5 x 2^52 rounds 32 x to a whole number in its low bits
     double c[6];       // (ln 2)^k / k!
@@ -242,6 +242,8 @@ __constant__ Exp2Constants kExp2 = {6755399441055744.0,
                                     {1.0, 0.69314718055994530942, 0.24022650695910071233, 0.05550410866482157995,
                                      0.00961812910762847716, 0.00133335581464284434}};
 __device__ __forceinline__ double exp2_64(double x, const double* roots) {
+    // of negative numbers the high words ascend with the magnitude (-1000: 0xc08f4000); those of others are lower
+    x = __hiloint2double((int)min((unsigned)__double2hiint(x), 0xc08f4000u), __double2loint(x));
     const double t = fma(x, 32.0, kExp2.big);
     const int k = __double2loint(t);
     const double g = fma(t - kExp2.big, kExp2.back, x);
@@ -426,15 +428,17 @@ __global__ void __launch_bounds__(kDrawThreads, kDrawPerSm) verify_draw(const __
     const int sub = (per + kSubs - 1) / kSubs;
     const int g0 = min(groups, ((int)rank * kDrawWarps + warp) * per), g1 = min(groups, g0 + per);
     const int d = st.minus == 2 ? a.tokens[stop + 1] : -1;
-    const double cm = -c64 * (double)st.m;
-    // Logits are held to 2^-1000 of the largest, and weights up to 2^-990 are 0: those of tokens that are not allowed.
-    const float least = fmaxf((float)((double)st.m - 999.0 / c64), -3.4028235e38f);
-    constexpr double kLeastWeight = PROBS ? 0.0 : 9.555938177272168e-299;  // 2^-990
+    // x = c l - c m in one operation, off by what the rounding of c m is: the same for all of a row, so no matter, as
+    // long as it is small.  From c = 2^35 / |m| on the next FP32 number below m has a weight of 2^-2048 or less, which
+    // is 0 here, so a larger c (temperatures from |m| 2^-35 down) changes nothing, and c m stays below 2^35.
+    const double c_draw = fmin(c64, 34359738368.0 / fabs((double)st.m)), cm = -c_draw * (double)st.m;
+    // weights up to 2^-990 are 0: those of tokens that are not allowed, among others
+    constexpr double kLeastWeight = PROBS ? 0.0 : 9.555938177272168e-299;
     bool bad = false;
     double z = 1.0;
     constexpr float kOutside = PROBS ? 0.0f : -INFINITY;  // has no weight
     auto weight = [&](float l) {                          // e, or p
-        if (!PROBS) return exp2_64(fma((double)fmaxf(l, least), c64, cm), roots);
+        if (!PROBS) return exp2_64(fma((double)l, c_draw, cm), roots);
         bad |= is_none(l);
         return (double)l;
     };
