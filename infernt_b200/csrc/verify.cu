@@ -150,8 +150,9 @@ __global__ void __launch_bounds__(kStatThreads) verify_rows(const VerifyArgs a) 
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 top = fmaxf(top, x[i][j]);
-                // (what lies outside the row is -infinity)
-                bad |= PROBS ? !(x[i][j] < INFINITY) || (x[i][j] < 0.0f && x[i][j] > -INFINITY) : !(x[i][j] < INFINITY);
+                // what lies outside the row is -infinity, which in it a logit may be and a probability not
+                const int k = base + (i * kStatThreads + tid) * N + j;
+                bad |= PROBS ? is_none(x[i][j]) && k >= 0 && k < a.V : !(x[i][j] < INFINITY);
             }
         const float ref = fmaxf(m, top);
         if (!greedy && ref > -INFINITY) {
