@@ -711,10 +711,10 @@ int launch_rows(const AttnArgs& a, cudaStream_t st) {
 // items as can be, of up to four n-tiles, and as many n-tiles in each: a
 // part's rows cost their softmax whether they are there or not (40 rows as 24 and
 // 16 take 40 us in the first of the cases above, as 32 and 8 they took 52 when they
-// were 43).
+// were 43).  rows may be 0: the kernel then has the sequences' error bits to set.
 template <typename T, int D>
 int launch(const AttnArgs& a, long long rows, cudaStream_t st) {
-    const long long tiles = (rows + 7) / 8, items = (tiles + 3) / 4, each = (tiles + items - 1) / items;
+    const long long tiles = std::max(1ll, (rows + 7) / 8), items = (tiles + 3) / 4, each = (tiles + items - 1) / items;
     if (each <= 1) return launch_rows<T, D, 1>(a, st);
     if (each == 2) return launch_rows<T, D, 2>(a, st);
     if (each == 3) return launch_rows<T, D, 3>(a, st);
