@@ -63,6 +63,11 @@ constexpr float kMostWeight = 16384.0f;
 // Scales below it (vectors of zeros have the least) do not lower m further, and
 // m moves too where a 2^(s - m) passes 2^80: their sum stays in FP32.
 constexpr float kLeastLog = -40.0f, kMostSingle = 1.2089258196146292e24f;
+// sum + l 2^d, d <= 0, for sums of weights: the m of two parts are up to 165 apart
+// by their V scales alone, and their sums as far the other way.
+__device__ __forceinline__ float add_lowered(float sum, float l, float d) {
+    return fmaf(l * ex2(fminf(d + 120.0f, 0.0f)), ex2(fmaxf(d, -120.0f)), sum);
+}
 
 // Shared memory: a ring of its own for each warp, per stage the codes of its K
 // and V rows and their scale words.  When a part is done the ring is empty, and
@@ -474,10 +479,10 @@ __device__ __forceinline__ void consume(const AttnArgs& a, const PagedSeq& seq, 
                         }
                         const unsigned bit = 1u << (2 * n + e);
                         if (set & bit ? high_w > kMostWeight || high_p > kMostSingle : top != -INFINITY) {
-                            const float x = set & bit ? ex2(s.m[n][e] - top) : 0.0f;
+                            const float down = set & bit ? s.m[n][e] - top : -INFINITY, x = ex2(down);
                             set |= bit;
                             s.m[n][e] = top;
-                            s.l[n][e] *= x;
+                            s.l[n][e] = add_lowered(0.0f, s.l[n][e], down);
 #pragma unroll
                             for (int b = 0; b < KC; ++b) {
                                 s.acc[n][b][e] *= x;
@@ -580,15 +585,15 @@ __device__ __forceinline__ void join_item(const AttnArgs& a, const PagedSeq& seq
                 if (b + i > p.last) mb[i] = -INFINITY;
                 up = fmaxf(up, mb[i]);
             }
-            const float f = top == -INFINITY ? 0.0f : ex2(top - up);
+            const float down = top == -INFINITY ? top : top - up, f = ex2(down);
             top = up;
-            l *= f;
+            l = add_lowered(0.0f, l, down);
             o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 // (of a row whose scores are NaN, m is -infinity and l NaN)
-                const float w = mb[i] == -INFINITY ? 0.0f : ex2(mb[i] - top);
-                l = fmaf(lb[i], w, l);
+                const float d = mb[i] == -INFINITY ? mb[i] : mb[i] - top, w = ex2(d);
+                l = add_lowered(l, lb[i], d);
                 o.x = fmaf(v[i].x, w, o.x);
                 o.y = fmaf(v[i].y, w, o.y);
                 o.z = fmaf(v[i].z, w, o.z);
@@ -653,9 +658,9 @@ __global__ void __launch_bounds__(kThreads, (Layout<D, RB>::kPerSm)) paged4_attn
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
                 const float* set = sets + w * (L::kRing / 4);
-                const float f = m[w] == -INFINITY ? 0.0f : ex2(m[w] - top);
+                const float d = m[w] == -INFINITY ? m[w] : m[w] - top, f = ex2(d);
                 const float4 v = *reinterpret_cast<const float4*>(set + set_at<D>(r, i, gg));
-                l = fmaf(set[M * D + M + r], f, l);
+                l = add_lowered(l, set[M * D + M + r], d);
                 o.x = fmaf(v.x, f, o.x);
                 o.y = fmaf(v.y, f, o.y);
                 o.z = fmaf(v.z, f, o.z);

@@ -21,6 +21,28 @@ def workspace(torch):
     return ref.new_workspace(torch)
 
 
+@pytest.mark.parametrize("n", [1, 5])
+@pytest.mark.parametrize("length", [33, 129, 161, 289, 20001])
+@pytest.mark.parametrize("power", [40, 90])
+def test_zeros_beside_large_values(torch, workspace, n, length, power):
+    """One warp, and one CTA, has keys with V vectors of zeros alone, the others
+    large ones: each one's weights still count in the sum."""
+    def stretch(k, v):
+        for s, (_, l) in enumerate(seqs):
+            at = torch.arange(l, device="cuda")
+            pages = torch.tensor(case.pages[s], device="cuda")[at // 16]
+            zero = (at >= l // 32 * 32) | (at < l // 3)  # the first third, and the last part of 32
+            v[pages[zero], :, at[zero] % 16] = 0.0
+        return k, v
+
+    seqs = [(n, length), (n, 64)]
+    case = ref4.Case4(torch, seqs, 4, 2, 128, 16, "bf16", seed=n)  # whose pages the next one has too
+    case = ref4.Case4(torch, seqs, 4, 2, 128, 16, "bf16", seed=n,
+                      stretch=lambda k, v: stretch(k * 0.1, v * 2.0 ** power))
+    run(torch, case, workspace)
+    ref.check_attention(case)
+
+
 @pytest.mark.parametrize("four", [True, False])
 def test_a_call_for_no_new_tokens(torch, workspace, four):
     """max_q_len 0: sequences without new tokens leave all rows; one that has
