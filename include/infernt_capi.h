@@ -727,7 +727,8 @@ INFERNT_API int infernt_paged4_rope_append(void* q_out, int ldo, const void* q, 
  * workspace (the same bytes; calls that share it must not overlap, of either
  * kind) and error bits, over the values that the codes stand for.  Any page
  * size is served alike.  A V vector of NaN makes the results of the rows that
- * see it NaN. */
+ * see it NaN.  Beside V vectors of a scale 2^x, x above 90, weights below 2^(x -
+ * 130) of a row's largest may count as 0. */
 INFERNT_API int infernt_paged4_attention(void* out, int ldo, const void* q, int ldq, int nq,
                                          const infernt_paged_cache4* cache, const infernt_ragged_batch* batch,
                                          int window, int sinks, float scale, float* lse, void* workspace,

@@ -60,10 +60,13 @@ constexpr int most_rows(int dim) { return dim == 64 ? 64 : 48; }
 // down to 2^-18 of it.
 constexpr float kUp = 4.0f;
 constexpr float kMostWeight = 16384.0f;
-// Scales below it (vectors of zeros have the least) do not lower m further, and
-// m moves too where a 2^(s - m) passes 2^80: their sum stays in FP32.
-constexpr float kLeastLog = -40.0f, kMostSingle = 1.2089258196146292e24f;
-// sum + l 2^d, d <= 0, for sums of weights: the m of two parts are up to 165 apart
+// Scales below 2^-92 (the least is 2^-100, of vectors of zeros too) do not lower
+// m further, and m moves too where a 2^(s - m) passes 2^97: the sum of 2^30 of
+// them stays in FP32.  Weights beside the least scale are 2^-4 to 2^-3 at a row's
+// largest, and normal numbers down to 2^-10 of it.  At the other end, beside V
+// vectors of scale 2^x, a 2^(s - m) below 2^(x - 130) of the row's largest is 0.
+constexpr float kLeastLog = -92.0f, kMostSingle = 1.5845632502852868e29f;
+// sum + l 2^d, d <= 0, for sums of weights: the m of two parts are up to 217 apart
 // by their V scales alone, and their sums as far the other way.
 __device__ __forceinline__ float add_lowered(float sum, float l, float d) {
     return fmaf(l * ex2(fminf(d + 120.0f, 0.0f)), ex2(fmaxf(d, -120.0f)), sum);

@@ -21,6 +21,17 @@ def workspace(torch):
     return ref.new_workspace(torch)
 
 
+@pytest.mark.parametrize("n", [1, 5, 70])
+@pytest.mark.parametrize("power", [-95, -80, -64, -50, 60, 115])
+def test_v_vectors_all_tiny_or_all_large(torch, workspace, n, power):
+    """Every V vector 2^power times an ordinary one: the bound is relative to
+    the largest of them."""
+    case = ref4.Case4(torch, [(n, 300), (n, 5000), (n, n)], 8, 2, 64, 16, "bf16", seed=n,
+                      stretch=lambda k, v: (k, v * 2.0 ** power))
+    run(torch, case, workspace)
+    ref.check_attention(case, rows=range(0, n, 23))
+
+
 @pytest.mark.parametrize("n", [1, 5])
 @pytest.mark.parametrize("length", [33, 129, 161, 289, 20001])
 @pytest.mark.parametrize("power", [40, 90])
