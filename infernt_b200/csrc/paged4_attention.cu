@@ -245,8 +245,9 @@ __device__ __forceinline__ uint32_t largest_of(const uint4 (&q)[W]) {
         }
     return __reduce_max_sync(0xffffffffu, top);
 }
-// The power of two that brings it to 2^14 (within what both it and its inverse can be).
-__device__ __forceinline__ int shift_of(uint32_t top) { return min(max(14 - ((int)(top >> 23) - 127), -100), 100); }
+// The power of two that brings it to 2^14: -113 for the largest numbers of bf16, at
+// most 126 (rows below 2^-112), so that it and its inverse are normal numbers.
+__device__ __forceinline__ int shift_of(uint32_t top) { return min(14 - ((int)(top >> 23) - 127), 126); }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }
 
 // The tiles [j0, j1) of an item, 32 keys of each by every warp.

@@ -54,6 +54,22 @@ def test_zeros_beside_large_values(torch, workspace, n, length, power):
     ref.check_attention(case)
 
 
+@pytest.mark.parametrize("n", [1, 9, 70])
+@pytest.mark.parametrize("power", [-120, -60, 60, 110, 124])
+def test_queries_of_every_size(torch, workspace, n, power):
+    """Queries 2^power times ordinary ones, keys as much smaller as the format
+    goes: scores in FP32 as ever."""
+    back = 2.0 ** -min(power, 94)
+    case = ref4.Case4(torch, [(n, 200), (n, n + 3)], 8, 2, 64, 16, "bf16", seed=n,
+                      stretch=lambda k, v: (k * back, v))
+    case.q = (case.q.double() / 8 * 2.0 ** power).to(case.dtype)
+    assert bool(case.q.isfinite().all())
+    scale = 2.0 ** -max(0, power - 94) / 8
+    run(torch, case, workspace, scale=scale)
+    ref.check_attention(case, scale=scale, rows=range(0, n, 9))
+    assert bool(case.out[:case.starts[-1]].isfinite().all())
+
+
 @pytest.mark.parametrize("four", [True, False])
 def test_a_call_for_no_new_tokens(torch, workspace, four):
     """max_q_len 0: sequences without new tokens leave all rows; one that has
