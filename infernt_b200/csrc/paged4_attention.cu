@@ -740,23 +740,27 @@ extern "C" int infernt_paged4_attention(void* out, int ldo, const void* q, int l
     using namespace infernt;
     const char* op = "paged4_attention";
     if (int s = check_paged_cache4(op, cache)) return s;
+    if (int s = check_ragged_batch(op, batch)) return s;
     const infernt_paged_cache geometry = geometry4(*cache);
+    const int D = cache->head_dim, G = nq / cache->num_kv_heads;
+    // Sequences of up to most_rows query rows a KV head are bound by their keys,
+    // longer ones by their products.  Where the batch's counts do not say that
+    // all sequences are as long as the longest, each kernel takes its own.
+    const long long most = (long long)batch->max_q_len * G, all = (long long)batch->num_rows * G;
+    const bool chunks = most > most_rows(D), both = chunks && batch->num_rows < (long long)batch->num_seqs * batch->max_q_len;
+    // of the kernels that run; the few-row kernel's sequences have most_rows at most
+    const WorkBound long_rows = {all, kTcItemRows, kTcTileKeys},
+                    few_rows = {std::min(all, (long long)batch->num_seqs * most_rows(D)), 8, kKeys},
+                    first = chunks ? long_rows : few_rows;
     AttnArgs a;
     bool empty;
-    // tiles of both kernels, for the bound on the call's work: the smaller of each
-    if (int s = attention_args(op, out, ldo, q, ldq, nq, &geometry, batch, window, sinks, scale, lse, workspace, err, 8,
-                               kTcTileKeys, &a, &empty))
+    if (int s = attention_args(op, out, ldo, q, ldq, nq, &geometry, batch, window, sinks, scale, lse, workspace, err,
+                               {first, both ? few_rows : first}, &a, &empty))
         return s;
     if (empty) return INFERNT_OK;
     if (int s = check_device_pointer(op, "the scales", cache->scales)) return s;
     a.scales = cache->scales;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int D = cache->head_dim;
-    // Sequences of up to most_rows query rows a KV head are bound by their keys,
-    // longer ones by their products.  Where the batch's counts do not say that
-    // all sequences are as long as the longest, each kernel takes its own.
-    const long long most = (long long)batch->max_q_len * a.G;
-    const bool chunks = most > most_rows(D), both = chunks && batch->num_rows < (long long)batch->num_seqs * batch->max_q_len;
     if (!chunks || both) {
         // rows of an item: those of the longest sequence, or, beside a chunk, what the others have on average
         long long rows = most;

@@ -526,7 +526,7 @@ namespace infernt {
 
 int attention_args(const char* op, void* out, int ldo, const void* q, int ldq, int nq, const infernt_paged_cache* cache,
                    const infernt_ragged_batch* batch, int window, int sinks, float scale, float* lse, void* workspace,
-                   unsigned* err, int item_rows, int tile_keys, AttnArgs* args, bool* empty) {
+                   unsigned* err, std::initializer_list<WorkBound> work, AttnArgs* args, bool* empty) {
     if (int s = check_paged_cache(op, cache)) return s;
     if (int s = check_ragged_batch(op, batch)) return s;
     INFERNT_REQUIRE(q && out && workspace, "%s: null pointer", op);
@@ -546,10 +546,11 @@ int attention_args(const char* op, void* out, int ldo, const void* q, int ldq, i
     INFERNT_REQUIRE((long long)batch->num_rows * G < kMaxPositions, "%s: %d rows of %d heads", op, batch->num_rows, nq);
     // the units of the schedule are counted in 32 bits
     const long long most_kv = std::min<long long>((long long)batch->table_stride * cache->page_size, kMaxPositions);
-    const long long items = ((long long)batch->num_rows * G / item_rows + batch->num_seqs) * nkv;
-    INFERNT_REQUIRE(items < (1ll << 30) / (most_kv / tile_keys + 2 + kItemCost),
-                    "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
-                    most_kv);
+    for (const WorkBound& w : work)
+        INFERNT_REQUIRE((w.rows / w.item_rows + batch->num_seqs) * nkv <
+                            (1ll << 30) / (most_kv / w.tile_keys + 2 + kItemCost),
+                        "%s: %d rows of %d heads over up to %lld positions (split the call)", op, batch->num_rows, nq,
+                        most_kv);
     *empty = batch->num_seqs == 0 || batch->num_rows == 0;
     if (*empty) return INFERNT_OK;
     if (int s = check_batch_pointers(op, cache, batch, err)) return s;
@@ -595,10 +596,12 @@ extern "C" int infernt_paged_attention(void* out, int ldo, const void* q, int ld
     if (int s = check_ragged_batch(op, batch)) return s;
     const int D = cache->head_dim, nkv = cache->num_kv_heads, G = nq / nkv;
     const bool chunks = paged_attention_boxes(cache->page_size) && (long long)batch->max_q_len * G > kItemRows;
+    const WorkBound work = {(long long)batch->num_rows * G, chunks ? kTcItemRows : kItemRows,
+                            chunks ? kTcTileKeys : kTileKeys};
     AttnArgs a;
     bool empty;
     if (int s = attention_args(op, out, ldo, q, ldq, nq, cache, batch, window, sinks, scale, lse, workspace, err,
-                               chunks ? kTcItemRows : kItemRows, chunks ? kTcTileKeys : kTileKeys, &a, &empty))
+                               {work}, &a, &empty))
         return s;
     if (empty) return INFERNT_OK;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

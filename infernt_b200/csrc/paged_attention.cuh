@@ -5,6 +5,8 @@
 
 #include <cuda.h>
 
+#include <initializer_list>
+
 #include "paged.cuh"
 
 namespace infernt {
@@ -75,13 +77,18 @@ int paged_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_ot
 // The same over pages of 4 bits; the other kernel is paged4_attn.
 int paged4_attention_tc(const AttnArgs& a, int head_dim, int dtype, bool after_other, cudaStream_t st);
 
-// Checks of an attention call's arguments and its AttnArgs but for `scales`
-// (paged_attention.cu).  Items of at least item_rows query rows (but for a
-// sequence's last) and tiles of at least tile_keys keys bound its work;
-// *empty: nothing to do.
+// What a kernel of a call has to do at most: `rows` query rows of a KV head, as
+// items of at least item_rows (but for a sequence's last), over tiles of at
+// least tile_keys keys.
+struct WorkBound {
+    long long rows;
+    int item_rows, tile_keys;
+};
+// Checks of an attention call's arguments, the work of its kernels among them,
+// and its AttnArgs but for `scales` (paged_attention.cu); *empty: nothing to do.
 int attention_args(const char* op, void* out, int ldo, const void* q, int ldq, int nq, const infernt_paged_cache* cache,
                    const infernt_ragged_batch* batch, int window, int sinks, float scale, float* lse, void* workspace,
-                   unsigned* err, int item_rows, int tile_keys, AttnArgs* args, bool* empty);
+                   unsigned* err, std::initializer_list<WorkBound> work, AttnArgs* args, bool* empty);
 
 // Rows [row0, row0 + rows) of the query rows of (sequence, KV head), and the
 // keys that they see: [0, sink_end) and [lo, hi), as tiles of N keys.

@@ -85,3 +85,19 @@ def test_a_call_for_no_new_tokens(torch, workspace, four):
     call(case.out, case.q, cache, case.batch(), workspace, lse=case.lse, err=case.err)
     torch.cuda.synchronize()
     assert int(case.err) == 16 and bool((case.out == 7).all())
+
+
+@pytest.mark.parametrize("rest", [0, 3])
+def test_a_long_chunk_over_a_wide_table(torch, workspace, rest):
+    """8192 tokens of 64/8 heads, alone and beside sequences of a few, in a
+    table of 2^20 positions: the same rows as in one that just holds them."""
+    case = ref4.Case4(torch, [(8192, 8500), (rest, 300), (rest, 700)], 64, 8, 64, 1024, "bf16", seed=1)
+    run(torch, case, workspace)
+    out, lse = case.out.clone(), case.lse.clone()
+    ref.check_attention(case, rows=[0, 1, 2, 5000, 8191])
+    wide = torch.full((3, 1024), -1, dtype=torch.int32, device="cuda")
+    wide[:, :case.table.shape[1]] = case.table
+    case.table = wide
+    case.out.fill_(7)
+    run(torch, case, workspace)
+    assert bool((out == case.out).all()) and bool((lse == case.lse).all())
