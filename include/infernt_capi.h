@@ -699,7 +699,8 @@ INFERNT_API int infernt_batch_engine_copy_pages(infernt_batch_engine* e, const i
  * 2^-100 (bf16) or 2^-21 (fp16).  Word: the upper twelve bits of s as a bf16,
  * z in the low four.  scales has the K vector's word in the low half of each
  * element, the V vector's in the high half.  A vector with a value that is
- * not finite in the cache's type is stored as one of NaN.
+ * NaN, or larger than the largest number of the cache's type, is stored as one
+ * of NaN.
  *
  * k and v 16-byte aligned; page numbers, block tables and infernt_pages_copy
  * (for pools whose pages are multiples of 16 bytes) as for 16-bit pools. */
@@ -715,9 +716,11 @@ typedef struct infernt_paged_cache4 {
 } infernt_paged_cache4;
 
 /* infernt_paged_rope_append into such pages, its arguments, rows and error
- * bits.  q_out as there; K is turned in 64 bits and rounded once to FP32
- * before it is held in 4 bits, so what a page holds does not depend on the
- * last bits of an FP32 sine. */
+ * bits.  q_out as there (cosines and sines may be rounded from 64 bits, so its
+ * last bits may differ from there, and with whether k is given and how rows are
+ * aligned); K is turned in 64 bits and rounded once to FP32 before it is held
+ * in 4 bits, so what a page holds does not depend on the last bits of an FP32
+ * sine. */
 INFERNT_API int infernt_paged4_rope_append(void* q_out, int ldo, const void* q, int ldq, int nq, const void* k,
                                            int ldk, const void* v, int ldv, int src_dtype,
                                            const infernt_paged_cache4* cache, const infernt_ragged_batch* batch,

@@ -12,9 +12,10 @@
 // take either the values or the whole numbers c - z with s applied to the
 // sums, and both are exact (with a scale of bf16's eight bits the values would
 // be rounded in one kernel and not in the other).  The step is at most 1/8
-// wider than the range needs; |x_i - value| <= s / 2 always.
+// wider than the range needs, or kLeastScale4.  |x_i - value| <= s / 2, but up to
+// s where the nearest multiple of s is past the largest number of T.
 // The word: the upper twelve bits of s as a bf16, z in the low four.  A vector
-// with a value that is not finite (or that T does not hold) has a scale of NaN.
+// with a value that is NaN or past the largest number of T has a scale of NaN.
 #pragma once
 
 #include "paged.cuh"

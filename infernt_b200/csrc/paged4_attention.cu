@@ -17,10 +17,12 @@
 //     without a shuffle; for V^T it takes D / 8 neighbouring elements of four
 //     keys.  P^T comes out of the scores by a transposition of 8 x 8 blocks.
 // 16 sequences of 32768 positions, 32/8 heads of 128 (554 MB, 85 us of HBM): 137
-// us, 4.0 TB/s, of which 111 grow with the keys: some 23 instructions a key and
+// to 145 us, 4.0 TB/s, of which 111 grow with the keys: some 23 instructions a key and
 // warp, and the rest is the first loads, unequal ends and the joins.  64
 // sequences of 512 to 2048 with 40 query rows of 64: 40 us, where 2 instructions
 // of 4 that could be issue a cycle: 12 warps an SM with their waits for products.
+// Spilled, in bytes a thread: 24 to 56 where registers are held to let 3 or 4 CTAs
+// an SM run (D 128 of 8 rows, D 64 of 16 and 24), 244 at D 128 of 32 rows.
 #include <algorithm>
 #include <cmath>
 #include <cstdint>

@@ -179,8 +179,10 @@ __device__ __noinline__ void restore_values(const AttnArgs& a, const Current& cu
 // in which they come out of a word, (0, 4) (1, 5) (2, 6) (3, 7): the row warps
 // put Q into that order too, and take the result out of it.
 // The 512 x 128 registers of a launch are 176 a thread of the row warps and 80
-// of the others.  4096 tokens at 12288 positions, 32/8 heads of 128, bf16: 621
-// us, the time of 16-bit pages.  Before: 1259 us with the first four warps' two
+// of the others; some 130 bytes a thread are spilled.  4096 tokens at 12288
+// positions, 32/8 heads of 128, bf16: 621 to 670 us in bursts, where 16-bit pages
+// take 555 to 578 (the row warps have 32 registers less, joins read one part at
+// a time).  Before: 1259 us with the first four warps' two
 // idle ones in place of four more (a tile is 1600 instructions, one behind the
 // other), 1931 as straight code for whole tiles (waiting for instructions),
 // 705 with 64 registers, 889 with 48.
