@@ -812,7 +812,8 @@ INFERNT_API int infernt_paged_batch_plan(const infernt_page_tables* tables, cons
  *   they are p, and only what is asked of them is read.  temperature
  *   [num_seqs] FP32, or NULL for 1; where it is not above 0 the sequence is
  *   greedy: p is 1 at the row's largest element (the lowest of equal ones)
- *   and drafts are accepted where they are it.
+ *   and drafts are accepted where they are it.  Others are held to 1.4e-30 to
+ *   1.4e30.
  * Logits of -infinity have probability 0.  A row that has to be read and has
  * a NaN, an infinite or no finite logit (a NaN, negative or infinite
  * probability, or none above 0) ends its sequence there with its largest
